@@ -225,6 +225,102 @@ int ib_attention_split(const float* q, const float* kc, const float* vc, float* 
                        const int32_t* pos_dev, float scale, float* part, int32_t* counters,
                        void* stream);
 
+/* ---- paged KV cache -----------------------------------------------------------
+ * Many sequences in one pool of pages.  No counterpart in the reference (one contiguous
+ * cache per model, src/models/model_cuda.cpp:204-211).  The structs below are read on the
+ * host during the call; what their pointers name is device memory that the caller owns.
+ *
+ * Pool: k and v each [n_layers][n_pages][n_kv_heads][page_size][head_dim], F32 or F16
+ * (values rounded to nearest when written), 16-byte aligned; head_dim a multiple of 8 up to
+ * 256, any page_size up to IB_KV_MAX_PAGE_SIZE. */
+#define IB_KV_MAX_PAGES (1 << 20)
+#define IB_KV_MAX_SLOTS 16384
+#define IB_KV_MAX_PAGE_SIZE 4096
+typedef struct {
+    int32_t type; /* IB_TYPE_F32 or IB_TYPE_F16 */
+    int32_t n_layers, n_pages, n_kv_heads, page_size, head_dim;
+    void *k, *v;
+} ib_kv_pages;
+
+/* Sequences: slot s holds len[s] positions, position p in page table[s][p / page_size] at
+ * row p % page_size.  table [n_slots][max_pages]: -1 behind the last page, and where a page
+ * was given back early (its positions are then passed over).  refs [n_pages]: how many table
+ * entries hold the page, 0 = free.  An empty cache is table = -1, len = 0, refs = 0; the
+ * calls below keep it so.  max_pages * page_size <= 2^30. */
+typedef struct {
+    int32_t n_slots, max_pages;
+    int32_t *table, *len, *refs;
+} ib_kv_seqs;
+
+/* A step's new tokens: rows cu_q[b] .. cu_q[b + 1] of the step's tensors are the LAST tokens
+ * of sequence b, which is slot slots[b] (or slot b when slots is NULL; no slot twice), and
+ * are already counted in its len.  cu_q [n_seqs + 1] and slots are device memory.  n_tokens:
+ * rows of the tensors; rows from cu_q[n_seqs] on belong to nobody and are left as they were.
+ * max_q: the most tokens of one sequence where the caller knows it (0: n_tokens); it chooses
+ * kernels, results do not depend on it beyond rounding. */
+typedef struct {
+    int32_t n_seqs, n_tokens, max_q;
+    const int32_t *cu_q, *slots;
+} ib_kv_batch;
+
+/* Values in device memory cannot be checked by the host.  A slot, length, cu_q or table entry
+ * out of range is clamped or passed over by the kernel, never used as an address, and
+ * recorded: ib_check_fault then returns IB_ERR_INVALID with code 71 (slot), 72 (table entry),
+ * 73 (len or cu_q), 74 (refs below the tables' entries) or 75 (position behind rope_table).
+ *
+ * ib_kv_extend: room for n_new[i] more tokens of slot slots[i], i < n: len grows and the
+ * pages that this takes are entered in its row, with refs 1.  Free pages go out lowest first,
+ * in list order; once an entry finds too few, it and all later ones that need any get none.
+ * status[i]: 1 done, 0 no room (in the pool or in the row), -1 refused (slot out of range or
+ * named by an earlier entry, n_new < 0). */
+int ib_kv_extend(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const int32_t* slots,
+                 const int32_t* n_new, int32_t* status, void* stream);
+/* ib_kv_fork: children[i] becomes a copy of parents[i]: whole pages are shared (refs + 1), the
+ * filled rows of a partial last page are copied, in every layer, to a page of its own (handed
+ * out as above).  status as above; refused: a slot out of range, a child that is its own
+ * parent, is not empty (len > 0) or was named by an earlier entry. */
+int ib_kv_fork(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const int32_t* parents,
+               const int32_t* children, int32_t* status, void* stream);
+/* ib_kv_release: the slots give up their pages (refs - 1) and are empty. */
+int ib_kv_release(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const int32_t* slots,
+                  void* stream);
+/* ib_kv_compact: moves the pages in use to the lowest indices.  With n_live of them, the i-th
+ * used page at an index >= n_live goes to the i-th free one below, in every layer; the others
+ * stay, and the moved pages' old places keep their bytes.  Written: info = {n_live, moves},
+ * moves [n_pages] (pairs old, new), map [n_pages] (new index of each page, -1 for a free one),
+ * and the renamed table_out [n_slots][max_pages] and refs_out [n_pages], which may be seqs'
+ * own arrays. */
+int ib_kv_compact(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int32_t* table_out,
+                  int32_t* refs_out, int32_t* map, int32_t* moves, int32_t* info, void* stream);
+
+/* ib_kv_append: a step's projections into `layer` of the cache, ib_rope_batch and
+ * ib_kv_write_batch in one pass.  q [n_tokens][n_heads][head_dim], k and v [n_tokens]
+ * [n_kv_heads][head_dim], FP32 with rows q_stride .. elements apart (multiples of 4, so they
+ * may be slices of one projection; 16-byte aligned).  Rotated q goes to q_out (may be q),
+ * rotated k and v into the pages.  rope_table: [rope_len][head_dim / 2][2] cos and sin, as
+ * ib_rope takes.  Tokens without a position (len below the number of new tokens) or behind
+ * rope_len are passed over; where the page is -1 only q_out is written. */
+int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                 int layer, int n_heads, const float* q, int64_t q_stride, const float* k,
+                 int64_t k_stride, const float* v, int64_t v_stride, float* q_out,
+                 int64_t q_out_stride, const float* rope_table, int rope_len, void* stream);
+
+/* ib_attention_paged: causal attention of a step's new tokens over `layer` of the cache
+ * (their own K and V appended before): token i of a sequence with n new of len positions
+ * sees positions 0 .. len - n + i whose pages are there.  A row that sees none is 0.  Same
+ * result contract as ib_attention_batch (softmax of scale * q.k, grouped heads).  q and out
+ * [n_tokens][n_heads][head_dim] FP32, rows q_stride / out_stride elements apart (multiples
+ * of 4, 16-byte aligned).  A NaN or infinity in a position that a row does not see leaves the
+ * row alone; in one that it sees, the row's outputs are not finite.
+ * workspace: ib_attention_paged_workspace(...) bytes, 256-byte aligned, that no other call
+ * uses at the same time; it needs no initial value. */
+size_t ib_attention_paged_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                    const ib_kv_batch* batch, int n_heads);
+int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                       int layer, int n_heads, const float* q, int64_t q_stride, float* out,
+                       int64_t out_stride, float scale, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 /* Index of the first maximum of x[0..n) (reference sample_argmax,
  * src/ops/ops.cpp:424-438), written to *dev_out. */
 int ib_argmax(const float* x, int n, int32_t* dev_out, void* stream);

@@ -111,13 +111,21 @@ SIGNATURES = {
     "ib_attention_batch": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp],
     "ib_attention_split_part_bytes": [_i, _i],
     "ib_attention_split": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _f, _vp, _vp, _vp],
+    "ib_kv_extend": [_vp, _vp, _i, _vp, _vp, _vp, _vp],
+    "ib_kv_fork": [_vp, _vp, _i, _vp, _vp, _vp, _vp],
+    "ib_kv_release": [_vp, _vp, _i, _vp, _vp],
+    "ib_kv_compact": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ib_kv_append": [_vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i,
+                     _vp],
+    "ib_attention_paged_workspace": [_vp, _vp, _vp, _i],
+    "ib_attention_paged": [_vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _f, _vp, _sz, _vp],
     "ib_argmax": [_vp, _i, _vp, _vp],
     "ib_synth_host": [_i, _i64, _i64, _u64, _f, _vp, _i],
     "ib_synth_device": [_i, _i64, _i64, _u64, _f, _vp, _vp],
     "ib_synth_values_host": [_i64, _u64, _f, _vp],
 }
 _RESTYPE = {"ib_last_error": _c.c_char_p, "ib_attention_split_part_bytes": _c.c_size_t,
-            "ib_gemm_planes_bytes": _c.c_size_t}
+            "ib_gemm_planes_bytes": _c.c_size_t, "ib_attention_paged_workspace": _c.c_size_t}
 
 _lib = None
 
@@ -473,6 +481,270 @@ def attention_batch(q, kc, vc, out, n_heads, n_kv_heads, head_dim, max_seq, star
 
 def argmax(x, n, out, stream=None):
     call("ib_argmax", _ptr(x), n, _ptr(out), _stream(stream))
+
+
+# ---------------------------------------------------------------------------
+# paged KV cache (ib_kv_*, ib_attention_paged)
+# ---------------------------------------------------------------------------
+
+class _CKVPages(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("n_layers", ctypes.c_int32),
+                ("n_pages", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
+
+
+class _CKVSeqs(ctypes.Structure):
+    _fields_ = [("n_slots", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+                ("table", ctypes.c_void_p), ("len", ctypes.c_void_p), ("refs", ctypes.c_void_p)]
+
+
+class _CKVBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_int32), ("n_tokens", ctypes.c_int32),
+                ("max_q", ctypes.c_int32), ("cu_q", ctypes.c_void_p), ("slots", ctypes.c_void_p)]
+
+
+def _paged_tensor(t, name, dtype, shape, device):
+    """t as the paged calls take it: a contiguous CUDA tensor; -1 in shape is any size."""
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if t.dim() != len(shape) or any(w not in (-1, g) for g, w in zip(t.shape, shape)):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name}: on {t.device}, expected {device or 'a CUDA device'}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: not contiguous")
+    return t
+
+
+class KVPages:
+    """A pool of KV pages: k and v each [n_layers, n_pages, n_kv_heads, page_size, head_dim],
+    float32 or float16 CUDA tensors (kept here; the calls work on them in place)."""
+
+    def __init__(self, k, v):
+        import torch
+        if k.dtype not in (torch.float32, torch.float16):
+            raise ValueError(f"k: dtype {k.dtype}, expected float32 or float16")
+        self.k = _paged_tensor(k, "k", k.dtype, (-1,) * 5, None)
+        self.v = _paged_tensor(v, "v", k.dtype, k.shape, k.device)
+        self.device = k.device
+        self.type = F32 if k.dtype == torch.float32 else F16
+        self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self._c = _CKVPages(self.type, self.n_layers, self.n_pages, self.n_kv_heads,
+                            self.page_size, self.head_dim, k.data_ptr(), v.data_ptr())
+        self._p = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, n_layers, n_pages, n_kv_heads, page_size, head_dim, type_=F32, device="cuda"):
+        import torch
+        dt = {F32: torch.float32, F16: torch.float16}.get(type_)
+        if dt is None:
+            raise ValueError(f"pages must be F32 or F16, not {TYPE_NAMES.get(type_, type_)}")
+        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
+        return cls(torch.empty(shape, dtype=dt, device=device),
+                   torch.empty(shape, dtype=dt, device=device))
+
+
+class KVSeqs:
+    """The sequences of a pool: table [n_slots, max_pages] (-1: no page), len [n_slots] and
+    refs [n_pages], int32 CUDA tensors (kept here; the calls work on them in place)."""
+
+    def __init__(self, table, len, refs):
+        import torch
+        self.table = _paged_tensor(table, "table", torch.int32, (-1, -1), None)
+        self.device = table.device
+        self.n_slots, self.max_pages = table.shape
+        self.len = _paged_tensor(len, "len", torch.int32, (self.n_slots,), self.device)
+        self.refs = _paged_tensor(refs, "refs", torch.int32, (-1,), self.device)
+        self._c = _CKVSeqs(self.n_slots, self.max_pages, table.data_ptr(), len.data_ptr(),
+                           refs.data_ptr())
+        self._p = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, n_slots, max_pages, n_pages, device="cuda"):
+        import torch
+        return cls(torch.full((n_slots, max_pages), -1, dtype=torch.int32, device=device),
+                   torch.zeros(n_slots, dtype=torch.int32, device=device),
+                   torch.zeros(n_pages, dtype=torch.int32, device=device))
+
+
+class KVBatch:
+    """A step's new tokens: rows cu_q[b] .. cu_q[b + 1] of its n_tokens rows are the last
+    tokens of sequence b (slot slots[b], or slot b).  cu_q, slots: int32 CUDA tensors.  max_q:
+    the most tokens of one sequence where known (chooses kernels only)."""
+
+    def __init__(self, cu_q, n_tokens, max_q=0, slots=None):
+        import torch
+        self.cu_q = _paged_tensor(cu_q, "cu_q", torch.int32, (-1,), None)
+        self.device = cu_q.device
+        self.n_seqs, self.n_tokens = cu_q.numel() - 1, int(n_tokens)
+        self.slots = slots
+        if slots is not None:
+            _paged_tensor(slots, "slots", torch.int32, (self.n_seqs,), self.device)
+        self._c = _CKVBatch(self.n_seqs, self.n_tokens, int(max_q), cu_q.data_ptr(), _ptr(slots))
+        self._p = ctypes.addressof(self._c)
+
+
+def _paged_stream(pages, stream, *others):
+    """The stream to launch on, after checking that everything is on the current device."""
+    import torch
+    dev = pages.device
+    for o in others:
+        if o.device != dev:
+            raise ValueError(f"arguments on {dev} and {o.device}")
+    if torch.cuda.current_device() != dev.index:
+        raise ValueError(f"the pages are on {dev}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return _stream(stream)
+
+
+def _seqs_of(pages, seqs):
+    if seqs.refs.numel() != pages.n_pages:
+        raise ValueError(f"refs: {seqs.refs.numel()} entries for {pages.n_pages} pages")
+    return seqs._p
+
+
+def _paged_lists(pages, *named):
+    import torch
+    n = named[0][1].numel()
+    for name, t in named:
+        _paged_tensor(t, name, torch.int32, (n,), pages.device)
+    return n
+
+
+def kv_extend(pages, seqs, slots, n_new, status=None, stream=None):
+    """Room for n_new[i] more tokens of each slot; returns status (1 done, 0 no room,
+    -1 refused), int32 tensors on the pages' device."""
+    import torch
+    if status is None:
+        status = torch.empty_like(slots)
+    n = _paged_lists(pages, ("slots", slots), ("n_new", n_new), ("status", status))
+    st = _paged_stream(pages, stream, seqs)
+    call("ib_kv_extend", pages._p, _seqs_of(pages, seqs), n, slots.data_ptr(), n_new.data_ptr(),
+         status.data_ptr(), st)
+    return status
+
+
+def kv_fork(pages, seqs, parents, children, status=None, stream=None):
+    """children[i] becomes a copy of parents[i], sharing its whole pages; returns status."""
+    import torch
+    if status is None:
+        status = torch.empty_like(parents)
+    n = _paged_lists(pages, ("parents", parents), ("children", children), ("status", status))
+    st = _paged_stream(pages, stream, seqs)
+    call("ib_kv_fork", pages._p, _seqs_of(pages, seqs), n, parents.data_ptr(),
+         children.data_ptr(), status.data_ptr(), st)
+    return status
+
+
+def kv_release(pages, seqs, slots, stream=None):
+    """The slots give up their pages."""
+    n = _paged_lists(pages, ("slots", slots))
+    st = _paged_stream(pages, stream, seqs)
+    call("ib_kv_release", pages._p, _seqs_of(pages, seqs), n, slots.data_ptr(), st)
+
+
+class KVCompactPlan:
+    """What kv_compact did: map [n_pages] (new index of each page, -1 for a free one), info
+    {pages in use, pages moved} and the moves' (old, new) pairs."""
+
+    def __init__(self, pages):
+        import torch
+        n = pages.n_pages
+        self.map = torch.empty(n, dtype=torch.int32, device=pages.device)
+        self.moves = torch.empty(n, dtype=torch.int32, device=pages.device)
+        self.info = torch.empty(2, dtype=torch.int32, device=pages.device)
+        self.n_live, self.n_moves = self.info[0], self.info[1]
+        self.n_pages, self.device = n, pages.device
+
+
+def kv_compact_plan(pages):
+    return KVCompactPlan(pages)
+
+
+def kv_compact(pages, seqs, out=None, plan=None, stream=None):
+    """Moves the used pages to the lowest indices; the renamed table and refs go to `out` (a
+    KVSeqs; default: seqs itself).  Returns the plan."""
+    out = seqs if out is None else out
+    plan = KVCompactPlan(pages) if plan is None else plan
+    st = _paged_stream(pages, stream, seqs, out, plan)
+    if out.table.shape != seqs.table.shape or plan.n_pages != pages.n_pages:
+        raise ValueError("out or plan of another cache")
+    _seqs_of(pages, out)
+    call("ib_kv_compact", pages._p, _seqs_of(pages, seqs), out.table.data_ptr(),
+         out.refs.data_ptr(), plan.map.data_ptr(), plan.moves.data_ptr(), plan.info.data_ptr(),
+         st)
+    return plan
+
+
+def _paged_rows(t, name, tokens, heads, head_dim, device):
+    """(pointer, row stride) of a float32 [tokens, heads, head_dim] tensor whose rows may be
+    apart (slices of a projection's output)."""
+    import torch
+    shape, strides = t.shape, t.stride()
+    if t.dtype != torch.float32 or t.device != device:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, expected float32 on {device}")
+    if len(shape) != 3 or shape[0] != tokens or (heads and shape[1] != heads) \
+            or shape[2] != head_dim:
+        raise ValueError(f"{name}: shape {tuple(shape)}, expected "
+                         f"({tokens}, {heads or 'heads'}, {head_dim})")
+    if strides[2] != 1 or (strides[1] != head_dim and shape[1] != 1):
+        raise ValueError(f"{name}: the heads of a token are not contiguous")
+    return t.data_ptr(), strides[0] if tokens > 1 else shape[1] * head_dim
+
+
+def kv_append(pages, seqs, batch, layer, q, k, v, rope_table, q_out=None, stream=None):
+    """RoPE on q and k and the write of k and v into the layer's pages.  q [tokens, heads,
+    head_dim], k and v [tokens, kv heads, head_dim] float32 (rows may be slices);
+    rope_table [positions, head_dim / 2, 2].  Returns q_out."""
+    import torch
+    T, HD, dev = batch.n_tokens, pages.head_dim, pages.device
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=torch.float32, device=dev)
+    qp, qs = _paged_rows(q, "q", T, 0, HD, dev)
+    H = q.shape[1]
+    kp, ks = _paged_rows(k, "k", T, pages.n_kv_heads, HD, dev)
+    vp, vs = _paged_rows(v, "v", T, pages.n_kv_heads, HD, dev)
+    op, os_ = _paged_rows(q_out, "q_out", T, H, HD, dev)
+    _paged_tensor(rope_table, "rope_table", torch.float32, (-1, HD // 2, 2), dev)
+    st = _paged_stream(pages, stream, seqs, batch)
+    call("ib_kv_append", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, kp, ks, vp,
+         vs, op, os_, rope_table.data_ptr(), rope_table.shape[0], st)
+    return q_out
+
+
+def attention_paged_workspace(pages, seqs, batch, n_heads):
+    """Scratch for attention_paged calls of this shape, one at a time (a uint8 CUDA tensor)."""
+    import torch
+    n = lib().ib_attention_paged_workspace(pages._p, seqs._p, batch._p, n_heads)
+    if n == 0:
+        raise ValueError(last_error())
+    return torch.empty(n, dtype=torch.uint8, device=pages.device)
+
+
+def attention_paged(pages, seqs, batch, layer, q, scale, out=None, workspace=None, stream=None):
+    """Causal attention of the batch's new tokens over the layer's pages.  q, out [tokens,
+    heads, head_dim] float32 (rows may be slices).  workspace: attention_paged_workspace(),
+    allocated for the call when None.  Returns out (rows of nobody: as they were)."""
+    import torch
+    T, HD, dev = batch.n_tokens, pages.head_dim, pages.device
+    qp, qs = _paged_rows(q, "q", T, 0, HD, dev)
+    H = q.shape[1]
+    if out is None:
+        out = torch.zeros(q.shape, dtype=torch.float32, device=dev)
+    op, os_ = _paged_rows(out, "out", T, H, HD, dev)
+    st = _paged_stream(pages, stream, seqs, batch)
+    if workspace is None:
+        # of the launch stream's memory pool: it may be handed out again, in stream order,
+        # as soon as the call returns
+        with torch.cuda.stream(torch.cuda.ExternalStream(st, dev) if st else
+                               torch.cuda.default_stream(dev)):
+            workspace = attention_paged_workspace(pages, seqs, batch, H)
+    elif workspace.device != dev:
+        raise ValueError(f"workspace on {workspace.device}, expected {dev}")
+    call("ib_attention_paged", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, op,
+         os_, scale, workspace.data_ptr(), workspace.numel() * workspace.element_size(), st)
+    return out
 
 
 # ---------------------------------------------------------------------------

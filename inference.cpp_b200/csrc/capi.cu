@@ -10,6 +10,7 @@
 #include "step.cuh"
 #include "gemv_mma.cuh"
 #include "ops.cuh"
+#include "paged.cuh"
 
 namespace ib {
 
@@ -149,6 +150,19 @@ extern "C" int ib_check_fault(int* code) {
     if (!*code) *code = c2;
     if ((st = step_fault_take(&c2)) != IB_OK) return st;
     if (!*code) *code = c2;
+    if (!*code) {
+        if ((st = paged_fault_take(&c2)) != IB_OK) return st;
+        int c3 = 0;
+        if ((st = paged_attention_fault_take(&c3)) != IB_OK) return st;
+        *code = c2 ? c2 : c3;
+        if (*code && *code != PAGED_BAD_WAIT) {
+            static const char* const what[] = {"a slot", "a table entry", "a length or cu_q value",
+                                               "a reference count", "a RoPE position"};
+            set_error(std::string("CUDA: paged KV cache: ") + what[*code - PAGED_BAD_SLOT] +
+                      " was out of range (code " + std::to_string(*code) + ")");
+            return IB_ERR_INVALID;
+        }
+    }
     if (*code) {
         set_error("CUDA: a pipeline wait expired in a GEMV kernel (code " + std::to_string(*code) +
                   "); results of the calls since the last check are invalid");
