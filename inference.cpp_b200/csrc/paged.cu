@@ -65,13 +65,12 @@ int paged_check_batch(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_bat
     if (!b || !b->cu_q) return paged_refuse(who, "null pointer argument");
     if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_q < 0)
         return paged_refuse(who, "bad batch sizes");
-    if (!b->slots && b->n_seqs > s->n_slots)
-        return paged_refuse(who, "more sequences than slots");
+    if (b->n_seqs > s->n_slots) return paged_refuse(who, "more sequences than slots");
     if (layer < 0 || layer >= p->n_layers) return paged_refuse(who, "layer out of range");
     if (n_heads <= 0 || n_heads % p->n_kv_heads || n_heads > 65536)
         return paged_refuse(who, "n_heads must be a multiple of n_kv_heads");
-    if ((int64_t)b->n_tokens * n_heads > (1 << 30))
-        return paged_refuse(who, "n_tokens x n_heads must be at most 2^30");
+    if ((int64_t)b->n_tokens * n_heads > (1 << 26))
+        return paged_refuse(who, "n_tokens x n_heads must be at most 2^26");
     return IB_OK;
 }
 

@@ -1,66 +1,786 @@
 // ib_attention_paged: causal GQA attention of a batch of new tokens over the paged cache.
+//
+// The query rows of a sequence that share a kv head -- (token, head of the group), token by
+// token -- are consecutive: row r is token r / G, head r % G.  A work item is a tile of such
+// rows against a range of the sequence's positions; items whose range is not the whole leave
+// a partial result (running maximum m, exponential sum l, unnormalised sum of p v), and a
+// second kernel joins them:
+//     out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.
+// Lengths are device data, so every CTA works the split out for itself from cu_q and len (one
+// pass over the batch; no planning launch), and grids are sized by the host's bounds.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <mutex>
 #include <string>
 
 #include "common.cuh"
-#include "kv.cuh"
+#include "mma_tile.cuh"
 #include "paged.cuh"
+#include "pdl.cuh"
+#include "pipeline.cuh"
 
 namespace ib {
 
 int paged_attention_fault_take(int* code) { return paged_fault_take_here(code); }
 
-// One warp per (token, head): positions one after another, lanes share head_dim, running
-// maximum and sum.
+// ---- the split of a batch into items -----------------------------------------------------
+// Sequences with rows in [min_rows, max_rows] take part.  A sequence has ceil(rows / R) row
+// tiles per kv head, each over ceil(L / KT) key tiles; the ranges are as long as it takes to
+// have about `target` items, but at least `least` key tiles.
+struct SplitRule {
+    int R, KT, min_rows, max_rows, target, least;
+};
+
+// Item `item` of the batch.  n_parts: ranges of its row tile; part_base: index of the first
+// of their partials (unused when n_parts == 1).
+struct Item {
+    int b, hk, tile, part, n_parts, part_base;
+    int kt0, kt1;  // key tiles of the range
+    SeqInfo s;
+};
+
+struct SeqSplit {
+    int tiles, nkt, parts;  // row tiles per kv head, key tiles, ranges
+};
+
+__device__ __forceinline__ void seq_shape(const PagedView& w, const SplitRule& rule,
+                                          const SeqInfo& s, int& tiles, int& nkt) {
+    const int rows = s.n * (w.H / w.Hkv);
+    const bool in = rows >= rule.min_rows && rows <= rule.max_rows;
+    tiles = in ? (rows + rule.R - 1) / rule.R : 0;
+    nkt = max(1, (s.L + rule.KT - 1) / rule.KT);  // a sequence without positions: zeros
+}
+
+// Every thread of the CTA (NT threads) calls it; false when there are fewer items.  BY_TILE
+// counts row tiles instead of items (the joining kernel).
+template <int NT, bool BY_TILE>
+__device__ __forceinline__ bool find_item(const PagedView& w, const SplitRule& rule, int item,
+                                          Item& out) {
+    __shared__ long long sh_units[NT / 32];
+    __shared__ int sh_scan[NT / 32][2];
+    __shared__ Item sh_item;
+    __shared__ int sh_found;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    SeqInfo s0{};
+    int tiles0 = 0, nkt0 = 1;
+    long long units = 0;
+    for (int b = tid; b < w.n_seqs; b += NT) {
+        const SeqInfo s = seq_info(w, b);
+        int tiles, nkt;
+        seq_shape(w, rule, s, tiles, nkt);
+        units += min((long long)tiles * nkt, 1ll << 40);
+        if (b == tid) s0 = s, tiles0 = tiles, nkt0 = nkt;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+    if (lane == 0) sh_units[warp] = units;
+    if (tid == 0) sh_found = 0;
+    __syncthreads();
+    units = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) units += sh_units[i];
+    units = min(units, 1ll << 45) * w.Hkv;
+    const int len = (int)min(max((long long)rule.least, (units + rule.target - 1) / rule.target),
+                             0x3fffffffll);
+    // cu_q can hold anything: counts are clamped to what cannot be, so that sums stay in range
+    // (valid batches have at most 2^22 + n_seqs row tiles, see paged_check_batch)
+    constexpr long long MOST = 1 << 23;
+    const int room = 2 * rule.target;  // partials in the workspace
+    long long items_before = 0;
+    int parts_before = 0;
+    for (int b0 = 0; b0 < w.n_seqs; b0 += NT) {
+        const int b = b0 + tid;
+        SeqInfo s = s0;
+        int tiles = tiles0, nkt = nkt0;
+        if (b0 > 0) {
+            tiles = 0;
+            if (b < w.n_seqs) {
+                s = seq_info(w, b);
+                seq_shape(w, rule, s, tiles, nkt);
+            }
+        }
+        const int parts = (nkt + len - 1) / len;
+        const long long n_tiles = b < w.n_seqs ? (long long)tiles * w.Hkv : 0;
+        const int n_items = (int)min(BY_TILE ? n_tiles : n_tiles * parts, MOST);
+        const int n_parts = parts > 1 ? (int)min(n_tiles * parts, (long long)room + 1) : 0;
+        int a = n_items, p = n_parts;  // inclusive scans
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int xa = __shfl_up_sync(0xffffffffu, a, o), xp = __shfl_up_sync(0xffffffffu, p, o);
+            if (lane >= o) a += xa, p += xp;
+        }
+        if (lane == 31) sh_scan[warp][0] = a, sh_scan[warp][1] = p;
+        __syncthreads();
+        int ta = 0, tp = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 32; ++i) {
+            if (i == warp) a += ta, p += tp;
+            ta += sh_scan[i][0], tp += sh_scan[i][1];
+        }
+        const long long at = item - items_before - (a - n_items);
+        if (at >= 0 && at < n_items) {
+            const int local = (int)at;
+            Item it;
+            it.b = b;
+            it.s = s;
+            it.n_parts = parts;
+            const int t = BY_TILE ? local : local / parts;
+            it.part = BY_TILE ? 0 : local - t * parts;
+            it.tile = t / w.Hkv;
+            it.hk = t - it.tile * w.Hkv;
+            it.part_base = parts_before + (p - n_parts) + t * parts;
+            // ranges of equal length, to one key tile
+            it.kt0 = (int)((long long)nkt * it.part / parts);
+            it.kt1 = (int)((long long)nkt * (it.part + 1) / parts);
+            sh_item = it;
+            sh_found = parts == 1 || it.part_base + parts <= room ? 1 : 2;
+        }
+        __syncthreads();
+        if (sh_found) break;
+        items_before += ta;
+        parts_before += tp;
+    }
+    __syncthreads();
+    out = sh_item;
+    if (sh_found == 2) paged_fault(PAGED_BAD_LEN);  // more partials than a valid batch has
+    return sh_found == 1;
+}
+
+// ---- rows on mma.sync --------------------------------------------------------------------
+// For few rows (single tokens, short drafts), where the bound is reading K and V once, and
+// for FP32 pages.  A CTA holds 16 rows (WR = 1: its four warps take a quarter of each key
+// tile's positions each, and join at the end) or WR tiles of 16 rows (one per warp, all over
+// the same key tiles).  Products of FP32 operands keep about 2^-20:
+//   FP16 pages  q = hi + lo and p = hi + lo in FP16, K and V as they are: two m16n8k16 per
+//               product.  q rows are scaled to a largest element in [256, 512) and p by 2^10,
+//               powers of two that keep the lo parts out of FP16's subnormals.
+//   FP32 pages  both operands as TF32 hi + lo, hi hi + hi lo + lo hi: three m16n8k8, with the
+//               range of FP32.
+// Positions that a row does not see get a score of -inf; pages that are not there are filled
+// with zeros, and in tiles where some row does not see a position that has a page, V is
+// checked for values that are not finite (0 x inf).
+struct RowsArgs {
+    PagedView w;
+    SplitRule rule;
+    const float* q;
+    float* out;
+    int64_t q_stride, out_stride;
+    const void *k, *v;  // the layer
+    float* part_acc;    // [partial][R][HD]
+    float2* part_ml;    // [partial][R]
+    float scale_log2;   // scale * log2(e)
+};
+
+template <typename KV, int HDP, int WR>
+struct RowsCfg {
+    static constexpr bool F32 = sizeof(KV) == 4;
+    static constexpr int NW = WR == 1 ? 4 : WR, NT = NW * 32, R = 16 * WR;
+    static constexpr int ROWB = HDP * (int)sizeof(KV);  // bytes of a K or V row
+    static constexpr int LD = ROWB + 16;                // padded: 8 rows of an ldmatrix, and the
+                                                        // TF32 V columns, hit distinct banks
+    static constexpr int KT = !F32 ? 64 : HDP == 256 && WR > 1 ? 16 : 32;
+    static constexpr int STAGES = ROWB > 256 ? 2 : F32 ? 4 : 3;
+    static constexpr int KW = WR == 1 ? KT / NW : KT;  // positions of a warp
+    static constexpr int QLD = HDP * (F32 ? 4 : 2) + 16;
+    static constexpr int Q_BYTES = 2 * R * QLD;  // hi and lo
+    static constexpr int STAGE = 2 * KT * LD;
+    static constexpr int RING = STAGES + 1;  // of row offsets
+    static constexpr int MERGE = WR == 1 ? NW * 16 * (HDP + 4) * 4 : 0;  // joins the warps
+    static constexpr int BODY = STAGES * STAGE > MERGE ? STAGES * STAGE : MERGE;
+    // q fragments that stay in registers are staged in the ring's last slot, whose first copy
+    // is issued after they were read
+    static constexpr bool QREG = !F32 && HDP <= 128;
+    static constexpr int Q_OFF = QREG ? (STAGES - 1) * STAGE : BODY;
+    static constexpr size_t SMEM = Q_OFF + Q_BYTES > BODY ? Q_OFF + Q_BYTES : BODY;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(valid ? 16 : 0)
+                 : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two FP16 values with those that are not finite as zero; odd is set when there were any.
+__device__ __forceinline__ uint32_t finite16x2(uint32_t x, bool& odd) {
+    if ((x & 0x7c00u) == 0x7c00u) odd = true, x &= 0xffff0000u;
+    if ((x & 0x7c000000u) == 0x7c000000u) odd = true, x &= 0x0000ffffu;
+    return x;
+}
+
+template <typename KV, int HDP, int WR>
+__global__ void __launch_bounds__(RowsCfg<KV, HDP, WR>::NT)
+    attn_rows_kernel(const __grid_constant__ RowsArgs A) {
+    using C = RowsCfg<KV, HDP, WR>;
+    constexpr int NT = C::NT, R = C::R, KT = C::KT, KW = C::KW, LD = C::LD;
+    constexpr bool F32 = C::F32;
+    constexpr int NB = KW / 8;     // score columns of a warp, in blocks of 8
+    constexpr int DB = HDP / 8;    // output columns, in blocks of 8
+    constexpr int KS = F32 ? HDP / 8 : HDP / 16;  // k-steps of q.k
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ long long row_off[C::RING][KT];  // element offset of a position's row, -1: none
+    __shared__ __align__(8) int key_pos[C::RING][KT];  // its position, INT_MAX: none
+    __shared__ float row_scale[R];
+    __shared__ int row_lim[R];  // last position that the row sees
+    const PagedView& w = A.w;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t4 = lane & 3;
+    pdl_wait();
+    pdl_launch_dependents();
+    Item it;
+    if (!find_item<NT, false>(w, A.rule, blockIdx.x, it)) return;
+    const int G = w.H / w.Hkv, HD = w.HD;
+    const int rows = min(R, it.s.n * G - it.tile * R);
+    const int first_lim = it.s.L - it.s.n + it.tile * R / G;
+    const int last_lim = it.s.L - it.s.n + (it.tile * R + rows - 1) / G;
+    uint8_t* q_smem = smem + C::Q_OFF;
+    const uint32_t kv_base = smem_u32(smem), q_base = kv_base + C::Q_OFF;
+
+    // key tiles that some row sees
+    const int kt0 = it.kt0, kt1 = min(it.kt1, last_lim < 0 ? 0 : last_lim / KT + 1);
+    const int n_kt = max(0, kt1 - kt0);
+
+    // table entries are read one tile ahead of the copies that need them
+    auto entry_of = [&](int kt) -> int {
+        const int pos = kt * KT + tid;
+        if (tid >= KT || kt >= kt1 || pos > last_lim) return -1;
+        return page_at(w, it.s.row[w.ps.div((uint32_t)pos)]);
+    };
+    auto put_offsets = [&](int i, int page) {  // tile i of the range
+        if (tid >= KT) return;
+        const int pos = (kt0 + i) * KT + tid;
+        const int in_page = pos - (int)w.ps.div((uint32_t)pos) * w.page_size;
+        row_off[i % C::RING][tid] =
+            page < 0 ? -1 : (((long long)page * w.Hkv + it.hk) * w.page_size + in_page) * HD;
+        key_pos[i % C::RING][tid] = page < 0 ? 0x7fffffff : pos;
+    };
+    const int cpr = HD * (int)sizeof(KV) / 16;  // 16-byte chunks of a row that exist
+    auto issue = [&](int i) {
+        if (i < n_kt) {
+            const uint32_t kd = kv_base + (uint32_t)((i % C::STAGES) * C::STAGE);
+            constexpr int CH = C::ROWB / 16, N = KT * CH;
+#pragma unroll 4
+            for (int c = tid; c < N; c += NT) {
+                const int r = c / CH, x = c % CH;
+                const long long off = row_off[i % C::RING][r];
+                const bool ok = off >= 0 && x < cpr;
+                const size_t byte = ok ? (size_t)off * sizeof(KV) + (size_t)x * 16 : 0;
+                const uint32_t d = kd + (uint32_t)(r * LD + x * 16);
+                cp16(d, (const uint8_t*)A.k + byte, ok);
+                cp16(d + KT * LD, (const uint8_t*)A.v + byte, ok);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) put_offsets(i, entry_of(kt0 + i));
+    __syncthreads();
+    for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
+    int next_page = entry_of(kt0 + C::STAGES - 1);
+
+    // q rows to shared memory as hi and lo parts
+    for (int r = warp; r < R; r += C::NW) {
+        float x[HDP / 32];
+        const int gr = it.tile * R + r, tok = gr / G, head = it.hk * G + gr - tok * G;
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < HDP / 32; ++i) {
+            const int d = lane + 32 * i;
+            x[i] = r < rows && d < HD
+                       ? A.q[(int64_t)(it.s.q0 + tok) * A.q_stride + (int64_t)head * HD + d]
+                       : 0.f;
+            top = fmaxf(top, fabsf(x[i]));
+        }
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < HDP / 32; ++i) {
+                uint32_t h, l;
+                split_tf32(x[i], h, l);
+                const int o = r * C::QLD + (lane + 32 * i) * 4;
+                *reinterpret_cast<uint32_t*>(q_smem + o) = h;
+                *reinterpret_cast<uint32_t*>(q_smem + R * C::QLD + o) = l;
+            }
+            if (lane == 0) row_scale[r] = A.scale_log2;
+        } else {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // 2^(8 - e) with e the exponent of the largest element, and its inverse
+            const int e = max(-100, (int)((__float_as_uint(top) >> 23) & 255u) - 127);
+            const bool plain = top == 0.f || e > 127;
+            const float up = plain ? 1.f : __uint_as_float((uint32_t)(8 - e + 127) << 23);
+            const float down = plain ? 1.f : __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+#pragma unroll
+            for (int i = 0; i < HDP / 32; ++i) {
+                const float y = x[i] * up;
+                const __half h = __float2half_rn(y);
+                const int o = r * C::QLD + (lane + 32 * i) * 2;
+                *reinterpret_cast<__half*>(q_smem + o) = h;
+                *reinterpret_cast<__half*>(q_smem + R * C::QLD + o) =
+                    __float2half_rn(y - __half2float(h));
+            }
+            if (lane == 0) row_scale[r] = A.scale_log2 * down;
+        }
+        if (lane == 0) row_lim[r] = r < rows ? it.s.L - it.s.n + tok : -1;
+    }
+    __syncthreads();
+
+    const int wr = WR == 1 ? 0 : warp * 16;    // first row of this warp
+    const int wk = WR == 1 ? warp * KW : 0;    // its first position in a tile
+    const uint32_t q_frag = q_base + (uint32_t)((wr + (lane & 15)) * C::QLD + (lane >> 4) * 16);
+    const int lim0 = row_lim[wr + g], lim1 = row_lim[wr + g + 8];
+    const float sc0 = row_scale[wr + g], sc1 = row_scale[wr + g + 8];
+    uint32_t qh[C::QREG ? KS : 1][4], ql[C::QREG ? KS : 1][4];
+    if constexpr (C::QREG) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            ldsm_x4(q_frag + k * 32, qh[k][0], qh[k][1], qh[k][2], qh[k][3]);
+            ldsm_x4(q_frag + R * C::QLD + k * 32, ql[k][0], ql[k][1], ql[k][2], ql[k][3]);
+        }
+    }
+    float acc[DB][4];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[d][i] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    // p is carried times 2^10 (FP16 pages): see above
+    constexpr float P_BIAS = F32 ? 0.f : 10.f;
+
+    for (int i = 0; i < n_kt; ++i) {
+        if (i + C::STAGES - 1 < n_kt) put_offsets(i + C::STAGES - 1, next_page);
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
+        __syncthreads();
+        issue(i + C::STAGES - 1);
+        next_page = entry_of(kt0 + i + C::STAGES);
+        const uint32_t kd = kv_base + (uint32_t)((i % C::STAGES) * C::STAGE + wk * LD);
+        const uint32_t vd = kd + KT * LD;
+        const int* kp = &key_pos[i % C::RING][wk];
+
+        // scores: 16 rows x KW positions
+        float s[NB][4];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+        if constexpr (!F32) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t ah[4], al[4];
+                if constexpr (C::QREG) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) ah[j] = qh[k][j], al[j] = ql[k][j];
+                } else {
+                    ldsm_x4(q_frag + k * 32, ah[0], ah[1], ah[2], ah[3]);
+                    ldsm_x4(q_frag + R * C::QLD + k * 32, al[0], al[1], al[2], al[3]);
+                }
+#pragma unroll
+                for (int n = 0; n < NB; n += 2) {  // 16 positions x 16 dimensions
+                    uint32_t b[4];
+                    ldsm_x4(kd + (uint32_t)((n * 8 + (lane & 7) + ((lane >> 4) << 3)) * LD + k * 32 +
+                                            ((lane >> 3) & 1) * 16),
+                            b[0], b[1], b[2], b[3]);
+                    mma16816(s[n], ah, b[0], b[1]);
+                    mma16816(s[n + 1], ah, b[2], b[3]);
+                    mma16816(s[n], al, b[0], b[1]);
+                    mma16816(s[n + 1], al, b[2], b[3]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; k += 2) {
+                uint32_t ah[2][4], al[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    ldsm_x4(q_frag + (k + j) * 32, ah[j][0], ah[j][1], ah[j][2], ah[j][3]);
+                    ldsm_x4(q_frag + R * C::QLD + (k + j) * 32, al[j][0], al[j][1], al[j][2],
+                            al[j][3]);
+                }
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {  // 8 positions x 16 dimensions
+                    uint32_t b[4], h[4], e[4];
+                    ldsm_x4(kd + (uint32_t)((n * 8 + (lane & 7)) * LD + k * 32 + (lane >> 3) * 16),
+                            b[0], b[1], b[2], b[3]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(b[j]), h[j], e[j]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        mma1688_tf32(s[n], ah[j], h[2 * j], h[2 * j + 1]);
+                        mma1688_tf32(s[n], ah[j], e[2 * j], e[2 * j + 1]);
+                        mma1688_tf32(s[n], al[j], h[2 * j], h[2 * j + 1]);
+                    }
+                }
+            }
+        }
+        // what the rows do not see, and the running maximum
+        float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int2 p = *reinterpret_cast<const int2*>(kp + n * 8 + 2 * t4);
+            s[n][0] = p.x <= lim0 ? s[n][0] * sc0 : -INFINITY;
+            s[n][1] = p.y <= lim0 ? s[n][1] * sc0 : -INFINITY;
+            s[n][2] = p.x <= lim1 ? s[n][2] * sc1 : -INFINITY;
+            s[n][3] = p.y <= lim1 ? s[n][3] * sc1 : -INFINITY;
+            x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
+            x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
+        }
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+        }
+        if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+            const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+            const float c0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0);
+            const float c1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
+            m0 = n0, m1 = n1;
+            l0 *= c0, l1 *= c1;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                acc[d][0] *= c0, acc[d][1] *= c0;
+                acc[d][2] *= c1, acc[d][3] *= c1;
+            }
+        }
+        const float b0 = m0 == -INFINITY ? 0.f : m0 - P_BIAS, b1 = m1 == -INFINITY ? 0.f : m1 - P_BIAS;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            s[n][0] = ex2(s[n][0] - b0), s[n][1] = ex2(s[n][1] - b0);
+            s[n][2] = ex2(s[n][2] - b1), s[n][3] = ex2(s[n][3] - b1);
+            l0 += s[n][0] + s[n][1];
+            l1 += s[n][2] + s[n][3];
+        }
+        // p v; `careful` where some row does not see all of the tile
+        const bool careful = (kt0 + i) * KT + KT - 1 > first_lim;
+        bool odd = false;  // a V value that is not finite, among this thread's
+        if constexpr (!F32) {
+#pragma unroll
+            for (int k = 0; k < KW / 16; ++k) {
+                uint32_t ph[4], pl[4];
+                split2(s[2 * k][0], s[2 * k][1], ph[0], pl[0]);
+                split2(s[2 * k][2], s[2 * k][3], ph[1], pl[1]);
+                split2(s[2 * k + 1][0], s[2 * k + 1][1], ph[2], pl[2]);
+                split2(s[2 * k + 1][2], s[2 * k + 1][3], ph[3], pl[3]);
+#pragma unroll
+                for (int d = 0; d < DB; d += 2) {
+                    uint32_t b[4];
+                    ldsm_x4_t(vd + (uint32_t)((k * 16 + (lane & 15)) * LD + d * 16 + (lane >> 4) * 16),
+                              b[0], b[1], b[2], b[3]);
+                    if (careful) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) b[j] = finite16x2(b[j], odd);
+                    }
+                    mma16816(acc[d], ph, b[0], b[1]);
+                    mma16816(acc[d + 1], ph, b[2], b[3]);
+                    mma16816(acc[d], pl, b[0], b[1]);
+                    mma16816(acc[d + 1], pl, b[2], b[3]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KW / 8; ++k) {
+                // the MMA's k index t holds position 2 t, t + 4 position 2 t + 1, in both operands:
+                // then the scores' accumulator is the A operand as it lies
+                uint32_t ph[4], pl[4];
+                split_tf32(s[k][0], ph[0], pl[0]);
+                split_tf32(s[k][2], ph[1], pl[1]);
+                split_tf32(s[k][1], ph[2], pl[2]);
+                split_tf32(s[k][3], ph[3], pl[3]);
+                const uint8_t* v0 = smem + (vd - kv_base) + (k * 8 + 2 * t4) * LD + g * 4;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    float y0 = *reinterpret_cast<const float*>(v0 + d * 32);
+                    float y1 = *reinterpret_cast<const float*>(v0 + LD + d * 32);
+                    if (careful) {
+                        if (!(fabsf(y0) < INFINITY)) odd = true, y0 = 0.f;
+                        if (!(fabsf(y1) < INFINITY)) odd = true, y1 = 0.f;
+                    }
+                    uint32_t h0, e0, h1, e1;
+                    split_tf32(y0, h0, e0);
+                    split_tf32(y1, h1, e1);
+                    mma1688_tf32(acc[d], ph, h0, h1);
+                    mma1688_tf32(acc[d], ph, e0, e1);
+                    mma1688_tf32(acc[d], pl, h0, h1);
+                }
+            }
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+            // rows that see such a value are not finite there
+#pragma unroll 1
+            for (int j = 0; j < KW; ++j) {
+                const int pos = kp[j];
+                const uint8_t* vr = smem + (vd - kv_base) + j * LD;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int x = d * 8 + 2 * t4 + c;
+                        float y;
+                        if constexpr (F32) y = reinterpret_cast<const float*>(vr)[x];
+                        else y = __half2float(reinterpret_cast<const __half*>(vr)[x]);
+                        if (fabsf(y) < INFINITY) continue;
+                        if (pos <= lim0) acc[d][c] = NAN;
+                        if (pos <= lim1) acc[d][2 + c] = NAN;
+                    }
+            }
+        }
+    }
+
+    // ---- the item's result ----
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    }
+    const int first_head = it.hk * G, row0 = it.tile * R;
+    const int64_t pidx = (int64_t)it.part_base + it.part;
+    auto out_row = [&](int r) {
+        const int gr = row0 + r, tok = gr / G;
+        return A.out + (int64_t)(it.s.q0 + tok) * A.out_stride + (int64_t)(first_head + gr - tok * G) * HD;
+    };
+    if constexpr (WR == 1) {
+        __shared__ float sh_m[C::NW][16], sh_l[C::NW][16];
+        constexpr int MLD = HDP + 4;
+        float* ma = reinterpret_cast<float*>(smem);
+        __syncthreads();  // every warp is done with the ring
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            float* p = ma + (warp * 16 + g) * MLD + d * 8 + 2 * t4;
+            *reinterpret_cast<float2*>(p) = make_float2(acc[d][0], acc[d][1]);
+            *reinterpret_cast<float2*>(p + 8 * MLD) = make_float2(acc[d][2], acc[d][3]);
+        }
+        if (t4 == 0) {
+            sh_m[warp][g] = m0, sh_m[warp][g + 8] = m1;
+            sh_l[warp][g] = l0, sh_l[warp][g + 8] = l1;
+        }
+        __syncthreads();
+        const int v4 = HD / 4;
+        for (int e = tid; e < rows * v4; e += NT) {
+            const int r = e / v4, x = (e - r * v4) * 4;
+            float M = sh_m[0][r], l = 0.f;
+#pragma unroll
+            for (int i = 1; i < C::NW; ++i) M = fmaxf(M, sh_m[i][r]);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < C::NW; ++i) {
+                const float c = M == -INFINITY ? 1.f : ex2(sh_m[i][r] - M);
+                const float4 y = *reinterpret_cast<const float4*>(ma + (i * 16 + r) * MLD + x);
+                l += c * sh_l[i][r];
+                o.x += c * y.x, o.y += c * y.y, o.z += c * y.z, o.w += c * y.w;
+            }
+            if (it.n_parts == 1) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                *reinterpret_cast<float4*>(out_row(r) + x) =
+                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            } else {
+                *reinterpret_cast<float4*>(A.part_acc + (pidx * R + r) * HD + x) = o;
+                if (x == 0) A.part_ml[pidx * R + r] = make_float2(M, l);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = wr + g + 8 * h;
+            if (r >= rows) continue;
+            const float m = h ? m1 : m0, l = h ? l1 : l0;
+            const bool whole = it.n_parts == 1;
+            const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            float* p = whole ? out_row(r) : A.part_acc + (pidx * R + r) * HD;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+                if (d * 8 < HD)
+                    *reinterpret_cast<float2*>(p + d * 8 + 2 * t4) =
+                        make_float2(acc[d][2 * h] * inv, acc[d][2 * h + 1] * inv);
+            if (!whole && t4 == 0) A.part_ml[pidx * R + r] = make_float2(m, l);
+        }
+    }
+}
+
+// ---- joining the ranges of a row tile ----------------------------------------------------
+// One CTA per (row tile, row): its four warps take every fourth range each.
+struct JoinArgs {
+    PagedView w;
+    SplitRule rule;
+    float* out;
+    int64_t out_stride;
+    const float* part_acc;
+    const float2* part_ml;
+};
+
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ JoinArgs A) {
+    constexpr int NT = 128, MAXV = 2;  // float4 per lane: head_dim 256
+    __shared__ float4 sh_acc[4][32 * MAXV];
+    __shared__ float sh_l[4];
+    const PagedView& w = A.w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Item it;
+    // cu_q and len were complete before the attention kernel started; its partials follow
+    const bool any = find_item<NT, true>(w, A.rule, blockIdx.x, it);
+    pdl_wait();
+    if (!any || it.n_parts == 1) return;
+    const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R, r = blockIdx.y;
+    if (r >= it.s.n * G - it.tile * R) return;
+    float M = -INFINITY, l = 0.f;
+    float4 o[MAXV];
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float2* ml = A.part_ml + (int64_t)it.part_base * R + r;
+    for (int p = lane; p < it.n_parts; p += 32) M = fmaxf(M, ml[(int64_t)p * R].x);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+#pragma unroll 4
+    for (int p = warp; p < it.n_parts; p += 4) {
+        const float2 y = ml[(int64_t)p * R];
+        const float c = M == -INFINITY ? 1.f : ex2(y.x - M);
+        l += c * y.y;
+        const float4* a =
+            reinterpret_cast<const float4*>(A.part_acc + ((int64_t)(it.part_base + p) * R + r) * HD);
+#pragma unroll
+        for (int i = 0; i < MAXV; ++i)
+            if (lane + 32 * i < HD / 4) {
+                const float4 x = a[lane + 32 * i];
+                o[i].x += c * x.x, o[i].y += c * x.y, o[i].z += c * x.z, o[i].w += c * x.w;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i) sh_acc[warp][lane + 32 * i] = o[i];
+    if (lane == 0) sh_l[warp] = l;
+    __syncthreads();
+    l = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int gr = it.tile * R + r, tok = gr / G;
+    float* out = A.out + (int64_t)(it.s.q0 + tok) * A.out_stride +
+                 (int64_t)(it.hk * G + gr - tok * G) * HD;
+    for (int x = threadIdx.x; x < HD / 4; x += NT) {
+        float4 y = sh_acc[0][x];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            const float4 z = sh_acc[i][x];
+            y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+        }
+        reinterpret_cast<float4*>(out)[x] = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    }
+}
+
+// ---- launches ----------------------------------------------------------------------------
+constexpr int kSMs = 148;  // of a B200: the items aimed at, and so the workspace, follow it
+
+// One kernel's share of a call.
+struct Share {
+    SplitRule rule;
+    int64_t tiles;  // most row tiles, over all kv heads
+    size_t acc_off, ml_off;
+};
+
+struct Plan {
+    int n = 0;
+    Share share[2];
+    size_t bytes = 0;
+};
+
+template <typename KV, int HDP, int WR>
+static SplitRule rows_rule(int min_rows, int max_rows) {
+    using C = RowsCfg<KV, HDP, WR>;
+    // two CTAs per SM for the narrow kernel, one for the wide: two rounds of them, so that
+    // uneven ranges even out; at least 128 positions, below which joining costs more
+    return SplitRule{C::R, C::KT, min_rows, max_rows, kSMs * (WR == 1 ? 4 : 2),
+                     std::max(1, 128 / C::KT)};
+}
+
+template <typename KV, int HDP, int WR>
+static int rows_launch(const RowsArgs& a, int64_t tiles, cudaStream_t st) {
+    using C = RowsCfg<KV, HDP, WR>;
+    auto kern = attn_rows_kernel<KV, HDP, WR>;
+    IB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)C::SMEM));
+    const int64_t grid = tiles + a.rule.target;
+    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(C::NT), C::SMEM, st, true, a));
+    return IB_OK;
+}
+
+// The kernels of a call, by the rows (new tokens x group) that a sequence may have: up to 16
+// on the narrow kernel, more on the wide one.  With one sequence, or a bound that rules the
+// wide one out, a single kernel takes everything.
+template <typename KV, int HDP>
+static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
+    constexpr int WIDE = HDP == 256 ? 4 : 8;
+    constexpr int ALL = 0x7fffffff;
+    const int64_t G = n_heads / p->n_kv_heads;
+    const int64_t most_q = b->max_q > 0 ? std::min(b->max_q, b->n_tokens) : b->n_tokens;
+    const int64_t seqs = std::min(b->n_seqs, b->n_tokens);
+    Plan plan;
+    auto add = [&](const SplitRule& r, int64_t tiles_per_head) {
+        Share& s = plan.share[plan.n++];
+        s.rule = r;
+        s.tiles = tiles_per_head * p->n_kv_heads;
+        auto take = [&](size_t n) {
+            const size_t at = plan.bytes;
+            plan.bytes += (n + 255) / 256 * 256;
+            return at;
+        };
+        // at most 2 x target partials: a tile of k > len key tiles has ceil(k / len) <= 2 k / len
+        s.acc_off = take((size_t)2 * r.target * r.R * p->head_dim * sizeof(float));
+        s.ml_off = take((size_t)2 * r.target * r.R * sizeof(float2));
+    };
+    const int64_t rows = b->n_tokens * G;
+    if (most_q * G <= 16) {
+        add(rows_rule<KV, HDP, 1>(1, ALL), seqs + rows / 16);
+    } else {
+        if (b->n_seqs > 1) add(rows_rule<KV, HDP, 1>(1, 16), seqs);
+        add(rows_rule<KV, HDP, WIDE>(b->n_seqs > 1 ? 17 : 1, ALL), seqs + rows / (16 * WIDE));
+    }
+    return plan;
+}
+
+template <typename KV, int HDP>
+static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan, RowsArgs a,
+                    uint8_t* ws, int64_t max_pos, cudaStream_t st) {
+    constexpr int WIDE = HDP == 256 ? 4 : 8;
+    for (int i = 0; i < plan.n; ++i) {
+        const Share& s = plan.share[i];
+        a.rule = s.rule;
+        a.part_acc = reinterpret_cast<float*>(ws + s.acc_off);
+        a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
+        const int r = s.rule.R == 16 ? rows_launch<KV, HDP, 1>(a, s.tiles, st)
+                                     : rows_launch<KV, HDP, WIDE>(a, s.tiles, st);
+        if (r != IB_OK) return r;
+        // no range is cut where the longest row of a table is no longer than the least
+        if (max_pos > (int64_t)s.rule.least * s.rule.KT) {
+            const JoinArgs j{a.w, s.rule, a.out, a.out_stride, a.part_acc, a.part_ml};
+            const int64_t G = a.w.H / a.w.Hkv;
+            const int64_t most_rows = std::min<int64_t>(s.rule.R, b->n_tokens * G);
+            IB_CUDA_CHECK(launch_pdl(attn_join_kernel, dim3((unsigned)s.tiles, (unsigned)most_rows),
+                                     dim3(128), 0, st, true, j));
+        }
+    }
+    return IB_OK;
+}
+
 template <typename KV>
-__global__ void __launch_bounds__(128)
-    attn_paged_kernel(const PagedView w, const float* __restrict__ q, int64_t q_stride,
-                      float* __restrict__ out, int64_t out_stride, const KV* __restrict__ kp,
-                      const KV* __restrict__ vp, float scale) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int t = row / w.H, h = row % w.H;
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < w.n_seqs; i += 128) seq_info(w, i);  // records bad values
-    if (t >= w.n_tokens) return;
-    int b = -1;
-    for (int i = 0; i < w.n_seqs; ++i)
-        if (t >= w.cu_q[i] && t < w.cu_q[i + 1]) b = i;
-    if (b < 0) return;
-    const SeqInfo s = seq_info(w, b);
-    const int pos = s.L - s.n + (t - s.q0);
-    float qv[8], acc[8] = {}, m = -INFINITY, l = 0.f;
-    const int hk = h / (w.H / w.Hkv);
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        qv[i] = d < w.HD ? q[t * q_stride + (int64_t)h * w.HD + d] : 0.f;
-    }
-    for (int p = 0; p <= pos; ++p) {
-        const int col = (int)w.ps.div((uint32_t)p);
-        const int page = page_at(w, s.row[col]);
-        if (page < 0) continue;
-        const size_t base = (((size_t)page * w.Hkv + hk) * w.page_size + (p - col * w.page_size)) * w.HD;
-        float x = 0.f;
-        for (int i = 0; i < 8; ++i) {
-            const int d = lane + 32 * i;
-            if (d < w.HD) x += qv[i] * kv_at(kp, base + d);
+static int attention_paged(const ib_kv_pages* p, const ib_kv_batch* b, RowsArgs a, void* ws,
+                           size_t* bytes, int64_t max_pos, cudaStream_t st) {
+    auto go = [&](auto hdp) {
+        constexpr int HDP = decltype(hdp)::value;
+        const Plan plan = make_plan<KV, HDP>(p, b, a.w.H);
+        if (bytes) {
+            *bytes = plan.bytes;
+            return (int)IB_OK;
         }
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        x *= scale;
-        const float mn = fmaxf(m, x);
-        const float c = expf(m - mn), e = expf(x - mn);
-        l = l * c + e;
-        for (int i = 0; i < 8; ++i) {
-            const int d = lane + 32 * i;
-            if (d < w.HD) acc[i] = acc[i] * c + e * kv_at(vp, base + d);
-        }
-        m = mn;
-    }
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        if (d < w.HD)
-            out[t * out_stride + (int64_t)h * w.HD + d] = m == -INFINITY && l == 0.f ? 0.f : acc[i] / l;
-    }
+        return run_plan<KV, HDP>(p, b, plan, a, (uint8_t*)ws, max_pos, st);
+    };
+    if (p->head_dim <= 64) return go(std::integral_constant<int, 64>{});
+    if (p->head_dim <= 128) return go(std::integral_constant<int, 128>{});
+    return go(std::integral_constant<int, 256>{});
+}
+
+static int attention_paged_any(const ib_kv_pages* p, const ib_kv_batch* b, const RowsArgs& a,
+                               void* ws, size_t* bytes, int64_t max_pos, cudaStream_t st) {
+    return p->type == IB_TYPE_F32 ? attention_paged<float>(p, b, a, ws, bytes, max_pos, st)
+                                  : attention_paged<__half>(p, b, a, ws, bytes, max_pos, st);
 }
 
 }  // namespace ib
@@ -71,7 +791,12 @@ extern "C" size_t ib_attention_paged_workspace(const ib_kv_pages* pages, const i
                                                const ib_kv_batch* batch, int n_heads) {
     if (paged_check_batch(pages, seqs, batch, 0, n_heads, "ib_attention_paged_workspace") != IB_OK)
         return 0;
-    return 256;
+    if (batch->n_tokens == 0 || batch->n_seqs == 0) return 256;
+    RowsArgs a{};
+    a.w = paged_view(pages, seqs, batch, n_heads);
+    size_t n = 0;
+    attention_paged_any(pages, batch, a, nullptr, &n, 0, nullptr);
+    return n;
 }
 
 extern "C" int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
@@ -86,23 +811,21 @@ extern "C" int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* se
                "multiples of 4");
     IB_REQUIRE(q_stride >= 0 && out_stride >= (int64_t)n_heads * pages->head_dim,
                "ib_attention_paged: bad row strides");
-    IB_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0 &&
-                   workspace_bytes >= ib_attention_paged_workspace(pages, seqs, batch, n_heads),
+    RowsArgs a{};
+    a.w = paged_view(pages, seqs, batch, n_heads);
+    size_t need = 0;
+    attention_paged_any(pages, batch, a, nullptr, &need, 0, nullptr);
+    IB_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need,
                "ib_attention_paged: workspace missing, too small or not 256-byte aligned");
-    const PagedView w = paged_view(pages, seqs, batch, n_heads);
-    const int64_t rows = (int64_t)batch->n_tokens * n_heads;
-    const int64_t off = (int64_t)layer * pages->n_pages * pages->n_kv_heads * pages->page_size *
-                        pages->head_dim;
-    const dim3 grid((unsigned)((rows + 3) / 4));
-    cudaStream_t st = as_stream(stream);
-    if (pages->type == IB_TYPE_F32)
-        attn_paged_kernel<float><<<grid, 128, 0, st>>>(w, q, q_stride, out, out_stride,
-                                                       (const float*)pages->k + off,
-                                                       (const float*)pages->v + off, scale);
-    else
-        attn_paged_kernel<__half><<<grid, 128, 0, st>>>(w, q, q_stride, out, out_stride,
-                                                        (const __half*)pages->k + off,
-                                                        (const __half*)pages->v + off, scale);
-    IB_LAUNCH_CHECK("attn_paged_kernel");
-    return IB_OK;
+    const int64_t layer_bytes = (int64_t)pages->n_pages * pages->n_kv_heads * pages->page_size *
+                                pages->head_dim * (pages->type == IB_TYPE_F32 ? 4 : 2);
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.k = (const uint8_t*)pages->k + layer * layer_bytes;
+    a.v = (const uint8_t*)pages->v + layer * layer_bytes;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    return attention_paged_any(pages, batch, a, workspace, nullptr,
+                               (int64_t)seqs->max_pages * pages->page_size, as_stream(stream));
 }
