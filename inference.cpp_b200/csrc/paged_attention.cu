@@ -147,19 +147,22 @@ __device__ __forceinline__ bool find_item(const PagedView& w, const SplitRule& r
     return sh_found == 1;
 }
 
-// ---- rows on mma.sync --------------------------------------------------------------------
-// For few rows (single tokens, short drafts), where the bound is reading K and V once, and
-// for FP32 pages.  A CTA holds 16 rows (WR = 1: its four warps take a quarter of each key
-// tile's positions each, and join at the end) or WR tiles of 16 rows (one per warp, all over
-// the same key tiles).  Products of FP32 operands keep about 2^-20:
+// ---- 16 rows on mma.sync -----------------------------------------------------------------
+// A warp's 16 query rows against KW positions at a time.  Products of FP32 operands keep about
+// 2^-21:
 //   FP16 pages  q = hi + lo and p = hi + lo in FP16, K and V as they are: two m16n8k16 per
 //               product.  q rows are scaled to a largest element in [256, 512) and p by 2^10,
 //               powers of two that keep the lo parts out of FP16's subnormals.
 //   FP32 pages  both operands as TF32 hi + lo, hi hi + hi lo + lo hi: three m16n8k8, with the
 //               range of FP32.
+// The MMA adds to its FP32 accumulator by cutting, half a unit of the accumulator per step on
+// average and always towards zero: a running sum over a long sequence would drift (2.6e-6 of
+// the result over 131072 positions).  So lo parts have accumulators of their own, and p v of
+// each tile starts from zero and is added to the running sum by FFMA, which rounds and takes
+// the rescaling with it.
 // Positions that a row does not see get a score of -inf; pages that are not there are filled
-// with zeros, and in tiles where some row does not see a position that has a page, V is
-// checked for values that are not finite (0 x inf).
+// with zeros, and in tiles where some row does not see a position that has a page (`careful`),
+// V is checked for values that are not finite (0 x inf).
 struct RowsArgs {
     PagedView w;
     SplitRule rule;
@@ -170,29 +173,6 @@ struct RowsArgs {
     float* part_acc;    // [partial][R][HD]
     float2* part_ml;    // [partial][R]
     float scale_log2;   // scale * log2(e)
-};
-
-template <typename KV, int HDP, int WR>
-struct RowsCfg {
-    static constexpr bool F32 = sizeof(KV) == 4;
-    static constexpr int NW = WR == 1 ? 4 : WR, NT = NW * 32, R = 16 * WR;
-    static constexpr int ROWB = HDP * (int)sizeof(KV);  // bytes of a K or V row
-    static constexpr int LD = ROWB + 16;                // padded: 8 rows of an ldmatrix, and the
-                                                        // TF32 V columns, hit distinct banks
-    static constexpr int KT = !F32 ? 64 : HDP == 256 && WR > 1 ? 16 : 32;
-    static constexpr int STAGES = ROWB > 256 ? 2 : F32 ? 4 : 3;
-    static constexpr int KW = WR == 1 ? KT / NW : KT;  // positions of a warp
-    static constexpr int QLD = HDP * (F32 ? 4 : 2) + 16;
-    static constexpr int Q_BYTES = 2 * R * QLD;  // hi and lo
-    static constexpr int STAGE = 2 * KT * LD;
-    static constexpr int RING = STAGES + 1;  // of row offsets
-    static constexpr int MERGE = WR == 1 ? NW * 16 * (HDP + 4) * 4 : 0;  // joins the warps
-    static constexpr int BODY = STAGES * STAGE > MERGE ? STAGES * STAGE : MERGE;
-    // q fragments that stay in registers are staged in the ring's last slot, whose first copy
-    // is issued after they were read
-    static constexpr bool QREG = !F32 && HDP <= 128;
-    static constexpr int Q_OFF = QREG ? (STAGES - 1) * STAGE : BODY;
-    static constexpr size_t SMEM = Q_OFF + Q_BYTES > BODY ? Q_OFF + Q_BYTES : BODY;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
@@ -214,40 +194,499 @@ __device__ __forceinline__ uint32_t finite16x2(uint32_t x, bool& odd) {
     return x;
 }
 
-template <typename KV, int HDP, int WR>
-__global__ void __launch_bounds__(RowsCfg<KV, HDP, WR>::NT)
-    attn_rows_kernel(const __grid_constant__ RowsArgs A) {
-    using C = RowsCfg<KV, HDP, WR>;
-    constexpr int NT = C::NT, R = C::R, KT = C::KT, KW = C::KW, LD = C::LD;
-    constexpr bool F32 = C::F32;
-    constexpr int NB = KW / 8;     // score columns of a warp, in blocks of 8
-    constexpr int DB = HDP / 8;    // output columns, in blocks of 8
-    constexpr int KS = F32 ? HDP / 8 : HDP / 16;  // k-steps of q.k
+// One query row into shared memory as hi and lo parts, by one warp.  Returns the factor that
+// turns its scores into base-2 exponents.
+template <bool F32, int HDP>
+__device__ __forceinline__ float stage_q_row(const float* row, int HD, uint8_t* hi, uint8_t* lo,
+                                             float scale_log2) {
+    const int lane = threadIdx.x & 31;
+    float x[HDP / 32], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < HDP / 32; ++i) {
+        const int d = lane + 32 * i;
+        x[i] = row && d < HD ? row[d] : 0.f;
+        top = fmaxf(top, fabsf(x[i]));
+    }
+    if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < HDP / 32; ++i)
+            split_tf32(x[i], reinterpret_cast<uint32_t*>(hi)[lane + 32 * i],
+                       reinterpret_cast<uint32_t*>(lo)[lane + 32 * i]);
+        return scale_log2;
+    } else {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // 2^(8 - e) with e the exponent of the largest element, and its inverse
+        const int e = max(-100, (int)((__float_as_uint(top) >> 23) & 255u) - 127);
+        const bool plain = top == 0.f || e > 127;
+        const float up = plain ? 1.f : __uint_as_float((uint32_t)(8 - e + 127) << 23);
+        const float down = plain ? 1.f : __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+#pragma unroll
+        for (int i = 0; i < HDP / 32; ++i) {
+            const float y = x[i] * up;
+            const __half h = __float2half_rn(y);
+            reinterpret_cast<__half*>(hi)[lane + 32 * i] = h;
+            reinterpret_cast<__half*>(lo)[lane + 32 * i] = __float2half_rn(y - __half2float(h));
+        }
+        return scale_log2 * down;
+    }
+}
+
+// QREG: the q fragments stay in registers.  LD: bytes between K or V rows in shared memory
+// (16 more than a row: the 8 rows of an ldmatrix, and the TF32 V columns, hit distinct banks);
+// QLD: the same for q.
+template <typename KV, int HDP, int KW, bool QREG>
+struct WarpRows {
+    static constexpr bool F32 = sizeof(KV) == 4;
+    static constexpr int LD = HDP * (int)sizeof(KV) + 16, QLD = HDP * (F32 ? 4 : 2) + 16;
+    static constexpr int NB = KW / 8, DB = HDP / 8, KS = F32 ? HDP / 8 : HDP / 16;
+    // p is carried times 2^10 (FP16 pages)
+    static constexpr float P_BIAS = F32 ? 0.f : 10.f;
+
+    float acc[DB][4];
+    float m[2], l[2];
+    int lim[2];     // last positions that rows g and g + 8 see
+    float sc[2];
+    uint32_t qh[QREG ? KS : 1][4], ql[QREG ? KS : 1][4];
+    uint32_t q_hi, q_lo;  // this lane's fragment addresses
+
+    __device__ __forceinline__ void start(uint32_t hi, uint32_t lo) {
+        const int lane = threadIdx.x & 31;
+        q_hi = hi + (uint32_t)((lane & 15) * QLD + (lane >> 4) * 16);
+        q_lo = lo + (uint32_t)((lane & 15) * QLD + (lane >> 4) * 16);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[d][i] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+        if constexpr (QREG) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) load_q(k, qh[k], ql[k]);
+        }
+    }
+
+    __device__ __forceinline__ void load_q(int k, uint32_t (&h)[4], uint32_t (&e)[4]) const {
+        ldsm_x4(q_hi + k * 32, h[0], h[1], h[2], h[3]);
+        ldsm_x4(q_lo + k * 32, e[0], e[1], e[2], e[3]);
+    }
+
+    // kd, vd: the tile's K and V in shared memory (v_ptr: vd as a pointer); pos_of(j): the
+    // position of tile row j, j = 8 n + 2 t4 + (0 or 1) of this lane or, for a j that is the
+    // same in the whole warp, any.
+    template <typename Pos>
+    __device__ __forceinline__ void step(uint32_t kd, uint32_t vd, const uint8_t* v_ptr, bool careful,
+                                         Pos pos_of) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+        float s[NB][4], e[NB][4];
+        zero(s), zero(e);
+        if constexpr (!F32) {
+            float s2[NB <= 2 ? NB : 1][4];  // a second chain for the upper half of head_dim
+            zero(s2);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t ah[4], al[4];
+                if constexpr (QREG) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) ah[j] = qh[k][j], al[j] = ql[k][j];
+                } else {
+                    load_q(k, ah, al);
+                }
+#pragma unroll
+                for (int n = 0; n < NB; n += 2) {  // 16 positions x 16 dimensions
+                    uint32_t b[4];
+                    ldsm_x4(kd + (uint32_t)((n * 8 + (lane & 7) + ((lane >> 4) << 3)) * LD + k * 32 +
+                                            ((lane >> 3) & 1) * 16),
+                            b[0], b[1], b[2], b[3]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if constexpr (NB <= 2) mma16816(k < KS / 2 ? s[n + j] : s2[n + j], ah, b[2 * j], b[2 * j + 1]);
+                        else mma16816(s[n + j], ah, b[2 * j], b[2 * j + 1]);
+                        mma16816(e[n + j], al, b[2 * j], b[2 * j + 1]);
+                    }
+                }
+            }
+            if constexpr (NB <= 2) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[n][j] += s2[n][j];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; k += 2) {
+                uint32_t ah[2][4], al[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) load_q(k + j, ah[j], al[j]);
+                float t[NB][4];  // two k-steps at a time
+                zero(t);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {  // 8 positions x 16 dimensions
+                    uint32_t b[4], h[4], r[4];
+                    ldsm_x4(kd + (uint32_t)((n * 8 + (lane & 7)) * LD + k * 32 + (lane >> 3) * 16),
+                            b[0], b[1], b[2], b[3]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(b[j]), h[j], r[j]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        mma1688_tf32(t[n], ah[j], h[2 * j], h[2 * j + 1]);
+                        mma1688_tf32(e[n], ah[j], r[2 * j], r[2 * j + 1]);
+                        mma1688_tf32(e[n], al[j], h[2 * j], h[2 * j + 1]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[n][j] += t[n][j];
+                }
+            }
+        }
+        // what the rows do not see, and the running maximum
+        float x[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int p0 = pos_of(n * 8 + 2 * t4), p1 = pos_of(n * 8 + 2 * t4 + 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float &a = s[n][2 * h], &b = s[n][2 * h + 1];
+                a = p0 <= lim[h] ? (a + e[n][2 * h]) * sc[h] : -INFINITY;
+                b = p1 <= lim[h] ? (b + e[n][2 * h + 1]) * sc[h] : -INFINITY;
+                x[h] = fmaxf(x[h], fmaxf(a, b));
+            }
+        }
+        float c[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int o = 1; o <= 2; o <<= 1) x[h] = fmaxf(x[h], __shfl_xor_sync(0xffffffffu, x[h], o));
+            x[h] = fmaxf(m[h], x[h]);
+            c[h] = x[h] == -INFINITY ? 1.f : ex2(m[h] - x[h]);
+            m[h] = x[h];
+            l[h] *= c[h];
+            const float base = m[h] == -INFINITY ? 0.f : m[h] - P_BIAS;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float &a = s[n][2 * h], &b = s[n][2 * h + 1];
+                a = ex2(a - base), b = ex2(b - base);
+                l[h] += a + b;
+            }
+        }
+        bool odd = false;  // a V value that is not finite, among this thread's
+        if constexpr (!F32) {
+            uint32_t ph[KW / 16][4], pl[KW / 16][4];
+#pragma unroll
+            for (int k = 0; k < KW / 16; ++k) {
+                split2(s[2 * k][0], s[2 * k][1], ph[k][0], pl[k][0]);
+                split2(s[2 * k][2], s[2 * k][3], ph[k][1], pl[k][1]);
+                split2(s[2 * k + 1][0], s[2 * k + 1][1], ph[k][2], pl[k][2]);
+                split2(s[2 * k + 1][2], s[2 * k + 1][3], ph[k][3], pl[k][3]);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; d += 2) {
+                float t[2][4];
+                zero(t);
+#pragma unroll
+                for (int k = 0; k < KW / 16; ++k) {
+                    uint32_t b[4];
+                    ldsm_x4_t(vd + (uint32_t)((k * 16 + (lane & 15)) * LD + d * 16 + (lane >> 4) * 16),
+                              b[0], b[1], b[2], b[3]);
+                    if (careful) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) b[j] = finite16x2(b[j], odd);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        mma16816(t[j], pl[k], b[2 * j], b[2 * j + 1]);
+                        mma16816(t[j], ph[k], b[2 * j], b[2 * j + 1]);
+                    }
+                }
+                add(d, t[0], c), add(d + 1, t[1], c);
+            }
+        } else {
+            // the MMA's k index t holds position 2 t, t + 4 position 2 t + 1, in both operands:
+            // then the scores' accumulator is the A operand as it lies
+            uint32_t ph[NB][4], pl[NB][4];
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+                split_tf32(s[k][0], ph[k][0], pl[k][0]);
+                split_tf32(s[k][2], ph[k][1], pl[k][1]);
+                split_tf32(s[k][1], ph[k][2], pl[k][2]);
+                split_tf32(s[k][3], ph[k][3], pl[k][3]);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                float t[1][4], r[1][4];
+                zero(t), zero(r);
+#pragma unroll
+                for (int k = 0; k < NB; ++k) {
+                    const uint8_t* v0 = v_ptr + (k * 8 + 2 * t4) * LD + d * 32 + g * 4;
+                    float y0 = *reinterpret_cast<const float*>(v0);
+                    float y1 = *reinterpret_cast<const float*>(v0 + LD);
+                    if (careful) {
+                        if (!(fabsf(y0) < INFINITY)) odd = true, y0 = 0.f;
+                        if (!(fabsf(y1) < INFINITY)) odd = true, y1 = 0.f;
+                    }
+                    uint32_t h0, r0, h1, r1;
+                    split_tf32(y0, h0, r0);
+                    split_tf32(y1, h1, r1);
+                    mma1688_tf32(t[0], ph[k], h0, h1);
+                    mma1688_tf32(r[0], ph[k], r0, r1);
+                    mma1688_tf32(r[0], pl[k], h0, h1);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) t[0][j] += r[0][j];
+                add(d, t[0], c);
+            }
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+            // rows that see such a value are not finite there
+#pragma unroll 1
+            for (int j = 0; j < KW; ++j) {
+                const int pos = pos_of(j);
+                const uint8_t* vr = v_ptr + j * LD;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = d * 8 + 2 * t4 + i;
+                        float y;
+                        if constexpr (F32) y = reinterpret_cast<const float*>(vr)[at];
+                        else y = __half2float(reinterpret_cast<const __half*>(vr)[at]);
+                        if (fabsf(y) < INFINITY) continue;
+                        if (pos <= lim[0]) acc[d][i] = NAN;
+                        if (pos <= lim[1]) acc[d][2 + i] = NAN;
+                    }
+            }
+        }
+    }
+
+    // the sums of a row are spread over its four lanes
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int o = 1; o <= 2; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+    }
+
+    template <int N>
+    static __device__ __forceinline__ void zero(float (&x)[N][4]) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[n][j] = 0.f;
+    }
+    __device__ __forceinline__ void add(int d, const float (&t)[4], const float (&c)[2]) {
+        acc[d][0] = fmaf(acc[d][0], c[0], t[0]), acc[d][1] = fmaf(acc[d][1], c[0], t[1]);
+        acc[d][2] = fmaf(acc[d][2], c[1], t[2]), acc[d][3] = fmaf(acc[d][3], c[1], t[3]);
+    }
+};
+
+__device__ __forceinline__ float* out_row(const RowsArgs& A, const Item& it, int G, int gr) {
+    const int tok = gr / G;
+    return A.out + (int64_t)(it.s.q0 + tok) * A.out_stride +
+           (int64_t)(it.hk * G + gr - tok * G) * A.w.HD;
+}
+
+// ---- up to 16 rows: single tokens and short drafts ---------------------------------------
+// The bound is reading K and V once.  A CTA holds the 16 rows; each of its warps runs through
+// every NW-th group of KW positions by itself -- its own ring in shared memory, filled by its
+// own cp.async, no barrier in the loop -- so that one warp's chain of loads, scores, maximum and
+// products hides behind the others'; they join at the end.
+template <typename KV, int HDP>
+struct NarrowCfg {
+    static constexpr bool F32 = sizeof(KV) == 4;
+    static constexpr int KW = F32 ? 8 : 16;
+    static constexpr bool QREG = !F32 && HDP <= 128;
+    using Tile = WarpRows<KV, HDP, KW, QREG>;
+    static constexpr int NW = HDP == 256 ? 4 : 8, NT = NW * 32;
+    static constexpr int STAGES = F32 && HDP == 256 ? 2 : 3;
+    static constexpr int STAGE = 2 * KW * Tile::LD;
+    static constexpr int Q_BYTES = 2 * 16 * Tile::QLD;
+    static constexpr int RING = NW * STAGES * STAGE;
+    static constexpr int MERGE = NW * 16 * (HDP + 4) * 4;  // of the warps' results, in the ring
+    static constexpr size_t SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
+    // CTAs that an SM holds
+    static constexpr int CTAS = HDP == 64 ? 2 : 1;
+};
+
+template <typename KV, int HDP>
+__global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CTAS)
+    attn_narrow_kernel(const __grid_constant__ RowsArgs A) {
+    using C = NarrowCfg<KV, HDP>;
+    using T = typename C::Tile;
+    constexpr int KW = C::KW, LD = T::LD, S = C::STAGES, NW = C::NW;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ long long row_off[C::RING][KT];  // element offset of a position's row, -1: none
-    __shared__ __align__(8) int key_pos[C::RING][KT];  // its position, INT_MAX: none
-    __shared__ float row_scale[R];
-    __shared__ int row_lim[R];  // last position that the row sees
+    __shared__ float row_scale[16], sh_m[NW][16], sh_l[NW][16];
     const PagedView& w = A.w;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = lane >> 2, t4 = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
+    pdl_wait();
+    pdl_launch_dependents();
+    Item it;
+    if (!find_item<C::NT, false>(w, A.rule, blockIdx.x, it)) return;
+    const int G = w.H / w.Hkv, HD = w.HD, row0 = it.tile * 16;
+    const int rows = min(16, it.s.n * G - row0);
+    const int start = it.s.L - it.s.n;  // position of the first new token
+    const int first_lim = start + row0 / G, last_lim = start + (row0 + rows - 1) / G;
+    const int kt0 = it.kt0 + warp, kt1 = min(it.kt1, last_lim < 0 ? 0 : last_lim / KW + 1);
+    uint8_t* ring = smem + C::Q_BYTES + warp * S * C::STAGE;
+    const uint32_t ring_a = smem_u32(ring);
+
+    // Lane j holds position j of a tile (j < KW, twice or four times over): where its row starts
+    // in the layer (-1: nowhere) and the position itself (INT_MAX: none).
+    auto entry_of = [&](int kt) -> int {  // read a tile ahead of the copies that need it
+        const int pos = kt * KW + (lane & (KW - 1));
+        if (kt >= kt1 || pos > last_lim) return -1;
+        return page_at(w, it.s.row[w.ps.div((uint32_t)pos)]);
+    };
+    const int cpr = HD * (int)sizeof(KV) / 16;  // 16-byte chunks of a row that exist
+    constexpr int CH = HDP * (int)sizeof(KV) / 16;  // and with padding
+    auto issue = [&](int kt, int slot, int page) -> int {
+        const int pos = kt * KW + (lane & (KW - 1));
+        if (kt < kt1) {
+            const int in_page = pos - (int)w.ps.div((uint32_t)pos) * w.page_size;
+            const long long off =
+                page < 0 ? -1 : (((long long)page * w.Hkv + it.hk) * w.page_size + in_page) * HD;
+            const uint32_t d0 = ring_a + (uint32_t)(slot * C::STAGE);
+#pragma unroll
+            for (int c = lane; c < KW * CH; c += 32) {
+                const int r = c / CH, x = c % CH;  // CH: 8 or more, so r is within the lanes
+                const long long o = __shfl_sync(0xffffffffu, off, r);
+                const bool ok = o >= 0 && x < cpr;
+                const size_t byte = ok ? (size_t)o * sizeof(KV) + (size_t)x * 16 : 0;
+                const uint32_t d = d0 + (uint32_t)(r * LD + x * 16);
+                cp16(d, (const uint8_t*)A.k + byte, ok);
+                cp16(d + KW * LD, (const uint8_t*)A.v + byte, ok);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return page < 0 ? 0x7fffffff : pos;
+    };
+    int pos[S];  // of the tiles in flight, the oldest first
+    {
+        int page[S - 1];
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) page[i] = entry_of(kt0 + i * NW);
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) pos[i] = issue(kt0 + i * NW, i, page[i]);
+    }
+    int next_page = entry_of(kt0 + (S - 1) * NW);
+
+    for (int r = warp; r < 16; r += NW) {
+        const int gr = row0 + r, tok = gr / G;
+        const float* src = r < rows ? A.q + (int64_t)(it.s.q0 + tok) * A.q_stride +
+                                          (int64_t)(it.hk * G + gr - tok * G) * HD
+                                    : nullptr;
+        uint8_t* hi = smem + r * T::QLD;
+        const float f = stage_q_row<C::F32, HDP>(src, HD, hi, hi + 16 * T::QLD, A.scale_log2);
+        if (lane == 0) row_scale[r] = f;
+    }
+    __syncthreads();
+    T t;
+    t.start(smem_u32(smem), smem_u32(smem) + 16 * T::QLD);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = g + 8 * h;
+        t.lim[h] = r < rows ? start + (row0 + r) / G : -1;
+        t.sc[h] = row_scale[r];
+    }
+    int slot = 0;
+    for (int kt = kt0; kt < kt1; kt += NW) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        __syncwarp();  // every lane's copies of this tile, and its reads of the one before
+        const int fill = slot == 0 ? S - 1 : slot - 1;  // the slot before: the tile of last time
+        pos[S - 1] = issue(kt + (S - 1) * NW, fill, next_page);
+        next_page = entry_of(kt + S * NW);
+        const uint32_t kd = ring_a + (uint32_t)(slot * C::STAGE);
+        const int mine = pos[0];
+        t.step(kd, kd + KW * LD, ring + slot * C::STAGE + KW * LD, kt * KW + KW - 1 > first_lim,
+               [&](int j) { return __shfl_sync(0xffffffffu, mine, j); });
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) pos[i] = pos[i + 1];
+        slot = slot == S - 1 ? 0 : slot + 1;
+    }
+    t.finish();
+
+    // ---- the warps' results together, in the ring ----
+    constexpr int MLD = HDP + 4;
+    float* ma = reinterpret_cast<float*>(smem + C::Q_BYTES);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < T::DB; ++d) {
+        float* p = ma + (warp * 16 + g) * MLD + d * 8 + 2 * (lane & 3);
+        *reinterpret_cast<float2*>(p) = make_float2(t.acc[d][0], t.acc[d][1]);
+        *reinterpret_cast<float2*>(p + 8 * MLD) = make_float2(t.acc[d][2], t.acc[d][3]);
+    }
+    if ((lane & 3) == 0) {
+        sh_m[warp][g] = t.m[0], sh_m[warp][g + 8] = t.m[1];
+        sh_l[warp][g] = t.l[0], sh_l[warp][g + 8] = t.l[1];
+    }
+    __syncthreads();
+    const int64_t pidx = (int64_t)it.part_base + it.part;
+    const int v4 = HD / 4;
+    for (int e = tid; e < rows * v4; e += C::NT) {
+        const int r = e / v4, x = (e - r * v4) * 4;
+        float M = sh_m[0][r], l = 0.f;
+#pragma unroll
+        for (int i = 1; i < NW; ++i) M = fmaxf(M, sh_m[i][r]);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const float c = M == -INFINITY ? 1.f : ex2(sh_m[i][r] - M);
+            const float4 y = *reinterpret_cast<const float4*>(ma + (i * 16 + r) * MLD + x);
+            l += c * sh_l[i][r];
+            o.x += c * y.x, o.y += c * y.y, o.z += c * y.z, o.w += c * y.w;
+        }
+        if (it.n_parts == 1) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            *reinterpret_cast<float4*>(out_row(A, it, G, row0 + r) + x) =
+                make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        } else {
+            *reinterpret_cast<float4*>(A.part_acc + (pidx * 16 + r) * HD + x) = o;
+            if (x == 0) A.part_ml[pidx * 16 + r] = make_float2(M, l);
+        }
+    }
+}
+
+// ---- more rows on mma.sync ---------------------------------------------------------------
+// WR warps of 16 rows each over the same key tiles, which the CTA brings in together.
+template <typename KV, int HDP>
+struct WideCfg {
+    static constexpr bool F32 = sizeof(KV) == 4;
+    static constexpr int WR = HDP == 256 ? 4 : 8, NT = WR * 32, R = 16 * WR;
+    static constexpr int ROWB = HDP * (int)sizeof(KV);
+    static constexpr int KT = ROWB <= 128 ? 64 : ROWB <= 512 ? 32 : 16;
+    static constexpr bool QREG = !F32 && HDP <= 128;
+    using Tile = WarpRows<KV, HDP, KT, QREG>;
+    static constexpr int STAGES = ROWB > 256 ? 2 : 4;
+    static constexpr int Q_BYTES = 2 * R * Tile::QLD;
+    static constexpr int STAGE = 2 * KT * Tile::LD;
+    static constexpr int RING = STAGES + 1;  // of row offsets: a tile's outlive its copies
+    static constexpr size_t SMEM = (size_t)Q_BYTES + STAGES * STAGE;
+};
+
+template <typename KV, int HDP>
+__global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
+    attn_wide_kernel(const __grid_constant__ RowsArgs A) {
+    using C = WideCfg<KV, HDP>;
+    using T = typename C::Tile;
+    constexpr int NT = C::NT, R = C::R, KT = C::KT, LD = T::LD, S = C::STAGES;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ long long row_off[C::RING][KT];  // where a position's row starts, -1: nowhere
+    __shared__ int key_pos[C::RING][KT];        // its position, INT_MAX: none
+    __shared__ float row_scale[R];
+    const PagedView& w = A.w;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
     pdl_wait();
     pdl_launch_dependents();
     Item it;
     if (!find_item<NT, false>(w, A.rule, blockIdx.x, it)) return;
-    const int G = w.H / w.Hkv, HD = w.HD;
-    const int rows = min(R, it.s.n * G - it.tile * R);
-    const int first_lim = it.s.L - it.s.n + it.tile * R / G;
-    const int last_lim = it.s.L - it.s.n + (it.tile * R + rows - 1) / G;
-    uint8_t* q_smem = smem + C::Q_OFF;
-    const uint32_t kv_base = smem_u32(smem), q_base = kv_base + C::Q_OFF;
-
-    // key tiles that some row sees
+    const int G = w.H / w.Hkv, HD = w.HD, row0 = it.tile * R;
+    const int rows = min(R, it.s.n * G - row0);
+    const int start = it.s.L - it.s.n;
+    const int first_lim = start + row0 / G, last_lim = start + (row0 + rows - 1) / G;
     const int kt0 = it.kt0, kt1 = min(it.kt1, last_lim < 0 ? 0 : last_lim / KT + 1);
     const int n_kt = max(0, kt1 - kt0);
+    const uint32_t q_base = smem_u32(smem), kv_base = q_base + C::Q_BYTES;
 
-    // table entries are read one tile ahead of the copies that need them
-    auto entry_of = [&](int kt) -> int {
+    auto entry_of = [&](int kt) -> int {  // read a tile ahead of the copies that need it
         const int pos = kt * KT + tid;
         if (tid >= KT || kt >= kt1 || pos > last_lim) return -1;
         return page_at(w, it.s.row[w.ps.div((uint32_t)pos)]);
@@ -260,10 +699,10 @@ __global__ void __launch_bounds__(RowsCfg<KV, HDP, WR>::NT)
             page < 0 ? -1 : (((long long)page * w.Hkv + it.hk) * w.page_size + in_page) * HD;
         key_pos[i % C::RING][tid] = page < 0 ? 0x7fffffff : pos;
     };
-    const int cpr = HD * (int)sizeof(KV) / 16;  // 16-byte chunks of a row that exist
+    const int cpr = HD * (int)sizeof(KV) / 16;
     auto issue = [&](int i) {
         if (i < n_kt) {
-            const uint32_t kd = kv_base + (uint32_t)((i % C::STAGES) * C::STAGE);
+            const uint32_t kd = kv_base + (uint32_t)((i % S) * C::STAGE);
             constexpr int CH = C::ROWB / 16, N = KT * CH;
 #pragma unroll 4
             for (int c = tid; c < N; c += NT) {
@@ -279,324 +718,55 @@ __global__ void __launch_bounds__(RowsCfg<KV, HDP, WR>::NT)
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) put_offsets(i, entry_of(kt0 + i));
+    for (int i = 0; i < S - 1; ++i) put_offsets(i, entry_of(kt0 + i));
     __syncthreads();
-    for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
-    int next_page = entry_of(kt0 + C::STAGES - 1);
+    for (int i = 0; i < S - 1; ++i) issue(i);
+    int next_page = entry_of(kt0 + S - 1);
 
-    // q rows to shared memory as hi and lo parts
-    for (int r = warp; r < R; r += C::NW) {
-        float x[HDP / 32];
-        const int gr = it.tile * R + r, tok = gr / G, head = it.hk * G + gr - tok * G;
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < HDP / 32; ++i) {
-            const int d = lane + 32 * i;
-            x[i] = r < rows && d < HD
-                       ? A.q[(int64_t)(it.s.q0 + tok) * A.q_stride + (int64_t)head * HD + d]
-                       : 0.f;
-            top = fmaxf(top, fabsf(x[i]));
-        }
-        if constexpr (F32) {
-#pragma unroll
-            for (int i = 0; i < HDP / 32; ++i) {
-                uint32_t h, l;
-                split_tf32(x[i], h, l);
-                const int o = r * C::QLD + (lane + 32 * i) * 4;
-                *reinterpret_cast<uint32_t*>(q_smem + o) = h;
-                *reinterpret_cast<uint32_t*>(q_smem + R * C::QLD + o) = l;
-            }
-            if (lane == 0) row_scale[r] = A.scale_log2;
-        } else {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // 2^(8 - e) with e the exponent of the largest element, and its inverse
-            const int e = max(-100, (int)((__float_as_uint(top) >> 23) & 255u) - 127);
-            const bool plain = top == 0.f || e > 127;
-            const float up = plain ? 1.f : __uint_as_float((uint32_t)(8 - e + 127) << 23);
-            const float down = plain ? 1.f : __uint_as_float((uint32_t)(e - 8 + 127) << 23);
-#pragma unroll
-            for (int i = 0; i < HDP / 32; ++i) {
-                const float y = x[i] * up;
-                const __half h = __float2half_rn(y);
-                const int o = r * C::QLD + (lane + 32 * i) * 2;
-                *reinterpret_cast<__half*>(q_smem + o) = h;
-                *reinterpret_cast<__half*>(q_smem + R * C::QLD + o) =
-                    __float2half_rn(y - __half2float(h));
-            }
-            if (lane == 0) row_scale[r] = A.scale_log2 * down;
-        }
-        if (lane == 0) row_lim[r] = r < rows ? it.s.L - it.s.n + tok : -1;
-    }
-    __syncthreads();
-
-    const int wr = WR == 1 ? 0 : warp * 16;    // first row of this warp
-    const int wk = WR == 1 ? warp * KW : 0;    // its first position in a tile
-    const uint32_t q_frag = q_base + (uint32_t)((wr + (lane & 15)) * C::QLD + (lane >> 4) * 16);
-    const int lim0 = row_lim[wr + g], lim1 = row_lim[wr + g + 8];
-    const float sc0 = row_scale[wr + g], sc1 = row_scale[wr + g + 8];
-    uint32_t qh[C::QREG ? KS : 1][4], ql[C::QREG ? KS : 1][4];
-    if constexpr (C::QREG) {
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            ldsm_x4(q_frag + k * 32, qh[k][0], qh[k][1], qh[k][2], qh[k][3]);
-            ldsm_x4(q_frag + R * C::QLD + k * 32, ql[k][0], ql[k][1], ql[k][2], ql[k][3]);
-        }
-    }
-    float acc[DB][4];
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[d][i] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    // p is carried times 2^10 (FP16 pages): see above
-    constexpr float P_BIAS = F32 ? 0.f : 10.f;
-
-    for (int i = 0; i < n_kt; ++i) {
-        if (i + C::STAGES - 1 < n_kt) put_offsets(i + C::STAGES - 1, next_page);
-        asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
-        __syncthreads();
-        issue(i + C::STAGES - 1);
-        next_page = entry_of(kt0 + i + C::STAGES);
-        const uint32_t kd = kv_base + (uint32_t)((i % C::STAGES) * C::STAGE + wk * LD);
-        const uint32_t vd = kd + KT * LD;
-        const int* kp = &key_pos[i % C::RING][wk];
-
-        // scores: 16 rows x KW positions
-        float s[NB][4];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
-        if constexpr (!F32) {
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint32_t ah[4], al[4];
-                if constexpr (C::QREG) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) ah[j] = qh[k][j], al[j] = ql[k][j];
-                } else {
-                    ldsm_x4(q_frag + k * 32, ah[0], ah[1], ah[2], ah[3]);
-                    ldsm_x4(q_frag + R * C::QLD + k * 32, al[0], al[1], al[2], al[3]);
-                }
-#pragma unroll
-                for (int n = 0; n < NB; n += 2) {  // 16 positions x 16 dimensions
-                    uint32_t b[4];
-                    ldsm_x4(kd + (uint32_t)((n * 8 + (lane & 7) + ((lane >> 4) << 3)) * LD + k * 32 +
-                                            ((lane >> 3) & 1) * 16),
-                            b[0], b[1], b[2], b[3]);
-                    mma16816(s[n], ah, b[0], b[1]);
-                    mma16816(s[n + 1], ah, b[2], b[3]);
-                    mma16816(s[n], al, b[0], b[1]);
-                    mma16816(s[n + 1], al, b[2], b[3]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < KS; k += 2) {
-                uint32_t ah[2][4], al[2][4];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    ldsm_x4(q_frag + (k + j) * 32, ah[j][0], ah[j][1], ah[j][2], ah[j][3]);
-                    ldsm_x4(q_frag + R * C::QLD + (k + j) * 32, al[j][0], al[j][1], al[j][2],
-                            al[j][3]);
-                }
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {  // 8 positions x 16 dimensions
-                    uint32_t b[4], h[4], e[4];
-                    ldsm_x4(kd + (uint32_t)((n * 8 + (lane & 7)) * LD + k * 32 + (lane >> 3) * 16),
-                            b[0], b[1], b[2], b[3]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(b[j]), h[j], e[j]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        mma1688_tf32(s[n], ah[j], h[2 * j], h[2 * j + 1]);
-                        mma1688_tf32(s[n], ah[j], e[2 * j], e[2 * j + 1]);
-                        mma1688_tf32(s[n], al[j], h[2 * j], h[2 * j + 1]);
-                    }
-                }
-            }
-        }
-        // what the rows do not see, and the running maximum
-        float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int2 p = *reinterpret_cast<const int2*>(kp + n * 8 + 2 * t4);
-            s[n][0] = p.x <= lim0 ? s[n][0] * sc0 : -INFINITY;
-            s[n][1] = p.y <= lim0 ? s[n][1] * sc0 : -INFINITY;
-            s[n][2] = p.x <= lim1 ? s[n][2] * sc1 : -INFINITY;
-            s[n][3] = p.y <= lim1 ? s[n][3] * sc1 : -INFINITY;
-            x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
-            x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
-        }
-#pragma unroll
-        for (int o = 1; o <= 2; o <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
-        }
-        if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-            const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-            const float c0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0);
-            const float c1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
-            m0 = n0, m1 = n1;
-            l0 *= c0, l1 *= c1;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                acc[d][0] *= c0, acc[d][1] *= c0;
-                acc[d][2] *= c1, acc[d][3] *= c1;
-            }
-        }
-        const float b0 = m0 == -INFINITY ? 0.f : m0 - P_BIAS, b1 = m1 == -INFINITY ? 0.f : m1 - P_BIAS;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            s[n][0] = ex2(s[n][0] - b0), s[n][1] = ex2(s[n][1] - b0);
-            s[n][2] = ex2(s[n][2] - b1), s[n][3] = ex2(s[n][3] - b1);
-            l0 += s[n][0] + s[n][1];
-            l1 += s[n][2] + s[n][3];
-        }
-        // p v; `careful` where some row does not see all of the tile
-        const bool careful = (kt0 + i) * KT + KT - 1 > first_lim;
-        bool odd = false;  // a V value that is not finite, among this thread's
-        if constexpr (!F32) {
-#pragma unroll
-            for (int k = 0; k < KW / 16; ++k) {
-                uint32_t ph[4], pl[4];
-                split2(s[2 * k][0], s[2 * k][1], ph[0], pl[0]);
-                split2(s[2 * k][2], s[2 * k][3], ph[1], pl[1]);
-                split2(s[2 * k + 1][0], s[2 * k + 1][1], ph[2], pl[2]);
-                split2(s[2 * k + 1][2], s[2 * k + 1][3], ph[3], pl[3]);
-#pragma unroll
-                for (int d = 0; d < DB; d += 2) {
-                    uint32_t b[4];
-                    ldsm_x4_t(vd + (uint32_t)((k * 16 + (lane & 15)) * LD + d * 16 + (lane >> 4) * 16),
-                              b[0], b[1], b[2], b[3]);
-                    if (careful) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) b[j] = finite16x2(b[j], odd);
-                    }
-                    mma16816(acc[d], ph, b[0], b[1]);
-                    mma16816(acc[d + 1], ph, b[2], b[3]);
-                    mma16816(acc[d], pl, b[0], b[1]);
-                    mma16816(acc[d + 1], pl, b[2], b[3]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < KW / 8; ++k) {
-                // the MMA's k index t holds position 2 t, t + 4 position 2 t + 1, in both operands:
-                // then the scores' accumulator is the A operand as it lies
-                uint32_t ph[4], pl[4];
-                split_tf32(s[k][0], ph[0], pl[0]);
-                split_tf32(s[k][2], ph[1], pl[1]);
-                split_tf32(s[k][1], ph[2], pl[2]);
-                split_tf32(s[k][3], ph[3], pl[3]);
-                const uint8_t* v0 = smem + (vd - kv_base) + (k * 8 + 2 * t4) * LD + g * 4;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    float y0 = *reinterpret_cast<const float*>(v0 + d * 32);
-                    float y1 = *reinterpret_cast<const float*>(v0 + LD + d * 32);
-                    if (careful) {
-                        if (!(fabsf(y0) < INFINITY)) odd = true, y0 = 0.f;
-                        if (!(fabsf(y1) < INFINITY)) odd = true, y1 = 0.f;
-                    }
-                    uint32_t h0, e0, h1, e1;
-                    split_tf32(y0, h0, e0);
-                    split_tf32(y1, h1, e1);
-                    mma1688_tf32(acc[d], ph, h0, h1);
-                    mma1688_tf32(acc[d], ph, e0, e1);
-                    mma1688_tf32(acc[d], pl, h0, h1);
-                }
-            }
-        }
-        if (__any_sync(0xffffffffu, odd)) {
-            // rows that see such a value are not finite there
-#pragma unroll 1
-            for (int j = 0; j < KW; ++j) {
-                const int pos = kp[j];
-                const uint8_t* vr = smem + (vd - kv_base) + j * LD;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int x = d * 8 + 2 * t4 + c;
-                        float y;
-                        if constexpr (F32) y = reinterpret_cast<const float*>(vr)[x];
-                        else y = __half2float(reinterpret_cast<const __half*>(vr)[x]);
-                        if (fabsf(y) < INFINITY) continue;
-                        if (pos <= lim0) acc[d][c] = NAN;
-                        if (pos <= lim1) acc[d][2 + c] = NAN;
-                    }
-            }
-        }
-    }
-
-    // ---- the item's result ----
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-    }
-    const int first_head = it.hk * G, row0 = it.tile * R;
-    const int64_t pidx = (int64_t)it.part_base + it.part;
-    auto out_row = [&](int r) {
+    for (int r = warp; r < R; r += C::WR) {
         const int gr = row0 + r, tok = gr / G;
-        return A.out + (int64_t)(it.s.q0 + tok) * A.out_stride + (int64_t)(first_head + gr - tok * G) * HD;
-    };
-    if constexpr (WR == 1) {
-        __shared__ float sh_m[C::NW][16], sh_l[C::NW][16];
-        constexpr int MLD = HDP + 4;
-        float* ma = reinterpret_cast<float*>(smem);
-        __syncthreads();  // every warp is done with the ring
+        const float* src = r < rows ? A.q + (int64_t)(it.s.q0 + tok) * A.q_stride +
+                                          (int64_t)(it.hk * G + gr - tok * G) * HD
+                                    : nullptr;
+        uint8_t* hi = smem + r * T::QLD;
+        const float f = stage_q_row<C::F32, HDP>(src, HD, hi, hi + R * T::QLD, A.scale_log2);
+        if (lane == 0) row_scale[r] = f;
+    }
+    __syncthreads();
+    T t;
+    t.start(q_base + warp * 16 * T::QLD, q_base + (R + warp * 16) * T::QLD);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            float* p = ma + (warp * 16 + g) * MLD + d * 8 + 2 * t4;
-            *reinterpret_cast<float2*>(p) = make_float2(acc[d][0], acc[d][1]);
-            *reinterpret_cast<float2*>(p + 8 * MLD) = make_float2(acc[d][2], acc[d][3]);
-        }
-        if (t4 == 0) {
-            sh_m[warp][g] = m0, sh_m[warp][g + 8] = m1;
-            sh_l[warp][g] = l0, sh_l[warp][g + 8] = l1;
-        }
+    for (int h = 0; h < 2; ++h) {
+        const int r = warp * 16 + g + 8 * h;
+        t.lim[h] = r < rows ? start + (row0 + r) / G : -1;
+        t.sc[h] = row_scale[r];
+    }
+    for (int i = 0; i < n_kt; ++i) {
+        if (i + S - 1 < n_kt) put_offsets(i + S - 1, next_page);
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
         __syncthreads();
-        const int v4 = HD / 4;
-        for (int e = tid; e < rows * v4; e += NT) {
-            const int r = e / v4, x = (e - r * v4) * 4;
-            float M = sh_m[0][r], l = 0.f;
+        issue(i + S - 1);
+        next_page = entry_of(kt0 + i + S);
+        const uint32_t kd = kv_base + (uint32_t)((i % S) * C::STAGE);
+        const int* kp = key_pos[i % C::RING];
+        t.step(kd, kd + KT * LD, smem + (kd - q_base) + KT * LD, (kt0 + i) * KT + KT - 1 > first_lim,
+               [&](int j) { return kp[j]; });
+    }
+    t.finish();
+    const int64_t pidx = (int64_t)it.part_base + it.part;
 #pragma unroll
-            for (int i = 1; i < C::NW; ++i) M = fmaxf(M, sh_m[i][r]);
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int h = 0; h < 2; ++h) {
+        const int r = warp * 16 + g + 8 * h;
+        if (r >= rows) continue;
+        const bool whole = it.n_parts == 1;
+        const float inv = !whole ? 1.f : t.l[h] == 0.f ? 0.f : 1.f / t.l[h];
+        float* p = whole ? out_row(A, it, G, row0 + r) : A.part_acc + (pidx * R + r) * HD;
 #pragma unroll
-            for (int i = 0; i < C::NW; ++i) {
-                const float c = M == -INFINITY ? 1.f : ex2(sh_m[i][r] - M);
-                const float4 y = *reinterpret_cast<const float4*>(ma + (i * 16 + r) * MLD + x);
-                l += c * sh_l[i][r];
-                o.x += c * y.x, o.y += c * y.y, o.z += c * y.z, o.w += c * y.w;
-            }
-            if (it.n_parts == 1) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                *reinterpret_cast<float4*>(out_row(r) + x) =
-                    make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-            } else {
-                *reinterpret_cast<float4*>(A.part_acc + (pidx * R + r) * HD + x) = o;
-                if (x == 0) A.part_ml[pidx * R + r] = make_float2(M, l);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = wr + g + 8 * h;
-            if (r >= rows) continue;
-            const float m = h ? m1 : m0, l = h ? l1 : l0;
-            const bool whole = it.n_parts == 1;
-            const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            float* p = whole ? out_row(r) : A.part_acc + (pidx * R + r) * HD;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-                if (d * 8 < HD)
-                    *reinterpret_cast<float2*>(p + d * 8 + 2 * t4) =
-                        make_float2(acc[d][2 * h] * inv, acc[d][2 * h + 1] * inv);
-            if (!whole && t4 == 0) A.part_ml[pidx * R + r] = make_float2(m, l);
-        }
+        for (int d = 0; d < T::DB; ++d)
+            if (d * 8 < HD)
+                *reinterpret_cast<float2*>(p + d * 8 + 2 * (lane & 3)) =
+                    make_float2(t.acc[d][2 * h] * inv, t.acc[d][2 * h + 1] * inv);
+        if (!whole && (lane & 3) == 0) A.part_ml[pidx * R + r] = make_float2(t.m[h], t.l[h]);
     }
 }
 
@@ -682,23 +852,25 @@ struct Plan {
     size_t bytes = 0;
 };
 
-template <typename KV, int HDP, int WR>
-static SplitRule rows_rule(int min_rows, int max_rows) {
-    using C = RowsCfg<KV, HDP, WR>;
-    // two CTAs per SM for the narrow kernel, one for the wide: two rounds of them, so that
-    // uneven ranges even out; at least 128 positions, below which joining costs more
-    return SplitRule{C::R, C::KT, min_rows, max_rows, kSMs * (WR == 1 ? 4 : 2),
-                     std::max(1, 128 / C::KT)};
+// Rules of the two: about two rounds of CTAs, so that uneven ranges even out, and at least 128
+// positions a range, below which joining costs more.
+template <typename KV, int HDP>
+static SplitRule narrow_rule(int min_rows, int max_rows) {
+    using C = NarrowCfg<KV, HDP>;
+    return SplitRule{16, C::KW, min_rows, max_rows, kSMs * C::CTAS * 2, 128 / C::KW};
+}
+template <typename KV, int HDP>
+static SplitRule wide_rule(int min_rows, int max_rows) {
+    using C = WideCfg<KV, HDP>;
+    return SplitRule{C::R, C::KT, min_rows, max_rows, kSMs * 2, 128 / C::KT};
 }
 
-template <typename KV, int HDP, int WR>
-static int rows_launch(const RowsArgs& a, int64_t tiles, cudaStream_t st) {
-    using C = RowsCfg<KV, HDP, WR>;
-    auto kern = attn_rows_kernel<KV, HDP, WR>;
-    IB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)C::SMEM));
+template <typename Kern>
+static int rows_launch(Kern kern, int threads, size_t smem, const RowsArgs& a, int64_t tiles,
+                       cudaStream_t st) {
+    IB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int64_t grid = tiles + a.rule.target;
-    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(C::NT), C::SMEM, st, true, a));
+    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(threads), smem, st, true, a));
     return IB_OK;
 }
 
@@ -707,8 +879,8 @@ static int rows_launch(const RowsArgs& a, int64_t tiles, cudaStream_t st) {
 // wide one out, a single kernel takes everything.
 template <typename KV, int HDP>
 static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
-    constexpr int WIDE = HDP == 256 ? 4 : 8;
     constexpr int ALL = 0x7fffffff;
+    constexpr int WIDE = WideCfg<KV, HDP>::R;
     const int64_t G = n_heads / p->n_kv_heads;
     const int64_t most_q = b->max_q > 0 ? std::min(b->max_q, b->n_tokens) : b->n_tokens;
     const int64_t seqs = std::min(b->n_seqs, b->n_tokens);
@@ -728,10 +900,10 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     };
     const int64_t rows = b->n_tokens * G;
     if (most_q * G <= 16) {
-        add(rows_rule<KV, HDP, 1>(1, ALL), seqs + rows / 16);
+        add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 16);
     } else {
-        if (b->n_seqs > 1) add(rows_rule<KV, HDP, 1>(1, 16), seqs);
-        add(rows_rule<KV, HDP, WIDE>(b->n_seqs > 1 ? 17 : 1, ALL), seqs + rows / (16 * WIDE));
+        if (b->n_seqs > 1) add(narrow_rule<KV, HDP>(1, 16), seqs);
+        add(wide_rule<KV, HDP>(b->n_seqs > 1 ? 17 : 1, ALL), seqs + rows / WIDE);
     }
     return plan;
 }
@@ -739,14 +911,17 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
 template <typename KV, int HDP>
 static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan, RowsArgs a,
                     uint8_t* ws, int64_t max_pos, cudaStream_t st) {
-    constexpr int WIDE = HDP == 256 ? 4 : 8;
+    using N = NarrowCfg<KV, HDP>;
+    using W = WideCfg<KV, HDP>;
     for (int i = 0; i < plan.n; ++i) {
         const Share& s = plan.share[i];
         a.rule = s.rule;
         a.part_acc = reinterpret_cast<float*>(ws + s.acc_off);
         a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
-        const int r = s.rule.R == 16 ? rows_launch<KV, HDP, 1>(a, s.tiles, st)
-                                     : rows_launch<KV, HDP, WIDE>(a, s.tiles, st);
+        const int r =
+            s.rule.R == 16
+                ? rows_launch(attn_narrow_kernel<KV, HDP>, N::NT, N::SMEM, a, s.tiles, st)
+                : rows_launch(attn_wide_kernel<KV, HDP>, W::NT, W::SMEM, a, s.tiles, st);
         if (r != IB_OK) return r;
         // no range is cut where the longest row of a table is no longer than the least
         if (max_pos > (int64_t)s.rule.least * s.rule.KT) {
