@@ -232,7 +232,7 @@ int ib_attention_split(const float* q, const float* kc, const float* vc, float* 
  *
  * Pool: k and v each [n_layers][n_pages][n_kv_heads][page_size][head_dim], F32 or F16
  * (values rounded to nearest when written), 16-byte aligned; head_dim a multiple of 8 up to
- * 256, any page_size up to IB_KV_MAX_PAGE_SIZE. */
+ * 256, any page_size up to IB_KV_MAX_PAGE_SIZE, n_pages * n_kv_heads * page_size < 2^31. */
 #define IB_KV_MAX_PAGES (1 << 20)
 #define IB_KV_MAX_SLOTS 16384
 #define IB_KV_MAX_PAGE_SIZE 4096
@@ -246,7 +246,7 @@ typedef struct {
  * row p % page_size.  table [n_slots][max_pages]: -1 behind the last page, and where a page
  * was given back early (its positions are then passed over).  refs [n_pages]: how many table
  * entries hold the page, 0 = free.  An empty cache is table = -1, len = 0, refs = 0; the
- * calls below keep it so.  max_pages * page_size <= 2^30. */
+ * calls below keep it so.  max_pages * page_size <= 2^28. */
 typedef struct {
     int32_t n_slots, max_pages;
     int32_t *table, *len, *refs;
@@ -257,7 +257,7 @@ typedef struct {
  * are already counted in its len.  cu_q [n_seqs + 1] and slots are device memory.  n_tokens:
  * rows of the tensors; rows from cu_q[n_seqs] on belong to nobody and are left as they were.
  * max_q: the most tokens of one sequence where the caller knows it (0: n_tokens); it chooses
- * kernels, results do not depend on it beyond rounding.  n_tokens * n_heads <= 2^26. */
+ * kernels, results do not depend on it beyond rounding.  n_tokens * n_heads <= 2^26, n_heads <= 1024. */
 typedef struct {
     int32_t n_seqs, n_tokens, max_q;
     const int32_t *cu_q, *slots;

@@ -49,12 +49,15 @@ int paged_check(const ib_kv_pages* p, const ib_kv_seqs* s, const char* who) {
         return paged_refuse(who, "head_dim must be a multiple of 8 in [8, 256]");
     if (p->page_size < 1 || p->page_size > IB_KV_MAX_PAGE_SIZE)
         return paged_refuse(who, "page_size out of range");
+    // kernels number the rows of a layer with 31 bits
+    if ((int64_t)p->n_pages * p->n_kv_heads * p->page_size >= (1ll << 31))
+        return paged_refuse(who, "n_pages x n_kv_heads x page_size must be below 2^31");
     if (((uintptr_t)p->k & 15) || ((uintptr_t)p->v & 15))
         return paged_refuse(who, "the pages must be 16-byte aligned");
     if (s->n_slots < 1 || s->n_slots > IB_KV_MAX_SLOTS || s->max_pages < 1)
         return paged_refuse(who, "n_slots or max_pages out of range");
-    if ((int64_t)s->max_pages * p->page_size > (1 << 30))
-        return paged_refuse(who, "max_pages x page_size must be at most 2^30");
+    if ((int64_t)s->max_pages * p->page_size > (1 << 28))
+        return paged_refuse(who, "max_pages x page_size must be at most 2^28");
     return IB_OK;
 }
 
@@ -67,8 +70,9 @@ int paged_check_batch(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_bat
         return paged_refuse(who, "bad batch sizes");
     if (b->n_seqs > s->n_slots) return paged_refuse(who, "more sequences than slots");
     if (layer < 0 || layer >= p->n_layers) return paged_refuse(who, "layer out of range");
-    if (n_heads <= 0 || n_heads % p->n_kv_heads || n_heads > 65536)
+    if (n_heads <= 0 || n_heads % p->n_kv_heads)
         return paged_refuse(who, "n_heads must be a multiple of n_kv_heads");
+    if (n_heads > 1024) return paged_refuse(who, "n_heads must be at most 1024");
     if ((int64_t)b->n_tokens * n_heads > (1 << 26))
         return paged_refuse(who, "n_tokens x n_heads must be at most 2^26");
     return IB_OK;

@@ -76,7 +76,7 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedView& w, int b) {
         s.row = w.table;
         return s;
     }
-    const int cap = w.max_pages * w.page_size;  // the host keeps this below 2^30
+    const int cap = w.max_pages * w.page_size;  // at most 2^28 (paged_check)
     const int L = w.len[slot];
     s.L = min(max(L, 0), cap);
     if (s.L != L) paged_fault(PAGED_BAD_LEN);

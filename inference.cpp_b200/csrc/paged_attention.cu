@@ -1,13 +1,14 @@
 // ib_attention_paged: causal GQA attention of a batch of new tokens over the paged cache.
 //
 // The query rows of a sequence that share a kv head -- (token, head of the group), token by
-// token -- are consecutive: row r is token r / G, head r % G.  A work item is a tile of such
-// rows against a range of the sequence's positions; items whose range is not the whole leave
-// a partial result (running maximum m, exponential sum l, unnormalised sum of p v), and a
-// second kernel joins them:
+// token -- are consecutive: row r is token r / G, head r % G.  A tile is R such rows against the
+// positions they see.  The tiles of a call are laid end to end and cut into as many pieces of
+// equal work as there are workers (CTAs, or single warps), so that a batch of any mix of
+// lengths keeps every SM busy to the end.  A tile that is cut leaves partial results (running maximum
+// m, exponential sum l, unnormalised sum of p v), and a second kernel joins them:
 //     out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.
-// Lengths are device data, so every CTA works the split out for itself from cu_q and len (one
-// pass over the batch; no planning launch), and grids are sized by the host's bounds.
+// Lengths are device data: every CTA works the cuts out for itself from cu_q and len (one pass
+// over the batch; no planning launch).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -24,27 +25,204 @@ namespace ib {
 
 int paged_attention_fault_take(int* code) { return paged_fault_take_here(code); }
 
-// ---- the split of a batch into items -----------------------------------------------------
-// Sequences with rows in [min_rows, max_rows] take part.  A sequence has ceil(rows / R) row
-// tiles per kv head, each over ceil(L / KT) key tiles; the ranges are as long as it takes to
-// have about `target` items, but at least `least` key tiles.
-struct SplitRule {
-    int R, KT, min_rows, max_rows, target, least;
+// ---- cutting a batch into pieces ---------------------------------------------------------
+// Sequences with rows in [min_rows, max_rows] take part, in tiles of R rows and key tiles of KT
+// positions, in n_pieces pieces of at least `least` positions of one token.
+struct CutRule {
+    int R, KT, min_rows, max_rows, n_pieces, least;
 };
 
-// Item `item` of the batch.  n_parts: ranges of its row tile; part_base: index of the first
-// of their partials (unused when n_parts == 1).
+// Work is counted in rows x positions, roughly: tile i of a sequence whose first new token is
+// at `start` counts G start + (i + 1) R, which has a closed sum over tiles.
+struct SeqWork {
+    SeqInfo s;
+    int tiles;          // row tiles per kv head, 0: the sequence does not take part
+    long long per_head, all;
+};
+
+constexpr unsigned long long kMostWork = 1ull << 62;  // sums of what device memory says saturate
+__device__ __forceinline__ long long add_work(long long a, long long b) {
+    return (long long)min((unsigned long long)a + (unsigned long long)b, kMostWork);
+}
+
+__device__ __forceinline__ long long tiles_work(long long t, long long start_g, int R) {
+    return t * start_g + (long long)R * (t * (t + 1) / 2);
+}
+
+__device__ __forceinline__ SeqWork seq_work(const PagedView& w, const CutRule& rule, int b) {
+    SeqWork x;
+    x.s = seq_info(w, b);
+    const int G = w.H / w.Hkv, rows = x.s.n * G;
+    const bool in = rows >= rule.min_rows && rows <= rule.max_rows;
+    x.tiles = in ? (rows + rule.R - 1) / rule.R : 0;
+    x.per_head = tiles_work(x.tiles, (long long)G * max(x.s.L - x.s.n, 0), rule.R);
+    // at most 2^23 tiles of at most 2^38 each (paged_check_batch)
+    x.all = x.per_head * w.Hkv;
+    return x;
+}
+
+// One tile, or a part of one, in a worker's piece.
+struct Segment {
+    SeqInfo s;
+    int hk, tile, rows;
+    int start;      // position of the sequence's first new token
+    int kt0, kt1;   // key tiles
+    int part;       // where its partial result goes, -1: it is the whole tile
+    int row0;       // first row
+};
+
+struct Piece {
+    long long at, end, len;  // work left to do: [at, end); of a piece
+    long long base;          // where sequence b begins
+    int b, no;
+    SeqWork x;
+};
+
+// The NP pieces from number `first` on: out[i] (shared memory) is piece first + i, found[i]
+// whether there is one.  BY_TILE: `first` counts tiles over all heads instead, and tile_no is
+// the tile's number in its sequence.  Every thread of the CTA (NT of them) calls it.
+template <int NT, int NP, bool BY_TILE>
+__device__ __forceinline__ void find_pieces(const PagedView& w, const CutRule& rule, long long first,
+                                            Piece* out, int* found, long long* tile_no) {
+    __shared__ long long sh_sum[NT / 32][2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    SeqWork x0{};
+    long long work = 0, tokens = 0;
+    for (int b = tid; b < w.n_seqs; b += NT) {
+        const SeqWork x = seq_work(w, rule, b);
+        work = add_work(work, x.all);
+        tokens += x.s.n;
+        if (b == tid) x0 = x;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        work = add_work(work, __shfl_xor_sync(0xffffffffu, work, o));
+        tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+    }
+    if (lane == 0) sh_sum[warp][0] = work, sh_sum[warp][1] = tokens;
+    if (tid < NP) found[tid] = 0;
+    __syncthreads();
+    work = tokens = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+        work = add_work(work, sh_sum[i][0]);
+        tokens += sh_sum[i][1];
+    }
+    if (tokens > w.n_tokens) {  // a cu_q that is not in order names rows twice: no work
+        if (tid == 0) paged_fault(PAGED_BAD_LEN);
+        return;
+    }
+    const long long len = max((work + rule.n_pieces - 1) / rule.n_pieces,
+                              (long long)rule.least * (w.H / w.Hkv));
+    __syncthreads();
+    if (!BY_TILE && first * len >= work) return;
+    long long work_before = 0, tiles_before = 0;
+    for (int b0 = 0; b0 < w.n_seqs; b0 += NT) {
+        const int b = b0 + tid;
+        SeqWork x = x0;
+        if (b0 > 0 && b < w.n_seqs) x = seq_work(w, rule, b);
+        if (b >= w.n_seqs) x.tiles = 0, x.all = 0;
+        const long long n_tiles = (long long)x.tiles * w.Hkv;
+        long long a = x.all, t = n_tiles;  // inclusive sums
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long ya = __shfl_up_sync(0xffffffffu, a, o);
+            const long long yt = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) a = add_work(a, ya), t += yt;
+        }
+        if (lane == 31) sh_sum[warp][0] = a, sh_sum[warp][1] = t;
+        __syncthreads();
+        long long sa = 0, st = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 32; ++i) {
+            if (i == warp) a = add_work(a, sa), t += st;
+            sa = add_work(sa, sh_sum[i][0]), st += sh_sum[i][1];
+        }
+        const long long a0 = add_work(work_before, a - x.all);
+        const long long t0 = tiles_before + (t - n_tiles);
+        bool last = false;  // the last piece of these, or of all, begins in what was seen
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const long long want = BY_TILE ? first : (first + i) * len;
+            if (BY_TILE ? want >= t0 && want < t0 + n_tiles
+                        : want < work && want >= a0 && want < a0 + x.all) {
+                out[i] = Piece{want, min(work, want + len), len, a0, b, (int)first + i, x};
+                if (BY_TILE) *tile_no = want - t0;
+                found[i] = 1;
+            }
+            last = BY_TILE ? want < tiles_before + st : min(want, work - 1) < work_before + sa;
+        }
+        work_before = add_work(work_before, sa);
+        tiles_before += st;
+        __syncthreads();
+        if (last) break;  // the same for every thread
+    }
+}
+
+// The next segment of a piece; false at its end.  Called by whole warps, each for itself.
+// A call, not inlined: it runs once a segment and would crowd the loops' instruction cache.
+__device__ __noinline__ bool next_segment(const PagedView& w, const CutRule& rule, Piece& p,
+                                          Segment& g) {
+    if (p.at >= p.end) return false;
+    if (p.at >= p.base + p.x.all) {  // on to the next sequence that takes part
+        p.base += p.x.all;
+        for (int b0 = p.b + 1;; b0 += 32) {
+            if (b0 >= w.n_seqs) return false;
+            const int b = b0 + (int)(threadIdx.x & 31);
+            SeqWork x{};
+            if (b < w.n_seqs) x = seq_work(w, rule, b);
+            const unsigned has = __ballot_sync(0xffffffffu, x.all > 0);
+            if (has) {
+                p.b = b0 + __ffs(has) - 1;
+                p.x = seq_work(w, rule, p.b);
+                break;
+            }
+        }
+    }
+    const int G = w.H / w.Hkv;
+    const SeqInfo& s = p.x.s;
+    const long long start_g = (long long)G * max(s.L - s.n, 0);
+    long long u = p.at - p.base;
+    g.s = s;
+    g.start = s.L - s.n;
+    g.hk = (int)(u / p.x.per_head);
+    u -= g.hk * p.x.per_head;
+    int lo = 0, hi = p.x.tiles;  // the tile: the last whose work begins at or before u
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tiles_work(mid, start_g, rule.R) <= u) lo = mid;
+        else hi = mid;
+    }
+    g.tile = lo;
+    g.row0 = lo * rule.R;
+    g.rows = min(rule.R, s.n * G - g.row0);
+    const long long all = start_g + (long long)(lo + 1) * rule.R;
+    const long long x0 = u - tiles_work(lo, start_g, rule.R);
+    const long long x1 = min(all, x0 + (p.end - p.at));
+    const int seen = max(0, g.start + (g.row0 + g.rows - 1) / G + 1);
+    const int nkt = (seen + rule.KT - 1) / rule.KT;
+    // the same value for a piece's end and the next one's beginning
+    g.kt0 = x0 == 0 ? 0 : (int)((double)nkt * (double)x0 / (double)all);
+    g.kt1 = x1 == all ? nkt : (int)((double)nkt * (double)x1 / (double)all);
+    const bool whole = x0 == 0 && x1 == all;
+    g.part = whole ? -1 : 2 * p.no + (p.at == p.no * p.len ? 0 : 1);
+    p.at += x1 - x0;
+    return true;
+}
+
+// ---- or into parts of tiles ----------------------------------------------------------------
+// The other way to cut, for tiles of few rows: every tile by itself into parts of equal length,
+// about n_pieces parts in all, each a CTA's only work.  Where several CTAs share an SM the
+// scheduler evens them out, and no CTA has to refill its pipeline on the way: 64 single tokens
+// over 200..4096 positions (32 heads on 8) take 119 us this way, 141 us in equal pieces that
+// run on from tile to tile.
 struct Item {
     int b, hk, tile, part, n_parts, part_base;
-    int kt0, kt1;  // key tiles of the range
+    int kt0, kt1;  // key tiles of the part
     SeqInfo s;
 };
 
-struct SeqSplit {
-    int tiles, nkt, parts;  // row tiles per kv head, key tiles, ranges
-};
-
-__device__ __forceinline__ void seq_shape(const PagedView& w, const SplitRule& rule,
+__device__ __forceinline__ void seq_shape(const PagedView& w, const CutRule& rule,
                                           const SeqInfo& s, int& tiles, int& nkt) {
     const int rows = s.n * (w.H / w.Hkv);
     const bool in = rows >= rule.min_rows && rows <= rule.max_rows;
@@ -55,7 +233,7 @@ __device__ __forceinline__ void seq_shape(const PagedView& w, const SplitRule& r
 // Every thread of the CTA (NT threads) calls it; false when there are fewer items.  BY_TILE
 // counts row tiles instead of items (the joining kernel).
 template <int NT, bool BY_TILE>
-__device__ __forceinline__ bool find_item(const PagedView& w, const SplitRule& rule, int item,
+__device__ __forceinline__ bool find_item(const PagedView& w, const CutRule& rule, int item,
                                           Item& out) {
     __shared__ long long sh_units[NT / 32];
     __shared__ int sh_scan[NT / 32][2];
@@ -81,12 +259,12 @@ __device__ __forceinline__ bool find_item(const PagedView& w, const SplitRule& r
 #pragma unroll
     for (int i = 0; i < NT / 32; ++i) units += sh_units[i];
     units = min(units, 1ll << 45) * w.Hkv;
-    const int len = (int)min(max((long long)rule.least, (units + rule.target - 1) / rule.target),
+    const int len = (int)min(max((long long)(rule.least / rule.KT), (units + rule.n_pieces - 1) / rule.n_pieces),
                              0x3fffffffll);
     // cu_q can hold anything: counts are clamped to what cannot be, so that sums stay in range
     // (valid batches have at most 2^22 + n_seqs row tiles, see paged_check_batch)
     constexpr long long MOST = 1 << 23;
-    const int room = 2 * rule.target;  // partials in the workspace
+    const int room = 2 * rule.n_pieces;  // partials in the workspace
     long long items_before = 0;
     int parts_before = 0;
     for (int b0 = 0; b0 < w.n_seqs; b0 += NT) {
@@ -165,7 +343,7 @@ __device__ __forceinline__ bool find_item(const PagedView& w, const SplitRule& r
 // V is checked for values that are not finite (0 x inf).
 struct RowsArgs {
     PagedView w;
-    SplitRule rule;
+    CutRule rule;
     const float* q;
     float* out;
     int64_t q_stride, out_stride;
@@ -194,6 +372,15 @@ __device__ __forceinline__ uint32_t finite16x2(uint32_t x, bool& odd) {
     return x;
 }
 
+// 2^(8 - e) for a largest element of exponent e, and its inverse (1 and 1 for zero, infinity
+// and NaN).
+__device__ __forceinline__ float pow2_scale(float top, float& inverse) {
+    const int e = max(-100, (int)((__float_as_uint(top) >> 23) & 255u) - 127);
+    const bool plain = top == 0.f || e > 127;
+    inverse = plain ? 1.f : __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+    return plain ? 1.f : __uint_as_float((uint32_t)(8 - e + 127) << 23);
+}
+
 // One query row into shared memory as hi and lo parts, by one warp.  Returns the factor that
 // turns its scores into base-2 exponents.
 template <bool F32, int HDP>
@@ -216,11 +403,8 @@ __device__ __forceinline__ float stage_q_row(const float* row, int HD, uint8_t* 
     } else {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // 2^(8 - e) with e the exponent of the largest element, and its inverse
-        const int e = max(-100, (int)((__float_as_uint(top) >> 23) & 255u) - 127);
-        const bool plain = top == 0.f || e > 127;
-        const float up = plain ? 1.f : __uint_as_float((uint32_t)(8 - e + 127) << 23);
-        const float down = plain ? 1.f : __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+        float down;
+        const float up = pow2_scale(top, down);
 #pragma unroll
         for (int i = 0; i < HDP / 32; ++i) {
             const float y = x[i] * up;
@@ -300,9 +484,9 @@ struct WarpRows {
                             b[0], b[1], b[2], b[3]);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        if constexpr (NB <= 2) mma16816(k < KS / 2 ? s[n + j] : s2[n + j], ah, b[2 * j], b[2 * j + 1]);
-                        else mma16816(s[n + j], ah, b[2 * j], b[2 * j + 1]);
-                        mma16816(e[n + j], al, b[2 * j], b[2 * j + 1]);
+                        float(&x)[4] = NB <= 2 && k >= KS / 2 ? s2[NB <= 2 ? n + j : 0] : s[n + j];
+                        mma_f16(x, ah, b[2 * j], b[2 * j + 1], x);
+                        mma_f16(e[n + j], al, b[2 * j], b[2 * j + 1], e[n + j]);
                     }
                 }
             }
@@ -329,9 +513,9 @@ struct WarpRows {
                     for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(b[j]), h[j], r[j]);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        mma1688_tf32(t[n], ah[j], h[2 * j], h[2 * j + 1]);
-                        mma1688_tf32(e[n], ah[j], r[2 * j], r[2 * j + 1]);
-                        mma1688_tf32(e[n], al[j], h[2 * j], h[2 * j + 1]);
+                        mma_tf32(t[n], ah[j], h[2 * j], h[2 * j + 1], t[n]);
+                        mma_tf32(e[n], ah[j], r[2 * j], r[2 * j + 1], e[n]);
+                        mma_tf32(e[n], al[j], h[2 * j], h[2 * j + 1], e[n]);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s[n][j] += t[n][j];
@@ -393,8 +577,8 @@ struct WarpRows {
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        mma16816(t[j], pl[k], b[2 * j], b[2 * j + 1]);
-                        mma16816(t[j], ph[k], b[2 * j], b[2 * j + 1]);
+                        mma_f16(t[j], pl[k], b[2 * j], b[2 * j + 1], t[j]);
+                        mma_f16(t[j], ph[k], b[2 * j], b[2 * j + 1], t[j]);
                     }
                 }
                 add(d, t[0], c), add(d + 1, t[1], c);
@@ -426,9 +610,9 @@ struct WarpRows {
                     uint32_t h0, r0, h1, r1;
                     split_tf32(y0, h0, r0);
                     split_tf32(y1, h1, r1);
-                    mma1688_tf32(t[0], ph[k], h0, h1);
-                    mma1688_tf32(r[0], ph[k], r0, r1);
-                    mma1688_tf32(r[0], pl[k], h0, h1);
+                    mma_tf32(t[0], ph[k], h0, h1, t[0]);
+                    mma_tf32(r[0], ph[k], r0, r1, r[0]);
+                    mma_tf32(r[0], pl[k], h0, h1, r[0]);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) t[0][j] += r[0][j];
@@ -478,169 +662,426 @@ struct WarpRows {
     }
 };
 
-__device__ __forceinline__ float* out_row(const RowsArgs& A, const Item& it, int G, int gr) {
+// Row `gr` of the segment's sequence and kv head.
+__device__ __forceinline__ float* out_row(const RowsArgs& A, const Segment& it, int G, int gr) {
     const int tok = gr / G;
     return A.out + (int64_t)(it.s.q0 + tok) * A.out_stride +
            (int64_t)(it.hk * G + gr - tok * G) * A.w.HD;
 }
+__device__ __forceinline__ const float* q_row(const RowsArgs& A, const Segment& it, int G, int gr) {
+    const int tok = gr / G;
+    return A.q + (int64_t)(it.s.q0 + tok) * A.q_stride + (int64_t)(it.hk * G + gr - tok * G) * A.w.HD;
+}
 
 // ---- up to 16 rows: single tokens and short drafts ---------------------------------------
-// The bound is reading K and V once.  A CTA holds the 16 rows; each of its warps runs through
-// every NW-th group of KW positions by itself -- its own ring in shared memory, filled by its
-// own cp.async, no barrier in the loop -- so that one warp's chain of loads, scores, maximum and
-// products hides behind the others'; they join at the end.
-template <typename KV, int HDP>
+// The bound is reading K and V once, and next to it a warp's own chain of loads, scores, maximum
+// and products.  So the products are turned round -- 16 positions are the MMA's M, eight query
+// rows its N: scores K q', outputs V' p -- which halves the instructions and registers of eight
+// rows against 16-row tiles (four query heads on a kv head fill half of N, not a quarter of M);
+// and each of a CTA's warps runs through every NW-th tile of 16 positions by itself, with its
+// own ring in shared memory filled by its own cp.async and no barrier in the loop; they join at
+// the end.  A ring slot is one half of a tile, K or V.  (Warps with pieces of their own, their
+// copies running on from tile to tile, took 135 us against 119 us for 64 single tokens over
+// 200..4096 positions: warps far apart in the code miss the instruction cache.)
+// RB: blocks of eight rows.
+template <typename KV, int HDP, int RB>
 struct NarrowCfg {
     static constexpr bool F32 = sizeof(KV) == 4;
-    static constexpr int KW = F32 ? 8 : 16;
-    static constexpr bool QREG = !F32 && HDP <= 128;
-    using Tile = WarpRows<KV, HDP, KW, QREG>;
-    static constexpr int NW = HDP == 256 ? 4 : 8, NT = NW * 32;
-    static constexpr int STAGES = F32 && HDP == 256 ? 2 : 3;
-    static constexpr int STAGE = 2 * KW * Tile::LD;
-    static constexpr int Q_BYTES = 2 * 16 * Tile::QLD;
-    static constexpr int RING = NW * STAGES * STAGE;
-    static constexpr int MERGE = NW * 16 * (HDP + 4) * 4;  // of the warps' results, in the ring
-    static constexpr size_t SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
-    // CTAs that an SM holds
-    static constexpr int CTAS = HDP == 64 ? 2 : 1;
+    static constexpr int R = 8 * RB, KW = 16;
+    static constexpr int LD = HDP * (int)sizeof(KV) + 16, QLD = HDP * 4 + 16;
+    static constexpr int HALF = KW * LD;
+    // 64 single tokens at head_dim 128 in FP16: 117 us with three CTAs of four warps to an SM,
+    // 126 us with two, 130 us with four of three half tiles a warp
+    static constexpr int ROWB = HDP * (int)sizeof(KV);
+    static constexpr int D = ROWB <= 256 ? 4 : ROWB <= 512 ? 3 : 2;  // ring slots of a warp
+    static constexpr int CTAS = ROWB <= 256 && RB == 1 ? 3 : ROWB <= 512 ? 2 : 1;  // to an SM
+    static constexpr int NW = 4, NT = NW * 32;
+    static constexpr bool QREG = HDP * (F32 ? 2 : 1) <= 256;  // q fragments stay in registers
+    static constexpr int Q_BYTES = QREG ? 0 : 2 * R * QLD;  // or lie in shared memory (FP32)
+    static constexpr size_t RING = (size_t)NW * (Q_BYTES + D * HALF);
+    static constexpr size_t MERGE = (size_t)NW * R * (HDP + 4) * 4;  // of the warps' results
+    static constexpr size_t SMEM = RING > MERGE ? RING : MERGE;
+    static_assert(QREG || F32, "");
 };
 
-template <typename KV, int HDP>
-__global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CTAS)
+template <typename KV, int HDP, int RB>
+__global__ void __launch_bounds__(NarrowCfg<KV, HDP, RB>::NT, NarrowCfg<KV, HDP, RB>::CTAS)
     attn_narrow_kernel(const __grid_constant__ RowsArgs A) {
-    using C = NarrowCfg<KV, HDP>;
-    using T = typename C::Tile;
-    constexpr int KW = C::KW, LD = T::LD, S = C::STAGES, NW = C::NW;
+    using C = NarrowCfg<KV, HDP, RB>;
+    constexpr bool F32 = C::F32;
+    constexpr int R = C::R, KW = C::KW, LD = C::LD, QLD = C::QLD, D = C::D, NW = C::NW;
+    constexpr int KS = F32 ? HDP / 8 : HDP / 16, DB = HDP / 16;
+    constexpr float P_BIAS = F32 ? 0.f : 10.f;  // p is carried times 2^10 (FP16 pages)
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float row_scale[16], sh_m[NW][16], sh_l[NW][16];
+    __shared__ float sh_m[NW][R], sh_l[NW][R];
     const PagedView& w = A.w;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     pdl_wait();
     pdl_launch_dependents();
-    Item it;
-    if (!find_item<C::NT, false>(w, A.rule, blockIdx.x, it)) return;
-    const int G = w.H / w.Hkv, HD = w.HD, row0 = it.tile * 16;
-    const int rows = min(16, it.s.n * G - row0);
-    const int start = it.s.L - it.s.n;  // position of the first new token
-    const int first_lim = start + row0 / G, last_lim = start + (row0 + rows - 1) / G;
-    const int kt0 = it.kt0 + warp, kt1 = min(it.kt1, last_lim < 0 ? 0 : last_lim / KW + 1);
-    uint8_t* ring = smem + C::Q_BYTES + warp * S * C::STAGE;
+    Item item;
+    if (!find_item<C::NT, false>(w, A.rule, blockIdx.x, item)) return;
+    const int G = w.H / w.Hkv, HD = w.HD;
+    Segment it;
+    it.s = item.s;
+    it.hk = item.hk;
+    it.row0 = item.tile * R;
+    it.rows = min(R, it.s.n * G - it.row0);
+    it.start = it.s.L - it.s.n;
+    it.part = item.n_parts == 1 ? -1 : item.part_base + item.part;
+    const int first_lim = it.start + it.row0 / G, last_lim = it.start + (it.row0 + it.rows - 1) / G;
+    // this warp's tiles: kt0, kt0 + NW ..
+    const int kt0 = item.kt0 + warp, kt1 = min(item.kt1, last_lim < 0 ? 0 : last_lim / KW + 1);
+    uint8_t* ring = smem + warp * (C::Q_BYTES + D * C::HALF);
     const uint32_t ring_a = smem_u32(ring);
+    uint8_t* q_smem = ring + D * C::HALF;
 
-    // Lane j holds position j of a tile (j < KW, twice or four times over): where its row starts
-    // in the layer (-1: nowhere) and the position itself (INT_MAX: none).
-    auto entry_of = [&](int kt) -> int {  // read a tile ahead of the copies that need it
+    // ---- copies ----
+    // Lane j (and j + 16) sees to position j of a tile: its table entry is read a tile ahead of
+    // the copies, its row number in the layer is shuffled to the lanes that copy the row.
+    auto entry_of = [&](int kt) -> int {
         const int pos = kt * KW + (lane & (KW - 1));
         if (kt >= kt1 || pos > last_lim) return -1;
         return page_at(w, it.s.row[w.ps.div((uint32_t)pos)]);
     };
-    const int cpr = HD * (int)sizeof(KV) / 16;  // 16-byte chunks of a row that exist
-    constexpr int CH = HDP * (int)sizeof(KV) / 16;  // and with padding
-    auto issue = [&](int kt, int slot, int page) -> int {
-        const int pos = kt * KW + (lane & (KW - 1));
-        if (kt < kt1) {
-            const int in_page = pos - (int)w.ps.div((uint32_t)pos) * w.page_size;
-            const long long off =
-                page < 0 ? -1 : (((long long)page * w.Hkv + it.hk) * w.page_size + in_page) * HD;
-            const uint32_t d0 = ring_a + (uint32_t)(slot * C::STAGE);
+    const int row_bytes = HD * (int)sizeof(KV);
+    constexpr int CH = HDP * (int)sizeof(KV) / 16, CHL = CH < 32 ? CH : 32, RL = 32 / CHL;
+    const int x0 = (lane % CHL) * 16, r0 = lane / CHL;
+    const uint8_t* k_src = (const uint8_t*)A.k + x0;
+    const uint8_t* v_src = (const uint8_t*)A.v + x0;
+    const uint32_t dst0 = ring_a + (uint32_t)(r0 * LD + x0);
+    int in_kt = kt0, page = entry_of(kt0), row = -1, slot_in = 0;
+    uint32_t gone[3] = {0, 0, 0};  // positions without a page: of the tile at work and those after
+    auto copy_half = [&](const uint8_t* src) {
+        if (in_kt < kt1) {
+            const uint32_t d0 = dst0 + (uint32_t)(slot_in * C::HALF);
 #pragma unroll
-            for (int c = lane; c < KW * CH; c += 32) {
-                const int r = c / CH, x = c % CH;  // CH: 8 or more, so r is within the lanes
-                const long long o = __shfl_sync(0xffffffffu, off, r);
-                const bool ok = o >= 0 && x < cpr;
-                const size_t byte = ok ? (size_t)o * sizeof(KV) + (size_t)x * 16 : 0;
-                const uint32_t d = d0 + (uint32_t)(r * LD + x * 16);
-                cp16(d, (const uint8_t*)A.k + byte, ok);
-                cp16(d + KW * LD, (const uint8_t*)A.v + byte, ok);
+            for (int i = 0; i < KW / RL; ++i) {
+                const int r = __shfl_sync(0xffffffffu, row, i * RL + r0);
+                const int64_t at = (int64_t)max(r, 0) * row_bytes;
+#pragma unroll
+                for (int x = 0; x < CH / CHL; ++x) {
+                    const bool ok = r >= 0 && x0 + x * 512 < row_bytes;
+                    // nothing is read through the address of a chunk that is not there
+                    cp16(d0 + (uint32_t)(i * RL * LD + x * 512), src + (ok ? at + x * 512 : 0), ok);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        return page < 0 ? 0x7fffffff : pos;
+        slot_in = slot_in == D - 1 ? 0 : slot_in + 1;
     };
-    int pos[S];  // of the tiles in flight, the oldest first
-    {
-        int page[S - 1];
+    auto copy_k = [&](int place) {  // place: of this tile in gone[]
+        const int pos = in_kt * KW + (lane & (KW - 1));
+        const int in_page = pos - (int)w.ps.div((uint32_t)pos) * w.page_size;
+        row = page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + in_page;
+        gone[place] = __ballot_sync(0xffffffffu, page < 0);
+        page = entry_of(in_kt + NW);
+        copy_half(k_src);
+    };
+    auto copy_v = [&]() {
+        copy_half(v_src);
+        in_kt += NW;
+    };
 #pragma unroll
-        for (int i = 0; i < S - 1; ++i) page[i] = entry_of(kt0 + i * NW);
-#pragma unroll
-        for (int i = 0; i < S - 1; ++i) pos[i] = issue(kt0 + i * NW, i, page[i]);
+    for (int h = 0; h < D - 1; ++h) {
+        if (h & 1) copy_v();
+        else copy_k(h / 2);
     }
-    int next_page = entry_of(kt0 + (S - 1) * NW);
 
-    for (int r = warp; r < 16; r += NW) {
-        const int gr = row0 + r, tok = gr / G;
-        const float* src = r < rows ? A.q + (int64_t)(it.s.q0 + tok) * A.q_stride +
-                                          (int64_t)(it.hk * G + gr - tok * G) * HD
-                                    : nullptr;
-        uint8_t* hi = smem + r * T::QLD;
-        const float f = stage_q_row<C::F32, HDP>(src, HD, hi, hi + 16 * T::QLD, A.scale_log2);
-        if (lane == 0) row_scale[r] = f;
-    }
-    __syncthreads();
-    T t;
-    t.start(smem_u32(smem), smem_u32(smem) + 16 * T::QLD);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = g + 8 * h;
-        t.lim[h] = r < rows ? start + (row0 + r) / G : -1;
-        t.sc[h] = row_scale[r];
-    }
     int slot = 0;
-    for (int kt = kt0; kt < kt1; kt += NW) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-        __syncwarp();  // every lane's copies of this tile, and its reads of the one before
-        const int fill = slot == 0 ? S - 1 : slot - 1;  // the slot before: the tile of last time
-        pos[S - 1] = issue(kt + (S - 1) * NW, fill, next_page);
-        next_page = entry_of(kt + S * NW);
-        const uint32_t kd = ring_a + (uint32_t)(slot * C::STAGE);
-        const int mine = pos[0];
-        t.step(kd, kd + KW * LD, ring + slot * C::STAGE + KW * LD, kt * KW + KW - 1 > first_lim,
-               [&](int j) { return __shfl_sync(0xffffffffu, mine, j); });
+    const uint32_t k_frag = (uint32_t)((lane & 15) * LD + (lane >> 4) * 16);
+    const uint32_t v_frag = (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * LD + ((lane >> 3) & 1) * 16);
+        // this lane's rows are 2 t4 and 2 t4 + 1 of each block
+        int lim[RB][2];
+        float sc[RB][2], m[RB][2], l[RB][2], acc[DB][RB][4];
+        uint32_t qh[C::QREG ? KS : 1][RB][2], ql[C::QREG ? KS : 1][RB][2];
+        // q as B: row g of a block; FP16 k-steps of dimensions 2 t4, + 1, + 8, + 9, TF32 t4, + 4
 #pragma unroll
-        for (int i = 0; i < S - 1; ++i) pos[i] = pos[i + 1];
-        slot = slot == S - 1 ? 0 : slot + 1;
-    }
-    t.finish();
+        for (int b = 0; b < RB; ++b) {
+            const int r = 8 * b + g;
+            const float* src = r < it.rows ? q_row(A, it, G, it.row0 + r) : nullptr;
+            float f = A.scale_log2;
+            if constexpr (F32) {
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int d = k * 8 + t4 + 4 * j;
+                        const float x = src && d < HD ? __ldg(src + d) : 0.f;
+                        uint32_t hi, lo;
+                        split_tf32(x, hi, lo);
+                        if constexpr (C::QREG) {
+                            qh[k][b][j] = hi, ql[k][b][j] = lo;
+                        } else {
+                            *reinterpret_cast<uint32_t*>(q_smem + r * QLD + d * 4) = hi;
+                            *reinterpret_cast<uint32_t*>(q_smem + (R + r) * QLD + d * 4) = lo;
+                        }
+                    }
+                if constexpr (!C::QREG) __syncwarp();
+            } else {
+                float2 x[KS][2];
+                float top = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int d = k * 16 + 2 * t4 + 8 * j;
+                        x[k][j] = src && d < HD ? __ldg(reinterpret_cast<const float2*>(src + d))
+                                                : make_float2(0.f, 0.f);
+                        top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                float down;
+                const float up = pow2_scale(top, down);
+                f *= down;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        split2(x[k][j].x * up, x[k][j].y * up, qh[k][b][j], ql[k][b][j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int mine = 8 * b + 2 * t4 + j;
+                lim[b][j] = mine < it.rows ? it.start + (it.row0 + mine) / G : -1;
+                sc[b][j] = __shfl_sync(0xffffffffu, f, (2 * t4 + j) * 4);
+                m[b][j] = -INFINITY;
+                l[b][j] = 0.f;
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[d][b][j] = 0.f;
+        }
+        for (int kt = kt0; kt < kt1; kt += NW) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+            __syncwarp();  // every lane's copies of K, and its reads of the half before
+            if constexpr (D & 1) copy_k((D - 1) / 2);
+            else copy_v();
+            const uint32_t kd = ring_a + (uint32_t)(slot * C::HALF) + k_frag;
+            slot = slot == D - 1 ? 0 : slot + 1;
+            // scores: rows of a fragment are positions g and g + 8, columns the lane's two rows.
+            // sa, sb: two chains; e: the lo parts.
+            float s[RB][4];
+            {
+                float sa[RB][4], sb[RB][4], e[RB][4];
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sa[b][j] = sb[b][j] = e[b][j] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t a[4];
+                    ldsm_x4(kd + k * 32, a[0], a[1], a[2], a[3]);
+                    uint32_t ah[4], al[4];
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
+                    }
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        uint32_t q0, q1, r0, r1;
+                        if constexpr (C::QREG) {
+                            q0 = qh[k][b][0], q1 = qh[k][b][1], r0 = ql[k][b][0], r1 = ql[k][b][1];
+                        } else {
+                            const uint8_t* p = q_smem + (8 * b + g) * QLD + (k * 8 + t4) * 4;
+                            q0 = *reinterpret_cast<const uint32_t*>(p);
+                            q1 = *reinterpret_cast<const uint32_t*>(p + 16);
+                            r0 = *reinterpret_cast<const uint32_t*>(p + R * QLD);
+                            r1 = *reinterpret_cast<const uint32_t*>(p + R * QLD + 16);
+                        }
+                        float(&x)[4] = k & 1 ? sb[b] : sa[b];
+                        if constexpr (F32) {
+                            mma_tf32(x, ah, q0, q1, x);
+                            mma_tf32(e[b], ah, r0, r1, e[b]);
+                            mma_tf32(e[b], al, q0, q1, e[b]);
+                        } else {
+                            mma_f16(x, a, q0, q1, x);
+                            mma_f16(e[b], a, r0, r1, e[b]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[b][j] = (sa[b][j] + sb[b][j]) + e[b][j];
+            }
+            // what the rows do not see, the running maximum, p
+            const uint32_t missing = gone[0];
+            const int p0 = (missing >> g) & 1 ? 0x7fffffff : kt * KW + g;
+            const int p1 = (missing >> (g + 8)) & 1 ? 0x7fffffff : kt * KW + g + 8;
+            float c[RB][2];
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float &x = s[b][j], &y = s[b][2 + j];
+                    x = p0 <= lim[b][j] ? x * sc[b][j] : -INFINITY;
+                    y = p1 <= lim[b][j] ? y * sc[b][j] : -INFINITY;
+                    float top = fmaxf(x, y);
+#pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    top = fmaxf(top, m[b][j]);
+                    c[b][j] = top == -INFINITY ? 1.f : ex2(m[b][j] - top);
+                    m[b][j] = top;
+                    const float base = top == -INFINITY ? 0.f : top - P_BIAS;
+                    x = ex2(x - base), y = ex2(y - base);
+                    l[b][j] = fmaf(l[b][j], c[b][j], x + y);
+                }
+            // p as B: positions along k, the row along n
+            uint32_t ph[RB][F32 ? 4 : 2], pl[RB][F32 ? 4 : 2];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                if constexpr (F32) {
+                    // the MMA's k index t holds position 2 t, t + 4 position 2 t + 1, as V below
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int from = 8 * t4 + 4 * j + (g >> 1);
+                            const float x = __shfl_sync(0xffffffffu, s[b][2 * i], from);
+                            const float y = __shfl_sync(0xffffffffu, s[b][2 * i + 1], from);
+                            split_tf32(g & 1 ? y : x, ph[b][2 * i + j], pl[b][2 * i + j]);
+                        }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        split2(s[b][2 * i], s[b][2 * i + 1], ph[b][i], pl[b][i]);
+                        ph[b][i] = movm(ph[b][i]), pl[b][i] = movm(pl[b][i]);
+                    }
+                }
+            }
+            asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+            __syncwarp();
+            gone[0] = gone[1], gone[1] = gone[2];
+            if constexpr (D & 1) copy_v();
+            else copy_k((D - 1) / 2);
+            const uint32_t vd = ring_a + (uint32_t)(slot * C::HALF);
+            const uint8_t* v_ptr = ring + slot * C::HALF;
+            slot = slot == D - 1 ? 0 : slot + 1;
+            const bool careful = kt * KW + KW - 1 > first_lim;
+            bool odd = false;  // a V value that is not finite, among this lane's
+            // outputs: rows of a fragment are dimensions g and g + 8 of a block of 16
+            auto products = [&](auto check) {
+                constexpr bool CHECK = decltype(check)::value;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    uint32_t a[F32 ? 2 : 1][4];
+                    [[maybe_unused]] uint32_t al[2][4];
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {  // position 2 t4 + (j >> 1), dimension g + 8 (j & 1)
+                                float y = *reinterpret_cast<const float*>(
+                                    v_ptr + (i * 8 + 2 * t4 + (j >> 1)) * LD +
+                                    (d * 16 + g + 8 * (j & 1)) * 4);
+                                if (CHECK && !(fabsf(y) < INFINITY)) odd = true, y = 0.f;
+                                split_tf32(y, a[i][j], al[i][j]);
+                            }
+                    } else {
+                        ldsm_x4_t(vd + v_frag + d * 32, a[0][0], a[0][1], a[0][2], a[0][3]);
+                        if (CHECK) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) a[0][j] = finite16x2(a[0][j], odd);
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        const float none[4] = {0.f, 0.f, 0.f, 0.f};
+                        float t[4];
+                        if constexpr (F32) {
+                            float r[4];
+                            mma_tf32(t, a[0], ph[b][0], ph[b][1], none);
+                            mma_tf32(t, a[1], ph[b][2], ph[b][3], t);
+                            mma_tf32(r, a[0], pl[b][0], pl[b][1], none);
+                            mma_tf32(r, al[0], ph[b][0], ph[b][1], r);
+                            mma_tf32(r, a[1], pl[b][2], pl[b][3], r);
+                            mma_tf32(r, al[1], ph[b][2], ph[b][3], r);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) t[j] += r[j];
+                        } else {
+                            mma_f16(t, a[0], pl[b][0], pl[b][1], none);
+                            mma_f16(t, a[0], ph[b][0], ph[b][1], t);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[d][b][j] = fmaf(acc[d][b][j], c[b][j & 1], t[j]);
+                    }
+                }
+            };
+            if (careful) products(std::true_type{});
+            else products(std::false_type{});
+            if (careful && __any_sync(0xffffffffu, odd)) {
+                // rows that see such a value are not finite there
+#pragma unroll 1
+                for (int i = 0; i < KW; ++i) {
+                    if ((missing >> i) & 1) continue;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int at = i * LD / (int)sizeof(KV) + d * 16 + g + 8 * (j >> 1);
+                            float y;
+                            if constexpr (F32) y = reinterpret_cast<const float*>(v_ptr)[at];
+                            else y = __half2float(reinterpret_cast<const __half*>(v_ptr)[at]);
+                            if (fabsf(y) < INFINITY) continue;
+#pragma unroll
+                            for (int b = 0; b < RB; ++b)
+                                if (kt * KW + i <= lim[b][j & 1]) acc[d][b][j] = NAN;
+                        }
+                }
+            }
+        }
 
-    // ---- the warps' results together, in the ring ----
+    // ---- the warps' results together, in the rings ----
     constexpr int MLD = HDP + 4;
-    float* ma = reinterpret_cast<float*>(smem + C::Q_BYTES);
+    float* ma = reinterpret_cast<float*>(smem);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
 #pragma unroll
-    for (int d = 0; d < T::DB; ++d) {
-        float* p = ma + (warp * 16 + g) * MLD + d * 8 + 2 * (lane & 3);
-        *reinterpret_cast<float2*>(p) = make_float2(t.acc[d][0], t.acc[d][1]);
-        *reinterpret_cast<float2*>(p + 8 * MLD) = make_float2(t.acc[d][2], t.acc[d][3]);
-    }
-    if ((lane & 3) == 0) {
-        sh_m[warp][g] = t.m[0], sh_m[warp][g + 8] = t.m[1];
-        sh_l[warp][g] = t.l[0], sh_l[warp][g + 8] = t.l[1];
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                ma[(warp * R + 8 * b + 2 * t4 + (j & 1)) * MLD + d * 16 + g + 8 * (j >> 1)] =
+                    acc[d][b][j];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {  // a row's sum is spread over eight lanes
+            float x = l[b][j];
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            if (g == 0) {
+                sh_m[warp][8 * b + 2 * t4 + j] = m[b][j];
+                sh_l[warp][8 * b + 2 * t4 + j] = x;
+            }
+        }
     }
     __syncthreads();
-    const int64_t pidx = (int64_t)it.part_base + it.part;
     const int v4 = HD / 4;
-    for (int e = tid; e < rows * v4; e += C::NT) {
+    for (int e = tid; e < it.rows * v4; e += C::NT) {
         const int r = e / v4, x = (e - r * v4) * 4;
-        float M = sh_m[0][r], l = 0.f;
+        float M = sh_m[0][r], sum = 0.f;
 #pragma unroll
         for (int i = 1; i < NW; ++i) M = fmaxf(M, sh_m[i][r]);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            const float c = M == -INFINITY ? 1.f : ex2(sh_m[i][r] - M);
-            const float4 y = *reinterpret_cast<const float4*>(ma + (i * 16 + r) * MLD + x);
-            l += c * sh_l[i][r];
-            o.x += c * y.x, o.y += c * y.y, o.z += c * y.z, o.w += c * y.w;
+            const float f = M == -INFINITY ? 1.f : ex2(sh_m[i][r] - M);
+            const float4 y = *reinterpret_cast<const float4*>(ma + (i * R + r) * MLD + x);
+            sum += f * sh_l[i][r];
+            o.x += f * y.x, o.y += f * y.y, o.z += f * y.z, o.w += f * y.w;
         }
-        if (it.n_parts == 1) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            *reinterpret_cast<float4*>(out_row(A, it, G, row0 + r) + x) =
+        if (it.part < 0) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            *reinterpret_cast<float4*>(out_row(A, it, G, it.row0 + r) + x) =
                 make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         } else {
-            *reinterpret_cast<float4*>(A.part_acc + (pidx * 16 + r) * HD + x) = o;
-            if (x == 0) A.part_ml[pidx * 16 + r] = make_float2(M, l);
+            const int64_t at = (int64_t)it.part * R + r;
+            *reinterpret_cast<float4*>(A.part_acc + at * HD + x) = o;
+            if (x == 0) A.part_ml[at] = make_float2(M, sum);
         }
     }
 }
@@ -676,13 +1117,18 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
     pdl_wait();
     pdl_launch_dependents();
-    Item it;
-    if (!find_item<NT, false>(w, A.rule, blockIdx.x, it)) return;
-    const int G = w.H / w.Hkv, HD = w.HD, row0 = it.tile * R;
-    const int rows = min(R, it.s.n * G - row0);
-    const int start = it.s.L - it.s.n;
+    __shared__ Piece sh_piece;
+    __shared__ int found;
+    find_pieces<NT, 1, false>(w, A.rule, blockIdx.x, &sh_piece, &found, nullptr);
+    __syncthreads();
+    if (!found) return;
+    Piece piece = sh_piece;
+    Segment it;
+    const int G = w.H / w.Hkv, HD = w.HD;
+    while (next_segment(w, A.rule, piece, it)) {
+    const int row0 = it.row0, rows = it.rows, start = it.start;
     const int first_lim = start + row0 / G, last_lim = start + (row0 + rows - 1) / G;
-    const int kt0 = it.kt0, kt1 = min(it.kt1, last_lim < 0 ? 0 : last_lim / KT + 1);
+    const int kt0 = it.kt0, kt1 = it.kt1;
     const int n_kt = max(0, kt1 - kt0);
     const uint32_t q_base = smem_u32(smem), kv_base = q_base + C::Q_BYTES;
 
@@ -724,10 +1170,7 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     int next_page = entry_of(kt0 + S - 1);
 
     for (int r = warp; r < R; r += C::WR) {
-        const int gr = row0 + r, tok = gr / G;
-        const float* src = r < rows ? A.q + (int64_t)(it.s.q0 + tok) * A.q_stride +
-                                          (int64_t)(it.hk * G + gr - tok * G) * HD
-                                    : nullptr;
+        const float* src = r < rows ? q_row(A, it, G, row0 + r) : nullptr;
         uint8_t* hi = smem + r * T::QLD;
         const float f = stage_q_row<C::F32, HDP>(src, HD, hi, hi + R * T::QLD, A.scale_log2);
         if (lane == 0) row_scale[r] = f;
@@ -753,78 +1196,110 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
                [&](int j) { return kp[j]; });
     }
     t.finish();
-    const int64_t pidx = (int64_t)it.part_base + it.part;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int r = warp * 16 + g + 8 * h;
         if (r >= rows) continue;
-        const bool whole = it.n_parts == 1;
+        const bool whole = it.part < 0;
+        const int64_t at = (int64_t)it.part * R + r;
         const float inv = !whole ? 1.f : t.l[h] == 0.f ? 0.f : 1.f / t.l[h];
-        float* p = whole ? out_row(A, it, G, row0 + r) : A.part_acc + (pidx * R + r) * HD;
+        float* p = whole ? out_row(A, it, G, row0 + r) : A.part_acc + at * HD;
 #pragma unroll
         for (int d = 0; d < T::DB; ++d)
             if (d * 8 < HD)
                 *reinterpret_cast<float2*>(p + d * 8 + 2 * (lane & 3)) =
                     make_float2(t.acc[d][2 * h] * inv, t.acc[d][2 * h + 1] * inv);
-        if (!whole && (lane & 3) == 0) A.part_ml[pidx * R + r] = make_float2(t.m[h], t.l[h]);
+        if (!whole && (lane & 3) == 0) A.part_ml[at] = make_float2(t.m[h], t.l[h]);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the ring and q are free for the next segment
     }
 }
 
-// ---- joining the ranges of a row tile ----------------------------------------------------
-// One CTA per (row tile, row): its four warps take every fourth range each.
+// ---- joining the parts of a tile ---------------------------------------------------------
+// One CTA per (tile, row): its four warps take every fourth part each.  PIECES: the tiles were
+// cut by find_pieces, otherwise by find_item.
 struct JoinArgs {
     PagedView w;
-    SplitRule rule;
+    CutRule rule;
     float* out;
     int64_t out_stride;
     const float* part_acc;
     const float2* part_ml;
 };
 
+template <bool PIECES>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ JoinArgs A) {
     constexpr int NT = 128, MAXV = 2;  // float4 per lane: head_dim 256
     __shared__ float4 sh_acc[4][32 * MAXV];
     __shared__ float sh_l[4];
     const PagedView& w = A.w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Item it;
-    // cu_q and len were complete before the attention kernel started; its partials follow
-    const bool any = find_item<NT, true>(w, A.rule, blockIdx.x, it);
-    pdl_wait();
-    if (!any || it.n_parts == 1) return;
     const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R, r = blockIdx.y;
-    if (r >= it.s.n * G - it.tile * R) return;
+    // cu_q and len were complete before the attention kernel started; its partials follow
+    int hk, tile, n_parts, first, rest;  // the first part's place, that of part i > 0 less i * step
+    constexpr int step = PIECES ? 2 : 1;
+    SeqInfo s;
+    if constexpr (PIECES) {
+        __shared__ Piece p;
+        __shared__ long long tile_no;
+        __shared__ int found;
+        find_pieces<NT, 1, true>(w, A.rule, blockIdx.x, &p, &found, &tile_no);
+        __syncthreads();
+        pdl_wait();
+        if (!found) return;
+        s = p.x.s;
+        hk = (int)(tile_no / p.x.tiles), tile = (int)(tile_no - (long long)hk * p.x.tiles);
+        const long long start_g = (long long)G * max(s.L - s.n, 0);
+        const long long a = p.base + hk * p.x.per_head + tiles_work(tile, start_g, R);
+        const long long b = a + start_g + (long long)(tile + 1) * R;
+        // the pieces that hold a share of the tile: the first one's is its last segment (unless
+        // the tile begins with the piece), the others' is their first
+        const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
+        if (c1 >= A.rule.n_pieces) return;
+        n_parts = c1 - c0 + 1;
+        rest = 2 * c0;
+        first = rest + (a == c0 * p.len ? 0 : 1);
+    } else {
+        Item it;
+        const bool any = find_item<NT, true>(w, A.rule, blockIdx.x, it);
+        pdl_wait();
+        if (!any) return;
+        s = it.s;
+        hk = it.hk, tile = it.tile, n_parts = it.n_parts;
+        first = rest = it.part_base;
+    }
+    if (n_parts == 1 || r >= s.n * G - tile * R) return;
+    auto at = [&](int i) { return (int64_t)(i == 0 ? first : rest + i * step) * R + r; };
     float M = -INFINITY, l = 0.f;
     float4 o[MAXV];
 #pragma unroll
     for (int i = 0; i < MAXV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float2* ml = A.part_ml + (int64_t)it.part_base * R + r;
-    for (int p = lane; p < it.n_parts; p += 32) M = fmaxf(M, ml[(int64_t)p * R].x);
+    for (int i = lane; i < n_parts; i += 32) M = fmaxf(M, A.part_ml[at(i)].x);
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+    for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
 #pragma unroll 4
-    for (int p = warp; p < it.n_parts; p += 4) {
-        const float2 y = ml[(int64_t)p * R];
+    for (int i = warp; i < n_parts; i += 4) {
+        const float2 y = A.part_ml[at(i)];
         const float c = M == -INFINITY ? 1.f : ex2(y.x - M);
         l += c * y.y;
-        const float4* a =
-            reinterpret_cast<const float4*>(A.part_acc + ((int64_t)(it.part_base + p) * R + r) * HD);
+        const float4* acc = reinterpret_cast<const float4*>(A.part_acc + at(i) * HD);
 #pragma unroll
-        for (int i = 0; i < MAXV; ++i)
-            if (lane + 32 * i < HD / 4) {
-                const float4 x = a[lane + 32 * i];
-                o[i].x += c * x.x, o[i].y += c * x.y, o[i].z += c * x.z, o[i].w += c * x.w;
+        for (int k = 0; k < MAXV; ++k)
+            if (lane + 32 * k < HD / 4) {
+                const float4 x = acc[lane + 32 * k];
+                o[k].x += c * x.x, o[k].y += c * x.y, o[k].z += c * x.z, o[k].w += c * x.w;
             }
     }
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i) sh_acc[warp][lane + 32 * i] = o[i];
+    for (int k = 0; k < MAXV; ++k) sh_acc[warp][lane + 32 * k] = o[k];
     if (lane == 0) sh_l[warp] = l;
     __syncthreads();
     l = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int gr = it.tile * R + r, tok = gr / G;
-    float* out = A.out + (int64_t)(it.s.q0 + tok) * A.out_stride +
-                 (int64_t)(it.hk * G + gr - tok * G) * HD;
+    const int gr = tile * R + r, tok = gr / G;
+    float* out =
+        A.out + (int64_t)(s.q0 + tok) * A.out_stride + (int64_t)(hk * G + gr - tok * G) * HD;
     for (int x = threadIdx.x; x < HD / 4; x += NT) {
         float4 y = sh_acc[0][x];
 #pragma unroll
@@ -841,7 +1316,7 @@ constexpr int kSMs = 148;  // of a B200: the items aimed at, and so the workspac
 
 // One kernel's share of a call.
 struct Share {
-    SplitRule rule;
+    CutRule rule;
     int64_t tiles;  // most row tiles, over all kv heads
     size_t acc_off, ml_off;
 };
@@ -852,31 +1327,34 @@ struct Plan {
     size_t bytes = 0;
 };
 
-// Rules of the two: about two rounds of CTAs, so that uneven ranges even out, and at least 128
-// positions a range, below which joining costs more.
-template <typename KV, int HDP>
-static SplitRule narrow_rule(int min_rows, int max_rows) {
-    using C = NarrowCfg<KV, HDP>;
-    return SplitRule{16, C::KW, min_rows, max_rows, kSMs * C::CTAS * 2, 128 / C::KW};
+// Parts for two rounds of the CTAs that the GPU holds at once, or one piece for each of them,
+// of at least 128 positions: below that joining costs more.
+template <typename KV, int HDP, int RB>
+static CutRule narrow_rule(int min_rows, int max_rows) {
+    using C = NarrowCfg<KV, HDP, RB>;
+    return CutRule{C::R, C::KW, min_rows, max_rows, kSMs * C::CTAS * 2, 128};
 }
 template <typename KV, int HDP>
-static SplitRule wide_rule(int min_rows, int max_rows) {
+static CutRule wide_rule(int min_rows, int max_rows) {
     using C = WideCfg<KV, HDP>;
-    return SplitRule{C::R, C::KT, min_rows, max_rows, kSMs * 2, 128 / C::KT};
+    return CutRule{C::R, C::KT, min_rows, max_rows, kSMs, 128};
 }
 
 template <typename Kern>
-static int rows_launch(Kern kern, int threads, size_t smem, const RowsArgs& a, int64_t tiles,
-                       cudaStream_t st) {
+static int rows_launch(Kern kern, int threads, size_t smem, bool pieces, const RowsArgs& a,
+                       int64_t tiles, int64_t max_pos, cudaStream_t st) {
     IB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int64_t grid = tiles + a.rule.target;
+    // pieces: no more than `least` allows; parts: at most one more per tile
+    const int64_t most = tiles * (max_pos / a.rule.least + 1 + a.rule.R);
+    const int64_t grid = std::min<int64_t>(a.rule.n_pieces + (pieces ? 0 : tiles), most);
     IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(threads), smem, st, true, a));
     return IB_OK;
 }
 
-// The kernels of a call, by the rows (new tokens x group) that a sequence may have: up to 16
-// on the narrow kernel, more on the wide one.  With one sequence, or a bound that rules the
-// wide one out, a single kernel takes everything.
+// The kernels of a call, by the rows (new tokens x group) that a sequence may have.  Where the
+// caller's bound allows no more than 16, one narrow kernel takes everything; otherwise the
+// narrow one takes the sequences with up to 8 rows (16 where a single token has more) and the
+// wide one the rest, or everything where there is one sequence or a token has over 16.
 template <typename KV, int HDP>
 static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     constexpr int ALL = 0x7fffffff;
@@ -885,7 +1363,7 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     const int64_t most_q = b->max_q > 0 ? std::min(b->max_q, b->n_tokens) : b->n_tokens;
     const int64_t seqs = std::min(b->n_seqs, b->n_tokens);
     Plan plan;
-    auto add = [&](const SplitRule& r, int64_t tiles_per_head) {
+    auto add = [&](const CutRule& r, int64_t tiles_per_head) {
         Share& s = plan.share[plan.n++];
         s.rule = r;
         s.tiles = tiles_per_head * p->n_kv_heads;
@@ -894,16 +1372,23 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
             plan.bytes += (n + 255) / 256 * 256;
             return at;
         };
-        // at most 2 x target partials: a tile of k > len key tiles has ceil(k / len) <= 2 k / len
-        s.acc_off = take((size_t)2 * r.target * r.R * p->head_dim * sizeof(float));
-        s.ml_off = take((size_t)2 * r.target * r.R * sizeof(float2));
+        // a piece cuts at most the tile it begins in and the one it ends in; a tile of k > len key
+        // tiles has ceil(k / len) <= 2 k / len parts
+        s.acc_off = take((size_t)2 * r.n_pieces * r.R * p->head_dim * sizeof(float));
+        s.ml_off = take((size_t)2 * r.n_pieces * r.R * sizeof(float2));
     };
     const int64_t rows = b->n_tokens * G;
-    if (most_q * G <= 16) {
-        add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 16);
+    constexpr bool TWO = HDP * sizeof(KV) <= 256;  // 16 rows fit a warp's registers
+    if (most_q * G <= 8) {
+        add(narrow_rule<KV, HDP, 1>(1, ALL), seqs + rows / 8);
+    } else if (TWO && most_q * G <= 16) {
+        if constexpr (TWO) add(narrow_rule<KV, HDP, 2>(1, ALL), seqs + rows / 16);
     } else {
-        if (b->n_seqs > 1) add(narrow_rule<KV, HDP>(1, 16), seqs);
-        add(wide_rule<KV, HDP>(b->n_seqs > 1 ? 17 : 1, ALL), seqs + rows / WIDE);
+        const int narrow = b->n_seqs == 1 ? 0 : G <= 8 ? 8 : TWO && G <= 16 ? 16 : 0;
+        if (narrow == 8) add(narrow_rule<KV, HDP, 1>(1, 8), seqs);
+        if constexpr (TWO)
+            if (narrow == 16) add(narrow_rule<KV, HDP, 2>(1, 16), seqs);
+        add(wide_rule<KV, HDP>(narrow + 1, ALL), seqs + rows / WIDE);
     }
     return plan;
 }
@@ -911,25 +1396,30 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
 template <typename KV, int HDP>
 static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan, RowsArgs a,
                     uint8_t* ws, int64_t max_pos, cudaStream_t st) {
-    using N = NarrowCfg<KV, HDP>;
+    constexpr int RB2 = HDP * sizeof(KV) <= 256 ? 2 : 1;
+    using N1 = NarrowCfg<KV, HDP, 1>;
+    using N2 = NarrowCfg<KV, HDP, RB2>;
     using W = WideCfg<KV, HDP>;
     for (int i = 0; i < plan.n; ++i) {
         const Share& s = plan.share[i];
         a.rule = s.rule;
+        const bool wide = s.rule.R == W::R;
         a.part_acc = reinterpret_cast<float*>(ws + s.acc_off);
         a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
         const int r =
-            s.rule.R == 16
-                ? rows_launch(attn_narrow_kernel<KV, HDP>, N::NT, N::SMEM, a, s.tiles, st)
-                : rows_launch(attn_wide_kernel<KV, HDP>, W::NT, W::SMEM, a, s.tiles, st);
+            s.rule.R == 8
+                ? rows_launch(attn_narrow_kernel<KV, HDP, 1>, N1::NT, N1::SMEM, false, a, s.tiles, max_pos, st)
+            : s.rule.R == 16
+                ? rows_launch(attn_narrow_kernel<KV, HDP, RB2>, N2::NT, N2::SMEM, false, a, s.tiles, max_pos, st)
+                : rows_launch(attn_wide_kernel<KV, HDP>, W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
         if (r != IB_OK) return r;
-        // no range is cut where the longest row of a table is no longer than the least
-        if (max_pos > (int64_t)s.rule.least * s.rule.KT) {
+        {
             const JoinArgs j{a.w, s.rule, a.out, a.out_stride, a.part_acc, a.part_ml};
             const int64_t G = a.w.H / a.w.Hkv;
             const int64_t most_rows = std::min<int64_t>(s.rule.R, b->n_tokens * G);
-            IB_CUDA_CHECK(launch_pdl(attn_join_kernel, dim3((unsigned)s.tiles, (unsigned)most_rows),
-                                     dim3(128), 0, st, true, j));
+            const auto join = wide ? attn_join_kernel<true> : attn_join_kernel<false>;
+            IB_CUDA_CHECK(launch_pdl(join, dim3((unsigned)s.tiles, (unsigned)most_rows), dim3(128),
+                                     0, st, true, j));
         }
     }
     return IB_OK;

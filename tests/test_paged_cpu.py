@@ -51,7 +51,7 @@ BAD_POOL = [dict(p=pages(k=None)), dict(p=pages(v=None)), dict(p=pages(k=PTR + 8
             dict(p=pages(head_dim=0)), dict(p=pages(head_dim=20)), dict(p=pages(head_dim=264)),
             dict(s=seqs(table=None)), dict(s=seqs(len=None)), dict(s=seqs(refs=None)),
             dict(s=seqs(n_slots=0)), dict(s=seqs(n_slots=16385)), dict(s=seqs(max_pages=0)),
-            dict(s=seqs(max_pages=2 ** 26 + 1))]
+            dict(s=seqs(max_pages=2 ** 24 + 1))]
 BAD_BATCH = [dict(b=batch(cu_q=None)), dict(b=batch(n_seqs=-1)), dict(b=batch(n_tokens=-1)),
              dict(b=batch(max_q=-1)), dict(b=batch(slots=None, n_seqs=5)), dict(layer=-1),
              dict(layer=2), dict(H=0), dict(H=3), dict(b=batch(n_tokens=2 ** 28 + 1)),
