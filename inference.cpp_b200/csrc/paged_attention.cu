@@ -872,8 +872,10 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
 }
 
 // ---- joining the parts of a tile ---------------------------------------------------------
-// One CTA per (tile, row): its four warps take every fourth part each.  PIECES: the tiles were
-// cut by find_pieces, otherwise by find_item.
+// PIECES: the tiles were cut by find_pieces -- most are whole, the others in two or three -- and
+// a CTA sees to JOIN_ROWS rows of a tile, a warp to one after another.  Otherwise by find_item,
+// into many parts, and a CTA sees to one row, its four warps to every fourth part each.
+constexpr int JOIN_ROWS = 64;
 struct JoinArgs {
     PagedView w;
     CutRule rule;
@@ -890,7 +892,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     __shared__ float sh_l[4];
     const PagedView& w = A.w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R, r = blockIdx.y;
+    const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R;
     // cu_q and len were complete before the attention kernel started; its partials follow
     int hk, tile, n_parts, first, rest;  // the first part's place, that of part i > 0 less i * step
     constexpr int step = PIECES ? 2 : 1;
@@ -924,45 +926,55 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
         hk = it.hk, tile = it.tile, n_parts = it.n_parts;
         first = rest = it.part_base;
     }
-    if (n_parts == 1 || r >= s.n * G - tile * R) return;
-    auto at = [&](int i) { return (int64_t)(i == 0 ? first : rest + i * step) * R + r; };
-    float M = -INFINITY, l = 0.f;
-    float4 o[MAXV];
+    const int rows = min(R, s.n * G - tile * R);
+    const int r0 = PIECES ? blockIdx.y * JOIN_ROWS + warp : blockIdx.y;
+    if (n_parts == 1) return;
+    for (int r = r0; r < min(rows, PIECES ? (int)(blockIdx.y + 1) * JOIN_ROWS : r0 + 1); r += 4) {
+        auto at = [&](int i) { return (int64_t)(i == 0 ? first : rest + i * step) * R + r; };
+        float M = -INFINITY, l = 0.f;
+        float4 o[MAXV];
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = lane; i < n_parts; i += 32) M = fmaxf(M, A.part_ml[at(i)].x);
+        for (int i = 0; i < MAXV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = lane; i < n_parts; i += 32) M = fmaxf(M, A.part_ml[at(i)].x);
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+        for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
 #pragma unroll 4
-    for (int i = warp; i < n_parts; i += 4) {
-        const float2 y = A.part_ml[at(i)];
-        const float c = M == -INFINITY ? 1.f : ex2(y.x - M);
-        l += c * y.y;
-        const float4* acc = reinterpret_cast<const float4*>(A.part_acc + at(i) * HD);
+        for (int i = PIECES ? 0 : warp; i < n_parts; i += PIECES ? 1 : 4) {
+            const float2 y = A.part_ml[at(i)];
+            const float c = M == -INFINITY ? 1.f : ex2(y.x - M);
+            l += c * y.y;
+            const float4* acc = reinterpret_cast<const float4*>(A.part_acc + at(i) * HD);
+#pragma unroll
+            for (int k = 0; k < MAXV; ++k)
+                if (lane + 32 * k < HD / 4) {
+                    const float4 x = acc[lane + 32 * k];
+                    o[k].x += c * x.x, o[k].y += c * x.y, o[k].z += c * x.z, o[k].w += c * x.w;
+                }
+        }
+        if constexpr (!PIECES) {
+#pragma unroll
+            for (int k = 0; k < MAXV; ++k) sh_acc[warp][lane + 32 * k] = o[k];
+            if (lane == 0) sh_l[warp] = l;
+            __syncthreads();
+            if (warp > 0) return;
+            l = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
+#pragma unroll
+            for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+                for (int i = 1; i < 4; ++i) {
+                    const float4 z = sh_acc[i][lane + 32 * k];
+                    o[k].x += z.x, o[k].y += z.y, o[k].z += z.z, o[k].w += z.w;
+                }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int gr = tile * R + r, tok = gr / G;
+        float4* out = reinterpret_cast<float4*>(A.out + (int64_t)(s.q0 + tok) * A.out_stride +
+                                                (int64_t)(hk * G + gr - tok * G) * HD);
 #pragma unroll
         for (int k = 0; k < MAXV; ++k)
-            if (lane + 32 * k < HD / 4) {
-                const float4 x = acc[lane + 32 * k];
-                o[k].x += c * x.x, o[k].y += c * x.y, o[k].z += c * x.z, o[k].w += c * x.w;
-            }
-    }
-#pragma unroll
-    for (int k = 0; k < MAXV; ++k) sh_acc[warp][lane + 32 * k] = o[k];
-    if (lane == 0) sh_l[warp] = l;
-    __syncthreads();
-    l = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int gr = tile * R + r, tok = gr / G;
-    float* out =
-        A.out + (int64_t)(s.q0 + tok) * A.out_stride + (int64_t)(hk * G + gr - tok * G) * HD;
-    for (int x = threadIdx.x; x < HD / 4; x += NT) {
-        float4 y = sh_acc[0][x];
-#pragma unroll
-        for (int i = 1; i < 4; ++i) {
-            const float4 z = sh_acc[i][x];
-            y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
-        }
-        reinterpret_cast<float4*>(out)[x] = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+            if (lane + 32 * k < HD / 4)
+                out[lane + 32 * k] =
+                    make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
     }
 }
 
@@ -1085,8 +1097,9 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
             const JoinArgs j{a.w, s.rule, a.out, a.out_stride, a.part_acc, a.part_ml};
             const int64_t G = a.w.H / a.w.Hkv;
             const int64_t most_rows = std::min<int64_t>(s.rule.R, b->n_tokens * G);
+            const int64_t per = wide ? JOIN_ROWS : 1;
             const auto join = wide ? attn_join_kernel<true> : attn_join_kernel<false>;
-            IB_CUDA_CHECK(launch_pdl(join, dim3((unsigned)s.tiles, (unsigned)most_rows), dim3(128),
+            IB_CUDA_CHECK(launch_pdl(join, dim3((unsigned)s.tiles, (unsigned)((most_rows + per - 1) / per)), dim3(128),
                                      0, st, true, j));
         }
     }

@@ -11,8 +11,8 @@
 // thread, where acc = acc c + O takes the softmax's rescaling with it.
 //
 // Tensor memory, 512 columns: S of both query tiles (128 each), O of both (128 each).  p lies
-// over its S: thread and chunk of 32 scores write hi into the chunk's first 16 columns and lo
-// into the other 16, which that thread alone has read.
+// over its S: of a chunk of 16 scores a thread writes hi into the first 8 columns and lo into the
+// other 8, and an MMA's 16 positions are one chunk.
 // Shared memory: q of both tiles as hi and lo (128 KB at head_dim 128) and a ring of three slots
 // for K and V tiles in turn.  Rows are 128 bytes (64 elements) under the 128-byte swizzle; K is
 // read with head_dim along the MMA's K (K-major), V with positions along it (MN-major), so both
@@ -75,51 +75,74 @@ constexpr uint32_t pt_idesc(int M, int N, bool b_mn) {
            ((uint32_t)(M >> 4) << 24);
 }
 
+// The whole warp comes here with the same operands and `leader` lets one thread issue: the
+// operands then are uniform registers, as the instruction takes them.  Issued inside a branch of
+// one thread, every operand is moved there first, and an MMA took 134 cycles instead of 64.
 __device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t add) {
+                                          uint32_t add, uint32_t leader) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
         : "memory");
 }
 __device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t add) {
+                                          uint32_t add, uint32_t leader) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(add)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
         : "memory");
 }
 
-__device__ __forceinline__ void pt_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void pt_commit(uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(
+            smem_u32(bar)),
+        "r"(leader)
+        : "memory");
 }
 
-// 32 columns of this warp's 32 lanes
-__device__ __forceinline__ void pt_ld32(uint32_t taddr, float (&v)[32]) {
+// One thread of the (converged) warp.
+__device__ __forceinline__ uint32_t pt_elect() {
+    uint32_t x;
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-        "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-        "%30, %31}, [%32];"
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(x));
+    return x;
+}
+
+// 16 columns of this warp's 32 lanes, to be waited for
+__device__ __forceinline__ void pt_ld16(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15}, [%16];"
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
           "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
-          "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
-          "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
-          "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+          "=f"(v[14]), "=f"(v[15])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+// The loads' registers pass through the wait, so that nothing uses them before it.
+__device__ __forceinline__ void pt_wait_ld(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                   "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                   "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void pt_st8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
         : "memory");
 }
 
@@ -274,10 +297,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 pt_fence_after();
 #pragma unroll
                 for (int d0 = 0; d0 < HDP; d0 += 32) {
-                    float o[32];
-                    pt_ld32(o_at + d0, o);
+                    float o[16], o2[16];
+                    pt_ld16(o_at + d0, o);
+                    pt_ld16(o_at + d0 + 16, o2);
+                    pt_wait_ld(o);
+                    pt_wait_ld(o2);
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) acc[d0 + d] = fmaf(acc[d0 + d], c_last, o[d]);
+                    for (int d = 0; d < 16; ++d) {
+                        acc[d0 + d] = fmaf(acc[d0 + d], c_last, o[d]);
+                        acc[d0 + 16 + d] = fmaf(acc[d0 + 16 + d], c_last, o2[d]);
+                    }
                 }
                 pt_fence_before();
                 mbar_arrive(&bar.o_empty[t]);
@@ -302,19 +331,29 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     all = all && (gone.x | gone.y | gone.z | gone.w) == 0;
                 }
                 all = __all_sync(0xffffffffu, all);
+                // the next 16 scores are on their way while these are worked on
+                auto mask = [&](float (&s)[16], int i) {
+                    const uint32_t see = visible(j, i >> 1) >> (16 * (i & 1));
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (!((see >> k) & 1)) s[k] = -INFINITY;
+                };
                 float top = -INFINITY;
+                auto maximum = [&](float (&s)[16], int i) {
+                    if (!all) mask(s, i);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float s[32];
-                    pt_ld32(s_at + 32 * i, s);
-                    if (!all) {
-                        const uint32_t see = visible(j, i);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (!((see >> k) & 1)) s[k] = -INFINITY;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) top = fmaxf(top, s[k]);
+                    for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
+                };
+                float s0[16], s1[16];
+                pt_ld16(s_at, s0);
+#pragma unroll 1
+                for (int i = 0; i < 8; i += 2) {
+                    pt_wait_ld(s0);
+                    pt_ld16(s_at + 16 * i + 16, s1);
+                    maximum(s0, i);
+                    pt_wait_ld(s1);
+                    pt_ld16(s_at + ((16 * i + 32) & 127), s0);  // the last: the first, for below
+                    maximum(s1, i + 1);
                 }
                 top = fmaxf(m, top);  // of the scores before scaling
                 const bool none = top == -INFINITY;
@@ -322,26 +361,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 const float off = none ? 0.f : 10.f - top * sc;
                 m = top;
                 float sum = 0.f;
+                auto weights = [&](float (&s)[16], int i) {
+                    if (!all) mask(s, i);
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float s[32];
-                    pt_ld32(s_at + 32 * i, s);
-                    if (!all) {
-                        const uint32_t see = visible(j, i);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (!((see >> k) & 1)) s[k] = -INFINITY;
-                    }
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
+                    for (int k = 0; k < 8; ++k) {
                         const float x = ex2(fmaf(s[2 * k], sc, off));
                         const float y = ex2(fmaf(s[2 * k + 1], sc, off));
                         sum += x + y;
                         split2(x, y, hi[k], lo[k]);
                     }
-                    pt_st16(s_at + 32 * i, hi);
-                    pt_st16(s_at + 32 * i + 16, lo);
+                    pt_st8(s_at + 16 * i, hi);
+                    pt_st8(s_at + 16 * i + 8, lo);
+                };
+#pragma unroll 1
+                for (int i = 0; i < 8; i += 2) {
+                    pt_wait_ld(s0);
+                    pt_ld16(s_at + 16 * i + 16, s1);
+                    weights(s0, i);
+                    pt_wait_ld(s1);
+                    if (i < 6) pt_ld16(s_at + 16 * i + 32, s0);
+                    weights(s1, i + 1);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 l = fmaf(l, c, sum);
@@ -383,26 +423,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             int half = 0;               // K and V tiles so far: the ring's order
             int n_q[2] = {0, 0}, n_s[2] = {0, 0};  // q tiles and key tiles so far
             bool ok = true;
+            const uint32_t leader = pt_elect();
             auto scores = [&](int t, uint32_t k_at) {
-                const uint32_t q_at = base + (uint32_t)(2 * t * C::TILE);
+                const uint64_t qa = pt_desc(base + (uint32_t)(2 * t * C::TILE), 16);
+                const uint64_t kb = pt_desc(k_at, 16);
 #pragma unroll
                 for (int part = 1; part >= 0; --part)  // lo, then hi
 #pragma unroll
                     for (int k = 0; k < HDP / 16; ++k) {
-                        const uint32_t off = (uint32_t)((k >> 2) * C::BLOCK + (k & 3) * 32);
-                        pt_mma_ss(tmem + 128 * t, pt_desc(q_at + part * C::TILE + off, 16),
-                                  pt_desc(k_at + off, 16), id_s, part == 0 || k > 0);
+                        const uint32_t off = (uint32_t)((k >> 2) * (C::BLOCK >> 4) + (k & 3) * 2);
+                        pt_mma_ss(tmem + 128 * t, qa + (uint32_t)(part * (C::TILE >> 4)) + off, kb + off,
+                                  id_s, part == 0 || k > 0, leader);
                     }
             };
             auto outputs = [&](int t, uint32_t v_at) {
+                const uint64_t vb = pt_desc(v_at, C::BLOCK);
 #pragma unroll
                 for (int part = 1; part >= 0; --part)
 #pragma unroll
-                    for (int k = 0; k < PT_KT / 16; ++k)
-                        pt_mma_ts(tmem + 256 + 128 * t,
-                                  tmem + 128 * t + 32 * (k >> 1) + 16 * part + 8 * (k & 1),
-                                  pt_desc(v_at + (uint32_t)(k * 2048), C::BLOCK), id_o,
-                                  part == 0 || k > 0);
+                    for (int k = 0; k < PT_KT / 16; ++k)  // 16 rows, 2048 bytes, a step
+                        pt_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 16 * k + 8 * part,
+                                  vb + (uint32_t)(k * 128), id_o, part == 0 || k > 0, leader);
             };
             while (ok && next()) {
                 const int n_kt = it.kt1 - it.kt0, n_t = it.rows > 128 ? 2 : 1;
@@ -416,10 +457,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 for (int t = 0; t < n_t && ok; ++t) {
                     ok = wait(&bar.q_full[t], n_q[t]++);
                     pt_fence_after();
-                    if (ok && lane == 0) {
+                    if (ok) {
                         scores(t, slot_at(half));
-                        pt_commit(&bar.s_full[t]);
-                        if (t == n_t - 1) pt_commit(&bar.kv_empty[half % PT_SLOTS]);
+                        pt_commit(&bar.s_full[t], leader);
+                        if (t == n_t - 1) pt_commit(&bar.kv_empty[half % PT_SLOTS], leader);
                     }
                 }
                 for (int j = 0; j < n_kt && ok; ++j) {
@@ -430,17 +471,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                         if (n_s[t] > 0) ok = ok && wait(&bar.o_empty[t], n_s[t] - 1);
                         ++n_s[t];
                         pt_fence_after();
-                        if (ok && lane == 0) {
+                        if (ok) {
                             outputs(t, slot_at(hv));
-                            pt_commit(&bar.o_full[t]);
-                            if (t == n_t - 1) pt_commit(&bar.kv_empty[hv % PT_SLOTS]);
+                            pt_commit(&bar.o_full[t], leader);
+                            if (t == n_t - 1) pt_commit(&bar.kv_empty[hv % PT_SLOTS], leader);
                         }
                         if (j + 1 < n_kt) {
                             if (t == 0) arrived(hk);
-                            if (ok && lane == 0) {
+                            if (ok) {
                                 scores(t, slot_at(hk));
-                                pt_commit(&bar.s_full[t]);
-                                if (t == n_t - 1) pt_commit(&bar.kv_empty[hk % PT_SLOTS]);
+                                pt_commit(&bar.s_full[t], leader);
+                                if (t == n_t - 1) pt_commit(&bar.kv_empty[hk % PT_SLOTS], leader);
                             }
                         }
                         __syncwarp();
@@ -449,8 +490,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 half += 2 * n_kt;
             }
             // the MMAs issued are done before tensor memory is given back
-            if (lane == 0) pt_commit(&bar.done);
-            __syncwarp();
+            pt_commit(&bar.done, leader);
             wait(&bar.done, 0);
         } else {
             // ---- copies: 16 rows at a time, lane j (and j + 16) sees to row j ----
@@ -466,16 +506,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
                 const int first_lim = it.start + it.row0 / G;
                 for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
-                    int row[3];
+                    // the tile's table entries, for K and V; -1: no page, or not seen
+                    int rows3[3];
 #pragma unroll
                     for (int i = 0; i < 3; ++i) {
                         const int pos = kt * PT_KT + (lw + 3 * i) * 16 + (lane & 15);
-                        row[i] = -1;
+                        rows3[i] = -1;
                         if (lw + 3 * i < 8 && pos <= last_lim) {
                             const int col = (int)w.ps.div((uint32_t)pos);
                             const int page = page_at(w, it.s.row[col]);
                             if (page >= 0)
-                                row[i] = (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
+                                rows3[i] = (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
                         }
                     }
                     const bool careful = kt * PT_KT + PT_KT - 1 > first_lim;
@@ -488,37 +529,44 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                         }
                         const uint32_t dst = ring + (uint32_t)(slot * C::TILE + (x >> 3) * C::BLOCK);
                         const uint8_t* src = src_x[kv];
-#pragma unroll
+                        // small loops: this code shares the instruction cache with the softmax
+#pragma unroll 1
                         for (int i = 0; i < 3; ++i) {
                             const int g16 = lw + 3 * i;
-                            if (g16 >= 8) continue;
+                            if (g16 >= 8) break;
+                            const int row = i == 0 ? rows3[0] : i == 1 ? rows3[1] : rows3[2];
                             uint32_t bad = 0;
-#pragma unroll
-                            for (int k = 0; k < 16 / RL; ++k) {
-                                const int from = k * RL + r0;
-                                const int n = __shfl_sync(0xffffffffu, row[i], from);
-                                const bool there = n >= 0 && in_row;
-                                const uint8_t* p = src + (there ? (int64_t)n * row_bytes : 0);
-                                const uint32_t d = dst + pt_off(g16 * 16 + from, x & 7);
-                                if (kv == 0 || !careful) {
-                                    cp16(d, p, there);
-                                } else {
+                            if (kv == 0 || !careful) {
+#pragma unroll 4
+                                for (int k = 0; k < 16 / RL; ++k) {
+                                    const int from = k * RL + r0;
+                                    const int n = __shfl_sync(0xffffffffu, row, from);
+                                    const bool there = n >= 0 && in_row;
+                                    cp16(dst + pt_off(g16 * 16 + from, x & 7),
+                                         src + (there ? (int64_t)n * row_bytes : 0), there);
+                                }
+                            } else {
+#pragma unroll 1
+                                for (int k = 0; k < 16 / RL; ++k) {
+                                    const int from = k * RL + r0;
+                                    const int n = __shfl_sync(0xffffffffu, row, from);
                                     uint4 v = make_uint4(0, 0, 0, 0);
-                                    if (there) v = __ldg(reinterpret_cast<const uint4*>(p));
+                                    if (n >= 0 && in_row)
+                                        v = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)n * row_bytes));
                                     bool odd = false;
                                     v.x = finite16x2(v.x, odd), v.y = finite16x2(v.y, odd);
                                     v.z = finite16x2(v.z, odd), v.w = finite16x2(v.w, odd);
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(d),
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                                     dst + pt_off(g16 * 16 + from, x & 7)),
                                                  "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                                                  : "memory");
                                     const uint32_t any = __ballot_sync(0xffffffffu, odd);
 #pragma unroll
                                     for (int b = 0; b < RL; ++b)
-                                        if (any & (((CH == 32 ? 0u : (1u << CH)) - 1u) << (b * CH)))
-                                            bad |= 1u << (k * RL + b);
+                                        if (any & (((1u << CH) - 1u) << (b * CH))) bad |= 1u << (k * RL + b);
                                 }
                             }
-                            const uint32_t none = __ballot_sync(0xffffffffu, row[i] < 0) & 0xffffu;
+                            const uint32_t none = __ballot_sync(0xffffffffu, row < 0) & 0xffffu;
                             if (lane == 0) {
                                 if (kv == 0) sh_gone[tile_no & 3][g16] = (uint16_t)none;
                                 else sh_bad[tile_no & 3][g16] = (uint16_t)bad;
