@@ -94,6 +94,7 @@ PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batc
     w.HD = p->head_dim;
     w.page_size = p->page_size;
     w.ps = FastDiv::make((uint32_t)p->page_size);
+    w.group = FastDiv::make((uint32_t)(n_heads / p->n_kv_heads));
     return w;
 }
 

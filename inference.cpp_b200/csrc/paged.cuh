@@ -49,7 +49,8 @@ struct PagedView {
     int n_slots, max_pages, n_pages;
     int n_seqs, n_tokens;
     int H, Hkv, HD, page_size;
-    FastDiv ps;
+    FastDiv ps;     // of page_size
+    FastDiv group;  // of H / Hkv
 };
 
 // Each translation unit's kernels record their first fault here.

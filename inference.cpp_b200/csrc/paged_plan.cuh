@@ -185,8 +185,9 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     const int seen = max(0, g.start + (g.row0 + g.rows - 1) / G + 1);
     const int nkt = (seen + rule.KT - 1) / rule.KT;
     // the same value for a piece's end and the next one's beginning
-    g.kt0 = x0 == 0 ? 0 : (int)((double)nkt * (double)x0 / (double)all);
-    g.kt1 = x1 == all ? nkt : (int)((double)nkt * (double)x1 / (double)all);
+    // (below 2^24 x 2^38: paged_check_batch)
+    g.kt0 = x0 == 0 ? 0 : (int)(nkt * x0 / all);
+    g.kt1 = x1 == all ? nkt : (int)(nkt * x1 / all);
     const bool whole = x0 == 0 && x1 == all;
     g.part = whole ? -1 : 2 * p.no + (p.at == p.no * p.len ? 0 : 1);
     p.at += x1 - x0;
@@ -323,12 +324,12 @@ struct RowsArgs {
 
 // Row `gr` of the segment's sequence and kv head.
 __device__ __forceinline__ float* out_row(const RowsArgs& A, const Segment& it, int G, int gr) {
-    const int tok = gr / G;
+    const int tok = (int)A.w.group.div((uint32_t)gr);
     return A.out + (int64_t)(it.s.q0 + tok) * A.out_stride +
            (int64_t)(it.hk * G + gr - tok * G) * A.w.HD;
 }
 __device__ __forceinline__ const float* q_row(const RowsArgs& A, const Segment& it, int G, int gr) {
-    const int tok = gr / G;
+    const int tok = (int)A.w.group.div((uint32_t)gr);
     return A.q + (int64_t)(it.s.q0 + tok) * A.q_stride + (int64_t)(it.hk * G + gr - tok * G) * A.w.HD;
 }
 

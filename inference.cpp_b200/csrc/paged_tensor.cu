@@ -18,14 +18,20 @@
 // read with head_dim along the MMA's K (K-major), V with positions along it (MN-major), so both
 // are stored as they lie in the pages.
 // Warps: 0-3 and 4-7 the softmax of a query tile each (thread = row), 8 issues the MMAs, 9-11
-// copy K and V row by row with cp.async, since pages end anywhere.  The order of MMAs is
+// bring K and V in: with TMA in boxes of as many rows as divide both a page and the tile (8 at
+// least; a box of a page that is not there lies outside the tensor and reads as zeros), or, for
+// other page sizes, row by row.  In tiles where some row does not see a position, they make V
+// finite before it is used (0 x inf).  The order of MMAs is
 //     O0(j) S0(j+1) O1(j) S1(j+1) O0(j+1) ...
 // so that a tile's softmax has the other tile's MMAs to hide behind.
 // Work per CTA is a piece of the batch (paged_plan.cuh); the copies run on into the next
 // segment.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <mutex>
 #include <string>
 
 #include "common.cuh"
@@ -120,22 +126,29 @@ __device__ __forceinline__ uint32_t pt_elect() {
     return x;
 }
 
-// 16 columns of this warp's 32 lanes, to be waited for
-__device__ __forceinline__ void pt_ld16(uint32_t taddr, float (&v)[16]) {
+// 32 columns of this warp's 32 lanes, to be waited for
+__device__ __forceinline__ void pt_ld32(uint32_t taddr, float (&v)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-        "%12, %13, %14, %15}, [%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31}, [%32];"
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
-          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
-          "=f"(v[14]), "=f"(v[15])
+          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]),
+          "=f"(v[31])
         : "r"(taddr));
 }
 // The loads' registers pass through the wait, so that nothing uses them before it.
-__device__ __forceinline__ void pt_wait_ld(float (&v)[16]) {
+__device__ __forceinline__ void pt_wait_ld(float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
-                   "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
-                   "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
+                   "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]),
+                   "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]),
+                   "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                   "+f"(v[30]), "+f"(v[31])
                  :
                  : "memory");
 }
@@ -146,19 +159,61 @@ __device__ __forceinline__ void pt_st8(uint32_t taddr, const uint32_t (&v)[8]) {
         : "memory");
 }
 
+// Two FP32 operations in one instruction: x = a b + c and x + a, element by element.
+__device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b0, float b1,
+                                     float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 c, a, b, c;\n\t"
+        "mov.b64 {%0, %1}, c;\n\t}"
+        : "=f"(x0), "=f"(x1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
+    asm("{\n\t.reg .b64 a, c;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 c, {%0, %1};\n\t"
+        "add.rn.f32x2 c, a, c;\n\t"
+        "mov.b64 {%0, %1}, c;\n\t}"
+        : "+f"(x0), "+f"(x1)
+        : "f"(a0), "f"(a1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float x;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(x) : "f"(a), "f"(b), "f"(c));
+    return x;
+}
+
 // Byte offset of 16-byte chunk c (0-7) of row r in a swizzled block.
 __device__ __forceinline__ uint32_t pt_off(int r, int c) {
     return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
 }
 
+// 2-D tiled TMA load (no multicast) of the box at (x = column, y = row), completing on bar.  x is
+// a multiple of 64 FP16 (128 bytes).
+__device__ __forceinline__ void pt_tma(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                       uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+
+struct TensorArgs {
+    RowsArgs rows;
+    CUtensorMap k, v;  // the layer's rows [page, kv head, position in page][head_dim]
+    int box;           // log2 of a box's rows, 0: no TMA
+};
+
 struct TensorBars {
     uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS];
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], done;
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], v_there, done;
 };
 
 template <int HDP>
 __global__ void __launch_bounds__(PT_THREADS, 1)
-    attn_tensor_kernel(const __grid_constant__ RowsArgs A) {
+    attn_tensor_kernel(const __grid_constant__ TensorArgs TA) {
+    const RowsArgs& A = TA.rows;
     using C = TensorCfg<HDP>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) TensorBars bar;
@@ -178,6 +233,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
     if (tid == 0) {
+        if (TA.box) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.k)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.v)) : "memory");
+        }
         for (int i = 0; i < PT_SLOTS; ++i) {
             mbar_init(&bar.kv_full[i], PT_LOADERS + PT_LOADERS / 32);
             mbar_init(&bar.kv_empty[i], 1);
@@ -188,8 +247,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             mbar_init(&bar.s_full[i], 1);
             mbar_init(&bar.p_full[i], 128);
             mbar_init(&bar.o_full[i], 1);
-            mbar_init(&bar.o_empty[i], 128);
         }
+        mbar_init(&bar.v_there, 1);
         mbar_init(&bar.done, 1);
         fence_mbar_init();
     }
@@ -223,7 +282,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 
     if (warp < 8) {
         // ---- softmax of query tile t: thread = row ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int t = warp >> 2, wr = (warp & 3) * 32;  // this warp's rows of the tile, its lanes
         uint8_t* const q_ptr = base_ptr + 2 * t * C::TILE;
         const uint32_t s_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(128 * t);
@@ -237,8 +296,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             const uint32_t first = seen;
             seen += (uint32_t)n_kt;
             if (rows <= 0) continue;
-            // q: this warp's 32 rows, HDP / 4 lanes to a row
-            constexpr int LPR = HDP / 4, RPI = 32 / LPR;  // lanes per row, rows at a time
+            // q: this warp's 32 rows, HDP / 8 lanes to a row
+            constexpr int LPR = HDP / 8, RPI = 32 / LPR;  // lanes per row, rows at a time
             float my_scale = 0.f;
             const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
             // every warp of the tile has stored the last segment's rows from here
@@ -246,30 +305,41 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             ++segs;
             if (!ok) break;
             if (n_kt > 0) {
-#pragma unroll 4
-                for (int i = 0; i < 32; i += RPI) {
-                    const int r = wr + i + lane / LPR, d = (lane % LPR) * 4;
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < rows && d < HD)
-                        x = __ldg(reinterpret_cast<const float4*>(
-                            q_row(A, it, G, it.row0 + 128 * t + r) + d));
-                    float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                const int d = (lane % LPR) * 8;
+                constexpr int AT_ONCE = 4;  // loads on their way
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += AT_ONCE * RPI) {
+                    float4 x[AT_ONCE][2];
 #pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1)
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    float down;
-                    const float up = pow2_scale(top, down) * sign;
-                    uint32_t h[2], l[2];
-                    split2(x.x * up, x.y * up, h[0], l[0]);
-                    split2(x.z * up, x.w * up, h[1], l[1]);
-                    const uint32_t at = (uint32_t)((d >> 6) * C::BLOCK) + pt_off(r, (d & 63) >> 3) +
-                                        (uint32_t)((d & 4) << 1);
-                    *reinterpret_cast<uint2*>(q_ptr + at) = make_uint2(h[0], h[1]);
-                    *reinterpret_cast<uint2*>(q_ptr + C::TILE + at) = make_uint2(l[0], l[1]);
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int r = wr + i0 + k * RPI + lane / LPR;
+                        x[k][0] = x[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (r < rows && d < HD) {
+                            const float4* p = reinterpret_cast<const float4*>(
+                                q_row(A, it, G, it.row0 + 128 * t + r) + d);
+                            x[k][0] = __ldg(p), x[k][1] = __ldg(p + 1);
+                        }
+                    }
 #pragma unroll
-                    for (int k = 0; k < RPI; ++k) {
-                        const float f = __shfl_sync(0xffffffffu, down, k * LPR);
-                        if (lane == i + k) my_scale = f;
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int i = i0 + k * RPI, r = wr + i + lane / LPR;
+                        const float* y = &x[k][0].x;
+                        float top = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
+#pragma unroll
+                        for (int o = LPR / 2; o > 0; o >>= 1)
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        float down;
+                        const float up = pow2_scale(top, down) * sign;
+                        uint32_t h[4], l[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split2(y[2 * e] * up, y[2 * e + 1] * up, h[e], l[e]);
+                        uint8_t* const at = q_ptr + (d >> 6) * C::BLOCK + pt_off(r, (d & 63) >> 3);
+                        *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4*>(at + C::TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+                        const float f = __shfl_sync(0xffffffffu, down, ((lane - i) & (RPI - 1)) * LPR);
+                        if (lane >= i && lane < i + RPI) my_scale = f;
                     }
                 }
                 pt_fence_async();
@@ -297,19 +367,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 pt_fence_after();
 #pragma unroll
                 for (int d0 = 0; d0 < HDP; d0 += 32) {
-                    float o[16], o2[16];
-                    pt_ld16(o_at + d0, o);
-                    pt_ld16(o_at + d0 + 16, o2);
+                    float o[32];
+                    pt_ld32(o_at + d0, o);
                     pt_wait_ld(o);
-                    pt_wait_ld(o2);
 #pragma unroll
-                    for (int d = 0; d < 16; ++d) {
-                        acc[d0 + d] = fmaf(acc[d0 + d], c_last, o[d]);
-                        acc[d0 + 16 + d] = fmaf(acc[d0 + 16 + d], c_last, o2[d]);
+                    for (int d = 0; d < 32; d += 2) {
+                        float* a = acc + d0 + d;
+                        fma2(a[0], a[1], a[0], a[1], c_last, c_last, o[d], o[d + 1]);
                     }
                 }
-                pt_fence_before();
-                mbar_arrive(&bar.o_empty[t]);
                 if ((it.kt0 + j) * PT_KT + PT_KT - 1 > it.start + it.row0 / G) {
                     // where some row does not see all of the tile, V was made finite: rows that
                     // see such a position are not
@@ -331,60 +397,72 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     all = all && (gone.x | gone.y | gone.z | gone.w) == 0;
                 }
                 all = __all_sync(0xffffffffu, all);
-                // the next 16 scores are on their way while these are worked on
-                auto mask = [&](float (&s)[16], int i) {
-                    const uint32_t see = visible(j, i >> 1) >> (16 * (i & 1));
+                auto mask = [&](float (&s)[32], int i) {
+                    const uint32_t see = visible(j, i);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k)
+                    for (int k = 0; k < 32; ++k)
                         if (!((see >> k) & 1)) s[k] = -INFINITY;
                 };
+                // The row's maximum over two chunks of 32 at a time; the last two stay for below.
+                // (Small loops: the softmax shares the instruction cache with the MMAs' thread.)
                 float top = -INFINITY;
-                auto maximum = [&](float (&s)[16], int i) {
-                    if (!all) mask(s, i);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
-                };
-                float s0[16], s1[16];
-                pt_ld16(s_at, s0);
+                float s0[32], s1[32];
 #pragma unroll 1
-                for (int i = 0; i < 8; i += 2) {
+                for (int i = 0; i < 4; i += 2) {
+                    pt_ld32(s_at + 32 * i, s0);
+                    pt_ld32(s_at + 32 * i + 32, s1);
                     pt_wait_ld(s0);
-                    pt_ld16(s_at + 16 * i + 16, s1);
-                    maximum(s0, i);
                     pt_wait_ld(s1);
-                    pt_ld16(s_at + ((16 * i + 32) & 127), s0);  // the last: the first, for below
-                    maximum(s1, i + 1);
+                    if (!all) mask(s0, i), mask(s1, i + 1);
+                    float top1 = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        top = max3(top, s0[k], s0[k + 1]);
+                        top1 = max3(top1, s1[k], s1[k + 1]);
+                    }
+                    top = fmaxf(top, top1);
                 }
                 top = fmaxf(m, top);  // of the scores before scaling
                 const bool none = top == -INFINITY;
                 const float c = none ? 1.f : ex2((m - top) * sc);
                 const float off = none ? 0.f : 10.f - top * sc;
                 m = top;
-                float sum = 0.f;
-                auto weights = [&](float (&s)[16], int i) {
-                    if (!all) mask(s, i);
-                    uint32_t hi[8], lo[8];
+                float sum0 = 0.f, sum1 = 0.f;
+                auto weights = [&](float (&s)[32], int i) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float x = ex2(fmaf(s[2 * k], sc, off));
-                        const float y = ex2(fmaf(s[2 * k + 1], sc, off));
-                        sum += x + y;
-                        split2(x, y, hi[k], lo[k]);
+                    for (int c16 = 0; c16 < 2; ++c16) {
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            float x, y;
+                            fma2(x, y, s[16 * c16 + 2 * k], s[16 * c16 + 2 * k + 1], sc, sc, off, off);
+                            x = ex2(x), y = ex2(y);
+                            add2(sum0, sum1, x, y);
+                            const __half2 h = __floats2half2_rn(x, y);
+                            const float2 back = __half22float2(h);
+                            fma2(x, y, back.x, back.y, -1.f, -1.f, x, y);
+                            const __half2 r = __floats2half2_rn(x, y);
+                            hi[k] = *reinterpret_cast<const uint32_t*>(&h);
+                            lo[k] = *reinterpret_cast<const uint32_t*>(&r);
+                        }
+                        pt_st8(s_at + 32 * i + 16 * c16, hi);
+                        pt_st8(s_at + 32 * i + 16 * c16 + 8, lo);
                     }
-                    pt_st8(s_at + 16 * i, hi);
-                    pt_st8(s_at + 16 * i + 8, lo);
                 };
 #pragma unroll 1
-                for (int i = 0; i < 8; i += 2) {
-                    pt_wait_ld(s0);
-                    pt_ld16(s_at + 16 * i + 16, s1);
-                    weights(s0, i);
-                    pt_wait_ld(s1);
-                    if (i < 6) pt_ld16(s_at + 16 * i + 32, s0);
+                for (int i = 2; i >= 0; i -= 2) {
                     weights(s1, i + 1);
+                    if (i) pt_ld32(s_at + 32, s1);
+                    weights(s0, i);
+                    if (i) {
+                        pt_ld32(s_at, s0);
+                        pt_wait_ld(s0);
+                        pt_wait_ld(s1);
+                        if (!all) mask(s0, 0), mask(s1, 1);
+                    }
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                l = fmaf(l, c, sum);
+                l = fmaf(l, c, sum0 + sum1);
                 c_last = c;
                 pt_fence_before();
                 mbar_arrive(&bar.p_full[t]);
@@ -403,8 +481,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     make_float4(acc[4 * c4] * f, acc[4 * c4 + 1] * f, acc[4 * c4 + 2] * f,
                                 acc[4 * c4 + 3] * f);
             __syncwarp();
-            for (int i = 0; i < 32; i += RPI) {
-                const int rr = i + lane / LPR, c4 = lane % LPR, row = wr + rr;
+            constexpr int OPR = HDP / 4, OPI = 32 / OPR;  // lanes per row, rows at a time
+#pragma unroll 4
+            for (int i = 0; i < 32; i += OPI) {
+                const int rr = i + lane / OPR, c4 = lane % OPR, row = wr + rr;
                 if (row >= rows || c4 * 4 >= HD) continue;
                 const float4 x = *reinterpret_cast<const float4*>(mine + rr * RB + ((c4 ^ (rr & 7)) << 4));
                 float* p = whole ? out_row(A, it, G, it.row0 + 128 * t + row)
@@ -416,7 +496,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 A.part_ml[(int64_t)it.part * PT_R + 128 * t + r] = make_float2(m * sc, l);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
             // ---- MMAs ----
             constexpr uint32_t id_s = pt_idesc(128, 128, false), id_o = pt_idesc(128, HDP, true);
@@ -424,26 +504,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             int n_q[2] = {0, 0}, n_s[2] = {0, 0};  // q tiles and key tiles so far
             bool ok = true;
             const uint32_t leader = pt_elect();
+            // loops of a few MMAs: the code stays in the instruction cache, 64 cycles an MMA are time
             auto scores = [&](int t, uint32_t k_at) {
-                const uint64_t qa = pt_desc(base + (uint32_t)(2 * t * C::TILE), 16);
+                uint64_t qa = pt_desc(base + (uint32_t)((2 * t + 1) * C::TILE), 16);  // lo, then hi
                 const uint64_t kb = pt_desc(k_at, 16);
+                uint32_t add = 0;
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part, qa -= C::TILE >> 4)
+#pragma unroll 1
+                    for (uint32_t off = 0; off < (uint32_t)C::TILE >> 4; off += C::BLOCK >> 4)
 #pragma unroll
-                for (int part = 1; part >= 0; --part)  // lo, then hi
-#pragma unroll
-                    for (int k = 0; k < HDP / 16; ++k) {
-                        const uint32_t off = (uint32_t)((k >> 2) * (C::BLOCK >> 4) + (k & 3) * 2);
-                        pt_mma_ss(tmem + 128 * t, qa + (uint32_t)(part * (C::TILE >> 4)) + off, kb + off,
-                                  id_s, part == 0 || k > 0, leader);
-                    }
+                        for (int k = 0; k < 4; ++k, add = 1)  // 32 bytes a step
+                            pt_mma_ss(tmem + 128 * t, qa + off + 2 * k, kb + off + 2 * k, id_s, add,
+                                      leader);
             };
             auto outputs = [&](int t, uint32_t v_at) {
-                const uint64_t vb = pt_desc(v_at, C::BLOCK);
+                uint32_t add = 0;
+#pragma unroll 1
+                for (int part = 1; part >= 0; --part) {
+                    uint64_t vb = pt_desc(v_at, C::BLOCK);
+                    uint32_t pa = tmem + 128 * t + 8 * part;
+#pragma unroll 1
+                    for (int k0 = 0; k0 < PT_KT / 16; k0 += 4, vb += 4 * 128, pa += 64)
 #pragma unroll
-                for (int part = 1; part >= 0; --part)
-#pragma unroll
-                    for (int k = 0; k < PT_KT / 16; ++k)  // 16 rows, 2048 bytes, a step
-                        pt_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 16 * k + 8 * part,
-                                  vb + (uint32_t)(k * 128), id_o, part == 0 || k > 0, leader);
+                        for (int k = 0; k < 4; ++k, add = 1)  // 16 rows, 2048 bytes, a step
+                            pt_mma_ts(tmem + 256 + 128 * t, pa + 16 * k, vb + 128 * k, id_o, add, leader);
+                }
             };
             while (ok && next()) {
                 const int n_kt = it.kt1 - it.kt0, n_t = it.rows > 128 ? 2 : 1;
@@ -467,9 +553,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     const int hv = half + 2 * j + 1, hk = hv + 1;
                     for (int t = 0; t < n_t && ok; ++t) {
                         if (t == 0) arrived(hv);
-                        ok = ok && wait(&bar.p_full[t], n_s[t]);
-                        if (n_s[t] > 0) ok = ok && wait(&bar.o_empty[t], n_s[t] - 1);
-                        ++n_s[t];
+                        // p of this key tile is there, and O of the one before has been read
+                        ok = ok && wait(&bar.p_full[t], n_s[t]++);
                         pt_fence_after();
                         if (ok) {
                             outputs(t, slot_at(hv));
@@ -493,33 +578,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             pt_commit(&bar.done, leader);
             wait(&bar.done, 0);
         } else {
-            // ---- copies: 16 rows at a time, lane j (and j + 16) sees to row j ----
+            // ---- copies.  Row by row: 16 rows at a time, lane j (and j + 16) sees to row j; with
+            // TMA: lane i of warp 9 sees to box i. ----
             const int lw = warp - 9;
             constexpr int CH = HDP / 8, RL = 32 / CH;  // chunks of a row, rows at a time
             const int row_bytes = HD * 2, x = lane % CH, r0 = lane / CH;
             const bool in_row = x * 16 < row_bytes;
             const uint8_t* const src_x[2] = {(const uint8_t*)A.k + x * 16, (const uint8_t*)A.v + x * 16};
+            const int box = TA.box, box_row = (lane / C::BLOCKS) << box, box_col = lane % C::BLOCKS;
+            const bool has_box = box && box_row < PT_KT;
             int half = 0;
             uint32_t tile_no = 0;
+            int n_look = 0;
             bool ok = true;
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
                 const int first_lim = it.start + it.row0 / G;
+                auto row_of = [&](int pos) -> int {  // in the layer; -1: no page, or not seen
+                    if (pos > last_lim) return -1;
+                    const int col = (int)w.ps.div((uint32_t)pos);
+                    const int page = page_at(w, it.s.row[col]);
+                    return page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
+                };
                 for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
-                    // the tile's table entries, for K and V; -1: no page, or not seen
-                    int rows3[3];
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) {
-                        const int pos = kt * PT_KT + (lw + 3 * i) * 16 + (lane & 15);
-                        rows3[i] = -1;
-                        if (lw + 3 * i < 8 && pos <= last_lim) {
-                            const int col = (int)w.ps.div((uint32_t)pos);
-                            const int page = page_at(w, it.s.row[col]);
-                            if (page >= 0)
-                                rows3[i] = (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
-                        }
-                    }
                     const bool careful = kt * PT_KT + PT_KT - 1 > first_lim;
+                    int box_at = -1, rows3[3] = {-1, -1, -1};
+                    if (lw == 0 && has_box) box_at = row_of(kt * PT_KT + box_row);
+                    if (!box) {
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)
+                            if (lw + 3 * i < 8)
+                                rows3[i] = row_of(kt * PT_KT + (lw + 3 * i) * 16 + (lane & 15));
+                    }
 #pragma unroll 1
                     for (int kv = 0; kv < 2 && ok; ++kv, ++half) {
                         const int slot = half % PT_SLOTS, use = half / PT_SLOTS;
@@ -527,64 +617,91 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                             ok = false;
                             break;
                         }
-                        const uint32_t dst = ring + (uint32_t)(slot * C::TILE + (x >> 3) * C::BLOCK);
-                        const uint8_t* src = src_x[kv];
-                        // small loops: this code shares the instruction cache with the softmax
+                        const bool look = kv == 1 && careful;  // V to be looked through
+                        const uint32_t tile_at = ring + (uint32_t)(slot * C::TILE);
+                        if (box) {
+                            uint64_t* const there = look ? &bar.v_there : &bar.kv_full[slot];
+                            if (lw == 0) {
+                                if (lane == 0) mbar_arrive_expect_tx(there, C::TILE);
+                                __syncwarp();
+                                if (has_box) {
+                                    pt_tma(tile_at + (uint32_t)(box_col * C::BLOCK + box_row * 128),
+                                           kv ? &TA.v : &TA.k, box_col * 64, box_at < 0 ? -PT_KT : box_at,
+                                           there);
+                                    if (kv == 0 && box_col == 0)
+                                        for (int b = 0; b < 1 << (box - 3); ++b)
+                                            reinterpret_cast<uint8_t*>(sh_gone[tile_no & 3])[box_row / 8 + b] =
+                                                box_at < 0 ? 0xff : 0;
+                                }
+                            }
+                            if (look && !wait(&bar.v_there, n_look++)) {
+                                ok = false;
+                                break;
+                            }
+                        } else {
+                            const uint8_t* src = src_x[kv];
+                            // small loops: this code shares the instruction cache with the softmax
 #pragma unroll 1
-                        for (int i = 0; i < 3; ++i) {
-                            const int g16 = lw + 3 * i;
-                            if (g16 >= 8) break;
-                            const int row = i == 0 ? rows3[0] : i == 1 ? rows3[1] : rows3[2];
-                            uint32_t bad = 0;
-                            if (kv == 0 || !careful) {
+                            for (int i = 0; i < 3; ++i) {
+                                const int g16 = lw + 3 * i;
+                                if (g16 >= 8) break;
+                                const int row = i == 0 ? rows3[0] : i == 1 ? rows3[1] : rows3[2];
 #pragma unroll 4
                                 for (int k = 0; k < 16 / RL; ++k) {
                                     const int from = k * RL + r0;
                                     const int n = __shfl_sync(0xffffffffu, row, from);
                                     const bool there = n >= 0 && in_row;
-                                    cp16(dst + pt_off(g16 * 16 + from, x & 7),
+                                    cp16(tile_at + (uint32_t)((x >> 3) * C::BLOCK) +
+                                             pt_off(g16 * 16 + from, x & 7),
                                          src + (there ? (int64_t)n * row_bytes : 0), there);
                                 }
-                            } else {
+                                const uint32_t none = __ballot_sync(0xffffffffu, row < 0) & 0xffffu;
+                                if (kv == 0 && lane == 0) sh_gone[tile_no & 3][g16] = (uint16_t)none;
+                            }
+                            if (look) {
+                                asm volatile("cp.async.wait_all;" ::: "memory");
+                                __syncwarp();  // a warp looks through the rows it has copied
+                            }
+                        }
+                        if (look) {
+                            uint8_t* const tile = base_ptr + (tile_at - base);
 #pragma unroll 1
-                                for (int k = 0; k < 16 / RL; ++k) {
-                                    const int from = k * RL + r0;
-                                    const int n = __shfl_sync(0xffffffffu, row, from);
-                                    uint4 v = make_uint4(0, 0, 0, 0);
-                                    if (n >= 0 && in_row)
-                                        v = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)n * row_bytes));
+                            for (int g16 = lw; g16 < 8; g16 += 3) {
+                                uint32_t bad = 0;
+#pragma unroll 4
+                                for (int k = 0; k < 4 * C::BLOCKS; ++k) {  // four rows of a block
+                                    uint4* const at = reinterpret_cast<uint4*>(
+                                        tile + (k >> 2) * C::BLOCK + (g16 * 16 + (k & 3) * 4) * 128 + lane * 16);
+                                    uint4 v = *at;
                                     bool odd = false;
                                     v.x = finite16x2(v.x, odd), v.y = finite16x2(v.y, odd);
                                     v.z = finite16x2(v.z, odd), v.w = finite16x2(v.w, odd);
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                                     dst + pt_off(g16 * 16 + from, x & 7)),
-                                                 "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                                                 : "memory");
+                                    if (odd) *at = v;
                                     const uint32_t any = __ballot_sync(0xffffffffu, odd);
-#pragma unroll
-                                    for (int b = 0; b < RL; ++b)
-                                        if (any & (((1u << CH) - 1u) << (b * CH))) bad |= 1u << (k * RL + b);
+                                    if (any)
+                                        for (int r = 0; r < 4; ++r)
+                                            if (any & (0xffu << (8 * r))) bad |= 1u << ((k & 3) * 4 + r);
                                 }
+                                if (lane == 0) sh_bad[tile_no & 3][g16] = (uint16_t)bad;
                             }
-                            const uint32_t none = __ballot_sync(0xffffffffu, row < 0) & 0xffffu;
-                            if (lane == 0) {
-                                if (kv == 0) sh_gone[tile_no & 3][g16] = (uint16_t)none;
-                                else sh_bad[tile_no & 3][g16] = (uint16_t)bad;
-                            }
-                        }
-                        if (kv == 1 && careful) {
                             pt_fence_async();
-                            mbar_arrive(&bar.kv_full[slot]);
-                        } else {
+                        }
+                        // 33 arrivals a warp, whichever way: with TMA one of them is the bytes'
+                        if (box || look) mbar_arrive(&bar.kv_full[slot]);
+                        else
                             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
                                              smem_u32(&bar.kv_full[slot]))
                                          : "memory");
-                        }
-                        if (lane == 0) mbar_arrive(&bar.kv_full[slot]);  // sh_gone, sh_bad
+                        // after sh_gone and sh_bad
+                        __syncwarp();
+                        if (lane == 0 && !(box && !look && lw == 0)) mbar_arrive(&bar.kv_full[slot]);
                     }
                 }
             }
+            // no copy may still be landing when the CTA ends
             asm volatile("cp.async.wait_all;" ::: "memory");
+            for (int h = max(0, half - PT_SLOTS); h < half; ++h)
+                wait(&bar.kv_full[h % PT_SLOTS], h / PT_SLOTS);
         }
     }
     // every use of tensor memory is over before it is given back
@@ -597,13 +714,44 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     }
 }
 
+// The layer's rows as a tensor of FP16 [rows][head_dim], in boxes of 64 columns.
+static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head_dim, int box_rows) {
+    static PFN_cuTensorMapEncodeTiled encode = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) ==
+                cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            encode = (PFN_cuTensorMapEncodeTiled)fn;
+    });
+    if (!encode) {
+        set_error("ib_attention_paged: cuTensorMapEncodeTiled is not available");
+        return IB_ERR_CUDA;
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+                              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("ib_attention_paged: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+        return IB_ERR_CUDA;
+    }
+    return IB_OK;
+}
+
 CutRule tensor_rule(int min_rows, int max_rows) {
     // one CTA to an SM (148 of a B200), a piece for each
     return CutRule{PT_R, PT_KT, min_rows, max_rows, 148, 128};
 }
 
 template <int HDP>
-static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
+static int launch(const TensorArgs& a, int64_t grid, cudaStream_t st) {
     auto kern = attn_tensor_kernel<HDP>;
     IB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)TensorCfg<HDP>::SMEM));
@@ -615,7 +763,21 @@ static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st) {
     const int64_t most = tiles * (max_pos / a.rule.least + 1 + a.rule.R);
     const int64_t grid = std::min<int64_t>(a.rule.n_pieces, most);
-    return a.w.HD <= 64 ? launch<64>(a, grid, st) : launch<128>(a, grid, st);
+    TensorArgs t{};
+    t.rows = a;
+    const PagedView& w = a.w;
+    // the largest power of two that divides the page, up to the tile; fewer than 8 rows would not
+    // fill a swizzled group
+    int box = 0;
+    while (box < 7 && w.page_size % (2 << box) == 0) ++box;
+    if (box >= 3) {
+        const int64_t rows = (int64_t)w.n_pages * w.Hkv * w.page_size;
+        int r = tensor_map(&t.k, a.k, rows, w.HD, 1 << box);
+        if (r == IB_OK) r = tensor_map(&t.v, a.v, rows, w.HD, 1 << box);
+        if (r != IB_OK) return r;
+        t.box = box;
+    }
+    return w.HD <= 64 ? launch<64>(t, grid, st) : launch<128>(t, grid, st);
 }
 
 }  // namespace ib
