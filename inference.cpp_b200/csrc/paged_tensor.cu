@@ -207,7 +207,7 @@ struct TensorArgs {
 
 struct TensorBars {
     uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS];
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], v_there, done;
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], v_there, done;
 };
 
 template <int HDP>
@@ -243,7 +243,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.q_full[i], 128);
-            mbar_init(&bar.q_empty[i], 128);
             mbar_init(&bar.s_full[i], 1);
             mbar_init(&bar.p_full[i], 128);
             mbar_init(&bar.o_full[i], 1);
@@ -287,76 +286,83 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         uint8_t* const q_ptr = base_ptr + 2 * t * C::TILE;
         const uint32_t s_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(128 * t);
         const uint32_t o_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(256 + 128 * t);
-        int tiles = 0, segs = 0;  // key tiles so far, of all segments; segments so far
+        int tiles = 0;      // key tiles so far, of all segments
         uint32_t seen = 0;  // and counted as the copies do (both query tiles)
         bool ok = true;
-        while (ok && next()) {
-            const int n_kt = it.kt1 - it.kt0;
-            const int rows = it.rows - 128 * t;  // of this query tile
-            const uint32_t first = seen;
-            seen += (uint32_t)n_kt;
-            if (rows <= 0) continue;
-            // q: this warp's 32 rows, HDP / 8 lanes to a row
-            constexpr int LPR = HDP / 8, RPI = 32 / LPR;  // lanes per row, rows at a time
-            float my_scale = 0.f;
-            const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
-            // every warp of the tile has stored the last segment's rows from here
-            if (segs > 0) ok = wait(&bar.q_empty[t], segs - 1);
-            ++segs;
-            if (!ok) break;
-            if (n_kt > 0) {
-                const int d = (lane % LPR) * 8;
-                constexpr int AT_ONCE = 4;  // loads on their way
+        const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
+        // The segment's q into this warp's 32 rows of the tile, HDP / 8 lanes to a row; returns the
+        // factor of row `lane`.  The last segment's scores are done (this warp has read some), so
+        // nothing reads the rows any more.
+        auto stage_q = [&](const Segment& sg) -> float {
+            constexpr int LPR = HDP / 8, RPI = 32 / LPR, AT_ONCE = 4;  // loads on their way
+            const int rows = sg.rows - 128 * t, d = (lane % LPR) * 8;
+            float mine = 0.f;
+            if (rows <= 0 || sg.kt0 == sg.kt1) return mine;
 #pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += AT_ONCE * RPI) {
-                    float4 x[AT_ONCE][2];
+            for (int i0 = 0; i0 < 32; i0 += AT_ONCE * RPI) {
+                float4 x[AT_ONCE][2];
 #pragma unroll
-                    for (int k = 0; k < AT_ONCE; ++k) {
-                        const int r = wr + i0 + k * RPI + lane / LPR;
-                        x[k][0] = x[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (r < rows && d < HD) {
-                            const float4* p = reinterpret_cast<const float4*>(
-                                q_row(A, it, G, it.row0 + 128 * t + r) + d);
-                            x[k][0] = __ldg(p), x[k][1] = __ldg(p + 1);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < AT_ONCE; ++k) {
-                        const int i = i0 + k * RPI, r = wr + i + lane / LPR;
-                        const float* y = &x[k][0].x;
-                        float top = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
-#pragma unroll
-                        for (int o = LPR / 2; o > 0; o >>= 1)
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        float down;
-                        const float up = pow2_scale(top, down) * sign;
-                        uint32_t h[4], l[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) split2(y[2 * e] * up, y[2 * e + 1] * up, h[e], l[e]);
-                        uint8_t* const at = q_ptr + (d >> 6) * C::BLOCK + pt_off(r, (d & 63) >> 3);
-                        *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4*>(at + C::TILE) = make_uint4(l[0], l[1], l[2], l[3]);
-                        const float f = __shfl_sync(0xffffffffu, down, ((lane - i) & (RPI - 1)) * LPR);
-                        if (lane >= i && lane < i + RPI) my_scale = f;
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    const int r = wr + i0 + k * RPI + lane / LPR;
+                    x[k][0] = x[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r < rows && d < HD) {
+                        const float4* p = reinterpret_cast<const float4*>(
+                            q_row(A, sg, G, sg.row0 + 128 * t + r) + d);
+                        x[k][0] = __ldg(p), x[k][1] = __ldg(p + 1);
                     }
                 }
-                pt_fence_async();
-                mbar_arrive(&bar.q_full[t]);
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    const int i = i0 + k * RPI, r = wr + i + lane / LPR;
+                    const float* y = &x[k][0].x;
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    float down;
+                    const float up = pow2_scale(top, down) * sign;
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split2(y[2 * e] * up, y[2 * e + 1] * up, h[e], l[e]);
+                    uint8_t* const at = q_ptr + (d >> 6) * C::BLOCK + pt_off(r, (d & 63) >> 3);
+                    *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(at + C::TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+                    const float f = __shfl_sync(0xffffffffu, down, ((lane - i) & (RPI - 1)) * LPR);
+                    if (lane >= i && lane < i + RPI) mine = f;
+                }
             }
+            pt_fence_async();
+            mbar_arrive(&bar.q_full[t]);
+            return mine;
+        };
+        bool more = next();
+        float next_scale = more ? stage_q(it) : 0.f;
+        while (ok && more) {
+            const Segment cur = it;
+            const int n_kt = cur.kt1 - cur.kt0;
+            const int rows = cur.rows - 128 * t;  // of this query tile
+            const uint32_t first = seen;
+            seen += (uint32_t)n_kt;
             // scores are multiplied by this; kept off zero, where -inf would turn into NaN
-            const float sc = fmaxf(fabsf(A.scale_log2) * my_scale, 1e-37f);
+            const float sc = fmaxf(fabsf(A.scale_log2) * next_scale, 1e-37f);
+            if (rows <= 0 || n_kt == 0) {
+                more = next();
+                if (more) next_scale = stage_q(it);
+                if (rows <= 0) continue;
+            }
             const int r = wr + lane;
-            const int lim = r < rows ? it.start + (it.row0 + 128 * t + r) / G : -1;
-            const int first_lim = it.start + (it.row0 + 128 * t) / G;  // of the tile's first row
+            const int row = cur.row0 + 128 * t + r;  // of the sequence
+            const int lim = r < rows ? cur.start + (int)w.group.div((uint32_t)row) : -1;
+            const int first_lim = cur.start + (cur.row0 + 128 * t) / G;  // of the tile's first row
             float acc[HDP];
 #pragma unroll
             for (int d = 0; d < HDP; ++d) acc[d] = 0.f;
             float m = -INFINITY, l = 0.f, c_last = 1.f;
             // positions of key tile j (of the segment) that this row sees and that have a page
             auto visible = [&](int j, int word) -> uint32_t {
-                const int n = lim + 1 - ((it.kt0 + j) * PT_KT + 32 * word);
+                const int n = lim + 1 - ((cur.kt0 + j) * PT_KT + 32 * word);
                 const uint32_t below = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
                 const uint16_t* gone = sh_gone[(first + j) & 3];
                 return below & ~((uint32_t)gone[2 * word] | ((uint32_t)gone[2 * word + 1] << 16));
@@ -376,7 +382,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                         fma2(a[0], a[1], a[0], a[1], c_last, c_last, o[d], o[d + 1]);
                     }
                 }
-                if ((it.kt0 + j) * PT_KT + PT_KT - 1 > it.start + it.row0 / G) {
+                if ((cur.kt0 + j) * PT_KT + PT_KT - 1 > cur.start + cur.row0 / G) {
                     // where some row does not see all of the tile, V was made finite: rows that
                     // see such a position are not
                     const uint16_t* bad = sh_bad[(first + j) & 3];
@@ -391,7 +397,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 ok = wait(&bar.s_full[t], tiles) && ok;
                 ++tiles;
                 pt_fence_after();
-                bool all = (it.kt0 + j) * PT_KT + PT_KT - 1 <= first_lim && r < rows;
+                bool all = (cur.kt0 + j) * PT_KT + PT_KT - 1 <= first_lim && r < rows;
                 {
                     const uint4 gone = *reinterpret_cast<const uint4*>(sh_gone[(first + j) & 3]);
                     all = all && (gone.x | gone.y | gone.z | gone.w) == 0;
@@ -467,33 +473,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 pt_fence_before();
                 mbar_arrive(&bar.p_full[t]);
             }
-            if (n_kt > 0 && ok) add_o(n_kt - 1);
-
-            // ---- the segment's rows, through this warp's quarter of the q tile (every MMA on
-            // it is done), so that they go out row by row ----
-            const bool whole = it.part < 0;
-            const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            constexpr int RB = HDP * 4;  // bytes of a row
-            uint8_t* const mine = q_ptr + (warp & 3) * 32 * RB;
-#pragma unroll
-            for (int c4 = 0; c4 < HDP / 4; ++c4)
-                *reinterpret_cast<float4*>(mine + lane * RB + ((c4 ^ (lane & 7)) << 4)) =
-                    make_float4(acc[4 * c4] * f, acc[4 * c4 + 1] * f, acc[4 * c4 + 2] * f,
-                                acc[4 * c4 + 3] * f);
-            __syncwarp();
-            constexpr int OPR = HDP / 4, OPI = 32 / OPR;  // lanes per row, rows at a time
-#pragma unroll 4
-            for (int i = 0; i < 32; i += OPI) {
-                const int rr = i + lane / OPR, c4 = lane % OPR, row = wr + rr;
-                if (row >= rows || c4 * 4 >= HD) continue;
-                const float4 x = *reinterpret_cast<const float4*>(mine + rr * RB + ((c4 ^ (rr & 7)) << 4));
-                float* p = whole ? out_row(A, it, G, it.row0 + 128 * t + row)
-                                 : A.part_acc + ((int64_t)it.part * PT_R + 128 * t + row) * HD;
-                *reinterpret_cast<float4*>(p + 4 * c4) = x;
+            // the next segment's q goes in while the last O is computed; its first scores follow
+            if (n_kt > 0 && ok) {
+                more = next();
+                if (more) next_scale = stage_q(it);
+                add_o(n_kt - 1);
             }
-            mbar_arrive(&bar.q_empty[t]);
-            if (!whole && r < rows)
-                A.part_ml[(int64_t)it.part * PT_R + 128 * t + r] = make_float2(m * sc, l);
+            if (r < rows && ok) {  // a row per thread
+                const bool whole = cur.part < 0;
+                const int64_t at = (int64_t)cur.part * PT_R + 128 * t + r;
+                const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                float* p = whole ? out_row(A, cur, G, row) : A.part_acc + at * HD;
+#pragma unroll
+                for (int d = 0; d < HDP; d += 4)
+                    if (d < HD)
+                        *reinterpret_cast<float4*>(p + d) =
+                            make_float4(acc[d] * f, acc[d + 1] * f, acc[d + 2] * f, acc[d + 3] * f);
+                if (!whole) A.part_ml[at] = make_float2(m * sc, l);
+            }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -594,6 +591,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
                 const int first_lim = it.start + it.row0 / G;
+                if (lw == 1) {  // the softmax warps ask for the segment's q soon
+                    const int bytes = HD * 4;
+                    for (int r = lane; r < it.rows; r += 32) {
+                        const uint8_t* p = (const uint8_t*)q_row(A, it, G, it.row0 + r);
+                        for (int b = 0; b < bytes; b += 128)
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
+                    }
+                }
                 auto row_of = [&](int pos) -> int {  // in the layer; -1: no page, or not seen
                     if (pos > last_lim) return -1;
                     const int col = (int)w.ps.div((uint32_t)pos);
