@@ -338,18 +338,17 @@ struct WarpRows {
 // the end.  A ring slot is one half of a tile, K or V.  (Warps with pieces of their own, their
 // copies running on from tile to tile, took 135 us against 119 us for 64 single tokens over
 // 200..4096 positions: warps far apart in the code miss the instruction cache.)
-// RB: blocks of eight rows.
-template <typename KV, int HDP, int RB>
+template <typename KV, int HDP>
 struct NarrowCfg {
     static constexpr bool F32 = sizeof(KV) == 4;
-    static constexpr int R = 8 * RB, KW = 16;
+    static constexpr int R = 8, KW = 16;
     static constexpr int LD = HDP * (int)sizeof(KV) + 16, QLD = HDP * 4 + 16;
     static constexpr int HALF = KW * LD;
     // 64 single tokens at head_dim 128 in FP16: 117 us with three CTAs of four warps to an SM,
     // 126 us with two, 130 us with four of three half tiles a warp
     static constexpr int ROWB = HDP * (int)sizeof(KV);
     static constexpr int D = ROWB <= 256 ? 4 : ROWB <= 512 ? 3 : 2;  // ring slots of a warp
-    static constexpr int CTAS = ROWB <= 256 && RB == 1 ? 3 : ROWB <= 512 ? 2 : 1;  // to an SM
+    static constexpr int CTAS = ROWB <= 256 ? 3 : ROWB <= 512 ? 2 : 1;  // to an SM
     static constexpr int NW = 4, NT = NW * 32;
     static constexpr bool QREG = HDP * (F32 ? 2 : 1) <= 256;  // q fragments stay in registers
     static constexpr int Q_BYTES = QREG ? 0 : 2 * R * QLD;  // or lie in shared memory (FP32)
@@ -359,10 +358,10 @@ struct NarrowCfg {
     static_assert(QREG || F32, "");
 };
 
-template <typename KV, int HDP, int RB>
-__global__ void __launch_bounds__(NarrowCfg<KV, HDP, RB>::NT, NarrowCfg<KV, HDP, RB>::CTAS)
+template <typename KV, int HDP>
+__global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CTAS)
     attn_narrow_kernel(const __grid_constant__ RowsArgs A) {
-    using C = NarrowCfg<KV, HDP, RB>;
+    using C = NarrowCfg<KV, HDP>;
     constexpr bool F32 = C::F32;
     constexpr int R = C::R, KW = C::KW, LD = C::LD, QLD = C::QLD, D = C::D, NW = C::NW;
     constexpr int KS = F32 ? HDP / 8 : HDP / 16, DB = HDP / 16;
@@ -445,250 +444,229 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP, RB>::NT, NarrowCfg<KV, HDP,
     int slot = 0;
     const uint32_t k_frag = (uint32_t)((lane & 15) * LD + (lane >> 4) * 16);
     const uint32_t v_frag = (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * LD + ((lane >> 3) & 1) * 16);
-        // this lane's rows are 2 t4 and 2 t4 + 1 of each block
-        int lim[RB][2];
-        float sc[RB][2], m[RB][2], l[RB][2], acc[DB][RB][4];
-        uint32_t qh[C::QREG ? KS : 1][RB][2], ql[C::QREG ? KS : 1][RB][2];
-        // q as B: row g of a block; FP16 k-steps of dimensions 2 t4, + 1, + 8, + 9, TF32 t4, + 4
+    // this lane's rows are 2 t4 and 2 t4 + 1
+    int lim[2];
+    float sc[2], m[2], l[2], acc[DB][4];
+    uint32_t qh[C::QREG ? KS : 1][2], ql[C::QREG ? KS : 1][2];
+    // q as B: row g; FP16 k-steps of dimensions 2 t4, + 1, + 8, + 9, TF32 t4, + 4
+    const float* src = g < it.rows ? q_row(A, it, G, it.row0 + g) : nullptr;
+    float f = A.scale_log2;
+    if constexpr (F32) {
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            const int r = 8 * b + g;
-            const float* src = r < it.rows ? q_row(A, it, G, it.row0 + r) : nullptr;
-            float f = A.scale_log2;
-            if constexpr (F32) {
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int d = k * 8 + t4 + 4 * j;
-                        const float x = src && d < HD ? __ldg(src + d) : 0.f;
-                        uint32_t hi, lo;
-                        split_tf32(x, hi, lo);
-                        if constexpr (C::QREG) {
-                            qh[k][b][j] = hi, ql[k][b][j] = lo;
-                        } else {
-                            *reinterpret_cast<uint32_t*>(q_smem + r * QLD + d * 4) = hi;
-                            *reinterpret_cast<uint32_t*>(q_smem + (R + r) * QLD + d * 4) = lo;
-                        }
-                    }
-                if constexpr (!C::QREG) __syncwarp();
-            } else {
-                float2 x[KS][2];
-                float top = 0.f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int d = k * 16 + 2 * t4 + 8 * j;
-                        x[k][j] = src && d < HD ? __ldg(reinterpret_cast<const float2*>(src + d))
-                                                : make_float2(0.f, 0.f);
-                        top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                float down;
-                const float up = pow2_scale(top, down);
-                f *= down;
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        split2(x[k][j].x * up, x[k][j].y * up, qh[k][b][j], ql[k][b][j]);
-            }
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int mine = 8 * b + 2 * t4 + j;
-                lim[b][j] = mine < it.rows ? it.start + (it.row0 + mine) / G : -1;
-                sc[b][j] = __shfl_sync(0xffffffffu, f, (2 * t4 + j) * 4);
-                m[b][j] = -INFINITY;
-                l[b][j] = 0.f;
+            const int d = k * 8 + t4 + 4 * j;
+            const float x = src && d < HD ? __ldg(src + d) : 0.f;
+            uint32_t hi, lo;
+            split_tf32(x, hi, lo);
+            if constexpr (C::QREG) {
+                qh[k][j] = hi, ql[k][j] = lo;
+            } else {
+                *reinterpret_cast<uint32_t*>(q_smem + g * QLD + d * 4) = hi;
+                *reinterpret_cast<uint32_t*>(q_smem + (R + g) * QLD + d * 4) = lo;
             }
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[d][b][j] = 0.f;
         }
-        for (int kt = kt0; kt < kt1; kt += NW) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
-            __syncwarp();  // every lane's copies of K, and its reads of the half before
-            if constexpr (D & 1) copy_k((D - 1) / 2);
-            else copy_v();
-            const uint32_t kd = ring_a + (uint32_t)(slot * C::HALF) + k_frag;
-            slot = slot == D - 1 ? 0 : slot + 1;
-            // scores: rows of a fragment are positions g and g + 8, columns the lane's two rows.
-            // sa, sb: two chains; e: the lo parts.
-            float s[RB][4];
-            {
-                float sa[RB][4], sb[RB][4], e[RB][4];
+        if constexpr (!C::QREG) __syncwarp();
+    } else {
+        float2 x[KS][2];
+        float top = 0.f;
 #pragma unroll
-                for (int b = 0; b < RB; ++b)
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sa[b][j] = sb[b][j] = e[b][j] = 0.f;
+            for (int j = 0; j < 2; ++j) {
+            const int d = k * 16 + 2 * t4 + 8 * j;
+            x[k][j] = src && d < HD ? __ldg(reinterpret_cast<const float2*>(src + d))
+                                    : make_float2(0.f, 0.f);
+            top = fmaxf(top, fmaxf(fabsf(x[k][j].x), fabsf(x[k][j].y)));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        float down;
+        const float up = pow2_scale(top, down);
+        f *= down;
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    uint32_t a[4];
-                    ldsm_x4(kd + k * 32, a[0], a[1], a[2], a[3]);
-                    uint32_t ah[4], al[4];
-                    if constexpr (F32) {
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
-                    }
+            for (int j = 0; j < 2; ++j)
+                split2(x[k][j].x * up, x[k][j].y * up, qh[k][j], ql[k][j]);
+    }
 #pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        uint32_t q0, q1, r0, r1;
-                        if constexpr (C::QREG) {
-                            q0 = qh[k][b][0], q1 = qh[k][b][1], r0 = ql[k][b][0], r1 = ql[k][b][1];
-                        } else {
-                            const uint8_t* p = q_smem + (8 * b + g) * QLD + (k * 8 + t4) * 4;
-                            q0 = *reinterpret_cast<const uint32_t*>(p);
-                            q1 = *reinterpret_cast<const uint32_t*>(p + 16);
-                            r0 = *reinterpret_cast<const uint32_t*>(p + R * QLD);
-                            r1 = *reinterpret_cast<const uint32_t*>(p + R * QLD + 16);
-                        }
-                        float(&x)[4] = k & 1 ? sb[b] : sa[b];
-                        if constexpr (F32) {
-                            mma_tf32(x, ah, q0, q1, x);
-                            mma_tf32(e[b], ah, r0, r1, e[b]);
-                            mma_tf32(e[b], al, q0, q1, e[b]);
-                        } else {
-                            mma_f16(x, a, q0, q1, x);
-                            mma_f16(e[b], a, r0, r1, e[b]);
-                        }
-                    }
+    for (int j = 0; j < 2; ++j) {
+        const int mine = 2 * t4 + j;
+        lim[j] = mine < it.rows ? it.start + (it.row0 + mine) / G : -1;
+        sc[j] = __shfl_sync(0xffffffffu, f, (2 * t4 + j) * 4);
+        m[j] = -INFINITY;
+        l[j] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[d][j] = 0.f;
+    for (int kt = kt0; kt < kt1; kt += NW) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+        __syncwarp();  // every lane's copies of K, and its reads of the half before
+        if constexpr (D & 1) copy_k((D - 1) / 2);
+        else copy_v();
+        const uint32_t kd = ring_a + (uint32_t)(slot * C::HALF) + k_frag;
+        slot = slot == D - 1 ? 0 : slot + 1;
+        // scores: rows of a fragment are positions g and g + 8, columns the lane's two rows.
+        // sa, sb: two chains; e: the lo parts.
+        float s[4];
+        {
+            float sa[4], sb[4], e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sa[j] = sb[j] = e[j] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t a[4];
+                ldsm_x4(kd + k * 32, a[0], a[1], a[2], a[3]);
+                uint32_t ah[4], al[4];
+                if constexpr (F32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
                 }
-#pragma unroll
-                for (int b = 0; b < RB; ++b)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[b][j] = (sa[b][j] + sb[b][j]) + e[b][j];
+                uint32_t q0, q1, r0, r1;
+                if constexpr (C::QREG) {
+                    q0 = qh[k][0], q1 = qh[k][1], r0 = ql[k][0], r1 = ql[k][1];
+                } else {
+                    const uint8_t* p = q_smem + g * QLD + (k * 8 + t4) * 4;
+                    q0 = *reinterpret_cast<const uint32_t*>(p);
+                    q1 = *reinterpret_cast<const uint32_t*>(p + 16);
+                    r0 = *reinterpret_cast<const uint32_t*>(p + R * QLD);
+                    r1 = *reinterpret_cast<const uint32_t*>(p + R * QLD + 16);
+                }
+                float(&x)[4] = k & 1 ? sb : sa;
+                if constexpr (F32) {
+                    mma_tf32(x, ah, q0, q1, x);
+                    mma_tf32(e, ah, r0, r1, e);
+                    mma_tf32(e, al, q0, q1, e);
+                } else {
+                    mma_f16(x, a, q0, q1, x);
+                    mma_f16(e, a, r0, r1, e);
+                }
             }
-            // what the rows do not see, the running maximum, p
-            const uint32_t missing = gone[0];
-            const int p0 = (missing >> g) & 1 ? 0x7fffffff : kt * KW + g;
-            const int p1 = (missing >> (g + 8)) & 1 ? 0x7fffffff : kt * KW + g + 8;
-            float c[RB][2];
 #pragma unroll
-            for (int b = 0; b < RB; ++b)
+            for (int j = 0; j < 4; ++j) s[j] = (sa[j] + sb[j]) + e[j];
+        }
+        // what the rows do not see, the running maximum, p
+        const uint32_t missing = gone[0];
+        const int p0 = (missing >> g) & 1 ? 0x7fffffff : kt * KW + g;
+        const int p1 = (missing >> (g + 8)) & 1 ? 0x7fffffff : kt * KW + g + 8;
+        float c[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float &x = s[j], &y = s[2 + j];
+            x = p0 <= lim[j] ? x * sc[j] : -INFINITY;
+            y = p1 <= lim[j] ? y * sc[j] : -INFINITY;
+            float top = fmaxf(x, y);
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, m[j]);
+            c[j] = top == -INFINITY ? 1.f : ex2(m[j] - top);
+            m[j] = top;
+            const float base = top == -INFINITY ? 0.f : top - P_BIAS;
+            x = ex2(x - base), y = ex2(y - base);
+            l[j] = fmaf(l[j], c[j], x + y);
+        }
+        // p as B: positions along k, the row along n
+        uint32_t ph[F32 ? 4 : 2], pl[F32 ? 4 : 2];
+        if constexpr (F32) {
+            // the MMA's k index t holds position 2 t, t + 4 position 2 t + 1, as V below
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float &x = s[b][j], &y = s[b][2 + j];
-                    x = p0 <= lim[b][j] ? x * sc[b][j] : -INFINITY;
-                    y = p1 <= lim[b][j] ? y * sc[b][j] : -INFINITY;
-                    float top = fmaxf(x, y);
+                const int from = 8 * t4 + 4 * j + (g >> 1);
+                const float x = __shfl_sync(0xffffffffu, s[2 * i], from);
+                const float y = __shfl_sync(0xffffffffu, s[2 * i + 1], from);
+                split_tf32(g & 1 ? y : x, ph[2 * i + j], pl[2 * i + j]);
+            }
+        } else {
 #pragma unroll
-                    for (int o = 4; o <= 16; o <<= 1)
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    top = fmaxf(top, m[b][j]);
-                    c[b][j] = top == -INFINITY ? 1.f : ex2(m[b][j] - top);
-                    m[b][j] = top;
-                    const float base = top == -INFINITY ? 0.f : top - P_BIAS;
-                    x = ex2(x - base), y = ex2(y - base);
-                    l[b][j] = fmaf(l[b][j], c[b][j], x + y);
-                }
-            // p as B: positions along k, the row along n
-            uint32_t ph[RB][F32 ? 4 : 2], pl[RB][F32 ? 4 : 2];
+            for (int i = 0; i < 2; ++i) {
+                split2(s[2 * i], s[2 * i + 1], ph[i], pl[i]);
+                ph[i] = movm(ph[i]), pl[i] = movm(pl[i]);
+            }
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+        __syncwarp();
+        gone[0] = gone[1], gone[1] = gone[2];
+        if constexpr (D & 1) copy_v();
+        else copy_k((D - 1) / 2);
+        const uint32_t vd = ring_a + (uint32_t)(slot * C::HALF);
+        const uint8_t* v_ptr = ring + slot * C::HALF;
+        slot = slot == D - 1 ? 0 : slot + 1;
+        const bool careful = kt * KW + KW - 1 > first_lim;
+        bool odd = false;  // a V value that is not finite, among this lane's
+        // outputs: rows of a fragment are dimensions g and g + 8 of a block of 16
+        auto products = [&](auto check) {
+            constexpr bool CHECK = decltype(check)::value;
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
+            for (int d = 0; d < DB; ++d) {
+                uint32_t a[F32 ? 2 : 1][4];
+                [[maybe_unused]] uint32_t al[2][4];
                 if constexpr (F32) {
-                    // the MMA's k index t holds position 2 t, t + 4 position 2 t + 1, as V below
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int from = 8 * t4 + 4 * j + (g >> 1);
-                            const float x = __shfl_sync(0xffffffffu, s[b][2 * i], from);
-                            const float y = __shfl_sync(0xffffffffu, s[b][2 * i + 1], from);
-                            split_tf32(g & 1 ? y : x, ph[b][2 * i + j], pl[b][2 * i + j]);
-                        }
+                        for (int j = 0; j < 4; ++j) {  // position 2 t4 + (j >> 1), dimension g + 8 (j & 1)
+                        float y = *reinterpret_cast<const float*>(
+                            v_ptr + (i * 8 + 2 * t4 + (j >> 1)) * LD +
+                            (d * 16 + g + 8 * (j & 1)) * 4);
+                        if (CHECK && !(fabsf(y) < INFINITY)) odd = true, y = 0.f;
+                        split_tf32(y, a[i][j], al[i][j]);
+                    }
                 } else {
+                    ldsm_x4_t(vd + v_frag + d * 32, a[0][0], a[0][1], a[0][2], a[0][3]);
+                    if (CHECK) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        split2(s[b][2 * i], s[b][2 * i + 1], ph[b][i], pl[b][i]);
-                        ph[b][i] = movm(ph[b][i]), pl[b][i] = movm(pl[b][i]);
+                        for (int j = 0; j < 4; ++j) a[0][j] = finite16x2(a[0][j], odd);
                     }
                 }
+                const float none[4] = {0.f, 0.f, 0.f, 0.f};
+                float t[4];
+                if constexpr (F32) {
+                    float r[4];
+                    mma_tf32(t, a[0], ph[0], ph[1], none);
+                    mma_tf32(t, a[1], ph[2], ph[3], t);
+                    mma_tf32(r, a[0], pl[0], pl[1], none);
+                    mma_tf32(r, al[0], ph[0], ph[1], r);
+                    mma_tf32(r, a[1], pl[2], pl[3], r);
+                    mma_tf32(r, al[1], ph[2], ph[3], r);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t[j] += r[j];
+                } else {
+                    mma_f16(t, a[0], pl[0], pl[1], none);
+                    mma_f16(t, a[0], ph[0], ph[1], t);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[d][j] = fmaf(acc[d][j], c[j & 1], t[j]);
             }
-            asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
-            __syncwarp();
-            gone[0] = gone[1], gone[1] = gone[2];
-            if constexpr (D & 1) copy_v();
-            else copy_k((D - 1) / 2);
-            const uint32_t vd = ring_a + (uint32_t)(slot * C::HALF);
-            const uint8_t* v_ptr = ring + slot * C::HALF;
-            slot = slot == D - 1 ? 0 : slot + 1;
-            const bool careful = kt * KW + KW - 1 > first_lim;
-            bool odd = false;  // a V value that is not finite, among this lane's
-            // outputs: rows of a fragment are dimensions g and g + 8 of a block of 16
-            auto products = [&](auto check) {
-                constexpr bool CHECK = decltype(check)::value;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    uint32_t a[F32 ? 2 : 1][4];
-                    [[maybe_unused]] uint32_t al[2][4];
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {  // position 2 t4 + (j >> 1), dimension g + 8 (j & 1)
-                                float y = *reinterpret_cast<const float*>(
-                                    v_ptr + (i * 8 + 2 * t4 + (j >> 1)) * LD +
-                                    (d * 16 + g + 8 * (j & 1)) * 4);
-                                if (CHECK && !(fabsf(y) < INFINITY)) odd = true, y = 0.f;
-                                split_tf32(y, a[i][j], al[i][j]);
-                            }
-                    } else {
-                        ldsm_x4_t(vd + v_frag + d * 32, a[0][0], a[0][1], a[0][2], a[0][3]);
-                        if (CHECK) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) a[0][j] = finite16x2(a[0][j], odd);
-                        }
-                    }
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        const float none[4] = {0.f, 0.f, 0.f, 0.f};
-                        float t[4];
-                        if constexpr (F32) {
-                            float r[4];
-                            mma_tf32(t, a[0], ph[b][0], ph[b][1], none);
-                            mma_tf32(t, a[1], ph[b][2], ph[b][3], t);
-                            mma_tf32(r, a[0], pl[b][0], pl[b][1], none);
-                            mma_tf32(r, al[0], ph[b][0], ph[b][1], r);
-                            mma_tf32(r, a[1], pl[b][2], pl[b][3], r);
-                            mma_tf32(r, al[1], ph[b][2], ph[b][3], r);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) t[j] += r[j];
-                        } else {
-                            mma_f16(t, a[0], pl[b][0], pl[b][1], none);
-                            mma_f16(t, a[0], ph[b][0], ph[b][1], t);
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            acc[d][b][j] = fmaf(acc[d][b][j], c[b][j & 1], t[j]);
-                    }
-                }
-            };
-            if (careful) products(std::true_type{});
-            else products(std::false_type{});
-            if (careful && __any_sync(0xffffffffu, odd)) {
-                // rows that see such a value are not finite there
+        };
+        if (careful) products(std::true_type{});
+        else products(std::false_type{});
+        if (careful && __any_sync(0xffffffffu, odd)) {
+            // rows that see such a value are not finite there
 #pragma unroll 1
-                for (int i = 0; i < KW; ++i) {
-                    if ((missing >> i) & 1) continue;
+            for (int i = 0; i < KW; ++i) {
+                if ((missing >> i) & 1) continue;
 #pragma unroll
-                    for (int d = 0; d < DB; ++d)
+                for (int d = 0; d < DB; ++d)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int at = i * LD / (int)sizeof(KV) + d * 16 + g + 8 * (j >> 1);
-                            float y;
-                            if constexpr (F32) y = reinterpret_cast<const float*>(v_ptr)[at];
-                            else y = __half2float(reinterpret_cast<const __half*>(v_ptr)[at]);
-                            if (fabsf(y) < INFINITY) continue;
-#pragma unroll
-                            for (int b = 0; b < RB; ++b)
-                                if (kt * KW + i <= lim[b][j & 1]) acc[d][b][j] = NAN;
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                    const int at = i * LD / (int)sizeof(KV) + d * 16 + g + 8 * (j >> 1);
+                    float y;
+                    if constexpr (F32) y = reinterpret_cast<const float*>(v_ptr)[at];
+                    else y = __half2float(reinterpret_cast<const __half*>(v_ptr)[at]);
+                    if (fabsf(y) < INFINITY) continue;
+                    if (kt * KW + i <= lim[j & 1]) acc[d][j] = NAN;
                 }
             }
         }
+    }
 
     // ---- the warps' results together, in the rings ----
     constexpr int MLD = HDP + 4;
@@ -696,22 +674,19 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP, RB>::NT, NarrowCfg<KV, HDP,
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int j = 0; j < 4; ++j)
+            ma[(warp * R + 2 * t4 + (j & 1)) * MLD + d * 16 + g + 8 * (j >> 1)] =
+                acc[d][j];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                ma[(warp * R + 8 * b + 2 * t4 + (j & 1)) * MLD + d * 16 + g + 8 * (j >> 1)] =
-                    acc[d][b][j];
+    for (int j = 0; j < 2; ++j) {  // a row's sum is spread over eight lanes
+        float x = l[j];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {  // a row's sum is spread over eight lanes
-            float x = l[b][j];
-#pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            if (g == 0) {
-                sh_m[warp][8 * b + 2 * t4 + j] = m[b][j];
-                sh_l[warp][8 * b + 2 * t4 + j] = x;
-            }
+        for (int o = 4; o <= 16; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (g == 0) {
+            sh_m[warp][2 * t4 + j] = m[j];
+            sh_l[warp][2 * t4 + j] = x;
         }
     }
     __syncthreads();
@@ -996,9 +971,9 @@ struct Plan {
 
 // Parts for two rounds of the CTAs that the GPU holds at once, or one piece for each of them,
 // of at least 128 positions: below that joining costs more.
-template <typename KV, int HDP, int RB>
+template <typename KV, int HDP>
 static CutRule narrow_rule(int min_rows, int max_rows) {
-    using C = NarrowCfg<KV, HDP, RB>;
+    using C = NarrowCfg<KV, HDP>;
     return CutRule{C::R, C::KW, min_rows, max_rows, kSMs * C::CTAS * 2, 128};
 }
 template <typename KV, int HDP>
@@ -1022,10 +997,12 @@ static int rows_launch(Kern kern, int threads, size_t smem, bool pieces, const R
 template <typename KV, int HDP>
 constexpr bool on_tensor = sizeof(KV) == 2 && HDP <= 128;
 
-// The kernels of a call, by the rows (new tokens x group) that a sequence may have.  Where the
-// caller's bound allows no more than 16, one narrow kernel takes everything; otherwise the
-// narrow one takes the sequences with up to 8 rows (16 where a single token has more) and the
-// wide one the rest, or everything where there is one sequence or a token has over 16.
+// The kernels of a call, by the rows (new tokens x group) that a sequence may have: up to
+// NARROW_ROWS in tiles of eight on the narrow kernel, more on the wide one, by the caller's bound
+// one of them alone.  32 sequences over 200..4096 positions (32 heads on 8, FP16), narrow against
+// wide: with 4 tokens, 16 rows, 105 us against 150; with 8 tokens 174 against 214.
+constexpr int NARROW_ROWS = 32;
+
 template <typename KV, int HDP>
 static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     constexpr int ALL = 0x7fffffff;
@@ -1049,16 +1026,11 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
         s.ml_off = take((size_t)2 * r.n_pieces * r.R * sizeof(float2));
     };
     const int64_t rows = b->n_tokens * G;
-    constexpr bool TWO = HDP * sizeof(KV) <= 256;  // 16 rows fit a warp's registers
-    if (most_q * G <= 8) {
-        add(narrow_rule<KV, HDP, 1>(1, ALL), seqs + rows / 8);
-    } else if (TWO && most_q * G <= 16) {
-        if constexpr (TWO) add(narrow_rule<KV, HDP, 2>(1, ALL), seqs + rows / 16);
+    if (most_q * G <= NARROW_ROWS) {
+        add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
     } else {
-        const int narrow = b->n_seqs == 1 ? 0 : G <= 8 ? 8 : TWO && G <= 16 ? 16 : 0;
-        if (narrow == 8) add(narrow_rule<KV, HDP, 1>(1, 8), seqs);
-        if constexpr (TWO)
-            if (narrow == 16) add(narrow_rule<KV, HDP, 2>(1, 16), seqs);
+        const int narrow = b->n_seqs == 1 || G > NARROW_ROWS ? 0 : NARROW_ROWS;
+        if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
         CutRule r;
         if constexpr (TENSOR) r = tensor_rule(narrow + 1, ALL);
         else r = wide_rule<KV, HDP>(narrow + 1, ALL);
@@ -1070,22 +1042,16 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
 template <typename KV, int HDP>
 static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan, RowsArgs a,
                     uint8_t* ws, int64_t max_pos, cudaStream_t st) {
-    constexpr int RB2 = HDP * sizeof(KV) <= 256 ? 2 : 1;
-    using N1 = NarrowCfg<KV, HDP, 1>;
-    using N2 = NarrowCfg<KV, HDP, RB2>;
+    using N = NarrowCfg<KV, HDP>;
     for (int i = 0; i < plan.n; ++i) {
         const Share& s = plan.share[i];
         a.rule = s.rule;
-        const bool wide = s.rule.R > 16;
+        const bool wide = s.rule.R > 8;
         a.part_acc = reinterpret_cast<float*>(ws + s.acc_off);
         a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
         int r;
         if (s.rule.R == 8) {
-            r = rows_launch(attn_narrow_kernel<KV, HDP, 1>, N1::NT, N1::SMEM, false, a, s.tiles,
-                            max_pos, st);
-        } else if (s.rule.R == 16) {
-            r = rows_launch(attn_narrow_kernel<KV, HDP, RB2>, N2::NT, N2::SMEM, false, a, s.tiles,
-                            max_pos, st);
+            r = rows_launch(attn_narrow_kernel<KV, HDP>, N::NT, N::SMEM, false, a, s.tiles, max_pos, st);
         } else if constexpr (on_tensor<KV, HDP>) {
             r = attn_tensor_launch(a, s.tiles, max_pos, st);
         } else {
