@@ -15,6 +15,7 @@ The directory name is not a Python identifier; load it with
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -487,6 +488,31 @@ def argmax(x, n, out, stream=None):
 # paged KV cache (ib_kv_*, ib_attention_paged)
 # ---------------------------------------------------------------------------
 
+@functools.cache
+def _torch():
+    import torch
+    return torch
+
+
+@functools.cache
+def _raw_stream():
+    """Device index -> handle of its current stream, without building a Stream object where torch
+    offers that (a tenth of a microsecond instead of two, on calls of ten)."""
+    fast = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
+    return fast or (lambda index: _torch().cuda.current_stream(index).cuda_stream)
+
+
+@functools.cache
+def _entry(name):
+    return getattr(lib(), name)
+
+
+def _call(name, *args):  # call(), without looking the function up again
+    status = _entry(name)(*args)
+    if status != IB_OK:
+        check(status, name)
+
+
 class _CKVPages(ctypes.Structure):
     _fields_ = [("type", ctypes.c_int32), ("n_layers", ctypes.c_int32),
                 ("n_pages", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
@@ -556,6 +582,7 @@ class KVSeqs:
         self.n_slots, self.max_pages = table.shape
         self.len = _paged_tensor(len, "len", torch.int32, (self.n_slots,), self.device)
         self.refs = _paged_tensor(refs, "refs", torch.int32, (-1,), self.device)
+        self.n_refs = refs.numel()
         self._c = _CKVSeqs(self.n_slots, self.max_pages, table.data_ptr(), len.data_ptr(),
                            refs.data_ptr())
         self._p = ctypes.addressof(self._c)
@@ -587,62 +614,67 @@ class KVBatch:
 
 def _paged_stream(pages, stream, *others):
     """The stream to launch on, after checking that everything is on the current device."""
-    import torch
     dev = pages.device
     for o in others:
         if o.device != dev:
             raise ValueError(f"arguments on {dev} and {o.device}")
-    if torch.cuda.current_device() != dev.index:
+    cuda, index = _torch().cuda, dev.index
+    if cuda.current_device() != index:
         raise ValueError(f"the pages are on {dev}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
-    # with the index given the stream is looked up in 1 us instead of 6
-    return torch.cuda.current_stream(dev.index).cuda_stream or None if stream is None else stream
+                         f"cuda:{cuda.current_device()}")
+    return (_raw_stream()(index) or None) if stream is None else stream
 
 
 def _seqs_of(pages, seqs):
-    if seqs.refs.numel() != pages.n_pages:
-        raise ValueError(f"refs: {seqs.refs.numel()} entries for {pages.n_pages} pages")
+    if seqs.n_refs != pages.n_pages:
+        raise ValueError(f"refs: {seqs.n_refs} entries for {pages.n_pages} pages")
     return seqs._p
 
 
-def _paged_lists(pages, *named):
-    import torch
-    n = named[0][1].numel()
-    for name, t in named:
-        _paged_tensor(t, name, torch.int32, (n,), pages.device)
-    return n
+def _paged_list(pages, t, name, n):
+    """Pointer of a contiguous int32 list of n entries on the pages' device."""
+    if t.dtype != _torch().int32:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected torch.int32")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected ({n},)")
+    if t.device != pages.device or not t.is_contiguous():
+        raise ValueError(f"{name}: on {t.device}, contiguous {t.is_contiguous()}; expected "
+                         f"contiguous on {pages.device}")
+    return t.data_ptr()
 
 
 def kv_extend(pages, seqs, slots, n_new, status=None, stream=None):
     """Room for n_new[i] more tokens of each slot; returns status (1 done, 0 no room,
     -1 refused), int32 tensors on the pages' device."""
-    import torch
     if status is None:
-        status = torch.empty_like(slots)
-    n = _paged_lists(pages, ("slots", slots), ("n_new", n_new), ("status", status))
+        status = _torch().empty_like(slots)
+    n = slots.numel()
+    a, b, c = (_paged_list(pages, slots, "slots", n), _paged_list(pages, n_new, "n_new", n),
+               _paged_list(pages, status, "status", n))
     st = _paged_stream(pages, stream, seqs)
-    call("ib_kv_extend", pages._p, _seqs_of(pages, seqs), n, slots.data_ptr(), n_new.data_ptr(),
-         status.data_ptr(), st)
+    _call("ib_kv_extend", pages._p, _seqs_of(pages, seqs), n, a, b, c, st)
     return status
 
 
 def kv_fork(pages, seqs, parents, children, status=None, stream=None):
     """children[i] becomes a copy of parents[i], sharing its whole pages; returns status."""
-    import torch
     if status is None:
-        status = torch.empty_like(parents)
-    n = _paged_lists(pages, ("parents", parents), ("children", children), ("status", status))
+        status = _torch().empty_like(parents)
+    n = parents.numel()
+    a, b, c = (_paged_list(pages, parents, "parents", n),
+               _paged_list(pages, children, "children", n),
+               _paged_list(pages, status, "status", n))
     st = _paged_stream(pages, stream, seqs)
-    call("ib_kv_fork", pages._p, _seqs_of(pages, seqs), n, parents.data_ptr(),
-         children.data_ptr(), status.data_ptr(), st)
+    _call("ib_kv_fork", pages._p, _seqs_of(pages, seqs), n, a, b, c, st)
     return status
 
 
 def kv_release(pages, seqs, slots, stream=None):
     """The slots give up their pages."""
-    n = _paged_lists(pages, ("slots", slots))
+    n = slots.numel()
+    a = _paged_list(pages, slots, "slots", n)
     st = _paged_stream(pages, stream, seqs)
-    call("ib_kv_release", pages._p, _seqs_of(pages, seqs), n, slots.data_ptr(), st)
+    _call("ib_kv_release", pages._p, _seqs_of(pages, seqs), n, a, st)
 
 
 class KVCompactPlan:
@@ -672,45 +704,46 @@ def kv_compact(pages, seqs, out=None, plan=None, stream=None):
     if out.table.shape != seqs.table.shape or plan.n_pages != pages.n_pages:
         raise ValueError("out or plan of another cache")
     _seqs_of(pages, out)
-    call("ib_kv_compact", pages._p, _seqs_of(pages, seqs), out.table.data_ptr(),
+    _call("ib_kv_compact", pages._p, _seqs_of(pages, seqs), out.table.data_ptr(),
          out.refs.data_ptr(), plan.map.data_ptr(), plan.moves.data_ptr(), plan.info.data_ptr(),
          st)
     return plan
 
 
 def _paged_rows(t, name, tokens, heads, head_dim, device):
-    """(pointer, row stride) of a float32 [tokens, heads, head_dim] tensor whose rows may be
-    apart (slices of a projection's output)."""
-    import torch
-    shape, strides = t.shape, t.stride()
-    if t.dtype != torch.float32 or t.device != device:
+    """(pointer, row stride, heads) of a float32 [tokens, heads, head_dim] tensor whose rows may
+    be apart (slices of a projection's output); heads None: any number."""
+    shape = t.shape
+    if t.dtype != _torch().float32 or t.device != device:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, expected float32 on {device}")
-    if len(shape) != 3 or shape[0] != tokens or (heads and shape[1] != heads) \
-            or shape[2] != head_dim:
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != head_dim \
+            or (heads is not None and shape[1] != heads):
         raise ValueError(f"{name}: shape {tuple(shape)}, expected "
                          f"({tokens}, {heads or 'heads'}, {head_dim})")
-    if strides[2] != 1 or (strides[1] != head_dim and shape[1] != 1):
+    row, head, one = t.stride()
+    heads = shape[1]
+    if one != 1 or (head != head_dim and heads != 1):
         raise ValueError(f"{name}: the heads of a token are not contiguous")
-    return t.data_ptr(), strides[0] if tokens > 1 else shape[1] * head_dim
+    return t.data_ptr(), row if tokens > 1 else heads * head_dim, heads
 
 
 def kv_append(pages, seqs, batch, layer, q, k, v, rope_table, q_out=None, stream=None):
     """RoPE on q and k and the write of k and v into the layer's pages.  q [tokens, heads,
     head_dim], k and v [tokens, kv heads, head_dim] float32 (rows may be slices);
     rope_table [positions, head_dim / 2, 2].  Returns q_out."""
-    import torch
-    T, HD, dev = batch.n_tokens, pages.head_dim, pages.device
+    torch = _torch()
+    T, HD, Hkv, dev = batch.n_tokens, pages.head_dim, pages.n_kv_heads, pages.device
     if q_out is None:
         q_out = torch.empty(q.shape, dtype=torch.float32, device=dev)
-    qp, qs = _paged_rows(q, "q", T, 0, HD, dev)
-    H = q.shape[1]
-    kp, ks = _paged_rows(k, "k", T, pages.n_kv_heads, HD, dev)
-    vp, vs = _paged_rows(v, "v", T, pages.n_kv_heads, HD, dev)
-    op, os_ = _paged_rows(q_out, "q_out", T, H, HD, dev)
-    _paged_tensor(rope_table, "rope_table", torch.float32, (-1, HD // 2, 2), dev)
+    qp, qs, H = _paged_rows(q, "q", T, None, HD, dev)
+    kp, ks, _ = _paged_rows(k, "k", T, Hkv, HD, dev)
+    vp, vs, _ = _paged_rows(v, "v", T, Hkv, HD, dev)
+    op, os_, _ = _paged_rows(q_out, "q_out", T, H, HD, dev)
+    n = rope_table.shape[0]
+    _paged_tensor(rope_table, "rope_table", torch.float32, (n, HD // 2, 2), dev)
     st = _paged_stream(pages, stream, seqs, batch)
-    call("ib_kv_append", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, kp, ks, vp,
-         vs, op, os_, rope_table.data_ptr(), rope_table.shape[0], st)
+    _call("ib_kv_append", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, kp, ks, vp,
+          vs, op, os_, rope_table.data_ptr(), n, st)
     return q_out
 
 
@@ -727,13 +760,12 @@ def attention_paged(pages, seqs, batch, layer, q, scale, out=None, workspace=Non
     """Causal attention of the batch's new tokens over the layer's pages.  q, out [tokens,
     heads, head_dim] float32 (rows may be slices).  workspace: attention_paged_workspace(),
     allocated for the call when None.  Returns out (rows of nobody: as they were)."""
-    import torch
+    torch = _torch()
     T, HD, dev = batch.n_tokens, pages.head_dim, pages.device
-    qp, qs = _paged_rows(q, "q", T, 0, HD, dev)
-    H = q.shape[1]
+    qp, qs, H = _paged_rows(q, "q", T, None, HD, dev)
     if out is None:
         out = torch.zeros(q.shape, dtype=torch.float32, device=dev)
-    op, os_ = _paged_rows(out, "out", T, H, HD, dev)
+    op, os_, _ = _paged_rows(out, "out", T, H, HD, dev)
     st = _paged_stream(pages, stream, seqs, batch)
     if workspace is None:
         # of the launch stream's memory pool: it may be handed out again, in stream order,
@@ -741,10 +773,10 @@ def attention_paged(pages, seqs, batch, layer, q, scale, out=None, workspace=Non
         with torch.cuda.stream(torch.cuda.ExternalStream(st, dev) if st else
                                torch.cuda.default_stream(dev)):
             workspace = attention_paged_workspace(pages, seqs, batch, H)
-    elif workspace.device != dev:
-        raise ValueError(f"workspace on {workspace.device}, expected {dev}")
-    call("ib_attention_paged", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, op,
-         os_, scale, workspace.data_ptr(), workspace.numel() * workspace.element_size(), st)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace: on {workspace.device}, expected contiguous on {dev}")
+    _call("ib_attention_paged", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, op,
+          os_, scale, workspace.data_ptr(), workspace.nbytes, st)
     return out
 
 

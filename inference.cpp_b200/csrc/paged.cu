@@ -587,10 +587,11 @@ template <bool FORK>
 static int assign_launch(const KvSeqsDev& s, int n, const int32_t* a, const int32_t* b,
                          int32_t* status, cudaStream_t st) {
     const size_t sm = assign_smem(s.n_slots, n);
-    if (sm > 48 * 1024)
-        IB_CUDA_CHECK(cudaFuncSetAttribute(kv_assign_kernel<FORK>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           KV_ASSIGN_SMEM_MAX));
+    static DeviceOnce once;
+    IB_CUDA_CHECK(once.run([] {
+        return cudaFuncSetAttribute(kv_assign_kernel<FORK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    KV_ASSIGN_SMEM_MAX);
+    }));
     kv_assign_kernel<FORK><<<1, KV_PLAN_THREADS, sm, st>>>(s, n, a, b, status);
     IB_LAUNCH_CHECK("kv_assign_kernel");
     return IB_OK;

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ib {
@@ -91,6 +93,22 @@ __device__ __forceinline__ int page_at(const PagedView& w, int e) {
     if (e != -1) paged_fault(PAGED_BAD_PAGE);
     return -1;
 }
+
+// Runs a set-up once per device; a failure is returned and tried again by the next call.
+struct DeviceOnce {
+    std::atomic<uint64_t> done{0};  // a bit per device
+    template <typename F>
+    cudaError_t run(F f) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        e = f();
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
 
 // Reads and clears this translation unit's fault word.
 static inline int paged_fault_take_here(int* code) {

@@ -982,14 +982,18 @@ static CutRule wide_rule(int min_rows, int max_rows) {
     return CutRule{C::R, C::KT, min_rows, max_rows, kSMs, 128};
 }
 
-template <typename Kern>
-static int rows_launch(Kern kern, int threads, size_t smem, bool pieces, const RowsArgs& a,
+// KERN: the kernel
+template <auto KERN>
+static int rows_launch(int threads, size_t smem, bool pieces, const RowsArgs& a,
                        int64_t tiles, int64_t max_pos, cudaStream_t st) {
-    IB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static DeviceOnce once;  // of each kernel
+    IB_CUDA_CHECK(once.run([&] {
+        return cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    }));
     // pieces: no more than `least` allows; parts: at most one more per tile
     const int64_t most = tiles * (max_pos / a.rule.least + 1 + a.rule.R);
     const int64_t grid = std::min<int64_t>(a.rule.n_pieces + (pieces ? 0 : tiles), most);
-    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(threads), smem, st, true, a));
+    IB_CUDA_CHECK(launch_pdl(KERN, dim3((unsigned)grid), dim3(threads), smem, st, true, a));
     return IB_OK;
 }
 
@@ -1051,15 +1055,16 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
         int r;
         if (s.rule.R == 8) {
-            r = rows_launch(attn_narrow_kernel<KV, HDP>, N::NT, N::SMEM, false, a, s.tiles, max_pos, st);
+            r = rows_launch<attn_narrow_kernel<KV, HDP>>(N::NT, N::SMEM, false, a, s.tiles, max_pos, st);
         } else if constexpr (on_tensor<KV, HDP>) {
             r = attn_tensor_launch(a, s.tiles, max_pos, st);
         } else {
             using W = WideCfg<KV, HDP>;
-            r = rows_launch(attn_wide_kernel<KV, HDP>, W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
+            r = rows_launch<attn_wide_kernel<KV, HDP>>(W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
         }
         if (r != IB_OK) return r;
-        {
+        // no tile is cut into parts where the tables' rows are no longer than the least part
+        if (wide || max_pos > s.rule.least) {
             const JoinArgs j{a.w, s.rule, a.out, a.out_stride, a.part_acc, a.part_ml};
             const int64_t G = a.w.H / a.w.Hkv;
             const int64_t most_rows = std::min<int64_t>(s.rule.R, b->n_tokens * G);

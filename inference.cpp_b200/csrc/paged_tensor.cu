@@ -758,8 +758,11 @@ CutRule tensor_rule(int min_rows, int max_rows) {
 template <int HDP>
 static int launch(const TensorArgs& a, int64_t grid, cudaStream_t st) {
     auto kern = attn_tensor_kernel<HDP>;
-    IB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)TensorCfg<HDP>::SMEM));
+    static DeviceOnce once;
+    IB_CUDA_CHECK(once.run([&] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)TensorCfg<HDP>::SMEM);
+    }));
     IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(PT_THREADS), TensorCfg<HDP>::SMEM, st,
                              true, a));
     return IB_OK;
