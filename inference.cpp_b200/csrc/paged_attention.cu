@@ -966,6 +966,7 @@ struct Share {
 struct Plan {
     int n = 0;
     Share share[2];
+    bool tensor = false;  // the wide tiles run on tcgen05
     size_t bytes = 0;
 };
 
@@ -997,20 +998,19 @@ static int rows_launch(int threads, size_t smem, bool pieces, const RowsArgs& a,
     return IB_OK;
 }
 
-// FP16 pages with head_dim up to 128 have their wide tiles on tcgen05, the others on mma.sync.
-template <typename KV, int HDP>
-constexpr bool on_tensor = sizeof(KV) == 2 && HDP <= 128;
-
 // The kernels of a call, by the rows (new tokens x group) that a sequence may have: up to
 // NARROW_ROWS in tiles of eight on the narrow kernel, more on the wide one, by the caller's bound
 // one of them alone.  32 sequences over 200..4096 positions (32 heads on 8, FP16), narrow against
 // wide: with 4 tokens, 16 rows, 105 us against 150; with 8 tokens 174 against 214.
 constexpr int NARROW_ROWS = 32;
 
+// FP16 pages with head_dim up to 128 have all wide tiles on tcgen05.
+template <typename KV, int HDP>
+constexpr bool has_wide = sizeof(KV) == 4 || HDP > 128;
+
 template <typename KV, int HDP>
 static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     constexpr int ALL = 0x7fffffff;
-    constexpr bool TENSOR = on_tensor<KV, HDP>;
     const int64_t G = n_heads / p->n_kv_heads;
     const int64_t most_q = b->max_q > 0 ? std::min(b->max_q, b->n_tokens) : b->n_tokens;
     const int64_t seqs = std::min(b->n_seqs, b->n_tokens);
@@ -1035,10 +1035,12 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     } else {
         const int narrow = b->n_seqs == 1 || G > NARROW_ROWS ? 0 : NARROW_ROWS;
         if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
-        CutRule r;
-        if constexpr (TENSOR) r = tensor_rule(narrow + 1, ALL);
-        else r = wide_rule<KV, HDP>(narrow + 1, ALL);
+        const bool tensor = tensor_takes<KV>(p->head_dim, p->page_size);
+        CutRule r = tensor_rule<KV>(p->head_dim, narrow + 1, ALL);
+        if constexpr (has_wide<KV, HDP>)
+            if (!tensor) r = wide_rule<KV, HDP>(narrow + 1, ALL);
         add(r, seqs + rows / r.R);
+        plan.tensor = tensor;
     }
     return plan;
 }
@@ -1053,12 +1055,12 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         const bool wide = s.rule.R > 8;
         a.part_acc = reinterpret_cast<float*>(ws + s.acc_off);
         a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
-        int r;
-        if (s.rule.R == 8) {
+        int r = IB_OK;
+        if (!wide) {
             r = rows_launch<attn_narrow_kernel<KV, HDP>>(N::NT, N::SMEM, false, a, s.tiles, max_pos, st);
-        } else if constexpr (on_tensor<KV, HDP>) {
-            r = attn_tensor_launch(a, s.tiles, max_pos, st);
-        } else {
+        } else if (plan.tensor) {
+            r = attn_tensor_launch<KV>(a, s.tiles, max_pos, st);
+        } else if constexpr (has_wide<KV, HDP>) {
             using W = WideCfg<KV, HDP>;
             r = rows_launch<attn_wide_kernel<KV, HDP>>(W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
         }

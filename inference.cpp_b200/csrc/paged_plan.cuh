@@ -361,8 +361,12 @@ __device__ __forceinline__ float pow2_scale(float top, float& inverse) {
     return plain ? 1.f : __uint_as_float((uint32_t)(8 - e + 127) << 23);
 }
 
-// FP16 pages with head_dim up to 128 on tcgen05 (paged_tensor.cu).
-CutRule tensor_rule(int min_rows, int max_rows);
+// Tiles of many rows on tcgen05, where head_dim and page size allow (paged_tensor.cu).
+template <typename KV>
+bool tensor_takes(int head_dim, int page_size);
+template <typename KV>
+CutRule tensor_rule(int head_dim, int min_rows, int max_rows);
+template <typename KV>
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st);
 int paged_tensor_fault_take(int* code);
 

@@ -45,15 +45,27 @@ namespace ib {
 
 int paged_tensor_fault_take(int* code) { return paged_fault_take_here(code); }
 
-constexpr int PT_R = 256, PT_KT = 128, PT_SLOTS = 3, PT_THREADS = 384;
-constexpr int PT_LOADERS = 96;
+constexpr int PT_THREADS = 384, PT_LOADERS = 96;
 
-template <int HDP>
+template <typename KV, int HDP>
 struct TensorCfg {
-    static constexpr int BLOCKS = HDP / 64;           // of 64 columns
-    static constexpr int BLOCK = 128 * 128;           // bytes: 128 rows of 64 elements
-    static constexpr int TILE = BLOCKS * BLOCK;       // a K or V tile, or a part of a q tile
-    static constexpr size_t SMEM = 4 * TILE + PT_SLOTS * TILE + 1024;
+    static constexpr bool F32 = sizeof(KV) == 4;
+    static constexpr int QT = F32 && HDP == 128 ? 1 : 2;  // query tiles of 128 rows
+    static constexpr int R = 128 * QT;
+    static constexpr int KT = !F32 ? 128 : HDP == 64 ? 64 : 32;  // positions of a key tile
+    static constexpr int EB = F32 ? 4 : 2;                       // bytes of an operand element
+    static constexpr int ROW = 128 / EB;                         // elements of a swizzled row
+    static constexpr int Q_PLANE = 128 * HDP * EB;               // hi or lo of a query tile
+    static constexpr int PLANE = KT * HDP * EB;                  // a K or V tile, or its hi or lo
+    static constexpr int TILE = F32 ? 2 * PLANE : PLANE;         // a ring slot
+    static constexpr int SLOTS = F32 ? 2 : 3;
+    static constexpr int RAW = F32 ? 2 * PLANE : 0;              // FP32 K and V as they come
+    static constexpr int Q_BLOCK = 128 * 128;                    // ROW columns of a query tile
+    static constexpr int K_BLOCK = KT * 128;                     // and of a K tile
+    // V: FP16 as it lies (K_BLOCK: 64 dimensions of all positions), FP32 turned round (32
+    // positions of all dimensions)
+    static constexpr int V_BLOCK = F32 ? HDP * 128 : K_BLOCK;
+    static constexpr size_t SMEM = QT * 2 * Q_PLANE + SLOTS * TILE + RAW + 1024;
 };
 
 // ---- tcgen05 ---------------------------------------------------------------------------
@@ -68,41 +80,61 @@ __device__ __forceinline__ void pt_fence_async() {
 }
 
 // 128-byte swizzle (layout type 2), 8-row groups 1024 bytes apart, sm_100 descriptor (version
-// 1).  K-major: 64 columns to a row.  MN-major: the 64 columns are the MN dimension, the next
-// 64 lie TILE rows on (the leading offset), the groups of eight rows run along K.
+// 1).  K-major: a row's 128 bytes lie along K.  MN-major (FP16): they lie along the MN dimension,
+// its next 64 elements `lead` bytes on, and the groups of eight rows run along K.
 __device__ __forceinline__ uint64_t pt_desc(uint32_t saddr, uint32_t lead) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) |
            ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// kind::f16: D FP32, A and B FP16; b_mn: B is MN-major.
-constexpr uint32_t pt_idesc(int M, int N, bool b_mn) {
-    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+// D FP32, A and B FP16 (kind::f16) or TF32 (kind::tf32); b_mn: B is MN-major.
+constexpr uint32_t pt_idesc(int M, int N, bool b_mn, bool tf32 = false) {
+    return (1u << 4) | (tf32 ? 2u << 7 | 2u << 10 : 0u) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
 
 // The whole warp comes here with the same operands and `leader` lets one thread issue: the
 // operands then are uniform registers, as the instruction takes them.  Issued inside a branch of
 // one thread, every operand is moved there first, and an MMA took 134 cycles instead of 64.
+template <bool TF32>
 __device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                           uint32_t add, uint32_t leader) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
-        : "memory");
+    if constexpr (TF32)
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "setp.ne.b32 q, %5, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "setp.ne.b32 q, %5, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+            : "memory");
 }
+template <bool TF32>
 __device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                           uint32_t add, uint32_t leader) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
-        : "memory");
+    if constexpr (TF32)
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "setp.ne.b32 q, %5, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "setp.ne.b32 q, %5, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+            : "memory");
 }
 
 __device__ __forceinline__ void pt_commit(uint64_t* bar, uint32_t leader) {
@@ -151,6 +183,14 @@ __device__ __forceinline__ void pt_wait_ld(float (&v)[32]) {
                    "+f"(v[30]), "+f"(v[31])
                  :
                  : "memory");
+}
+__device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
 }
 __device__ __forceinline__ void pt_st8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile(
@@ -202,26 +242,30 @@ __device__ __forceinline__ void pt_tma(uint32_t dst, const CUtensorMap* map, int
 struct TensorArgs {
     RowsArgs rows;
     CUtensorMap k, v;  // the layer's rows [page, kv head, position in page][head_dim]
-    int box;           // log2 of a box's rows, 0: no TMA
+    int box;           // log2 of a box's rows, 0: no TMA (FP16 only)
 };
 
 struct TensorBars {
-    uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS];
+    uint64_t kv_full[3], kv_empty[3], raw_full[2], raw_empty[2];
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], v_there, done;
 };
 
-template <int HDP>
+template <typename KV, int HDP>
 __global__ void __launch_bounds__(PT_THREADS, 1)
     attn_tensor_kernel(const __grid_constant__ TensorArgs TA) {
     const RowsArgs& A = TA.rows;
-    using C = TensorCfg<HDP>;
+    using C = TensorCfg<KV, HDP>;
+    constexpr bool F32 = C::F32;
+    constexpr int KT = C::KT;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) TensorBars bar;
     __shared__ uint32_t tmem_base;
     __shared__ Piece sh_piece[PT_THREADS / 32];  // the same one for each warp, out of its registers
     __shared__ int found;
     // of the last four key tiles: positions without a page; positions whose V is not finite
-    __shared__ __align__(16) uint16_t sh_gone[4][8], sh_bad[4][8];
+    __shared__ __align__(16) uint16_t sh_gone[4][8];
+    __shared__ __align__(16) uint16_t sh_bad[4][8];
+    __shared__ uint32_t sh_bad32[4][3][2];  // the same for FP32, of each of the three warps
     const PagedView& w = A.w;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
@@ -237,11 +281,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.k)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.v)) : "memory");
         }
-        for (int i = 0; i < PT_SLOTS; ++i) {
+        for (int i = 0; i < C::SLOTS; ++i) {
             mbar_init(&bar.kv_full[i], PT_LOADERS + PT_LOADERS / 32);
             mbar_init(&bar.kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.raw_full[i], 1);
+            mbar_init(&bar.raw_empty[i], PT_LOADERS / 32);
             mbar_init(&bar.q_full[i], 128);
             mbar_init(&bar.s_full[i], 1);
             mbar_init(&bar.p_full[i], 128);
@@ -262,7 +308,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     __syncthreads();
     pt_fence_after();
     const uint32_t tmem = tmem_base;
-    const uint32_t ring = base + 4 * C::TILE;
+    const uint32_t ring = base + C::QT * 2 * C::Q_PLANE;
     const int G = w.H / w.Hkv, HD = w.HD;
     Segment it;
     auto next = [&]() -> bool {
@@ -283,7 +329,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         // ---- softmax of query tile t: thread = row ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int t = warp >> 2, wr = (warp & 3) * 32;  // this warp's rows of the tile, its lanes
-        uint8_t* const q_ptr = base_ptr + 2 * t * C::TILE;
+        uint8_t* const q_ptr = base_ptr + 2 * t * C::Q_PLANE;
         const uint32_t s_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(128 * t);
         const uint32_t o_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(256 + 128 * t);
         int tiles = 0;      // key tiles so far, of all segments
@@ -315,22 +361,37 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 for (int k = 0; k < AT_ONCE; ++k) {
                     const int i = i0 + k * RPI, r = wr + i + lane / LPR;
                     const float* y = &x[k][0].x;
-                    float top = 0.f;
+                    if constexpr (F32) {
+                        uint32_t h[8], l[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
+                        for (int e = 0; e < 8; ++e) split_tf32(y[e] * sign, h[e], l[e]);
 #pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1)
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    float down;
-                    const float up = pow2_scale(top, down) * sign;
-                    uint32_t h[4], l[4];
+                        for (int e = 0; e < 8; e += 4) {
+                            uint8_t* const at =
+                                q_ptr + (d >> 5) * C::Q_BLOCK + pt_off(r, ((d & 31) + e) >> 2);
+                            *reinterpret_cast<uint4*>(at) = make_uint4(h[e], h[e + 1], h[e + 2], h[e + 3]);
+                            *reinterpret_cast<uint4*>(at + C::Q_PLANE) =
+                                make_uint4(l[e], l[e + 1], l[e + 2], l[e + 3]);
+                        }
+                        mine = 1.f;
+                    } else {
+                        float top = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) split2(y[2 * e] * up, y[2 * e + 1] * up, h[e], l[e]);
-                    uint8_t* const at = q_ptr + (d >> 6) * C::BLOCK + pt_off(r, (d & 63) >> 3);
-                    *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(at + C::TILE) = make_uint4(l[0], l[1], l[2], l[3]);
-                    const float f = __shfl_sync(0xffffffffu, down, ((lane - i) & (RPI - 1)) * LPR);
-                    if (lane >= i && lane < i + RPI) mine = f;
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
+#pragma unroll
+                        for (int o = LPR / 2; o > 0; o >>= 1)
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        float down;
+                        const float up = pow2_scale(top, down) * sign;
+                        uint32_t h[4], l[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split2(y[2 * e] * up, y[2 * e + 1] * up, h[e], l[e]);
+                        uint8_t* const at = q_ptr + (d >> 6) * C::Q_BLOCK + pt_off(r, (d & 63) >> 3);
+                        *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4*>(at + C::Q_PLANE) = make_uint4(l[0], l[1], l[2], l[3]);
+                        const float f = __shfl_sync(0xffffffffu, down, ((lane - i) & (RPI - 1)) * LPR);
+                        if (lane >= i && lane < i + RPI) mine = f;
+                    }
                 }
             }
             pt_fence_async();
@@ -362,7 +423,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             float m = -INFINITY, l = 0.f, c_last = 1.f;
             // positions of key tile j (of the segment) that this row sees and that have a page
             auto visible = [&](int j, int word) -> uint32_t {
-                const int n = lim + 1 - ((cur.kt0 + j) * PT_KT + 32 * word);
+                const int n = lim + 1 - ((cur.kt0 + j) * KT + 32 * word);
                 const uint32_t below = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
                 const uint16_t* gone = sh_gone[(first + j) & 3];
                 return below & ~((uint32_t)gone[2 * word] | ((uint32_t)gone[2 * word + 1] << 16));
@@ -382,14 +443,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                         fma2(a[0], a[1], a[0], a[1], c_last, c_last, o[d], o[d + 1]);
                     }
                 }
-                if ((cur.kt0 + j) * PT_KT + PT_KT - 1 > cur.start + cur.row0 / G) {
+                if ((cur.kt0 + j) * KT + KT - 1 > cur.start + cur.row0 / G) {
                     // where some row does not see all of the tile, V was made finite: rows that
                     // see such a position are not
-                    const uint16_t* bad = sh_bad[(first + j) & 3];
+                    const uint16_t* bad16 = sh_bad[(first + j) & 3];
+                    const auto& bad32 = sh_bad32[(first + j) & 3];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (visible(j, i) & ((uint32_t)bad[2 * i] | ((uint32_t)bad[2 * i + 1] << 16)))
-                            l = NAN;
+                    for (int i = 0; i < KT / 32; ++i) {
+                        uint32_t bad;
+                        if constexpr (F32) bad = bad32[0][i] | bad32[1][i] | bad32[2][i];
+                        else bad = (uint32_t)bad16[2 * i] | ((uint32_t)bad16[2 * i + 1] << 16);
+                        if (visible(j, i) & bad) l = NAN;
+                    }
                 }
             };
             for (int j = 0; j < n_kt && ok; ++j) {
@@ -397,10 +462,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 ok = wait(&bar.s_full[t], tiles) && ok;
                 ++tiles;
                 pt_fence_after();
-                bool all = (cur.kt0 + j) * PT_KT + PT_KT - 1 <= first_lim && r < rows;
+                bool all = (cur.kt0 + j) * KT + KT - 1 <= first_lim && r < rows;
                 {
                     const uint4 gone = *reinterpret_cast<const uint4*>(sh_gone[(first + j) & 3]);
-                    all = all && (gone.x | gone.y | gone.z | gone.w) == 0;
+                    all = all && (gone.x | (KT > 32 ? gone.y : 0) | (KT > 64 ? gone.z | gone.w : 0)) == 0;
                 }
                 all = __all_sync(0xffffffffu, all);
                 auto mask = [&](float (&s)[32], int i) {
@@ -414,50 +479,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 float top = -INFINITY;
                 float s0[32], s1[32];
 #pragma unroll 1
-                for (int i = 0; i < 4; i += 2) {
+                for (int i = 0; i < KT / 32; i += 2) {
                     pt_ld32(s_at + 32 * i, s0);
-                    pt_ld32(s_at + 32 * i + 32, s1);
+                    if constexpr (KT > 32) pt_ld32(s_at + 32 * i + 32, s1);
                     pt_wait_ld(s0);
-                    pt_wait_ld(s1);
-                    if (!all) mask(s0, i), mask(s1, i + 1);
+                    if constexpr (KT > 32) pt_wait_ld(s1);
+                    if (!all) {
+                        mask(s0, i);
+                        if constexpr (KT > 32) mask(s1, i + 1);
+                    }
                     float top1 = -INFINITY;
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
                         top = max3(top, s0[k], s0[k + 1]);
-                        top1 = max3(top1, s1[k], s1[k + 1]);
+                        if constexpr (KT > 32) top1 = max3(top1, s1[k], s1[k + 1]);
                     }
                     top = fmaxf(top, top1);
                 }
                 top = fmaxf(m, top);  // of the scores before scaling
                 const bool none = top == -INFINITY;
                 const float c = none ? 1.f : ex2((m - top) * sc);
-                const float off = none ? 0.f : 10.f - top * sc;
+                const float off = none ? 0.f : (F32 ? 0.f : 10.f) - top * sc;
                 m = top;
                 float sum0 = 0.f, sum1 = 0.f;
                 auto weights = [&](float (&s)[32], int i) {
 #pragma unroll
                     for (int c16 = 0; c16 < 2; ++c16) {
-                        uint32_t hi[8], lo[8];
+                        if constexpr (F32) {  // hi over the scores, lo KT columns on
+                            uint32_t hi[16], lo[16];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            float x, y;
-                            fma2(x, y, s[16 * c16 + 2 * k], s[16 * c16 + 2 * k + 1], sc, sc, off, off);
-                            x = ex2(x), y = ex2(y);
-                            add2(sum0, sum1, x, y);
-                            const __half2 h = __floats2half2_rn(x, y);
-                            const float2 back = __half22float2(h);
-                            fma2(x, y, back.x, back.y, -1.f, -1.f, x, y);
-                            const __half2 r = __floats2half2_rn(x, y);
-                            hi[k] = *reinterpret_cast<const uint32_t*>(&h);
-                            lo[k] = *reinterpret_cast<const uint32_t*>(&r);
+                            for (int k = 0; k < 16; k += 2) {
+                                float x, y;
+                                fma2(x, y, s[16 * c16 + k], s[16 * c16 + k + 1], sc, sc, off, off);
+                                x = ex2(x), y = ex2(y);
+                                add2(sum0, sum1, x, y);
+                                split_tf32(x, hi[k], lo[k]);
+                                split_tf32(y, hi[k + 1], lo[k + 1]);
+                            }
+                            pt_st16(s_at + 32 * i + 16 * c16, hi);
+                            pt_st16(s_at + KT + 32 * i + 16 * c16, lo);
+                        } else {
+                            uint32_t hi[8], lo[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                float x, y;
+                                fma2(x, y, s[16 * c16 + 2 * k], s[16 * c16 + 2 * k + 1], sc, sc, off, off);
+                                x = ex2(x), y = ex2(y);
+                                add2(sum0, sum1, x, y);
+                                const __half2 h = __floats2half2_rn(x, y);
+                                const float2 back = __half22float2(h);
+                                fma2(x, y, back.x, back.y, -1.f, -1.f, x, y);
+                                const __half2 r = __floats2half2_rn(x, y);
+                                hi[k] = *reinterpret_cast<const uint32_t*>(&h);
+                                lo[k] = *reinterpret_cast<const uint32_t*>(&r);
+                            }
+                            pt_st8(s_at + 32 * i + 16 * c16, hi);
+                            pt_st8(s_at + 32 * i + 16 * c16 + 8, lo);
                         }
-                        pt_st8(s_at + 32 * i + 16 * c16, hi);
-                        pt_st8(s_at + 32 * i + 16 * c16 + 8, lo);
                     }
                 };
 #pragma unroll 1
-                for (int i = 2; i >= 0; i -= 2) {
-                    weights(s1, i + 1);
+                for (int i = KT == 128 ? 2 : 0; i >= 0; i -= 2) {
+                    if constexpr (KT > 32) weights(s1, i + 1);
                     if (i) pt_ld32(s_at + 32, s1);
                     weights(s0, i);
                     if (i) {
@@ -481,7 +564,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             }
             if (r < rows && ok) {  // a row per thread
                 const bool whole = cur.part < 0;
-                const int64_t at = (int64_t)cur.part * PT_R + 128 * t + r;
+                const int64_t at = (int64_t)cur.part * C::R + 128 * t + r;
                 const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
                 float* p = whole ? out_row(A, cur, G, row) : A.part_acc + at * HD;
 #pragma unroll
@@ -496,44 +579,59 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
             // ---- MMAs ----
-            constexpr uint32_t id_s = pt_idesc(128, 128, false), id_o = pt_idesc(128, HDP, true);
+            constexpr uint32_t id_s = pt_idesc(128, KT, false, F32), id_o = pt_idesc(128, HDP, !F32, F32);
             int half = 0;               // K and V tiles so far: the ring's order
             int n_q[2] = {0, 0}, n_s[2] = {0, 0};  // q tiles and key tiles so far
             bool ok = true;
             const uint32_t leader = pt_elect();
-            // loops of a few MMAs: the code stays in the instruction cache, 64 cycles an MMA are time
+            // loops of a few MMAs: the code stays in the instruction cache, 64 cycles an MMA are time.
+            // FP16: lo k, hi k.  FP32: lo hi, hi lo, hi hi (pass 0, 1, 2).
+            constexpr int PASSES = F32 ? 3 : 2;
             auto scores = [&](int t, uint32_t k_at) {
-                uint64_t qa = pt_desc(base + (uint32_t)((2 * t + 1) * C::TILE), 16);  // lo, then hi
-                const uint64_t kb = pt_desc(k_at, 16);
+                const uint32_t q_at = base + (uint32_t)(2 * t * C::Q_PLANE);
                 uint32_t add = 0;
 #pragma unroll 1
-                for (int part = 0; part < 2; ++part, qa -= C::TILE >> 4)
+                for (int pass = 0; pass < PASSES; ++pass) {
+                    uint64_t qa = pt_desc(q_at + (pass == 0 ? C::Q_PLANE : 0), 16);
+                    uint64_t kb = pt_desc(k_at + (F32 && pass == 1 ? C::PLANE : 0), 16);
 #pragma unroll 1
-                    for (uint32_t off = 0; off < (uint32_t)C::TILE >> 4; off += C::BLOCK >> 4)
+                    for (int b = 0; b < HDP / C::ROW; ++b, qa += C::Q_BLOCK >> 4, kb += C::K_BLOCK >> 4)
 #pragma unroll
                         for (int k = 0; k < 4; ++k, add = 1)  // 32 bytes a step
-                            pt_mma_ss(tmem + 128 * t, qa + off + 2 * k, kb + off + 2 * k, id_s, add,
-                                      leader);
+                            pt_mma_ss<F32>(tmem + 128 * t, qa + 2 * k, kb + 2 * k, id_s, add, leader);
+                }
             };
             auto outputs = [&](int t, uint32_t v_at) {
                 uint32_t add = 0;
 #pragma unroll 1
-                for (int part = 1; part >= 0; --part) {
-                    uint64_t vb = pt_desc(v_at, C::BLOCK);
-                    uint32_t pa = tmem + 128 * t + 8 * part;
+                for (int pass = 0; pass < PASSES; ++pass) {
+                    if constexpr (F32) {
+                        uint64_t vb = pt_desc(v_at + (pass == 1 ? C::PLANE : 0), 16);
+                        uint32_t pa = tmem + 128 * t + (pass == 0 ? KT : 0);
 #pragma unroll 1
-                    for (int k0 = 0; k0 < PT_KT / 16; k0 += 4, vb += 4 * 128, pa += 64)
+                        for (int b = 0; b < KT / 32; ++b, vb += C::V_BLOCK >> 4, pa += 32)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k, add = 1)  // 16 rows, 2048 bytes, a step
-                            pt_mma_ts(tmem + 256 + 128 * t, pa + 16 * k, vb + 128 * k, id_o, add, leader);
+                            for (int k = 0; k < 4; ++k, add = 1)  // 8 positions, 32 bytes, a step
+                                pt_mma_ts<true>(tmem + 256 + 128 * t, pa + 8 * k, vb + 2 * k, id_o, add,
+                                                leader);
+                    } else {
+                        uint64_t vb = pt_desc(v_at, C::V_BLOCK);
+                        uint32_t pa = tmem + 128 * t + (pass == 0 ? 8 : 0);
+#pragma unroll 1
+                        for (int k0 = 0; k0 < KT / 16; k0 += 4, vb += 4 * 128, pa += 64)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k, add = 1)  // 16 rows, 2048 bytes, a step
+                                pt_mma_ts<false>(tmem + 256 + 128 * t, pa + 16 * k, vb + 128 * k, id_o,
+                                                 add, leader);
+                    }
                 }
             };
             while (ok && next()) {
                 const int n_kt = it.kt1 - it.kt0, n_t = it.rows > 128 ? 2 : 1;
                 if (n_kt == 0) continue;
-                auto slot_at = [&](int h) { return ring + (uint32_t)((h % PT_SLOTS) * C::TILE); };
+                auto slot_at = [&](int h) { return ring + (uint32_t)((h % C::SLOTS) * C::TILE); };
                 auto arrived = [&](int h) {
-                    ok = ok && wait(&bar.kv_full[h % PT_SLOTS], h / PT_SLOTS);
+                    ok = ok && wait(&bar.kv_full[h % C::SLOTS], h / C::SLOTS);
                     pt_fence_async();  // written by cp.async and stores, read by the tensor core
                 };
                 arrived(half);
@@ -543,7 +641,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     if (ok) {
                         scores(t, slot_at(half));
                         pt_commit(&bar.s_full[t], leader);
-                        if (t == n_t - 1) pt_commit(&bar.kv_empty[half % PT_SLOTS], leader);
+                        if (t == n_t - 1) pt_commit(&bar.kv_empty[half % C::SLOTS], leader);
                     }
                 }
                 for (int j = 0; j < n_kt && ok; ++j) {
@@ -556,14 +654,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                         if (ok) {
                             outputs(t, slot_at(hv));
                             pt_commit(&bar.o_full[t], leader);
-                            if (t == n_t - 1) pt_commit(&bar.kv_empty[hv % PT_SLOTS], leader);
+                            if (t == n_t - 1) pt_commit(&bar.kv_empty[hv % C::SLOTS], leader);
                         }
                         if (j + 1 < n_kt) {
                             if (t == 0) arrived(hk);
                             if (ok) {
                                 scores(t, slot_at(hk));
                                 pt_commit(&bar.s_full[t], leader);
-                                if (t == n_t - 1) pt_commit(&bar.kv_empty[hk % PT_SLOTS], leader);
+                                if (t == n_t - 1) pt_commit(&bar.kv_empty[hk % C::SLOTS], leader);
                             }
                         }
                         __syncwarp();
@@ -574,16 +672,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             // the MMAs issued are done before tensor memory is given back
             pt_commit(&bar.done, leader);
             wait(&bar.done, 0);
-        } else {
+        } else if constexpr (!F32) {
             // ---- copies.  Row by row: 16 rows at a time, lane j (and j + 16) sees to row j; with
             // TMA: lane i of warp 9 sees to box i. ----
             const int lw = warp - 9;
             constexpr int CH = HDP / 8, RL = 32 / CH;  // chunks of a row, rows at a time
+            constexpr int BLOCKS = HDP / 64;
             const int row_bytes = HD * 2, x = lane % CH, r0 = lane / CH;
             const bool in_row = x * 16 < row_bytes;
             const uint8_t* const src_x[2] = {(const uint8_t*)A.k + x * 16, (const uint8_t*)A.v + x * 16};
-            const int box = TA.box, box_row = (lane / C::BLOCKS) << box, box_col = lane % C::BLOCKS;
-            const bool has_box = box && box_row < PT_KT;
+            const int box = TA.box, box_row = (lane / BLOCKS) << box, box_col = lane % BLOCKS;
+            const bool has_box = box && box_row < KT;
             int half = 0;
             uint32_t tile_no = 0;
             int n_look = 0;
@@ -606,18 +705,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     return page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
                 };
                 for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
-                    const bool careful = kt * PT_KT + PT_KT - 1 > first_lim;
+                    const bool careful = kt * KT + KT - 1 > first_lim;
                     int box_at = -1, rows3[3] = {-1, -1, -1};
-                    if (lw == 0 && has_box) box_at = row_of(kt * PT_KT + box_row);
+                    if (lw == 0 && has_box) box_at = row_of(kt * KT + box_row);
                     if (!box) {
 #pragma unroll
                         for (int i = 0; i < 3; ++i)
                             if (lw + 3 * i < 8)
-                                rows3[i] = row_of(kt * PT_KT + (lw + 3 * i) * 16 + (lane & 15));
+                                rows3[i] = row_of(kt * KT + (lw + 3 * i) * 16 + (lane & 15));
                     }
 #pragma unroll 1
                     for (int kv = 0; kv < 2 && ok; ++kv, ++half) {
-                        const int slot = half % PT_SLOTS, use = half / PT_SLOTS;
+                        const int slot = half % C::SLOTS, use = half / C::SLOTS;
                         if (use > 0 && !wait(&bar.kv_empty[slot], use - 1)) {
                             ok = false;
                             break;
@@ -630,8 +729,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                                 if (lane == 0) mbar_arrive_expect_tx(there, C::TILE);
                                 __syncwarp();
                                 if (has_box) {
-                                    pt_tma(tile_at + (uint32_t)(box_col * C::BLOCK + box_row * 128),
-                                           kv ? &TA.v : &TA.k, box_col * 64, box_at < 0 ? -PT_KT : box_at,
+                                    pt_tma(tile_at + (uint32_t)(box_col * C::K_BLOCK + box_row * 128),
+                                           kv ? &TA.v : &TA.k, box_col * 64, box_at < 0 ? -KT : box_at,
                                            there);
                                     if (kv == 0 && box_col == 0)
                                         for (int b = 0; b < 1 << (box - 3); ++b)
@@ -656,7 +755,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                                     const int from = k * RL + r0;
                                     const int n = __shfl_sync(0xffffffffu, row, from);
                                     const bool there = n >= 0 && in_row;
-                                    cp16(tile_at + (uint32_t)((x >> 3) * C::BLOCK) +
+                                    cp16(tile_at + (uint32_t)((x >> 3) * C::K_BLOCK) +
                                              pt_off(g16 * 16 + from, x & 7),
                                          src + (there ? (int64_t)n * row_bytes : 0), there);
                                 }
@@ -674,9 +773,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                             for (int g16 = lw; g16 < 8; g16 += 3) {
                                 uint32_t bad = 0;
 #pragma unroll 4
-                                for (int k = 0; k < 4 * C::BLOCKS; ++k) {  // four rows of a block
+                                for (int k = 0; k < 4 * BLOCKS; ++k) {  // four rows of a block
                                     uint4* const at = reinterpret_cast<uint4*>(
-                                        tile + (k >> 2) * C::BLOCK + (g16 * 16 + (k & 3) * 4) * 128 + lane * 16);
+                                        tile + (k >> 2) * C::K_BLOCK + (g16 * 16 + (k & 3) * 4) * 128 + lane * 16);
                                     uint4 v = *at;
                                     bool odd = false;
                                     v.x = finite16x2(v.x, odd), v.y = finite16x2(v.y, odd);
@@ -705,8 +804,127 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             }
             // no copy may still be landing when the CTA ends
             asm volatile("cp.async.wait_all;" ::: "memory");
-            for (int h = max(0, half - PT_SLOTS); h < half; ++h)
-                wait(&bar.kv_full[h % PT_SLOTS], h / PT_SLOTS);
+            for (int h = max(0, half - C::SLOTS); h < half; ++h)
+                wait(&bar.kv_full[h % C::SLOTS], h / C::SLOTS);
+        } else {
+            // ---- copies of FP32 pages: TMA brings K and V as they are, the three warps split them
+            // into TF32 parts, hi in the slot's first half, lo in the second.  K: rows are positions,
+            // 128 bytes 32 dimensions.  V is turned round, since TF32 operands have to lie along K:
+            // rows are dimensions, 128 bytes 32 positions. ----
+            const int lw = warp - 9;
+            const int box = TA.box, box_row = lane << box;
+            const bool has_box = box_row < KT;
+            const uint32_t raw_a = ring + C::SLOTS * C::TILE;
+            const uint8_t* const raw_ptr = base_ptr + (raw_a - base);
+            int half = 0, issued[2] = {0, 0}, used[2] = {0, 0};  // tiles brought in and split, K and V
+            uint32_t tile_no = 0;
+            bool ok = true;
+            while (ok && next()) {
+                const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
+                const int first_lim = it.start + it.row0 / G;
+                if (lw == 1) {  // the softmax warps ask for the segment's q soon
+                    for (int r = lane; r < it.rows; r += 32) {
+                        const uint8_t* p = (const uint8_t*)q_row(A, it, G, it.row0 + r);
+                        for (int b = 0; b < HD * 4; b += 128)
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
+                    }
+                }
+                auto box_of = [&](int kt) -> int {  // this lane's box of key tile kt, -1: none
+                    const int pos = kt * KT + box_row;
+                    if (lw != 0 || !has_box || kt >= it.kt1 || pos > last_lim) return -1;
+                    const int col = (int)w.ps.div((uint32_t)pos);
+                    const int page = page_at(w, it.s.row[col]);
+                    return page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
+                };
+                auto bring = [&](int kv, int at) {  // warp 9
+                    if (issued[kv] > 0) ok = ok && wait(&bar.raw_empty[kv], issued[kv] - 1);
+                    if (!ok) return;
+                    if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[kv], C::PLANE);
+                    __syncwarp();
+                    if (has_box)
+                        pt_tma(raw_a + (uint32_t)(kv * C::PLANE + box_row * HDP * 4), kv ? &TA.v : &TA.k, 0,
+                               at < 0 ? -KT : at, &bar.raw_full[kv]);
+                    ++issued[kv];
+                };
+                int box_at = box_of(it.kt0), box_next = -1;
+                if (lw == 0 && it.kt0 < it.kt1) bring(0, box_at), bring(1, box_at);
+                for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
+                    const bool careful = kt * KT + KT - 1 > first_lim;
+                    box_next = box_of(kt + 1);
+#pragma unroll 1
+                    for (int kv = 0; kv < 2 && ok; ++kv, ++half) {
+                        const int slot = half % C::SLOTS, use = half / C::SLOTS;
+                        ok = wait(&bar.raw_full[kv], used[kv]);
+                        if (use > 0) ok = ok && wait(&bar.kv_empty[slot], use - 1);
+                        if (!ok) break;
+                        uint8_t* const tile = base_ptr + (ring - base) + slot * C::TILE;
+                        const uint8_t* const raw = raw_ptr + kv * C::PLANE;
+                        if (kv == 0) {
+                            if (lw == 0 && has_box)
+                                for (int b = 0; b < 1 << (box - 3); ++b)
+                                    reinterpret_cast<uint8_t*>(sh_gone[tile_no & 3])[box_row / 8 + b] =
+                                        box_at < 0 ? 0xff : 0;
+#pragma unroll 4
+                            for (int i = lw * 32 + lane; i < C::PLANE / 16; i += PT_LOADERS) {
+                                const int r = i / (HDP / 4), d = (i % (HDP / 4)) * 4;
+                                const float4 x = *reinterpret_cast<const float4*>(raw + i * 16);
+                                uint4 h, l;
+                                split_tf32(x.x, h.x, l.x), split_tf32(x.y, h.y, l.y);
+                                split_tf32(x.z, h.z, l.z), split_tf32(x.w, h.w, l.w);
+                                uint8_t* const at = tile + (d >> 5) * C::K_BLOCK + pt_off(r, (d & 31) >> 2);
+                                *reinterpret_cast<uint4*>(at) = h;
+                                *reinterpret_cast<uint4*>(at + C::PLANE) = l;
+                            }
+                        } else {
+                            uint32_t bad0 = 0, bad1 = 0;
+                            // four positions of 32 dimensions at a time, a dimension to a lane
+#pragma unroll 2
+                            for (int u = lw; u < KT / 4 * (HDP / 32); u += PT_LOADERS / 32) {
+                                const int p4 = u / (HDP / 32), d = (u % (HDP / 32)) * 32 + lane;
+                                float y[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    y[j] = *reinterpret_cast<const float*>(raw + ((p4 * 4 + j) * HDP + d) * 4);
+                                if (careful) {
+                                    uint32_t odd4 = 0;
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        const bool odd = !(fabsf(y[j]) < INFINITY);
+                                        if (odd) y[j] = 0.f;
+                                        if (__any_sync(0xffffffffu, odd)) odd4 |= 1u << j;
+                                    }
+                                    if (p4 < 8) bad0 |= odd4 << (4 * p4);
+                                    else bad1 |= odd4 << (4 * p4 - 32);
+                                }
+                                uint4 h, l;
+                                split_tf32(y[0], h.x, l.x), split_tf32(y[1], h.y, l.y);
+                                split_tf32(y[2], h.z, l.z), split_tf32(y[3], h.w, l.w);
+                                uint8_t* const at = tile + (p4 >> 3) * C::V_BLOCK + pt_off(d, p4 & 7);
+                                *reinterpret_cast<uint4*>(at) = h;
+                                *reinterpret_cast<uint4*>(at + C::PLANE) = l;
+                            }
+                            if (lane == 0) {
+                                sh_bad32[tile_no & 3][lw][0] = bad0;
+                                sh_bad32[tile_no & 3][lw][1] = bad1;
+                            }
+                        }
+                        pt_fence_async();
+                        mbar_arrive(&bar.kv_full[slot]);
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&bar.kv_full[slot]);
+                            mbar_arrive(&bar.raw_empty[kv]);
+                        }
+                        ++used[kv];
+                        if (lw == 0 && kt + 1 < it.kt1) bring(kv, box_next);
+                    }
+                    box_at = box_next;
+                }
+            }
+            // no copy may still be landing when the CTA ends
+            if (lw == 0)
+                for (int kv = 0; kv < 2; ++kv)
+                    if (issued[kv] > used[kv]) wait(&bar.raw_full[kv], issued[kv] - 1);
         }
     }
     // every use of tensor memory is over before it is given back
@@ -719,8 +937,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     }
 }
 
-// The layer's rows as a tensor of FP16 [rows][head_dim], in boxes of 64 columns.
+// The layer's rows as a tensor [rows][head_dim]: FP16 in swizzled boxes of 64 columns, FP32 in
+// plain boxes of all (padded) columns.
+template <typename KV, int HDP>
 static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head_dim, int box_rows) {
+    constexpr bool F32 = sizeof(KV) == 4;
     static PFN_cuTensorMapEncodeTiled encode = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
@@ -736,13 +957,14 @@ static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head
         return IB_ERR_CUDA;
     }
     const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)head_dim * sizeof(KV)};
+    const cuuint32_t box[2] = {F32 ? HDP : 64, (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
-                              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = encode(
+        map, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        F32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("ib_attention_paged: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
         return IB_ERR_CUDA;
@@ -750,42 +972,60 @@ static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head
     return IB_OK;
 }
 
-CutRule tensor_rule(int min_rows, int max_rows) {
+template <typename KV>
+CutRule tensor_rule(int head_dim, int min_rows, int max_rows) {
     // one CTA to an SM (148 of a B200), a piece for each
-    return CutRule{PT_R, PT_KT, min_rows, max_rows, 148, 128};
+    using S = TensorCfg<KV, 64>;
+    using L = TensorCfg<KV, 128>;
+    return head_dim <= 64 ? CutRule{S::R, S::KT, min_rows, max_rows, 148, 128}
+                          : CutRule{L::R, L::KT, min_rows, max_rows, 148, 128};
 }
+template CutRule tensor_rule<float>(int, int, int);
+template CutRule tensor_rule<__half>(int, int, int);
 
-template <int HDP>
-static int launch(const TensorArgs& a, int64_t grid, cudaStream_t st) {
-    auto kern = attn_tensor_kernel<HDP>;
-    static DeviceOnce once;
-    IB_CUDA_CHECK(once.run([&] {
-        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)TensorCfg<HDP>::SMEM);
-    }));
-    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(PT_THREADS), TensorCfg<HDP>::SMEM, st,
-                             true, a));
-    return IB_OK;
-}
-
-int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st) {
-    const int64_t most = tiles * (max_pos / a.rule.least + 1 + a.rule.R);
-    const int64_t grid = std::min<int64_t>(a.rule.n_pieces, most);
+template <typename KV, int HDP>
+static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
+    using C = TensorCfg<KV, HDP>;
+    auto kern = attn_tensor_kernel<KV, HDP>;
     TensorArgs t{};
     t.rows = a;
     const PagedView& w = a.w;
-    // the largest power of two that divides the page, up to the tile; fewer than 8 rows would not
-    // fill a swizzled group
+    // a box: the largest power of two that divides the page, up to the tile
     int box = 0;
-    while (box < 7 && w.page_size % (2 << box) == 0) ++box;
+    while (2 << box <= C::KT && w.page_size % (2 << box) == 0) ++box;
     if (box >= 3) {
         const int64_t rows = (int64_t)w.n_pages * w.Hkv * w.page_size;
-        int r = tensor_map(&t.k, a.k, rows, w.HD, 1 << box);
-        if (r == IB_OK) r = tensor_map(&t.v, a.v, rows, w.HD, 1 << box);
+        int r = tensor_map<KV, HDP>(&t.k, a.k, rows, w.HD, 1 << box);
+        if (r == IB_OK) r = tensor_map<KV, HDP>(&t.v, a.v, rows, w.HD, 1 << box);
         if (r != IB_OK) return r;
         t.box = box;
+    } else if (C::F32) {  // not taken: tensor_takes
+        set_error("ib_attention_paged: no boxes for this page size");
+        return IB_ERR_INVALID;
     }
-    return w.HD <= 64 ? launch<64>(t, grid, st) : launch<128>(t, grid, st);
+    static DeviceOnce once;
+    IB_CUDA_CHECK(once.run([&] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    }));
+    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(PT_THREADS), C::SMEM, st, true, t));
+    return IB_OK;
 }
+
+template <typename KV>
+bool tensor_takes(int head_dim, int page_size) {
+    // FP32 tiles come by TMA alone, in boxes of 8 rows or more
+    return head_dim <= 128 && (sizeof(KV) == 2 || page_size % 8 == 0);
+}
+template bool tensor_takes<float>(int, int);
+template bool tensor_takes<__half>(int, int);
+
+template <typename KV>
+int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st) {
+    const int64_t most = tiles * (max_pos / a.rule.least + 1 + a.rule.R);
+    const int64_t grid = std::min<int64_t>(a.rule.n_pieces, most);
+    return a.w.HD <= 64 ? launch<KV, 64>(a, grid, st) : launch<KV, 128>(a, grid, st);
+}
+template int attn_tensor_launch<float>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
+template int attn_tensor_launch<__half>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
 
 }  // namespace ib
