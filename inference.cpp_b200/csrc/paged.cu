@@ -22,6 +22,7 @@
 #include "common.cuh"
 #include "kv.cuh"
 #include "paged.cuh"
+#include "pdl.cuh"
 
 namespace ib {
 
@@ -157,60 +158,67 @@ struct KvSeqsDev {
 // last page is copied to.  Otherwise a = slots, b = tokens to make room for.  Pages go out
 // lowest first in list order; once an entry finds too few, it and every later entry that
 // needs pages get none.  status: 1 done, 0 no room, -1 refused.
+// What the entries need stays in shared memory: the kernel is a chain of dependent accesses (list,
+// length, table, refs, hand-out) and little else, 12 us with each step going back to global
+// memory.
 template <bool FORK>
 __global__ void __launch_bounds__(KV_PLAN_THREADS)
     kv_assign_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ a,
                      const int32_t* __restrict__ b, int32_t* __restrict__ status) {
     extern __shared__ int sh[];
     __shared__ int warp_sums[32];
-    int* first = sh;               // [n_slots]: lowest list index naming the slot
-    int* off = sh + s.n_slots;     // [n + 1]: pages needed by the entries before
+    const int n_first = max(s.n_slots, n);
+    int* first = sh;                // [n_slots]: lowest list index naming the slot; then
+    int* len = sh;                  // [n]: length of the entry's source
+    int* off = sh + n_first;        // [n + 1]: pages needed by the entries before
+    uint16_t* slot_of = reinterpret_cast<uint16_t*>(off + n + 1);  // [n]
+    int8_t* state = reinterpret_cast<int8_t*>(slot_of + n);        // [n]
     const int tid = threadIdx.x, cap = s.max_pages * s.page_size;
     const int32_t* slots = FORK ? b : a;
+    pdl_launch_dependents();
+    int r[KV_SCAN];
+    load_refs(s.refs, 0, s.n_pages, r);  // the first scan's, on their way
     for (int i = tid; i < n; i += KV_PLAN_THREADS) {
         const int slot = slots[i];
-        if (slot >= 0 && slot < s.n_slots) first[slot] = 0x7fffffff;
+        const bool in = slot >= 0 && slot < s.n_slots;
+        slot_of[i] = (uint16_t)(in ? slot : 0xffff);
+        if (in) first[slot] = 0x7fffffff;
     }
     __syncthreads();
-    for (int i = tid; i < n; i += KV_PLAN_THREADS) {
-        const int slot = slots[i];
-        if (slot >= 0 && slot < s.n_slots) atomicMin(&first[slot], i);
-    }
+    for (int i = tid; i < n; i += KV_PLAN_THREADS)
+        if (slot_of[i] != 0xffff) atomicMin(&first[slot_of[i]], i);
     __syncthreads();
+    for (int i = tid; i < n; i += KV_PLAN_THREADS)
+        state[i] = slot_of[i] != 0xffff && first[slot_of[i]] == i ? 1 : -1;
+    __syncthreads();  // first is done with
     int total = 0;
     for (int i0 = 0; i0 < n; i0 += KV_PLAN_THREADS) {
         const int i = i0 + tid;
         int need = 0;
         if (i < n) {
-            const int slot = slots[i];
+            const int slot = slot_of[i], src = FORK ? a[i] : slot;
             int st = -1;
-            if (slot >= 0 && slot < s.n_slots && first[slot] == i) {
-                const int src = FORK ? a[i] : slot;
-                if (src >= 0 && src < s.n_slots && (!FORK || (src != slot && s.len[slot] == 0))) {
-                    const int L = s.len[src];
-                    const int more = FORK ? 0 : b[i];
-                    if (L < 0 || L > cap) {
-                        paged_fault(PAGED_BAD_LEN);
-                    } else if (FORK) {
-                        const int full = L / s.page_size;
-                        st = 1;
-                        // a page that was given back (-1) has nothing to copy
-                        if (L % s.page_size) {
-                            const int t = s.table[(size_t)src * s.max_pages + full];
-                            if (t < -1 || t >= s.n_pages) paged_fault(PAGED_BAD_PAGE);
-                            need = t >= 0 && t < s.n_pages;
-                        }
-                    } else if (more >= 0) {
-                        if (more > cap - L) st = 0;
-                        else {
-                            st = 1;
-                            need = (L + more + s.page_size - 1) / s.page_size -
-                                   (L + s.page_size - 1) / s.page_size;
-                        }
+            if (state[i] == 1 && src >= 0 && src < s.n_slots &&
+                (!FORK || (src != slot && s.len[slot] == 0))) {
+                const int L = s.len[src], more = FORK ? 0 : b[i];
+                len[i] = L;
+                if (L < 0 || L > cap) {
+                    paged_fault(PAGED_BAD_LEN);
+                } else if (FORK) {
+                    st = 1;
+                    if (L % s.page_size) {  // a page that was given back (-1) has nothing to copy
+                        const int t = s.table[(size_t)src * s.max_pages + L / s.page_size];
+                        if (t < -1 || t >= s.n_pages) paged_fault(PAGED_BAD_PAGE);
+                        need = t >= 0 && t < s.n_pages;
                     }
+                } else if (more >= 0) {
+                    st = more > cap - L ? 0 : 1;
+                    if (st)
+                        need = (L + more + s.page_size - 1) / s.page_size -
+                               (L + s.page_size - 1) / s.page_size;
                 }
             }
-            status[i] = st == 1 && need ? 2 : st;  // 2: if the pages are there
+            state[i] = (int8_t)(st == 1 && need ? 2 : st);  // 2: if the pages are there
         }
         // more than the pool holds is as good as one page more: the sums stay in 31 bits
         // (1024 x (2^20 + 1)), and a saturated end is past any number of free pages
@@ -221,25 +229,31 @@ __global__ void __launch_bounds__(KV_PLAN_THREADS)
         total = min(total + sum, most);
     }
     if (tid == 0) off[n] = total;
-    __syncthreads();
-    // free pages, up to what is asked for
-    int avail = 0;
-    for (int base = 0; base < s.n_pages && avail < total; base += KV_PLAN_THREADS * KV_SCAN) {
-        int r[KV_SCAN], c = 0, sum;
-        load_refs(s.refs, base, s.n_pages, r);
+    // free pages, up to what is asked for; with one round of refs they are numbered with it
+    constexpr int ROUND = KV_PLAN_THREADS * KV_SCAN;
+    const bool one_round = s.n_pages <= ROUND;
+    int avail = 0, number = 0;
+    for (int base = 0; base < s.n_pages && avail < total; base += ROUND) {
+        int c = 0, sum;
+        if (base) load_refs(s.refs, base, s.n_pages, r);
 #pragma unroll
         for (int k = 0; k < KV_SCAN; ++k) c += r[k] <= 0;
-        block_scan(c, warp_sums, sum);
+        number = block_scan(c, warp_sums, sum);
         avail += sum;
     }
+    __syncthreads();  // off
     // entry i is served when the pages up to and with its own are there
     int served = 0;  // pages handed out
-    for (int i = tid; i < n; i += KV_PLAN_THREADS)
-        if (status[i] == 2) {
-            const bool room = off[i + 1] <= avail;
-            status[i] = room ? 1 : 0;
-            if (room) served = max(served, off[i + 1]);
+    for (int i = tid; i < n; i += KV_PLAN_THREADS) {
+        int st = state[i];
+        if (st == 2) {
+            st = off[i + 1] <= avail;
+            if (st) served = max(served, off[i + 1]);
+            state[i] = (int8_t)st;
         }
+        status[i] = st;
+        if (st == 1) s.len[slot_of[i]] = FORK ? len[i] : len[i] + b[i];
+    }
     for (int o = 16; o > 0; o >>= 1) served = max(served, __shfl_xor_sync(0xffffffffu, served, o));
     if ((tid & 31) == 0) warp_sums[tid >> 5] = served;
     __syncthreads();
@@ -247,13 +261,18 @@ __global__ void __launch_bounds__(KV_PLAN_THREADS)
     __syncthreads();
     // hand them out: the k-th free page belongs to the entry with off[i] <= k < off[i + 1]
     int given = 0;
-    for (int base = 0; base < s.n_pages && given < served; base += KV_PLAN_THREADS * KV_SCAN) {
-        int r[KV_SCAN], c = 0, sum;
-        load_refs(s.refs, base, s.n_pages, r);
+    for (int base = 0; base < s.n_pages && given < served; base += ROUND) {
+        int k = number;
+        if (one_round) {
+            given = avail;
+        } else {
+            int c = 0, sum;
+            load_refs(s.refs, base, s.n_pages, r);
 #pragma unroll
-        for (int k = 0; k < KV_SCAN; ++k) c += r[k] <= 0;
-        int k = given + block_scan(c, warp_sums, sum);
-        given += sum;
+            for (int j = 0; j < KV_SCAN; ++j) c += r[j] <= 0;
+            k = given + block_scan(c, warp_sums, sum);
+            given += sum;
+        }
 #pragma unroll
         for (int j = 0; j < KV_SCAN; ++j) {
             if (r[j] > 0) continue;
@@ -264,22 +283,15 @@ __global__ void __launch_bounds__(KV_PLAN_THREADS)
                     if (off[mid] <= k) lo = mid;
                     else hi = mid;
                 }
-                const int page = base + tid * KV_SCAN + j;
-                const int L = s.len[a[lo]];  // of the parent, or of the slot itself
+                const int page = base + tid * KV_SCAN + j, L = len[lo];
                 const int col = FORK ? L / s.page_size
                                      : (L + s.page_size - 1) / s.page_size + (k - off[lo]);
-                s.table[(size_t)slots[lo] * s.max_pages + col] = page;
+                s.table[(size_t)slot_of[lo] * s.max_pages + col] = page;
                 s.refs[page] = 1;
             }
             ++k;
         }
     }
-    __syncthreads();
-    for (int i = tid; i < n; i += KV_PLAN_THREADS)
-        if (status[i] == 1) {
-            if (FORK) s.len[b[i]] = s.len[a[i]];
-            else s.len[a[i]] += b[i];
-        }
 }
 
 // Copies `bytes` (a multiple of 16, both sides 16-byte aligned) by one warp, eight 16-byte
@@ -313,6 +325,7 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
                    const int32_t* __restrict__ status) {
     const int n_warps = gridDim.x * (KV_COPY_THREADS / 32);
     const int w0 = blockIdx.x * (KV_COPY_THREADS / 32) + (threadIdx.x >> 5);
+    pdl_wait();
     for (int i = blockIdx.x; i < n; i += gridDim.x) {  // rows: one CTA per child
         if (status[i] != 1) continue;
         const int full = s.len[children[i]] / s.page_size;
@@ -393,9 +406,11 @@ __global__ void __launch_bounds__(KV_PLAN_THREADS)
     __shared__ int warp_sums[32];
     constexpr int STEP = KV_PLAN_THREADS * KV_SCAN;
     const int tid = threadIdx.x;
+    pdl_launch_dependents();
+    int r[KV_SCAN];  // of the last round; with one round they are read once
     int n_live = 0;
     for (int base = 0; base < n_pages; base += STEP) {
-        int r[KV_SCAN], c = 0, sum;
+        int c = 0, sum;
         load_refs(refs, base, n_pages, r);
 #pragma unroll
         for (int k = 0; k < KV_SCAN; ++k)
@@ -403,10 +418,10 @@ __global__ void __launch_bounds__(KV_PLAN_THREADS)
         block_scan(c, warp_sums, sum);
         n_live += sum;
     }
-    int holes = 0, movers = 0;  // of the iterations before
+    int holes = 0, movers = 0;  // of the rounds before
     for (int base = 0; base < n_pages; base += STEP) {
-        int r[KV_SCAN], h = 0, m = 0, sum;
-        load_refs(refs, base, n_pages, r);
+        int h = 0, m = 0, sum;
+        if (n_pages > STEP) load_refs(refs, base, n_pages, r);
         const int p0 = base + tid * KV_SCAN;
 #pragma unroll
         for (int k = 0; k < KV_SCAN; ++k) {
@@ -450,6 +465,7 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
     kv_compact_kernel(const int32_t* table, int32_t* table_out, int64_t n_entries, int n_pages,
                       const int32_t* __restrict__ map, const int32_t* __restrict__ moves,
                       const int32_t* __restrict__ info, const PoolBytes pool) {
+    pdl_wait();
     for (int64_t e = (int64_t)blockIdx.x * KV_COPY_THREADS + threadIdx.x; e < n_entries;
          e += (int64_t)gridDim.x * KV_COPY_THREADS) {
         const int t = table[e];
@@ -579,9 +595,11 @@ static PoolBytes pool_bytes(const ib_kv_pages* p) {
     return b;
 }
 
-// first[] and off[] of kv_assign_kernel
-static size_t assign_smem(int n_slots, int n) { return ((size_t)n_slots + n + 1) * sizeof(int); }
-constexpr int KV_ASSIGN_SMEM_MAX = (2 * IB_KV_MAX_SLOTS + 1) * (int)sizeof(int);
+// kv_assign_kernel's arrays
+constexpr size_t assign_smem(int n_slots, int n) {
+    return ((size_t)(n_slots > n ? n_slots : n) + n + 1) * 4 + (size_t)n * 3;
+}
+constexpr int KV_ASSIGN_SMEM_MAX = (int)assign_smem(IB_KV_MAX_SLOTS, IB_KV_MAX_SLOTS);
 
 template <bool FORK>
 static int assign_launch(const KvSeqsDev& s, int n, const int32_t* a, const int32_t* b,
@@ -638,9 +656,8 @@ extern "C" int ib_kv_fork(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int 
     const int64_t warps = (int64_t)n * pages->n_layers * 2 * pages->n_kv_heads;
     const int grid = (int)std::min<int64_t>(
         (int64_t)sms * 8, std::max<int64_t>(n, (warps + KV_COPY_THREADS / 32 - 1) / (KV_COPY_THREADS / 32)));
-    kv_fork_kernel<<<grid, KV_COPY_THREADS, 0, st>>>(s, pool_bytes(pages), n, parents, children,
-                                                     status);
-    IB_LAUNCH_CHECK("kv_fork_kernel");
+    IB_CUDA_CHECK(launch_pdl(kv_fork_kernel, dim3(grid), dim3(KV_COPY_THREADS), 0, st, true, s,
+                             pool_bytes(pages), n, parents, children, (const int32_t*)status));
     return IB_OK;
 }
 
@@ -667,10 +684,11 @@ extern "C" int ib_kv_compact(const ib_kv_pages* pages, const ib_kv_seqs* seqs, i
     kv_compact_plan_kernel<<<1, KV_PLAN_THREADS, 0, st>>>(seqs->refs, refs_out, pages->n_pages, map,
                                                           moves, info);
     IB_LAUNCH_CHECK("kv_compact_plan_kernel");
-    kv_compact_kernel<<<sms * 8, KV_COPY_THREADS, 0, st>>>(
-        seqs->table, table_out, (int64_t)seqs->n_slots * seqs->max_pages, pages->n_pages, map, moves,
-        info, pool_bytes(pages));
-    IB_LAUNCH_CHECK("kv_compact_kernel");
+    IB_CUDA_CHECK(launch_pdl(kv_compact_kernel, dim3(sms * 8), dim3(KV_COPY_THREADS), 0, st, true,
+                             (const int32_t*)seqs->table, table_out,
+                             (int64_t)seqs->n_slots * seqs->max_pages, (int)pages->n_pages,
+                             (const int32_t*)map, (const int32_t*)moves, (const int32_t*)info,
+                             pool_bytes(pages)));
     return IB_OK;
 }
 

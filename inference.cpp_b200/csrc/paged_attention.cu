@@ -847,9 +847,11 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
 }
 
 // ---- joining the parts of a tile ---------------------------------------------------------
-// PIECES: the tiles were cut by find_pieces -- most are whole, the others in two or three -- and
-// a CTA sees to JOIN_ROWS rows of a tile, a warp to one after another.  Otherwise by find_item,
-// into many parts, and a CTA sees to one row, its four warps to every fourth part each.
+// WPR 0: the tiles were cut by find_pieces -- most are whole, the others in two or three -- and a
+// CTA sees to JOIN_ROWS rows of a tile, a warp to one after another.  Otherwise by find_item:
+// tiles of 8 rows, which can have many parts, and a CTA sees to a tile, WPR warps to a row.  (A
+// CTA to a row took 16 us against 6 on 64 single tokens: each of them plans.)  Two warps keep
+// four CTAs on an SM for many tiles; four get through the parts of a few long ones sooner.
 constexpr int JOIN_ROWS = 64;
 struct JoinArgs {
     PagedView w;
@@ -860,11 +862,16 @@ struct JoinArgs {
     const float2* part_ml;
 };
 
-template <bool PIECES>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ JoinArgs A) {
-    constexpr int NT = 128, MAXV = 2;  // float4 per lane: head_dim 256
-    __shared__ float4 sh_acc[4][32 * MAXV];
-    __shared__ float sh_l[4];
+template <int WPR>
+constexpr int join_threads = WPR == 0 ? 128 : 8 * WPR * 32;
+
+template <int WPR>
+__global__ void __launch_bounds__(join_threads<WPR>)
+    attn_join_kernel(const __grid_constant__ JoinArgs A) {
+    constexpr bool PIECES = WPR == 0;
+    constexpr int NT = join_threads<WPR>, MAXV = 2;  // float4 per lane: head_dim 256
+    __shared__ float4 sh_acc[PIECES ? 1 : 8 * WPR][32 * MAXV];
+    __shared__ float sh_l[PIECES ? 1 : 8 * WPR];
     const PagedView& w = A.w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R;
@@ -902,19 +909,22 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
         first = rest = it.part_base;
     }
     const int rows = min(R, s.n * G - tile * R);
-    const int r0 = PIECES ? blockIdx.y * JOIN_ROWS + warp : blockIdx.y;
     if (n_parts == 1) return;
-    for (int r = r0; r < min(rows, PIECES ? (int)(blockIdx.y + 1) * JOIN_ROWS : r0 + 1); r += 4) {
+    const int r0 = PIECES ? blockIdx.y * JOIN_ROWS + warp : warp / (PIECES ? 1 : WPR);
+    const int r1 = PIECES ? min(rows, (int)(blockIdx.y + 1) * JOIN_ROWS) : r0 + 1;
+    for (int r = r0; r < r1; r += 4) {
         auto at = [&](int i) { return (int64_t)(i == 0 ? first : rest + i * step) * R + r; };
         float M = -INFINITY, l = 0.f;
         float4 o[MAXV];
 #pragma unroll
         for (int i = 0; i < MAXV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = lane; i < n_parts; i += 32) M = fmaxf(M, A.part_ml[at(i)].x);
+        const bool some = PIECES || r < rows;  // the other warps come along to the barrier
+        for (int i = lane; some && i < n_parts; i += 32) M = fmaxf(M, A.part_ml[at(i)].x);
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-#pragma unroll 4
-        for (int i = PIECES ? 0 : warp; i < n_parts; i += PIECES ? 1 : 4) {
+#pragma unroll 8
+        for (int i = PIECES ? 0 : warp % (PIECES ? 1 : WPR); i < (some ? n_parts : 0);
+             i += PIECES ? 1 : WPR) {
             const float2 y = A.part_ml[at(i)];
             const float c = M == -INFINITY ? 1.f : ex2(y.x - M);
             l += c * y.y;
@@ -931,15 +941,16 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
             for (int k = 0; k < MAXV; ++k) sh_acc[warp][lane + 32 * k] = o[k];
             if (lane == 0) sh_l[warp] = l;
             __syncthreads();
-            if (warp > 0) return;
-            l = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
+            if (warp % WPR || !some) return;
 #pragma unroll
-            for (int k = 0; k < MAXV; ++k)
+            for (int i = 1; i < WPR; ++i) {
+                l += sh_l[warp + i];
 #pragma unroll
-                for (int i = 1; i < 4; ++i) {
-                    const float4 z = sh_acc[i][lane + 32 * k];
+                for (int k = 0; k < MAXV; ++k) {
+                    const float4 z = sh_acc[warp + i][lane + 32 * k];
                     o[k].x += z.x, o[k].y += z.y, o[k].z += z.z, o[k].w += z.w;
                 }
+            }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int gr = tile * R + r, tok = gr / G;
@@ -1068,12 +1079,18 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         // no tile is cut into parts where the tables' rows are no longer than the least part
         if (wide || max_pos > s.rule.least) {
             const JoinArgs j{a.w, s.rule, a.out, a.out_stride, a.part_acc, a.part_ml};
-            const int64_t G = a.w.H / a.w.Hkv;
-            const int64_t most_rows = std::min<int64_t>(s.rule.R, b->n_tokens * G);
-            const int64_t per = wide ? JOIN_ROWS : 1;
-            const auto join = wide ? attn_join_kernel<true> : attn_join_kernel<false>;
-            IB_CUDA_CHECK(launch_pdl(join, dim3((unsigned)s.tiles, (unsigned)((most_rows + per - 1) / per)), dim3(128),
-                                     0, st, true, j));
+            const int64_t most_rows = std::min<int64_t>(s.rule.R, (int64_t)b->n_tokens * (a.w.H / a.w.Hkv));
+            const unsigned tiles = (unsigned)s.tiles;
+            if (wide)
+                IB_CUDA_CHECK(launch_pdl(attn_join_kernel<0>,
+                                         dim3(tiles, (unsigned)((most_rows + JOIN_ROWS - 1) / JOIN_ROWS)),
+                                         dim3(join_threads<0>), 0, st, true, j));
+            else if (s.tiles <= kSMs)
+                IB_CUDA_CHECK(launch_pdl(attn_join_kernel<4>, dim3(tiles), dim3(join_threads<4>), 0, st,
+                                         true, j));
+            else
+                IB_CUDA_CHECK(launch_pdl(attn_join_kernel<2>, dim3(tiles), dim3(join_threads<2>), 0, st,
+                                         true, j));
         }
     }
     return IB_OK;
