@@ -2,13 +2,27 @@
 //
 // The query rows of a sequence that share a kv head -- (token, head of the group), token by
 // token -- are consecutive: row r is token r / G, head r % G.  A tile is R such rows against the
-// positions they see.  The tiles of a call are laid end to end and cut into as many pieces of
-// equal work as there are workers (CTAs, or single warps), so that a batch of any mix of
-// lengths keeps every SM busy to the end.  A tile that is cut leaves partial results (running maximum
-// m, exponential sum l, unnormalised sum of p v), and a second kernel joins them:
+// positions they see.  Tiles are cut so that a batch of any mix of lengths keeps every SM busy to
+// the end (paged_plan.cuh); a tile that is cut leaves partial results (running maximum m,
+// exponential sum l, unnormalised sum of p v), and a second kernel joins them:
 //     out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.
 // Lengths are device data: every CTA works the cuts out for itself from cu_q and len (one pass
 // over the batch; no planning launch).
+//
+// Products of FP32 operands keep about 2^-21 on the tensor cores:
+//   FP16 pages  q = hi + lo and p = hi + lo in FP16, K and V as they are: two products.  q rows
+//               are scaled to a largest element in [256, 512) and p by 2^10, powers of two that
+//               keep the lo parts out of FP16's subnormals.
+//   FP32 pages  both operands as TF32 hi + lo, hi hi + hi lo + lo hi: three products, with the
+//               range of FP32.
+// The MMA adds to its FP32 accumulator by cutting, half a unit of the accumulator per step on
+// average and always towards zero: a running sum over a long sequence would drift (2.6e-6 of
+// the result over 131072 positions, 4e-7 this way).  So lo parts have accumulators of their own
+// or go first, and p v of each tile starts from zero and is added to the running sum by FFMA,
+// which rounds and takes the rescaling with it.
+// Positions that a row does not see get a score of -inf; pages that are not there are filled
+// with zeros, and in tiles where some row does not see a position that has a page (`careful`),
+// V is checked for values that are not finite (0 x inf).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -31,22 +45,7 @@ int paged_attention_fault_take(int* code) {
     return r;
 }
 
-// ---- 16 rows on mma.sync -----------------------------------------------------------------
-// A warp's 16 query rows against KW positions at a time.  Products of FP32 operands keep about
-// 2^-21:
-//   FP16 pages  q = hi + lo and p = hi + lo in FP16, K and V as they are: two m16n8k16 per
-//               product.  q rows are scaled to a largest element in [256, 512) and p by 2^10,
-//               powers of two that keep the lo parts out of FP16's subnormals.
-//   FP32 pages  both operands as TF32 hi + lo, hi hi + hi lo + lo hi: three m16n8k8, with the
-//               range of FP32.
-// The MMA adds to its FP32 accumulator by cutting, half a unit of the accumulator per step on
-// average and always towards zero: a running sum over a long sequence would drift (2.6e-6 of
-// the result over 131072 positions).  So lo parts have accumulators of their own, and p v of
-// each tile starts from zero and is added to the running sum by FFMA, which rounds and takes
-// the rescaling with it.
-// Positions that a row does not see get a score of -inf; pages that are not there are filled
-// with zeros, and in tiles where some row does not see a position that has a page (`careful`),
-// V is checked for values that are not finite (0 x inf).
+// ---- a warp's 16 rows on mma.sync, for the wide kernel ---------------------------------------
 // One query row into shared memory as hi and lo parts, by one warp.  Returns the factor that
 // turns its scores into base-2 exponents.
 template <bool F32, int HDP>
@@ -82,10 +81,9 @@ __device__ __forceinline__ float stage_q_row(const float* row, int HD, uint8_t* 
     }
 }
 
-// QREG: the q fragments stay in registers.  LD: bytes between K or V rows in shared memory
-// (16 more than a row: the 8 rows of an ldmatrix, and the TF32 V columns, hit distinct banks);
-// QLD: the same for q.
-template <typename KV, int HDP, int KW, bool QREG>
+// LD: bytes between K or V rows in shared memory (16 more than a row: the 8 rows of an ldmatrix,
+// and the TF32 V columns, hit distinct banks); QLD: the same for q.
+template <typename KV, int HDP, int KW>
 struct WarpRows {
     static constexpr bool F32 = sizeof(KV) == 4;
     static constexpr int LD = HDP * (int)sizeof(KV) + 16, QLD = HDP * (F32 ? 4 : 2) + 16;
@@ -97,7 +95,6 @@ struct WarpRows {
     float m[2], l[2];
     int lim[2];     // last positions that rows g and g + 8 see
     float sc[2];
-    uint32_t qh[QREG ? KS : 1][4], ql[QREG ? KS : 1][4];
     uint32_t q_hi, q_lo;  // this lane's fragment addresses
 
     __device__ __forceinline__ void start(uint32_t hi, uint32_t lo) {
@@ -110,10 +107,6 @@ struct WarpRows {
             for (int i = 0; i < 4; ++i) acc[d][i] = 0.f;
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.f;
-        if constexpr (QREG) {
-#pragma unroll
-            for (int k = 0; k < KS; ++k) load_q(k, qh[k], ql[k]);
-        }
     }
 
     __device__ __forceinline__ void load_q(int k, uint32_t (&h)[4], uint32_t (&e)[4]) const {
@@ -136,12 +129,7 @@ struct WarpRows {
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t ah[4], al[4];
-                if constexpr (QREG) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) ah[j] = qh[k][j], al[j] = ql[k][j];
-                } else {
-                    load_q(k, ah, al);
-                }
+                load_q(k, ah, al);
 #pragma unroll
                 for (int n = 0; n < NB; n += 2) {  // 16 positions x 16 dimensions
                     uint32_t b[4];
@@ -724,8 +712,7 @@ struct WideCfg {
     static constexpr int WR = HDP == 256 ? 4 : 8, NT = WR * 32, R = 16 * WR;
     static constexpr int ROWB = HDP * (int)sizeof(KV);
     static constexpr int KT = ROWB <= 128 ? 64 : ROWB <= 512 ? 32 : 16;
-    static constexpr bool QREG = !F32 && HDP <= 128;
-    using Tile = WarpRows<KV, HDP, KT, QREG>;
+    using Tile = WarpRows<KV, HDP, KT>;
     static constexpr int STAGES = ROWB > 256 ? 2 : 4;
     static constexpr int Q_BYTES = 2 * R * Tile::QLD;
     static constexpr int STAGE = 2 * KT * Tile::LD;
@@ -749,7 +736,7 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     pdl_launch_dependents();
     __shared__ Piece sh_piece;
     __shared__ int found;
-    find_pieces<NT, 1, false>(w, A.rule, blockIdx.x, &sh_piece, &found, nullptr);
+    find_piece<NT>(w, A.rule, blockIdx.x, &sh_piece, &found);
     __syncthreads();
     if (!found) return;
     Piece piece = sh_piece;
@@ -847,12 +834,6 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
 }
 
 // ---- joining the parts of a tile ---------------------------------------------------------
-// WPR 0: the tiles were cut by find_pieces -- most are whole, the others in two or three -- and a
-// CTA sees to JOIN_ROWS rows of a tile, a warp to one after another.  Otherwise by find_item:
-// tiles of 8 rows, which can have many parts, and a CTA sees to a tile, WPR warps to a row.  (A
-// CTA to a row took 16 us against 6 on 64 single tokens: each of them plans.)  Two warps keep
-// four CTAs on an SM for many tiles; four get through the parts of a few long ones sooner.
-constexpr int JOIN_ROWS = 64;
 struct JoinArgs {
     PagedView w;
     CutRule rule;
@@ -862,106 +843,133 @@ struct JoinArgs {
     const float2* part_ml;
 };
 
-template <int WPR>
-constexpr int join_threads = WPR == 0 ? 128 : 8 * WPR * 32;
+__device__ __forceinline__ void join_store(const JoinArgs& A, const SeqInfo& s, int hk, int gr, int x4,
+                                           const float4& o, float l) {
+    const int G = A.w.H / A.w.Hkv, tok = (int)A.w.group.div((uint32_t)gr);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float* out = A.out + (int64_t)(s.q0 + tok) * A.out_stride + (int64_t)(hk * G + gr - tok * G) * A.w.HD;
+    reinterpret_cast<float4*>(out)[x4] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
 
+// Tiles of 8 rows that find_item cut, into many parts where they are long: a CTA to a tile, WPR
+// warps to a row.  (A CTA to a row took 16 us against 6 on 64 single tokens: each of them plans.)
+// Two warps keep four CTAs on an SM for many tiles; four get through the parts of a few long
+// ones sooner.
 template <int WPR>
-__global__ void __launch_bounds__(join_threads<WPR>)
-    attn_join_kernel(const __grid_constant__ JoinArgs A) {
-    constexpr bool PIECES = WPR == 0;
-    constexpr int NT = join_threads<WPR>, MAXV = 2;  // float4 per lane: head_dim 256
-    __shared__ float4 sh_acc[PIECES ? 1 : 8 * WPR][32 * MAXV];
-    __shared__ float sh_l[PIECES ? 1 : 8 * WPR];
-    const PagedView& w = A.w;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R;
+__global__ void __launch_bounds__(8 * WPR * 32) join_parts_kernel(const __grid_constant__ JoinArgs A) {
+    constexpr int NT = 8 * WPR * 32, MAXV = 2;  // float4 per lane: head_dim 256
+    __shared__ float4 sh_acc[8 * WPR][32 * MAXV];
+    __shared__ float sh_l[8 * WPR];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = warp / WPR;
+    const int G = A.w.H / A.w.Hkv, HD = A.w.HD;
+    Item it;
     // cu_q and len were complete before the attention kernel started; its partials follow
-    int hk, tile, n_parts, first, rest;  // the first part's place, that of part i > 0 less i * step
-    constexpr int step = PIECES ? 2 : 1;
-    SeqInfo s;
-    if constexpr (PIECES) {
-        __shared__ Piece p;
-        __shared__ long long tile_no;
-        __shared__ int found;
-        find_pieces<NT, 1, true>(w, A.rule, blockIdx.x, &p, &found, &tile_no);
-        __syncthreads();
-        pdl_wait();
-        if (!found) return;
-        s = p.x.s;
-        hk = (int)(tile_no / p.x.tiles), tile = (int)(tile_no - (long long)hk * p.x.tiles);
-        const long long start_g = (long long)G * max(s.L - s.n, 0);
-        const long long a = p.base + hk * p.x.per_head + tiles_work(tile, start_g, R);
-        const long long b = a + start_g + (long long)(tile + 1) * R;
-        // the pieces that hold a share of the tile: the first one's is its last segment (unless
-        // the tile begins with the piece), the others' is their first
-        const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
-        if (c1 >= A.rule.n_pieces) return;
-        n_parts = c1 - c0 + 1;
-        rest = 2 * c0;
-        first = rest + (a == c0 * p.len ? 0 : 1);
-    } else {
-        Item it;
-        const bool any = find_item<NT, true>(w, A.rule, blockIdx.x, it);
-        pdl_wait();
-        if (!any) return;
-        s = it.s;
-        hk = it.hk, tile = it.tile, n_parts = it.n_parts;
-        first = rest = it.part_base;
-    }
-    const int rows = min(R, s.n * G - tile * R);
-    if (n_parts == 1) return;
-    const int r0 = PIECES ? blockIdx.y * JOIN_ROWS + warp : warp / (PIECES ? 1 : WPR);
-    const int r1 = PIECES ? min(rows, (int)(blockIdx.y + 1) * JOIN_ROWS) : r0 + 1;
-    for (int r = r0; r < r1; r += 4) {
-        auto at = [&](int i) { return (int64_t)(i == 0 ? first : rest + i * step) * R + r; };
-        float M = -INFINITY, l = 0.f;
-        float4 o[MAXV];
+    const bool any = find_item<NT, true>(A.w, A.rule, blockIdx.x, it);
+    pdl_wait();
+    if (!any || it.n_parts == 1) return;
+    const bool some = r < it.s.n * G - it.tile * 8;  // the other warps come along to the barrier
+    auto at = [&](int i) { return (int64_t)(it.part_base + i) * 8 + r; };
+    float M = -INFINITY, l = 0.f;
+    float4 o[MAXV];
 #pragma unroll
-        for (int i = 0; i < MAXV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const bool some = PIECES || r < rows;  // the other warps come along to the barrier
-        for (int i = lane; some && i < n_parts; i += 32) M = fmaxf(M, A.part_ml[at(i)].x);
+    for (int i = 0; i < MAXV; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = lane; some && i < it.n_parts; i += 32) M = fmaxf(M, A.part_ml[at(i)].x);
 #pragma unroll
-        for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+    for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
 #pragma unroll 8
-        for (int i = PIECES ? 0 : warp % (PIECES ? 1 : WPR); i < (some ? n_parts : 0);
-             i += PIECES ? 1 : WPR) {
-            const float2 y = A.part_ml[at(i)];
-            const float c = M == -INFINITY ? 1.f : ex2(y.x - M);
-            l += c * y.y;
-            const float4* acc = reinterpret_cast<const float4*>(A.part_acc + at(i) * HD);
+    for (int i = warp % WPR; i < (some ? it.n_parts : 0); i += WPR) {
+        const float2 y = A.part_ml[at(i)];
+        const float c = M == -INFINITY ? 1.f : ex2(y.x - M);
+        l += c * y.y;
+        const float4* acc = reinterpret_cast<const float4*>(A.part_acc + at(i) * HD);
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+            if (lane + 32 * k < HD / 4) {
+                const float4 x = acc[lane + 32 * k];
+                o[k].x += c * x.x, o[k].y += c * x.y, o[k].z += c * x.z, o[k].w += c * x.w;
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < MAXV; ++k) sh_acc[warp][lane + 32 * k] = o[k];
+    if (lane == 0) sh_l[warp] = l;
+    __syncthreads();
+    if (warp % WPR || !some) return;
+#pragma unroll
+    for (int i = 1; i < WPR; ++i) {
+        l += sh_l[warp + i];
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k) {
+            const float4 z = sh_acc[warp + i][lane + 32 * k];
+            o[k].x += z.x, o[k].y += z.y, o[k].z += z.z, o[k].w += z.w;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < MAXV; ++k)
+        if (lane + 32 * k < HD / 4) join_store(A, it.s, it.hk, it.tile * 8 + r, lane + 32 * k, o[k], l);
+}
+
+// Tiles of many rows that find_piece cut, mostly in two: CTA (c, y) looks whether piece c begins
+// inside a tile, and is the first to do so there, and sees to its rows 32 y ...  (A CTA to a tile
+// and 64 rows of it one after another: 36 us against 8 behind a chunk of 2048 tokens.)
+constexpr int JOIN_ROWS = 32, JOIN_THREADS = 256;
+__global__ void __launch_bounds__(JOIN_THREADS) join_pieces_kernel(const __grid_constant__ JoinArgs A) {
+    constexpr int MAXV = 2, RPW = JOIN_ROWS / (JOIN_THREADS / 32);  // rows of a warp, all at once
+    __shared__ Piece sh_piece;
+    __shared__ int found;
+    const PagedView& w = A.w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, no = blockIdx.x;
+    const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R;
+    find_piece<JOIN_THREADS>(w, A.rule, no, &sh_piece, &found);
+    __syncthreads();
+    pdl_wait();
+    if (!found) return;
+    Piece p = sh_piece;
+    Segment sg;
+    if (!next_segment(w, A.rule, p, sg)) return;
+    // the tile's work is [a, b), and pieces c0 .. c1 hold shares of it: the first one's is its last
+    // segment (unless the tile begins with the piece), the others' is their first
+    const long long start_g = (long long)G * max(sg.start, 0);
+    const long long a = p.base + sg.hk * p.x.per_head + tiles_work(sg.tile, start_g, R);
+    const long long b = a + start_g + (long long)(sg.tile + 1) * R;
+    const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
+    if (c0 != no - 1 || c1 >= A.rule.n_pieces) return;
+    const int n_parts = c1 - c0 + 1, first = 2 * c0 + (a == c0 * p.len ? 0 : 1);
+    const int r0 = blockIdx.y * JOIN_ROWS + warp * RPW;
+    auto at = [&](int i, int r) { return (int64_t)(i == 0 ? first : 2 * (c0 + i)) * R + r; };
+    float M[RPW], l[RPW];
+    float4 o[RPW][MAXV];
+#pragma unroll
+    for (int j = 0; j < RPW; ++j) {
+        M[j] = -INFINITY, l[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k) o[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int i = 0; i < n_parts; ++i)
+#pragma unroll
+        for (int j = 0; j < RPW; ++j)
+            if (r0 + j < sg.rows) M[j] = fmaxf(M[j], A.part_ml[at(i, r0 + j)].x);
+    for (int i = 0; i < n_parts; ++i)
+#pragma unroll
+        for (int j = 0; j < RPW; ++j) {
+            if (r0 + j >= sg.rows) continue;
+            const float2 y = A.part_ml[at(i, r0 + j)];
+            const float c = M[j] == -INFINITY ? 1.f : ex2(y.x - M[j]);
+            l[j] += c * y.y;
+            const float4* acc = reinterpret_cast<const float4*>(A.part_acc + at(i, r0 + j) * HD);
 #pragma unroll
             for (int k = 0; k < MAXV; ++k)
                 if (lane + 32 * k < HD / 4) {
                     const float4 x = acc[lane + 32 * k];
-                    o[k].x += c * x.x, o[k].y += c * x.y, o[k].z += c * x.z, o[k].w += c * x.w;
+                    o[j][k].x += c * x.x, o[j][k].y += c * x.y;
+                    o[j][k].z += c * x.z, o[j][k].w += c * x.w;
                 }
         }
-        if constexpr (!PIECES) {
 #pragma unroll
-            for (int k = 0; k < MAXV; ++k) sh_acc[warp][lane + 32 * k] = o[k];
-            if (lane == 0) sh_l[warp] = l;
-            __syncthreads();
-            if (warp % WPR || !some) return;
-#pragma unroll
-            for (int i = 1; i < WPR; ++i) {
-                l += sh_l[warp + i];
-#pragma unroll
-                for (int k = 0; k < MAXV; ++k) {
-                    const float4 z = sh_acc[warp + i][lane + 32 * k];
-                    o[k].x += z.x, o[k].y += z.y, o[k].z += z.z, o[k].w += z.w;
-                }
-            }
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int gr = tile * R + r, tok = gr / G;
-        float4* out = reinterpret_cast<float4*>(A.out + (int64_t)(s.q0 + tok) * A.out_stride +
-                                                (int64_t)(hk * G + gr - tok * G) * HD);
+    for (int j = 0; j < RPW; ++j)
 #pragma unroll
         for (int k = 0; k < MAXV; ++k)
-            if (lane + 32 * k < HD / 4)
-                out[lane + 32 * k] =
-                    make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
-    }
+            if (r0 + j < sg.rows && lane + 32 * k < HD / 4)
+                join_store(A, sg.s, sg.hk, sg.row0 + r0 + j, lane + 32 * k, o[j][k], l[j]);
 }
 
 // ---- launches ----------------------------------------------------------------------------
@@ -1011,8 +1019,9 @@ static int rows_launch(int threads, size_t smem, bool pieces, const RowsArgs& a,
 
 // The kernels of a call, by the rows (new tokens x group) that a sequence may have: up to
 // NARROW_ROWS in tiles of eight on the narrow kernel, more on the wide one, by the caller's bound
-// one of them alone.  32 sequences over 200..4096 positions (32 heads on 8, FP16), narrow against
-// wide: with 4 tokens, 16 rows, 105 us against 150; with 8 tokens 174 against 214.
+// one of them alone.  32 sequences over 200..4096 positions (32 heads on 8, head_dim 128, FP16),
+// narrow against tcgen05: with 16 rows 101 us against 197, with 32 rows 167 against 215, with 64
+// rows 316 against 253 (the sequences' rows fill half of one of its two query tiles).
 constexpr int NARROW_ROWS = 32;
 
 // FP16 pages with head_dim up to 128 have all wide tiles on tcgen05.
@@ -1079,18 +1088,16 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         // no tile is cut into parts where the tables' rows are no longer than the least part
         if (wide || max_pos > s.rule.least) {
             const JoinArgs j{a.w, s.rule, a.out, a.out_stride, a.part_acc, a.part_ml};
-            const int64_t most_rows = std::min<int64_t>(s.rule.R, (int64_t)b->n_tokens * (a.w.H / a.w.Hkv));
-            const unsigned tiles = (unsigned)s.tiles;
-            if (wide)
-                IB_CUDA_CHECK(launch_pdl(attn_join_kernel<0>,
-                                         dim3(tiles, (unsigned)((most_rows + JOIN_ROWS - 1) / JOIN_ROWS)),
-                                         dim3(join_threads<0>), 0, st, true, j));
-            else if (s.tiles <= kSMs)
-                IB_CUDA_CHECK(launch_pdl(attn_join_kernel<4>, dim3(tiles), dim3(join_threads<4>), 0, st,
-                                         true, j));
-            else
-                IB_CUDA_CHECK(launch_pdl(attn_join_kernel<2>, dim3(tiles), dim3(join_threads<2>), 0, st,
-                                         true, j));
+            if (wide) {
+                const dim3 grid((unsigned)s.rule.n_pieces, (unsigned)(s.rule.R / JOIN_ROWS));
+                IB_CUDA_CHECK(launch_pdl(join_pieces_kernel, grid, dim3(JOIN_THREADS), 0, st, true, j));
+            } else if (s.tiles <= kSMs) {
+                IB_CUDA_CHECK(launch_pdl(join_parts_kernel<4>, dim3((unsigned)s.tiles), dim3(8 * 4 * 32), 0,
+                                         st, true, j));
+            } else {
+                IB_CUDA_CHECK(launch_pdl(join_parts_kernel<2>, dim3((unsigned)s.tiles), dim3(8 * 2 * 32), 0,
+                                         st, true, j));
+            }
         }
     }
     return IB_OK;

@@ -62,12 +62,11 @@ struct Piece {
     SeqWork x;
 };
 
-// The NP pieces from number `first` on: out[i] (shared memory) is piece first + i, found[i]
-// whether there is one.  BY_TILE: `first` counts tiles over all heads instead, and tile_no is
-// the tile's number in its sequence.  Every thread of the CTA (NT of them) calls it.
-template <int NT, int NP, bool BY_TILE>
-__device__ __forceinline__ void find_pieces(const PagedView& w, const CutRule& rule, long long first,
-                                            Piece* out, int* found, long long* tile_no) {
+// Piece `no` of the batch, into shared memory; found: whether there is one.  Every thread of the
+// CTA (NT of them) calls it; a barrier has to follow.
+template <int NT>
+__device__ __forceinline__ void find_piece(const PagedView& w, const CutRule& rule, int no, Piece* out,
+                                           int* found) {
     __shared__ long long sh_sum[NT / 32][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     SeqWork x0{};
@@ -84,7 +83,7 @@ __device__ __forceinline__ void find_pieces(const PagedView& w, const CutRule& r
         tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
     }
     if (lane == 0) sh_sum[warp][0] = work, sh_sum[warp][1] = tokens;
-    if (tid < NP) found[tid] = 0;
+    if (tid == 0) *found = 0;
     __syncthreads();
     work = tokens = 0;
 #pragma unroll
@@ -98,48 +97,36 @@ __device__ __forceinline__ void find_pieces(const PagedView& w, const CutRule& r
     }
     const long long len = max((work + rule.n_pieces - 1) / rule.n_pieces,
                               (long long)rule.least * (w.H / w.Hkv));
-    __syncthreads();
-    if (!BY_TILE && first * len >= work) return;
-    long long work_before = 0, tiles_before = 0;
+    const long long want = no * len;
+    if (want >= work) return;
+    long long before = 0;
     for (int b0 = 0; b0 < w.n_seqs; b0 += NT) {
         const int b = b0 + tid;
         SeqWork x = x0;
         if (b0 > 0 && b < w.n_seqs) x = seq_work(w, rule, b);
-        if (b >= w.n_seqs) x.tiles = 0, x.all = 0;
-        const long long n_tiles = (long long)x.tiles * w.Hkv;
-        long long a = x.all, t = n_tiles;  // inclusive sums
+        if (b >= w.n_seqs) x.all = 0;
+        long long a = x.all;  // inclusive sum
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long ya = __shfl_up_sync(0xffffffffu, a, o);
-            const long long yt = __shfl_up_sync(0xffffffffu, t, o);
-            if (lane >= o) a = add_work(a, ya), t += yt;
+            const long long y = __shfl_up_sync(0xffffffffu, a, o);
+            if (lane >= o) a = add_work(a, y);
         }
-        if (lane == 31) sh_sum[warp][0] = a, sh_sum[warp][1] = t;
+        __syncthreads();  // sh_sum has been read
+        if (lane == 31) sh_sum[warp][0] = a;
         __syncthreads();
-        long long sa = 0, st = 0;
+        long long all = 0;
 #pragma unroll
         for (int i = 0; i < NT / 32; ++i) {
-            if (i == warp) a = add_work(a, sa), t += st;
-            sa = add_work(sa, sh_sum[i][0]), st += sh_sum[i][1];
+            if (i == warp) a = add_work(a, all);
+            all = add_work(all, sh_sum[i][0]);
         }
-        const long long a0 = add_work(work_before, a - x.all);
-        const long long t0 = tiles_before + (t - n_tiles);
-        bool last = false;  // the last piece of these, or of all, begins in what was seen
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const long long want = BY_TILE ? first : (first + i) * len;
-            if (BY_TILE ? want >= t0 && want < t0 + n_tiles
-                        : want < work && want >= a0 && want < a0 + x.all) {
-                out[i] = Piece{want, min(work, want + len), len, a0, b, (int)first + i, x};
-                if (BY_TILE) *tile_no = want - t0;
-                found[i] = 1;
-            }
-            last = BY_TILE ? want < tiles_before + st : min(want, work - 1) < work_before + sa;
+        const long long a0 = add_work(before, a - x.all);
+        if (want >= a0 && want < a0 + x.all) {
+            *out = Piece{want, min(work, want + len), len, a0, b, no, x};
+            *found = 1;
         }
-        work_before = add_work(work_before, sa);
-        tiles_before += st;
-        __syncthreads();
-        if (last) break;  // the same for every thread
+        before = add_work(before, all);
+        if (want < before) break;  // the same for every thread
     }
 }
 

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_launch_dependents();
-    find_pieces<PT_THREADS, 1, false>(w, A.rule, blockIdx.x, sh_piece, &found, nullptr);
+    find_piece<PT_THREADS>(w, A.rule, blockIdx.x, sh_piece, &found);
     __syncthreads();
     if (!found) return;
     if (tid > 0 && tid < PT_THREADS / 32) sh_piece[tid] = sh_piece[0];
