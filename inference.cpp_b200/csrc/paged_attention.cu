@@ -732,13 +732,16 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     __shared__ float row_scale[R];
     const PagedView& w = A.w;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
-    pdl_wait();
+    if (!A.beside) pdl_wait();
     pdl_launch_dependents();
     __shared__ Piece sh_piece;
     __shared__ int found;
     find_piece<NT>(w, A.rule, blockIdx.x, &sh_piece, &found);
     __syncthreads();
-    if (!found) return;
+    if (!found) {
+        if (A.beside) pdl_wait();
+        return;
+    }
     Piece piece = sh_piece;
     Segment it;
     const int G = w.H / w.Hkv, HD = w.HD;
@@ -831,6 +834,7 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();  // the ring and q are free for the next segment
     }
+    if (A.beside) pdl_wait();
 }
 
 // ---- joining the parts of a tile ---------------------------------------------------------
@@ -909,15 +913,18 @@ __global__ void __launch_bounds__(8 * WPR * 32) join_parts_kernel(const __grid_c
 }
 
 // Tiles of many rows that find_piece cut, mostly in two: CTA (c, y) looks whether piece c begins
-// inside a tile, and is the first to do so there, and sees to its rows 32 y ...  (A CTA to a tile
-// and 64 rows of it one after another: 36 us against 8 behind a chunk of 2048 tokens.)
-constexpr int JOIN_ROWS = 32, JOIN_THREADS = 256;
-__global__ void __launch_bounds__(JOIN_THREADS) join_pieces_kernel(const __grid_constant__ JoinArgs A) {
-    constexpr int MAXV = 2, RPW = JOIN_ROWS / (JOIN_THREADS / 32);  // rows of a warp, all at once
+// inside a tile, and is the first to do so there, and sees to its rows JOIN_ROWS y ...  All CTAs
+// are on the SMs at once, since each has to plan first.
+constexpr int JOIN_ROWS = 128, JOIN_THREADS = 512;
+template <int HDP>
+__global__ void __launch_bounds__(JOIN_THREADS, 2)
+    join_pieces_kernel(const __grid_constant__ JoinArgs A) {
+    constexpr int LPR = HDP / 4 < 32 ? HDP / 4 : 32, V = HDP / 4 / LPR;  // lanes of a row, float4 of a lane
+    constexpr int U = V == 1 ? 4 : 2;                                    // rows of a lane at once
     __shared__ Piece sh_piece;
     __shared__ int found;
     const PagedView& w = A.w;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, no = blockIdx.x;
+    const int tid = threadIdx.x, no = blockIdx.x;
     const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R;
     find_piece<JOIN_THREADS>(w, A.rule, no, &sh_piece, &found);
     __syncthreads();
@@ -934,42 +941,53 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_pieces_kernel(const __grid_
     const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
     if (c0 != no - 1 || c1 >= A.rule.n_pieces) return;
     const int n_parts = c1 - c0 + 1, first = 2 * c0 + (a == c0 * p.len ? 0 : 1);
-    const int r0 = blockIdx.y * JOIN_ROWS + warp * RPW;
-    auto at = [&](int i, int r) { return (int64_t)(i == 0 ? first : 2 * (c0 + i)) * R + r; };
-    float M[RPW], l[RPW];
-    float4 o[RPW][MAXV];
+    const int x = tid % LPR, end = min(sg.rows, (int)(blockIdx.y + 1) * JOIN_ROWS);
+    constexpr int STEP = JOIN_THREADS / LPR;
+    for (int r0 = blockIdx.y * JOIN_ROWS + tid / LPR; r0 < end; r0 += U * STEP) {
+        float M[U], l[U];
+        float4 o[U][V];
 #pragma unroll
-    for (int j = 0; j < RPW; ++j) {
-        M[j] = -INFINITY, l[j] = 0.f;
+        for (int j = 0; j < U; ++j) {
+            M[j] = -INFINITY, l[j] = 0.f;
 #pragma unroll
-        for (int k = 0; k < MAXV; ++k) o[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    for (int i = 0; i < n_parts; ++i)
+            for (int k = 0; k < V; ++k) o[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll 2
+        for (int i = 0; i < n_parts; ++i) {
+            const int64_t at = (int64_t)(i == 0 ? first : 2 * (c0 + i)) * R;
+            float2 ml[U];
+            float4 y[U][V];
 #pragma unroll
-        for (int j = 0; j < RPW; ++j)
-            if (r0 + j < sg.rows) M[j] = fmaxf(M[j], A.part_ml[at(i, r0 + j)].x);
-    for (int i = 0; i < n_parts; ++i)
+            for (int j = 0; j < U; ++j) {
+                const int r = r0 + j * STEP;
+                ml[j] = r < end ? A.part_ml[at + r] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int j = 0; j < RPW; ++j) {
-            if (r0 + j >= sg.rows) continue;
-            const float2 y = A.part_ml[at(i, r0 + j)];
-            const float c = M[j] == -INFINITY ? 1.f : ex2(y.x - M[j]);
-            l[j] += c * y.y;
-            const float4* acc = reinterpret_cast<const float4*>(A.part_acc + at(i, r0 + j) * HD);
+                for (int k = 0; k < V; ++k)
+                    y[j][k] = r < end && x + LPR * k < HD / 4
+                                  ? reinterpret_cast<const float4*>(A.part_acc + (at + r) * HD)[x + LPR * k]
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
 #pragma unroll
-            for (int k = 0; k < MAXV; ++k)
-                if (lane + 32 * k < HD / 4) {
-                    const float4 x = acc[lane + 32 * k];
-                    o[j][k].x += c * x.x, o[j][k].y += c * x.y;
-                    o[j][k].z += c * x.z, o[j][k].w += c * x.w;
+            for (int j = 0; j < U; ++j) {
+                const float top = fmaxf(M[j], ml[j].x);
+                const float f = top == -INFINITY ? 1.f : ex2(M[j] - top);
+                const float c = top == -INFINITY ? 1.f : ex2(ml[j].x - top);
+                M[j] = top;
+                l[j] = fmaf(l[j], f, c * ml[j].y);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    o[j][k].x = fmaf(o[j][k].x, f, c * y[j][k].x), o[j][k].y = fmaf(o[j][k].y, f, c * y[j][k].y);
+                    o[j][k].z = fmaf(o[j][k].z, f, c * y[j][k].z), o[j][k].w = fmaf(o[j][k].w, f, c * y[j][k].w);
                 }
+            }
         }
 #pragma unroll
-    for (int j = 0; j < RPW; ++j)
+        for (int j = 0; j < U; ++j)
 #pragma unroll
-        for (int k = 0; k < MAXV; ++k)
-            if (r0 + j < sg.rows && lane + 32 * k < HD / 4)
-                join_store(A, sg.s, sg.hk, sg.row0 + r0 + j, lane + 32 * k, o[j][k], l[j]);
+            for (int k = 0; k < V; ++k)
+                if (r0 + j * STEP < end && x + LPR * k < HD / 4)
+                    join_store(A, sg.s, sg.hk, sg.row0 + r0 + j * STEP, x + LPR * k, o[j][k], l[j]);
+    }
 }
 
 // ---- launches ----------------------------------------------------------------------------
@@ -1073,6 +1091,7 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         const Share& s = plan.share[i];
         a.rule = s.rule;
         const bool wide = s.rule.R > 8;
+        a.beside = i > 0;
         a.part_acc = reinterpret_cast<float*>(ws + s.acc_off);
         a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
         int r = IB_OK;
@@ -1085,12 +1104,17 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
             r = rows_launch<attn_wide_kernel<KV, HDP>>(W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
         }
         if (r != IB_OK) return r;
+    }
+    for (int i = 0; i < plan.n; ++i) {
+        const Share& s = plan.share[i];
+        const bool wide = s.rule.R > 8;
         // no tile is cut into parts where the tables' rows are no longer than the least part
         if (wide || max_pos > s.rule.least) {
-            const JoinArgs j{a.w, s.rule, a.out, a.out_stride, a.part_acc, a.part_ml};
+            const JoinArgs j{a.w, s.rule, a.out, a.out_stride, reinterpret_cast<float*>(ws + s.acc_off),
+                             reinterpret_cast<float2*>(ws + s.ml_off)};
             if (wide) {
-                const dim3 grid((unsigned)s.rule.n_pieces, (unsigned)(s.rule.R / JOIN_ROWS));
-                IB_CUDA_CHECK(launch_pdl(join_pieces_kernel, grid, dim3(JOIN_THREADS), 0, st, true, j));
+                const dim3 grid((unsigned)s.rule.n_pieces, (unsigned)((s.rule.R + JOIN_ROWS - 1) / JOIN_ROWS));
+                IB_CUDA_CHECK(launch_pdl(join_pieces_kernel<HDP>, grid, dim3(JOIN_THREADS), 0, st, true, j));
             } else if (s.tiles <= kSMs) {
                 IB_CUDA_CHECK(launch_pdl(join_parts_kernel<4>, dim3((unsigned)s.tiles), dim3(8 * 4 * 32), 0,
                                          st, true, j));

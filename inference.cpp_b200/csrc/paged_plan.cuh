@@ -307,6 +307,11 @@ struct RowsArgs {
     float* part_acc;    // [partial][R][HD]
     float2* part_ml;    // [partial][R]
     float scale_log2;   // scale * log2(e)
+    // The kernel before is the call's narrow one, which writes other rows and workspace: this one
+    // starts beside its last CTAs and waits for it at its own end only, so that what follows
+    // finds both complete.  (The narrow kernel lets it start after its own wait for what came
+    // before the call.)
+    bool beside;
 };
 
 // Row `gr` of the segment's sequence and kv head.

@@ -268,11 +268,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     __shared__ uint32_t sh_bad32[4][3][2];  // the same for FP32, of each of the three warps
     const PagedView& w = A.w;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_wait();
+    if (!A.beside) pdl_wait();
     pdl_launch_dependents();
     find_piece<PT_THREADS>(w, A.rule, blockIdx.x, sh_piece, &found);
     __syncthreads();
-    if (!found) return;
+    if (!found) {
+        if (A.beside) pdl_wait();
+        return;
+    }
     if (tid > 0 && tid < PT_THREADS / 32) sh_piece[tid] = sh_piece[0];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -935,6 +938,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
                      : "memory");
     }
+    if (A.beside) pdl_wait();
 }
 
 // The layer's rows as a tensor [rows][head_dim]: FP16 in swizzled boxes of 64 columns, FP32 in
