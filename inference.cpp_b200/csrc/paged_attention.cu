@@ -860,7 +860,7 @@ __device__ __forceinline__ void join_store(const JoinArgs& A, const SeqInfo& s, 
 // Two warps keep four CTAs on an SM for many tiles; four get through the parts of a few long
 // ones sooner.
 template <int WPR>
-__global__ void __launch_bounds__(8 * WPR * 32) join_parts_kernel(const __grid_constant__ JoinArgs A) {
+__device__ __forceinline__ void join_parts(const JoinArgs& A, int item) {
     constexpr int NT = 8 * WPR * 32, MAXV = 2;  // float4 per lane: head_dim 256
     __shared__ float4 sh_acc[8 * WPR][32 * MAXV];
     __shared__ float sh_l[8 * WPR];
@@ -868,7 +868,7 @@ __global__ void __launch_bounds__(8 * WPR * 32) join_parts_kernel(const __grid_c
     const int G = A.w.H / A.w.Hkv, HD = A.w.HD;
     Item it;
     // cu_q and len were complete before the attention kernel started; its partials follow
-    const bool any = find_item<NT, true>(A.w, A.rule, blockIdx.x, it);
+    const bool any = find_item<NT, true>(A.w, A.rule, item, it);
     pdl_wait();
     if (!any || it.n_parts == 1) return;
     const bool some = r < it.s.n * G - it.tile * 8;  // the other warps come along to the barrier
@@ -912,19 +912,19 @@ __global__ void __launch_bounds__(8 * WPR * 32) join_parts_kernel(const __grid_c
         if (lane + 32 * k < HD / 4) join_store(A, it.s, it.hk, it.tile * 8 + r, lane + 32 * k, o[k], l);
 }
 
-// Tiles of many rows that find_piece cut, mostly in two: CTA (c, y) looks whether piece c begins
-// inside a tile, and is the first to do so there, and sees to its rows JOIN_ROWS y ...  All CTAs
-// are on the SMs at once, since each has to plan first.
+// Tiles of many rows that find_piece cut, mostly in two: CTA (no, y) looks whether piece `no`
+// begins inside a tile, and is the first to do so there, and sees to its rows JOIN_ROWS y ...
+// All CTAs are on the SMs at once, since each has to plan first: with 32 rows to a CTA, four times
+// as many of them, the join behind a chunk of 2048 tokens took 36 us against 22 (cold caches).
 constexpr int JOIN_ROWS = 128, JOIN_THREADS = 512;
 template <int HDP>
-__global__ void __launch_bounds__(JOIN_THREADS, 2)
-    join_pieces_kernel(const __grid_constant__ JoinArgs A) {
+__device__ __forceinline__ void join_pieces(const JoinArgs& A, int no, int y) {
     constexpr int LPR = HDP / 4 < 32 ? HDP / 4 : 32, V = HDP / 4 / LPR;  // lanes of a row, float4 of a lane
     constexpr int U = V == 1 ? 4 : 2;                                    // rows of a lane at once
     __shared__ Piece sh_piece;
     __shared__ int found;
     const PagedView& w = A.w;
-    const int tid = threadIdx.x, no = blockIdx.x;
+    const int tid = threadIdx.x;
     const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R;
     find_piece<JOIN_THREADS>(w, A.rule, no, &sh_piece, &found);
     __syncthreads();
@@ -941,9 +941,9 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2)
     const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
     if (c0 != no - 1 || c1 >= A.rule.n_pieces) return;
     const int n_parts = c1 - c0 + 1, first = 2 * c0 + (a == c0 * p.len ? 0 : 1);
-    const int x = tid % LPR, end = min(sg.rows, (int)(blockIdx.y + 1) * JOIN_ROWS);
+    const int x = tid % LPR, end = min(sg.rows, (y + 1) * JOIN_ROWS);
     constexpr int STEP = JOIN_THREADS / LPR;
-    for (int r0 = blockIdx.y * JOIN_ROWS + tid / LPR; r0 < end; r0 += U * STEP) {
+    for (int r0 = y * JOIN_ROWS + tid / LPR; r0 < end; r0 += U * STEP) {
         float M[U], l[U];
         float4 o[U][V];
 #pragma unroll
@@ -956,14 +956,14 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2)
         for (int i = 0; i < n_parts; ++i) {
             const int64_t at = (int64_t)(i == 0 ? first : 2 * (c0 + i)) * R;
             float2 ml[U];
-            float4 y[U][V];
+            float4 v[U][V];
 #pragma unroll
             for (int j = 0; j < U; ++j) {
                 const int r = r0 + j * STEP;
                 ml[j] = r < end ? A.part_ml[at + r] : make_float2(-INFINITY, 0.f);
 #pragma unroll
                 for (int k = 0; k < V; ++k)
-                    y[j][k] = r < end && x + LPR * k < HD / 4
+                    v[j][k] = r < end && x + LPR * k < HD / 4
                                   ? reinterpret_cast<const float4*>(A.part_acc + (at + r) * HD)[x + LPR * k]
                                   : make_float4(0.f, 0.f, 0.f, 0.f);
             }
@@ -976,8 +976,8 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2)
                 l[j] = fmaf(l[j], f, c * ml[j].y);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    o[j][k].x = fmaf(o[j][k].x, f, c * y[j][k].x), o[j][k].y = fmaf(o[j][k].y, f, c * y[j][k].y);
-                    o[j][k].z = fmaf(o[j][k].z, f, c * y[j][k].z), o[j][k].w = fmaf(o[j][k].w, f, c * y[j][k].w);
+                    o[j][k].x = fmaf(o[j][k].x, f, c * v[j][k].x), o[j][k].y = fmaf(o[j][k].y, f, c * v[j][k].y);
+                    o[j][k].z = fmaf(o[j][k].z, f, c * v[j][k].z), o[j][k].w = fmaf(o[j][k].w, f, c * v[j][k].w);
                 }
             }
         }
@@ -988,6 +988,25 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2)
                 if (r0 + j * STEP < end && x + LPR * k < HD / 4)
                     join_store(A, sg.s, sg.hk, sg.row0 + r0 + j * STEP, x + LPR * k, o[j][k], l[j]);
     }
+}
+
+template <int WPR>
+__global__ void __launch_bounds__(8 * WPR * 32) join_parts_kernel(const __grid_constant__ JoinArgs A) {
+    join_parts<WPR>(A, blockIdx.x);
+}
+template <int HDP>
+__global__ void __launch_bounds__(JOIN_THREADS, 2)
+    join_pieces_kernel(const __grid_constant__ JoinArgs A) {
+    join_pieces<HDP>(A, blockIdx.x, blockIdx.y);
+}
+// Both in one launch, the pieces first.
+template <int HDP>
+__global__ void __launch_bounds__(JOIN_THREADS, 2)
+    join_both_kernel(const __grid_constant__ JoinArgs parts, const __grid_constant__ JoinArgs pieces) {
+    constexpr int WPR = JOIN_THREADS / 256;
+    const int n = pieces.rule.n_pieces, y = blockIdx.x / n;
+    if (y * JOIN_ROWS < pieces.rule.R) join_pieces<HDP>(pieces, blockIdx.x - y * n, y);
+    else join_parts<WPR>(parts, blockIdx.x - (pieces.rule.R + JOIN_ROWS - 1) / JOIN_ROWS * n);
 }
 
 // ---- launches ----------------------------------------------------------------------------
@@ -1105,25 +1124,34 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         }
         if (r != IB_OK) return r;
     }
+    JoinArgs parts{}, pieces{};
+    int64_t n_parts = 0, n_pieces = 0;  // CTAs
     for (int i = 0; i < plan.n; ++i) {
         const Share& s = plan.share[i];
-        const bool wide = s.rule.R > 8;
-        // no tile is cut into parts where the tables' rows are no longer than the least part
-        if (wide || max_pos > s.rule.least) {
-            const JoinArgs j{a.w, s.rule, a.out, a.out_stride, reinterpret_cast<float*>(ws + s.acc_off),
-                             reinterpret_cast<float2*>(ws + s.ml_off)};
-            if (wide) {
-                const dim3 grid((unsigned)s.rule.n_pieces, (unsigned)((s.rule.R + JOIN_ROWS - 1) / JOIN_ROWS));
-                IB_CUDA_CHECK(launch_pdl(join_pieces_kernel<HDP>, grid, dim3(JOIN_THREADS), 0, st, true, j));
-            } else if (s.tiles <= kSMs) {
-                IB_CUDA_CHECK(launch_pdl(join_parts_kernel<4>, dim3((unsigned)s.tiles), dim3(8 * 4 * 32), 0,
-                                         st, true, j));
-            } else {
-                IB_CUDA_CHECK(launch_pdl(join_parts_kernel<2>, dim3((unsigned)s.tiles), dim3(8 * 2 * 32), 0,
-                                         st, true, j));
-            }
+        const JoinArgs j{a.w, s.rule, a.out, a.out_stride, reinterpret_cast<float*>(ws + s.acc_off),
+                         reinterpret_cast<float2*>(ws + s.ml_off)};
+        if (s.rule.R > 8) {
+            pieces = j;
+            n_pieces = (int64_t)s.rule.n_pieces * ((s.rule.R + JOIN_ROWS - 1) / JOIN_ROWS);
+        } else if (max_pos > s.rule.least) {
+            // (no tile is cut into parts where the tables' rows are no longer than the least part)
+            parts = j;
+            n_parts = s.tiles;
         }
     }
+    const unsigned rounds = n_pieces ? (unsigned)(n_pieces / pieces.rule.n_pieces) : 0;
+    if (n_parts && n_pieces)
+        IB_CUDA_CHECK(launch_pdl(join_both_kernel<HDP>, dim3((unsigned)(n_pieces + n_parts)),
+                                 dim3(JOIN_THREADS), 0, st, true, parts, pieces));
+    else if (n_pieces)
+        IB_CUDA_CHECK(launch_pdl(join_pieces_kernel<HDP>, dim3((unsigned)pieces.rule.n_pieces, rounds),
+                                 dim3(JOIN_THREADS), 0, st, true, pieces));
+    else if (n_parts && n_parts <= kSMs)
+        IB_CUDA_CHECK(launch_pdl(join_parts_kernel<4>, dim3((unsigned)n_parts), dim3(8 * 4 * 32), 0, st,
+                                 true, parts));
+    else if (n_parts)
+        IB_CUDA_CHECK(launch_pdl(join_parts_kernel<2>, dim3((unsigned)n_parts), dim3(8 * 2 * 32), 0, st,
+                                 true, parts));
     return IB_OK;
 }
 
