@@ -310,7 +310,7 @@ int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_b
  * sees positions 0 .. len - n + i whose pages are there.  A row that sees none is 0.  Same
  * result contract as ib_attention_batch (softmax of scale * q.k, grouped heads).  q and out
  * [n_tokens][n_heads][head_dim] FP32, rows q_stride / out_stride elements apart (multiples
- * of 4, 16-byte aligned).  A NaN or infinity in a position that a row does not see leaves the
+ * of 4, 16-byte aligned); out may be q itself.  A NaN or infinity in a position that a row does not see leaves the
  * row alone; in one that it sees, the row's outputs are not specified (NaN, as a rule).
  * workspace: ib_attention_paged_workspace(...) bytes, 256-byte aligned, that no other call
  * uses at the same time; it needs no initial value. */

@@ -14,6 +14,7 @@ The directory name is not a Python identifier; load it with
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -625,6 +626,16 @@ def _paged_stream(pages, stream, *others):
     return (_raw_stream()(index) or None) if stream is None else stream
 
 
+def _allocating(pages, stream):
+    """Context for the tensors that a call makes: of the launch stream's memory pool, where they
+    may be handed out again, in stream order, once they are dropped."""
+    if stream is None:
+        return contextlib.nullcontext()
+    cuda = _torch().cuda
+    return cuda.stream(cuda.ExternalStream(stream, pages.device) if stream else
+                       cuda.default_stream(pages.device))
+
+
 def _seqs_of(pages, seqs):
     if seqs.n_refs != pages.n_pages:
         raise ValueError(f"refs: {seqs.n_refs} entries for {pages.n_pages} pages")
@@ -647,7 +658,8 @@ def kv_extend(pages, seqs, slots, n_new, status=None, stream=None):
     """Room for n_new[i] more tokens of each slot; returns status (1 done, 0 no room,
     -1 refused), int32 tensors on the pages' device."""
     if status is None:
-        status = _torch().empty_like(slots)
+        with _allocating(pages, stream):
+            status = _torch().empty_like(slots)
     n = slots.numel()
     a, b, c = (_paged_list(pages, slots, "slots", n), _paged_list(pages, n_new, "n_new", n),
                _paged_list(pages, status, "status", n))
@@ -659,7 +671,8 @@ def kv_extend(pages, seqs, slots, n_new, status=None, stream=None):
 def kv_fork(pages, seqs, parents, children, status=None, stream=None):
     """children[i] becomes a copy of parents[i], sharing its whole pages; returns status."""
     if status is None:
-        status = _torch().empty_like(parents)
+        with _allocating(pages, stream):
+            status = _torch().empty_like(parents)
     n = parents.numel()
     a, b, c = (_paged_list(pages, parents, "parents", n),
                _paged_list(pages, children, "children", n),
@@ -699,7 +712,9 @@ def kv_compact(pages, seqs, out=None, plan=None, stream=None):
     """Moves the used pages to the lowest indices; the renamed table and refs go to `out` (a
     KVSeqs; default: seqs itself).  Returns the plan."""
     out = seqs if out is None else out
-    plan = KVCompactPlan(pages) if plan is None else plan
+    if plan is None:
+        with _allocating(pages, stream):
+            plan = KVCompactPlan(pages)
     st = _paged_stream(pages, stream, seqs, out, plan)
     if out.table.shape != seqs.table.shape or plan.n_pages != pages.n_pages:
         raise ValueError("out or plan of another cache")
@@ -734,7 +749,8 @@ def kv_append(pages, seqs, batch, layer, q, k, v, rope_table, q_out=None, stream
     torch = _torch()
     T, HD, Hkv, dev = batch.n_tokens, pages.head_dim, pages.n_kv_heads, pages.device
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=torch.float32, device=dev)
+        with _allocating(pages, stream):
+            q_out = torch.empty(q.shape, dtype=torch.float32, device=dev)
     qp, qs, H = _paged_rows(q, "q", T, None, HD, dev)
     kp, ks, _ = _paged_rows(k, "k", T, Hkv, HD, dev)
     vp, vs, _ = _paged_rows(v, "v", T, Hkv, HD, dev)
@@ -764,14 +780,12 @@ def attention_paged(pages, seqs, batch, layer, q, scale, out=None, workspace=Non
     T, HD, dev = batch.n_tokens, pages.head_dim, pages.device
     qp, qs, H = _paged_rows(q, "q", T, None, HD, dev)
     if out is None:
-        out = torch.zeros(q.shape, dtype=torch.float32, device=dev)
+        with _allocating(pages, stream):
+            out = torch.zeros(q.shape, dtype=torch.float32, device=dev)
     op, os_, _ = _paged_rows(out, "out", T, H, HD, dev)
     st = _paged_stream(pages, stream, seqs, batch)
     if workspace is None:
-        # of the launch stream's memory pool: it may be handed out again, in stream order,
-        # as soon as the call returns
-        with torch.cuda.stream(torch.cuda.ExternalStream(st, dev) if st else
-                               torch.cuda.default_stream(dev)):
+        with _allocating(pages, stream):
             workspace = attention_paged_workspace(pages, seqs, batch, H)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise ValueError(f"workspace: on {workspace.device}, expected contiguous on {dev}")

@@ -497,7 +497,7 @@ def attention_ref(cuda, pages, layer, table, slots, cu, q_lens, ctx, q, scale):
 
 
 def run_attention(cuda, type_, H, Hkv, HD, page, q_lens, ctx, pad=0, with_slots=True, holes=0.0,
-                  seed=0, spoil=False, max_q=None, q_size=1.5):
+                  seed=0, spoil=False, max_q=None, q_size=1.5, scale=None):
     rng = random.Random(seed + HD * 7 + page)
     seqs, batch, table, slots, n_pages, cu = make(cuda, rng, page, q_lens, ctx, pad, with_slots)
     pages = pool(cuda, 2, n_pages, Hkv, page, HD, type_, seed + 1)
@@ -520,7 +520,7 @@ def run_attention(cuda, type_, H, Hkv, HD, page, q_lens, ctx, pad=0, with_slots=
             x.copy_(cuda.where(held[None, :, None, :, None], x, fill))
     T = batch.n_tokens
     gen = cuda.Generator(device="cuda").manual_seed(seed + 2)
-    scale = 1.0 / math.sqrt(HD)
+    scale = 1.0 / math.sqrt(HD) if scale is None else scale
     buf = q_size * cuda.randn(T, H + 2 * Hkv, HD, generator=gen, device="cuda")
     q = buf[:, :H]  # rows apart
     obuf = cuda.full((T, H + 1, HD), 3.0, device="cuda")
@@ -719,6 +719,96 @@ def test_attention_on_two_streams_at_once(cuda):
     cuda.cuda.synchronize()
     for i, job in enumerate(jobs):
         assert all(cuda.equal(o, job[4]) for o in outs[i])
+
+
+@TYPES
+@pytest.mark.parametrize("n,H,Hkv,HD", [(700, 4, 1, 64), (1100, 2, 2, 128)])
+def test_attention_many_sequences(cuda, type_, n, H, Hkv, HD):
+    """More sequences than a planning CTA has threads, of every kind side by side."""
+    rng = random.Random(n)
+    q_lens = [rng.choice([0, 1, 1, 1, 2, 8, 9, 40]) for _ in range(n)]
+    ctx = [x + rng.choice([0, 1, 30, 200]) for x in q_lens]
+    q_lens[n - 3], ctx[n - 3] = 330, 700
+    run_attention(cuda, type_, H, Hkv, HD, 16, q_lens, ctx, pad=3, seed=n)
+    q_lens = [min(x, 2) for x in q_lens]
+    run_attention(cuda, type_, H, Hkv, HD, 16, q_lens, ctx, pad=3, seed=n)
+
+
+@TYPES
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-30, -4.0])
+def test_attention_scales(cuda, type_, scale):
+    run_attention(cuda, type_, 8, 2, 64, 16, [1, 90, 3], [70, 300, 40], scale=scale)
+
+
+@TYPES
+@pytest.mark.parametrize("H,Hkv,HD", [(71, 1, 64), (33, 1, 128), (99, 3, 40), (300, 1, 8)])
+def test_attention_large_groups(cuda, type_, H, Hkv, HD):
+    run_attention(cuda, type_, H, Hkv, HD, 16, [1], [900])
+    run_attention(cuda, type_, H, Hkv, HD, 16, [1, 0, 2, 7], [300, 5, 2, 130])
+
+
+@TYPES
+def test_attention_in_place(cuda, type_):
+    for q_lens, ctx in (([1] * 9, [2000] * 9), ([400], [2000]), ([300, 1, 5], [700, 900, 1000])):
+        pages, seqs, batch, q, out, scale = run_attention(cuda, type_, 8, 2, 128, 16, q_lens, ctx)
+        for _ in range(3):
+            x = q.clone()
+            assert ib.attention_paged(pages, seqs, batch, 1, x, scale, out=x) is x
+            assert cuda.equal(x, out)
+
+
+@TYPES
+def test_attention_mixed_batch_in_a_graph(cuda, type_):
+    """The kernels of a mixed batch overlap; what is around them in the graph does not."""
+    pages, seqs, batch, q, out, scale = run_attention(
+        cuda, type_, 8, 2, 128, 16, [260, 1, 1, 5, 90, 1], [900, 4000, 33, 2500, 90, 1000])
+    ws = ib.attention_paged_workspace(pages, seqs, batch, 8)
+    x, y = cuda.empty_like(q.contiguous()), cuda.zeros(q.shape, device="cuda")
+    side = cuda.cuda.Stream()
+    side.wait_stream(cuda.cuda.current_stream())
+    with cuda.cuda.stream(side):
+        graph = cuda.cuda.CUDAGraph()
+        with cuda.cuda.graph(graph, stream=side):
+            total = cuda.zeros_like(y)
+            for i in range(3):  # one workspace, one after the other
+                x.copy_(q)
+                y.fill_(-1)
+                ib.attention_paged(pages, seqs, batch, 1, x, scale, out=y, workspace=ws)
+                x.zero_()
+                total += y
+        for _ in range(5):
+            graph.replay()
+    side.synchronize()
+    assert cuda.equal(y, out) and cuda.equal(total, out + out + out)
+
+
+def test_calls_on_another_stream_make_their_tensors_there(cuda):
+    """What a call allocates and clears itself belongs to the stream that it runs on."""
+    pages, seqs, batch, q, out, scale = run_attention(cuda, ib.F16, 8, 2, 64, 16, [3, 1], [50, 90])
+    other = cuda.cuda.Stream()
+    for i in range(2):  # memory of both streams to be handed out again (a new piece waits)
+        got = ib.attention_paged(pages, seqs, batch, 1, q, scale, stream=other.cuda_stream)
+        more = ib.attention_paged(pages, seqs, batch, 1, q, scale)
+        cuda.cuda.synchronize()
+        del got, more
+    cuda.cuda._sleep(50_000_000)  # the current stream is busy for some 25 ms
+    got = ib.attention_paged(pages, seqs, batch, 1, q, scale, stream=other.cuda_stream)
+    cuda.cuda.synchronize()
+    assert cuda.equal(got, out)
+    slots = i32(cuda, [batch.slots[0].item()])
+    kv = cuda.randn(4, 2, 64, device="cuda")
+    rope = rope_table(cuda, 128, 64)
+    want = ib.kv_append(pages, seqs, batch, 0, q, kv, kv, rope)
+    none = cuda.zeros_like(slots)
+    cuda.cuda.synchronize()
+    cuda.cuda._sleep(50_000_000)
+    new = ib.kv_append(pages, seqs, batch, 0, q, kv, kv, rope, stream=other.cuda_stream)
+    status = ib.kv_extend(pages, seqs, slots, none, stream=other.cuda_stream)
+    plan = ib.kv_compact(pages, seqs, stream=other.cuda_stream)
+    trash = [cuda.full_like(t, 5) for t in (new, status, plan.map) for _ in range(4)]
+    cuda.cuda.synchronize()
+    assert cuda.equal(new, want) and status.tolist() == [1] and len(trash) == 12
+    assert plan.info[0].item() == int((seqs.refs > 0).sum())
 
 
 def test_attention_records_bad_values_and_reads_nothing_there(cuda):
