@@ -257,7 +257,8 @@ typedef struct {
  * are already counted in its len.  cu_q [n_seqs + 1] and slots are device memory.  n_tokens:
  * rows of the tensors; rows from cu_q[n_seqs] on belong to nobody and are left as they were.
  * max_q: the most tokens of one sequence where the caller knows it (0: n_tokens); it chooses
- * kernels, results do not depend on it beyond rounding.  n_tokens * n_heads <= 2^26, n_heads <= 1024. */
+ * kernels, results do not depend on it beyond rounding.  n_tokens * n_heads <= 2^26,
+ * n_heads <= 1024. */
 typedef struct {
     int32_t n_seqs, n_tokens, max_q;
     const int32_t *cu_q, *slots;
@@ -310,8 +311,9 @@ int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_b
  * sees positions 0 .. len - n + i whose pages are there.  A row that sees none is 0.  Same
  * result contract as ib_attention_batch (softmax of scale * q.k, grouped heads).  q and out
  * [n_tokens][n_heads][head_dim] FP32, rows q_stride / out_stride elements apart (multiples
- * of 4, 16-byte aligned); out may be q itself.  A NaN or infinity in a position that a row does not see leaves the
- * row alone; in one that it sees, the row's outputs are not specified (NaN, as a rule).
+ * of 4, 16-byte aligned); out may be q itself.  A NaN or infinity in a position that a row
+ * does not see leaves the row alone; in one that it sees, the row's outputs are not specified
+ * (NaN, as a rule).
  * workspace: ib_attention_paged_workspace(...) bytes, 256-byte aligned, that no other call
  * uses at the same time; it needs no initial value. */
 size_t ib_attention_paged_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,

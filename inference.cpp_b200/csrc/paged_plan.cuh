@@ -20,8 +20,7 @@ struct CutRule {
 // at `start` counts G start + (i + 1) R, which has a closed sum over tiles.
 struct SeqWork {
     SeqInfo s;
-    int tiles;          // row tiles per kv head, 0: the sequence does not take part
-    long long per_head, all;
+    long long per_head, all;  // per kv head; 0: the sequence does not take part
 };
 
 constexpr unsigned long long kMostWork = 1ull << 62;  // sums of what device memory says saturate
@@ -38,8 +37,8 @@ __device__ __forceinline__ SeqWork seq_work(const PagedView& w, const CutRule& r
     x.s = seq_info(w, b);
     const int G = w.H / w.Hkv, rows = x.s.n * G;
     const bool in = rows >= rule.min_rows && rows <= rule.max_rows;
-    x.tiles = in ? (rows + rule.R - 1) / rule.R : 0;
-    x.per_head = tiles_work(x.tiles, (long long)G * max(x.s.L - x.s.n, 0), rule.R);
+    const int tiles = in ? (rows + rule.R - 1) / rule.R : 0;
+    x.per_head = tiles_work(tiles, (long long)G * max(x.s.L - x.s.n, 0), rule.R);
     // at most 2^23 tiles of at most 2^38 each (paged_check_batch)
     x.all = x.per_head * w.Hkv;
     return x;
@@ -157,7 +156,7 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     g.start = s.L - s.n;
     g.hk = (int)(u / p.x.per_head);
     u -= g.hk * p.x.per_head;
-    int lo = 0, hi = p.x.tiles;  // the tile: the last whose work begins at or before u
+    int lo = 0, hi = (s.n * G + rule.R - 1) / rule.R;  // the tile: the last whose work begins at or before u
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (tiles_work(mid, start_g, rule.R) <= u) lo = mid;

@@ -1,31 +1,43 @@
-// ib_attention_paged on tcgen05: FP16 pages, head_dim up to 128, tiles of 256 query rows -- the
-// chunks of prompts.
+// ib_attention_paged on tcgen05: head_dim up to 128, tiles of 256 query rows (128 for FP32 pages
+// with head_dim over 64) -- the chunks of prompts.
 //
-// Two query tiles of 128 rows share each key tile of 128 positions.  As on mma.sync, q and p are
-// FP16 pairs hi + lo (q scaled to a largest element in [256, 512), p by 2^10), K and V are taken
-// as they are, so every product is two MMAs and 2^-21 of it is kept:
+// Two query tiles of 128 rows share each key tile.  As on mma.sync, FP32 operands are pairs hi + lo
+// and 2^-21 of every product is kept:
+//   FP16 pages  q and p as FP16 pairs (q scaled to a largest element in [256, 512), p by 2^10),
+//               K and V as they are: two MMAs; key tiles of 128 positions
 //     S = q_lo K' + q_hi K'      A: q in shared memory, B: K            M 128, N 128
 //     O = p_lo V  + p_hi V       A: p in tensor memory, B: V            M 128, N head_dim
+//   FP32 pages  both operands as TF32 pairs: three MMAs (lo hi + hi lo + hi hi); key tiles of 64
+//               positions, 32 for head_dim over 64
 // The tensor core adds to its accumulator by cutting, which over a long sequence would drift; so
 // O starts from zero in every key tile and the running sum is kept in registers, one row per
 // thread, where acc = acc c + O takes the softmax's rescaling with it.
 //
 // Tensor memory, 512 columns: S of both query tiles (128 each), O of both (128 each).  p lies
-// over its S: of a chunk of 16 scores a thread writes hi into the first 8 columns and lo into the
-// other 8, and an MMA's 16 positions are one chunk.
-// Shared memory: q of both tiles as hi and lo (128 KB at head_dim 128) and a ring of three slots
-// for K and V tiles in turn.  Rows are 128 bytes (64 elements) under the 128-byte swizzle; K is
-// read with head_dim along the MMA's K (K-major), V with positions along it (MN-major), so both
-// are stored as they lie in the pages.
-// Warps: 0-3 and 4-7 the softmax of a query tile each (thread = row), 8 issues the MMAs, 9-11
-// bring K and V in: with TMA in boxes of as many rows as divide both a page and the tile (8 at
-// least; a box of a page that is not there lies outside the tensor and reads as zeros), or, for
-// other page sizes, row by row.  In tiles where some row does not see a position, they make V
-// finite before it is used (0 x inf).  The order of MMAs is
+// over its S: FP16, of a chunk of 16 scores a thread writes hi into the first 8 columns and lo into
+// the other 8, and an MMA's 16 positions are one chunk; FP32, hi over the scores and lo behind.
+// Shared memory: q of both tiles as hi and lo (128 KB) and a ring of slots for K and V tiles in
+// turn (three FP16 tiles, or two of FP32 parts and the FP32 tiles as they come).  Rows are 128
+// bytes under the 128-byte swizzle; K is read with head_dim along the MMA's K (K-major).  FP16 V is
+// read with positions along it (MN-major) and so stored as it lies in the pages; TF32 operands are
+// K-major only, so FP32 V is turned round on the way.
+// Warps: 0-3 and 4-7 the softmax of a query tile each (thread = row), 8 issues the MMAs, the others
+// bring K and V in, with TMA in boxes of as many rows as divide both a page and the tile (8 at
+// least; a box of a page that is not there lies outside the tensor and reads as zeros).  FP16: 9-11,
+// row by row for other page sizes.  FP32: 9 by TMA, 10-15 split the parts.  In tiles where some row
+// does not see a position, they make V finite before it is used (0 x inf).  The order of MMAs is
 //     O0(j) S0(j+1) O1(j) S1(j+1) O0(j+1) ...
-// so that a tile's softmax has the other tile's MMAs to hide behind.
+// so that a tile's softmax has the other tile's MMAs to hide behind, and FP16 O begins with the
+// second half of the positions while p of the first is computed (435 us without, 415 with).
 // Work per CTA is a piece of the batch (paged_plan.cuh); the copies run on into the next
 // segment.
+//
+// Measured: 2048 tokens behind 6144 (32 heads on 8, head_dim 128, FP16) 420 us, 1145 TFLOP/s of
+// MMAs, 0.70 of the measured rate of library FP16 products; the tensor pipe is busy 0.60 of the
+// cycles.  A step of both query tiles takes 6.3k cycles to the MMAs' 4.1k: the bound is the softmax
+// between a tile's S and its p, 3.8k cycles of dependent instructions with two warps to a scheduler
+// (the registers hold no more), which only half overlaps.  FP32 pages at head_dim 64: a step of
+// 6.3k cycles to 4.6k; 8.4k while the warp that starts the copies split them too.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -45,7 +57,6 @@ namespace ib {
 
 int paged_tensor_fault_take(int* code) { return paged_fault_take_here(code); }
 
-constexpr int PT_THREADS = 384, PT_LOADERS = 96;
 
 template <typename KV, int HDP>
 struct TensorCfg {
@@ -65,6 +76,12 @@ struct TensorCfg {
     // V: FP16 as it lies (K_BLOCK: 64 dimensions of all positions), FP32 turned round (32
     // positions of all dimensions)
     static constexpr int V_BLOCK = F32 ? HDP * 128 : K_BLOCK;
+    // warps that fill ring slots: copies (FP16), or splitting what warp 9 brings in (FP32)
+    static constexpr int SPLIT_WARPS = 6, FILL_WARPS = F32 ? SPLIT_WARPS : 3;
+    static constexpr int WARPS = F32 ? 10 + FILL_WARPS : 9 + FILL_WARPS, THREADS = 32 * WARPS;
+    // registers of the softmax warps and of the others, within what the launch has
+    static constexpr int MANY = F32 ? 184 : 224, FEW = F32 ? 72 : 56;
+    static_assert(256 * MANY + (THREADS - 256) * FEW <= THREADS * (65536 / THREADS / 8 * 8), "");
     static constexpr size_t SMEM = QT * 2 * Q_PLANE + SLOTS * TILE + RAW + 1024;
 };
 
@@ -93,9 +110,9 @@ constexpr uint32_t pt_idesc(int M, int N, bool b_mn, bool tf32 = false) {
            ((uint32_t)(M >> 4) << 24);
 }
 
-// The whole warp comes here with the same operands and `leader` lets one thread issue: the
-// operands then are uniform registers, as the instruction takes them.  Issued inside a branch of
-// one thread, every operand is moved there first, and an MMA took 134 cycles instead of 64.
+// The whole warp comes here with the same operands and `leader` lets one thread issue.  (The loops
+// around it are kept short: unrolled, 64 MMAs missed the instruction cache and took 134 cycles each
+// instead of 64.)
 template <bool TF32>
 __device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                           uint32_t add, uint32_t leader) {
@@ -158,31 +175,43 @@ __device__ __forceinline__ uint32_t pt_elect() {
     return x;
 }
 
-// 32 columns of this warp's 32 lanes, to be waited for
-__device__ __forceinline__ void pt_ld32(uint32_t taddr, float (&v)[32]) {
+// 32 columns of this warp's 32 lanes, or 64; the wait is part of the statement, so that nothing
+// uses the registers before it.
+__device__ __forceinline__ void pt_read32(uint32_t at, float (&a)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-        "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-        "%30, %31}, [%32];"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
-          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
-          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
-          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]),
-          "=f"(v[31])
-        : "r"(taddr));
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+        "%28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]),
+          "=f"(a[7]), "=f"(a[8]), "=f"(a[9]), "=f"(a[10]), "=f"(a[11]), "=f"(a[12]), "=f"(a[13]),
+          "=f"(a[14]), "=f"(a[15]), "=f"(a[16]), "=f"(a[17]), "=f"(a[18]), "=f"(a[19]),
+          "=f"(a[20]), "=f"(a[21]), "=f"(a[22]), "=f"(a[23]), "=f"(a[24]), "=f"(a[25]),
+          "=f"(a[26]), "=f"(a[27]), "=f"(a[28]), "=f"(a[29]), "=f"(a[30]), "=f"(a[31])
+        : "r"(at)
+        : "memory");
 }
-// The loads' registers pass through the wait, so that nothing uses them before it.
-__device__ __forceinline__ void pt_wait_ld(float (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
-                   "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]),
-                   "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]),
-                   "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
-                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
-                   "+f"(v[30]), "+f"(v[31])
-                 :
-                 : "memory");
+__device__ __forceinline__ void pt_read64(uint32_t at, float (&a)[32], float (&b)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+        "%28, %29, %30, %31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, "
+        "%41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, "
+        "%58, %59, %60, %61, %62, %63}, [%65];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]),
+          "=f"(a[7]), "=f"(a[8]), "=f"(a[9]), "=f"(a[10]), "=f"(a[11]), "=f"(a[12]), "=f"(a[13]),
+          "=f"(a[14]), "=f"(a[15]), "=f"(a[16]), "=f"(a[17]), "=f"(a[18]), "=f"(a[19]),
+          "=f"(a[20]), "=f"(a[21]), "=f"(a[22]), "=f"(a[23]), "=f"(a[24]), "=f"(a[25]),
+          "=f"(a[26]), "=f"(a[27]), "=f"(a[28]), "=f"(a[29]), "=f"(a[30]), "=f"(a[31]), "=f"(b[0]),
+          "=f"(b[1]), "=f"(b[2]), "=f"(b[3]), "=f"(b[4]), "=f"(b[5]), "=f"(b[6]), "=f"(b[7]),
+          "=f"(b[8]), "=f"(b[9]), "=f"(b[10]), "=f"(b[11]), "=f"(b[12]), "=f"(b[13]), "=f"(b[14]),
+          "=f"(b[15]), "=f"(b[16]), "=f"(b[17]), "=f"(b[18]), "=f"(b[19]), "=f"(b[20]),
+          "=f"(b[21]), "=f"(b[22]), "=f"(b[23]), "=f"(b[24]), "=f"(b[25]), "=f"(b[26]),
+          "=f"(b[27]), "=f"(b[28]), "=f"(b[29]), "=f"(b[30]), "=f"(b[31])
+        : "r"(at), "r"(at + 32)
+        : "memory");
 }
 __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
@@ -190,12 +219,6 @@ __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&v)[16])
         "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
         "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-        : "memory");
-}
-__device__ __forceinline__ void pt_st8(uint32_t taddr, const uint32_t (&v)[8]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
         : "memory");
 }
 
@@ -216,6 +239,17 @@ __device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
         "mov.b64 {%0, %1}, c;\n\t}"
         : "+f"(x0), "+f"(x1)
         : "f"(a0), "f"(a1));
+}
+// x - h, exact where h is x rounded
+__device__ __forceinline__ float less_half(float x, __half h) {
+    const uint16_t u = __half_as_ushort(h);
+    float y;
+    asm("{\n\t.reg .b16 m;\n\t"
+        "mov.b16 m, 0xbc00;\n\t"  // -1
+        "fma.rn.f32.f16 %0, %1, m, %2;\n\t}"
+        : "=f"(y)
+        : "h"(u), "f"(x));
+    return y;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float x;
@@ -247,11 +281,11 @@ struct TensorArgs {
 
 struct TensorBars {
     uint64_t kv_full[3], kv_empty[3], raw_full[2], raw_empty[2];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], v_there, done;
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], seg_done[2], v_there, done;
 };
 
 template <typename KV, int HDP>
-__global__ void __launch_bounds__(PT_THREADS, 1)
+__global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
     attn_tensor_kernel(const __grid_constant__ TensorArgs TA) {
     const RowsArgs& A = TA.rows;
     using C = TensorCfg<KV, HDP>;
@@ -260,23 +294,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) TensorBars bar;
     __shared__ uint32_t tmem_base;
-    __shared__ Piece sh_piece[PT_THREADS / 32];  // the same one for each warp, out of its registers
+    __shared__ Piece sh_piece[C::WARPS];  // the same one for each warp, out of its registers
     __shared__ int found;
     // of the last four key tiles: positions without a page; positions whose V is not finite
     __shared__ __align__(16) uint16_t sh_gone[4][8];
     __shared__ __align__(16) uint16_t sh_bad[4][8];
-    __shared__ uint32_t sh_bad32[4][3][2];  // the same for FP32, of each of the three warps
+    __shared__ uint32_t sh_bad32[4][C::SPLIT_WARPS][2];  // the same for FP32, of each splitting warp
     const PagedView& w = A.w;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (!A.beside) pdl_wait();
     pdl_launch_dependents();
-    find_piece<PT_THREADS>(w, A.rule, blockIdx.x, sh_piece, &found);
+    find_piece<C::THREADS>(w, A.rule, blockIdx.x, sh_piece, &found);
     __syncthreads();
     if (!found) {
         if (A.beside) pdl_wait();
         return;
     }
-    if (tid > 0 && tid < PT_THREADS / 32) sh_piece[tid] = sh_piece[0];
+    if (tid > 0 && tid < C::WARPS) sh_piece[tid] = sh_piece[0];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
     if (tid == 0) {
@@ -285,16 +319,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.v)) : "memory");
         }
         for (int i = 0; i < C::SLOTS; ++i) {
-            mbar_init(&bar.kv_full[i], PT_LOADERS + PT_LOADERS / 32);
+            mbar_init(&bar.kv_full[i], 33 * C::FILL_WARPS);
             mbar_init(&bar.kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.raw_full[i], 1);
-            mbar_init(&bar.raw_empty[i], PT_LOADERS / 32);
+            mbar_init(&bar.raw_empty[i], C::FILL_WARPS);
             mbar_init(&bar.q_full[i], 128);
             mbar_init(&bar.s_full[i], 1);
             mbar_init(&bar.p_full[i], 128);
+            mbar_init(&bar.p_half[i], 128);
             mbar_init(&bar.o_full[i], 1);
+            mbar_init(&bar.seg_done[i], 128);
         }
         mbar_init(&bar.v_there, 1);
         mbar_init(&bar.done, 1);
@@ -330,7 +366,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 
     if (warp < 8) {
         // ---- softmax of query tile t: thread = row ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::MANY));
         const int t = warp >> 2, wr = (warp & 3) * 32;  // this warp's rows of the tile, its lanes
         uint8_t* const q_ptr = base_ptr + 2 * t * C::Q_PLANE;
         const uint32_t s_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(128 * t);
@@ -438,8 +474,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 #pragma unroll
                 for (int d0 = 0; d0 < HDP; d0 += 32) {
                     float o[32];
-                    pt_ld32(o_at + d0, o);
-                    pt_wait_ld(o);
+                    pt_read32(o_at + d0, o);
 #pragma unroll
                     for (int d = 0; d < 32; d += 2) {
                         float* a = acc + d0 + d;
@@ -454,7 +489,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 #pragma unroll
                     for (int i = 0; i < KT / 32; ++i) {
                         uint32_t bad;
-                        if constexpr (F32) bad = bad32[0][i] | bad32[1][i] | bad32[2][i];
+                        if constexpr (F32) {
+                            bad = 0;
+#pragma unroll
+                            for (int k = 0; k < C::SPLIT_WARPS; ++k) bad |= bad32[k][i];
+                        }
                         else bad = (uint32_t)bad16[2 * i] | ((uint32_t)bad16[2 * i + 1] << 16);
                         if (visible(j, i) & bad) l = NAN;
                     }
@@ -483,10 +522,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 float s0[32], s1[32];
 #pragma unroll 1
                 for (int i = 0; i < KT / 32; i += 2) {
-                    pt_ld32(s_at + 32 * i, s0);
-                    if constexpr (KT > 32) pt_ld32(s_at + 32 * i + 32, s1);
-                    pt_wait_ld(s0);
-                    if constexpr (KT > 32) pt_wait_ld(s1);
+                    if constexpr (KT > 32) pt_read64(s_at + 32 * i, s0, s1);
+                    else pt_read32(s_at + 32 * i, s0);
                     if (!all) {
                         mask(s0, i);
                         if constexpr (KT > 32) mask(s1, i + 1);
@@ -522,7 +559,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                             pt_st16(s_at + 32 * i + 16 * c16, hi);
                             pt_st16(s_at + KT + 32 * i + 16 * c16, lo);
                         } else {
-                            uint32_t hi[8], lo[8];
+                            uint32_t hl[16];
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
                                 float x, y;
@@ -530,26 +567,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                                 x = ex2(x), y = ex2(y);
                                 add2(sum0, sum1, x, y);
                                 const __half2 h = __floats2half2_rn(x, y);
-                                const float2 back = __half22float2(h);
-                                fma2(x, y, back.x, back.y, -1.f, -1.f, x, y);
+                                x = less_half(x, __low2half(h)), y = less_half(y, __high2half(h));
                                 const __half2 r = __floats2half2_rn(x, y);
-                                hi[k] = *reinterpret_cast<const uint32_t*>(&h);
-                                lo[k] = *reinterpret_cast<const uint32_t*>(&r);
+                                hl[k] = *reinterpret_cast<const uint32_t*>(&h);
+                                hl[8 + k] = *reinterpret_cast<const uint32_t*>(&r);
                             }
-                            pt_st8(s_at + 32 * i + 16 * c16, hi);
-                            pt_st8(s_at + 32 * i + 16 * c16 + 8, lo);
+                            pt_st16(s_at + 32 * i + 16 * c16, hl);
                         }
                     }
                 };
 #pragma unroll 1
                 for (int i = KT == 128 ? 2 : 0; i >= 0; i -= 2) {
                     if constexpr (KT > 32) weights(s1, i + 1);
-                    if (i) pt_ld32(s_at + 32, s1);
                     weights(s0, i);
                     if (i) {
-                        pt_ld32(s_at, s0);
-                        pt_wait_ld(s0);
-                        pt_wait_ld(s1);
+                        if constexpr (!F32) {  // O can begin
+                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                            pt_fence_before();
+                            mbar_arrive(&bar.p_half[t]);
+                        }
+                        pt_read64(s_at, s0, s1);
                         if (!all) mask(s0, 0), mask(s1, 1);
                     }
                 }
@@ -564,6 +601,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 more = next();
                 if (more) next_scale = stage_q(it);
                 add_o(n_kt - 1);
+                mbar_arrive(&bar.seg_done[t]);
             }
             if (r < rows && ok) {  // a row per thread
                 const bool whole = cur.part < 0;
@@ -579,12 +617,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
         if (warp == 8) {
             // ---- MMAs ----
             constexpr uint32_t id_s = pt_idesc(128, KT, false, F32), id_o = pt_idesc(128, HDP, !F32, F32);
             int half = 0;               // K and V tiles so far: the ring's order
-            int n_q[2] = {0, 0}, n_s[2] = {0, 0};  // q tiles and key tiles so far
+            int n_q[2] = {0, 0}, n_s[2] = {0, 0};  // q tiles (segments) and key tiles so far
+            // A segment's last sh_gone and sh_bad are read after its last MMA: the next segment's
+            // second key tile waits for that, before the copies come round to them.
+            uint32_t owed = 0;  // of which query tiles
             bool ok = true;
             const uint32_t leader = pt_elect();
             // loops of a few MMAs: the code stays in the instruction cache, 64 cycles an MMA are time.
@@ -604,8 +645,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                             pt_mma_ss<F32>(tmem + 128 * t, qa + 2 * k, kb + 2 * k, id_s, add, leader);
                 }
             };
-            auto outputs = [&](int t, uint32_t v_at) {
-                uint32_t add = 0;
+            // FP16: half h of the positions, the second one first
+            auto outputs = [&](int t, uint32_t v_at, int h) {
+                uint32_t add = !F32 && h == 0;
 #pragma unroll 1
                 for (int pass = 0; pass < PASSES; ++pass) {
                     if constexpr (F32) {
@@ -618,10 +660,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                                 pt_mma_ts<true>(tmem + 256 + 128 * t, pa + 8 * k, vb + 2 * k, id_o, add,
                                                 leader);
                     } else {
-                        uint64_t vb = pt_desc(v_at, C::V_BLOCK);
-                        uint32_t pa = tmem + 128 * t + (pass == 0 ? 8 : 0);
-#pragma unroll 1
-                        for (int k0 = 0; k0 < KT / 16; k0 += 4, vb += 4 * 128, pa += 64)
+                        uint64_t vb = pt_desc(v_at, C::V_BLOCK) + h * 4 * 128;
+                        uint32_t pa = tmem + 128 * t + (pass == 0 ? 8 : 0) + h * 64;
 #pragma unroll
                             for (int k = 0; k < 4; ++k, add = 1)  // 16 rows, 2048 bytes, a step
                                 pt_mma_ts<false>(tmem + 256 + 128 * t, pa + 16 * k, vb + 128 * k, id_o,
@@ -647,15 +687,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                         if (t == n_t - 1) pt_commit(&bar.kv_empty[half % C::SLOTS], leader);
                     }
                 }
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t, owed >>= 1)  // phase: of the segment before
+                    if (owed & 1) ok = ok && wait(&bar.seg_done[t], n_q[t] - (t < n_t ? 2 : 1));
+                owed = (1u << n_t) - 1;
                 for (int j = 0; j < n_kt && ok; ++j) {
                     const int hv = half + 2 * j + 1, hk = hv + 1;
                     for (int t = 0; t < n_t && ok; ++t) {
                         if (t == 0) arrived(hv);
-                        // p of this key tile is there, and O of the one before has been read
-                        ok = ok && wait(&bar.p_full[t], n_s[t]++);
+                        // p of this key tile (half of it) is there, and O of the one before has been
+                        // read
+                        ok = ok && wait(F32 ? &bar.p_full[t] : &bar.p_half[t], n_s[t]++);
                         pt_fence_after();
                         if (ok) {
-                            outputs(t, slot_at(hv));
+                            if constexpr (!F32) {
+                                outputs(t, slot_at(hv), 1);
+                                ok = wait(&bar.p_full[t], n_s[t] - 1);
+                                pt_fence_after();
+                                if (ok) outputs(t, slot_at(hv), 0);
+                            } else {
+                                outputs(t, slot_at(hv), 0);
+                            }
                             pt_commit(&bar.o_full[t], leader);
                             if (t == n_t - 1) pt_commit(&bar.kv_empty[hv % C::SLOTS], leader);
                         }
@@ -809,66 +861,76 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             asm volatile("cp.async.wait_all;" ::: "memory");
             for (int h = max(0, half - C::SLOTS); h < half; ++h)
                 wait(&bar.kv_full[h % C::SLOTS], h / C::SLOTS);
-        } else {
-            // ---- copies of FP32 pages: TMA brings K and V as they are, the three warps split them
-            // into TF32 parts, hi in the slot's first half, lo in the second.  K: rows are positions,
-            // 128 bytes 32 dimensions.  V is turned round, since TF32 operands have to lie along K:
-            // rows are dimensions, 128 bytes 32 positions. ----
-            const int lw = warp - 9;
+        } else if (warp == 9) {
+            // ---- copies of FP32 pages: TMA brings K and V as they are ----
             const int box = TA.box, box_row = lane << box;
             const bool has_box = box_row < KT;
             const uint32_t raw_a = ring + C::SLOTS * C::TILE;
-            const uint8_t* const raw_ptr = base_ptr + (raw_a - base);
-            int half = 0, issued[2] = {0, 0}, used[2] = {0, 0};  // tiles brought in and split, K and V
-            uint32_t tile_no = 0;
+            int issued = 0;  // tiles
             bool ok = true;
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
-                const int first_lim = it.start + it.row0 / G;
-                if (lw == 1) {  // the softmax warps ask for the segment's q soon
-                    for (int r = lane; r < it.rows; r += 32) {
-                        const uint8_t* p = (const uint8_t*)q_row(A, it, G, it.row0 + r);
-                        for (int b = 0; b < HD * 4; b += 128)
-                            asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
-                    }
-                }
                 auto box_of = [&](int kt) -> int {  // this lane's box of key tile kt, -1: none
                     const int pos = kt * KT + box_row;
-                    if (lw != 0 || !has_box || kt >= it.kt1 || pos > last_lim) return -1;
+                    if (!has_box || kt >= it.kt1 || pos > last_lim) return -1;
                     const int col = (int)w.ps.div((uint32_t)pos);
                     const int page = page_at(w, it.s.row[col]);
                     return page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
                 };
-                auto bring = [&](int kv, int at) {  // warp 9
-                    if (issued[kv] > 0) ok = ok && wait(&bar.raw_empty[kv], issued[kv] - 1);
-                    if (!ok) return;
-                    if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[kv], C::PLANE);
-                    __syncwarp();
-                    if (has_box)
-                        pt_tma(raw_a + (uint32_t)(kv * C::PLANE + box_row * HDP * 4), kv ? &TA.v : &TA.k, 0,
-                               at < 0 ? -KT : at, &bar.raw_full[kv]);
-                    ++issued[kv];
-                };
-                int box_at = box_of(it.kt0), box_next = -1;
-                if (lw == 0 && it.kt0 < it.kt1) bring(0, box_at), bring(1, box_at);
+                int at = box_of(it.kt0);
+                // the softmax warps ask for the segment's q soon
+                for (int r = lane; r < it.rows; r += 32) {
+                    const uint8_t* p = (const uint8_t*)q_row(A, it, G, it.row0 + r);
+                    for (int b = 0; b < HD * 4; b += 128)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
+                }
+                for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++issued) {
+                    const int at_next = box_of(kt + 1);
+#pragma unroll 1
+                    for (int kv = 0; kv < 2 && ok; ++kv) {
+                        if (issued > 0) ok = wait(&bar.raw_empty[kv], issued - 1);
+                        if (!ok) break;
+                        if (kv == 0 && has_box)
+                            for (int b = 0; b < 1 << (box - 3); ++b)
+                                reinterpret_cast<uint8_t*>(sh_gone[issued & 3])[box_row / 8 + b] =
+                                    at < 0 ? 0xff : 0;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[kv], C::PLANE);
+                        __syncwarp();
+                        if (has_box)
+                            pt_tma(raw_a + (uint32_t)(kv * C::PLANE + box_row * HDP * 4),
+                                   kv ? &TA.v : &TA.k, 0, at < 0 ? -KT : at, &bar.raw_full[kv]);
+                        if (kv == 1) at = at_next;
+                    }
+                }
+            }
+            // no copy may still be landing when the CTA ends (a count that stopped early: one each)
+            for (int kv = 0; kv < 2; ++kv)
+                if (issued > 0) wait(&bar.raw_full[kv], issued - 1);
+        } else {
+            // ---- and these warps split them into TF32 parts, hi in a slot's first half, lo in the
+            // second.  K: rows are positions, 128 bytes 32 dimensions.  V is turned round, since TF32
+            // operands have to lie along K: rows are dimensions, 128 bytes 32 positions. ----
+            const int sw = warp - 10;
+            const uint8_t* const raw_ptr = base_ptr + (ring - base) + C::SLOTS * C::TILE;
+            int half = 0;
+            uint32_t tile_no = 0;
+            bool ok = true;
+            while (ok && next()) {
+                const int first_lim = it.start + it.row0 / G;
                 for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
                     const bool careful = kt * KT + KT - 1 > first_lim;
-                    box_next = box_of(kt + 1);
 #pragma unroll 1
-                    for (int kv = 0; kv < 2 && ok; ++kv, ++half) {
+                    for (int kv = 0; kv < 2; ++kv, ++half) {
                         const int slot = half % C::SLOTS, use = half / C::SLOTS;
-                        ok = wait(&bar.raw_full[kv], used[kv]);
+                        ok = wait(&bar.raw_full[kv], (int)tile_no);
                         if (use > 0) ok = ok && wait(&bar.kv_empty[slot], use - 1);
                         if (!ok) break;
                         uint8_t* const tile = base_ptr + (ring - base) + slot * C::TILE;
                         const uint8_t* const raw = raw_ptr + kv * C::PLANE;
                         if (kv == 0) {
-                            if (lw == 0 && has_box)
-                                for (int b = 0; b < 1 << (box - 3); ++b)
-                                    reinterpret_cast<uint8_t*>(sh_gone[tile_no & 3])[box_row / 8 + b] =
-                                        box_at < 0 ? 0xff : 0;
 #pragma unroll 4
-                            for (int i = lw * 32 + lane; i < C::PLANE / 16; i += PT_LOADERS) {
+                            for (int i = sw * 32 + lane; i < C::PLANE / 16; i += 32 * C::SPLIT_WARPS) {
                                 const int r = i / (HDP / 4), d = (i % (HDP / 4)) * 4;
                                 const float4 x = *reinterpret_cast<const float4*>(raw + i * 16);
                                 uint4 h, l;
@@ -882,7 +944,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                             uint32_t bad0 = 0, bad1 = 0;
                             // four positions of 32 dimensions at a time, a dimension to a lane
 #pragma unroll 2
-                            for (int u = lw; u < KT / 4 * (HDP / 32); u += PT_LOADERS / 32) {
+                            for (int u = sw; u < KT / 4 * (HDP / 32); u += C::SPLIT_WARPS) {
                                 const int p4 = u / (HDP / 32), d = (u % (HDP / 32)) * 32 + lane;
                                 float y[4];
 #pragma unroll
@@ -907,8 +969,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                                 *reinterpret_cast<uint4*>(at + C::PLANE) = l;
                             }
                             if (lane == 0) {
-                                sh_bad32[tile_no & 3][lw][0] = bad0;
-                                sh_bad32[tile_no & 3][lw][1] = bad1;
+                                sh_bad32[tile_no & 3][sw][0] = bad0;
+                                sh_bad32[tile_no & 3][sw][1] = bad1;
                             }
                         }
                         pt_fence_async();
@@ -918,16 +980,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                             mbar_arrive(&bar.kv_full[slot]);
                             mbar_arrive(&bar.raw_empty[kv]);
                         }
-                        ++used[kv];
-                        if (lw == 0 && kt + 1 < it.kt1) bring(kv, box_next);
                     }
-                    box_at = box_next;
                 }
             }
-            // no copy may still be landing when the CTA ends
-            if (lw == 0)
-                for (int kv = 0; kv < 2; ++kv)
-                    if (issued[kv] > used[kv]) wait(&bar.raw_full[kv], issued[kv] - 1);
         }
     }
     // every use of tensor memory is over before it is given back
@@ -1011,7 +1066,7 @@ static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
     IB_CUDA_CHECK(once.run([&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
     }));
-    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(PT_THREADS), C::SMEM, st, true, t));
+    IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, st, true, t));
     return IB_OK;
 }
 
