@@ -154,7 +154,9 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     long long u = p.at - p.base;
     g.s = s;
     g.start = s.L - s.n;
-    g.hk = (int)(u / p.x.per_head);
+    g.hk = min((int)__fdividef((float)u, (float)p.x.per_head), w.Hkv - 1);  // to one
+    if (g.hk * p.x.per_head > u) --g.hk;
+    else if ((g.hk + 1) * p.x.per_head <= u) ++g.hk;
     u -= g.hk * p.x.per_head;
     int lo = 0, hi = (s.n * G + rule.R - 1) / rule.R;  // the tile: the last whose work begins at or before u
     while (hi - lo > 1) {
@@ -170,10 +172,11 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     const long long x1 = min(all, x0 + (p.end - p.at));
     const int seen = max(0, g.start + (g.row0 + g.rows - 1) / G + 1);
     const int nkt = (seen + rule.KT - 1) / rule.KT;
-    // the same value for a piece's end and the next one's beginning
-    // (below 2^24 x 2^38: paged_check_batch)
-    g.kt0 = x0 == 0 ? 0 : (int)(nkt * x0 / all);
-    g.kt1 = x1 == all ? nkt : (int)(nkt * x1 / all);
+    // the same value for a piece's end and the next one's beginning, and more for more work: that
+    // is all a cut needs (three integer divisions of 64 bits took a thousand cycles)
+    const float per = __fdividef((float)nkt, (float)all);
+    g.kt0 = x0 == 0 ? 0 : min(nkt, (int)((float)x0 * per));
+    g.kt1 = x1 == all ? nkt : min(nkt, (int)((float)x1 * per));
     const bool whole = x0 == 0 && x1 == all;
     g.part = whole ? -1 : 2 * p.no + (p.at == p.no * p.len ? 0 : 1);
     p.at += x1 - x0;

@@ -377,60 +377,65 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
         const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
         // The segment's q into this warp's 32 rows of the tile, HDP / 8 lanes to a row; returns the
         // factor of row `lane`.  The last segment's scores are done (this warp has read some), so
-        // nothing reads the rows any more.
+        // nothing reads the rows any more.  All of q is on its way at once, into the places of the
+        // parts that are made of it.
         auto stage_q = [&](const Segment& sg) -> float {
-            constexpr int LPR = HDP / 8, RPI = 32 / LPR, AT_ONCE = 4;  // loads on their way
+            constexpr int LPR = HDP / 8, RPI = 32 / LPR;
             const int rows = sg.rows - 128 * t, d = (lane % LPR) * 8;
-            float mine = 0.f;
+            float mine = F32 ? 1.f : 0.f;
             if (rows <= 0 || sg.kt0 == sg.kt1) return mine;
-#pragma unroll 1
-            for (int i0 = 0; i0 < 32; i0 += AT_ONCE * RPI) {
-                float4 x[AT_ONCE][2];
+            // 16 bytes of the values d .. of row r: FP16 hi, lo; FP32 the first four's hi, the others'
+            // (their lo parts Q_PLANE behind)
+            auto place = [&](int r, int d, int half) -> uint32_t {
+                if constexpr (F32)
+                    return (uint32_t)((d >> 5) * C::Q_BLOCK) + pt_off(r, ((d & 31) >> 2) + half);
+                else
+                    return (uint32_t)((d >> 6) * C::Q_BLOCK + half * C::Q_PLANE) + pt_off(r, (d & 63) >> 3);
+            };
+            const uint32_t q_a = base + (uint32_t)(2 * t * C::Q_PLANE);
+            constexpr int CPR = HDP / 4, RPC = 32 / CPR;  // 16-byte chunks of a row, rows at a time
+            const int dc = (lane % CPR) * 4;
+            const int64_t per_token = A.q_stride - (int64_t)G * HD;  // rows of a token are consecutive
+            const float* const q0 = A.q + (int64_t)sg.s.q0 * A.q_stride + (int64_t)sg.hk * G * HD + dc;
+            const int first_row = sg.row0 + 128 * t;
+            const FastDiv group = w.group;
+#pragma unroll 4
+            for (int i = 0; i < 32; i += RPC) {
+                const int r = wr + i + lane / CPR, row = first_row + r;
+                const bool there = r < rows && dc < HD;
+                const int64_t at = (int64_t)row * HD + (int64_t)group.div((uint32_t)row) * per_token;
+                cp16(q_a + place(r, dc & ~7, (dc >> 2) & 1), q0 + (there ? at : 0), there);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+#pragma unroll 2
+            for (int i = 0; i < 32; i += RPI) {
+                const int r = wr + i + lane / LPR;
+                uint4* const at0 = reinterpret_cast<uint4*>(q_ptr + place(r, d, 0));
+                uint4* const at1 = reinterpret_cast<uint4*>(q_ptr + place(r, d, 1));
+                const float4 x0 = *reinterpret_cast<const float4*>(at0);
+                const float4 x1 = *reinterpret_cast<const float4*>(at1);
+                uint4 h, l;
+                if constexpr (F32) {
+                    split_tf32(x0.x * sign, h.x, l.x), split_tf32(x0.y * sign, h.y, l.y);
+                    split_tf32(x0.z * sign, h.z, l.z), split_tf32(x0.w * sign, h.w, l.w);
+                    *at0 = h, at0[C::Q_PLANE / 16] = l;
+                    split_tf32(x1.x * sign, h.x, l.x), split_tf32(x1.y * sign, h.y, l.y);
+                    split_tf32(x1.z * sign, h.z, l.z), split_tf32(x1.w * sign, h.w, l.w);
+                    *at1 = h, at1[C::Q_PLANE / 16] = l;
+                } else {
+                    float top = fmaxf(fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x0.z), fabsf(x0.w))),
+                                      fmaxf(fmaxf(fabsf(x1.x), fabsf(x1.y)), fmaxf(fabsf(x1.z), fabsf(x1.w))));
 #pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k) {
-                    const int r = wr + i0 + k * RPI + lane / LPR;
-                    x[k][0] = x[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < rows && d < HD) {
-                        const float4* p = reinterpret_cast<const float4*>(
-                            q_row(A, sg, G, sg.row0 + 128 * t + r) + d);
-                        x[k][0] = __ldg(p), x[k][1] = __ldg(p + 1);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k) {
-                    const int i = i0 + k * RPI, r = wr + i + lane / LPR;
-                    const float* y = &x[k][0].x;
-                    if constexpr (F32) {
-                        uint32_t h[8], l[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) split_tf32(y[e] * sign, h[e], l[e]);
-#pragma unroll
-                        for (int e = 0; e < 8; e += 4) {
-                            uint8_t* const at =
-                                q_ptr + (d >> 5) * C::Q_BLOCK + pt_off(r, ((d & 31) + e) >> 2);
-                            *reinterpret_cast<uint4*>(at) = make_uint4(h[e], h[e + 1], h[e + 2], h[e + 3]);
-                            *reinterpret_cast<uint4*>(at + C::Q_PLANE) =
-                                make_uint4(l[e], l[e + 1], l[e + 2], l[e + 3]);
-                        }
-                        mine = 1.f;
-                    } else {
-                        float top = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
-#pragma unroll
-                        for (int o = LPR / 2; o > 0; o >>= 1)
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        float down;
-                        const float up = pow2_scale(top, down) * sign;
-                        uint32_t h[4], l[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) split2(y[2 * e] * up, y[2 * e + 1] * up, h[e], l[e]);
-                        uint8_t* const at = q_ptr + (d >> 6) * C::Q_BLOCK + pt_off(r, (d & 63) >> 3);
-                        *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4*>(at + C::Q_PLANE) = make_uint4(l[0], l[1], l[2], l[3]);
-                        const float f = __shfl_sync(0xffffffffu, down, ((lane - i) & (RPI - 1)) * LPR);
-                        if (lane >= i && lane < i + RPI) mine = f;
-                    }
+                    for (int o = LPR / 2; o > 0; o >>= 1)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    float down;
+                    const float up = pow2_scale(top, down) * sign;
+                    split2(x0.x * up, x0.y * up, h.x, l.x), split2(x0.z * up, x0.w * up, h.y, l.y);
+                    split2(x1.x * up, x1.y * up, h.z, l.z), split2(x1.z * up, x1.w * up, h.w, l.w);
+                    *at0 = h, *at1 = l;
+                    const float f = __shfl_sync(0xffffffffu, down, ((lane - i) & (RPI - 1)) * LPR);
+                    if (lane >= i && lane < i + RPI) mine = f;
                 }
             }
             pt_fence_async();
