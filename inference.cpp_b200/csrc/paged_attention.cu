@@ -823,12 +823,14 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
         const bool whole = it.part < 0;
         const int64_t at = (int64_t)it.part * R + r;
         const float inv = !whole ? 1.f : t.l[h] == 0.f ? 0.f : 1.f / t.l[h];
-        float* p = whole ? out_row(A, it, G, row0 + r) : A.part_acc + at * HD;
+        float* p = whole ? out_row(A, it, G, row0 + r) : nullptr;
 #pragma unroll
         for (int d = 0; d < T::DB; ++d)
-            if (d * 8 < HD)
-                *reinterpret_cast<float2*>(p + d * 8 + 2 * (lane & 3)) =
+            if (d * 8 < HD) {
+                const int x = d * 8 + 2 * (lane & 3);
+                *reinterpret_cast<float2*>(whole ? p + x : part_at(A, it.part, r, x)) =
                     make_float2(t.acc[d][2 * h] * inv, t.acc[d][2 * h + 1] * inv);
+            }
         if (!whole && (lane & 3) == 0) A.part_ml[at] = make_float2(t.m[h], t.l[h]);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -915,12 +917,11 @@ __device__ __forceinline__ void join_parts(const JoinArgs& A, int item) {
 // Tiles of many rows that find_piece cut, mostly in two: CTA (no, y) looks whether piece `no`
 // begins inside a tile, and is the first to do so there, and sees to its rows JOIN_ROWS y ...
 // All CTAs are on the SMs at once, since each has to plan first: with 32 rows to a CTA, four times
-// as many of them, the join behind a chunk of 2048 tokens took 36 us against 22 (cold caches).
+// as many of them, the join of a mixed step took 36 us against 22 (cold caches).
 constexpr int JOIN_ROWS = 128, JOIN_THREADS = 512;
+static_assert(JOIN_THREADS == 4 * JOIN_ROWS, "");
 template <int HDP>
 __device__ __forceinline__ void join_pieces(const JoinArgs& A, int no, int y) {
-    constexpr int LPR = HDP / 4 < 32 ? HDP / 4 : 32, V = HDP / 4 / LPR;  // lanes of a row, float4 of a lane
-    constexpr int U = V == 1 ? 4 : 2;                                    // rows of a lane at once
     __shared__ Piece sh_piece;
     __shared__ int found;
     const PagedView& w = A.w;
@@ -941,52 +942,39 @@ __device__ __forceinline__ void join_pieces(const JoinArgs& A, int no, int y) {
     const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
     if (c0 != no - 1 || c1 >= A.rule.n_pieces) return;
     const int n_parts = c1 - c0 + 1, first = 2 * c0 + (a == c0 * p.len ? 0 : 1);
-    const int x = tid % LPR, end = min(sg.rows, (y + 1) * JOIN_ROWS);
-    constexpr int STEP = JOIN_THREADS / LPR;
-    for (int r0 = y * JOIN_ROWS + tid / LPR; r0 < end; r0 += U * STEP) {
-        float M[U], l[U];
-        float4 o[U][V];
+    // four lanes to a row: they read four times 16 bytes of eight rows, and write 64 of each
+    const int r = y * JOIN_ROWS + tid / 4, x = tid % 4, D4 = HD / 4;
+    if (r >= sg.rows) return;
+#pragma unroll 1
+    for (int d = x; d < HDP / 4; d += 16) {
+        float M = -INFINITY, l = 0.f;
+        float4 o[4];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            M[j] = -INFINITY, l[j] = 0.f;
-#pragma unroll
-            for (int k = 0; k < V; ++k) o[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        for (int k = 0; k < 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
         for (int i = 0; i < n_parts; ++i) {
-            const int64_t at = (int64_t)(i == 0 ? first : 2 * (c0 + i)) * R;
-            float2 ml[U];
-            float4 v[U][V];
+            const int64_t part = i == 0 ? first : 2 * (c0 + i);
+            const float2 ml = A.part_ml[part * R + r];
+            float4 v[4];
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int r = r0 + j * STEP;
-                ml[j] = r < end ? A.part_ml[at + r] : make_float2(-INFINITY, 0.f);
+            for (int k = 0; k < 4; ++k)
+                v[k] = d + 4 * k < D4
+                           ? reinterpret_cast<const float4*>(A.part_acc)[(part * D4 + d + 4 * k) * R + r]
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float top = fmaxf(M, ml.x);
+            const float f = top == -INFINITY ? 1.f : ex2(M - top);
+            const float c = top == -INFINITY ? 1.f : ex2(ml.x - top);
+            M = top;
+            l = fmaf(l, f, c * ml.y);
 #pragma unroll
-                for (int k = 0; k < V; ++k)
-                    v[j][k] = r < end && x + LPR * k < HD / 4
-                                  ? reinterpret_cast<const float4*>(A.part_acc + (at + r) * HD)[x + LPR * k]
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const float top = fmaxf(M[j], ml[j].x);
-                const float f = top == -INFINITY ? 1.f : ex2(M[j] - top);
-                const float c = top == -INFINITY ? 1.f : ex2(ml[j].x - top);
-                M[j] = top;
-                l[j] = fmaf(l[j], f, c * ml[j].y);
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    o[j][k].x = fmaf(o[j][k].x, f, c * v[j][k].x), o[j][k].y = fmaf(o[j][k].y, f, c * v[j][k].y);
-                    o[j][k].z = fmaf(o[j][k].z, f, c * v[j][k].z), o[j][k].w = fmaf(o[j][k].w, f, c * v[j][k].w);
-                }
+            for (int k = 0; k < 4; ++k) {
+                o[k].x = fmaf(o[k].x, f, c * v[k].x), o[k].y = fmaf(o[k].y, f, c * v[k].y);
+                o[k].z = fmaf(o[k].z, f, c * v[k].z), o[k].w = fmaf(o[k].w, f, c * v[k].w);
             }
         }
 #pragma unroll
-        for (int j = 0; j < U; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k)
-                if (r0 + j * STEP < end && x + LPR * k < HD / 4)
-                    join_store(A, sg.s, sg.hk, sg.row0 + r0 + j * STEP, x + LPR * k, o[j][k], l[j]);
+        for (int k = 0; k < 4; ++k)
+            if (d + 4 * k < D4) join_store(A, sg.s, sg.hk, sg.row0 + r, d + 4 * k, o[k], l);
     }
 }
 

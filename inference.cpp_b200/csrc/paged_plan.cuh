@@ -306,7 +306,7 @@ struct RowsArgs {
     float* out;
     int64_t q_stride, out_stride;
     const void *k, *v;  // the layer
-    float* part_acc;    // [partial][R][HD]
+    float* part_acc;    // [partial][R][HD] of parts, [partial][HD / 4][R][4] of pieces
     float2* part_ml;    // [partial][R]
     float scale_log2;   // scale * log2(e)
     // The kernel before is the call's narrow one, which writes other rows and workspace: this one
@@ -325,6 +325,13 @@ __device__ __forceinline__ float* out_row(const RowsArgs& A, const Segment& it, 
 __device__ __forceinline__ const float* q_row(const RowsArgs& A, const Segment& it, int G, int gr) {
     const int tok = (int)A.w.group.div((uint32_t)gr);
     return A.q + (int64_t)(it.s.q0 + tok) * A.q_stride + (int64_t)(it.hk * G + gr - tok * G) * A.w.HD;
+}
+
+// Element d of row r of a piece's partial result.  Rows run along memory: they are a thread each
+// on tcgen05, and a warp's 16 bytes of each of 32 rows would be 32 lines (a chunk of 2048 tokens
+// takes 412 us against 417 that way, prompts on FP32 pages 111 against 114).
+__device__ __forceinline__ float* part_at(const RowsArgs& A, int part, int r, int d) {
+    return A.part_acc + (((int64_t)part * (A.w.HD / 4) + (d >> 2)) * A.rule.R + r) * 4 + (d & 3);
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {

@@ -612,11 +612,12 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                 const bool whole = cur.part < 0;
                 const int64_t at = (int64_t)cur.part * C::R + 128 * t + r;
                 const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                float* p = whole ? out_row(A, cur, G, row) : A.part_acc + at * HD;
+                float* p = whole ? out_row(A, cur, G, row) : part_at(A, cur.part, 128 * t + r, 0);
+                const int step = whole ? 4 : 4 * C::R;
 #pragma unroll
-                for (int d = 0; d < HDP; d += 4)
+                for (int d = 0; d < HDP; d += 4, p += step)
                     if (d < HD)
-                        *reinterpret_cast<float4*>(p + d) =
+                        *reinterpret_cast<float4*>(p) =
                             make_float4(acc[d] * f, acc[d + 1] * f, acc[d + 2] * f, acc[d + 3] * f);
                 if (!whole) A.part_ml[at] = make_float2(m * sc, l);
             }
