@@ -704,16 +704,19 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
     }
 }
 
-// ---- more rows on mma.sync ---------------------------------------------------------------
-// WR warps of 16 rows each over the same key tiles, which the CTA brings in together.
+// ---- more rows on mma.sync, for head_dim over 128 -----------------------------------------
+// WR warps of 16 rows each over the same key tiles, which the CTA brings in together.  Bound by
+// the legacy tensor path and the splitting of its operands: the last 1024 of 4096 positions (16
+// heads on 8, head_dim 256, FP16) 624 us, 96 TFLOP/s of the formula, where head_dim 128 on
+// tcgen05 has 540.
 template <typename KV, int HDP>
 struct WideCfg {
     static constexpr bool F32 = sizeof(KV) == 4;
-    static constexpr int WR = HDP == 256 ? 4 : 8, NT = WR * 32, R = 16 * WR;
+    static constexpr int WR = 4, NT = WR * 32, R = 16 * WR;
     static constexpr int ROWB = HDP * (int)sizeof(KV);
-    static constexpr int KT = ROWB <= 128 ? 64 : ROWB <= 512 ? 32 : 16;
+    static constexpr int KT = F32 ? 16 : 32;
     using Tile = WarpRows<KV, HDP, KT>;
-    static constexpr int STAGES = ROWB > 256 ? 2 : 4;
+    static constexpr int STAGES = 2;
     static constexpr int Q_BYTES = 2 * R * Tile::QLD;
     static constexpr int STAGE = 2 * KT * Tile::LD;
     static constexpr int RING = STAGES + 1;  // of row offsets: a tile's outlive its copies
@@ -1010,7 +1013,6 @@ struct Share {
 struct Plan {
     int n = 0;
     Share share[2];
-    bool tensor = false;  // the wide tiles run on tcgen05
     size_t bytes = 0;
 };
 
@@ -1049,9 +1051,10 @@ static int rows_launch(int threads, size_t smem, bool pieces, const RowsArgs& a,
 // rows 316 against 253 (the sequences' rows fill half of one of its two query tiles).
 constexpr int NARROW_ROWS = 32;
 
-// FP16 pages with head_dim up to 128 have all wide tiles on tcgen05.
-template <typename KV, int HDP>
-constexpr bool has_wide = sizeof(KV) == 4 || HDP > 128;
+// Wide tiles run on tcgen05 for head_dim up to 128.  Above, S and O of two query tiles do not fit
+// into tensor memory, nor FP32 sums of a row into a thread's registers.
+template <int HDP>
+constexpr bool on_tcgen05 = HDP <= 128;
 
 template <typename KV, int HDP>
 static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
@@ -1080,12 +1083,10 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     } else {
         const int narrow = b->n_seqs == 1 || G > NARROW_ROWS ? 0 : NARROW_ROWS;
         if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
-        const bool tensor = tensor_takes<KV>(p->head_dim, p->page_size);
-        CutRule r = tensor_rule<KV>(p->head_dim, narrow + 1, ALL);
-        if constexpr (has_wide<KV, HDP>)
-            if (!tensor) r = wide_rule<KV, HDP>(narrow + 1, ALL);
+        CutRule r;
+        if constexpr (on_tcgen05<HDP>) r = tensor_rule<KV>(p->head_dim, narrow + 1, ALL);
+        else r = wide_rule<KV, HDP>(narrow + 1, ALL);
         add(r, seqs + rows / r.R);
-        plan.tensor = tensor;
     }
     return plan;
 }
@@ -1104,9 +1105,9 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         int r = IB_OK;
         if (!wide) {
             r = rows_launch<attn_narrow_kernel<KV, HDP>>(N::NT, N::SMEM, false, a, s.tiles, max_pos, st);
-        } else if (plan.tensor) {
+        } else if constexpr (on_tcgen05<HDP>) {
             r = attn_tensor_launch<KV>(a, s.tiles, max_pos, st);
-        } else if constexpr (has_wide<KV, HDP>) {
+        } else {
             using W = WideCfg<KV, HDP>;
             r = rows_launch<attn_wide_kernel<KV, HDP>>(W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
         }

@@ -362,9 +362,7 @@ __device__ __forceinline__ float pow2_scale(float top, float& inverse) {
     return plain ? 1.f : __uint_as_float((uint32_t)(8 - e + 127) << 23);
 }
 
-// Tiles of many rows on tcgen05, where head_dim and page size allow (paged_tensor.cu).
-template <typename KV>
-bool tensor_takes(int head_dim, int page_size);
+// Tiles of many rows on tcgen05, for head_dim up to 128 (paged_tensor.cu).
 template <typename KV>
 CutRule tensor_rule(int head_dim, int min_rows, int max_rows);
 template <typename KV>

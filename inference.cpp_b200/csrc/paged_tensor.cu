@@ -22,9 +22,9 @@
 // read with positions along it (MN-major) and so stored as it lies in the pages; TF32 operands are
 // K-major only, so FP32 V is turned round on the way.
 // Warps: 0-3 and 4-7 the softmax of a query tile each (thread = row), 8 issues the MMAs, the others
-// bring K and V in, with TMA in boxes of as many rows as divide both a page and the tile (8 at
-// least; a box of a page that is not there lies outside the tensor and reads as zeros).  FP16: 9-11,
-// row by row for other page sizes.  FP32: 9 by TMA, 10-15 split the parts.  In tiles where some row
+// bring K and V in, with TMA in boxes of as many rows as divide both a page and the tile (a box of
+// a page that is not there lies outside the tensor and reads as zeros).  FP16: 9-11, row by row
+// where boxes would have fewer than 8 rows.  FP32: 9 by TMA, 10-15 split the parts.  In tiles where some row
 // does not see a position, they make V finite before it is used (0 x inf).  The order of MMAs is
 //     O0(j) S0(j+1) O1(j) S1(j+1) O0(j+1) ...
 // so that a tile's softmax has the other tile's MMAs to hide behind, and FP16 O begins with the
@@ -276,7 +276,7 @@ __device__ __forceinline__ void pt_tma(uint32_t dst, const CUtensorMap* map, int
 struct TensorArgs {
     RowsArgs rows;
     CUtensorMap k, v;  // the layer's rows [page, kv head, position in page][head_dim]
-    int box;           // log2 of a box's rows, 0: no TMA (FP16 only)
+    int box;           // log2 of a box's rows; FP16: 0 for no TMA
 };
 
 struct TensorBars {
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
     if (tid == 0) {
-        if (TA.box) {
+        if (F32 || TA.box) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.k)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.v)) : "memory");
         }
@@ -871,19 +871,20 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             // ---- copies of FP32 pages: TMA brings K and V as they are ----
             const int box = TA.box, box_row = lane << box;
             const bool has_box = box_row < KT;
+            const bool singles = KT > 32 && box == 0;  // odd page sizes: two rows for a lane
             const uint32_t raw_a = ring + C::SLOTS * C::TILE;
             int issued = 0;  // tiles
             bool ok = true;
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
-                auto box_of = [&](int kt) -> int {  // this lane's box of key tile kt, -1: none
-                    const int pos = kt * KT + box_row;
-                    if (!has_box || kt >= it.kt1 || pos > last_lim) return -1;
+                auto row_of = [&](int kt, int row) -> int {  // in the layer; -1: no page, or not seen
+                    const int pos = kt * KT + row;
+                    if (row >= KT || kt >= it.kt1 || pos > last_lim) return -1;
                     const int col = (int)w.ps.div((uint32_t)pos);
                     const int page = page_at(w, it.s.row[col]);
                     return page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
                 };
-                int at = box_of(it.kt0);
+                int at = row_of(it.kt0, box_row);
                 // the softmax warps ask for the segment's q soon
                 for (int r = lane; r < it.rows; r += 32) {
                     const uint8_t* p = (const uint8_t*)q_row(A, it, G, it.row0 + r);
@@ -891,23 +892,32 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
                 }
                 for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++issued) {
-                    const int at_next = box_of(kt + 1);
+                    const int at_next = row_of(kt + 1, box_row);
+                    uint64_t none = __ballot_sync(0xffffffffu, has_box && at < 0);
+                    int at2 = -1;
+                    if (singles) {
+                        at2 = row_of(kt, lane + 32);
+                        none |= (uint64_t)__ballot_sync(0xffffffffu, at2 < 0) << 32;
+                    }
+                    uint32_t gone = 0;  // of positions 16 lane ..
+                    if (none)
+                        for (int r = 0; r < 16; ++r)
+                            gone |= (uint32_t)((none >> (((lane * 16 + r) >> box) & 63)) & 1) << r;
 #pragma unroll 1
                     for (int kv = 0; kv < 2 && ok; ++kv) {
                         if (issued > 0) ok = wait(&bar.raw_empty[kv], issued - 1);
                         if (!ok) break;
-                        if (kv == 0 && has_box)
-                            for (int b = 0; b < 1 << (box - 3); ++b)
-                                reinterpret_cast<uint8_t*>(sh_gone[issued & 3])[box_row / 8 + b] =
-                                    at < 0 ? 0xff : 0;
+                        if (kv == 0 && lane < KT / 16) sh_gone[issued & 3][lane] = (uint16_t)gone;
                         __syncwarp();
                         if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[kv], C::PLANE);
                         __syncwarp();
-                        if (has_box)
-                            pt_tma(raw_a + (uint32_t)(kv * C::PLANE + box_row * HDP * 4),
-                                   kv ? &TA.v : &TA.k, 0, at < 0 ? -KT : at, &bar.raw_full[kv]);
-                        if (kv == 1) at = at_next;
+                        const uint32_t to = raw_a + (uint32_t)(kv * C::PLANE + box_row * HDP * 4);
+                        const CUtensorMap* const map = kv ? &TA.v : &TA.k;
+                        if (has_box) pt_tma(to, map, 0, at < 0 ? -KT : at, &bar.raw_full[kv]);
+                        if (singles)
+                            pt_tma(to + 32 * HDP * 4, map, 0, at2 < 0 ? -KT : at2, &bar.raw_full[kv]);
                     }
+                    at = at_next;
                 }
             }
             // no copy may still be landing when the CTA ends (a count that stopped early: one each)
@@ -1058,15 +1068,12 @@ static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
     // a box: the largest power of two that divides the page, up to the tile
     int box = 0;
     while (2 << box <= C::KT && w.page_size % (2 << box) == 0) ++box;
-    if (box >= 3) {
+    if (C::F32 || box >= 3) {
         const int64_t rows = (int64_t)w.n_pages * w.Hkv * w.page_size;
         int r = tensor_map<KV, HDP>(&t.k, a.k, rows, w.HD, 1 << box);
         if (r == IB_OK) r = tensor_map<KV, HDP>(&t.v, a.v, rows, w.HD, 1 << box);
         if (r != IB_OK) return r;
         t.box = box;
-    } else if (C::F32) {  // not taken: tensor_takes
-        set_error("ib_attention_paged: no boxes for this page size");
-        return IB_ERR_INVALID;
     }
     static DeviceOnce once;
     IB_CUDA_CHECK(once.run([&] {
@@ -1075,14 +1082,6 @@ static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
     IB_CUDA_CHECK(launch_pdl(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, st, true, t));
     return IB_OK;
 }
-
-template <typename KV>
-bool tensor_takes(int head_dim, int page_size) {
-    // FP32 tiles come by TMA alone, in boxes of 8 rows or more
-    return head_dim <= 128 && (sizeof(KV) == 2 || page_size % 8 == 0);
-}
-template bool tensor_takes<float>(int, int);
-template bool tensor_takes<__half>(int, int);
 
 template <typename KV>
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st) {

@@ -585,6 +585,15 @@ def test_attention_holes_and_empty_rows(cuda, type_, q_lens):
 
 
 @TYPES
+@pytest.mark.parametrize("page", [1, 2, 5, 7, 12, 100])
+@pytest.mark.parametrize("HD", [64, 96])
+def test_attention_odd_pages_with_holes(cuda, type_, page, HD):
+    q_lens, ctx = [150, 1, 300, 40], [400, 70, 333, 40]
+    run_attention(cuda, type_, 8, 2, HD, page, q_lens, ctx, holes=0.3, seed=page)
+    run_attention(cuda, type_, 8, 2, HD, page, q_lens, ctx, holes=0.3, seed=page, spoil=True)
+
+
+@TYPES
 @pytest.mark.parametrize("q_lens", [[1, 1, 4], [150, 1, 66]])
 def test_attention_ignores_what_no_sequence_holds(cuda, type_, q_lens):
     run_attention(cuda, type_, 8, 2, 128, 24, q_lens, [400, 33, 70], holes=0.3, spoil=True)
