@@ -159,8 +159,7 @@ struct KvSeqsDev {
 // lowest first in list order; once an entry finds too few, it and every later entry that
 // needs pages get none.  status: 1 done, 0 no room, -1 refused.
 // What the entries need stays in shared memory: the kernel is a chain of dependent accesses (list,
-// length, table, refs, hand-out) and little else, 12 us with each step going back to global
-// memory.
+// length, table, refs, hand-out) and little else: 11 us for 96 children or slots with cold caches.
 template <bool FORK>
 __global__ void __launch_bounds__(KV_PLAN_THREADS)
     kv_assign_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ a,
@@ -318,7 +317,8 @@ struct PoolBytes {
 };
 
 // Second half of a fork: children's rows, reference counts and the filled rows of the
-// partial pages, one warp per (child, layer, k or v, kv head) of those.
+// partial pages, one warp per (child, layer, k or v, kv head) of those.  Bound by HBM once there are
+// many: 96 children of 22 layers 18 us, most of 119 MB read and written.
 __global__ void __launch_bounds__(KV_COPY_THREADS)
     kv_fork_kernel(const KvSeqsDev s, const PoolBytes pool, int n,
                    const int32_t* __restrict__ parents, const int32_t* __restrict__ children,
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
 }
 
 // One CTA per list entry.  The length is taken with an exchange, so a slot named twice is
-// released once.
+// released once.  A chain of four dependent accesses: 5 us for 96 slots with cold caches.
 __global__ void __launch_bounds__(KV_COPY_THREADS)
     kv_release_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ slots) {
     __shared__ int len;
@@ -460,7 +460,8 @@ __global__ void __launch_bounds__(KV_PLAN_THREADS)
     }
 }
 
-// Renames the tables and copies the moved pages, one warp per 4 KB of a page of a layer.
+// Renames the tables and copies the moved pages, one warp per 4 KB of a page of a layer.  Bound by
+// HBM: 1.04 GB read and written in 169 us, 6.17 TB/s, 0.94 of the measured rate.
 __global__ void __launch_bounds__(KV_COPY_THREADS)
     kv_compact_kernel(const int32_t* table, int32_t* table_out, int64_t n_entries, int n_pages,
                       const int32_t* __restrict__ map, const int32_t* __restrict__ moves,
@@ -521,7 +522,9 @@ __device__ __forceinline__ int seq_of_token(const PagedView& w, int t) {
 // RoPE on q and k (interleaved pairs, the reference's table, src/ops/cuda_kernels.cu:372-400)
 // and the write of k and v into the pages: one CTA per token, one thread per eight elements
 // of a head.  Bound by HBM (every element read once and written once): the loads of a
-// thread's elements are issued before the page is looked up.
+// thread's elements are issued before the page is looked up.  6798 prompt tokens (32 heads on 8,
+// head_dim 128, FP32) take 55 us in a graph, 6.1 TB/s, 0.93 of the measured rate; 64 single tokens
+// 4.1 us, a launch and its dependent loads.
 template <typename KV>
 __global__ void __launch_bounds__(256)
     kv_append_kernel(const PagedView w, const float* q, int64_t q_stride,
