@@ -175,8 +175,8 @@ __device__ __forceinline__ uint32_t pt_elect() {
     return x;
 }
 
-// 32 columns of this warp's 32 lanes, or 64; the wait is part of the statement, so that nothing
-// uses the registers before it.
+// 32 columns of this warp's 32 lanes; the wait is part of the statement, so that nothing uses the
+// registers before it.
 __device__ __forceinline__ void pt_read32(uint32_t at, float (&a)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
@@ -189,28 +189,6 @@ __device__ __forceinline__ void pt_read32(uint32_t at, float (&a)[32]) {
           "=f"(a[20]), "=f"(a[21]), "=f"(a[22]), "=f"(a[23]), "=f"(a[24]), "=f"(a[25]),
           "=f"(a[26]), "=f"(a[27]), "=f"(a[28]), "=f"(a[29]), "=f"(a[30]), "=f"(a[31])
         : "r"(at)
-        : "memory");
-}
-__device__ __forceinline__ void pt_read64(uint32_t at, float (&a)[32], float (&b)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-        "%28, %29, %30, %31}, [%64];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, "
-        "%41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, "
-        "%58, %59, %60, %61, %62, %63}, [%65];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(a[4]), "=f"(a[5]), "=f"(a[6]),
-          "=f"(a[7]), "=f"(a[8]), "=f"(a[9]), "=f"(a[10]), "=f"(a[11]), "=f"(a[12]), "=f"(a[13]),
-          "=f"(a[14]), "=f"(a[15]), "=f"(a[16]), "=f"(a[17]), "=f"(a[18]), "=f"(a[19]),
-          "=f"(a[20]), "=f"(a[21]), "=f"(a[22]), "=f"(a[23]), "=f"(a[24]), "=f"(a[25]),
-          "=f"(a[26]), "=f"(a[27]), "=f"(a[28]), "=f"(a[29]), "=f"(a[30]), "=f"(a[31]), "=f"(b[0]),
-          "=f"(b[1]), "=f"(b[2]), "=f"(b[3]), "=f"(b[4]), "=f"(b[5]), "=f"(b[6]), "=f"(b[7]),
-          "=f"(b[8]), "=f"(b[9]), "=f"(b[10]), "=f"(b[11]), "=f"(b[12]), "=f"(b[13]), "=f"(b[14]),
-          "=f"(b[15]), "=f"(b[16]), "=f"(b[17]), "=f"(b[18]), "=f"(b[19]), "=f"(b[20]),
-          "=f"(b[21]), "=f"(b[22]), "=f"(b[23]), "=f"(b[24]), "=f"(b[25]), "=f"(b[26]),
-          "=f"(b[27]), "=f"(b[28]), "=f"(b[29]), "=f"(b[30]), "=f"(b[31])
-        : "r"(at), "r"(at + 32)
         : "memory");
 }
 __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -521,23 +499,19 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                     for (int k = 0; k < 32; ++k)
                         if (!((see >> k) & 1)) s[k] = -INFINITY;
                 };
-                // The row's maximum over two chunks of 32 at a time; the last two stay for below.
-                // (Small loops: the softmax shares the instruction cache with the MMAs' thread.)
+                // The row's maximum, 32 columns at a time; the last ones stay for below.  (Small loops:
+                // the softmax shares the instruction cache with the MMAs' thread.)
                 float top = -INFINITY;
-                float s0[32], s1[32];
+                float sv[32];
 #pragma unroll 1
-                for (int i = 0; i < KT / 32; i += 2) {
-                    if constexpr (KT > 32) pt_read64(s_at + 32 * i, s0, s1);
-                    else pt_read32(s_at + 32 * i, s0);
-                    if (!all) {
-                        mask(s0, i);
-                        if constexpr (KT > 32) mask(s1, i + 1);
-                    }
+                for (int i = 0; i < KT / 32; ++i) {
+                    pt_read32(s_at + 32 * i, sv);
+                    if (!all) mask(sv, i);
                     float top1 = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        top = max3(top, s0[k], s0[k + 1]);
-                        if constexpr (KT > 32) top1 = max3(top1, s1[k], s1[k + 1]);
+                    for (int k = 0; k < 32; k += 4) {
+                        top = max3(top, sv[k], sv[k + 1]);
+                        top1 = max3(top1, sv[k + 2], sv[k + 3]);
                     }
                     top = fmaxf(top, top1);
                 }
@@ -547,15 +521,21 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                 const float off = none ? 0.f : (F32 ? 0.f : 10.f) - top * sc;
                 m = top;
                 float sum0 = 0.f, sum1 = 0.f;
-                auto weights = [&](float (&s)[32], int i) {
+#pragma unroll 1
+                for (int i = KT / 32 - 1; i >= 0; --i) {
+                    if (i < KT / 32 - 1) {
+                        pt_read32(s_at + 32 * i, sv);
+                        if (!all) mask(sv, i);
+                    }
 #pragma unroll
                     for (int c16 = 0; c16 < 2; ++c16) {
+                        const float* const s = sv + 16 * c16;
                         if constexpr (F32) {  // hi over the scores, lo KT columns on
                             uint32_t hi[16], lo[16];
 #pragma unroll
                             for (int k = 0; k < 16; k += 2) {
                                 float x, y;
-                                fma2(x, y, s[16 * c16 + k], s[16 * c16 + k + 1], sc, sc, off, off);
+                                fma2(x, y, s[k], s[k + 1], sc, sc, off, off);
                                 x = ex2(x), y = ex2(y);
                                 add2(sum0, sum1, x, y);
                                 split_tf32(x, hi[k], lo[k]);
@@ -568,7 +548,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
                                 float x, y;
-                                fma2(x, y, s[16 * c16 + 2 * k], s[16 * c16 + 2 * k + 1], sc, sc, off, off);
+                                fma2(x, y, s[2 * k], s[2 * k + 1], sc, sc, off, off);
                                 x = ex2(x), y = ex2(y);
                                 add2(sum0, sum1, x, y);
                                 const __half2 h = __floats2half2_rn(x, y);
@@ -580,19 +560,10 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                             pt_st16(s_at + 32 * i + 16 * c16, hl);
                         }
                     }
-                };
-#pragma unroll 1
-                for (int i = KT == 128 ? 2 : 0; i >= 0; i -= 2) {
-                    if constexpr (KT > 32) weights(s1, i + 1);
-                    weights(s0, i);
-                    if (i) {
-                        if constexpr (!F32) {  // O can begin
-                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                            pt_fence_before();
-                            mbar_arrive(&bar.p_half[t]);
-                        }
-                        pt_read64(s_at, s0, s1);
-                        if (!all) mask(s0, 0), mask(s1, 1);
+                    if (!F32 && i == KT / 64) {  // half of p: O can begin
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        pt_fence_before();
+                        mbar_arrive(&bar.p_half[t]);
                     }
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -945,7 +916,9 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         uint8_t* const tile = base_ptr + (ring - base) + slot * C::TILE;
                         const uint8_t* const raw = raw_ptr + kv * C::PLANE;
                         if (kv == 0) {
-#pragma unroll 4
+                            // (small loops: unrolled four and two times they missed the instruction
+                            // cache, 91 us against 84.5 for prompts on pages of 24)
+#pragma unroll 1
                             for (int i = sw * 32 + lane; i < C::PLANE / 16; i += 32 * C::SPLIT_WARPS) {
                                 const int r = i / (HDP / 4), d = (i % (HDP / 4)) * 4;
                                 const float4 x = *reinterpret_cast<const float4*>(raw + i * 16);
@@ -959,7 +932,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         } else {
                             uint32_t bad0 = 0, bad1 = 0;
                             // four positions of 32 dimensions at a time, a dimension to a lane
-#pragma unroll 2
+#pragma unroll 1
                             for (int u = sw; u < KT / 4 * (HDP / 32); u += C::SPLIT_WARPS) {
                                 const int p4 = u / (HDP / 32), d = (u % (HDP / 32)) * 32 + lane;
                                 float y[4];
