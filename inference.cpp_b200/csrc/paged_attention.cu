@@ -856,7 +856,7 @@ __device__ __forceinline__ void join_store(const JoinArgs& A, const SeqInfo& s, 
 
 // Tiles of 8 rows that find_item cut, into many parts where they are long: a CTA to a tile, WPR
 // warps to a row.  (A CTA to a row took 16 us against 6 on 64 single tokens: each of them plans.)
-// Two warps keep four CTAs on an SM for many tiles; four get through the parts of a few long
+// Two warps keep two CTAs on an SM for many tiles; four get through the parts of a few long
 // ones sooner.
 template <int WPR>
 __device__ __forceinline__ void join_parts(const JoinArgs& A, int item) {
