@@ -1039,11 +1039,14 @@ static int rows_launch(int threads, size_t smem, bool pieces, const RowsArgs& a,
 }
 
 // The kernels of a call, by the rows (new tokens x group) that a sequence may have: up to
-// NARROW_ROWS in tiles of eight on the narrow kernel, more on the wide one, by the caller's bound
-// one of them alone.  32 sequences over 200..4096 positions (32 heads on 8, head_dim 128, FP16),
-// narrow against tcgen05: with 16 rows 101 us against 197, with 32 rows 167 against 215, with 64
-// rows 316 against 253 (the sequences' rows fill half of one of its two query tiles).
-constexpr int NARROW_ROWS = 32;
+// narrow_rows in tiles of eight on the narrow kernel, more on the wide one, by the caller's bound
+// one of them alone.  32 sequences over 200..4096 positions, narrow against tcgen05:
+//   FP16 pages, 32 heads on 8, head_dim 128   32 rows 167 us against 199, 64 rows 316 against 207
+//   FP32 pages, 32 heads on 4, head_dim 64    32 rows 116 us against 128, 64 rows 197 against 130
+//   FP32 pages, 32 heads on 8, head_dim 128   32 rows 417 us against 377 (V is split for every
+//                                             tile of eight rows), 64 rows 734 against 391
+template <typename KV, int HDP>
+constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 
 // Wide tiles run on tcgen05 for head_dim up to 128.  Above, S and O of two query tiles do not fit
 // into tensor memory, nor FP32 sums of a row into a thread's registers.
@@ -1072,10 +1075,11 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
         s.ml_off = take((size_t)2 * r.n_pieces * r.R * sizeof(float2));
     };
     const int64_t rows = b->n_tokens * G;
-    if (most_q * G <= NARROW_ROWS) {
+    constexpr int NARROW = narrow_rows<KV, HDP>;
+    if (most_q * G <= NARROW) {
         add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
     } else {
-        const int narrow = b->n_seqs == 1 || G > NARROW_ROWS ? 0 : NARROW_ROWS;
+        const int narrow = b->n_seqs == 1 || G > NARROW ? 0 : NARROW;
         if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
         CutRule r;
         if constexpr (on_tcgen05<HDP>) r = tensor_rule<KV>(p->head_dim, narrow + 1, ALL);
