@@ -50,6 +50,7 @@
 #include "mma_tile.cuh"
 #include "paged.cuh"
 #include "paged_plan.cuh"
+#include "paged_ring.h"
 #include "pdl.cuh"
 #include "pipeline.cuh"
 
@@ -259,7 +260,7 @@ struct TensorArgs {
 
 struct TensorBars {
     uint64_t kv_full[3], kv_empty[3], raw_full[2], raw_empty[2];
-    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], seg_done[2], v_there, done;
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], seg_done[2], v_there[3], done;
 };
 
 template <typename KV, int HDP>
@@ -299,6 +300,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
         for (int i = 0; i < C::SLOTS; ++i) {
             mbar_init(&bar.kv_full[i], 33 * C::FILL_WARPS);
             mbar_init(&bar.kv_empty[i], 1);
+            mbar_init(&bar.v_there[Looks::bar(i)], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.raw_full[i], 1);
@@ -310,7 +312,6 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             mbar_init(&bar.o_full[i], 1);
             mbar_init(&bar.seg_done[i], 128);
         }
-        mbar_init(&bar.v_there, 1);
         mbar_init(&bar.done, 1);
         fence_mbar_init();
     }
@@ -717,7 +718,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             const bool has_box = box && box_row < KT;
             int half = 0;
             uint32_t tile_no = 0;
-            int n_look = 0;
+            Looks looks;  // at V tiles, each on a barrier of its slot
             bool ok = true;
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
@@ -756,7 +757,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         const bool look = kv == 1 && careful;  // V to be looked through
                         const uint32_t tile_at = ring + (uint32_t)(slot * C::TILE);
                         if (box) {
-                            uint64_t* const there = look ? &bar.v_there : &bar.kv_full[slot];
+                            uint64_t* const there =
+                                look ? &bar.v_there[Looks::bar(slot)] : &bar.kv_full[slot];
                             if (lw == 0) {
                                 if (lane == 0) mbar_arrive_expect_tx(there, C::TILE);
                                 __syncwarp();
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                                                 box_at < 0 ? 0xff : 0;
                                 }
                             }
-                            if (look && !wait(&bar.v_there, n_look++)) {
+                            if (look && !wait(&bar.v_there[Looks::bar(slot)], looks.take(slot))) {
                                 ok = false;
                                 break;
                             }

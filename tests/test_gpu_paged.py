@@ -633,6 +633,16 @@ def test_attention_wide_range_of_values(cuda, type_):
         assert bool(((out.double() - ref).abs() <= tol).all()), size
 
 
+@TYPES
+@pytest.mark.parametrize("HD", [64, 128])
+def test_attention_diagonal_over_several_key_tiles(cuda, type_, HD):
+    """Without groups a tile's 256 rows see the ends of two and more key tiles in a row, all of
+    which are looked through for values that are not finite."""
+    for _ in range(3):
+        run_attention(cuda, type_, 8, 8, HD, 16, [900, 40, 700], [1500, 2000, 700], spoil=True)
+        run_attention(cuda, type_, 2, 2, HD, 128, [3000], [3100], spoil=True)
+
+
 def test_attention_fp32_pages_past_the_fp16_range(cuda):
     rng = random.Random(1)
     seqs, batch, table, slots, n_pages, cu = make(cuda, rng, 16, [1, 70], [300, 200])

@@ -131,3 +131,34 @@ def test_python_handles_refuse_host_tensors():
         ib.KVPages.empty(1, 2, 1, 4, 8, ib.Q8_0)
     with pytest.raises(ValueError, match="cpu"):
         ib.KVBatch(torch.zeros(2, dtype=torch.int32), 1)
+
+
+def _ring_test(tmp_path, *args):
+    import os
+    import shutil
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = str(tmp_path / "copy_ring_test")
+    r = subprocess.run([gxx, "-std=c++17", "-O2", "-Wall", "-Werror", "-I",
+                        os.path.join(root, "inference.cpp_b200", "csrc"),
+                        os.path.join(root, "tests", "cpp", "copy_ring_test.cpp"), "-o", exe],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe, *args], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
+    return r.stdout
+
+
+def test_copies_of_the_tensor_kernel_never_lose_a_wait(tmp_path):
+    """Every interleaving of the copying warps, the TMA and the MMAs, with the kernel's own
+    assignment of look barriers to ring slots."""
+    assert "0 of the patterns" in _ring_test(tmp_path)
+
+
+def test_the_search_finds_a_shared_look_barrier(tmp_path):
+    """The same search on one look barrier for all slots: two careful key tiles in a row can
+    lap a warp."""
+    assert "2 key tiles, careful 3: a wait that never ends" in _ring_test(tmp_path, "shared")
