@@ -719,6 +719,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             int half = 0;
             uint32_t tile_no = 0;
             Looks looks;  // at V tiles, each on a barrier of its slot
+            bool looking = false;  // such a wait ran out
             bool ok = true;
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
@@ -773,7 +774,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                                 }
                             }
                             if (look && !wait(&bar.v_there[Looks::bar(slot)], looks.take(slot))) {
-                                ok = false;
+                                ok = false, looking = true;
                                 break;
                             }
                         } else {
@@ -838,15 +839,17 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             }
             // no copy may still be landing when the CTA ends
             asm volatile("cp.async.wait_all;" ::: "memory");
-            for (int h = max(0, half - C::SLOTS); h < half; ++h)
-                wait(&bar.kv_full[h % C::SLOTS], h / C::SLOTS);
+            drain_copies<C::SLOTS>(
+                half, looking, looks, [&](int slot, int use) { wait(&bar.kv_full[slot], use); },
+                [&](int slot, int parity) { wait(&bar.v_there[Looks::bar(slot)], parity); });
         } else if (warp == 9) {
             // ---- copies of FP32 pages: TMA brings K and V as they are ----
             const int box = TA.box, box_row = lane << box;
             const bool has_box = box_row < KT;
             const bool singles = KT > 32 && box == 0;  // odd page sizes: two rows for a lane
             const uint32_t raw_a = ring + C::SLOTS * C::TILE;
-            int issued = 0;  // tiles
+            int issued = 0;  // key tiles
+            RawSent sent;
             bool ok = true;
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
@@ -883,6 +886,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         if (kv == 0 && lane < KT / 16) sh_gone[issued & 3][lane] = (uint16_t)gone;
                         __syncwarp();
                         if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[kv], C::PLANE);
+                        sent.add(kv);
                         __syncwarp();
                         const uint32_t to = raw_a + (uint32_t)(kv * C::PLANE + box_row * HDP * 4);
                         const CUtensorMap* const map = kv ? &TA.v : &TA.k;
@@ -893,9 +897,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                     at = at_next;
                 }
             }
-            // no copy may still be landing when the CTA ends (a count that stopped early: one each)
-            for (int kv = 0; kv < 2; ++kv)
-                if (issued > 0) wait(&bar.raw_full[kv], issued - 1);
+            // no copy may still be landing when the CTA ends
+            sent.drain([&](int kv, int phase) { wait(&bar.raw_full[kv], phase); });
         } else {
             // ---- and these warps split them into TF32 parts, hi in a slot's first half, lo in the
             // second.  K: rows are positions, 128 bytes 32 dimensions.  V is turned round, since TF32

@@ -60,6 +60,36 @@ struct State {
     }
 };
 
+// Warp 9 leaves wherever one of its waits runs out: every copy of its own that may still be landing
+// then has to be among those that it waits for before the CTA ends.
+static bool drained(const State<ib::Looks>& s) {
+    const auto& me = s.warp[0];
+    if (me.at != 0 && me.at != 2) return true;
+    ib::Looks looks = me.looks;
+    if (me.at == 2) looks.take(me.half % SLOTS);
+    bool full[SLOTS] = {}, look[SLOTS] = {};  // waits that cannot pass before the bytes are there
+    ib::drain_copies<SLOTS>(
+        me.half, me.at == 2, looks,
+        [&](int slot, int use) { full[slot] = (s.full[slot].phase & 1) == (use & 1); },
+        [&](int slot, int parity) { look[slot] = (s.look[slot].phase & 1) == parity; });
+    for (int h = 0; h < 2 * 8; ++h)
+        if (s.landing[h] && !(s.landing[h] == 2 ? look[h % SLOTS] : full[h % SLOTS])) return false;
+    return true;
+}
+static bool drained(const State<SharedLooks>&) { return true; }
+
+static bool raw_drained() {
+    ib::RawSent sent;
+    for (int i = 0, issued = 0; i < 6; ++i) {  // K, V, K, V ...: leaving before each of them
+        int k = -1, v = -1;
+        sent.drain([&](int kv, int phase) { (kv ? v : k) = phase; });
+        if (k != (issued + 1) / 2 - 1 || v != issued / 2 - 1) return false;
+        sent.add(i & 1);
+        ++issued;
+    }
+    return true;
+}
+
 static bool passes(const Bar& b, int parity) { return (b.phase & 1) != (parity & 1); }
 
 template <typename L>
@@ -78,6 +108,7 @@ static int search(int tiles, unsigned careful) {
         const S s = todo.back();
         todo.pop_back();
         bool moved = false;
+        if (!drained(s)) bad = 3;
         for (int w = 0; w < WARPS; ++w) {
             const auto& me = s.warp[w];
             if (me.half == halves) continue;
@@ -144,13 +175,15 @@ static int search(int tiles, unsigned careful) {
     }
     if (bad)
         printf("%d key tiles, careful %x: %s\n", tiles, careful,
-               bad == 2 ? "a wait that never ends" : "a wait that passes in another phase");
+               bad == 3   ? "a copy that nobody waits for"
+               : bad == 2 ? "a wait that never ends"
+                          : "a wait that passes in another phase");
     return bad;
 }
 
 int main(int argc, char** argv) {
     const bool shared = argc > 1 && !strcmp(argv[1], "shared");
-    int found = 0;
+    int found = !raw_drained();
     for (int tiles = 1; tiles <= 5; ++tiles)
         for (unsigned careful = 0; careful < 1u << tiles; ++careful)
             found += (shared ? search<SharedLooks>(tiles, careful)
