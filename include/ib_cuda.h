@@ -314,6 +314,8 @@ int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_b
  * of 4, 16-byte aligned); out may be q itself.  A NaN or infinity in a position that a row
  * does not see leaves the row alone; in one that it sees, the row's outputs are not specified
  * (NaN, as a rule).
+ * q, K and V may be of any finite size; the division by the sum of weights comes last, so
+ * the sum of e^(s - largest s) |v| over a row's positions has to stay below FP32's largest value.
  * workspace: ib_attention_paged_workspace(...) bytes, 256-byte aligned, that no other call
  * uses at the same time; it needs no initial value. */
 size_t ib_attention_paged_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,

@@ -55,11 +55,33 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
           "f"(c[2]), "f"(c[3]));
 }
 
-// x as TF32 parts: hi rounded to TF32's 10 mantissa bits (half a step added to the
-// bits, the rest cut), lo the exact remainder, of which the MMA reads the upper 10 bits.
+// FP32 operands as TF32 parts for three MMAs, hi hi + hi lo + lo hi, with 2^-20 of the product kept:
+// what the parts leave out is 2^-22 of each operand, and lo lo is 2^-22 of the product, or 2^-21 where
+// one operand is cut (its lo may be twice as large, the other's then has either sign).
+
+// hi rounded to TF32's 10 mantissa bits (half a step added to the bits, the rest cut); of lo, exact,
+// the MMA reads the upper 10 bits.  The largest values would round up to infinity: their hi is TF32's
+// largest instead.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    float y;  // the smaller magnitude, with x's sign
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(__uint_as_float(0x7f7fefffu)));
+    hi = (__float_as_uint(y) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+
+// The same for |x| up to 2^127 (weights of a softmax).
+__device__ __forceinline__ void split_tf32_weight(float x, uint32_t& hi, uint32_t& lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+
+// hi cut and lo, below 2^-10 of it, rounded: any size with the instructions of split_tf32_weight,
+// for the mma.sync kernels, where each warp splits what it multiplies (64 single tokens 233 us,
+// 241 with split_tf32).  hi + lo can be 2^128 for the largest values: sums of products with hi and with
+// lo are added towards zero.
+__device__ __forceinline__ void split_tf32_cut(float x, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
 }
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,

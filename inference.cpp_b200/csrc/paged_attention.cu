@@ -155,7 +155,7 @@ struct WarpRows {
                     ldsm_x4(kd + (uint32_t)((n * 8 + (lane & 7)) * LD + k * 32 + (lane >> 3) * 16),
                             b[0], b[1], b[2], b[3]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(b[j]), h[j], r[j]);
+                    for (int j = 0; j < 4; ++j) split_tf32_cut(__uint_as_float(b[j]), h[j], r[j]);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         mma_tf32(t[n], ah[j], h[2 * j], h[2 * j + 1], t[n]);
@@ -234,10 +234,10 @@ struct WarpRows {
             uint32_t ph[NB][4], pl[NB][4];
 #pragma unroll
             for (int k = 0; k < NB; ++k) {
-                split_tf32(s[k][0], ph[k][0], pl[k][0]);
-                split_tf32(s[k][2], ph[k][1], pl[k][1]);
-                split_tf32(s[k][1], ph[k][2], pl[k][2]);
-                split_tf32(s[k][3], ph[k][3], pl[k][3]);
+                split_tf32_weight(s[k][0], ph[k][0], pl[k][0]);
+                split_tf32_weight(s[k][2], ph[k][1], pl[k][1]);
+                split_tf32_weight(s[k][1], ph[k][2], pl[k][2]);
+                split_tf32_weight(s[k][3], ph[k][3], pl[k][3]);
             }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
@@ -253,14 +253,15 @@ struct WarpRows {
                         if (!(fabsf(y1) < INFINITY)) odd = true, y1 = 0.f;
                     }
                     uint32_t h0, r0, h1, r1;
-                    split_tf32(y0, h0, r0);
-                    split_tf32(y1, h1, r1);
+                    split_tf32_cut(y0, h0, r0);
+                    split_tf32_cut(y1, h1, r1);
                     mma_tf32(t[0], ph[k], h0, h1, t[0]);
                     mma_tf32(r[0], ph[k], r0, r1, r[0]);
                     mma_tf32(r[0], pl[k], h0, h1, r[0]);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) t[0][j] += r[0][j];
+                for (int j = 0; j < 4; ++j)  // towards zero: split_tf32_cut
+                    t[0][j] = __fadd_rz(t[0][j], r[0][j]);
                 add(d, t[0], c);
             }
         }
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
                 uint32_t ah[4], al[4];
                 if constexpr (F32) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
+                    for (int j = 0; j < 4; ++j) split_tf32_cut(__uint_as_float(a[j]), ah[j], al[j]);
                 }
                 uint32_t q0, q1, r0, r1;
                 if constexpr (C::QREG) {
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
                 const int from = 8 * t4 + 4 * j + (g >> 1);
                 const float x = __shfl_sync(0xffffffffu, s[2 * i], from);
                 const float y = __shfl_sync(0xffffffffu, s[2 * i + 1], from);
-                split_tf32(g & 1 ? y : x, ph[2 * i + j], pl[2 * i + j]);
+                split_tf32_weight(g & 1 ? y : x, ph[2 * i + j], pl[2 * i + j]);
             }
         } else {
 #pragma unroll
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
                             v_ptr + (i * 8 + 2 * t4 + (j >> 1)) * LD +
                             (d * 16 + g + 8 * (j & 1)) * 4);
                         if (CHECK && !(fabsf(y) < INFINITY)) odd = true, y = 0.f;
-                        split_tf32(y, a[i][j], al[i][j]);
+                        split_tf32_cut(y, a[i][j], al[i][j]);
                     }
                 } else {
                     ldsm_x4_t(vd + v_frag + d * 32, a[0][0], a[0][1], a[0][2], a[0][3]);
@@ -618,7 +619,8 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
                     mma_tf32(r, a[1], pl[2], pl[3], r);
                     mma_tf32(r, al[1], ph[2], ph[3], r);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) t[j] += r[j];
+                    for (int j = 0; j < 4; ++j)  // towards zero: split_tf32_cut
+                        t[j] = __fadd_rz(t[j], r[j]);
                 } else {
                     mma_f16(t, a[0], pl[0], pl[1], none);
                     mma_f16(t, a[0], ph[0], ph[1], t);

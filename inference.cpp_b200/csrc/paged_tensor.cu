@@ -519,7 +519,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                 top = fmaxf(m, top);  // of the scores before scaling
                 const bool none = top == -INFINITY;
                 const float c = none ? 1.f : ex2((m - top) * sc);
-                const float off = none ? 0.f : (F32 ? 0.f : 10.f) - top * sc;
+                // (FP32: rounded down, so that no p is above 1, which the largest V values need)
+                const float off = none ? 0.f : F32 ? __fmul_rd(-top, sc) : fmaf(-top, sc, 10.f);
                 m = top;
                 float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll 1
@@ -539,8 +540,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                                 fma2(x, y, s[k], s[k + 1], sc, sc, off, off);
                                 x = ex2(x), y = ex2(y);
                                 add2(sum0, sum1, x, y);
-                                split_tf32(x, hi[k], lo[k]);
-                                split_tf32(y, hi[k + 1], lo[k + 1]);
+                                split_tf32_weight(x, hi[k], lo[k]);
+                                split_tf32_weight(y, hi[k + 1], lo[k + 1]);
                             }
                             pt_st16(s_at + 32 * i + 16 * c16, hi);
                             pt_st16(s_at + KT + 32 * i + 16 * c16, lo);

@@ -1003,3 +1003,61 @@ def test_a_serving_run(cuda, type_):
     ib.kv_release(pages, seqs, i32(cuda, range(n_slots)))
     assert not bool(seqs.refs.any()) and bool((seqs.table == -1).all())
     assert ib.check_fault() == 0
+
+
+# ---- the largest FP32 values -------------------------------------------------------------
+
+LARGEST = 3.4028234663852886e38  # every FP32 value within 2^-12 of it rounds up in TF32
+
+
+@pytest.mark.parametrize("n,H,HD", [(6, 4, 64), (140, 8, 128), (300, 2, 64), (40, 8, 48), (5, 4, 256),
+                                    (90, 4, 256)])
+@pytest.mark.parametrize("what", [LARGEST, -LARGEST, 3.4023e38])
+def test_attention_rows_do_not_see_later_largest_values(cuda, n, H, HD, what):
+    """The last token's K and V are the type's largest: every row before it is as without it."""
+    ctx = n + 50
+    pages, seqs, batch, q, out, scale = run_attention(cuda, ib.F32, H, 2, HD, 16, [n], [ctx])
+    page = seqs.table[batch.slots[0].item(), (ctx - 1) // 16].item()
+    for x in (pages.k, pages.v):
+        x[1, page, :, (ctx - 1) % 16] = what
+    again = cuda.empty_like(q.contiguous())
+    ib.attention_paged(pages, seqs, batch, 1, q, scale, out=again)
+    assert cuda.equal(again[:n - 1], out[:n - 1])
+
+
+@pytest.mark.parametrize("HD", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 70])
+def test_attention_of_the_largest_values(cuda, n, HD):
+    """Seen values of that size are kept like any other: q, K and V at the top of the range, in
+    products that stay in it."""
+    rng = random.Random(n)
+    ctx = n + 20
+    seqs, batch, table, slots, n_pages, cu = make(cuda, rng, 16, [n], [ctx])
+    gen = cuda.Generator(device="cuda").manual_seed(n)
+
+    def check(pages, q, scale):
+        out = ib.attention_paged(pages, seqs, batch, 1, q, scale)
+        ref, tol = attention_ref(cuda, pages, 1, table, slots, cu, [n], [ctx], q, scale)
+        assert bool(out.isfinite().all()) and bool(((out.double() - ref).abs() <= tol).all())
+
+    # K: one component of the largest size against a q whose products stay in range
+    pages = pool(cuda, 2, n_pages, 2, 16, HD, ib.F32, 3)
+    sign = cuda.randn(pages.k.shape[:-1], generator=gen, device="cuda").sign()
+    pages.k.zero_()
+    pages.k[..., 3] = sign * LARGEST
+    q = cuda.zeros(n, 4, HD, device="cuda")
+    q[..., 3] = cuda.rand(n, 4, generator=gen, device="cuda") * 2.0 ** -100
+    check(pages, q, 2.0 ** -27)
+    # q: the same the other way round
+    pages.k[..., 3] = sign * 2.0 ** -100
+    q[..., 3] = LARGEST
+    check(pages, q, 2.0 ** -27)
+    # V: the first position takes the weight, with products that cannot add up past the range
+    pages = pool(cuda, 2, n_pages, 2, 16, HD, ib.F32, 3)
+    pages.k.zero_()
+    pages.k[1, table[slots[0]][0], :, 0, 0] = 100.0
+    pages.v[1, table[slots[0]][0], :, 0] = LARGEST * cuda.randn(2, HD, generator=gen, device="cuda").sign()
+    q = cuda.zeros(n, 4, HD, device="cuda")
+    q[..., 0] = 2.0
+    check(pages, q, 1.0)
+    assert ib.check_fault() == 0
