@@ -254,8 +254,9 @@ typedef struct {
 
 /* A step's new tokens: rows cu_q[b] .. cu_q[b + 1] of the step's tensors are the LAST tokens
  * of sequence b, which is slot slots[b] (or slot b when slots is NULL; no slot twice), and
- * are already counted in its len.  cu_q [n_seqs + 1] and slots are device memory.  n_tokens:
- * rows of the tensors; rows from cu_q[n_seqs] on belong to nobody and are left as they were.
+ * are already counted in its len.  Where slots[b] is -1 they belong to nobody, as do rows from
+ * cu_q[n_seqs] on: nothing is written for them, and their rows of results are left as they
+ * were.  cu_q [n_seqs + 1] and slots are device memory.  n_tokens: rows of the tensors.
  * max_q: the most tokens of one sequence where the caller knows it (0: n_tokens); it chooses
  * kernels, results do not depend on it beyond rounding.  n_tokens * n_heads <= 2^26,
  * n_heads <= 1024. */
@@ -273,7 +274,10 @@ typedef struct {
  * pages that this takes are entered in its row, with refs 1.  Free pages go out lowest first,
  * in list order; once an entry finds too few, it and all later ones that need any get none.
  * status[i]: 1 done, 0 no room (in the pool or in the row), -1 refused (slot out of range or
- * named by an earlier entry, n_new < 0). */
+ * named by an earlier entry, n_new < 0).
+ * A sequence without status 1 keeps its length, so a step that went on with it would take the
+ * last tokens that it has for new ones and write over them.  The step's batch has to leave it
+ * out: ib_kv_granted makes its slots without the host looking at the status. */
 int ib_kv_extend(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const int32_t* slots,
                  const int32_t* n_new, int32_t* status, void* stream);
 /* ib_kv_fork: children[i] becomes a copy of parents[i]: whole pages are shared (refs + 1), the
@@ -282,6 +286,12 @@ int ib_kv_extend(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const 
  * parent, is not empty (len > 0) or was named by an earlier entry. */
 int ib_kv_fork(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const int32_t* parents,
                const int32_t* children, int32_t* status, void* stream);
+/* ib_kv_granted: granted[i] = slots[i] where status[i] is 1, -1 elsewhere, for a list of slots
+ * (children) and the status that ib_kv_extend (ib_kv_fork) left for it: as a batch's slots it
+ * leaves out the sequences that got no room, and ib_kv_extend refuses its -1 in turn.  granted
+ * may be slots. */
+int ib_kv_granted(int n, const int32_t* slots, const int32_t* status, int32_t* granted,
+                  void* stream);
 /* ib_kv_release: the slots give up their pages (refs - 1) and are empty. */
 int ib_kv_release(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const int32_t* slots,
                   void* stream);

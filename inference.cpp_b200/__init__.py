@@ -115,6 +115,7 @@ SIGNATURES = {
     "ib_attention_split": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _f, _vp, _vp, _vp],
     "ib_kv_extend": [_vp, _vp, _i, _vp, _vp, _vp, _vp],
     "ib_kv_fork": [_vp, _vp, _i, _vp, _vp, _vp, _vp],
+    "ib_kv_granted": [_i, _vp, _vp, _vp, _vp],
     "ib_kv_release": [_vp, _vp, _i, _vp, _vp],
     "ib_kv_compact": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "ib_kv_append": [_vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i,
@@ -598,8 +599,9 @@ class KVSeqs:
 
 class KVBatch:
     """A step's new tokens: rows cu_q[b] .. cu_q[b + 1] of its n_tokens rows are the last
-    tokens of sequence b (slot slots[b], or slot b).  cu_q, slots: int32 CUDA tensors.  max_q:
-    the most tokens of one sequence where known (chooses kernels only)."""
+    tokens of sequence b (slot slots[b], or slot b; -1: left out of the step, kv_granted).  cu_q,
+    slots: int32 CUDA tensors.  max_q: the most tokens of one sequence where known (chooses
+    kernels only)."""
 
     def __init__(self, cu_q, n_tokens, max_q=0, slots=None):
         import torch
@@ -656,7 +658,8 @@ def _paged_list(pages, t, name, n):
 
 def kv_extend(pages, seqs, slots, n_new, status=None, stream=None):
     """Room for n_new[i] more tokens of each slot; returns status (1 done, 0 no room,
-    -1 refused), int32 tensors on the pages' device."""
+    -1 refused), int32 tensors on the pages' device.  A step must not go on with a sequence that
+    got no room (its last tokens would be written over): kv_granted makes the batch's slots."""
     if status is None:
         with _allocating(pages, stream):
             status = _torch().empty_like(slots)
@@ -680,6 +683,19 @@ def kv_fork(pages, seqs, parents, children, status=None, stream=None):
     st = _paged_stream(pages, stream, seqs)
     _call("ib_kv_fork", pages._p, _seqs_of(pages, seqs), n, a, b, c, st)
     return status
+
+
+def kv_granted(pages, slots, status, out=None, stream=None):
+    """slots with -1 where status (of kv_extend, or of kv_fork for its children) is not 1: the
+    slots of a step's batch, or of the kv_extend behind a kv_fork.  out may be slots."""
+    n = slots.numel()
+    if out is None:
+        with _allocating(pages, stream):
+            out = _torch().empty_like(slots)
+    a, b, c = (_paged_list(pages, slots, "slots", n), _paged_list(pages, status, "status", n),
+               _paged_list(pages, out, "out", n))
+    _call("ib_kv_granted", n, a, b, c, _paged_stream(pages, stream))
+    return out
 
 
 def kv_release(pages, seqs, slots, stream=None):

@@ -361,6 +361,13 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
     }
 }
 
+__global__ void __launch_bounds__(KV_COPY_THREADS)
+    kv_granted_kernel(int n, const int32_t* slots, const int32_t* __restrict__ status,
+                      int32_t* granted) {  // may be slots
+    const int i = blockIdx.x * KV_COPY_THREADS + threadIdx.x;
+    if (i < n) granted[i] = status[i] == 1 ? slots[i] : -1;
+}
+
 // One CTA per list entry.  The length is taken with an exchange, so a slot named twice is
 // released once.  A chain of four dependent accesses: 5 us for 96 slots with cold caches.
 __global__ void __launch_bounds__(KV_COPY_THREADS)
@@ -661,6 +668,17 @@ extern "C" int ib_kv_fork(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int 
         (int64_t)sms * 8, std::max<int64_t>(n, (warps + KV_COPY_THREADS / 32 - 1) / (KV_COPY_THREADS / 32)));
     IB_CUDA_CHECK(launch_pdl(kv_fork_kernel, dim3(grid), dim3(KV_COPY_THREADS), 0, st, true, s,
                              pool_bytes(pages), n, parents, children, (const int32_t*)status));
+    return IB_OK;
+}
+
+extern "C" int ib_kv_granted(int n, const int32_t* slots, const int32_t* status, int32_t* granted,
+                             void* stream) {
+    if (n == 0) return IB_OK;
+    const int r = check_list(n, slots && status ? granted : nullptr, "ib_kv_granted");
+    if (r != IB_OK) return r;
+    kv_granted_kernel<<<(n + KV_COPY_THREADS - 1) / KV_COPY_THREADS, KV_COPY_THREADS, 0,
+                        as_stream(stream)>>>(n, slots, status, granted);
+    IB_LAUNCH_CHECK("kv_granted_kernel");
     return IB_OK;
 }
 

@@ -74,7 +74,8 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedView& w, int b) {
     s.n = min(max(e, s.q0), w.n_tokens) - s.q0;
     if (s.q0 != a || s.q0 + s.n != e) paged_fault(PAGED_BAD_LEN);
     if (slot < 0 || slot >= w.n_slots) {
-        paged_fault(PAGED_BAD_SLOT);
+        if (slot == -1) s.n = 0;  // left out of the step: its rows are nobody's
+        else paged_fault(PAGED_BAD_SLOT);
         s.L = 0;
         s.row = w.table;
         return s;

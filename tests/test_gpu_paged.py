@@ -1061,3 +1061,130 @@ def test_attention_of_the_largest_values(cuda, n, HD):
     q[..., 0] = 2.0
     check(pages, q, 1.0)
     assert ib.check_fault() == 0
+
+
+# ---- sequences that got no room ------------------------------------------------------------
+
+def test_granted(cuda):
+    pages = pool(cuda, 1, 4, 1, 4, 8, ib.F16, 0)
+    slots, status = list(range(700)), [(i * 7) % 3 - 1 for i in range(700)]
+    want = [s if st == 1 else -1 for s, st in zip(slots, status)]
+    a = i32(cuda, slots)
+    assert ib.kv_granted(pages, a, i32(cuda, status)).tolist() == want
+    assert a.tolist() == slots
+    assert ib.kv_granted(pages, a, i32(cuda, status), out=a) is a and a.tolist() == want
+    assert ib.kv_granted(pages, i32(cuda, []), i32(cuda, [])).tolist() == []
+    with pytest.raises(ValueError, match="shape"):
+        ib.kv_granted(pages, a, i32(cuda, [1]))
+    with pytest.raises(ValueError, match="dtype"):
+        ib.kv_granted(pages, a, a.long())
+
+
+@TYPES
+@pytest.mark.parametrize("q_lens", [[1, 1, 1, 1], [9, 130, 1, 40], [40, 300, 64, 90]])
+def test_a_step_leaves_out_what_got_no_room(cuda, type_, q_lens):
+    """Entry 1 and the last of a step get no room: whatever kernel takes the step, their cache
+    and their rows stay as they were, and the others' are as in a step without them."""
+    H, Hkv, HD, page = 8, 2, 64, 16
+    first = [50, 33, 70, 20]
+    book = Book(4, 40, 60, page)
+    assert book.extend(range(4), first) == [1] * 4
+    seqs = seqs_of(cuda, book)
+    pages = pool(cuda, 2, 60, Hkv, page, HD, type_, 3)
+    slots = i32(cuda, [2, 0, 3, 1])  # entry b is slot slots[b]
+    status = i32(cuda, [1, 0, 1, -1])
+    grow = [n if st == 1 else 0 for n, st in zip(q_lens, [1, 0, 1, -1])]
+    assert book.extend([2, 0, 3, 1], grow) == [1] * 4
+    seqs = seqs_of(cuda, book)
+    cu = [0]
+    for n in q_lens:
+        cu.append(cu[-1] + n)
+    T = cu[-1]
+    granted = ib.kv_granted(pages, slots, status)
+    batch = ib.KVBatch(i32(cuda, cu), T, max_q=max(q_lens), slots=granted)
+    gen = cuda.Generator(device="cuda").manual_seed(7)
+    qkv = cuda.randn(T, H + 2 * Hkv, HD, generator=gen, device="cuda")
+    q, k, v = qkv.split([H, Hkv, Hkv], dim=1)
+    rope = rope_table(cuda, 640, HD)
+    k0, v0 = pages.k.clone(), pages.v.clone()
+    rot = ib.kv_append(pages, seqs, batch, 1, q, k, v, rope, q_out=cuda.full_like(q, 3.0))
+    out = ib.attention_paged(pages, seqs, batch, 1, rot, 0.125, out=cuda.full_like(q, 5.0))
+    for b in (1, 3):
+        rows = slice(cu[b], cu[b + 1])
+        assert bool((rot[rows] == 3).all()) and bool((out[rows] == 5).all())
+        for t in book.table[[2, 0, 3, 1][b]]:
+            if t >= 0:
+                assert cuda.equal(pages.k[:, t], k0[:, t]) and cuda.equal(pages.v[:, t], v0[:, t])
+    # the same step of entries 0 and 2 alone
+    keep = cuda.cat([cuda.arange(cu[b], cu[b + 1], device="cuda") for b in (0, 2)])
+    n0 = q_lens[0]
+    pages2 = ib.KVPages(k0, v0)
+    batch2 = ib.KVBatch(i32(cuda, [0, n0, n0 + q_lens[2]]), n0 + q_lens[2],
+                        max_q=max(n0, q_lens[2]), slots=i32(cuda, [2, 3]))
+    rot2 = ib.kv_append(pages2, seqs, batch2, 1, q[keep], k[keep], v[keep], rope)
+    assert cuda.equal(rot2, rot[keep])
+    assert cuda.equal(pages2.k, pages.k) and cuda.equal(pages2.v, pages.v)
+    ctx = [book.len[2], book.len[3]]
+    ref, tol = attention_ref(cuda, pages, 1, book.table, [2, 3], [0, n0, n0 + q_lens[2]],
+                             [n0, q_lens[2]], ctx, rot2, 0.125)
+    assert bool(((out[keep].double() - ref).abs() <= tol).all())
+    assert ib.check_fault() == 0
+
+
+def test_a_captured_step_whose_pool_runs_out(cuda):
+    """Forks share their prefix; step after step of one graph the pool runs out for one after the
+    other.  Nothing that a sequence has stored changes, and every length is what was granted."""
+    H, Hkv, HD, page, n_pages = 4, 2, 32, 4, 14
+    book = Book(5, 16, n_pages, page)
+    book.extend([0], [10])  # pages 0 .. 2
+    seqs, pages = seqs_of(cuda, book), pool(cuda, 1, n_pages, Hkv, page, HD, ib.F32, 1)
+    children = [1, 2, 3, 4]
+    want, copies = book.fork([0] * 4, children)
+    assert want == [1] * 4
+    status = ib.kv_fork(pages, seqs, i32(cuda, [0] * 4), i32(cuda, children))
+    slots = ib.kv_granted(pages, i32(cuda, children), status)
+    ones, status = i32(cuda, [1] * 4), i32(cuda, [0] * 4)
+    granted = i32(cuda, [0] * 4)
+    batch = ib.KVBatch(i32(cuda, range(5)), 4, max_q=1, slots=granted)
+    x = cuda.zeros(4, H + 2 * Hkv, HD, device="cuda")
+    rope = rope_table(cuda, 64, HD)
+    out = cuda.zeros(4, H, HD, device="cuda")
+
+    def step(ws, new=ones):
+        ib.kv_extend(pages, seqs, slots, new, status=status)
+        ib.kv_granted(pages, slots, status, out=granted)
+        q = ib.kv_append(pages, seqs, batch, 0, x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:], rope)
+        ib.attention_paged(pages, seqs, batch, 0, q, 0.2, out=out, workspace=ws)
+
+    side = cuda.cuda.Stream()
+    side.wait_stream(cuda.cuda.current_stream())
+    kept = [[] for _ in range(5)]  # V rows that each child has stored
+    short = 0
+    with cuda.cuda.stream(side):
+        ws = ib.attention_paged_workspace(pages, seqs, batch, H)
+        step(ws, new=i32(cuda, [-1] * 4))  # refused, all of it: nothing changes
+        side.synchronize()
+        same(book, seqs)
+        assert status.tolist() == granted.tolist() == [-1] * 4 and not bool(out.any())
+        graph = cuda.cuda.CUDAGraph()
+        with cuda.cuda.graph(graph, stream=side):
+            step(ws)
+        for i in range(30):
+            x.fill_(i + 1.0)
+            out.fill_(-1.0)
+            graph.replay()
+            side.synchronize()
+            got = book.extend(children, [1] * 4)
+            assert status.tolist() == got
+            same(book, seqs)
+            for j, c in enumerate(children):
+                assert bool((out[j] == -1).all()) == (got[j] != 1)
+                if got[j] == 1:
+                    kept[c].append(i + 1.0)
+                else:
+                    short += 1
+                for p, val in enumerate(kept[c], start=10):
+                    t = book.table[c][p // page]
+                    assert bool((pages.v[0, t, :, p % page] == val).all())
+    assert 0 < short < 120
+    assert ib.check_fault() == 0

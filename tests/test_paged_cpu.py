@@ -162,3 +162,15 @@ def test_the_search_finds_a_shared_look_barrier(tmp_path):
     """The same search on one look barrier for all slots: two careful key tiles in a row can
     lap a warp."""
     assert "2 key tiles, careful 3: a wait that never ends" in _ring_test(tmp_path, "shared")
+
+
+def test_granted_refuses_bad_lists():
+    L = ib.lib()
+    for n in (-1, 16385):
+        assert L.ib_kv_granted(n, PTR, PTR, PTR, None) == ib.IB_ERR_INVALID
+    for i in range(3):
+        a = [PTR] * 3
+        a[i] = None
+        assert L.ib_kv_granted(1, *a, None) == ib.IB_ERR_INVALID
+        assert "ib_kv_granted" in ib.last_error()
+    assert L.ib_kv_granted(0, None, None, None, None) == ib.IB_OK
