@@ -268,7 +268,8 @@ typedef struct {
 /* Values in device memory cannot be checked by the host.  A slot, length, cu_q or table entry
  * out of range is clamped or passed over by the kernel, never used as an address, and
  * recorded: ib_check_fault then returns IB_ERR_INVALID with code 71 (slot), 72 (table entry),
- * 73 (len or cu_q), 74 (refs below the tables' entries) or 75 (position behind rope_table).
+ * 73 (len or cu_q), 74 (refs below the tables' entries), 75 (position behind rope_table) or 77
+ * (a new token's page has refs over 1: ib_kv_append writes no page that others hold too).
  *
  * ib_kv_extend: room for n_new[i] more tokens of slot slots[i], i < n: len grows and the
  * pages that this takes are entered in its row, with refs 1.  Free pages go out lowest first,
@@ -310,7 +311,8 @@ int ib_kv_compact(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int32_t* tab
  * may be slices of one projection; 16-byte aligned).  Rotated q goes to q_out (may be q),
  * rotated k and v into the pages.  rope_table: [rope_len][head_dim / 2][2] cos and sin, as
  * ib_rope takes.  Tokens without a position (len below the number of new tokens) or behind
- * rope_len are passed over; where the page is -1 only q_out is written. */
+ * rope_len are passed over; where the page is -1, or held by other sequences too, only q_out
+ * is written. */
 int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
                  int layer, int n_heads, const float* q, int64_t q_stride, const float* k,
                  int64_t k_stride, const float* v, int64_t v_stride, float* q_out,

@@ -156,10 +156,13 @@ extern "C" int ib_check_fault(int* code) {
         if ((st = paged_attention_fault_take(&c3)) != IB_OK) return st;
         *code = c2 ? c2 : c3;
         if (*code && *code != PAGED_BAD_WAIT) {
-            static const char* const what[] = {"a slot", "a table entry", "a length or cu_q value",
-                                               "a reference count", "a RoPE position"};
+            static const char* const what[] = {
+                "a slot was out of range",          "a table entry was out of range",
+                "a length or cu_q value was out of range", "a reference count was out of range",
+                "a RoPE position was out of range", "",
+                "a new token's page is held by other sequences too"};
             set_error(std::string("CUDA: paged KV cache: ") + what[*code - PAGED_BAD_SLOT] +
-                      " was out of range (code " + std::to_string(*code) + ")");
+                      " (code " + std::to_string(*code) + ")");
             return IB_ERR_INVALID;
         }
     }

@@ -83,6 +83,7 @@ PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batc
     PagedView w;
     w.table = s->table;
     w.len = s->len;
+    w.refs = s->refs;
     w.cu_q = b->cu_q;
     w.slots = b->slots;
     w.n_slots = s->n_slots;
@@ -550,6 +551,9 @@ __global__ void __launch_bounds__(256)
     }
     const int col = (int)w.ps.div((uint32_t)pos), slot = pos - col * w.page_size;
     const int page = page_at(w, s.row[col]);
+    // a page that others hold too is not written: it would change what they have stored
+    const bool own = page >= 0 && w.refs[page] <= 1;
+    if (page >= 0 && !own && threadIdx.x == 0) paged_fault(PAGED_SHARED);
     const int per = w.HD / 8;
     const int total = (w.H + 2 * w.Hkv) * per;
     for (int e = threadIdx.x; e < total; e += blockDim.x) {
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(256)
             float4* o = reinterpret_cast<float4*>(q_out + t * qo_stride + (int64_t)h * w.HD + d);
             o[0] = x[0];
             o[1] = x[1];
-        } else if (page >= 0) {
+        } else if (own) {
             KV* pool = is_v ? vpool : kpool;
             KV* o = pool + (((int64_t)page * w.Hkv + h) * w.page_size + slot) * w.HD + d;
             if constexpr (sizeof(KV) == 4) {

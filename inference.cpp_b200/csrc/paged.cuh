@@ -20,7 +20,8 @@ enum {
     PAGED_BAD_LEN = 73,    // len or cu_q out of order or out of range
     PAGED_BAD_REFS = 74,   // a reference count that a release would take below zero
     PAGED_BAD_ROPE = 75,   // a position behind the end of the RoPE table
-    PAGED_BAD_WAIT = 76    // a pipeline wait expired
+    PAGED_BAD_WAIT = 76,   // a pipeline wait expired
+    PAGED_SHARED = 77      // a new token in a page that others hold too
 };
 
 // Unsigned division by a number that the host prepares (page sizes need not be powers of
@@ -46,6 +47,7 @@ struct FastDiv {
 struct PagedView {
     const int32_t* table;
     const int32_t* len;
+    const int32_t* refs;
     const int32_t* cu_q;
     const int32_t* slots;  // null: sequence b is slot b
     int n_slots, max_pages, n_pages;

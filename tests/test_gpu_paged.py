@@ -1188,3 +1188,31 @@ def test_a_captured_step_whose_pool_runs_out(cuda):
                     assert bool((pages.v[0, t, :, p % page] == val).all())
     assert 0 < short < 120
     assert ib.check_fault() == 0
+
+
+@TYPES
+def test_append_never_writes_a_shared_page(cuda, type_):
+    """A step that ignores the status of an extend without room: the sequence's last tokens are
+    taken for the new ones, but pages that forks share keep what they hold, and it is recorded."""
+    H, Hkv, HD, page = 4, 2, 32, 4
+    book = Book(3, 4, 4, page)
+    assert book.extend([0], [8]) == [1]
+    assert book.fork([0, 0], [1, 2])[0] == [1, 1]
+    assert book.extend([1], [8]) == [1]  # the last free pages
+    assert book.extend([2], [3]) == [0]
+    seqs, pages = seqs_of(cuda, book), pool(cuda, 2, 4, Hkv, page, HD, type_, 2)
+    k0, v0 = pages.k.clone(), pages.v.clone()
+    x = cuda.randn(3, H + 2 * Hkv, HD, device="cuda")
+    q, k, v = x.split([H, Hkv, Hkv], dim=1)
+    rope = rope_table(cuda, 16, HD)
+    batch = ib.KVBatch(i32(cuda, [0, 3]), 3, slots=i32(cuda, [2]))
+    out = ib.kv_append(pages, seqs, batch, 1, q, k, v, rope, q_out=cuda.zeros_like(q))
+    assert cuda.equal(pages.k, k0) and cuda.equal(pages.v, v0) and bool(out.any(-1).all())
+    with pytest.raises(RuntimeError, match="held by other sequences.*77"):
+        ib.check_fault()
+    # its own pages are written
+    batch = ib.KVBatch(i32(cuda, [0, 3]), 3, slots=i32(cuda, [1]))
+    ib.kv_append(pages, seqs, batch, 1, q, k, v, rope)
+    t = book.table[1][3]
+    assert cuda.equal(pages.v[1, t, :, 1:4], v.to(pages.v.dtype).transpose(0, 1))
+    assert ib.check_fault() == 0
