@@ -75,7 +75,8 @@ int ib_sync(void);                              /* device-wide synchronise */
 /* Every wait inside a pipelined kernel is bounded; an expired wait makes the
  * kernel record a code and return early instead of hanging.  This reads and
  * clears that record on the current device: IB_ERR_TIMEOUT (and *code != 0)
- * means results since the previous check are invalid. */
+ * means results since the previous check are invalid.  Bad values that kernels of the paged
+ * KV cache passed over are read and cleared too (IB_ERR_INVALID, codes below). */
 int ib_check_fault(int* code);
 int ib_shutdown(void);                          /* no-op: buffers stay valid to exit */
 
@@ -269,7 +270,10 @@ typedef struct {
  * out of range is clamped or passed over by the kernel, never used as an address, and
  * recorded: ib_check_fault then returns IB_ERR_INVALID with code 71 (slot), 72 (table entry),
  * 73 (len or cu_q), 74 (refs below the tables' entries), 75 (position behind rope_table) or 77
- * (a new token's page has refs over 1: ib_kv_append writes no page that others hold too).
+ * (a new token's page has refs over 1: ib_kv_append writes no page that others hold too).  An
+ * expired wait of ib_attention_paged is IB_ERR_TIMEOUT with code 76, also where values were bad
+ * as well: results are missing then.  ib_kv_wait_selftest records a bad table entry and lets a
+ * short wait run out, for a test of that.
  *
  * ib_kv_extend: room for n_new[i] more tokens of slot slots[i], i < n: len grows and the
  * pages that this takes are entered in its row, with refs 1.  Free pages go out lowest first,
@@ -304,6 +308,8 @@ int ib_kv_release(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const
  * own arrays. */
 int ib_kv_compact(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int32_t* table_out,
                   int32_t* refs_out, int32_t* map, int32_t* moves, int32_t* info, void* stream);
+
+int ib_kv_wait_selftest(void* stream);
 
 /* ib_kv_append: a step's projections into `layer` of the cache, ib_rope_batch and
  * ib_kv_write_batch in one pass.  q [n_tokens][n_heads][head_dim], k and v [n_tokens]

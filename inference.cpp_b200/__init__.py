@@ -118,6 +118,7 @@ SIGNATURES = {
     "ib_kv_granted": [_i, _vp, _vp, _vp, _vp],
     "ib_kv_release": [_vp, _vp, _i, _vp, _vp],
     "ib_kv_compact": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ib_kv_wait_selftest": [_vp],
     "ib_kv_append": [_vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i,
                      _vp],
     "ib_attention_paged_workspace": [_vp, _vp, _vp, _i],
@@ -207,7 +208,8 @@ def sync() -> None:
 
 
 def check_fault() -> int:
-    """Raises if a bounded pipeline wait expired since the last check."""
+    """Raises if a bounded pipeline wait expired since the last check, or a kernel of the paged
+    cache passed over a bad value."""
     code = ctypes.c_int()
     call("ib_check_fault", ctypes.byref(code))
     return code.value

@@ -150,21 +150,26 @@ extern "C" int ib_check_fault(int* code) {
     if (!*code) *code = c2;
     if ((st = step_fault_take(&c2)) != IB_OK) return st;
     if (!*code) *code = c2;
-    if (!*code) {
-        if ((st = paged_fault_take(&c2)) != IB_OK) return st;
-        int c3 = 0;
-        if ((st = paged_attention_fault_take(&c3)) != IB_OK) return st;
-        *code = c2 ? c2 : c3;
-        if (*code && *code != PAGED_BAD_WAIT) {
-            static const char* const what[] = {
-                "a slot was out of range",          "a table entry was out of range",
-                "a length or cu_q value was out of range", "a reference count was out of range",
-                "a RoPE position was out of range", "",
-                "a new token's page is held by other sequences too"};
-            set_error(std::string("CUDA: paged KV cache: ") + what[*code - PAGED_BAD_SLOT] +
-                      " (code " + std::to_string(*code) + ")");
-            return IB_ERR_INVALID;
+    int c3 = 0;
+    if ((st = paged_fault_take(&c2)) != IB_OK) return st;
+    if ((st = paged_attention_fault_take(&c3)) != IB_OK) return st;
+    c2 = paged_fault_worse(c2, c3);
+    if (!*code && c2) {
+        *code = c2;
+        const std::string tail = " (code " + std::to_string(c2) + ")";
+        if (c2 == PAGED_BAD_WAIT) {
+            set_error("CUDA: a pipeline wait expired in ib_attention_paged" + tail +
+                      "; results of the calls since the last check are invalid");
+            return IB_ERR_TIMEOUT;
         }
+        const char* what = c2 == PAGED_BAD_SLOT   ? "a slot was out of range"
+                           : c2 == PAGED_BAD_PAGE ? "a table entry was out of range"
+                           : c2 == PAGED_BAD_LEN  ? "a length or cu_q value was out of range"
+                           : c2 == PAGED_BAD_REFS ? "a reference count was out of range"
+                           : c2 == PAGED_BAD_ROPE ? "a RoPE position was out of range"
+                                                  : "a new token's page is held by other sequences too";
+        set_error(std::string("CUDA: paged KV cache: ") + what + tail);
+        return IB_ERR_INVALID;
     }
     if (*code) {
         set_error("CUDA: a pipeline wait expired in a GEMV kernel (code " + std::to_string(*code) +

@@ -57,8 +57,13 @@ struct PagedView {
     FastDiv group;  // of H / Hkv
 };
 
-// Each translation unit's kernels record their first fault here.
-static __device__ int g_paged_fault;
+// Each translation unit's kernels record their first fault here: of values in device memory, which
+// were passed over, and of waits that ran out, after which results are missing.  One does not hide
+// the other.
+struct PagedFaults {
+    int value, wait;
+};
+static __device__ PagedFaults g_paged_faults;
 
 // New tokens [q0, q0 + n) of sequence b, L positions in all, table row `row`.
 struct SeqInfo {
@@ -66,7 +71,7 @@ struct SeqInfo {
     const int32_t* row;
 };
 
-__device__ __forceinline__ void paged_fault(int code) { atomicCAS(&g_paged_fault, 0, code); }
+__device__ __forceinline__ void paged_fault(int code) { atomicCAS(&g_paged_faults.value, 0, code); }
 
 __device__ __forceinline__ SeqInfo seq_info(const PagedView& w, int b) {
     SeqInfo s;
@@ -113,12 +118,18 @@ struct DeviceOnce {
     }
 };
 
-// Reads and clears this translation unit's fault word.
+// The code to report of two: an expired wait before any value, else the first.
+static inline int paged_fault_worse(int a, int b) {
+    return a == PAGED_BAD_WAIT || b == PAGED_BAD_WAIT ? (int)PAGED_BAD_WAIT : a ? a : b;
+}
+
+// Reads and clears this translation unit's record.
 static inline int paged_fault_take_here(int* code) {
-    int v = 0, z = 0;
-    IB_CUDA_CHECK(cudaMemcpyFromSymbol(&v, g_paged_fault, sizeof(int)));
-    if (v) IB_CUDA_CHECK(cudaMemcpyToSymbol(g_paged_fault, &z, sizeof(int)));
-    *code = v;
+    PagedFaults v = {0, 0};
+    const PagedFaults none = {0, 0};
+    IB_CUDA_CHECK(cudaMemcpyFromSymbol(&v, g_paged_faults, sizeof(v)));
+    if (v.value || v.wait) IB_CUDA_CHECK(cudaMemcpyToSymbol(g_paged_faults, &none, sizeof(v)));
+    *code = paged_fault_worse(v.value, v.wait);
     return IB_OK;
 }
 

@@ -41,7 +41,7 @@ namespace ib {
 int paged_attention_fault_take(int* code) {
     int r = paged_fault_take_here(code), c = 0;
     if (r == IB_OK) r = paged_tensor_fault_take(&c);
-    if (*code == 0) *code = c;
+    *code = paged_fault_worse(*code, c);
     return r;
 }
 

@@ -58,6 +58,14 @@ namespace ib {
 
 int paged_tensor_fault_take(int* code) { return paged_fault_take_here(code); }
 
+// A bad table entry and then a wait for an arrival that nobody makes.
+__global__ void wait_selftest_kernel() {
+    __shared__ uint64_t bar;
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+    paged_fault(PAGED_BAD_PAGE);
+    mbar_wait(&bar, 0, &g_paged_faults.wait, PAGED_BAD_WAIT, 256);
+}
 
 template <typename KV, int HDP>
 struct TensorCfg {
@@ -340,7 +348,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
     // For the n-th completion, from 0; the same answer in a whole warp.  Every wait is bounded: a
     // role whose wait expired leaves its loop, and so do, one wait later, those that wait for it.
     auto wait = [&](uint64_t* b, int n) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(b, (uint32_t)(n & 1), &g_paged_fault, PAGED_BAD_WAIT));
+        return __all_sync(0xffffffffu, mbar_wait(b, (uint32_t)(n & 1), &g_paged_faults.wait, PAGED_BAD_WAIT));
     };
 
     if (warp < 8) {
@@ -1072,3 +1080,9 @@ template int attn_tensor_launch<float>(const RowsArgs&, int64_t, int64_t, cudaSt
 template int attn_tensor_launch<__half>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
 
 }  // namespace ib
+
+extern "C" int ib_kv_wait_selftest(void* stream) {
+    ib::wait_selftest_kernel<<<1, 1, 0, ib::as_stream(stream)>>>();
+    IB_LAUNCH_CHECK("wait_selftest_kernel");
+    return IB_OK;
+}

@@ -64,8 +64,9 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // Bounded wait for the phase with the given parity; false (and g_fault set) on expiry.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* fault, int code) {
-    for (uint32_t i = 0; i < kWaitPolls; ++i) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* fault, int code,
+                                          uint32_t polls = kWaitPolls) {
+    for (uint32_t i = 0; i < polls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (i > 64) __nanosleep(64);
     }

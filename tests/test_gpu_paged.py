@@ -1216,3 +1216,26 @@ def test_append_never_writes_a_shared_page(cuda, type_):
     t = book.table[1][3]
     assert cuda.equal(pages.v[1, t, :, 1:4], v.to(pages.v.dtype).transpose(0, 1))
     assert ib.check_fault() == 0
+
+
+def test_an_expired_wait_is_not_hidden_by_bad_values(cuda):
+    """Results are missing after an expired wait: it is reported before values that were passed
+    over, whichever kernel recorded them and in whatever order, and named as attention's."""
+    pages, seqs = pool(cuda, 1, 4, 1, 4, 8, ib.F16, 0), ib.KVSeqs.empty(2, 2, 4)
+
+    def bad_slot():
+        ib.kv_release(pages, seqs, i32(cuda, [7]))
+
+    def wait():  # records a bad table entry first
+        ib.call("ib_kv_wait_selftest", None)
+
+    for acts in ([wait], [bad_slot, wait], [wait, bad_slot]):
+        for act in acts:
+            act()
+        with pytest.raises(RuntimeError, match="attention_paged.*76"):
+            ib.check_fault()
+        assert ib.check_fault() == 0  # all of it read and cleared
+    bad_slot()
+    with pytest.raises(RuntimeError, match="slot was out of range.*71"):
+        ib.check_fault()
+    assert ib.check_fault() == 0
