@@ -305,7 +305,8 @@ int ib_kv_release(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const
  * stay, and the moved pages' old places keep their bytes.  Written: info = {n_live, moves},
  * moves [n_pages] (pairs old, new), map [n_pages] (new index of each page, -1 for a free one),
  * and the renamed table_out [n_slots][max_pages] and refs_out [n_pages], which may be seqs'
- * own arrays. */
+ * own arrays.  Lengths do not change: other sequences made of table_out and refs_out take
+ * seqs->len, or a copy. */
 int ib_kv_compact(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int32_t* table_out,
                   int32_t* refs_out, int32_t* map, int32_t* moves, int32_t* info, void* stream);
 

@@ -727,8 +727,9 @@ def kv_compact_plan(pages):
 
 
 def kv_compact(pages, seqs, out=None, plan=None, stream=None):
-    """Moves the used pages to the lowest indices; the renamed table and refs go to `out` (a
-    KVSeqs; default: seqs itself).  Returns the plan."""
+    """Moves the used pages to the lowest indices; the renamed table and refs, and the lengths, go
+    to `out` (a KVSeqs; default: seqs itself; it may share arrays with seqs).  Returns the
+    plan."""
     out = seqs if out is None else out
     if plan is None:
         with _allocating(pages, stream):
@@ -740,6 +741,9 @@ def kv_compact(pages, seqs, out=None, plan=None, stream=None):
     _call("ib_kv_compact", pages._p, _seqs_of(pages, seqs), out.table.data_ptr(),
          out.refs.data_ptr(), plan.map.data_ptr(), plan.moves.data_ptr(), plan.info.data_ptr(),
          st)
+    if out.len.data_ptr() != seqs.len.data_ptr():
+        with _allocating(pages, stream):  # on the launch stream
+            out.len.copy_(seqs.len)
     return plan
 
 

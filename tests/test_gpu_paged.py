@@ -1239,3 +1239,29 @@ def test_an_expired_wait_is_not_hidden_by_bad_values(cuda):
     with pytest.raises(RuntimeError, match="slot was out of range.*71"):
         ib.check_fault()
     assert ib.check_fault() == 0
+
+
+def test_compact_into_sequences_with_lengths_of_their_own(cuda):
+    """The second half of a double buffer: what the call leaves in `out` is a whole cache."""
+    book = Book(4, 6, 20, 4)
+    for s, n in ((0, 9), (1, 16), (2, 5), (3, 21)):
+        book.extend([s], [n])
+    book.release([1])
+    seqs, pages = seqs_of(cuda, book), pool(cuda, 1, 20, 1, 4, 8, ib.F16, 1)
+    old = [t.clone() for t in (seqs.table, seqs.len, seqs.refs)]
+    book.compact()
+    out = ib.KVSeqs.empty(4, 6, 20)
+    ib.kv_compact(pages, seqs, out=out)
+    same(book, out)
+    assert all(cuda.equal(a, b) for a, b in zip(old, (seqs.table, seqs.len, seqs.refs)))
+    # the same on a stream of its own, while the current one is busy
+    other, again = cuda.cuda.Stream(), ib.KVSeqs.empty(4, 6, 20)
+    plan = ib.kv_compact_plan(pages)
+    cuda.cuda.synchronize()
+    cuda.cuda._sleep(50_000_000)
+    ib.kv_compact(pages, seqs, out=again, plan=plan, stream=other.cuda_stream)
+    other.synchronize()
+    with cuda.cuda.stream(other):
+        same(book, again)
+    cuda.cuda.synchronize()
+    assert ib.check_fault() == 0
