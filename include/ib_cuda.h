@@ -315,11 +315,11 @@ int ib_kv_wait_selftest(void* stream);
 /* ib_kv_append: a step's projections into `layer` of the cache, ib_rope_batch and
  * ib_kv_write_batch in one pass.  q [n_tokens][n_heads][head_dim], k and v [n_tokens]
  * [n_kv_heads][head_dim], FP32 with rows q_stride .. elements apart (multiples of 4, so they
- * may be slices of one projection; 16-byte aligned).  Rotated q goes to q_out (may be q),
- * rotated k and v into the pages.  rope_table: [rope_len][head_dim / 2][2] cos and sin, as
- * ib_rope takes.  Tokens without a position (len below the number of new tokens) or behind
- * rope_len are passed over; where the page is -1, or held by other sequences too, only q_out
- * is written. */
+ * may be slices of one projection; 16-byte aligned).  Rotated q goes to q_out (q itself, with
+ * its stride, or rows that share nothing with q, k and v), rotated k and v into the pages.
+ * rope_table: [rope_len][head_dim / 2][2] cos and sin, as ib_rope takes.  Tokens without a
+ * position (len below the number of new tokens) or behind rope_len are passed over; where the
+ * page is -1, or held by other sequences too, only q_out is written. */
 int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
                  int layer, int n_heads, const float* q, int64_t q_stride, const float* k,
                  int64_t k_stride, const float* v, int64_t v_stride, float* q_out,
@@ -330,7 +330,7 @@ int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_b
  * sees positions 0 .. len - n + i whose pages are there.  A row that sees none is 0.  Same
  * result contract as ib_attention_batch (softmax of scale * q.k, grouped heads).  q and out
  * [n_tokens][n_heads][head_dim] FP32, rows q_stride / out_stride elements apart (multiples
- * of 4, 16-byte aligned); out may be q itself.  A NaN or infinity in a position that a row
+ * of 4, 16-byte aligned); out is q itself, with its stride, or shares nothing with it.  A NaN or infinity in a position that a row
  * does not see leaves the row alone; in one that it sees, the row's outputs are not specified
  * (NaN, as a rule).
  * q, K and V may be of any finite size; the division by the sum of weights comes last, so

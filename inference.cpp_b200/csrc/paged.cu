@@ -102,6 +102,18 @@ PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batc
 
 int paged_fault_take(int* code) { return paged_fault_take_here(code); }
 
+bool paged_rows_overlap(const float* a, int64_t sa, int64_t wa, const float* b, int64_t sb, int64_t wb,
+                        int64_t n) {
+    const int64_t d = ((intptr_t)b - (intptr_t)a) / (int64_t)sizeof(float);
+    if (sa != sb || sa <= 0)  // no common step: the whole ranges
+        return d < (n - 1) * sa + wa && -d < (n - 1) * sb + wb;
+    // row i of a and row i + k of b meet where -wb < d + k sa < wa, for k within n - 1 of 0: the
+    // least such k is the first one above (-wb - d) / sa
+    const int64_t x = -wb - d, floor = x >= 0 ? x / sa : -((-x + sa - 1) / sa);
+    const int64_t k = std::max(floor + 1, 1 - n);
+    return k <= n - 1 && d + k * sa < wa;
+}
+
 static int elem_bytes(const ib_kv_pages* p) { return p->type == IB_TYPE_F32 ? 4 : 2; }
 
 static int sm_count(int* n) {
@@ -734,6 +746,13 @@ extern "C" int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
     const int64_t qw = (int64_t)n_heads * pages->head_dim;
     IB_REQUIRE(q_stride >= 0 && k_stride >= 0 && v_stride >= 0 && q_out_stride >= qw,
                "ib_kv_append: bad row strides");
+    const int64_t kw = (int64_t)pages->n_kv_heads * pages->head_dim, n = batch->n_tokens;
+    IB_REQUIRE(((q_out == q && q_out_stride == q_stride) ||
+                !paged_rows_overlap(q_out, q_out_stride, qw, q, q_stride, qw, n)) &&
+                   !paged_rows_overlap(q_out, q_out_stride, qw, k, k_stride, kw, n) &&
+                   !paged_rows_overlap(q_out, q_out_stride, qw, v, v_stride, kw, n),
+               "ib_kv_append: q_out may be q, with its row stride, and must not overlap it otherwise, "
+               "nor k or v");
     const PagedView w = paged_view(pages, seqs, batch, n_heads);
     const int64_t layer_elems = pool_bytes(pages).layer_bytes / elem_bytes(pages);
     cudaStream_t st = as_stream(stream);

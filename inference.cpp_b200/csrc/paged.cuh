@@ -137,6 +137,10 @@ static inline int paged_fault_take_here(int* code) {
 int paged_check(const ib_kv_pages* p, const ib_kv_seqs* s, const char* who);
 int paged_check_batch(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int layer,
                       int n_heads, const char* who);
+// Whether any of n rows of wa floats, sa apart from a, shares a float with one of wb, sb apart from b
+// (rows of different strides: whether their whole ranges meet).
+bool paged_rows_overlap(const float* a, int64_t sa, int64_t wa, const float* b, int64_t sb, int64_t wb,
+                        int64_t n);
 PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int n_heads);
 int paged_fault_take(int* code);            // paged.cu
 int paged_attention_fault_take(int* code);  // paged_attention.cu

@@ -1195,6 +1195,11 @@ extern "C" int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* se
                "multiples of 4");
     IB_REQUIRE(q_stride >= 0 && out_stride >= (int64_t)n_heads * pages->head_dim,
                "ib_attention_paged: bad row strides");
+    const int64_t row = (int64_t)n_heads * pages->head_dim;
+    IB_REQUIRE((out == q && out_stride == q_stride) ||
+                   !paged_rows_overlap(out, out_stride, row, q, q_stride, row, batch->n_tokens),
+               "ib_attention_paged: out may be q, with its row stride, and must not overlap it "
+               "otherwise");
     RowsArgs a{};
     a.w = paged_view(pages, seqs, batch, n_heads);
     size_t need = 0;

@@ -174,3 +174,29 @@ def test_granted_refuses_bad_lists():
         assert L.ib_kv_granted(1, *a, None) == ib.IB_ERR_INVALID
         assert "ib_kv_granted" in ib.last_error()
     assert L.ib_kv_granted(0, None, None, None, None) == ib.IB_OK
+
+
+STEP = 4 * (256 + 2 * 128)  # bytes between rows of one projection's q (4 x 64), k and v (2 x 64)
+QKV = dict(q=PTR, qs=512, k=PTR + 1024, ks=512, v=PTR + 1024 + 512, vs=512)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(o=PTR, os_=256),                       # in place, rows of another step
+    dict(o=PTR + 16, os_=512),                  # beside q's rows by four elements
+    dict(o=PTR - 16, os_=512), dict(o=PTR + STEP, os_=512), dict(o=PTR - 2 * STEP, os_=512),
+    dict(o=PTR + 1024, os_=512),                # k and v
+    dict(o=PTR + 1024 + 512, os_=512),          # v, and the next row's q
+    dict(o=PTR + 2 * STEP + 1008, os_=256),     # another step, over the last row's end
+])
+def test_append_refuses_rows_that_overlap(bad):
+    assert append(**QKV, **bad) == ib.IB_ERR_INVALID
+    assert "ib_kv_append" in ib.last_error() and "overlap" in ib.last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(os_=260), dict(out=PTR + 16), dict(out=PTR - 1008),
+                                 dict(out=PTR + 2048), dict(qs=0), dict(qs=0, out=PTR + 1008),
+                                 dict(qs=512, os_=512, out=PTR + 1008),
+                                 dict(qs=512, os_=512, out=PTR + 2048 - 16)])
+def test_attention_refuses_rows_that_overlap(bad):
+    assert attention(**bad) == ib.IB_ERR_INVALID
+    assert "ib_attention_paged" in ib.last_error() and "overlap" in ib.last_error()
