@@ -279,7 +279,7 @@ typedef struct {
  * pages that this takes are entered in its row, with refs 1.  Free pages go out lowest first,
  * in list order; once an entry finds too few, it and all later ones that need any get none.
  * status[i]: 1 done, 0 no room (in the pool or in the row), -1 refused (slot out of range or
- * named by an earlier entry, n_new < 0).
+ * named by an earlier entry, n_new < 0).  status must not overlap the lists.
  * A sequence without status 1 keeps its length, so a step that went on with it would take the
  * last tokens that it has for new ones and write over them.  The step's batch has to leave it
  * out: ib_kv_granted makes its slots without the host looking at the status. */

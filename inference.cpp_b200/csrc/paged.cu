@@ -657,13 +657,25 @@ static int check_list(int n, const void* a, const char* who) {
     return IB_OK;
 }
 
+// status is written while the lists are still being read
+static int check_status(int n, const int32_t* a, const int32_t* b, const int32_t* status,
+                        const char* who) {
+    const int r = check_list(n, a && b ? status : nullptr, who);
+    if (r != IB_OK) return r;
+    for (const int32_t* list : {a, b})
+        if ((uintptr_t)status < (uintptr_t)(list + n) && (uintptr_t)list < (uintptr_t)(status + n)) {
+            set_error(std::string(who) + ": status must not overlap the lists");
+            return IB_ERR_INVALID;
+        }
+    return IB_OK;
+}
+
 extern "C" int ib_kv_extend(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n,
                             const int32_t* slots, const int32_t* n_new, int32_t* status,
                             void* stream) {
     int r = paged_check(pages, seqs, "ib_kv_extend");
     if (r != IB_OK || n == 0) return r;
-    if ((r = check_list(n, slots && n_new ? status : nullptr, "ib_kv_extend")) != IB_OK)
-        return r;
+    if ((r = check_status(n, slots, n_new, status, "ib_kv_extend")) != IB_OK) return r;
     return assign_launch<false>(seqs_dev(pages, seqs), n, slots, n_new, status, as_stream(stream));
 }
 
@@ -672,8 +684,7 @@ extern "C" int ib_kv_fork(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int 
                           void* stream) {
     int r = paged_check(pages, seqs, "ib_kv_fork");
     if (r != IB_OK || n == 0) return r;
-    if ((r = check_list(n, parents && children ? status : nullptr, "ib_kv_fork")) != IB_OK)
-        return r;
+    if ((r = check_status(n, parents, children, status, "ib_kv_fork")) != IB_OK) return r;
     const KvSeqsDev s = seqs_dev(pages, seqs);
     cudaStream_t st = as_stream(stream);
     if ((r = assign_launch<true>(s, n, parents, children, status, st)) != IB_OK) return r;

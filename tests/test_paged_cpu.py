@@ -200,3 +200,13 @@ def test_append_refuses_rows_that_overlap(bad):
 def test_attention_refuses_rows_that_overlap(bad):
     assert attention(**bad) == ib.IB_ERR_INVALID
     assert "ib_attention_paged" in ib.last_error() and "overlap" in ib.last_error()
+
+
+@pytest.mark.parametrize("entry", ["ib_kv_extend", "ib_kv_fork"])
+def test_status_must_not_overlap_the_lists(entry):
+    f, p, s = getattr(ib.lib(), entry), ref(pages()), ref(seqs())
+    far = PTR + (1 << 20)
+    for lists in ((PTR, far, PTR), (far, PTR, PTR), (PTR, far, PTR + 4 * 4), (far, PTR, PTR - 4 * 4),
+                  (PTR, PTR, PTR)):
+        assert f(p, s, 5, *lists, None) == ib.IB_ERR_INVALID
+        assert entry in ib.last_error() and "overlap" in ib.last_error()
