@@ -294,7 +294,7 @@ int ib_kv_fork(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const in
 /* ib_kv_granted: granted[i] = slots[i] where status[i] is 1, -1 elsewhere, for a list of slots
  * (children) and the status that ib_kv_extend (ib_kv_fork) left for it: as a batch's slots it
  * leaves out the sequences that got no room, and ib_kv_extend refuses its -1 in turn.  granted
- * may be slots. */
+ * may be slots, and must not overlap slots or status otherwise. */
 int ib_kv_granted(int n, const int32_t* slots, const int32_t* status, int32_t* granted,
                   void* stream);
 /* ib_kv_release: the slots give up their pages (refs - 1) and are empty. */

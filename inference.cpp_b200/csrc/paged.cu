@@ -657,14 +657,14 @@ static int check_list(int n, const void* a, const char* who) {
     return IB_OK;
 }
 
-// status is written while the lists are still being read
+// the result (status, granted) is written while the lists are still being read
 static int check_status(int n, const int32_t* a, const int32_t* b, const int32_t* status,
                         const char* who) {
     const int r = check_list(n, a && b ? status : nullptr, who);
     if (r != IB_OK) return r;
     for (const int32_t* list : {a, b})
         if ((uintptr_t)status < (uintptr_t)(list + n) && (uintptr_t)list < (uintptr_t)(status + n)) {
-            set_error(std::string(who) + ": status must not overlap the lists");
+            set_error(std::string(who) + ": the result must not overlap the lists");
             return IB_ERR_INVALID;
         }
     return IB_OK;
@@ -701,7 +701,7 @@ extern "C" int ib_kv_fork(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int 
 extern "C" int ib_kv_granted(int n, const int32_t* slots, const int32_t* status, int32_t* granted,
                              void* stream) {
     if (n == 0) return IB_OK;
-    const int r = check_list(n, slots && status ? granted : nullptr, "ib_kv_granted");
+    const int r = check_status(n, granted == slots ? status : slots, status, granted, "ib_kv_granted");
     if (r != IB_OK) return r;
     kv_granted_kernel<<<(n + KV_COPY_THREADS - 1) / KV_COPY_THREADS, KV_COPY_THREADS, 0,
                         as_stream(stream)>>>(n, slots, status, granted);

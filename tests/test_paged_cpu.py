@@ -210,3 +210,11 @@ def test_status_must_not_overlap_the_lists(entry):
                   (PTR, PTR, PTR)):
         assert f(p, s, 5, *lists, None) == ib.IB_ERR_INVALID
         assert entry in ib.last_error() and "overlap" in ib.last_error()
+
+
+def test_granted_must_not_overlap_its_lists():
+    f, far = ib.lib().ib_kv_granted, PTR + (1 << 20)
+    for slots, status, out in ((PTR, far, PTR + 4), (PTR, far, PTR - 16), (far, PTR, PTR),
+                               (PTR, PTR, PTR), (PTR, PTR + 16, PTR)):
+        assert f(5, slots, status, out, None) == ib.IB_ERR_INVALID
+        assert "ib_kv_granted" in ib.last_error() and "overlap" in ib.last_error()
