@@ -43,10 +43,10 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <mutex>
 #include <string>
 
 #include "common.cuh"
+#include "lookup.h"
 #include "mma_tile.cuh"
 #include "paged.cuh"
 #include "paged_plan.cuh"
@@ -1004,15 +1004,14 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
 template <typename KV, int HDP>
 static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head_dim, int box_rows) {
     constexpr bool F32 = sizeof(KV) == 4;
-    static PFN_cuTensorMapEncodeTiled encode = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
+    static Lookup<PFN_cuTensorMapEncodeTiled> lookup;
+    const PFN_cuTensorMapEncodeTiled encode = lookup.get([] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            encode = (PFN_cuTensorMapEncodeTiled)fn;
+        const bool there = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault,
+                                                   &q) == cudaSuccess &&
+                           q == cudaDriverEntryPointSuccess;
+        return there ? (PFN_cuTensorMapEncodeTiled)fn : nullptr;
     });
     if (!encode) {
         set_error("ib_attention_paged: cuTensorMapEncodeTiled is not available");

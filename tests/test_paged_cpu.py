@@ -133,7 +133,8 @@ def test_python_handles_refuse_host_tensors():
         ib.KVBatch(torch.zeros(2, dtype=torch.int32), 1)
 
 
-def _ring_test(tmp_path, *args):
+def _cpp(tmp_path, name, *args):
+    """Compiles tests/cpp/<name>.cpp against the kernels' host-side headers and runs it."""
     import os
     import shutil
     import subprocess
@@ -141,10 +142,10 @@ def _ring_test(tmp_path, *args):
     gxx = shutil.which("g++")
     if gxx is None:
         pytest.skip("g++ not available")
-    exe = str(tmp_path / "copy_ring_test")
+    exe = str(tmp_path / name)
     r = subprocess.run([gxx, "-std=c++17", "-O2", "-Wall", "-Werror", "-I",
                         os.path.join(root, "inference.cpp_b200", "csrc"),
-                        os.path.join(root, "tests", "cpp", "copy_ring_test.cpp"), "-o", exe],
+                        os.path.join(root, "tests", "cpp", name + ".cpp"), "-o", exe],
                        capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
     r = subprocess.run([exe, *args], capture_output=True, text=True, timeout=300)
@@ -155,13 +156,13 @@ def _ring_test(tmp_path, *args):
 def test_copies_of_the_tensor_kernel_never_lose_a_wait(tmp_path):
     """Every interleaving of the copying warps, the TMA and the MMAs, with the kernel's own
     assignment of look barriers to ring slots."""
-    assert "0 of the patterns" in _ring_test(tmp_path)
+    assert "0 of the patterns" in _cpp(tmp_path, "copy_ring_test")
 
 
 def test_the_search_finds_a_shared_look_barrier(tmp_path):
     """The same search on one look barrier for all slots: two careful key tiles in a row can
     lap a warp."""
-    assert "2 key tiles, careful 3: a wait that never ends" in _ring_test(tmp_path, "shared")
+    assert "2 key tiles, careful 3: a wait that never ends" in _cpp(tmp_path, "copy_ring_test", "shared")
 
 
 def test_granted_refuses_bad_lists():
@@ -218,3 +219,7 @@ def test_granted_must_not_overlap_its_lists():
                                (PTR, PTR, PTR), (PTR, PTR + 16, PTR)):
         assert f(5, slots, status, out, None) == ib.IB_ERR_INVALID
         assert "ib_kv_granted" in ib.last_error() and "overlap" in ib.last_error()
+
+
+def test_a_failed_lookup_is_tried_again(tmp_path):
+    _cpp(tmp_path, "lookup_test")
