@@ -1265,3 +1265,100 @@ def test_compact_into_sequences_with_lengths_of_their_own(cuda):
         same(book, again)
     cuda.cuda.synchronize()
     assert ib.check_fault() == 0
+
+
+# ---- head_dim above 128: kernels of its own --------------------------------------------------
+
+WIDE_HD = pytest.mark.parametrize("H,Hkv,HD", [(8, 2, 136), (4, 2, 256), (3, 3, 200), (16, 1, 256)])
+
+
+@TYPES
+@WIDE_HD
+def test_large_head_dim_holes_and_spoiled_memory(cuda, type_, H, Hkv, HD):
+    for page in (1, 7, 16, 100):
+        q_lens, ctx = [150, 1, 40, 9, 0, 3], [700, 300, 333, 12, 5, 65]
+        run_attention(cuda, type_, H, Hkv, HD, page, q_lens, ctx, pad=2, holes=0.3, seed=page,
+                      spoil=True)
+    run_attention(cuda, type_, H, Hkv, HD, 16, [1, 60, 4], [400, 90, 12], holes=1.0)
+    # more new tokens than positions: the first rows see nothing
+    run_attention(cuda, type_, H, Hkv, HD, 16, [9, 200, 3], [5, 130, 0], pad=1)
+
+
+@TYPES
+@WIDE_HD
+def test_large_head_dim_cut_over_many_pieces(cuda, type_, H, Hkv, HD):
+    run_attention(cuda, type_, H, Hkv, HD, 32, [300], [2500], spoil=True)
+    run_attention(cuda, type_, H, Hkv, HD, 16, [1], [9001])
+    run_attention(cuda, type_, H, Hkv, HD, 16, [1] * 40, [50 * i + 1 for i in range(40)])
+    run_attention(cuda, type_, H, Hkv, HD, 24, [257, 1, 33, 1, 8], [900, 4000, 33, 2500, 1000])
+
+
+@TYPES
+@pytest.mark.parametrize("n,H,HD", [(6, 4, 256), (140, 8, 136), (90, 4, 256), (40, 8, 200)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_large_head_dim_rows_do_not_see_later_positions(cuda, type_, n, H, HD, what):
+    test_attention_rows_do_not_see_later_positions(cuda, type_, n, H, HD, what)
+
+
+@TYPES
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-30, -4.0])
+@pytest.mark.parametrize("HD", [136, 256])
+def test_large_head_dim_scales(cuda, type_, scale, HD):
+    run_attention(cuda, type_, 8, 2, HD, 16, [1, 90, 3], [70, 300, 40], scale=scale)
+
+
+@TYPES
+@pytest.mark.parametrize("HD", [136, 256])
+def test_large_head_dim_in_place_hints_and_workspace(cuda, type_, HD):
+    for q_lens, ctx in (([1] * 9, [2000] * 9), ([400], [2000]), ([300, 1, 5], [700, 900, 1000])):
+        pages, seqs, batch, q, out, scale = run_attention(cuda, type_, 8, 2, HD, 16, q_lens, ctx)
+        ws = ib.attention_paged_workspace(pages, seqs, batch, 8)
+        for fill in (0, 255):
+            ws.fill_(fill)
+            x = q.clone()
+            assert ib.attention_paged(pages, seqs, batch, 1, x, scale, out=x, workspace=ws) is x
+            assert cuda.equal(x, out)
+    for hint in (0, 1, 4, 200, 10 ** 6):
+        run_attention(cuda, type_, 8, 2, HD, 16, [150, 1, 20], [300, 77, 20], max_q=hint)
+
+
+@TYPES
+@pytest.mark.parametrize("HD", [136, 256])
+def test_large_head_dim_mixed_batch_in_a_graph(cuda, type_, HD):
+    pages, seqs, batch, q, out, scale = run_attention(
+        cuda, type_, 8, 2, HD, 16, [260, 1, 1, 5, 90, 1], [900, 4000, 33, 2500, 90, 1000])
+    ws = ib.attention_paged_workspace(pages, seqs, batch, 8)
+    x, y = cuda.empty_like(q.contiguous()), cuda.zeros(q.shape, device="cuda")
+    side = cuda.cuda.Stream()
+    side.wait_stream(cuda.cuda.current_stream())
+    with cuda.cuda.stream(side):
+        graph = cuda.cuda.CUDAGraph()
+        with cuda.cuda.graph(graph, stream=side):
+            total = cuda.zeros_like(y)
+            for i in range(3):
+                x.copy_(q)
+                y.fill_(-1)
+                ib.attention_paged(pages, seqs, batch, 1, x, scale, out=y, workspace=ws)
+                x.zero_()
+                total += y
+        for _ in range(5):
+            graph.replay()
+    side.synchronize()
+    assert cuda.equal(y, out) and cuda.equal(total, out + out + out)
+    assert ib.check_fault() == 0
+
+
+@TYPES
+@pytest.mark.parametrize("HD", [136, 256])
+def test_large_head_dim_bad_values(cuda, type_, HD):
+    for q_len in (1, 100):
+        pages, seqs, batch, q, out, scale = run_attention(cuda, type_, 8, 2, HD, 16, [q_len], [300])
+        slot = batch.slots[0].item()
+        for bad in (2 ** 31 - 1, pages.n_pages, -2, -2 ** 31):
+            seqs.table[slot, 3] = bad
+            got = ib.attention_paged(pages, seqs, batch, 1, q, scale)
+            with pytest.raises(RuntimeError, match="72"):
+                ib.check_fault()
+            seqs.table[slot, 3] = -1
+            assert cuda.equal(got, ib.attention_paged(pages, seqs, batch, 1, q, scale))
+        assert ib.check_fault() == 0
