@@ -333,8 +333,9 @@ int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_b
  * of 4, 16-byte aligned); out is q itself, with its stride, or shares nothing with it.  A NaN or infinity in a position that a row
  * does not see leaves the row alone; in one that it sees, the row's outputs are not specified
  * (NaN, as a rule).
- * q, K and V may be of any finite size; the division by the sum of weights comes last, so
- * the sum of e^(s - largest s) |v| over a row's positions has to stay below FP32's largest value.
+ * q, K and V may be of any finite size as long as the sums of q.k and, since the division by
+ * the sum of weights comes last, of e^(s - largest s) |v| over a row's positions stay below
+ * FP32's largest value.
  * workspace: ib_attention_paged_workspace(...) bytes, 256-byte aligned, that no other call
  * uses at the same time; it needs no initial value. */
 size_t ib_attention_paged_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,

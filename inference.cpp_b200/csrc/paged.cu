@@ -541,10 +541,10 @@ __device__ __forceinline__ int seq_of_token(const PagedView& w, int t) {
 
 // RoPE on q and k (interleaved pairs, the reference's table, src/ops/cuda_kernels.cu:372-400)
 // and the write of k and v into the pages: one CTA per token, one thread per eight elements
-// of a head.  Bound by HBM (every element read once and written once): the loads of a
-// thread's elements are issued before the page is looked up.  6798 prompt tokens (32 heads on 8,
-// head_dim 128, FP32) take 55 us in a graph, 6.1 TB/s, 0.93 of the measured rate; 64 single tokens
-// 4.1 us, a launch and its dependent loads.
+// of a head.  Bound by HBM (every element read once and written once).  The page and its reference
+// count are looked up first: with a thread's first elements loaded before them 64 single tokens took
+// 4.33 us in a graph, 4.23 this way, a launch and its dependent loads; 6798 prompt tokens (32 heads
+// on 8, head_dim 128, FP32) 57.3 and 57.7 us, 5.8 TB/s, 0.89 of the measured rate.
 template <typename KV>
 __global__ void __launch_bounds__(256)
     kv_append_kernel(const PagedView w, const float* q, int64_t q_stride,

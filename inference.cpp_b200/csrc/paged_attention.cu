@@ -9,7 +9,7 @@
 // Lengths are device data: every CTA works the cuts out for itself from cu_q and len (one pass
 // over the batch; no planning launch).
 //
-// Products of FP32 operands keep about 2^-21 on the tensor cores:
+// Products of FP32 operands keep 2^-20 or better on the tensor cores:
 //   FP16 pages  q = hi + lo and p = hi + lo in FP16, K and V as they are: two products.  q rows
 //               are scaled to a largest element in [256, 512) and p by 2^10, powers of two that
 //               keep the lo parts out of FP16's subnormals.
@@ -317,8 +317,9 @@ struct WarpRows {
 // own ring in shared memory filled by its own cp.async and no barrier in the loop; they join at
 // the end.  A ring slot is one half of a tile, K or V.  64 single tokens over 200..4096 positions
 // (32 heads on 8, head_dim 128): 113 us with FP16 pages, 5.1 TB/s or 0.78 of the measured rate (join
-// included), 219 us with FP32 pages, 5.3 TB/s; two tokens over 100001..131072 positions (64 heads
-// on 8, FP16) 170 us, 5.5 TB/s.  (Warps with pieces of their own, their
+// included), 5.2 to 5.3 TB/s with FP32 pages (1.23 GB in 233 us); two tokens over 100001..131072
+// positions (64 heads on 8, FP16) 168 to 178 us, 5.2 to 5.5 TB/s.  At head_dim 256, with fewer and
+// longer ring slots to an SM, 3.7 TB/s (FP16) and 3.4 TB/s (FP32).  (Warps with pieces of their own, their
 // copies running on from tile to tile, took 135 us against 119 us for 64 single tokens over
 // 200..4096 positions: warps far apart in the code miss the instruction cache.)
 template <typename KV, int HDP>
@@ -703,8 +704,8 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
 // ---- more rows on mma.sync, for head_dim over 128 -----------------------------------------
 // WR warps of 16 rows each over the same key tiles, which the CTA brings in together.  Bound by
 // the legacy tensor path and the splitting of its operands: the last 1024 of 4096 positions (16
-// heads on 8, head_dim 256, FP16) 624 us, 96 TFLOP/s of the formula, where head_dim 128 on
-// tcgen05 has 540.
+// heads on 8, head_dim 256) 624 to 650 us on FP16 pages, 93 to 96 TFLOP/s of the formula, where
+// head_dim 128 on tcgen05 has 510 to 560; 1.95 ms on FP32 pages.
 template <typename KV, int HDP>
 struct WideCfg {
     static constexpr bool F32 = sizeof(KV) == 4;
@@ -997,8 +998,6 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2)
 }
 
 // ---- launches ----------------------------------------------------------------------------
-constexpr int kSMs = 148;  // of a B200: the items aimed at, and so the workspace, follow it
-
 // One kernel's share of a call.
 struct Share {
     CutRule rule;
@@ -1042,16 +1041,27 @@ static int rows_launch(int threads, size_t smem, bool pieces, const RowsArgs& a,
 
 // The kernels of a call, by the rows (new tokens x group) that a sequence may have: up to
 // narrow_rows in tiles of eight on the narrow kernel, more on the wide one, by the caller's bound
-// one of them alone.  32 sequences over 200..4096 positions, narrow against tcgen05:
-//   FP16 pages, 32 heads on 8, head_dim 128   32 rows 167 us against 199, 64 rows 316 against 207
-//   FP32 pages, 32 heads on 4, head_dim 64    32 rows 116 us against 128, 64 rows 197 against 130
-//   FP32 pages, 32 heads on 8, head_dim 128   32 rows 417 us against 377 (V is split for every
-//                                             tile of eight rows), 64 rows 734 against 391
+// one of them alone.  Narrow against tcgen05 in us, at 16, 32 and 64 rows, 32 heads:
+//   sequences over        FP16, 8 kv heads of 128         FP16, 4 kv heads of 64
+//   2 x 30000..32000      90:140  152:139  274:140        37:68   51:68   82:66
+//   8 x 200..4096         42:69   59:67    95:65          23:36   25:36   34:36
+//   32 x 200..4096        101:180 167:185  317:196        37:77   58:76   103:78
+//   96 x 200..2000        162:310 292:317  534:337        62:121  102:128 181:130
+//                         FP32, 8 kv heads of 128         FP32, 4 kv heads of 64
+//   2 x 30000..32000      209:305 393:305  769:310        59:112  103:112 177:112
+//   8 x 200..4096         76:113  120:115  202:120        33:49   44:48   64:49
+//   32 x 200..4096        215:362 426:370  750:385        72:119  115:119 199:121
+//   96 x 200..2000        352:588 633:609  1214:630       104:186 184:192 336:193
+// The number of sequences and their lengths move the crossing little: the kernel not taken is ahead
+// only for two long sequences of 32 rows (FP16, head_dim 128), by 8 %, and for 64 rows of a few short
+// ones (FP16, head_dim 64), by 6 %.
 template <typename KV, int HDP>
 constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 
 // Wide tiles run on tcgen05 for head_dim up to 128.  Above, S and O of two query tiles do not fit
-// into tensor memory, nor FP32 sums of a row into a thread's registers.
+// into tensor memory, nor FP32 sums of a row into a thread's registers; one query tile whose sums are
+// shared by both softmax groups would fit on FP16 pages and is not built, on FP32 pages the TF32 parts
+// of 128 query rows alone take 256 KB of shared memory.
 template <int HDP>
 constexpr bool on_tcgen05 = HDP <= 128;
 

@@ -32,12 +32,14 @@
 // Work per CTA is a piece of the batch (paged_plan.cuh); the copies run on into the next
 // segment.
 //
-// Measured: 2048 tokens behind 6144 (32 heads on 8, head_dim 128, FP16) 420 us, 1145 TFLOP/s of
-// MMAs, 0.70 of the measured rate of library FP16 products; the tensor pipe is busy 0.60 of the
-// cycles.  A step of both query tiles takes 6.3k cycles to the MMAs' 4.1k: the bound is the softmax
+// Measured: 2048 tokens behind 6144 (32 heads on 8, head_dim 128, FP16) 471 us, 1020 TFLOP/s of
+// MMAs, 0.63 of the measured rate of library FP16 products (421 to 427 us in runs of a few
+// milliseconds, before the power limit lowers the clock), and 299 us at head_dim 64; the tensor pipe
+// is busy 0.60 of the cycles.  A step of both query tiles takes 6.3k cycles to the MMAs' 4.1k: the bound is the softmax
 // between a tile's S and its p, 3.8k cycles of dependent instructions with two warps to a scheduler
-// (the registers hold no more), which only half overlaps.  FP32 pages at head_dim 64: a step of
-// 6.3k cycles to 4.6k; 8.4k while the warp that starts the copies split them too.
+// (a row's running sums in one thread leave registers for no more), which only half overlaps.  FP32
+// pages at head_dim 64: a step of 6.3k cycles to 4.6k; 8.4k while the warp that starts the copies
+// split them too.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -1035,11 +1037,11 @@ static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head
 
 template <typename KV>
 CutRule tensor_rule(int head_dim, int min_rows, int max_rows) {
-    // one CTA to an SM (148 of a B200), a piece for each
+    // one CTA to an SM, a piece for each
     using S = TensorCfg<KV, 64>;
     using L = TensorCfg<KV, 128>;
-    return head_dim <= 64 ? CutRule{S::R, S::KT, min_rows, max_rows, 148, 128}
-                          : CutRule{L::R, L::KT, min_rows, max_rows, 148, 128};
+    return head_dim <= 64 ? CutRule{S::R, S::KT, min_rows, max_rows, kSMs, 128}
+                          : CutRule{L::R, L::KT, min_rows, max_rows, kSMs, 128};
 }
 template CutRule tensor_rule<float>(int, int, int);
 template CutRule tensor_rule<__half>(int, int, int);
