@@ -245,7 +245,8 @@ typedef struct {
 
 /* Sequences: slot s holds len[s] positions, position p in page table[s][p / page_size] at
  * row p % page_size.  table [n_slots][max_pages]: -1 behind the last page, and where a page
- * was given back early (its positions are then passed over).  refs [n_pages]: how many table
+ * was given back early: the caller sets the entry to -1 and takes one from the page's refs (its
+ * positions are then passed over).  refs [n_pages]: how many table
  * entries hold the page, 0 = free.  An empty cache is table = -1, len = 0, refs = 0; the
  * calls below keep it so.  max_pages * page_size <= 2^28. */
 typedef struct {
