@@ -270,8 +270,9 @@ typedef struct {
 /* Values in device memory cannot be checked by the host.  A slot, length, cu_q or table entry
  * out of range is clamped or passed over by the kernel, never used as an address, and
  * recorded: ib_check_fault then returns IB_ERR_INVALID with code 71 (slot), 72 (table entry),
- * 73 (len or cu_q), 74 (refs below the tables' entries), 75 (position behind rope_table) or 77
- * (a new token's page has refs over 1: ib_kv_append writes no page that others hold too).  An
+ * 73 (len or cu_q), 74 (refs below the tables' entries), 75 (position behind rope_table), 77
+ * (a new token's page has refs over 1: ib_kv_append writes no page that others hold too) or 78 (a
+ * tree's node, parent, depth or path).  An
  * expired wait of ib_attention_paged is IB_ERR_TIMEOUT with code 76, also where values were bad
  * as well: results are missing then.  ib_kv_wait_selftest records a bad table entry and lets a
  * short wait run out, for a test of that.
@@ -345,6 +346,92 @@ int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const i
                        int layer, int n_heads, const float* q, int64_t q_stride, float* out,
                        int64_t out_stride, float scale, void* workspace, size_t workspace_bytes,
                        void* stream);
+
+/* ib_kv_reorder: slots[i] becomes what slots[parents[i]] held before the call, for all entries at
+ * once (a beam search's states behind ib_beam_select: its out_row as parents).  Whole pages are shared;
+ * a partial last page goes as it is to the entry whose slot holds it, else to the first that takes
+ * it, and its filled rows are copied, in every layer, for the others, to pages handed out lowest first
+ * in list order, out of those that are free once every slot of the list has given up what it held.
+ * parents[i] is -1: the slot is left empty.  status[i]: 1 done; 0 no page for the copy, the slot is
+ * left empty (not possible where all slots have the same length); -1 refused, the slot is as it was (a
+ * slot out of range or named by an earlier entry, parents[i] out of [-1, n) or naming a slot out of
+ * range).  Lists and status as above.  workspace: ib_kv_reorder_workspace(...) bytes, 256-byte
+ * aligned, no initial value, no other call's at the same time. */
+size_t ib_kv_reorder_workspace(const ib_kv_seqs* seqs, int n);
+int ib_kv_reorder(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n, const int32_t* slots,
+                  const int32_t* parents, int32_t* status, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* Trees of drafted tokens: a sequence's n new tokens are nodes 0 .. n - 1, stored as positions
+ * len - n + i as ever, each with a parent: an earlier node, or -1 where it follows the context.
+ * depth [n_tokens]: a node's ancestors in the tree, counted; mask [n_tokens][(max_nodes + 31) / 32]:
+ * bit c % 32 of word c / 32 of a node's row is set where node c of its sequence is the node itself or
+ * one of its ancestors.  max_nodes: in [1, IB_KV_MAX_NODES]; a sequence with more new tokens is left
+ * out, as one whose batch slot is -1, and recorded (code 78).
+ *
+ * ib_kv_tree_plan: depth and mask from the parents [n_tokens] of a batch's nodes (once a step: every
+ * layer uses them).  A parent that is no earlier node counts as -1 and is recorded (78).  Rows of
+ * nobody are left as they were. */
+#define IB_KV_MAX_NODES 1024
+typedef struct {
+    int32_t max_nodes;
+    const int32_t* depth;
+    const uint32_t* mask;
+} ib_kv_tree;
+int ib_kv_tree_plan(const ib_kv_batch* batch, const int32_t* parents, int max_nodes, int32_t* depth,
+                    uint32_t* mask, void* stream);
+/* ib_kv_append_tree: as ib_kv_append, with q and k rotated by position len - n + depth.  A depth that
+ * is negative or above the node's number passes the token over (78). */
+int ib_kv_append_tree(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                      const ib_kv_tree* tree, int layer, int n_heads, const float* q, int64_t q_stride,
+                      const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                      float* q_out, int64_t q_out_stride, const float* rope_table, int rope_len,
+                      void* stream);
+/* ib_attention_paged_tree: as ib_attention_paged, where node i sees the positions before len - n and
+ * those of the nodes in its mask row (up to and with i; bits of later nodes do not count). */
+size_t ib_attention_paged_tree_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                         const ib_kv_batch* batch, const ib_kv_tree* tree, int n_heads);
+int ib_attention_paged_tree(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                            const ib_kv_tree* tree, int layer, int n_heads, const float* q,
+                            int64_t q_stride, float* out, int64_t out_stride, float scale,
+                            void* workspace, size_t workspace_bytes, void* stream);
+/* ib_kv_tree_verify: greedy verification.  Node 0 holds a token that is certain; the path goes from
+ * a node to its first child whose token is best[node], what the model chose behind it (parents,
+ * tokens, best [n_tokens], ib_beam_select with k = 1 for the last).  Sequence b's path, n_path[b]
+ * nodes, is written to its rows of path [n_tokens] (-1 behind it), and next[b] = best of its last node,
+ * the token to go on with.  A sequence without nodes (left out, or more than IB_KV_MAX_NODES):
+ * n_path 0, next -1.  Results must not overlap the lists. */
+int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parents, const int32_t* tokens,
+                      const int32_t* best, int32_t* path, int32_t* n_path, int32_t* next, void* stream);
+/* ib_kv_tree_accept: of a batch's new tokens only the path stays, in every layer: the K and V of node
+ * path[j] move to position len - n + j (path in a sequence's rows, its nodes in order, as above or by
+ * the caller's own verification), len becomes len - n + n_path and the pages behind it are given back.
+ * n_path 0 drops all new tokens.  Recorded and passed over: n_path out of [0, n] (78: nothing is
+ * changed); an entry that is no node behind the one before (78: the path ends there); a move into a
+ * page that others hold too (77).  Moves from or to a page that is not there are passed over. */
+int ib_kv_tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                      const int32_t* path, const int32_t* n_path, void* stream);
+
+/* ib_beam_select: the k best continuations of each group of beams.  Row r of the logits [n_groups x
+ * beams][vocab] (F32 or F16, rows stride elements apart) offers every token t with the value
+ *     scores[r] + logits[r][t] - log sum_t' e^logits[r][t'];
+ * a row with ended[r] != 0 offers end_token alone, with the value scores[r], and its logits are not
+ * read.  A group's k largest go to out_score, out_token and out_row [n_groups][k] (out_row: the row),
+ * largest first, equal values in the order of row and token.  Values are compared in more than FP32
+ * and rounded once.  Those that are -inf or NaN are no candidates: a banned token's -inf, a row whose
+ * score is -inf, all of a row with a NaN or +inf logit.  Places without a candidate: -inf, -1, -1.
+ * scores and ended may be NULL (zeros).  With beams = 1 it is the rows' top k; with k = 1 their first
+ * maximum, as ib_argmax.  beams in [1, IB_BEAM_MAX_BEAMS], n_groups x beams <= 2^20, vocab <= 2^28,
+ * k in [1, IB_BEAM_MAX_K].  Results must not overlap the inputs or the workspace.  workspace:
+ * ib_beam_select_workspace(...) bytes, 256-byte aligned, no initial value, no other call's at the same
+ * time. */
+#define IB_BEAM_MAX_BEAMS 1024
+#define IB_BEAM_MAX_K 128
+size_t ib_beam_select_workspace(int n_groups, int beams, int vocab, int k);
+int ib_beam_select(int type, const void* logits, int64_t stride, const float* scores,
+                   const int32_t* ended, int end_token, int n_groups, int beams, int vocab, int k,
+                   float* out_score, int32_t* out_token, int32_t* out_row, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 /* Index of the first maximum of x[0..n) (reference sample_argmax,
  * src/ops/ops.cpp:424-438), written to *dev_out. */

@@ -18,6 +18,7 @@ import contextlib
 import ctypes
 import functools
 import os
+import typing
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libib_cuda.so")
@@ -123,13 +124,27 @@ SIGNATURES = {
                      _vp],
     "ib_attention_paged_workspace": [_vp, _vp, _vp, _i],
     "ib_attention_paged": [_vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _f, _vp, _sz, _vp],
+    "ib_kv_reorder_workspace": [_vp, _i],
+    "ib_kv_reorder": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp],
+    "ib_kv_tree_plan": [_vp, _vp, _i, _vp, _vp, _vp],
+    "ib_kv_append_tree": [_vp, _vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                          _vp, _i, _vp],
+    "ib_attention_paged_tree_workspace": [_vp, _vp, _vp, _vp, _i],
+    "ib_attention_paged_tree": [_vp, _vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _f, _vp, _sz,
+                                _vp],
+    "ib_kv_tree_verify": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ib_kv_tree_accept": [_vp, _vp, _vp, _vp, _vp, _vp],
+    "ib_beam_select_workspace": [_i, _i, _i, _i],
+    "ib_beam_select": [_i, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp],
     "ib_argmax": [_vp, _i, _vp, _vp],
     "ib_synth_host": [_i, _i64, _i64, _u64, _f, _vp, _i],
     "ib_synth_device": [_i, _i64, _i64, _u64, _f, _vp, _vp],
     "ib_synth_values_host": [_i64, _u64, _f, _vp],
 }
 _RESTYPE = {"ib_last_error": _c.c_char_p, "ib_attention_split_part_bytes": _c.c_size_t,
-            "ib_gemm_planes_bytes": _c.c_size_t, "ib_attention_paged_workspace": _c.c_size_t}
+            "ib_gemm_planes_bytes": _c.c_size_t, "ib_attention_paged_workspace": _c.c_size_t,
+            "ib_attention_paged_tree_workspace": _c.c_size_t,
+            "ib_kv_reorder_workspace": _c.c_size_t, "ib_beam_select_workspace": _c.c_size_t}
 
 _lib = None
 
@@ -610,7 +625,7 @@ class KVBatch:
         self.cu_q = _paged_tensor(cu_q, "cu_q", torch.int32, (-1,), None)
         self.device = cu_q.device
         self.n_seqs, self.n_tokens = cu_q.numel() - 1, int(n_tokens)
-        self.slots = slots
+        self.slots, self.max_q = slots, int(max_q)
         if slots is not None:
             _paged_tensor(slots, "slots", torch.int32, (self.n_seqs,), self.device)
         self._c = _CKVBatch(self.n_seqs, self.n_tokens, int(max_q), cu_q.data_ptr(), _ptr(slots))
@@ -708,6 +723,41 @@ def kv_release(pages, seqs, slots, stream=None):
     _call("ib_kv_release", pages._p, _seqs_of(pages, seqs), n, a, st)
 
 
+def _workspace(pages, workspace):
+    """(pointer, bytes) of a caller's workspace on the pages' device."""
+    if workspace.device != pages.device or not workspace.is_contiguous():
+        raise ValueError(f"workspace: on {workspace.device}, contiguous "
+                         f"{workspace.is_contiguous()}; expected contiguous on {pages.device}")
+    return workspace.data_ptr(), workspace.nbytes
+
+
+def kv_reorder_workspace(seqs, n):
+    """Scratch for kv_reorder calls with n slots, one at a time (a uint8 CUDA tensor)."""
+    size = lib().ib_kv_reorder_workspace(seqs._p, n)
+    if size == 0:
+        raise ValueError(last_error())
+    return _torch().empty(size, dtype=_torch().uint8, device=seqs.device)
+
+
+def kv_reorder(pages, seqs, slots, parents, status=None, workspace=None, stream=None):
+    """slots[i] becomes what slots[parents[i]] held, all at once (-1: it is left empty): the states
+    of a beam search behind beam_select, whose rows are the parents.  Whole pages are shared, a
+    partial last page goes to one of those that take it and is copied for the others.  Returns
+    status (1 done, 0 no page for the copy: left empty, -1 refused: as it was).  workspace:
+    kv_reorder_workspace(), allocated for the call when None."""
+    n = slots.numel()
+    st = _paged_stream(pages, stream, seqs)
+    if status is None or workspace is None:
+        with _allocating(pages, stream):
+            status = _torch().empty_like(slots) if status is None else status
+            workspace = kv_reorder_workspace(seqs, n) if workspace is None else workspace
+    a, b, c = (_paged_list(pages, slots, "slots", n), _paged_list(pages, parents, "parents", n),
+               _paged_list(pages, status, "status", n))
+    _call("ib_kv_reorder", pages._p, _seqs_of(pages, seqs), n, a, b, c, *_workspace(pages, workspace),
+          st)
+    return status
+
+
 class KVCompactPlan:
     """What kv_compact did: map [n_pages] (new index of each page, -1 for a free one), info
     {pages in use, pages moved} and the moves' (old, new) pairs."""
@@ -764,10 +814,98 @@ def _paged_rows(t, name, tokens, heads, head_dim, device):
     return t.data_ptr(), row if tokens > 1 else heads * head_dim, heads
 
 
-def kv_append(pages, seqs, batch, layer, q, k, v, rope_table, q_out=None, stream=None):
+class _CKVTree(ctypes.Structure):
+    _fields_ = [("max_nodes", ctypes.c_int32), ("depth", ctypes.c_void_p), ("mask", ctypes.c_void_p)]
+
+
+KV_MAX_NODES = 1024  # IB_KV_MAX_NODES
+
+
+class KVTree:
+    """The trees of a batch whose new tokens are drafts: parents [n_tokens] (an earlier node of the
+    same sequence, or -1: what follows the context), depth [n_tokens] and mask [n_tokens,
+    (max_nodes + 31) // 32] (bit c % 32 of word c // 32: node c is the row's own or an ancestor),
+    int32 CUDA tensors, kept here; kv_tree fills depth and mask from the parents."""
+
+    def __init__(self, parents, depth, mask, max_nodes):
+        import torch
+        max_nodes = int(max_nodes)
+        if not 1 <= max_nodes <= KV_MAX_NODES:
+            raise ValueError(f"max_nodes: {max_nodes}, expected 1 .. {KV_MAX_NODES}")
+        self.parents = _paged_tensor(parents, "parents", torch.int32, (-1,), None)
+        self.device, self.n_tokens, self.max_nodes = parents.device, parents.shape[0], max_nodes
+        self.depth = _paged_tensor(depth, "depth", torch.int32, (self.n_tokens,), self.device)
+        self.mask = _paged_tensor(mask, "mask", torch.int32,
+                                  (self.n_tokens, (max_nodes + 31) // 32), self.device)
+        self._c = _CKVTree(max_nodes, depth.data_ptr(), mask.data_ptr())
+        self._p = ctypes.addressof(self._c)
+
+
+def _tree_of(pages, batch, tree):
+    if tree.device != pages.device:
+        raise ValueError(f"arguments on {pages.device} and {tree.device}")
+    if tree.n_tokens != batch.n_tokens:
+        raise ValueError(f"tree: {tree.n_tokens} nodes for {batch.n_tokens} tokens")
+    return tree._p
+
+
+def kv_tree(batch, parents, max_nodes=0, out=None, stream=None):
+    """The trees of a batch's new tokens from their parents: once a step, for every layer's
+    kv_append and attention_paged.  max_nodes: the most nodes of one sequence (0: the batch's
+    max_q, or its n_tokens); a sequence with more is left out of the step and recorded.  out: a
+    KVTree of such a batch, whose depth and mask are filled again.  Returns the KVTree."""
+    torch, T = _torch(), batch.n_tokens
+    st = _paged_stream(batch, stream)
+    p = _paged_list(batch, parents, "parents", T)
+    if out is None:
+        max_nodes = int(max_nodes) or min(batch.max_q or T, T) or 1
+        with _allocating(batch, stream):
+            out = KVTree(parents, torch.zeros(T, dtype=torch.int32, device=batch.device),
+                         torch.zeros(T, (max_nodes + 31) // 32, dtype=torch.int32,
+                                     device=batch.device), max_nodes)
+    elif out.n_tokens != T or out.device != batch.device or max_nodes not in (0, out.max_nodes):
+        raise ValueError("out: a tree of another batch")
+    _call("ib_kv_tree_plan", batch._p, p, out.max_nodes, out.depth.data_ptr(), out.mask.data_ptr(),
+          st)
+    out.parents = parents
+    return out
+
+
+def kv_tree_verify(batch, parents, tokens, best, path=None, n_path=None, next=None, stream=None):
+    """Greedy verification of the batch's trees.  tokens: the nodes' tokens (node 0's is certain),
+    best: what the model chose behind each node (beam_select with k = 1), int32 [n_tokens].
+    Returns path [n_tokens] (the confirmed nodes of a sequence, in its rows, -1 behind them),
+    n_path and next [n_seqs] (the token behind the last confirmed node; -1: no nodes)."""
+    torch, T, n = _torch(), batch.n_tokens, batch.n_seqs
+    st = _paged_stream(batch, stream)
+    if path is None or n_path is None or next is None:
+        with _allocating(batch, stream):
+            make = lambda m: torch.full((m,), -1, dtype=torch.int32, device=batch.device)  # noqa: E731
+            path = make(T) if path is None else path
+            n_path = make(n) if n_path is None else n_path
+            next = make(n) if next is None else next
+    _call("ib_kv_tree_verify", batch._p, _paged_list(batch, parents, "parents", T),
+          _paged_list(batch, tokens, "tokens", T), _paged_list(batch, best, "best", T),
+          _paged_list(batch, path, "path", T), _paged_list(batch, n_path, "n_path", n),
+          _paged_list(batch, next, "next", n), st)
+    return path, n_path, next
+
+
+def kv_tree_accept(pages, seqs, batch, path, n_path, stream=None):
+    """Of the batch's new tokens only the path stays in the cache: its K and V move together in
+    every layer, the lengths follow, and the pages behind them are given back.  path, n_path: as
+    kv_tree_verify returns them, or the caller's own."""
+    st = _paged_stream(pages, stream, seqs, batch)
+    _call("ib_kv_tree_accept", pages._p, _seqs_of(pages, seqs), batch._p,
+          _paged_list(pages, path, "path", batch.n_tokens),
+          _paged_list(pages, n_path, "n_path", batch.n_seqs), st)
+
+
+def kv_append(pages, seqs, batch, layer, q, k, v, rope_table, q_out=None, stream=None, tree=None):
     """RoPE on q and k and the write of k and v into the layer's pages.  q [tokens, heads,
     head_dim], k and v [tokens, kv heads, head_dim] float32 (rows may be slices);
-    rope_table [positions, head_dim / 2, 2].  Returns q_out."""
+    rope_table [positions, head_dim / 2, 2].  tree: the new tokens are nodes of trees (kv_tree),
+    rotated by their depths.  Returns q_out."""
     torch = _torch()
     T, HD, Hkv, dev = batch.n_tokens, pages.head_dim, pages.n_kv_heads, pages.device
     if q_out is None:
@@ -780,24 +918,35 @@ def kv_append(pages, seqs, batch, layer, q, k, v, rope_table, q_out=None, stream
     n = rope_table.shape[0]
     _paged_tensor(rope_table, "rope_table", torch.float32, (n, HD // 2, 2), dev)
     st = _paged_stream(pages, stream, seqs, batch)
-    _call("ib_kv_append", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, kp, ks, vp,
-          vs, op, os_, rope_table.data_ptr(), n, st)
+    args = (layer, H, qp, qs, kp, ks, vp, vs, op, os_, rope_table.data_ptr(), n, st)
+    if tree is None:
+        _call("ib_kv_append", pages._p, _seqs_of(pages, seqs), batch._p, *args)
+    else:
+        _call("ib_kv_append_tree", pages._p, _seqs_of(pages, seqs), batch._p,
+              _tree_of(pages, batch, tree), *args)
     return q_out
 
 
-def attention_paged_workspace(pages, seqs, batch, n_heads):
+def attention_paged_workspace(pages, seqs, batch, n_heads, tree=None):
     """Scratch for attention_paged calls of this shape, one at a time (a uint8 CUDA tensor)."""
     import torch
-    n = lib().ib_attention_paged_workspace(pages._p, seqs._p, batch._p, n_heads)
+    if tree is None:
+        n = lib().ib_attention_paged_workspace(pages._p, seqs._p, batch._p, n_heads)
+    else:
+        n = lib().ib_attention_paged_tree_workspace(pages._p, seqs._p, batch._p,
+                                                    _tree_of(pages, batch, tree), n_heads)
     if n == 0:
         raise ValueError(last_error())
     return torch.empty(n, dtype=torch.uint8, device=pages.device)
 
 
-def attention_paged(pages, seqs, batch, layer, q, scale, out=None, workspace=None, stream=None):
+def attention_paged(pages, seqs, batch, layer, q, scale, out=None, workspace=None, stream=None,
+                    tree=None):
     """Causal attention of the batch's new tokens over the layer's pages.  q, out [tokens,
     heads, head_dim] float32 (rows may be slices).  workspace: attention_paged_workspace(),
-    allocated for the call when None.  Returns out (rows of nobody: as they were)."""
+    allocated for the call when None.  tree: the new tokens are nodes of trees (kv_tree): each sees
+    the context, its ancestors and itself; the workspace is then one made with the tree.  Returns
+    out (rows of nobody: as they were)."""
     torch = _torch()
     T, HD, dev = batch.n_tokens, pages.head_dim, pages.device
     qp, qs, H = _paged_rows(q, "q", T, None, HD, dev)
@@ -808,11 +957,84 @@ def attention_paged(pages, seqs, batch, layer, q, scale, out=None, workspace=Non
     st = _paged_stream(pages, stream, seqs, batch)
     if workspace is None:
         with _allocating(pages, stream):
-            workspace = attention_paged_workspace(pages, seqs, batch, H)
+            workspace = attention_paged_workspace(pages, seqs, batch, H, tree)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise ValueError(f"workspace: on {workspace.device}, expected contiguous on {dev}")
-    _call("ib_attention_paged", pages._p, _seqs_of(pages, seqs), batch._p, layer, H, qp, qs, op,
-          os_, scale, workspace.data_ptr(), workspace.nbytes, st)
+    args = (layer, H, qp, qs, op, os_, scale, workspace.data_ptr(), workspace.nbytes, st)
+    if tree is None:
+        _call("ib_attention_paged", pages._p, _seqs_of(pages, seqs), batch._p, *args)
+    else:
+        _call("ib_attention_paged_tree", pages._p, _seqs_of(pages, seqs), batch._p,
+              _tree_of(pages, batch, tree), *args)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# beam search (ib_beam_select; the beams' states follow with kv_reorder)
+# ---------------------------------------------------------------------------
+
+class BeamChoice(typing.NamedTuple):
+    """What beam_select chose, [groups, k], largest first: score float32, token and row int32
+    (-inf, -1, -1 where there was no candidate)."""
+    score: typing.Any
+    token: typing.Any
+    row: typing.Any
+
+
+def _beam_shape(logits, beams, k):
+    """(type, rows, vocab, groups, k) of a selection."""
+    torch = _torch()
+    type_ = {torch.float32: F32, torch.float16: F16}.get(logits.dtype)
+    if type_ is None or logits.dim() != 2 or not logits.is_cuda:
+        raise ValueError(f"logits: {logits.dtype} {tuple(logits.shape)} on {logits.device}, expected "
+                         f"float32 or float16 [rows, vocab] on a CUDA device")
+    rows, vocab = logits.shape
+    if beams < 1 or rows % beams:
+        raise ValueError(f"beams: {beams}, expected a divisor of {rows} rows")
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: the values of a row are not contiguous")
+    return type_, rows, vocab, rows // beams, beams if k is None else int(k)
+
+
+def beam_select_workspace(logits, beams=1, k=None):
+    """Scratch for beam_select calls of this shape, one at a time (a uint8 CUDA tensor)."""
+    _, _, vocab, groups, k = _beam_shape(logits, beams, k)
+    n = lib().ib_beam_select_workspace(groups, beams, vocab, k)
+    if n == 0:
+        raise ValueError(last_error())
+    return _torch().empty(n, dtype=_torch().uint8, device=logits.device)
+
+
+def beam_select(logits, scores=None, beams=1, k=None, ended=None, end_token=0, out=None,
+                workspace=None, stream=None):
+    """The k (default: beams) best continuations of each group of `beams` rows of the logits [rows,
+    vocab] (float32 or float16, rows may be apart): scores[row] + log_softmax(logits[row])[token],
+    equal ones in the order of row and token.  ended [rows] int32: a row with a value other than 0
+    offers (end_token, scores[row]) alone.  -inf and NaN are no candidates.  Returns a BeamChoice
+    (out: one to be filled).  With beams = 1, the rows' top k; with k = 1, their argmax.
+    workspace: beam_select_workspace(), allocated for the call when None."""
+    torch = _torch()
+    type_, rows, vocab, groups, k = _beam_shape(logits, beams, k)
+    dev = logits.device
+    st = _paged_stream(logits, stream)
+    if out is None or workspace is None:
+        with _allocating(logits, stream):
+            if out is None:
+                out = BeamChoice(torch.empty(groups, k, device=dev),
+                                 *(torch.empty(groups, k, dtype=torch.int32, device=dev)
+                                   for _ in range(2)))
+            if workspace is None:
+                workspace = beam_select_workspace(logits, beams, k)
+    for t, name, dtype, shape in ((scores, "scores", torch.float32, (rows,)),
+                                  (ended, "ended", torch.int32, (rows,)),
+                                  (out.score, "out.score", torch.float32, (groups, k)),
+                                  (out.token, "out.token", torch.int32, (groups, k)),
+                                  (out.row, "out.row", torch.int32, (groups, k))):
+        if t is not None:
+            _paged_tensor(t, name, dtype, shape, dev)
+    _call("ib_beam_select", type_, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+          _ptr(scores), _ptr(ended), end_token, groups, beams, vocab, k, out.score.data_ptr(),
+          out.token.data_ptr(), out.row.data_ptr(), *_workspace(logits, workspace), st)
     return out
 
 

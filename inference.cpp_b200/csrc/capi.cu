@@ -154,6 +154,8 @@ extern "C" int ib_check_fault(int* code) {
     if ((st = paged_fault_take(&c2)) != IB_OK) return st;
     if ((st = paged_attention_fault_take(&c3)) != IB_OK) return st;
     c2 = paged_fault_worse(c2, c3);
+    if ((st = paged_tree_fault_take(&c3)) != IB_OK) return st;
+    c2 = paged_fault_worse(c2, c3);
     if (!*code && c2) {
         *code = c2;
         const std::string tail = " (code " + std::to_string(c2) + ")";
@@ -167,7 +169,8 @@ extern "C" int ib_check_fault(int* code) {
                            : c2 == PAGED_BAD_LEN  ? "a length or cu_q value was out of range"
                            : c2 == PAGED_BAD_REFS ? "a reference count was out of range"
                            : c2 == PAGED_BAD_ROPE ? "a RoPE position was out of range"
-                                                  : "a new token's page is held by other sequences too";
+                           : c2 == PAGED_SHARED   ? "a new token's page is held by other sequences too"
+                                                  : "a tree's node, parent, depth or path was out of range";
         set_error(std::string("CUDA: paged KV cache: ") + what + tail);
         return IB_ERR_INVALID;
     }

@@ -31,7 +31,7 @@ constexpr int KV_SCAN = 8;  // refs per thread and iteration of a scan
 constexpr int KV_COPY_THREADS = 256;
 
 // ---- checks ----------------------------------------------------------------------------
-static int paged_refuse(const char* who, const char* what) {
+int paged_refuse(const char* who, const char* what) {
     set_error(std::string(who) + ": " + what);
     return IB_ERR_INVALID;
 }
@@ -79,7 +79,17 @@ int paged_check_batch(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_bat
     return IB_OK;
 }
 
-PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int n_heads) {
+int paged_check_tree(const ib_kv_batch* b, const ib_kv_tree* t, const char* who) {
+    if (!t) return paged_refuse(who, "null pointer argument");
+    if (t->max_nodes < 1 || t->max_nodes > IB_KV_MAX_NODES)
+        return paged_refuse(who, "max_nodes must be in [1, 1024]");
+    if (b->n_tokens > 0 && b->n_seqs > 0 && (!t->depth || !t->mask))
+        return paged_refuse(who, "null pointer argument");
+    return IB_OK;
+}
+
+PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int n_heads,
+                     const ib_kv_tree* t) {
     PagedView w;
     w.table = s->table;
     w.len = s->len;
@@ -91,6 +101,7 @@ PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batc
     w.n_pages = p->n_pages;
     w.n_seqs = b->n_seqs;
     w.n_tokens = b->n_tokens;
+    w.max_nodes = t ? t->max_nodes : 0;
     w.H = n_heads;
     w.Hkv = p->n_kv_heads;
     w.HD = p->head_dim;
@@ -322,13 +333,6 @@ __device__ __forceinline__ void warp_copy(uint4* __restrict__ d, const uint4* __
     }
 }
 
-// The pool as bytes: layer l, page p at l * layer_bytes + p * page_bytes.
-struct PoolBytes {
-    uint8_t *k, *v;
-    int n_layers, n_kv_heads, row_bytes;  // row: head_dim elements
-    int64_t page_bytes, layer_bytes;
-};
-
 // Second half of a fork: children's rows, reference counts and the filled rows of the
 // partial pages, one warp per (child, layer, k or v, kv head) of those.  Bound by HBM once there are
 // many: 96 children of 22 layers 18 us, most of 119 MB read and written.
@@ -412,6 +416,193 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
         } else if (t != -1) {
             paged_fault(PAGED_BAD_PAGE);
         }
+    }
+}
+
+// ---- reorder ---------------------------------------------------------------------------
+// slots[i] becomes what slots[parents[i]] held, for all entries at once: a beam search's states follow
+// the selection.  Three kernels: what the slots give up and the new rows' whole pages, counted and the
+// rows put aside (a CTA per entry); who keeps a partial last page and which pages the others copy it
+// to (one CTA, as above); rows, lengths and copies (wide).
+struct ReorderWs {
+    int32_t* row;   // [n][max_pages] the new rows
+    int32_t* len;   // [n] the new lengths, -1: the entry is refused
+    int32_t* used;  // [n] entries of the old row
+    int32_t* src;   // [n] the partial last page that the entry takes, -1: none
+    int32_t* dst;   // [n] the page it is copied to, -1: it is kept as it is
+};
+
+__device__ __forceinline__ int pages_of(const KvSeqsDev& s, int L) {
+    return (L + s.page_size - 1) / s.page_size;
+}
+
+__global__ void __launch_bounds__(KV_COPY_THREADS)
+    kv_reorder_rows_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ slots,
+                           const int32_t* __restrict__ parents, const ReorderWs ws) {
+    __shared__ int named;
+    const int i = blockIdx.x, tid = threadIdx.x;
+    pdl_launch_dependents();
+    if (tid == 0) named = 0;
+    __syncthreads();
+    const int slot = slots[i], p = parents[i];
+    bool ok = slot >= 0 && slot < s.n_slots && p >= -1 && p < n;
+    if (ok) {  // the first entry that names a slot has it
+        bool before = false;
+        for (int j = tid; j < i; j += KV_COPY_THREADS) before |= slots[j] == slot;
+        if (before) named = 1;
+    }
+    const int from = ok && p >= 0 ? slots[p] : -1;
+    if (p >= 0) ok = ok && from >= 0 && from < s.n_slots;
+    __syncthreads();
+    ok = ok && !named;
+    const int cap = s.max_pages * s.page_size;
+    const int L0 = ok ? s.len[slot] : 0, L = ok && p >= 0 ? s.len[from] : 0;
+    if (L0 < 0 || L0 > cap || L < 0 || L > cap) {
+        if (tid == 0) paged_fault(PAGED_BAD_LEN);
+        ok = false;
+    }
+    if (!ok) {
+        if (tid == 0) ws.len[i] = -1;
+        return;
+    }
+    const int used = pages_of(s, L0), now = pages_of(s, L), full = L / s.page_size;
+    const int32_t* const old = s.table + (size_t)slot * s.max_pages;
+    const int32_t* const row = s.table + (size_t)(p >= 0 ? from : slot) * s.max_pages;
+    int32_t* const out = ws.row + (size_t)i * s.max_pages;
+    for (int j = tid; j < max(used, now); j += KV_COPY_THREADS) {
+        const int a = j < used ? old[j] : -1, z = j < now ? row[j] : -1;
+        if (j < now) out[j] = z;
+        if (j == full && j < now) ws.src[i] = z >= 0 && z < s.n_pages ? z : -1;
+        const bool keeps = j < full && z >= 0 && z < s.n_pages;
+        if ((a < -1 || a >= s.n_pages) || (z < -1 || z >= s.n_pages)) paged_fault(PAGED_BAD_PAGE);
+        if (keeps && z == a) continue;  // most of a beam's pages
+        if (a >= 0 && a < s.n_pages && atomicSub(&s.refs[a], 1) <= 0) {
+            atomicAdd(&s.refs[a], 1);  // held by nobody: leave it free
+            paged_fault(PAGED_BAD_REFS);
+        }
+        if (keeps) atomicAdd(&s.refs[z], 1);
+    }
+    if (tid == 0) {
+        ws.len[i] = L;
+        ws.used[i] = used;
+        if (full == now) ws.src[i] = -1;
+    }
+}
+
+// One CTA.  A partial last page goes, as it is, to the entry whose slot has it already, else to the
+// first that takes it; one of a slot that keeps it (a refused entry's) to nobody.  The others get
+// pages, lowest first in list order; where there is none, status 0, and the slot is left empty.
+__global__ void __launch_bounds__(KV_PLAN_THREADS)
+    kv_reorder_plan_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ slots,
+                           const int32_t* __restrict__ parents, const ReorderWs ws,
+                           int32_t* __restrict__ status) {
+    extern __shared__ int sh[];
+    __shared__ int warp_sums[32];
+    int* const heir = sh;             // [n_slots] rank of the entry that keeps the slot's partial page
+    int* const want = sh + s.n_slots; // [n] place among those that need a page, -1: needs none
+    const int tid = threadIdx.x;
+    pdl_launch_dependents();
+    for (int i = tid; i < s.n_slots; i += KV_PLAN_THREADS) heir[i] = -2;  // nobody has given it up
+    pdl_wait();
+    __syncthreads();
+    for (int i = tid; i < n; i += KV_PLAN_THREADS)
+        if (ws.len[i] >= 0) heir[slots[i]] = 0x7fffffff;
+    __syncthreads();
+    // rank: -1 for the slot itself, the place in the list for others
+    auto source = [&](int i) { return parents[i] >= 0 ? slots[parents[i]] : -1; };
+    for (int i = tid; i < n; i += KV_PLAN_THREADS)
+        if (ws.len[i] >= 0 && ws.src[i] >= 0) {
+            const int f = source(i);
+            if (heir[f] != -2) atomicMin(&heir[f], f == slots[i] ? -1 : i);
+        }
+    __syncthreads();
+    int total = 0;
+    for (int i0 = 0; i0 < n; i0 += KV_PLAN_THREADS) {
+        const int i = i0 + tid;
+        bool need = false;
+        if (i < n) {
+            const bool ok = ws.len[i] >= 0;
+            int to = -1;
+            if (ok && ws.src[i] >= 0) {
+                const int f = source(i);
+                need = heir[f] != (f == slots[i] ? -1 : i);
+                if (!need) atomicAdd(&s.refs[ws.src[i]], 1);
+            }
+            ws.dst[i] = to;
+            status[i] = ok ? 1 : -1;
+        }
+        int sum;
+        const int before = block_scan(need, warp_sums, sum);
+        if (i < n) want[i] = need ? total + before : -1;
+        total += sum;
+    }
+    __syncthreads();
+    if (total == 0) return;
+    // the k-th free page goes to the entry whose place is k
+    constexpr int ROUND = KV_PLAN_THREADS * KV_SCAN;
+    int given = 0;
+    int* const page_of = heir;  // [min(total, n_slots)]: heir is done with, and at most n_slots entries are served
+    for (int base = 0; base < s.n_pages && given < total; base += ROUND) {
+        int r[KV_SCAN], c = 0, sum;
+        const int64_t p0 = (int64_t)base + (int64_t)tid * KV_SCAN;
+#pragma unroll
+        for (int k = 0; k < KV_SCAN; ++k) {
+            r[k] = p0 + k < s.n_pages ? __ldcg(&s.refs[p0 + k]) : 1;
+            c += r[k] <= 0;
+        }
+        int k0 = given + block_scan(c, warp_sums, sum);
+        given += sum;
+#pragma unroll
+        for (int k = 0; k < KV_SCAN; ++k)
+            if (r[k] <= 0) {
+                if (k0 < total) {
+                    page_of[k0] = (int)p0 + k;
+                    s.refs[p0 + k] = 1;
+                }
+                ++k0;
+            }
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += KV_PLAN_THREADS)
+        if (want[i] >= 0) {
+            if (want[i] < given) ws.dst[i] = page_of[want[i]];
+            else status[i] = 0;
+        }
+}
+
+__global__ void __launch_bounds__(KV_COPY_THREADS)
+    kv_reorder_kernel(const KvSeqsDev s, const PoolBytes pool, int n, const int32_t* __restrict__ slots,
+                      const ReorderWs ws, const int32_t* __restrict__ status) {
+    const int tid = threadIdx.x;
+    pdl_wait();
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {  // rows: one CTA per entry
+        if (status[i] < 0) continue;
+        const int L = ws.len[i], full = L / s.page_size, now = pages_of(s, L);
+        const bool room = status[i] == 1;
+        const int dst = ws.dst[i];
+        int32_t* const row = s.table + (size_t)slots[i] * s.max_pages;
+        const int32_t* const in = ws.row + (size_t)i * s.max_pages;
+        for (int j = tid; j < max(ws.used[i], now); j += KV_COPY_THREADS) {
+            const int z = j < now ? in[j] : -1;
+            if (!room && j < full && z >= 0 && z < s.n_pages) atomicSub(&s.refs[z], 1);
+            row[j] = !room ? -1 : j == full && dst >= 0 ? dst : z;
+        }
+        if (tid == 0) s.len[slots[i]] = room ? L : 0;
+    }
+    const int n_warps = gridDim.x * (KV_COPY_THREADS / 32);
+    const int per = pool.n_layers * 2 * pool.n_kv_heads;
+    const int64_t units = (int64_t)n * per;
+    for (int64_t u = blockIdx.x * (KV_COPY_THREADS / 32) + (tid >> 5); u < units; u += n_warps) {
+        const int i = (int)(u / per);
+        int r = (int)(u - (int64_t)i * per);
+        if (status[i] != 1 || ws.dst[i] < 0) continue;
+        const int part = ws.len[i] % s.page_size;
+        const int head = r % pool.n_kv_heads;
+        r /= pool.n_kv_heads;
+        uint8_t* const base = ((r & 1) ? pool.v : pool.k) + (int64_t)(r >> 1) * pool.layer_bytes +
+                              (int64_t)head * s.page_size * pool.row_bytes;
+        warp_copy((uint4*)(base + ws.dst[i] * pool.page_bytes),
+                  (const uint4*)(base + ws.src[i] * pool.page_bytes), part * pool.row_bytes / 16);
     }
 }
 
@@ -545,19 +736,30 @@ __device__ __forceinline__ int seq_of_token(const PagedView& w, int t) {
 // count are looked up first: with a thread's first elements loaded before them 64 single tokens took
 // 4.33 us in a graph, 4.23 this way, a launch and its dependent loads; 6798 prompt tokens (32 heads
 // on 8, head_dim 128, FP32) 57.3 and 57.7 us, 5.8 TB/s, 0.89 of the measured rate.
-template <typename KV>
+// TREE: token i of n is stored as position L - n + i all the same, but rotated by L - n + depth[t].
+template <typename KV, bool TREE>
 __global__ void __launch_bounds__(256)
     kv_append_kernel(const PagedView w, const float* q, int64_t q_stride,
                      const float* __restrict__ k, int64_t k_stride, const float* __restrict__ v,
                      int64_t v_stride, float* q_out, int64_t qo_stride,  // may be q
-                     const float* __restrict__ rope, int rope_len, KV* kpool, KV* vpool) {
+                     const float* __restrict__ rope, int rope_len, const int32_t* __restrict__ depth,
+                     KV* kpool, KV* vpool) {
     const int t = blockIdx.x;
     const int b = seq_of_token(w, t);
     if (b < 0) return;
     const SeqInfo s = seq_info(w, b);
     const int pos = s.L - s.n + (t - s.q0);
     if (t < s.q0 || t >= s.q0 + s.n || pos < 0) return;  // no position: nothing to do
-    if (pos >= rope_len) {
+    int angle = pos;  // the position that q and k are rotated by
+    if constexpr (TREE) {
+        const int d = depth[t];
+        if (d < 0 || d > t - s.q0) {
+            if (threadIdx.x == 0) paged_fault(PAGED_BAD_TREE);
+            return;
+        }
+        angle = max(s.L - s.n + d, 0);
+    }
+    if (angle >= rope_len) {
         if (threadIdx.x == 0) paged_fault(PAGED_BAD_ROPE);
         return;
     }
@@ -577,7 +779,7 @@ __global__ void __launch_bounds__(256)
         const float4* p = reinterpret_cast<const float4*>(src + (int64_t)h * w.HD + d);
         float4 x[2] = {p[0], p[1]};
         if (!is_v) {
-            const float4* r = reinterpret_cast<const float4*>(rope + (int64_t)pos * w.HD + d);
+            const float4* r = reinterpret_cast<const float4*>(rope + (int64_t)angle * w.HD + d);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float4 c = __ldg(r + i), y = x[i];
@@ -609,7 +811,7 @@ static KvSeqsDev seqs_dev(const ib_kv_pages* p, const ib_kv_seqs* s) {
     return KvSeqsDev{s->table, s->len, s->refs, s->n_slots, s->max_pages, p->n_pages, p->page_size};
 }
 
-static PoolBytes pool_bytes(const ib_kv_pages* p) {
+PoolBytes pool_bytes(const ib_kv_pages* p) {
     PoolBytes b;
     b.k = (uint8_t*)p->k;
     b.v = (uint8_t*)p->v;
@@ -709,6 +911,65 @@ extern "C" int ib_kv_granted(int n, const int32_t* slots, const int32_t* status,
     return IB_OK;
 }
 
+// The workspace's arrays, each on a boundary of 256 bytes; its size.
+static size_t reorder_ws(const ib_kv_seqs* s, int n, void* at, ReorderWs* ws) {
+    uint8_t* const base = (uint8_t*)at;
+    size_t end = 0;
+    auto take = [&](size_t count) {
+        int32_t* const p = (int32_t*)(base + end);
+        end += (count * 4 + 255) / 256 * 256;
+        return p;
+    };
+    ws->row = take((size_t)n * s->max_pages);
+    ws->len = take(n);
+    ws->used = take(n);
+    ws->src = take(n);
+    ws->dst = take(n);
+    return end;
+}
+
+extern "C" size_t ib_kv_reorder_workspace(const ib_kv_seqs* seqs, int n) {
+    if (!seqs || n < 0 || n > IB_KV_MAX_SLOTS || seqs->max_pages < 1 || seqs->max_pages > (1 << 28)) {
+        paged_refuse("ib_kv_reorder_workspace", "no sequences, or a list length out of range");
+        return 0;
+    }
+    ReorderWs ws;
+    return std::max<size_t>(256, reorder_ws(seqs, n, nullptr, &ws));
+}
+
+extern "C" int ib_kv_reorder(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n,
+                             const int32_t* slots, const int32_t* parents, int32_t* status,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "ib_kv_reorder";
+    int r = paged_check(pages, seqs, who);
+    if (r != IB_OK || n == 0) return r;
+    if ((r = check_status(n, slots, parents, status, who)) != IB_OK) return r;
+    ReorderWs ws;
+    const size_t need = reorder_ws(seqs, n, workspace, &ws);
+    if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)
+        return paged_refuse(who, "workspace missing, too small or not 256-byte aligned");
+    const KvSeqsDev s = seqs_dev(pages, seqs);
+    cudaStream_t st = as_stream(stream);
+    kv_reorder_rows_kernel<<<n, KV_COPY_THREADS, 0, st>>>(s, n, slots, parents, ws);
+    IB_LAUNCH_CHECK("kv_reorder_rows_kernel");
+    constexpr size_t MOST = 2 * (size_t)IB_KV_MAX_SLOTS * 4;
+    static DeviceOnce once;
+    IB_CUDA_CHECK(once.run([] {
+        return cudaFuncSetAttribute(kv_reorder_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)MOST);
+    }));
+    IB_CUDA_CHECK(launch_pdl(kv_reorder_plan_kernel, dim3(1), dim3(KV_PLAN_THREADS),
+                             ((size_t)s.n_slots + n) * 4, st, true, s, n, slots, parents, ws, status));
+    int sms = 0;
+    if ((r = sm_count(&sms)) != IB_OK) return r;
+    const int64_t warps = (int64_t)n * pages->n_layers * 2 * pages->n_kv_heads;
+    const int grid = (int)std::min<int64_t>(
+        (int64_t)sms * 8, std::max<int64_t>(n, (warps + KV_COPY_THREADS / 32 - 1) / (KV_COPY_THREADS / 32)));
+    IB_CUDA_CHECK(launch_pdl(kv_reorder_kernel, dim3(grid), dim3(KV_COPY_THREADS), 0, st, true, s,
+                             pool_bytes(pages), n, slots, ws, (const int32_t*)status));
+    return IB_OK;
+}
+
 extern "C" int ib_kv_release(const ib_kv_pages* pages, const ib_kv_seqs* seqs, int n,
                              const int32_t* slots, void* stream) {
     int r = paged_check(pages, seqs, "ib_kv_release");
@@ -740,41 +1001,65 @@ extern "C" int ib_kv_compact(const ib_kv_pages* pages, const ib_kv_seqs* seqs, i
     return IB_OK;
 }
 
+static int kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                     const ib_kv_tree* tree, int layer, int n_heads, const float* q, int64_t q_stride,
+                     const float* k, int64_t k_stride, const float* v, int64_t v_stride, float* q_out,
+                     int64_t q_out_stride, const float* rope_table, int rope_len, void* stream,
+                     const char* who) {
+    if (batch->n_tokens == 0 || batch->n_seqs == 0) return IB_OK;
+    if (!(q && k && v && q_out && rope_table && rope_len >= 0))
+        return paged_refuse(who, "null pointer argument");
+    if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)rope_table) & 15) ||
+        ((q_stride | k_stride | v_stride | q_out_stride) & 3))
+        return paged_refuse(who, "q, k, v, q_out and the RoPE table must be 16-byte aligned, with row "
+                                 "strides that are multiples of 4");
+    const int64_t qw = (int64_t)n_heads * pages->head_dim;
+    if (!(q_stride >= 0 && k_stride >= 0 && v_stride >= 0 && q_out_stride >= qw))
+        return paged_refuse(who, "bad row strides");
+    const int64_t kw = (int64_t)pages->n_kv_heads * pages->head_dim, n = batch->n_tokens;
+    if (!((q_out == q && q_out_stride == q_stride) ||
+          !paged_rows_overlap(q_out, q_out_stride, qw, q, q_stride, qw, n)) ||
+        paged_rows_overlap(q_out, q_out_stride, qw, k, k_stride, kw, n) ||
+        paged_rows_overlap(q_out, q_out_stride, qw, v, v_stride, kw, n))
+        return paged_refuse(who, "q_out may be q, with its row stride, and must not overlap it otherwise, "
+                                 "nor k or v");
+    const PagedView w = paged_view(pages, seqs, batch, n_heads, tree);
+    const int64_t layer_elems = pool_bytes(pages).layer_bytes / elem_bytes(pages);
+    cudaStream_t st = as_stream(stream);
+    auto launch = [&](auto* kern, auto* kpool, auto* vpool) {
+        kern<<<batch->n_tokens, 256, 0, st>>>(w, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride,
+                                              rope_table, rope_len, tree ? tree->depth : nullptr,
+                                              kpool + layer * layer_elems, vpool + layer * layer_elems);
+    };
+    if (pages->type == IB_TYPE_F32)
+        launch(tree ? kv_append_kernel<float, true> : kv_append_kernel<float, false>, (float*)pages->k,
+               (float*)pages->v);
+    else
+        launch(tree ? kv_append_kernel<__half, true> : kv_append_kernel<__half, false>,
+               (__half*)pages->k, (__half*)pages->v);
+    IB_LAUNCH_CHECK("kv_append_kernel");
+    return IB_OK;
+}
+
 extern "C" int ib_kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
                             const ib_kv_batch* batch, int layer, int n_heads, const float* q,
                             int64_t q_stride, const float* k, int64_t k_stride, const float* v,
                             int64_t v_stride, float* q_out, int64_t q_out_stride,
                             const float* rope_table, int rope_len, void* stream) {
-    int r = paged_check_batch(pages, seqs, batch, layer, n_heads, "ib_kv_append");
-    if (r != IB_OK || batch->n_tokens == 0 || batch->n_seqs == 0) return r;
-    IB_REQUIRE(q && k && v && q_out && rope_table && rope_len >= 0,
-               "ib_kv_append: null pointer argument");
-    IB_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out |
-                 (uintptr_t)rope_table) & 15) == 0 &&
-                   ((q_stride | k_stride | v_stride | q_out_stride) & 3) == 0,
-               "ib_kv_append: q, k, v, q_out and the RoPE table must be 16-byte aligned, with row "
-               "strides that are multiples of 4");
-    const int64_t qw = (int64_t)n_heads * pages->head_dim;
-    IB_REQUIRE(q_stride >= 0 && k_stride >= 0 && v_stride >= 0 && q_out_stride >= qw,
-               "ib_kv_append: bad row strides");
-    const int64_t kw = (int64_t)pages->n_kv_heads * pages->head_dim, n = batch->n_tokens;
-    IB_REQUIRE(((q_out == q && q_out_stride == q_stride) ||
-                !paged_rows_overlap(q_out, q_out_stride, qw, q, q_stride, qw, n)) &&
-                   !paged_rows_overlap(q_out, q_out_stride, qw, k, k_stride, kw, n) &&
-                   !paged_rows_overlap(q_out, q_out_stride, qw, v, v_stride, kw, n),
-               "ib_kv_append: q_out may be q, with its row stride, and must not overlap it otherwise, "
-               "nor k or v");
-    const PagedView w = paged_view(pages, seqs, batch, n_heads);
-    const int64_t layer_elems = pool_bytes(pages).layer_bytes / elem_bytes(pages);
-    cudaStream_t st = as_stream(stream);
-    if (pages->type == IB_TYPE_F32)
-        kv_append_kernel<float><<<batch->n_tokens, 256, 0, st>>>(
-            w, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, rope_table, rope_len,
-            (float*)pages->k + layer * layer_elems, (float*)pages->v + layer * layer_elems);
-    else
-        kv_append_kernel<__half><<<batch->n_tokens, 256, 0, st>>>(
-            w, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, rope_table, rope_len,
-            (__half*)pages->k + layer * layer_elems, (__half*)pages->v + layer * layer_elems);
-    IB_LAUNCH_CHECK("kv_append_kernel");
-    return IB_OK;
+    const int r = paged_check_batch(pages, seqs, batch, layer, n_heads, "ib_kv_append");
+    if (r != IB_OK) return r;
+    return kv_append(pages, seqs, batch, nullptr, layer, n_heads, q, q_stride, k, k_stride, v, v_stride,
+                     q_out, q_out_stride, rope_table, rope_len, stream, "ib_kv_append");
+}
+
+extern "C" int ib_kv_append_tree(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                 const ib_kv_batch* batch, const ib_kv_tree* tree, int layer, int n_heads,
+                                 const float* q, int64_t q_stride, const float* k, int64_t k_stride,
+                                 const float* v, int64_t v_stride, float* q_out, int64_t q_out_stride,
+                                 const float* rope_table, int rope_len, void* stream) {
+    int r = paged_check_batch(pages, seqs, batch, layer, n_heads, "ib_kv_append_tree");
+    if (r == IB_OK) r = paged_check_tree(batch, tree, "ib_kv_append_tree");
+    if (r != IB_OK) return r;
+    return kv_append(pages, seqs, batch, tree, layer, n_heads, q, q_stride, k, k_stride, v, v_stride, q_out,
+                     q_out_stride, rope_table, rope_len, stream, "ib_kv_append_tree");
 }

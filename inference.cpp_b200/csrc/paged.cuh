@@ -21,7 +21,8 @@ enum {
     PAGED_BAD_REFS = 74,   // a reference count that a release would take below zero
     PAGED_BAD_ROPE = 75,   // a position behind the end of the RoPE table
     PAGED_BAD_WAIT = 76,   // a pipeline wait expired
-    PAGED_SHARED = 77      // a new token in a page that others hold too
+    PAGED_SHARED = 77,     // a new token in a page that others hold too
+    PAGED_BAD_TREE = 78    // a node, parent, depth or accepted path that cannot be
 };
 
 // Unsigned division by a number that the host prepares (page sizes need not be powers of
@@ -52,6 +53,7 @@ struct PagedView {
     const int32_t* slots;  // null: sequence b is slot b
     int n_slots, max_pages, n_pages;
     int n_seqs, n_tokens;
+    int max_nodes;  // of a sequence's tree; 0: the new tokens are no trees
     int H, Hkv, HD, page_size;
     FastDiv ps;     // of page_size
     FastDiv group;  // of H / Hkv
@@ -92,7 +94,25 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedView& w, int b) {
     s.L = min(max(L, 0), cap);
     if (s.L != L) paged_fault(PAGED_BAD_LEN);
     s.row = w.table + (size_t)slot * w.max_pages;
+    if (w.max_nodes && s.n > w.max_nodes) {  // a tree that the masks have no room for: left out
+        paged_fault(PAGED_BAD_TREE);
+        s.n = 0;
+    }
     return s;
+}
+
+// Nodes [q0, q0 + n) of sequence b's tree, from the batch alone (at most `most`, else recorded and
+// none); the same range as seq_info's.
+__device__ __forceinline__ int tree_nodes(const int32_t* cu_q, const int32_t* slots, int n_tokens, int b,
+                                          int most, int& q0) {
+    const int a = cu_q[b], e = cu_q[b + 1];
+    q0 = min(max(a, 0), n_tokens);
+    const int n = min(max(e, q0), n_tokens) - q0;
+    if (q0 != a || q0 + n != e) paged_fault(PAGED_BAD_LEN);
+    if (slots && slots[b] == -1) return 0;  // its rows are nobody's
+    if (n <= most) return n;
+    paged_fault(PAGED_BAD_TREE);
+    return 0;
 }
 
 // Page of table entry e, or -1 (nothing there; out of range is recorded too).
@@ -137,12 +157,24 @@ static inline int paged_fault_take_here(int* code) {
 int paged_check(const ib_kv_pages* p, const ib_kv_seqs* s, const char* who);
 int paged_check_batch(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int layer,
                       int n_heads, const char* who);
+int paged_check_tree(const ib_kv_batch* b, const ib_kv_tree* t, const char* who);
+int paged_refuse(const char* who, const char* what);  // sets the error, returns IB_ERR_INVALID
 // Whether any of n rows of wa floats, sa apart from a, shares a float with one of wb, sb apart from b
 // (rows of different strides: whether their whole ranges meet).
 bool paged_rows_overlap(const float* a, int64_t sa, int64_t wa, const float* b, int64_t sb, int64_t wb,
                         int64_t n);
-PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int n_heads);
+PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int n_heads,
+                     const ib_kv_tree* t = nullptr);
 int paged_fault_take(int* code);            // paged.cu
 int paged_attention_fault_take(int* code);  // paged_attention.cu
+int paged_tree_fault_take(int* code);       // paged_tree.cu
+
+// The pool as bytes: layer l, page p at l * layer_bytes + p * page_bytes.
+struct PoolBytes {
+    uint8_t *k, *v;
+    int n_layers, n_kv_heads, row_bytes;  // row: head_dim elements
+    int64_t page_bytes, layer_bytes;
+};
+PoolBytes pool_bytes(const ib_kv_pages* p);
 
 }  // namespace ib

@@ -83,7 +83,7 @@ __device__ __forceinline__ float stage_q_row(const float* row, int HD, uint8_t* 
 
 // LD: bytes between K or V rows in shared memory (16 more than a row: the 8 rows of an ldmatrix,
 // and the TF32 V columns, hit distinct banks); QLD: the same for q.
-template <typename KV, int HDP, int KW>
+template <typename KV, int HDP, int KW, bool TREE>
 struct WarpRows {
     static constexpr bool F32 = sizeof(KV) == 4;
     static constexpr int LD = HDP * (int)sizeof(KV) + 16, QLD = HDP * (F32 ? 4 : 2) + 16;
@@ -96,6 +96,18 @@ struct WarpRows {
     int lim[2];     // last positions that rows g and g + 8 see
     float sc[2];
     uint32_t q_hi, q_lo;  // this lane's fragment addresses
+    [[maybe_unused]] const uint32_t* nodes[2];  // trees: the rows' masks
+    [[maybe_unused]] int first_node, words;     // position of bit 0
+
+    // whether row h sees position p
+    __device__ __forceinline__ bool sees(int h, int p) const {
+        if (p > lim[h]) return false;
+        if constexpr (TREE) {
+            const int c = p - first_node;
+            return c < 0 || (c < 32 * words && ((__ldg(nodes[h] + (c >> 5)) >> (c & 31)) & 1));
+        }
+        return true;
+    }
 
     __device__ __forceinline__ void start(uint32_t hi, uint32_t lo) {
         const int lane = threadIdx.x & 31;
@@ -175,8 +187,8 @@ struct WarpRows {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float &a = s[n][2 * h], &b = s[n][2 * h + 1];
-                a = p0 <= lim[h] ? (a + e[n][2 * h]) * sc[h] : -INFINITY;
-                b = p1 <= lim[h] ? (b + e[n][2 * h + 1]) * sc[h] : -INFINITY;
+                a = sees(h, p0) ? (a + e[n][2 * h]) * sc[h] : -INFINITY;
+                b = sees(h, p1) ? (b + e[n][2 * h + 1]) * sc[h] : -INFINITY;
                 x[h] = fmaxf(x[h], fmaxf(a, b));
             }
         }
@@ -280,8 +292,8 @@ struct WarpRows {
                         if constexpr (F32) y = reinterpret_cast<const float*>(vr)[at];
                         else y = __half2float(reinterpret_cast<const __half*>(vr)[at]);
                         if (fabsf(y) < INFINITY) continue;
-                        if (pos <= lim[0]) acc[d][i] = NAN;
-                        if (pos <= lim[1]) acc[d][2 + i] = NAN;
+                        if (sees(0, pos)) acc[d][i] = NAN;
+                        if (sees(1, pos)) acc[d][2 + i] = NAN;
                     }
             }
         }
@@ -342,7 +354,7 @@ struct NarrowCfg {
     static_assert(QREG || F32, "");
 };
 
-template <typename KV, int HDP>
+template <typename KV, int HDP, bool TREE>
 __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CTAS)
     attn_narrow_kernel(const __grid_constant__ RowsArgs A) {
     using C = NarrowCfg<KV, HDP>;
@@ -366,7 +378,8 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
     it.rows = min(R, it.s.n * G - it.row0);
     it.start = it.s.L - it.s.n;
     it.part = item.n_parts == 1 ? -1 : item.part_base + item.part;
-    const int first_lim = it.start + it.row0 / G, last_lim = it.start + (it.row0 + it.rows - 1) / G;
+    const int first_lim = all_see<TREE>(it.start, it.row0, G);
+    const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
     // this warp's tiles: kt0, kt0 + NW ..
     const int kt0 = item.kt0 + warp, kt1 = min(item.kt1, last_lim < 0 ? 0 : last_lim / KW + 1);
     uint8_t* ring = smem + warp * (C::Q_BYTES + D * C::HALF);
@@ -430,6 +443,7 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
     const uint32_t v_frag = (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * LD + ((lane >> 3) & 1) * 16);
     // this lane's rows are 2 t4 and 2 t4 + 1
     int lim[2];
+    [[maybe_unused]] const uint32_t* nodes[2];
     float sc[2], m[2], l[2], acc[DB][4];
     uint32_t qh[C::QREG ? KS : 1][2], ql[C::QREG ? KS : 1][2];
     // q as B: row g; FP16 k-steps of dimensions 2 t4, + 1, + 8, + 9, TF32 t4, + 4
@@ -479,6 +493,7 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
     for (int j = 0; j < 2; ++j) {
         const int mine = 2 * t4 + j;
         lim[j] = mine < it.rows ? it.start + (it.row0 + mine) / G : -1;
+        if constexpr (TREE) nodes[j] = mask_row(A, it.s.q0, it.row0 + mine, mine < it.rows);
         sc[j] = __shfl_sync(0xffffffffu, f, (2 * t4 + j) * 4);
         m[j] = -INFINITY;
         l[j] = 0.f;
@@ -537,12 +552,18 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
         const uint32_t missing = gone[0];
         const int p0 = (missing >> g) & 1 ? 0x7fffffff : kt * KW + g;
         const int p1 = (missing >> (g + 8)) & 1 ? 0x7fffffff : kt * KW + g + 8;
+        const bool careful = kt * KW + KW - 1 > first_lim;
+        [[maybe_unused]] uint32_t sees[2] = {0xffffffffu, 0xffffffffu};  // of the tile's positions
+        if constexpr (TREE)
+            if (careful)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) sees[j] = tree_bits(nodes[j], A.words, kt * KW - it.start);
         float c[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             float &x = s[j], &y = s[2 + j];
-            x = p0 <= lim[j] ? x * sc[j] : -INFINITY;
-            y = p1 <= lim[j] ? y * sc[j] : -INFINITY;
+            x = p0 <= lim[j] && (!TREE || ((sees[j] >> g) & 1)) ? x * sc[j] : -INFINITY;
+            y = p1 <= lim[j] && (!TREE || ((sees[j] >> (g + 8)) & 1)) ? y * sc[j] : -INFINITY;
             float top = fmaxf(x, y);
 #pragma unroll
             for (int o = 4; o <= 16; o <<= 1)
@@ -582,7 +603,6 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
         const uint32_t vd = ring_a + (uint32_t)(slot * C::HALF);
         const uint8_t* v_ptr = ring + slot * C::HALF;
         slot = slot == D - 1 ? 0 : slot + 1;
-        const bool careful = kt * KW + KW - 1 > first_lim;
         bool odd = false;  // a V value that is not finite, among this lane's
         // outputs: rows of a fragment are dimensions g and g + 8 of a block of 16
         auto products = [&](auto check) {
@@ -647,7 +667,8 @@ __global__ void __launch_bounds__(NarrowCfg<KV, HDP>::NT, NarrowCfg<KV, HDP>::CT
                     if constexpr (F32) y = reinterpret_cast<const float*>(v_ptr)[at];
                     else y = __half2float(reinterpret_cast<const __half*>(v_ptr)[at]);
                     if (fabsf(y) < INFINITY) continue;
-                    if (kt * KW + i <= lim[j & 1]) acc[d][j] = NAN;
+                    if (kt * KW + i <= lim[j & 1] && (!TREE || ((sees[j & 1] >> i) & 1)))
+                        acc[d][j] = NAN;
                 }
             }
         }
@@ -712,19 +733,20 @@ struct WideCfg {
     static constexpr int WR = 4, NT = WR * 32, R = 16 * WR;
     static constexpr int ROWB = HDP * (int)sizeof(KV);
     static constexpr int KT = F32 ? 16 : 32;
-    using Tile = WarpRows<KV, HDP, KT>;
+    template <bool TREE>
+    using Tile = WarpRows<KV, HDP, KT, TREE>;
     static constexpr int STAGES = 2;
-    static constexpr int Q_BYTES = 2 * R * Tile::QLD;
-    static constexpr int STAGE = 2 * KT * Tile::LD;
+    static constexpr int Q_BYTES = 2 * R * Tile<false>::QLD;
+    static constexpr int STAGE = 2 * KT * Tile<false>::LD;
     static constexpr int RING = STAGES + 1;  // of row offsets: a tile's outlive its copies
     static constexpr size_t SMEM = (size_t)Q_BYTES + STAGES * STAGE;
 };
 
-template <typename KV, int HDP>
+template <typename KV, int HDP, bool TREE>
 __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     attn_wide_kernel(const __grid_constant__ RowsArgs A) {
     using C = WideCfg<KV, HDP>;
-    using T = typename C::Tile;
+    using T = typename C::template Tile<TREE>;
     constexpr int NT = C::NT, R = C::R, KT = C::KT, LD = T::LD, S = C::STAGES;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long row_off[C::RING][KT];  // where a position's row starts, -1: nowhere
@@ -747,7 +769,7 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     const int G = w.H / w.Hkv, HD = w.HD;
     while (next_segment(w, A.rule, piece, it)) {
     const int row0 = it.row0, rows = it.rows, start = it.start;
-    const int first_lim = start + row0 / G, last_lim = start + (row0 + rows - 1) / G;
+    const int first_lim = all_see<TREE>(start, row0, G), last_lim = start + (row0 + rows - 1) / G;
     const int kt0 = it.kt0, kt1 = it.kt1;
     const int n_kt = max(0, kt1 - kt0);
     const uint32_t q_base = smem_u32(smem), kv_base = q_base + C::Q_BYTES;
@@ -803,6 +825,10 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
         const int r = warp * 16 + g + 8 * h;
         t.lim[h] = r < rows ? start + (row0 + r) / G : -1;
         t.sc[h] = row_scale[r];
+        if constexpr (TREE) {
+            t.nodes[h] = mask_row(A, it.s.q0, row0 + r, r < rows);
+            t.first_node = start, t.words = A.words;
+        }
     }
     for (int i = 0; i < n_kt; ++i) {
         if (i + S - 1 < n_kt) put_offsets(i + S - 1, next_page);
@@ -1101,7 +1127,7 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     return plan;
 }
 
-template <typename KV, int HDP>
+template <typename KV, int HDP, bool TREE>
 static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan, RowsArgs a,
                     uint8_t* ws, int64_t max_pos, cudaStream_t st) {
     using N = NarrowCfg<KV, HDP>;
@@ -1114,12 +1140,12 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         a.part_ml = reinterpret_cast<float2*>(ws + s.ml_off);
         int r = IB_OK;
         if (!wide) {
-            r = rows_launch<attn_narrow_kernel<KV, HDP>>(N::NT, N::SMEM, false, a, s.tiles, max_pos, st);
+            r = rows_launch<attn_narrow_kernel<KV, HDP, TREE>>(N::NT, N::SMEM, false, a, s.tiles, max_pos, st);
         } else if constexpr (on_tcgen05<HDP>) {
-            r = attn_tensor_launch<KV>(a, s.tiles, max_pos, st);
+            r = attn_tensor_launch<KV, TREE>(a, s.tiles, max_pos, st);
         } else {
             using W = WideCfg<KV, HDP>;
-            r = rows_launch<attn_wide_kernel<KV, HDP>>(W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
+            r = rows_launch<attn_wide_kernel<KV, HDP, TREE>>(W::NT, W::SMEM, true, a, s.tiles, max_pos, st);
         }
         if (r != IB_OK) return r;
     }
@@ -1164,7 +1190,8 @@ static int attention_paged(const ib_kv_pages* p, const ib_kv_batch* b, RowsArgs 
             *bytes = plan.bytes;
             return (int)IB_OK;
         }
-        return run_plan<KV, HDP>(p, b, plan, a, (uint8_t*)ws, max_pos, st);
+        return a.mask ? run_plan<KV, HDP, true>(p, b, plan, a, (uint8_t*)ws, max_pos, st)
+                      : run_plan<KV, HDP, false>(p, b, plan, a, (uint8_t*)ws, max_pos, st);
     };
     if (p->head_dim <= 64) return go(std::integral_constant<int, 64>{});
     if (p->head_dim <= 128) return go(std::integral_constant<int, 128>{});
@@ -1181,41 +1208,60 @@ static int attention_paged_any(const ib_kv_pages* p, const ib_kv_batch* b, const
 
 using namespace ib;
 
-extern "C" size_t ib_attention_paged_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
-                                               const ib_kv_batch* batch, int n_heads) {
-    if (paged_check_batch(pages, seqs, batch, 0, n_heads, "ib_attention_paged_workspace") != IB_OK)
-        return 0;
+static size_t attention_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                  const ib_kv_batch* batch, const ib_kv_tree* tree, int n_heads) {
     if (batch->n_tokens == 0 || batch->n_seqs == 0) return 256;
     RowsArgs a{};
-    a.w = paged_view(pages, seqs, batch, n_heads);
+    a.w = paged_view(pages, seqs, batch, n_heads, tree);
+    if (tree) a.mask = tree->mask;
     size_t n = 0;
     attention_paged_any(pages, batch, a, nullptr, &n, 0, nullptr);
     return n;
 }
 
-extern "C" int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
-                                  const ib_kv_batch* batch, int layer, int n_heads, const float* q,
-                                  int64_t q_stride, float* out, int64_t out_stride, float scale,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
-    int r = paged_check_batch(pages, seqs, batch, layer, n_heads, "ib_attention_paged");
-    if (r != IB_OK || batch->n_tokens == 0 || batch->n_seqs == 0) return r;
-    IB_REQUIRE(q && out, "ib_attention_paged: null pointer argument");
-    IB_REQUIRE((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && ((q_stride | out_stride) & 3) == 0,
-               "ib_attention_paged: q and out must be 16-byte aligned, with row strides that are "
-               "multiples of 4");
-    IB_REQUIRE(q_stride >= 0 && out_stride >= (int64_t)n_heads * pages->head_dim,
-               "ib_attention_paged: bad row strides");
+extern "C" size_t ib_attention_paged_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                               const ib_kv_batch* batch, int n_heads) {
+    if (paged_check_batch(pages, seqs, batch, 0, n_heads, "ib_attention_paged_workspace") != IB_OK)
+        return 0;
+    return attention_workspace(pages, seqs, batch, nullptr, n_heads);
+}
+
+extern "C" size_t ib_attention_paged_tree_workspace(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                                    const ib_kv_batch* batch, const ib_kv_tree* tree,
+                                                    int n_heads) {
+    const char* who = "ib_attention_paged_tree_workspace";
+    if (paged_check_batch(pages, seqs, batch, 0, n_heads, who) != IB_OK ||
+        paged_check_tree(batch, tree, who) != IB_OK)
+        return 0;
+    return attention_workspace(pages, seqs, batch, tree, n_heads);
+}
+
+// The structs are checked.
+static int attention_call(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                          const ib_kv_tree* tree, int layer, int n_heads, const float* q, int64_t q_stride,
+                          float* out, int64_t out_stride, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream, const char* who) {
+    if (batch->n_tokens == 0 || batch->n_seqs == 0) return IB_OK;
+    if (!(q && out)) return paged_refuse(who, "null pointer argument");
+    if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_stride | out_stride) & 3))
+        return paged_refuse(who, "q and out must be 16-byte aligned, with row strides that are "
+                                 "multiples of 4");
+    if (!(q_stride >= 0 && out_stride >= (int64_t)n_heads * pages->head_dim))
+        return paged_refuse(who, "bad row strides");
     const int64_t row = (int64_t)n_heads * pages->head_dim;
-    IB_REQUIRE((out == q && out_stride == q_stride) ||
-                   !paged_rows_overlap(out, out_stride, row, q, q_stride, row, batch->n_tokens),
-               "ib_attention_paged: out may be q, with its row stride, and must not overlap it "
-               "otherwise");
+    if (!((out == q && out_stride == q_stride) ||
+          !paged_rows_overlap(out, out_stride, row, q, q_stride, row, batch->n_tokens)))
+        return paged_refuse(who, "out may be q, with its row stride, and must not overlap it otherwise");
     RowsArgs a{};
-    a.w = paged_view(pages, seqs, batch, n_heads);
+    a.w = paged_view(pages, seqs, batch, n_heads, tree);
+    if (tree) {
+        a.mask = tree->mask;
+        a.words = (tree->max_nodes + 31) / 32;
+    }
     size_t need = 0;
     attention_paged_any(pages, batch, a, nullptr, &need, 0, nullptr);
-    IB_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need,
-               "ib_attention_paged: workspace missing, too small or not 256-byte aligned");
+    if (!(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need))
+        return paged_refuse(who, "workspace missing, too small or not 256-byte aligned");
     const int64_t layer_bytes = (int64_t)pages->n_pages * pages->n_kv_heads * pages->page_size *
                                 pages->head_dim * (pages->type == IB_TYPE_F32 ? 4 : 2);
     a.q = q;
@@ -1227,4 +1273,28 @@ extern "C" int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* se
     a.scale_log2 = scale * 1.4426950408889634f;
     return attention_paged_any(pages, batch, a, workspace, nullptr,
                                (int64_t)seqs->max_pages * pages->page_size, as_stream(stream));
+}
+
+extern "C" int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                  const ib_kv_batch* batch, int layer, int n_heads, const float* q,
+                                  int64_t q_stride, float* out, int64_t out_stride, float scale,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "ib_attention_paged";
+    const int r = paged_check_batch(pages, seqs, batch, layer, n_heads, who);
+    if (r != IB_OK) return r;
+    return attention_call(pages, seqs, batch, nullptr, layer, n_heads, q, q_stride, out, out_stride, scale,
+                          workspace, workspace_bytes, stream, who);
+}
+
+extern "C" int ib_attention_paged_tree(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                       const ib_kv_batch* batch, const ib_kv_tree* tree, int layer,
+                                       int n_heads, const float* q, int64_t q_stride, float* out,
+                                       int64_t out_stride, float scale, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    const char* who = "ib_attention_paged_tree";
+    int r = paged_check_batch(pages, seqs, batch, layer, n_heads, who);
+    if (r == IB_OK) r = paged_check_tree(batch, tree, who);
+    if (r != IB_OK) return r;
+    return attention_call(pages, seqs, batch, tree, layer, n_heads, q, q_stride, out, out_stride, scale,
+                          workspace, workspace_bytes, stream, who);
 }

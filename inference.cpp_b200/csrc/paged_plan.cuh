@@ -311,12 +311,35 @@ struct RowsArgs {
     float* part_acc;    // [partial][R][HD] of parts, [partial][HD / 4][R][4] of pieces
     float2* part_ml;    // [partial][R]
     float scale_log2;   // scale * log2(e)
+    const uint32_t* mask;  // trees: [token][words], see ib_kv_tree
+    int words;
     // The kernel before is the call's narrow one, which writes other rows and workspace: this one
     // starts beside its last CTAs and waits for it at its own end only, so that what follows
     // finds both complete.  (The narrow kernel lets it start after its own wait for what came
     // before the call.)
     bool beside;
 };
+
+// ---- what a node of a tree sees ------------------------------------------------------------
+// Row of the masks of the segment's row gr (of row 0 where the segment has none).
+__device__ __forceinline__ const uint32_t* mask_row(const RowsArgs& A, int q0, int gr, bool there) {
+    return A.mask + (int64_t)(q0 + (there ? (int)A.w.group.div((uint32_t)gr) : 0)) * A.words;
+}
+
+// Bits first .. first + 31 of a mask row, where negative ones are the context: all there.
+__device__ __forceinline__ uint32_t tree_bits(const uint32_t* row, int words, int first) {
+    if (first <= -32) return 0xffffffffu;
+    const int at = first >> 5;
+    auto word = [&](int i) { return i < 0 ? 0xffffffffu : i < words ? __ldg(row + i) : 0u; };
+    return __funnelshift_r(word(at), word(at + 1), first & 31);
+}
+
+// The last position that every row of a tile sees if it has a page, from its first row: a causal row
+// sees all before its own, a node of a tree all of the context.  Behind it tiles are masked.
+template <bool TREE>
+__device__ __forceinline__ int all_see(int start, int first_row, int G) {
+    return TREE ? start - 1 : start + first_row / G;
+}
 
 // Row `gr` of the segment's sequence and kv head.
 __device__ __forceinline__ float* out_row(const RowsArgs& A, const Segment& it, int G, int gr) {
@@ -367,7 +390,7 @@ __device__ __forceinline__ float pow2_scale(float top, float& inverse) {
 // Tiles of many rows on tcgen05, for head_dim up to 128 (paged_tensor.cu).
 template <typename KV>
 CutRule tensor_rule(int head_dim, int min_rows, int max_rows);
-template <typename KV>
+template <typename KV, bool TREE>
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st);
 int paged_tensor_fault_take(int* code);
 

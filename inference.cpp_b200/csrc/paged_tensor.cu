@@ -273,7 +273,7 @@ struct TensorBars {
     uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], seg_done[2], v_there[3], done;
 };
 
-template <typename KV, int HDP>
+template <typename KV, int HDP, bool TREE>
 __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
     attn_tensor_kernel(const __grid_constant__ TensorArgs TA) {
     const RowsArgs& A = TA.rows;
@@ -449,7 +449,9 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             const int r = wr + lane;
             const int row = cur.row0 + 128 * t + r;  // of the sequence
             const int lim = r < rows ? cur.start + (int)w.group.div((uint32_t)row) : -1;
-            const int first_lim = cur.start + (cur.row0 + 128 * t) / G;  // of the tile's first row
+            const int first_lim = all_see<TREE>(cur.start, cur.row0 + 128 * t, G);
+            [[maybe_unused]] const uint32_t* nodes = nullptr;
+            if constexpr (TREE) nodes = mask_row(A, cur.s.q0, row, r < rows);
             float acc[HDP];
 #pragma unroll
             for (int d = 0; d < HDP; ++d) acc[d] = 0.f;
@@ -457,7 +459,9 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             // positions of key tile j (of the segment) that this row sees and that have a page
             auto visible = [&](int j, int word) -> uint32_t {
                 const int n = lim + 1 - ((cur.kt0 + j) * KT + 32 * word);
-                const uint32_t below = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+                uint32_t below = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+                if constexpr (TREE)
+                    below &= tree_bits(nodes, A.words, (cur.kt0 + j) * KT + 32 * word - cur.start);
                 const uint16_t* gone = sh_gone[(first + j) & 3];
                 return below & ~((uint32_t)gone[2 * word] | ((uint32_t)gone[2 * word + 1] << 16));
             };
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         fma2(a[0], a[1], a[0], a[1], c_last, c_last, o[d], o[d + 1]);
                     }
                 }
-                if ((cur.kt0 + j) * KT + KT - 1 > cur.start + cur.row0 / G) {
+                if ((cur.kt0 + j) * KT + KT - 1 > all_see<TREE>(cur.start, cur.row0, G)) {
                     // where some row does not see all of the tile, V was made finite: rows that
                     // see such a position are not
                     const uint16_t* bad16 = sh_bad[(first + j) & 3];
@@ -734,7 +738,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             bool ok = true;
             while (ok && next()) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
-                const int first_lim = it.start + it.row0 / G;
+                const int first_lim = all_see<TREE>(it.start, it.row0, G);
                 if (lw == 1) {  // the softmax warps ask for the segment's q soon
                     const int bytes = HD * 4;
                     for (int r = lane; r < it.rows; r += 32) {
@@ -920,7 +924,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             uint32_t tile_no = 0;
             bool ok = true;
             while (ok && next()) {
-                const int first_lim = it.start + it.row0 / G;
+                const int first_lim = all_see<TREE>(it.start, it.row0, G);
                 for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
                     const bool careful = kt * KT + KT - 1 > first_lim;
 #pragma unroll 1
@@ -1046,10 +1050,10 @@ CutRule tensor_rule(int head_dim, int min_rows, int max_rows) {
 template CutRule tensor_rule<float>(int, int, int);
 template CutRule tensor_rule<__half>(int, int, int);
 
-template <typename KV, int HDP>
+template <typename KV, int HDP, bool TREE>
 static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
     using C = TensorCfg<KV, HDP>;
-    auto kern = attn_tensor_kernel<KV, HDP>;
+    auto kern = attn_tensor_kernel<KV, HDP, TREE>;
     TensorArgs t{};
     t.rows = a;
     const PagedView& w = a.w;
@@ -1071,14 +1075,16 @@ static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
     return IB_OK;
 }
 
-template <typename KV>
+template <typename KV, bool TREE>
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st) {
     const int64_t most = tiles * (max_pos / a.rule.least + 1 + a.rule.R);
     const int64_t grid = std::min<int64_t>(a.rule.n_pieces, most);
-    return a.w.HD <= 64 ? launch<KV, 64>(a, grid, st) : launch<KV, 128>(a, grid, st);
+    return a.w.HD <= 64 ? launch<KV, 64, TREE>(a, grid, st) : launch<KV, 128, TREE>(a, grid, st);
 }
-template int attn_tensor_launch<float>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
-template int attn_tensor_launch<__half>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
+template int attn_tensor_launch<float, false>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
+template int attn_tensor_launch<__half, false>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
+template int attn_tensor_launch<float, true>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
+template int attn_tensor_launch<__half, true>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
 
 }  // namespace ib
 

@@ -1,0 +1,267 @@
+// Trees of drafted tokens over the paged cache: what the tree's shape means for attention and RoPE
+// (ib_kv_tree_plan), which path through it the model confirms (ib_kv_tree_verify), and the cache with
+// that path alone (ib_kv_tree_accept).  No counterpart in the reference, which decodes one token at a
+// time (src/models/model_cuda.cpp:372-407).
+//
+// A sequence's n new tokens are nodes 0 .. n - 1; node i is stored at position L - n + i and stands
+// at L - n + depth(i) of the text, behind its ancestors: depth(i) = number of ancestors in the tree.
+#include <cooperative_groups.h>
+
+#include <string>
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "pdl.cuh"
+
+namespace ib {
+
+int paged_tree_fault_take(int* code) { return paged_fault_take_here(code); }
+
+constexpr int TREE_THREADS = 128;
+
+// ---- plan --------------------------------------------------------------------------------
+// One CTA per sequence, a thread per node that goes up to the root: parents come before their
+// children, so a row's words are met from the last to the first.  A chain of reads of shared memory,
+// as long as the tree is deep; what bounds a step's one call is its launch.
+__global__ void __launch_bounds__(TREE_THREADS)
+    tree_plan_kernel(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ slots, int n_tokens,
+                     const int32_t* __restrict__ parents, int max_nodes, int32_t* __restrict__ depth,
+                     uint32_t* __restrict__ mask) {
+    __shared__ int16_t up[IB_KV_MAX_NODES];
+    int q0;
+    const int n = tree_nodes(cu_q, slots, n_tokens, blockIdx.x, max_nodes, q0);
+    for (int i = threadIdx.x; i < n; i += TREE_THREADS) {
+        int p = parents[q0 + i];
+        if (p < -1 || p >= i) {
+            paged_fault(PAGED_BAD_TREE);
+            p = -1;
+        }
+        up[i] = (int16_t)p;
+    }
+    __syncthreads();
+    const int words = (max_nodes + 31) / 32;
+    for (int i = threadIdx.x; i < n; i += TREE_THREADS) {
+        uint32_t* const row = mask + (size_t)(q0 + i) * words;
+        int w = words - 1, d = 0;
+        uint32_t bits = 0;
+        for (int c = i; c >= 0; c = up[c], ++d) {
+            for (; w > c >> 5; --w, bits = 0) row[w] = bits;
+            bits |= 1u << (c & 31);
+        }
+        for (; w >= 0; --w, bits = 0) row[w] = bits;
+        depth[q0 + i] = d - 1;
+    }
+}
+
+// ---- verify ------------------------------------------------------------------------------
+// Node 0 holds a token that is certain; from a confirmed node the path goes on to its first child
+// whose token is what the model chose behind the node.  One warp per sequence over the nodes in order
+// (a child comes after its parent, so the search only moves on): n / 32 steps and one for each node
+// of the path.
+__global__ void __launch_bounds__(32)
+    tree_verify_kernel(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ slots, int n_tokens,
+                       const int32_t* __restrict__ parents, const int32_t* __restrict__ tokens,
+                       const int32_t* __restrict__ best, int32_t* __restrict__ path,
+                       int32_t* __restrict__ n_path, int32_t* __restrict__ next) {
+    const int lane = threadIdx.x;
+    int q0;
+    const int n = tree_nodes(cu_q, slots, n_tokens, blockIdx.x, IB_KV_MAX_NODES, q0);
+    int at = n > 0 ? 0 : -1, m = 0, want = 0;
+    pdl_launch_dependents();
+    if (at == 0) {
+        want = best[q0];
+        if (lane == 0) path[q0] = 0;
+        m = 1;
+    }
+    for (int c0 = 1; c0 < n; c0 += 32) {
+        const int c = c0 + lane;
+        const int p = c < n ? parents[q0 + c] : -2, t = c < n ? tokens[q0 + c] : 0;
+        const int b = c < n ? best[q0 + c] : 0;
+        for (;;) {
+            const unsigned hit = __ballot_sync(0xffffffffu, c > at && p == at && t == want);
+            if (!hit) break;
+            const int j = __ffs(hit) - 1;
+            at = c0 + j;
+            want = __shfl_sync(0xffffffffu, b, j);
+            if (lane == 0) path[q0 + m] = at;
+            ++m;
+        }
+    }
+    for (int i = m + lane; i < n; i += 32) path[q0 + i] = -1;
+    if (lane == 0) {
+        n_path[blockIdx.x] = m;
+        next[blockIdx.x] = m ? want : -1;
+    }
+}
+
+// ---- accept ------------------------------------------------------------------------------
+// A cluster of CTAs per sequence.  A path's nodes are in order, so entry j of it comes from a row at
+// or behind its own place and rows can be moved in that order; a thread has 16 bytes of a row of one
+// (layer, K or V, head) and takes them through all moves, a few loads in flight at a time, without
+// waiting for others.  Once every CTA of the cluster is through, the first one gives back the pages
+// behind the new end.
+constexpr int ACCEPT_THREADS = 512, ACCEPT_CLUSTER = 8, ACCEPT_BATCH = 4;
+
+__global__ void __cluster_dims__(ACCEPT_CLUSTER) __launch_bounds__(ACCEPT_THREADS)
+    tree_accept_kernel(const PagedView w, int32_t* table, int32_t* len, int32_t* refs, const PoolBytes pool,
+                       const int32_t* __restrict__ path, const int32_t* __restrict__ n_path) {
+    __shared__ int from[IB_KV_MAX_NODES], to[IB_KV_MAX_NODES];  // rows of head 0 in a layer, -1: no move
+    __shared__ int bad, first;
+    const int b = blockIdx.x / ACCEPT_CLUSTER, part = blockIdx.x % ACCEPT_CLUSTER;
+    const int tid = threadIdx.x;
+    if (tid == 0) bad = first = IB_KV_MAX_NODES;
+    pdl_wait();
+    const SeqInfo s = seq_info(w, b);
+    const int slot = w.slots ? w.slots[b] : b;
+    const int start = s.L - s.n;
+    int m = n_path[b];
+    // nothing to do: left out of the step, no new tokens, or a slot that is none
+    const bool idle = s.n == 0 || slot < 0 || slot >= w.n_slots;
+    if (idle || m < 0 || m > s.n || start < 0) {
+        if (!idle && part == 0 && tid == 0) paged_fault(start < 0 ? PAGED_BAD_LEN : PAGED_BAD_TREE);
+        m = -1;
+    }
+    __syncthreads();
+    for (int j = tid; j < m; j += ACCEPT_THREADS) {
+        const int c = path[s.q0 + j], before = j ? path[s.q0 + j - 1] : -1;
+        if (c <= before || c >= s.n) {
+            atomicMin(&bad, j);
+            continue;
+        }
+        if (c != j) atomicMin(&first, j);
+        auto row = [&](int pos, bool written) -> int {
+            const int col = (int)w.ps.div((uint32_t)pos);
+            const int page = page_at(w, s.row[col]);
+            if (page >= 0 && written && w.refs[page] > 1) {
+                paged_fault(PAGED_SHARED);  // others hold it too: not written
+                return -1;
+            }
+            return page < 0 ? -1 : page * w.Hkv * w.page_size + (pos - col * w.page_size);
+        };
+        const int a = c == j ? -1 : row(start + c, false);
+        const int z = c == j ? -1 : row(start + j, true);
+        from[j] = z < 0 ? -1 : a;
+        to[j] = z;
+    }
+    __syncthreads();
+    if (m > bad) {  // the path ends before an entry that is none of it
+        if (part == 0 && tid == 0) paged_fault(PAGED_BAD_TREE);
+        m = bad;
+    }
+    const int per_row = pool.row_bytes / 16;
+    const int per_layer = 2 * w.Hkv * per_row;
+    const int64_t items = first < m ? (int64_t)pool.n_layers * per_layer : 0;
+    for (int64_t i = (int64_t)part * ACCEPT_THREADS + tid; i < items; i += ACCEPT_CLUSTER * ACCEPT_THREADS) {
+        const int layer = (int)(i / per_layer);
+        int r = (int)(i - (int64_t)layer * per_layer);
+        const int x = r % per_row;
+        r /= per_row;
+        const int head = r % w.Hkv;
+        uint8_t* const base = (r >= w.Hkv ? pool.v : pool.k) + layer * pool.layer_bytes +
+                              (int64_t)head * w.page_size * pool.row_bytes + x * 16;
+        for (int j0 = first; j0 < m; j0 += ACCEPT_BATCH) {
+            uint4 y[ACCEPT_BATCH];
+#pragma unroll
+            for (int k = 0; k < ACCEPT_BATCH; ++k)
+                if (j0 + k < m && from[j0 + k] >= 0)
+                    y[k] = *reinterpret_cast<const uint4*>(base + (int64_t)from[j0 + k] * pool.row_bytes);
+#pragma unroll
+            for (int k = 0; k < ACCEPT_BATCH; ++k)
+                if (j0 + k < m && from[j0 + k] >= 0)
+                    *reinterpret_cast<uint4*>(base + (int64_t)to[j0 + k] * pool.row_bytes) = y[k];
+        }
+    }
+    // every CTA has read the length and the table
+    cooperative_groups::this_cluster().sync();
+    if (part || m < 0) return;
+    const int now = start + m;
+    const int keep = (now + w.page_size - 1) / w.page_size, used = (s.L + w.page_size - 1) / w.page_size;
+    int32_t* const row = table + (size_t)slot * w.max_pages;
+    for (int j = keep + tid; j < used; j += ACCEPT_THREADS) {
+        const int t = row[j];
+        row[j] = -1;
+        if (t >= 0 && t < w.n_pages) {
+            if (atomicSub(&refs[t], 1) <= 0) {  // held by nobody: leave it free
+                atomicAdd(&refs[t], 1);
+                paged_fault(PAGED_BAD_REFS);
+            }
+        } else if (t != -1) {
+            paged_fault(PAGED_BAD_PAGE);
+        }
+    }
+    if (tid == 0) len[slot] = now;
+}
+
+static int tree_batch(const ib_kv_batch* b, const char* who) {
+    if (!b || !b->cu_q) return paged_refuse(who, "null pointer argument");
+    if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_q < 0 || b->n_seqs > IB_KV_MAX_SLOTS ||
+        b->n_tokens > (1 << 26))
+        return paged_refuse(who, "bad batch sizes");
+    return IB_OK;
+}
+
+// Whether [a, a + na) and [b, b + nb) of 32-bit values share any.
+static bool meet(const void* a, int64_t na, const void* b, int64_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + 4 * nb && (uintptr_t)b < (uintptr_t)a + 4 * na;
+}
+
+}  // namespace ib
+
+using namespace ib;
+
+extern "C" int ib_kv_tree_plan(const ib_kv_batch* batch, const int32_t* parents, int max_nodes,
+                               int32_t* depth, uint32_t* mask, void* stream) {
+    const char* who = "ib_kv_tree_plan";
+    const int r = tree_batch(batch, who);
+    if (r != IB_OK) return r;
+    if (max_nodes < 1 || max_nodes > IB_KV_MAX_NODES)
+        return paged_refuse(who, "max_nodes must be in [1, 1024]");
+    const int64_t n = batch->n_tokens, nm = n * ((max_nodes + 31) / 32);
+    if (n == 0 || batch->n_seqs == 0) return IB_OK;
+    if (!parents || !depth || !mask) return paged_refuse(who, "null pointer argument");
+    if (meet(depth, n, parents, n) || meet(mask, nm, parents, n) || meet(depth, n, mask, nm))
+        return paged_refuse(who, "parents, depth and mask must not overlap");
+    tree_plan_kernel<<<batch->n_seqs, TREE_THREADS, 0, as_stream(stream)>>>(
+        batch->cu_q, batch->slots, batch->n_tokens, parents, max_nodes, depth, mask);
+    IB_LAUNCH_CHECK("tree_plan_kernel");
+    return IB_OK;
+}
+
+extern "C" int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parents, const int32_t* tokens,
+                                 const int32_t* best, int32_t* path, int32_t* n_path, int32_t* next,
+                                 void* stream) {
+    const char* who = "ib_kv_tree_verify";
+    const int r = tree_batch(batch, who);
+    if (r != IB_OK) return r;
+    if (batch->n_seqs == 0) return IB_OK;
+    if (!parents || !tokens || !best || !path || !n_path || !next)
+        return paged_refuse(who, "null pointer argument");
+    const int64_t T = batch->n_tokens, B = batch->n_seqs;
+    const void* const out[3] = {path, n_path, next};
+    const int64_t out_n[3] = {T, B, B};
+    for (int i = 0; i < 3; ++i) {
+        bool bad = meet(out[i], out_n[i], parents, T) || meet(out[i], out_n[i], tokens, T) ||
+                   meet(out[i], out_n[i], best, T);
+        for (int k = 0; k < i; ++k) bad = bad || meet(out[i], out_n[i], out[k], out_n[k]);
+        if (bad) return paged_refuse(who, "the results must not overlap the lists or one another");
+    }
+    tree_verify_kernel<<<batch->n_seqs, 32, 0, as_stream(stream)>>>(
+        batch->cu_q, batch->slots, batch->n_tokens, parents, tokens, best, path, n_path, next);
+    IB_LAUNCH_CHECK("tree_verify_kernel");
+    return IB_OK;
+}
+
+extern "C" int ib_kv_tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                 const ib_kv_batch* batch, const int32_t* path, const int32_t* n_path,
+                                 void* stream) {
+    const char* who = "ib_kv_tree_accept";
+    const int r = paged_check_batch(pages, seqs, batch, 0, pages ? pages->n_kv_heads : 0, who);
+    if (r != IB_OK || batch->n_seqs == 0) return r;
+    if (!path || !n_path) return paged_refuse(who, "null pointer argument");
+    ib_kv_tree none{IB_KV_MAX_NODES, nullptr, nullptr};
+    const PagedView w = paged_view(pages, seqs, batch, pages->n_kv_heads, &none);
+    IB_CUDA_CHECK(launch_pdl(tree_accept_kernel, dim3(batch->n_seqs * ACCEPT_CLUSTER), dim3(ACCEPT_THREADS),
+                             0, as_stream(stream), true, w, seqs->table, seqs->len, seqs->refs,
+                             pool_bytes(pages), path, n_path));
+    return IB_OK;
+}
