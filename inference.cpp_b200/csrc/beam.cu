@@ -5,11 +5,12 @@
 // first maximum of one row (src/ops/ops.cpp:424-438, ib_argmax).
 //
 // One pass over the logits: a CTA takes a slice of a row, keeps a running maximum and sum of
-// exponentials, and the slice's k best, found through a threshold: once k values are known to lie at or
-// above it, all others need is one comparison.  Inside a row the order of v is that of x, so a slice's
-// candidates are chosen by x alone.  A second kernel, a CTA per group, makes the rows' log sums of the
-// slices' and picks the group's k best in 64 bits: candidates of different beams may be closer than FP32
-// tells apart.
+// exponentials, and the slice's k best.  Inside a row the order of v is that of x, so they are chosen by
+// x alone, through a threshold that at least k values are known to reach: it comes from the first step's
+// 256 threads' maxima, and from then on a value costs one comparison; the few that pass lie in shared
+// memory and are ranked at the end.  A second kernel, a CTA per group, makes the rows' log sums of the
+// slices' and picks the group's k best in 64 bits, through a threshold again: candidates of different
+// beams may be closer than FP32 tells apart.
 #include <cuda_fp16.h>
 #include <float.h>
 
@@ -49,38 +50,27 @@ __device__ __forceinline__ uint64_t shfl_max(uint64_t x) {
     return x;
 }
 
-// Sum over the CTA; `turn` alternates, so that one barrier does.
-__device__ __forceinline__ int block_sum(int c, int (&sh)[2][BS_WARPS], int turn) {
-    c = __reduce_add_sync(0xffffffffu, c);
-    if ((threadIdx.x & 31) == 0) sh[turn & 1][threadIdx.x >> 5] = c;
-    __syncthreads();
-    int s = 0;
-#pragma unroll
-    for (int i = 0; i < BS_WARPS; ++i) s += sh[turn & 1][i];
-    return s;
+// Numbers that sort as the values do (no NaN).
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The largest key, or one less, such that at least k of the CTA's keys (N a thread, zeros are none) are at
-// or above it, and at most `most` where that can be had by halving; 1 where there are fewer than k.
-template <int N>
-__device__ __forceinline__ uint64_t threshold(const uint64_t (&key)[N], int k, int most, int (&sh)[2][BS_WARPS],
-                                              int& turn) {
-    uint64_t lo = 1, hi = ~0ull;  // at least k at lo, fewer at hi
-    auto count = [&](uint64_t t) {
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) c += key[i] >= t;
-        return block_sum(c, sh, turn++);
-    };
-    int at_lo = count(1);
-    if (at_lo < k) return 1;
-    while (at_lo > most && hi - lo > 1) {
-        const uint64_t mid = lo + (hi - lo) / 2;
-        const int c = count(mid);
-        if (c >= k) lo = mid, at_lo = c;
-        else hi = mid;
+// A number that at least k of the CTA's threads' `best` reach, where that many are above 0: the least
+// of the warps' n-th largest, n = k / BS_WARPS rounded up.  (The k-th largest of all would let fewer
+// values pass, and costs a sort: with this one about k (1 + 1/2 + 1/3 .. 1/8) pass for k = 8.)
+__device__ __forceinline__ uint32_t reached(uint32_t best, int k, uint32_t (&sh)[BS_WARPS]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t top = 0;
+    for (int n = (k + BS_WARPS - 1) / BS_WARPS; n > 0; --n) {
+        top = __reduce_max_sync(0xffffffffu, best);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, best == top)) - 1) best = 0;
     }
-    return lo;
+    if (lane == 0) sh[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BS_WARPS; ++i) top = min(top, sh[i]);
+    return top;
 }
 
 struct SliceMeta {
@@ -95,7 +85,7 @@ struct SelectArgs {
     const float* scores;     // null: zeros
     const int32_t* ended;    // null: none
     int rows, beams, vocab, k, slices, end_token;
-    int64_t per_slice;       // values, a multiple of BS_TILE
+    int64_t per_slice;       // values
     uint64_t* list;          // [row][slice][k] keys, largest first, zeros behind
     SliceMeta* meta;         // [row][slice]
     float* out_score;        // [group][k]
@@ -108,125 +98,157 @@ __device__ __forceinline__ float logit(T x) {
     else return __half2float(x);
 }
 
-// The n <= BS_CAP keys in buf: the k largest, in order, to the front (zeros behind the last).
-__device__ __forceinline__ void keep_best(uint64_t* buf, int n, int k, int (&sh)[2][BS_WARPS], int& turn,
-                                          int* count) {
+struct SliceShared {
+    uint64_t buf[BS_CAP];
+    int n;
+    uint32_t top[2][BS_WARPS];
+    double sum[BS_WARPS];
+    float m[BS_WARPS];
+};
+
+// The k largest of the first n <= BS_CAP keys in sh.buf, in order, to out (zeros behind the last).
+// Every thread of the CTA calls it, after a barrier.
+__device__ __forceinline__ void rank_best(SliceShared& sh, int n, int k, uint64_t* __restrict__ out) {
+    const int tid = threadIdx.x;
+    if (n > 2 * k && n > BS_THREADS) {  // a threshold again, of what has passed the first
+        constexpr int N = BS_CAP / BS_THREADS;
+        uint64_t key[N], best = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = i * BS_THREADS + tid;
+            key[i] = at < n ? sh.buf[at] : 0;
+            best = key[i] > best ? key[i] : best;
+        }
+        const uint32_t least = reached((uint32_t)(best >> 32), k, sh.top[1]);
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if ((uint32_t)(key[i] >> 32) >= least && key[i]) sh.buf[atomicAdd(&sh.n, 1)] = key[i];
+        __syncthreads();
+        n = sh.n;
+    }
+    for (int i = tid; i < n; i += BS_THREADS) {
+        const uint64_t mine = sh.buf[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += sh.buf[j] > mine;
+        if (rank < k) out[rank] = mine;
+    }
+    for (int j = n + tid; j < k; j += BS_THREADS) out[j] = 0;
+}
+
+// The slice's k best where too many values reached the threshold (many equal ones, or values that
+// rise): step by step and a value of each thread at a time, with a threshold that is raised whenever the
+// room is used up.  sh.buf holds the k best so far, in no order, and what has come since.
+template <typename T>
+__device__ __noinline__ void slice_again(SliceShared& sh, const T* x, int64_t begin, int64_t end, int k,
+                                         uint64_t* __restrict__ out) {
     constexpr int N = BS_CAP / BS_THREADS;
     const int tid = threadIdx.x;
+    uint64_t floor_key = 1;
     __syncthreads();
-    uint64_t key[N];
+    if (tid == 0) sh.n = 0;
+    for (int64_t at = begin; at < end; at += BS_THREADS) {
+        __syncthreads();
+        const int have = sh.n;
+        __syncthreads();  // everybody has read it
+        if (have > BS_CAP - BS_THREADS) {
+            // keys are all different: halving finds the k-th largest
+            uint64_t key[N], lo = 1, hi = ~0ull;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int at = i * BS_THREADS + tid;
-        key[i] = at < n ? buf[at] : 0;
-    }
-    // keys are all different, so exactly k can be had
-    const uint64_t t = threshold(key, k, k, sh, turn);
-    if (tid == 0) *count = 0;
-    __syncthreads();
+            for (int i = 0; i < N; ++i) key[i] = i * BS_THREADS + tid < have ? sh.buf[i * BS_THREADS + tid] : 0;
+            while (hi - lo > 1) {
+                const uint64_t half = lo + (hi - lo) / 2;
+                int c = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (key[i] >= t) buf[atomicAdd(count, 1)] = key[i];
-    __syncthreads();
-    const int c = min(*count, k);
-    uint64_t mine = 0;
-    int rank = 0;
-    if (tid < c) {
-        mine = buf[tid];
-        for (int j = 0; j < c; ++j) rank += buf[j] > mine;
+                for (int i = 0; i < N; ++i) c += __syncthreads_count(key[i] >= half);
+                if (c >= k) lo = half;
+                else hi = half;
+                if (c == k) break;
+            }
+            floor_key = lo;
+            __syncthreads();
+            if (tid == 0) sh.n = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (key[i] >= lo) sh.buf[atomicAdd(&sh.n, 1)] = key[i];
+            __syncthreads();
+        }
+        const int64_t p = at + tid;
+        const uint64_t key = p < end ? beam_key(logit(x[p]), (uint32_t)p) : 0;
+        if (key >= floor_key) sh.buf[atomicAdd(&sh.n, 1)] = key;
     }
     __syncthreads();
-    if (tid < c) buf[rank] = mine;
-    for (int j = c + tid; j < k; j += BS_THREADS) buf[j] = 0;
-    __syncthreads();
+    rank_best(sh, sh.n, k, out);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(BS_THREADS) beam_slice_kernel(const __grid_constant__ SelectArgs A) {
-    __shared__ uint64_t buf[BS_CAP];
-    __shared__ int sh[2][BS_WARPS];
-    __shared__ int n_buf, n_kept;
-    __shared__ double sh_sum[BS_WARPS];
-    __shared__ float sh_m[BS_WARPS];
+    __shared__ SliceShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / A.slices, slice = blockIdx.x - row * A.slices;
-    pdl_wait();
     pdl_launch_dependents();
     if (A.ended && A.ended[row]) return;
     const T* const x = static_cast<const T*>(A.logits) + (int64_t)row * A.stride;
-    const int64_t begin = slice * A.per_slice, end = min((int64_t)A.vocab, begin + A.per_slice);
-    int turn = 0;
-    if (tid == 0) n_buf = 0;
-    float m = -INFINITY, sum = 0.f;
-    uint64_t floor_key = 1;  // nothing below it is looked at
-    const int k = A.k;
-    for (int64_t at = begin; at < end; at += BS_TILE) {
+    const int begin = (int)(slice * A.per_slice), end = (int)min((int64_t)A.vocab, begin + A.per_slice);
+    if (tid == 0) sh.n = 0;
+    float m = -INFINITY, sum = 0.f, least = 0.f;
+    for (int at = begin; at < end; at += BS_TILE) {
         float v[16];
+        const T* const p = x + at + tid;
+        if (at + BS_TILE <= end) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int64_t p = at + i * BS_THREADS + tid;
-            v[i] = p < end ? logit(x[p]) : -INFINITY;
+            for (int i = 0; i < 16; ++i) v[i] = logit(p[i * BS_THREADS]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                v[i] = at + i * BS_THREADS + tid < end ? logit(p[i * BS_THREADS]) : -INFINITY;
         }
         float top = v[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, v[i]);
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, v[i]);  // (a NaN only where there is nothing else)
+        if (at == begin) {
+            const uint32_t o = reached(top > -INFINITY ? ordered(top) : 0, A.k, sh.top[0]);
+            // the value itself; where not enough threads have one, all that are no -inf pass
+            least = o ? __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o) : -FLT_MAX;
+        }
         if (top > m) {
             sum *= expf(m - top);
             m = top;
         }
-        if (m > -INFINITY || top != top) {
+        const float base = m > -INFINITY ? m : 0.f;  // e^-inf is 0, and a NaN stays one
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum += expf(v[i] - m);
-        } else {
+        for (int i = 0; i < 16; ++i) sum += expf(v[i] - base);
+        if (top >= least) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum += v[i] != v[i] ? NAN : 0.f;
-        }
-        uint64_t key[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) key[i] = beam_key(v[i], (uint32_t)(at + i * BS_THREADS + tid));
-        // a value for each thread that may take part, the same way in every step
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) c += key[i] >= floor_key;
-        int more = block_sum(c, sh, turn++);
-        if (n_buf + more > BS_CAP) {
-            // raise the floor: of what is here first, then of everything
-            const uint64_t t = threshold(key, k, k, sh, turn);
-            floor_key = t > floor_key ? t : floor_key;
-            keep_best(buf, n_buf, k, sh, turn, &n_kept);
-            if (tid == 0) n_buf = n_kept < k ? n_kept : k;
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (key[i] >= floor_key) buf[atomicAdd(&n_buf, 1)] = key[i];
-        __syncthreads();
-        if (at == begin && at + BS_TILE < end) {
-            keep_best(buf, n_buf, k, sh, turn, &n_kept);
-            if (tid == 0) n_buf = n_kept < k ? n_kept : k;
-            __syncthreads();
-            if (n_buf == k) floor_key = buf[k - 1];
+            for (int i = 0; i < 16; ++i)
+                if (v[i] >= least) {
+                    const int to = atomicAdd(&sh.n, 1);
+                    if (to < BS_CAP) sh.buf[to] = beam_key(v[i], (uint32_t)(at + i * BS_THREADS + tid));
+                }
         }
     }
-    keep_best(buf, n_buf, k, sh, turn, &n_kept);
-    const int64_t out = (int64_t)row * A.slices + slice;
-    for (int j = tid; j < k; j += BS_THREADS) A.list[out * k + j] = buf[j];
+    const int64_t place = (int64_t)row * A.slices + slice;
     // the slice's maximum and sum
     float M = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0) sh_m[warp] = M;
+    if (lane == 0) sh.m[warp] = M;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < BS_WARPS; ++i) M = fmaxf(M, sh_m[i]);
-    double d = m > -INFINITY ? (double)sum * exp((double)m - (double)M) : (double)sum;
+    for (int i = 0; i < BS_WARPS; ++i) M = fmaxf(M, sh.m[i]);
+    double d = (double)(m > -INFINITY ? sum * expf(m - M) : sum);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) sh_sum[warp] = d;
+    if (lane == 0) sh.sum[warp] = d;
+    const int n = sh.n;
+    if (n <= BS_CAP) rank_best(sh, n, A.k, A.list + place * A.k);
+    else slice_again(sh, x, (int64_t)begin, (int64_t)end, A.k, A.list + place * A.k);
     __syncthreads();
     if (tid == 0) {
-        for (int i = 1; i < BS_WARPS; ++i) d += sh_sum[i];
-        A.meta[out] = SliceMeta{M, 0.f, d};
+        for (int i = 1; i < BS_WARPS; ++i) d += sh.sum[i];
+        A.meta[place] = SliceMeta{M, 0.f, d};
     }
 }
 
@@ -238,59 +260,43 @@ __device__ __forceinline__ bool better(const Best& a, const Best& b) {
     return a.v > b.v || (a.v == b.v && a.place < b.place);
 }
 
-// One CTA per group.  Each thread has some of the group's lists (a row's slice each) and offers the best
-// of their heads; k rounds of a maximum over the CTA.
-__global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_constant__ SelectArgs A) {
-    extern __shared__ double base[];  // [beams] score - log sum of e^(x - M)
-    double* const row_m = base + A.beams;                      // [beams] M
-    int* const head = reinterpret_cast<int*>(row_m + A.beams);  // [beams * slices]
+constexpr int BS_GROUP_CAP = 1024;
+
+__device__ __forceinline__ void put_choice(const SelectArgs& A, int g, int j, const Best& y) {
+    const bool any = y.v > -INFINITY;
+    const int64_t at = (int64_t)g * A.k + j;
+    A.out_score[at] = any ? (float)y.v : -INFINITY;
+    A.out_token[at] = any ? (int32_t)(uint32_t)y.place : -1;
+    A.out_row[at] = any ? g * A.beams + (int32_t)(y.place >> 32) : -1;
+}
+
+// Candidate c of group g: entry c % k of list c / k, a row's slice; v is -inf where there is none.  base:
+// score - log sum e^(x - M), and M.
+__device__ __forceinline__ Best candidate(const SelectArgs& A, int g, int c, const double2* base) {
+    const int l = c / A.k, b = l / A.slices;
+    Best y = {-INFINITY, ~0ull};
+    if (A.ended && A.ended[g * A.beams + b]) {
+        if (c == b * A.slices * A.k) y = Best{base[b].x, ((uint64_t)b << 32) | (uint32_t)A.end_token};
+    } else if (const uint64_t key = A.list[(int64_t)g * A.beams * A.slices * A.k + c]) {
+        y = Best{base[b].x + ((double)key_value(key) - base[b].y), ((uint64_t)b << 32) | key_place(key)};
+    }
+    if (!(y.v > -INFINITY)) y.v = -INFINITY;  // NaN is no candidate
+    return y;
+}
+
+// The group's choice where too many candidates reached the threshold: k rounds of a maximum over the CTA,
+// each behind the last one's.
+__device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, const double2* base) {
     __shared__ Best sh_best[2][BS_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = blockIdx.x, row0 = g * A.beams, lists = A.beams * A.slices, k = A.k;
-    pdl_wait();
-    for (int b = warp; b < A.beams; b += BS_WARPS) {
-        const int row = row0 + b;
-        const bool end = A.ended && A.ended[row];
-        double log_sum = 0;
-        float M = 0.f;
-        if (!end) {
-            const SliceMeta* const meta = A.meta + (int64_t)row * A.slices;
-            double s = 0;
-            M = -INFINITY;
-            for (int i = lane; i < A.slices; i += 32) M = fmaxf(M, meta[i].m);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            for (int i = lane; i < A.slices; i += 32) {
-                const SliceMeta y = meta[i];
-                s += y.m > -INFINITY ? y.sum * exp((double)y.m - (double)M) : y.sum;
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            log_sum = log(s);  // (a row of nothing but -inf has no candidates)
+    Best last = {INFINITY, 0};
+    bool first = true;
+    for (int j = 0; j < A.k; ++j, first = false) {
+        Best top = {-INFINITY, ~0ull};
+        for (int c = tid; c < n; c += BS_THREADS) {
+            const Best y = candidate(A, g, c, base);
+            if ((first || better(last, y)) && better(y, top)) top = y;
         }
-        if (lane == 0) {
-            base[b] = (A.scores ? (double)A.scores[row] : 0.0) - log_sum;
-            row_m[b] = M;
-        }
-    }
-    for (int l = tid; l < lists; l += BS_THREADS) head[l] = 0;
-    __syncthreads();
-    const Best none = {-INFINITY, ~0ull};
-    for (int j = 0; j < k; ++j) {
-        Best best = none;
-        int from = -1;
-        for (int l = tid; l < lists; l += BS_THREADS) {
-            const int b = l / A.slices;
-            Best y = none;
-            if (A.ended && A.ended[row0 + b]) {
-                if (head[l] == 0 && l == b * A.slices) y = Best{base[b], ((uint64_t)b << 32) | (uint32_t)A.end_token};
-            } else if (head[l] < k) {
-                const uint64_t key = A.list[((int64_t)row0 * A.slices + l) * k + head[l]];
-                if (key) y = Best{base[b] + ((double)key_value(key) - row_m[b]), ((uint64_t)b << 32) | key_place(key)};
-            }
-            if (y.v > -INFINITY && better(y, best)) best = y, from = l;  // NaN: not a number is no candidate
-        }
-        Best top = best;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             Best y;
@@ -304,15 +310,68 @@ __global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_con
 #pragma unroll
         for (int i = 1; i < BS_WARPS; ++i)
             if (better(sh_best[j & 1][i], top)) top = sh_best[j & 1][i];
-        const bool any = top.v > -INFINITY;
-        if (any && from >= 0 && best.place == top.place) ++head[from];
-        if (tid == 0) {
-            const int64_t at = (int64_t)g * k + j;
-            A.out_score[at] = any ? (float)top.v : -INFINITY;
-            A.out_token[at] = any ? (int32_t)(uint32_t)top.place : -1;
-            A.out_row[at] = any ? row0 + (int32_t)(top.place >> 32) : -1;
+        if (tid == 0) put_choice(A, g, j, top);
+        last = top;
+    }
+}
+
+__global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_constant__ SelectArgs A) {
+    extern __shared__ __align__(16) double2 base[];  // [beams]
+    __shared__ Best buf[BS_GROUP_CAP];
+    __shared__ uint32_t sh_top[BS_WARPS];
+    __shared__ int sh_n;
+    const int tid = threadIdx.x, g = blockIdx.x, row0 = g * A.beams, k = A.k;
+    if (tid == 0) sh_n = 0;
+    pdl_wait();
+    // as many lanes to a row as it has slices
+    int lanes = 1;
+    while (lanes < 32 && lanes < A.slices) lanes *= 2;
+    const int sub = tid & (lanes - 1), per = BS_THREADS / lanes;
+    for (int b0 = 0; b0 < A.beams; b0 += per) {
+        const int b = b0 + tid / lanes, row = row0 + b;
+        const bool there = b < A.beams, end = there && A.ended && A.ended[row];
+        const SliceMeta* const meta = A.meta + (int64_t)row * A.slices;
+        const int n = there && !end ? A.slices : 0;
+        float M = -INFINITY;
+        double s = 0;
+        for (int i = sub; i < n; i += lanes) M = fmaxf(M, meta[i].m);
+        for (int o = lanes / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        for (int i = sub; i < n; i += lanes) {
+            const SliceMeta y = meta[i];
+            s += y.m > -INFINITY ? y.sum * exp((double)y.m - (double)M) : y.sum;
+        }
+        for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        // (a row of nothing but -inf has no candidates)
+        if (there && sub == 0)
+            base[b] = make_double2((A.scores ? (double)A.scores[row] : 0.0) - (end ? 0.0 : log(s)), end ? 0.0 : (double)M);
+    }
+    __syncthreads();
+    const int n = A.beams * A.slices * k;
+    // rounding down keeps the order, so that k values at or above it are above all below it
+    auto low = [](double v) { return v > -INFINITY ? ordered(__double2float_rd(v)) : 0u; };
+    uint32_t best = 0;
+    for (int c = tid; c < n; c += BS_THREADS) best = max(best, low(candidate(A, g, c, base).v));
+    const uint32_t least = max(reached(best, k, sh_top), 1u);
+    for (int c = tid; c < n; c += BS_THREADS) {
+        const Best y = candidate(A, g, c, base);
+        if (low(y.v) >= least) {
+            const int to = atomicAdd(&sh_n, 1);
+            if (to < BS_GROUP_CAP) buf[to] = y;
         }
     }
+    __syncthreads();
+    const int some = sh_n;
+    if (some > BS_GROUP_CAP) {
+        group_again(A, g, n, base);
+        return;
+    }
+    for (int i = tid; i < some; i += BS_THREADS) {
+        const Best mine = buf[i];
+        int rank = 0;
+        for (int j = 0; j < some; ++j) rank += better(buf[j], mine);
+        if (rank < k) put_choice(A, g, rank, mine);
+    }
+    for (int j = some + tid; j < k; j += BS_THREADS) put_choice(A, g, j, Best{-INFINITY, ~0ull});
 }
 
 // How a call is cut.
@@ -329,6 +388,9 @@ static SelectPlan select_plan(int64_t rows, int64_t vocab, int k) {
     const int64_t per = std::max<int64_t>(1, (tiles + want - 1) / want);
     p.per_slice = per * BS_TILE;
     p.slices = (int)((tiles + per - 1) / per);
+    // slices of equal length
+    p.per_slice = ((vocab + p.slices - 1) / p.slices + BS_THREADS - 1) / BS_THREADS * BS_THREADS;
+    p.slices = (int)((vocab + p.per_slice - 1) / p.per_slice);
     p.list_off = 0;
     p.meta_off = ((size_t)rows * p.slices * k * 8 + 255) / 256 * 256;
     p.bytes = p.meta_off + ((size_t)rows * p.slices * sizeof(SliceMeta) + 255) / 256 * 256;
@@ -392,7 +454,7 @@ extern "C" int ib_beam_select(int type, const void* logits, int64_t stride, cons
     const dim3 grid((unsigned)(rows * p.slices));
     IB_CUDA_CHECK(launch_pdl(type == IB_TYPE_F32 ? beam_slice_kernel<float> : beam_slice_kernel<__half>, grid,
                              dim3(BS_THREADS), 0, st, false, a));
-    const size_t smem = (size_t)beams * 16 + (size_t)beams * p.slices * 4;
+    const size_t smem = (size_t)beams * sizeof(double2);
     IB_CUDA_CHECK(launch_pdl(beam_group_kernel, dim3(n_groups), dim3(BS_THREADS), smem, st, true, a));
     return IB_OK;
 }

@@ -962,9 +962,9 @@ __device__ __forceinline__ void join_pieces(const JoinArgs& A, int no, int y) {
     if (!next_segment(w, A.rule, p, sg)) return;
     // the tile's work is [a, b), and pieces c0 .. c1 hold shares of it: the first one's is its last
     // segment (unless the tile begins with the piece), the others' is their first
-    const long long start_g = (long long)G * max(sg.start, 0);
-    const long long a = p.base + sg.hk * p.x.per_head + tiles_work(sg.tile, start_g, R);
-    const long long b = a + start_g + (long long)(sg.tile + 1) * R;
+    const long long start_g = start_work(A.rule, sg.s, G);
+    const long long a = p.base + sg.hk * p.x.per_head + tiles_work(sg.tile, start_g, A.rule.slope());
+    const long long b = a + start_g + (long long)(sg.tile + 1) * A.rule.slope();
     const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
     if (c0 != no - 1 || c1 >= A.rule.n_pieces) return;
     const int n_parts = c1 - c0 + 1, first = 2 * c0 + (a == c0 * p.len ? 0 : 1);
@@ -1084,6 +1084,21 @@ static int rows_launch(int threads, size_t smem, bool pieces, const RowsArgs& a,
 template <typename KV, int HDP>
 constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 
+// The same for trees, whose wide kernel takes one query tile and its key tiles in turn (us, 16, 24, 32
+// and 48 rows, 32 heads):
+//   sequences over   FP16, 8 kv heads of 128                  FP16, 4 kv heads of 64
+//   2 x 30000        91:102  123:103  156:101  217:102        43:54   44:55   61:54   81:54
+//   8 x 2000         42:53   51:54    59:54    76:55          22:30   24:30   29:30   34:31
+//   32 x 2000        102:120 135:120  169:120  226:122        43:61   54:62   67:62   91:63
+//   64 x 400         67:119  89:119   113:120  161:121        34:53   46:52   45:53   63:54
+//                    FP32, 8 kv heads of 128                  FP32, 4 kv heads of 64
+//   2 x 30000        219:319 318:320  410:321  571:324        67:95   73:96   103:94  141:95
+//   8 x 2000         78:114  90:115   115:114  160:116        30:43   34:44   43:44   54:44
+//   32 x 2000        212:346 296:347  389:347  581:349        65:103  86:104  109:102 147:103
+//   64 x 400         118:201 172:201  209:202  314:205        48:80   64:81   66:81   91:82
+template <int HDP>
+constexpr int narrow_tree_rows = HDP == 128 ? 24 : 32;
+
 // Wide tiles run on tcgen05 for head_dim up to 128.  Above, S and O of two query tiles do not fit
 // into tensor memory, nor FP32 sums of a row into a thread's registers; one query tile whose sums are
 // shared by both softmax groups would fit on FP16 pages and is not built, on FP32 pages the TF32 parts
@@ -1091,7 +1106,7 @@ constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 template <int HDP>
 constexpr bool on_tcgen05 = HDP <= 128;
 
-template <typename KV, int HDP>
+template <typename KV, int HDP, bool TREE>
 static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     constexpr int ALL = 0x7fffffff;
     const int64_t G = n_heads / p->n_kv_heads;
@@ -1113,14 +1128,17 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
         s.ml_off = take((size_t)2 * r.n_pieces * r.R * sizeof(float2));
     };
     const int64_t rows = b->n_tokens * G;
-    constexpr int NARROW = narrow_rows<KV, HDP>;
+    constexpr int NARROW = TREE ? narrow_tree_rows<HDP> : narrow_rows<KV, HDP>;
     if (most_q * G <= NARROW) {
         add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
     } else {
-        const int narrow = b->n_seqs == 1 || G > NARROW ? 0 : NARROW;
+        // trees: where a sequence has more rows on average, short ones are left to the wide kernel too (an
+        // empty launch of the narrow one and its share of the join take 10 us)
+        const bool few = b->n_seqs == 1 || G > NARROW || (TREE && rows > (int64_t)NARROW * b->n_seqs);
+        const int narrow = few ? 0 : NARROW;
         if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
         CutRule r;
-        if constexpr (on_tcgen05<HDP>) r = tensor_rule<KV>(p->head_dim, narrow + 1, ALL);
+        if constexpr (on_tcgen05<HDP>) r = tensor_rule<KV, TREE>(p->head_dim, narrow + 1, ALL);
         else r = wide_rule<KV, HDP>(narrow + 1, ALL);
         add(r, seqs + rows / r.R);
     }
@@ -1185,7 +1203,7 @@ static int attention_paged(const ib_kv_pages* p, const ib_kv_batch* b, RowsArgs 
                            size_t* bytes, int64_t max_pos, cudaStream_t st) {
     auto go = [&](auto hdp) {
         constexpr int HDP = decltype(hdp)::value;
-        const Plan plan = make_plan<KV, HDP>(p, b, a.w.H);
+        const Plan plan = a.mask ? make_plan<KV, HDP, true>(p, b, a.w.H) : make_plan<KV, HDP, false>(p, b, a.w.H);
         if (bytes) {
             *bytes = plan.bytes;
             return (int)IB_OK;
@@ -1271,6 +1289,7 @@ static int attention_call(const ib_kv_pages* pages, const ib_kv_seqs* seqs, cons
     a.k = (const uint8_t*)pages->k + layer * layer_bytes;
     a.v = (const uint8_t*)pages->v + layer * layer_bytes;
     a.scale_log2 = scale * 1.4426950408889634f;
+    a.sectors = (((uintptr_t)out | (uintptr_t)(out_stride * 4)) & 31) == 0;
     return attention_paged_any(pages, batch, a, workspace, nullptr,
                                (int64_t)seqs->max_pages * pages->page_size, as_stream(stream));
 }

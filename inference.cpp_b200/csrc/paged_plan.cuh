@@ -16,6 +16,10 @@ constexpr int kSMs = 148;  // of a B200: the pieces aimed at, and so the workspa
 // positions, in n_pieces pieces of at least `least` positions of one token.
 struct CutRule {
     int R, KT, min_rows, max_rows, n_pieces, least;
+    int fixed = 0;  // positions that beginning a tile costs as much as (pieces)
+    // trees: every tile of a sequence costs the same, whole key tiles
+    bool flat = false;
+    __device__ __forceinline__ int slope() const { return flat ? 0 : R; }
 };
 
 // Work is counted in rows x positions, roughly: tile i of a sequence whose first new token is
@@ -30,6 +34,12 @@ __device__ __forceinline__ long long add_work(long long a, long long b) {
     return (long long)min((unsigned long long)a + (unsigned long long)b, kMostWork);
 }
 
+// What a tile of a sequence costs before the rows' own positions.
+__device__ __forceinline__ long long start_work(const CutRule& rule, const SeqInfo& s, int G) {
+    const int seen = rule.flat ? (max(s.L, 0) + rule.KT - 1) / rule.KT * rule.KT : max(s.L - s.n, 0);
+    return (long long)G * (seen + rule.fixed);
+}
+
 __device__ __forceinline__ long long tiles_work(long long t, long long start_g, int R) {
     return t * start_g + (long long)R * (t * (t + 1) / 2);
 }
@@ -40,7 +50,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedView& w, const CutRule& r
     const int G = w.H / w.Hkv, rows = x.s.n * G;
     const bool in = rows >= rule.min_rows && rows <= rule.max_rows;
     const int tiles = in ? (rows + rule.R - 1) / rule.R : 0;
-    x.per_head = tiles_work(tiles, (long long)G * max(x.s.L - x.s.n, 0), rule.R);
+    x.per_head = tiles_work(tiles, start_work(rule, x.s, G), rule.slope());
     // at most 2^23 tiles of at most 2^38 each (paged_check_batch)
     x.all = x.per_head * w.Hkv;
     return x;
@@ -152,7 +162,7 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     }
     const int G = w.H / w.Hkv;
     const SeqInfo& s = p.x.s;
-    const long long start_g = (long long)G * max(s.L - s.n, 0);
+    const long long start_g = start_work(rule, s, G);
     long long u = p.at - p.base;
     g.s = s;
     g.start = s.L - s.n;
@@ -163,14 +173,14 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     int lo = 0, hi = (s.n * G + rule.R - 1) / rule.R;  // the tile: the last whose work begins at or before u
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (tiles_work(mid, start_g, rule.R) <= u) lo = mid;
+        if (tiles_work(mid, start_g, rule.slope()) <= u) lo = mid;
         else hi = mid;
     }
     g.tile = lo;
     g.row0 = lo * rule.R;
     g.rows = min(rule.R, s.n * G - g.row0);
-    const long long all = start_g + (long long)(lo + 1) * rule.R;
-    const long long x0 = u - tiles_work(lo, start_g, rule.R);
+    const long long all = start_g + (long long)(lo + 1) * rule.slope();
+    const long long x0 = u - tiles_work(lo, start_g, rule.slope());
     const long long x1 = min(all, x0 + (p.end - p.at));
     const int seen = max(0, g.start + (g.row0 + g.rows - 1) / G + 1);
     const int nkt = (seen + rule.KT - 1) / rule.KT;
@@ -313,6 +323,7 @@ struct RowsArgs {
     float scale_log2;   // scale * log2(e)
     const uint32_t* mask;  // trees: [token][words], see ib_kv_tree
     int words;
+    bool sectors;  // rows of out begin on boundaries of 32 bytes
     // The kernel before is the call's narrow one, which writes other rows and workspace: this one
     // starts beside its last CTAs and waits for it at its own end only, so that what follows
     // finds both complete.  (The narrow kernel lets it start after its own wait for what came
@@ -388,7 +399,7 @@ __device__ __forceinline__ float pow2_scale(float top, float& inverse) {
 }
 
 // Tiles of many rows on tcgen05, for head_dim up to 128 (paged_tensor.cu).
-template <typename KV>
+template <typename KV, bool TREE>
 CutRule tensor_rule(int head_dim, int min_rows, int max_rows);
 template <typename KV, bool TREE>
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st);

@@ -69,10 +69,11 @@ __global__ void wait_selftest_kernel() {
     mbar_wait(&bar, 0, &g_paged_faults.wait, PAGED_BAD_WAIT, 256);
 }
 
-template <typename KV, int HDP>
+// SPLIT (trees): one query tile, whose key tiles the two groups of softmax warps take in turn.
+template <typename KV, int HDP, bool SPLIT>
 struct TensorCfg {
     static constexpr bool F32 = sizeof(KV) == 4;
-    static constexpr int QT = F32 && HDP == 128 ? 1 : 2;  // query tiles of 128 rows
+    static constexpr int QT = SPLIT || (F32 && HDP == 128) ? 1 : 2;  // query tiles of 128 rows
     static constexpr int R = 128 * QT;
     static constexpr int KT = !F32 ? 128 : HDP == 64 ? 64 : 32;  // positions of a key tile
     static constexpr int EB = F32 ? 4 : 2;                       // bytes of an operand element
@@ -80,7 +81,10 @@ struct TensorCfg {
     static constexpr int Q_PLANE = 128 * HDP * EB;               // hi or lo of a query tile
     static constexpr int PLANE = KT * HDP * EB;                  // a K or V tile, or its hi or lo
     static constexpr int TILE = F32 ? 2 * PLANE : PLANE;         // a ring slot
-    static constexpr int SLOTS = F32 ? 2 : 3;
+    static constexpr int SLOTS = !SPLIT ? (F32 ? 2 : 3) : F32 ? (HDP == 64 ? 4 : 2) : HDP == 64 ? 6 : 5;
+    static constexpr int RECENT = SPLIT ? 8 : 4;                 // key tiles whose masks are kept
+    // tensor memory's columns for two more values of the second group's rows: behind its O, or its p
+    static constexpr int ML = HDP == 64 ? 256 + 128 + 64 : F32 ? 128 + 2 * KT : -1;
     static constexpr int RAW = F32 ? 2 * PLANE : 0;              // FP32 K and V as they come
     static constexpr int Q_BLOCK = 128 * 128;                    // ROW columns of a query tile
     static constexpr int K_BLOCK = KT * 128;                     // and of a K tile
@@ -93,7 +97,7 @@ struct TensorCfg {
     // registers of the softmax warps and of the others, within what the launch has
     static constexpr int MANY = F32 ? 184 : 224, FEW = F32 ? 72 : 56;
     static_assert(256 * MANY + (THREADS - 256) * FEW <= THREADS * (65536 / THREADS / 8 * 8), "");
-    static constexpr size_t SMEM = QT * 2 * Q_PLANE + SLOTS * TILE + RAW + 1024;
+    static constexpr size_t SMEM = QT * 2 * Q_PLANE + SLOTS * TILE + RAW;
 };
 
 // ---- tcgen05 ---------------------------------------------------------------------------
@@ -202,6 +206,20 @@ __device__ __forceinline__ void pt_read32(uint32_t at, float (&a)[32]) {
         : "r"(at)
         : "memory");
 }
+__device__ __forceinline__ float2 pt_read2(uint32_t at) {
+    float2 x;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(x.x), "=f"(x.y)
+        : "r"(at)
+        : "memory");
+    return x;
+}
+__device__ __forceinline__ void pt_st2(uint32_t at, float x, float y) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y)
+                 : "memory");
+}
 __device__ __forceinline__ void pt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
@@ -268,27 +286,44 @@ struct TensorArgs {
     int box;           // log2 of a box's rows; FP16: 0 for no TMA
 };
 
+template <int SLOTS>
 struct TensorBars {
-    uint64_t kv_full[3], kv_empty[3], raw_full[2], raw_empty[2];
-    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], seg_done[2], v_there[3], done;
+    uint64_t kv_full[SLOTS], kv_empty[SLOTS], raw_full[2], raw_empty[2];
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], seg_done[2], v_there[SLOTS], done;
+    uint64_t x_there, x_done;  // the second group's sums are in tensor memory; have been read
 };
 
+// K and V tiles of a segment of n key tiles in the order in which they are used: key tile 2 e or 2 e + 1
+// of tile number e.  SPLIT: K0 K1 V0 K2 V1 K3 ..
+template <bool SPLIT>
+__device__ __forceinline__ int tile_order(int e, int n) {
+    if constexpr (!SPLIT) return e;
+    if (e < 2) return e == 0 ? 0 : n > 1 ? 2 : 1;
+    if (e >= 2 * n - 2) return 2 * (e - n) + 1;
+    return e & 1 ? e + 1 : e - 1;  // K of e / 2 + 1/2, V of e / 2 - 1
+}
+
 template <typename KV, int HDP, bool TREE>
-__global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
+__global__ void __launch_bounds__(TensorCfg<KV, HDP, TREE>::THREADS, 1)
     attn_tensor_kernel(const __grid_constant__ TensorArgs TA) {
     const RowsArgs& A = TA.rows;
-    using C = TensorCfg<KV, HDP>;
+    constexpr bool SPLIT = TREE;
+    using C = TensorCfg<KV, HDP, SPLIT>;
     constexpr bool F32 = C::F32;
     constexpr int KT = C::KT;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) TensorBars bar;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) TensorBars<C::SLOTS> bar;
     __shared__ uint32_t tmem_base;
     __shared__ Piece sh_piece[C::WARPS];  // the same one for each warp, out of its registers
     __shared__ int found;
-    // of the last four key tiles: positions without a page; positions whose V is not finite
-    __shared__ __align__(16) uint16_t sh_gone[4][8];
-    __shared__ __align__(16) uint16_t sh_bad[4][8];
-    __shared__ uint32_t sh_bad32[4][C::SPLIT_WARPS][2];  // the same for FP32, of each splitting warp
+    // of the last key tiles: positions without a page; positions whose V is not finite
+    constexpr int RECENT = C::RECENT;
+    __shared__ __align__(16) uint16_t sh_gone[RECENT][8];
+    __shared__ __align__(16) uint16_t sh_bad[F32 ? 1 : RECENT][8];
+    __shared__ uint32_t sh_bad32[F32 ? RECENT : 1][C::SPLIT_WARPS][2];  // the same for FP32, of each splitting warp
+    __shared__ uint8_t sh_scale[2][SPLIT && !F32 ? 128 : 1];  // of the segment's rows (exponents), by its number
+    // the second group's maximum and sum, where tensor memory has no columns left for them
+    __shared__ float2 sh_ml[SPLIT && C::ML < 0 ? 128 : 1];
     const PagedView& w = A.w;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (!A.beside) pdl_wait();
@@ -300,15 +335,17 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
         return;
     }
     if (tid > 0 && tid < C::WARPS) sh_piece[tid] = sh_piece[0];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t base = smem_u32(smem_raw);  // on a boundary of 1024 bytes, for the swizzle
+    uint8_t* const base_ptr = smem_raw;
     if (tid == 0) {
         if (F32 || TA.box) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.k)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&TA.v)) : "memory");
         }
+        // SPLIT with TMA: one arrival, of the warp that sees to the tile
+        const int fill = SPLIT && !F32 && TA.box ? 1 : 33 * C::FILL_WARPS;
         for (int i = 0; i < C::SLOTS; ++i) {
-            mbar_init(&bar.kv_full[i], 33 * C::FILL_WARPS);
+            mbar_init(&bar.kv_full[i], fill);
             mbar_init(&bar.kv_empty[i], 1);
             mbar_init(&bar.v_there[Looks::bar(i)], 1);
         }
@@ -322,6 +359,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             mbar_init(&bar.o_full[i], 1);
             mbar_init(&bar.seg_done[i], 128);
         }
+        mbar_init(&bar.x_there, 128);
+        mbar_init(&bar.x_done, 128);
         mbar_init(&bar.done, 1);
         fence_mbar_init();
     }
@@ -353,15 +392,34 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
         return __all_sync(0xffffffffu, mbar_wait(b, (uint32_t)(n & 1), &g_paged_faults.wait, PAGED_BAD_WAIT));
     };
 
+    // The first segment here, for all roles: its code is brought in once.
+    bool first = false;
+    if constexpr (SPLIT) first = next();
+    auto go_on = [&](bool& begun) -> bool {  // `begun`: false at a role's beginning
+        if (!SPLIT || begun) return next();
+        begun = true;
+        return first;
+    };
     if (warp < 8) {
         // ---- softmax of query tile t: thread = row ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::MANY));
         const int t = warp >> 2, wr = (warp & 3) * 32;  // this warp's rows of the tile, its lanes
-        uint8_t* const q_ptr = base_ptr + 2 * t * C::Q_PLANE;
+        // SPLIT: both groups have the tile's rows.  The second one has key tiles 0, 2 .., the first one
+        // 1, 3 ..; the second one's sums go to the first through tensor memory, where both reach the same
+        // lanes, and the first one writes the results while the second brings in the next segment's q and
+        // begins with it.
+        const int qt = SPLIT ? 0 : t, j0 = SPLIT ? 1 - t : 0;
+        constexpr int DJ = SPLIT ? 2 : 1;
+        uint8_t* const q_ptr = base_ptr + 2 * qt * C::Q_PLANE;
         const uint32_t s_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(128 * t);
         const uint32_t o_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(256 + 128 * t);
+        [[maybe_unused]] const uint32_t ml_at = tmem + ((uint32_t)wr << 16) + (uint32_t)C::ML;
         int tiles = 0;      // key tiles so far, of all segments
-        uint32_t seen = 0;  // and counted as the copies do (both query tiles)
+        if constexpr (!SPLIT) first = next();
+        uint32_t seen = 0;  // and counted as the copies do (both groups')
+        // SPLIT: the first group's key tiles so far, the one that used q last
+        [[maybe_unused]] int firsts = 0, q_used = -1, exchanges = 0;
+        [[maybe_unused]] uint32_t segs = 0;
         bool ok = true;
         const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
         // The segment's q into this warp's 32 rows of the tile, HDP / 8 lanes to a row; returns the
@@ -370,7 +428,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
         // parts that are made of it.
         auto stage_q = [&](const Segment& sg) -> float {
             constexpr int LPR = HDP / 8, RPI = 32 / LPR;
-            const int rows = sg.rows - 128 * t, d = (lane % LPR) * 8;
+            const int rows = sg.rows - 128 * qt, d = (lane % LPR) * 8;
             float mine = F32 ? 1.f : 0.f;
             if (rows <= 0 || sg.kt0 == sg.kt1) return mine;
             // 16 bytes of the values d .. of row r: FP16 hi, lo; FP32 the first four's hi, the others'
@@ -381,12 +439,12 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                 else
                     return (uint32_t)((d >> 6) * C::Q_BLOCK + half * C::Q_PLANE) + pt_off(r, (d & 63) >> 3);
             };
-            const uint32_t q_a = base + (uint32_t)(2 * t * C::Q_PLANE);
+            const uint32_t q_a = base + (uint32_t)(2 * qt * C::Q_PLANE);
             constexpr int CPR = HDP / 4, RPC = 32 / CPR;  // 16-byte chunks of a row, rows at a time
             const int dc = (lane % CPR) * 4;
             const int64_t per_token = A.q_stride - (int64_t)G * HD;  // rows of a token are consecutive
             const float* const q0 = A.q + (int64_t)sg.s.q0 * A.q_stride + (int64_t)sg.hk * G * HD + dc;
-            const int first_row = sg.row0 + 128 * t;
+            const int first_row = sg.row0 + 128 * qt;
             const FastDiv group = w.group;
 #pragma unroll 4
             for (int i = 0; i < 32; i += RPC) {
@@ -428,41 +486,127 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                 }
             }
             pt_fence_async();
-            mbar_arrive(&bar.q_full[t]);
+            mbar_arrive(&bar.q_full[qt]);
             return mine;
         };
-        bool more = next();
-        float next_scale = more ? stage_q(it) : 0.f;
+        // SPLIT: by the second group, whose registers are free then, the rows that there are spread over
+        // its warps (the others' scores are not used).  The rows' factors, powers of two, go to sh_scale.
+        [[maybe_unused]] auto stage_split = [&](const Segment& sg, uint32_t seg) {
+            // (small loops: it is met once a segment, and its instructions come from far then)
+            constexpr int LPR = HDP / 8, RPI = 32 / LPR, CPR = HDP / 4, RPC = 32 / CPR;
+            if (sg.kt0 == sg.kt1) return;
+            const int d = (lane % LPR) * 8, dc = (lane % CPR) * 4, w4 = warp & 3;
+            // 16 bytes of the values d .. of row r: FP16 hi, lo; FP32 the first four's hi, the others'
+            // (their lo parts Q_PLANE behind)
+            auto place = [&](int r, int d, int half) -> uint32_t {
+                if constexpr (F32)
+                    return (uint32_t)((d >> 5) * C::Q_BLOCK) + pt_off(r, ((d & 31) >> 2) + half);
+                else
+                    return (uint32_t)((d >> 6) * C::Q_BLOCK + half * C::Q_PLANE) + pt_off(r, (d & 63) >> 3);
+            };
+            const int64_t per_token = A.q_stride - (int64_t)G * HD;  // rows of a token are consecutive
+            const float* const q0 = A.q + (int64_t)sg.s.q0 * A.q_stride + (int64_t)sg.hk * G * HD + dc;
+            const FastDiv group = w.group;
+            // warp w4 has rows RPI (w4 + 4 i) .. + RPI
+#pragma unroll 1
+            for (int r0 = w4 * RPI; r0 < sg.rows; r0 += 4 * RPI)
+#pragma unroll
+                for (int i = 0; i < RPI; i += RPC) {
+                    const int r = r0 + i + lane / CPR, row = sg.row0 + r;
+                    const bool there = r < sg.rows && dc < HD;
+                    const int64_t at = (int64_t)row * HD + (int64_t)group.div((uint32_t)row) * per_token;
+                    cp16(base + place(r, dc & ~7, (dc >> 2) & 1), q0 + (there ? at : 0), there);
+                }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+#pragma unroll 1
+            for (int r0 = w4 * RPI; r0 < sg.rows; r0 += 4 * RPI) {
+                const int r = r0 + lane / LPR;
+                uint4* const at0 = reinterpret_cast<uint4*>(q_ptr + place(r, d, 0));
+                uint4* const at1 = reinterpret_cast<uint4*>(q_ptr + place(r, d, 1));
+                const float4 x0 = *reinterpret_cast<const float4*>(at0);
+                const float4 x1 = *reinterpret_cast<const float4*>(at1);
+                uint4 h, l;
+                if constexpr (F32) {
+                    split_tf32(x0.x * sign, h.x, l.x), split_tf32(x0.y * sign, h.y, l.y);
+                    split_tf32(x0.z * sign, h.z, l.z), split_tf32(x0.w * sign, h.w, l.w);
+                    *at0 = h, at0[C::Q_PLANE / 16] = l;
+                    split_tf32(x1.x * sign, h.x, l.x), split_tf32(x1.y * sign, h.y, l.y);
+                    split_tf32(x1.z * sign, h.z, l.z), split_tf32(x1.w * sign, h.w, l.w);
+                    *at1 = h, at1[C::Q_PLANE / 16] = l;
+                } else {
+                    float top = fmaxf(fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x0.z), fabsf(x0.w))),
+                                      fmaxf(fmaxf(fabsf(x1.x), fabsf(x1.y)), fmaxf(fabsf(x1.z), fabsf(x1.w))));
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    float down;
+                    const float up = pow2_scale(top, down) * sign;
+                    split2(x0.x * up, x0.y * up, h.x, l.x), split2(x0.z * up, x0.w * up, h.y, l.y);
+                    split2(x1.x * up, x1.y * up, h.z, l.z), split2(x1.z * up, x1.w * up, h.w, l.w);
+                    *at0 = h, *at1 = l;
+                    if (d == 0) sh_scale[seg & 1][r] = (uint8_t)(__float_as_uint(down) >> 23);
+                }
+            }
+            pt_fence_async();
+            mbar_arrive(&bar.q_full[0]);
+        };
+        bool more = first;
+        float next_scale = 1.f;
+        if (!SPLIT && more) next_scale = stage_q(it);
         while (ok && more) {
             const Segment cur = it;
             const int n_kt = cur.kt1 - cur.kt0;
-            const int rows = cur.rows - 128 * t;  // of this query tile
+            const int rows = cur.rows - 128 * qt;  // of this query tile
             const uint32_t first = seen;
             seen += (uint32_t)n_kt;
+            if constexpr (SPLIT) {
+                if (t == 1) {
+                    // q's place is free once the last segment's scores are done, where the first group's came
+                    // last: this group has waited for its own
+                    if (q_used >= 0) ok = wait(&bar.s_full[0], q_used);
+                    q_used = -1;
+                    if (ok) stage_split(cur, segs);
+                }
+                firsts += n_kt / 2;
+                if (n_kt > 0 && !(n_kt & 1)) q_used = firsts - 1;
+            }
             // scores are multiplied by this; kept off zero, where -inf would turn into NaN
-            const float sc = fmaxf(fabsf(A.scale_log2) * next_scale, 1e-37f);
-            if (rows <= 0 || n_kt == 0) {
+            float sc = fmaxf(fabsf(A.scale_log2) * next_scale, 1e-37f);
+            if (!SPLIT && rows <= 0) {
                 more = next();
                 if (more) next_scale = stage_q(it);
-                if (rows <= 0) continue;
+                continue;
             }
             const int r = wr + lane;
-            const int row = cur.row0 + 128 * t + r;  // of the sequence
+            const int row = cur.row0 + 128 * qt + r;  // of the sequence
             const int lim = r < rows ? cur.start + (int)w.group.div((uint32_t)row) : -1;
-            const int first_lim = all_see<TREE>(cur.start, cur.row0 + 128 * t, G);
+            const int first_lim = all_see<TREE>(cur.start, cur.row0 + 128 * qt, G);
             [[maybe_unused]] const uint32_t* nodes = nullptr;
             if constexpr (TREE) nodes = mask_row(A, cur.s.q0, row, r < rows);
             float acc[HDP];
 #pragma unroll
             for (int d = 0; d < HDP; ++d) acc[d] = 0.f;
             float m = -INFINITY, l = 0.f, c_last = 1.f;
+            // SPLIT: sc, from what the second group has left
+            [[maybe_unused]] auto row_scale = [&]() -> float {
+                if constexpr (!SPLIT || F32) return sc;
+                else
+                    return fmaxf(fabsf(A.scale_log2) * __uint_as_float((uint32_t)sh_scale[segs & 1][r] << 23),
+                                 1e-37f);
+            };
+            // trees: the masks' bits of the key tile, read ahead of its scores; they serve until its O
+            [[maybe_unused]] uint32_t tree_see[TREE ? KT / 32 : 1];
             // positions of key tile j (of the segment) that this row sees and that have a page
             auto visible = [&](int j, int word) -> uint32_t {
                 const int n = lim + 1 - ((cur.kt0 + j) * KT + 32 * word);
                 uint32_t below = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-                if constexpr (TREE)
-                    below &= tree_bits(nodes, A.words, (cur.kt0 + j) * KT + 32 * word - cur.start);
-                const uint16_t* gone = sh_gone[(first + j) & 3];
+                if constexpr (TREE) {
+#pragma unroll
+                    for (int i = 0; i < KT / 32; ++i)
+                        if (i == word) below &= tree_see[i];
+                }
+                const uint16_t* gone = sh_gone[(first + j) & (RECENT - 1)];
                 return below & ~((uint32_t)gone[2 * word] | ((uint32_t)gone[2 * word + 1] << 16));
             };
             // O of key tile j into the running sum
@@ -482,8 +626,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                 if ((cur.kt0 + j) * KT + KT - 1 > all_see<TREE>(cur.start, cur.row0, G)) {
                     // where some row does not see all of the tile, V was made finite: rows that
                     // see such a position are not
-                    const uint16_t* bad16 = sh_bad[(first + j) & 3];
-                    const auto& bad32 = sh_bad32[(first + j) & 3];
+                    const uint16_t* bad16 = sh_bad[(first + j) & (RECENT - 1)];
+                    const auto& bad32 = sh_bad32[(first + j) & (RECENT - 1)];
 #pragma unroll
                     for (int i = 0; i < KT / 32; ++i) {
                         uint32_t bad;
@@ -497,14 +641,31 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                     }
                 }
             };
-            for (int j = 0; j < n_kt && ok; ++j) {
-                if (j > 0) add_o(j - 1);
+            // (each step of the code has one place: a CTA meets it for the first time a few times only, and
+            // its instructions come from far then)
+            for (int j = j0;; j += DJ) {
+                const bool end = j >= n_kt || !ok;
+                if (end) {
+                    more = next();
+                    // the next segment's q goes in while the last O is computed; its first scores follow
+                    if (!SPLIT && more) next_scale = stage_q(it);
+                }
+                if (j > j0 && ok) add_o(j - DJ);
+                if (end) break;
+                if constexpr (TREE) {
+                    const int p0 = (cur.kt0 + j) * KT;
+#pragma unroll
+                    for (int i = 0; i < KT / 32; ++i)
+                        tree_see[i] = p0 + KT > cur.start ? tree_bits(nodes, A.words, p0 + 32 * i - cur.start)
+                                                          : 0xffffffffu;
+                }
                 ok = wait(&bar.s_full[t], tiles) && ok;
                 ++tiles;
                 pt_fence_after();
+                if (SPLIT && j == j0) sc = row_scale();
                 bool all = (cur.kt0 + j) * KT + KT - 1 <= first_lim && r < rows;
                 {
-                    const uint4 gone = *reinterpret_cast<const uint4*>(sh_gone[(first + j) & 3]);
+                    const uint4 gone = *reinterpret_cast<const uint4*>(sh_gone[(first + j) & (RECENT - 1)]);
                     all = all && (gone.x | (KT > 32 ? gone.y : 0) | (KT > 64 ? gone.z | gone.w : 0)) == 0;
                 }
                 all = __all_sync(0xffffffffu, all);
@@ -588,24 +749,70 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                 pt_fence_before();
                 mbar_arrive(&bar.p_full[t]);
             }
-            // the next segment's q goes in while the last O is computed; its first scores follow
-            if (n_kt > 0 && ok) {
-                more = next();
-                if (more) next_scale = stage_q(it);
-                add_o(n_kt - 1);
-                mbar_arrive(&bar.seg_done[t]);
+            if (n_kt > j0 && ok) mbar_arrive(&bar.seg_done[t]);
+            if constexpr (SPLIT) {
+                if (n_kt > 0 && ok) {
+                    if (t == 1) {
+#pragma unroll
+                        for (int d0 = 0; d0 < HDP; d0 += 16) {
+                            uint32_t y[16];
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) y[d] = __float_as_uint(acc[d0 + d]);
+                            pt_st16(o_at + d0, y);
+                        }
+                        if constexpr (C::ML < 0) sh_ml[r] = make_float2(m, l);
+                        else pt_st2(ml_at, m, l);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        pt_fence_before();
+                        mbar_arrive(&bar.x_there);
+                    } else {
+                        ok = wait(&bar.x_there, exchanges++);
+                        pt_fence_after();
+                        sc = row_scale();  // (it may have had no key tile)
+                        float2 y;
+                        if constexpr (C::ML < 0) y = sh_ml[r];
+                        else y = pt_read2(ml_at);
+                        const float top = fmaxf(m, y.x);
+                        const float f = top == -INFINITY ? 1.f : ex2((m - top) * sc);
+                        const float g = top == -INFINITY ? 1.f : ex2((y.x - top) * sc);
+                        m = top;
+                        l = l * f + y.y * g;
+#pragma unroll
+                        for (int d0 = 0; d0 < HDP; d0 += 32) {
+                            float o[32];
+                            pt_read32(o_at + 128 + d0, o);
+#pragma unroll
+                            for (int d = 0; d < 32; ++d) acc[d0 + d] = fmaf(acc[d0 + d], f, o[d] * g);
+                        }
+                        pt_fence_before();
+                        mbar_arrive(&bar.x_done);
+                    }
+                }
+                ++segs;
+                if (t == 1) continue;
             }
             if (r < rows && ok) {  // a row per thread
                 const bool whole = cur.part < 0;
-                const int64_t at = (int64_t)cur.part * C::R + 128 * t + r;
+                const int64_t at = (int64_t)cur.part * C::R + 128 * qt + r;
                 const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                float* p = whole ? out_row(A, cur, G, row) : part_at(A, cur.part, 128 * t + r, 0);
+                float* p = whole ? out_row(A, cur, G, row) : part_at(A, cur.part, 128 * qt + r, 0);
                 const int step = whole ? 4 : 4 * C::R;
+                if (SPLIT && whole && A.sectors) {  // whole sectors of 32 bytes
 #pragma unroll
-                for (int d = 0; d < HDP; d += 4, p += step)
-                    if (d < HD)
-                        *reinterpret_cast<float4*>(p) =
-                            make_float4(acc[d] * f, acc[d + 1] * f, acc[d + 2] * f, acc[d + 3] * f);
+                    for (int d = 0; d < HDP; d += 8, p += 8)
+                        if (d < HD)
+                            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p),
+                                         "f"(acc[d] * f), "f"(acc[d + 1] * f), "f"(acc[d + 2] * f),
+                                         "f"(acc[d + 3] * f), "f"(acc[d + 4] * f), "f"(acc[d + 5] * f),
+                                         "f"(acc[d + 6] * f), "f"(acc[d + 7] * f)
+                                         : "memory");
+                } else {
+#pragma unroll
+                    for (int d = 0; d < HDP; d += 4, p += step)
+                        if (d < HD)
+                            *reinterpret_cast<float4*>(p) =
+                                make_float4(acc[d] * f, acc[d + 1] * f, acc[d + 2] * f, acc[d + 3] * f);
+                }
                 if (!whole) A.part_ml[at] = make_float2(m * sc, l);
             }
         }
@@ -615,7 +822,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             // ---- MMAs ----
             constexpr uint32_t id_s = pt_idesc(128, KT, false, F32), id_o = pt_idesc(128, HDP, !F32, F32);
             int half = 0;               // K and V tiles so far: the ring's order
-            int n_q[2] = {0, 0}, n_s[2] = {0, 0};  // q tiles (segments) and key tiles so far
+            // q tiles (segments) and key tiles so far; SPLIT: q tiles, then segments of the two groups
+            int n_q[3] = {0, 0, 0}, n_s[2] = {0, 0};
             // A segment's last sh_gone and sh_bad are read after its last MMA: the next segment's
             // second key tile waits for that, before the copies come round to them.
             uint32_t owed = 0;  // of which query tiles
@@ -625,7 +833,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             // FP16: lo k, hi k.  FP32: lo hi, hi lo, hi hi (pass 0, 1, 2).
             constexpr int PASSES = F32 ? 3 : 2;
             auto scores = [&](int t, uint32_t k_at) {
-                const uint32_t q_at = base + (uint32_t)(2 * t * C::Q_PLANE);
+                const uint32_t q_at = base + (uint32_t)(SPLIT ? 0 : 2 * t * C::Q_PLANE);
                 uint32_t add = 0;
 #pragma unroll 1
                 for (int pass = 0; pass < PASSES; ++pass) {
@@ -662,14 +870,80 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                     }
                 }
             };
-            while (ok && next()) {
+            [[maybe_unused]] int exchanges = 0;
+            [[maybe_unused]] bool x_owed = false;
+            // SPLIT: the next slot, how often it has been used, its place
+            [[maybe_unused]] int slot = 0, uses = 0;
+            [[maybe_unused]] uint32_t slot_a = ring;
+            [[maybe_unused]] auto advance = [&]() {
+                ++slot, slot_a += C::TILE;
+                if (slot == C::SLOTS) slot = 0, slot_a = ring, ++uses;
+            };
+            bool begun = false;
+            while (ok && go_on(begun)) {
                 const int n_kt = it.kt1 - it.kt0, n_t = it.rows > 128 ? 2 : 1;
                 if (n_kt == 0) continue;
                 auto slot_at = [&](int h) { return ring + (uint32_t)((h % C::SLOTS) * C::TILE); };
                 auto arrived = [&](int h) {
                     ok = ok && wait(&bar.kv_full[h % C::SLOTS], h / C::SLOTS);
-                    pt_fence_async();  // written by cp.async and stores, read by the tensor core
+                    // written by cp.async, read by the tensor core (stores are followed by a fence of their
+                    // own, TMA needs none)
+                    if (!SPLIT || (!F32 && !TA.box)) pt_fence_async();
                 };
+                if constexpr (SPLIT) {
+                    // Every K and V tile once, in the ring's order: O of key tile j, then the scores of key tile
+                    // j + 2 in the same columns.  Both tiles are waited for before O, so that between the two
+                    // the tensor core has the next MMA in time (4.0k cycles a key tile without that).
+#pragma unroll 1
+                    for (int j = -2; j < n_kt && ok; ++j) {
+                        const bool s = j + 2 < n_kt;
+                        const int t = ~j & 1;
+                        uint64_t* empty_v = nullptr;
+                        uint32_t v_at = 0;
+                        if (j >= 0) {
+                            ok = wait(&bar.kv_full[slot], uses);
+                            empty_v = &bar.kv_empty[slot], v_at = slot_a;
+                            advance();
+                        }
+                        if (s) ok = ok && wait(&bar.kv_full[slot], uses);
+                        if (!SPLIT || (!F32 && !TA.box)) pt_fence_async();  // written by cp.async
+                        if (j >= 0) {
+                            if (j == 0) {  // the last segment's masks and its second group's sums have been read
+#pragma unroll 1
+                                for (int g = 0; g < 2; ++g, owed >>= 1)
+                                    if (owed & 1) ok = ok && wait(&bar.seg_done[g], n_q[1 + g]++);
+                                if (x_owed) ok = ok && wait(&bar.x_done, exchanges++);
+                            }
+                            const int n = t ? n_s[1]++ : n_s[0]++;
+                            ok = ok && wait(F32 ? &bar.p_full[t] : &bar.p_half[t], n);
+                            pt_fence_after();
+                            if (ok) {
+                                if constexpr (!F32) {
+                                    outputs(t, v_at, 1);
+                                    ok = wait(&bar.p_full[t], n);
+                                    pt_fence_after();
+                                }
+                                if (ok) outputs(t, v_at, 0);
+                                pt_commit(&bar.o_full[t], leader);
+                                pt_commit(empty_v, leader);
+                            }
+                        }
+                        if (s) {
+                            if (j == -2) ok = ok && wait(&bar.q_full[0], n_q[0]++);
+                            pt_fence_after();
+                            if (ok) {
+                                scores(t, slot_a);
+                                pt_commit(&bar.s_full[t], leader);
+                                pt_commit(&bar.kv_empty[slot], leader);
+                            }
+                            advance();
+                        }
+                        __syncwarp();
+                    }
+                    owed = n_kt > 1 ? 3 : 2;
+                    x_owed = true;
+                    continue;
+                }
                 arrived(half);
                 for (int t = 0; t < n_t && ok; ++t) {
                     ok = wait(&bar.q_full[t], n_q[t]++);
@@ -730,13 +1004,14 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             const bool in_row = x * 16 < row_bytes;
             const uint8_t* const src_x[2] = {(const uint8_t*)A.k + x * 16, (const uint8_t*)A.v + x * 16};
             const int box = TA.box, box_row = (lane / BLOCKS) << box, box_col = lane % BLOCKS;
-            const bool has_box = box && box_row < KT;
+            const bool has_box = box && box_row < KT && (SPLIT || lw == 0);
             int half = 0;
-            uint32_t tile_no = 0;
+            uint32_t seg_tile = 0;
             Looks looks;  // at V tiles, each on a barrier of its slot
             bool looking = false;  // such a wait ran out
             bool ok = true;
-            while (ok && next()) {
+            bool begun = false;
+            while (ok && go_on(begun)) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
                 const int first_lim = all_see<TREE>(it.start, it.row0, G);
                 if (lw == 1) {  // the softmax warps ask for the segment's q soon
@@ -753,40 +1028,67 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                     const int page = page_at(w, it.s.row[col]);
                     return page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
                 };
-                for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
-                    const bool careful = kt * KT + KT - 1 > first_lim;
-                    int box_at = -1, rows3[3] = {-1, -1, -1};
-                    if (lw == 0 && has_box) box_at = row_of(kt * KT + box_row);
-                    if (!box) {
-#pragma unroll
-                        for (int i = 0; i < 3; ++i)
-                            if (lw + 3 * i < 8)
-                                rows3[i] = row_of(kt * KT + (lw + 3 * i) * 16 + (lane & 15));
-                    }
+                const int n_kt = it.kt1 - it.kt0;
+                int box_at = -1, rows3[3] = {-1, -1, -1};
+                // SPLIT with TMA: the warps see to a tile in turn (starting the 16 copies of one takes a
+                // warp 2.8k cycles, as long as the MMAs and the softmax need for it), each with the table
+                // entries of its next one on their way
+                auto entry = [&](int e) -> int {
+                    const int pos = (it.kt0 + (tile_order<SPLIT>(e, n_kt) >> 1)) * KT + box_row;
+                    return has_box && e < 2 * n_kt && pos <= last_lim ? it.s.row[w.ps.div((uint32_t)pos)] : -1;
+                };
+                int turn = half % 3 <= lw ? lw - half % 3 : 3 + lw - half % 3;  // this warp's next
+                [[maybe_unused]] int soon = SPLIT && box ? entry(turn) : -1;
 #pragma unroll 1
-                    for (int kv = 0; kv < 2 && ok; ++kv, ++half) {
+                for (int e = 0; e < 2 * n_kt && ok; ++e, ++half) {
+                    const int of = tile_order<SPLIT>(e, n_kt), j = of >> 1, kt = it.kt0 + j, kv = of & 1;
+                    const uint32_t tile_no = seg_tile + (uint32_t)j;
+                    const bool careful = kt * KT + KT - 1 > first_lim;
+                    const bool mine = !SPLIT || !box || e == turn;
+                    if (SPLIT && box) {
+                        if (!mine) {
+                            if (kv == 1 && careful) looks.take(half % C::SLOTS);  // the phases of all looks count
+                            continue;
+                        }
+                        const int page = page_at(w, soon), pos = kt * KT + box_row;
+                        box_at = page < 0 ? -1
+                                          : (page * w.Hkv + it.hk) * w.page_size +
+                                                (pos - (int)w.ps.div((uint32_t)pos) * w.page_size);
+                        turn += 3;
+                        soon = entry(turn);
+                    } else if (SPLIT || kv == 0) {  // (else V: those of K)
+                        if (has_box) box_at = row_of(kt * KT + box_row);
+                        if (!box) {
+#pragma unroll
+                            for (int i = 0; i < 3; ++i)
+                                if (lw + 3 * i < 8)
+                                    rows3[i] = row_of(kt * KT + (lw + 3 * i) * 16 + (lane & 15));
+                        }
+                    }
+                    {
                         const int slot = half % C::SLOTS, use = half / C::SLOTS;
                         if (use > 0 && !wait(&bar.kv_empty[slot], use - 1)) {
                             ok = false;
-                            break;
+                            break;  // (half is not counted)
                         }
                         const bool look = kv == 1 && careful;  // V to be looked through
                         const uint32_t tile_at = ring + (uint32_t)(slot * C::TILE);
                         if (box) {
                             uint64_t* const there =
                                 look ? &bar.v_there[Looks::bar(slot)] : &bar.kv_full[slot];
-                            if (lw == 0) {
+                            if (SPLIT || lw == 0) {
+                                // (before the arrival, which is the tile's only one with SPLIT)
+                                if (has_box && kv == 0 && box_col == 0)
+                                    for (int b = 0; b < 1 << (box - 3); ++b)
+                                        reinterpret_cast<uint8_t*>(sh_gone[tile_no & (RECENT - 1)])[box_row / 8 + b] =
+                                            box_at < 0 ? 0xff : 0;
+                                __syncwarp();
                                 if (lane == 0) mbar_arrive_expect_tx(there, C::TILE);
                                 __syncwarp();
-                                if (has_box) {
+                                if (has_box)
                                     pt_tma(tile_at + (uint32_t)(box_col * C::K_BLOCK + box_row * 128),
                                            kv ? &TA.v : &TA.k, box_col * 64, box_at < 0 ? -KT : box_at,
                                            there);
-                                    if (kv == 0 && box_col == 0)
-                                        for (int b = 0; b < 1 << (box - 3); ++b)
-                                            reinterpret_cast<uint8_t*>(sh_gone[tile_no & 3])[box_row / 8 + b] =
-                                                box_at < 0 ? 0xff : 0;
-                                }
                             }
                             if (look && !wait(&bar.v_there[Looks::bar(slot)], looks.take(slot))) {
                                 ok = false, looking = true;
@@ -810,7 +1112,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                                          src + (there ? (int64_t)n * row_bytes : 0), there);
                                 }
                                 const uint32_t none = __ballot_sync(0xffffffffu, row < 0) & 0xffffu;
-                                if (kv == 0 && lane == 0) sh_gone[tile_no & 3][g16] = (uint16_t)none;
+                                if (kv == 0 && lane == 0) sh_gone[tile_no & (RECENT - 1)][g16] = (uint16_t)none;
                             }
                             if (look) {
                                 asm volatile("cp.async.wait_all;" ::: "memory");
@@ -819,8 +1121,30 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         }
                         if (look) {
                             uint8_t* const tile = base_ptr + (tile_at - base);
+                            if (SPLIT && box) {
+                                // is there any such value at all?  0 x is 0 for every other one (two FP16 values an
+                                // instruction; with the loop below alone one warp took 24k cycles for a tile)
+                                const __half2 zero = __floats2half2_rn(0.f, 0.f);
+                                __half2 any[4] = {zero, zero, zero, zero};
+#pragma unroll 4
+                                for (int i = lane; i < C::TILE / 16; i += 32) {
+                                    const uint4 v = *reinterpret_cast<const uint4*>(tile + i * 16);
+                                    const __half2* const x = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) any[k] = __hfma2(x[k], zero, any[k]);
+                                }
+                                uint32_t bits = 0;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) bits |= *reinterpret_cast<const uint32_t*>(&any[k]);
+                                if (!__any_sync(0xffffffffu, (bits & 0x7fff7fffu) != 0)) {
+                                    if (lane < 8) sh_bad[tile_no & (RECENT - 1)][lane] = 0;
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive(&bar.kv_full[slot]);
+                                    continue;
+                                }
+                            }
 #pragma unroll 1
-                            for (int g16 = lw; g16 < 8; g16 += 3) {
+                            for (int g16 = SPLIT && box ? 0 : lw; g16 < 8; g16 += SPLIT && box ? 1 : 3) {
                                 uint32_t bad = 0;
 #pragma unroll 4
                                 for (int k = 0; k < 4 * BLOCKS; ++k) {  // four rows of a block
@@ -836,9 +1160,15 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                                         for (int r = 0; r < 4; ++r)
                                             if (any & (0xffu << (8 * r))) bad |= 1u << ((k & 3) * 4 + r);
                                 }
-                                if (lane == 0) sh_bad[tile_no & 3][g16] = (uint16_t)bad;
+                                if (lane == 0) sh_bad[tile_no & (RECENT - 1)][g16] = (uint16_t)bad;
                             }
                             pt_fence_async();
+                        }
+                        if (SPLIT && box) {
+                            // (else the bytes' arrival is the one)
+                            __syncwarp();
+                            if (lane == 0 && look) mbar_arrive(&bar.kv_full[slot]);
+                            continue;
                         }
                         // 33 arrivals a warp, whichever way: with TMA one of them is the bytes'
                         if (box || look) mbar_arrive(&bar.kv_full[slot]);
@@ -851,6 +1181,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         if (lane == 0 && !(box && !look && lw == 0)) mbar_arrive(&bar.kv_full[slot]);
                     }
                 }
+                seg_tile += (uint32_t)n_kt;
             }
             // no copy may still be landing when the CTA ends
             asm volatile("cp.async.wait_all;" ::: "memory");
@@ -866,7 +1197,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             int issued = 0;  // key tiles
             RawSent sent;
             bool ok = true;
-            while (ok && next()) {
+            bool begun = false;
+            while (ok && go_on(begun)) {
                 const int last_lim = it.start + (it.row0 + it.rows - 1) / G;
                 auto row_of = [&](int kt, int row) -> int {  // in the layer; -1: no page, or not seen
                     const int pos = kt * KT + row;
@@ -875,14 +1207,66 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                     const int page = page_at(w, it.s.row[col]);
                     return page < 0 ? -1 : (page * w.Hkv + it.hk) * w.page_size + (pos - col * w.page_size);
                 };
-                int at = row_of(it.kt0, box_row);
+                const int n_kt = it.kt1 - it.kt0;
+                int at = SPLIT ? -1 : row_of(it.kt0, box_row);
                 // the softmax warps ask for the segment's q soon
                 for (int r = lane; r < it.rows; r += 32) {
                     const uint8_t* p = (const uint8_t*)q_row(A, it, G, it.row0 + r);
                     for (int b = 0; b < HD * 4; b += 128)
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
                 }
-                for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++issued) {
+                if constexpr (SPLIT) {
+                    // table entries of the next two key tiles, on their way, and the rows of the last two
+                    auto entry = [&](int j, int row) -> int {
+                        const int pos = (it.kt0 + j) * KT + row;
+                        return row < KT && j < n_kt && pos <= last_lim ? it.s.row[w.ps.div((uint32_t)pos)] : -1;
+                    };
+                    auto layer_row = [&](int e, int j, int row) -> int {
+                        const int pos = (it.kt0 + j) * KT + row, page = page_at(w, e);
+                        return page < 0 ? -1
+                                        : (page * w.Hkv + it.hk) * w.page_size +
+                                              (pos - (int)w.ps.div((uint32_t)pos) * w.page_size);
+                    };
+                    int soon[2] = {entry(0, box_row), entry(1, box_row)}, rows[2] = {-1, -1};
+                    int soon2[2] = {-1, -1}, rows2[2] = {-1, -1};
+                    if (singles) soon2[0] = entry(0, lane + 32), soon2[1] = entry(1, lane + 32);
+#pragma unroll 1
+                    for (int e = 0; e < 2 * n_kt && ok; ++e) {
+                        const int of = tile_order<true>(e, n_kt), j = of >> 1, kv = of & 1;
+                        if (kv == 0) {
+                            rows[0] = rows[1], rows[1] = layer_row(soon[0], j, box_row);
+                            soon[0] = soon[1], soon[1] = entry(j + 2, box_row);
+                            if (singles) {
+                                rows2[0] = rows2[1], rows2[1] = layer_row(soon2[0], j, lane + 32);
+                                soon2[0] = soon2[1], soon2[1] = entry(j + 2, lane + 32);
+                            }
+                        }
+                        const bool newest = kv == 0 || j == n_kt - 1;
+                        at = newest ? rows[1] : rows[0];
+                        const int at2 = newest ? rows2[1] : rows2[0];
+                        uint64_t none = __ballot_sync(0xffffffffu, has_box && at < 0);
+                        if (singles) none |= (uint64_t)__ballot_sync(0xffffffffu, at2 < 0) << 32;
+                        uint32_t gone = 0;  // of positions 16 lane ..
+                        if (none)
+                            for (int r = 0; r < 16; ++r)
+                                gone |= (uint32_t)((none >> (((lane * 16 + r) >> box) & 63)) & 1) << r;
+                        const int n = issued + j;  // of its kind
+                        if (n > 0) ok = wait(&bar.raw_empty[kv], n - 1);
+                        if (!ok) break;
+                        if (kv == 0 && lane < KT / 16) sh_gone[n & (RECENT - 1)][lane] = (uint16_t)gone;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[kv], C::PLANE);
+                        sent.add(kv);
+                        __syncwarp();
+                        const uint32_t to = raw_a + (uint32_t)(kv * C::PLANE + box_row * HDP * 4);
+                        const CUtensorMap* const map = kv ? &TA.v : &TA.k;
+                        if (has_box) pt_tma(to, map, 0, at < 0 ? -KT : at, &bar.raw_full[kv]);
+                        if (singles)
+                            pt_tma(to + 32 * HDP * 4, map, 0, at2 < 0 ? -KT : at2, &bar.raw_full[kv]);
+                    }
+                    issued += n_kt;
+                }
+                for (int kt = SPLIT ? it.kt1 : it.kt0; kt < it.kt1 && ok; ++kt, ++issued) {
                     const int at_next = row_of(kt + 1, box_row);
                     uint64_t none = __ballot_sync(0xffffffffu, has_box && at < 0);
                     int at2 = -1;
@@ -898,7 +1282,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                     for (int kv = 0; kv < 2 && ok; ++kv) {
                         if (issued > 0) ok = wait(&bar.raw_empty[kv], issued - 1);
                         if (!ok) break;
-                        if (kv == 0 && lane < KT / 16) sh_gone[issued & 3][lane] = (uint16_t)gone;
+                        if (kv == 0 && lane < KT / 16) sh_gone[issued & (RECENT - 1)][lane] = (uint16_t)gone;
                         __syncwarp();
                         if (lane == 0) mbar_arrive_expect_tx(&bar.raw_full[kv], C::PLANE);
                         sent.add(kv);
@@ -921,14 +1305,18 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
             const int sw = warp - 10;
             const uint8_t* const raw_ptr = base_ptr + (ring - base) + C::SLOTS * C::TILE;
             int half = 0;
-            uint32_t tile_no = 0;
+            uint32_t seg_tile = 0;
             bool ok = true;
-            while (ok && next()) {
+            bool begun = false;
+            while (ok && go_on(begun)) {
                 const int first_lim = all_see<TREE>(it.start, it.row0, G);
-                for (int kt = it.kt0; kt < it.kt1 && ok; ++kt, ++tile_no) {
-                    const bool careful = kt * KT + KT - 1 > first_lim;
+                const int n_kt = it.kt1 - it.kt0;
 #pragma unroll 1
-                    for (int kv = 0; kv < 2; ++kv, ++half) {
+                for (int e = 0; e < 2 * n_kt && ok; ++e, ++half) {
+                    const int of = tile_order<SPLIT>(e, n_kt), kt = it.kt0 + (of >> 1), kv = of & 1;
+                    const uint32_t tile_no = seg_tile + (uint32_t)(of >> 1);
+                    const bool careful = kt * KT + KT - 1 > first_lim;
+                    {
                         const int slot = half % C::SLOTS, use = half / C::SLOTS;
                         ok = wait(&bar.raw_full[kv], (int)tile_no);
                         if (use > 0) ok = ok && wait(&bar.kv_empty[slot], use - 1);
@@ -978,8 +1366,8 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                                 *reinterpret_cast<uint4*>(at + C::PLANE) = l;
                             }
                             if (lane == 0) {
-                                sh_bad32[tile_no & 3][sw][0] = bad0;
-                                sh_bad32[tile_no & 3][sw][1] = bad1;
+                                sh_bad32[tile_no & (RECENT - 1)][sw][0] = bad0;
+                                sh_bad32[tile_no & (RECENT - 1)][sw][1] = bad1;
                             }
                         }
                         pt_fence_async();
@@ -991,6 +1379,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP>::THREADS, 1)
                         }
                     }
                 }
+                seg_tile += (uint32_t)n_kt;
             }
         }
     }
@@ -1039,20 +1428,25 @@ static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head
     return IB_OK;
 }
 
-template <typename KV>
+template <typename KV, bool TREE>
 CutRule tensor_rule(int head_dim, int min_rows, int max_rows) {
     // one CTA to an SM, a piece for each
-    using S = TensorCfg<KV, 64>;
-    using L = TensorCfg<KV, 128>;
-    return head_dim <= 64 ? CutRule{S::R, S::KT, min_rows, max_rows, kSMs, 128}
-                          : CutRule{L::R, L::KT, min_rows, max_rows, kSMs, 128};
+    using S = TensorCfg<KV, 64, TREE>;
+    using L = TensorCfg<KV, 128, TREE>;
+    CutRule r = head_dim <= 64 ? CutRule{S::R, S::KT, min_rows, max_rows, kSMs, 128}
+                               : CutRule{L::R, L::KT, min_rows, max_rows, kSMs, 128};
+    if (TREE) r.flat = true;
+    if (TREE) r.fixed = 800;
+    return r;
 }
-template CutRule tensor_rule<float>(int, int, int);
-template CutRule tensor_rule<__half>(int, int, int);
+template CutRule tensor_rule<float, false>(int, int, int);
+template CutRule tensor_rule<__half, false>(int, int, int);
+template CutRule tensor_rule<float, true>(int, int, int);
+template CutRule tensor_rule<__half, true>(int, int, int);
 
 template <typename KV, int HDP, bool TREE>
 static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
-    using C = TensorCfg<KV, HDP>;
+    using C = TensorCfg<KV, HDP, TREE>;
     auto kern = attn_tensor_kernel<KV, HDP, TREE>;
     TensorArgs t{};
     t.rows = a;
