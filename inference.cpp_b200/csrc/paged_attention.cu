@@ -1138,7 +1138,11 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
         const int narrow = few ? 0 : NARROW;
         if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
         CutRule r;
-        if constexpr (on_tcgen05<HDP>) r = tensor_rule<KV, TREE>(p->head_dim, narrow + 1, ALL);
+        // trees: two query tiles that share their key tiles where the sequences fill them on average, one
+        // elsewhere (two long documents of 33 to 63 nodes, FP32 pages: 181 us with two tiles, 203 with one; 32
+        // trees of 12 to 24 nodes, FP16: 213 and 133).  FP32 pages at head_dim above 64 have one anyway.
+        const bool split = TREE && ((sizeof(KV) == 4 && HDP == 128) || rows <= 128 * seqs);
+        if constexpr (on_tcgen05<HDP>) r = tensor_rule<KV, TREE>(p->head_dim, narrow + 1, ALL, split);
         else r = wide_rule<KV, HDP>(narrow + 1, ALL);
         add(r, seqs + rows / r.R);
     }

@@ -19,6 +19,7 @@ struct CutRule {
     int fixed = 0;  // positions that beginning a tile costs as much as (pieces)
     // trees: every tile of a sequence costs the same, whole key tiles
     bool flat = false;
+    bool split = false;  // tcgen05: one query tile, its key tiles shared out (paged_tensor.cu)
     __device__ __forceinline__ int slope() const { return flat ? 0 : R; }
 };
 
@@ -400,7 +401,7 @@ __device__ __forceinline__ float pow2_scale(float top, float& inverse) {
 
 // Tiles of many rows on tcgen05, for head_dim up to 128 (paged_tensor.cu).
 template <typename KV, bool TREE>
-CutRule tensor_rule(int head_dim, int min_rows, int max_rows);
+CutRule tensor_rule(int head_dim, int min_rows, int max_rows, bool split);
 template <typename KV, bool TREE>
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st);
 int paged_tensor_fault_take(int* code);

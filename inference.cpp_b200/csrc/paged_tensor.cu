@@ -303,11 +303,10 @@ __device__ __forceinline__ int tile_order(int e, int n) {
     return e & 1 ? e + 1 : e - 1;  // K of e / 2 + 1/2, V of e / 2 - 1
 }
 
-template <typename KV, int HDP, bool TREE>
-__global__ void __launch_bounds__(TensorCfg<KV, HDP, TREE>::THREADS, 1)
+template <typename KV, int HDP, bool TREE, bool SPLIT>
+__global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
     attn_tensor_kernel(const __grid_constant__ TensorArgs TA) {
     const RowsArgs& A = TA.rows;
-    constexpr bool SPLIT = TREE;
     using C = TensorCfg<KV, HDP, SPLIT>;
     constexpr bool F32 = C::F32;
     constexpr int KT = C::KT;
@@ -1428,26 +1427,37 @@ static int tensor_map(CUtensorMap* map, const void* base, int64_t rows, int head
     return IB_OK;
 }
 
-template <typename KV, bool TREE>
-CutRule tensor_rule(int head_dim, int min_rows, int max_rows) {
+template <typename KV, bool SPLIT>
+static CutRule rule_of(int head_dim, int min_rows, int max_rows) {
     // one CTA to an SM, a piece for each
-    using S = TensorCfg<KV, 64, TREE>;
-    using L = TensorCfg<KV, 128, TREE>;
-    CutRule r = head_dim <= 64 ? CutRule{S::R, S::KT, min_rows, max_rows, kSMs, 128}
-                               : CutRule{L::R, L::KT, min_rows, max_rows, kSMs, 128};
-    if (TREE) r.flat = true;
-    if (TREE) r.fixed = 800;
+    using S = TensorCfg<KV, 64, SPLIT>;
+    using L = TensorCfg<KV, 128, SPLIT>;
+    return head_dim <= 64 ? CutRule{S::R, S::KT, min_rows, max_rows, kSMs, 128}
+                          : CutRule{L::R, L::KT, min_rows, max_rows, kSMs, 128};
+}
+template <typename KV, bool TREE>
+CutRule tensor_rule(int head_dim, int min_rows, int max_rows, bool split) {
+    CutRule r = split ? rule_of<KV, true>(head_dim, min_rows, max_rows)
+                      : rule_of<KV, false>(head_dim, min_rows, max_rows);
+    if (TREE) {
+        // beginning a tile takes some 20k cycles, six key tiles' time: 32 trees of 12 to 24 nodes over
+        // 200 .. 4096 positions take 173 us with pieces of equal positions, 139 with 400 more to each
+        // tile, 132 with 700, 137 with 1500
+        r.flat = true;
+        r.fixed = 800;
+        r.split = split;
+    }
     return r;
 }
-template CutRule tensor_rule<float, false>(int, int, int);
-template CutRule tensor_rule<__half, false>(int, int, int);
-template CutRule tensor_rule<float, true>(int, int, int);
-template CutRule tensor_rule<__half, true>(int, int, int);
+template CutRule tensor_rule<float, false>(int, int, int, bool);
+template CutRule tensor_rule<__half, false>(int, int, int, bool);
+template CutRule tensor_rule<float, true>(int, int, int, bool);
+template CutRule tensor_rule<__half, true>(int, int, int, bool);
 
-template <typename KV, int HDP, bool TREE>
+template <typename KV, int HDP, bool TREE, bool SPLIT>
 static int launch(const RowsArgs& a, int64_t grid, cudaStream_t st) {
-    using C = TensorCfg<KV, HDP, TREE>;
-    auto kern = attn_tensor_kernel<KV, HDP, TREE>;
+    using C = TensorCfg<KV, HDP, SPLIT>;
+    auto kern = attn_tensor_kernel<KV, HDP, TREE, SPLIT>;
     TensorArgs t{};
     t.rows = a;
     const PagedView& w = a.w;
@@ -1473,7 +1483,11 @@ template <typename KV, bool TREE>
 int attn_tensor_launch(const RowsArgs& a, int64_t tiles, int64_t max_pos, cudaStream_t st) {
     const int64_t most = tiles * (max_pos / a.rule.least + 1 + a.rule.R);
     const int64_t grid = std::min<int64_t>(a.rule.n_pieces, most);
-    return a.w.HD <= 64 ? launch<KV, 64, TREE>(a, grid, st) : launch<KV, 128, TREE>(a, grid, st);
+    if constexpr (TREE) {
+        if (a.rule.split)
+            return a.w.HD <= 64 ? launch<KV, 64, true, true>(a, grid, st) : launch<KV, 128, true, true>(a, grid, st);
+    }
+    return a.w.HD <= 64 ? launch<KV, 64, TREE, false>(a, grid, st) : launch<KV, 128, TREE, false>(a, grid, st);
 }
 template int attn_tensor_launch<float, false>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
 template int attn_tensor_launch<__half, false>(const RowsArgs&, int64_t, int64_t, cudaStream_t);
