@@ -56,20 +56,31 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// A number that at least k of the CTA's threads' `best` reach, where that many are above 0: the least
-// of the warps' n-th largest, n = k / BS_WARPS rounded up.  (The k-th largest of all would let fewer
-// values pass, and costs a sort: with this one about k (1 + 1/2 + 1/3 .. 1/8) pass for k = 8.)
-__device__ __forceinline__ uint32_t reached(uint32_t best, int k, uint32_t (&sh)[BS_WARPS]) {
+// A number that at least k of the CTA's threads' `best` reach, where that many are above 0 (else 0).  First
+// the least of the warps' n-th largest, n = k / BS_WARPS rounded up; then, where many more reach it,
+// halving between it and the largest of all, a barrier a step, until a quarter more than k do or a few
+// steps are over.  n: how many reach it.
+__device__ __forceinline__ uint32_t reached(uint32_t best, int k, uint32_t (&sh)[2][BS_WARPS], int& n) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t top = 0;
-    for (int n = (k + BS_WARPS - 1) / BS_WARPS; n > 0; --n) {
-        top = __reduce_max_sync(0xffffffffu, best);
-        if (lane == __ffs(__ballot_sync(0xffffffffu, best == top)) - 1) best = 0;
+    uint32_t top = 0, most = 0, x = best;
+    for (int i = (k + BS_WARPS - 1) / BS_WARPS; i > 0; --i) {
+        top = __reduce_max_sync(0xffffffffu, x);
+        most = max(most, top);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, x == top)) - 1) x = 0;
     }
-    if (lane == 0) sh[warp] = top;
+    if (lane == 0) sh[0][warp] = top, sh[1][warp] = most;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < BS_WARPS; ++i) top = min(top, sh[i]);
+    for (int i = 0; i < BS_WARPS; ++i) top = min(top, sh[0][i]), most = max(most, sh[1][i]);
+    top = max(top, 1u);  // (a warp may have none)
+    n = __syncthreads_count(best >= top);
+    if (n < k) return 0;
+    for (int turn = 0; n > k + k / 4 && most - top > 1 && turn < 32; ++turn) {
+        const uint32_t half = top + (most - top) / 2;
+        const int c = __syncthreads_count(best >= half);
+        if (c >= k) top = half, n = c;
+        else most = half;
+    }
     return top;
 }
 
@@ -86,11 +97,19 @@ struct SelectArgs {
     const int32_t* ended;    // null: none
     int rows, beams, vocab, k, slices, end_token;
     int64_t per_slice;       // values
+    FastDiv of_k, of_slices;
     uint64_t* list;          // [row][slice][k] keys, largest first, zeros behind
     SliceMeta* meta;         // [row][slice]
     float* out_score;        // [group][k]
     int32_t *out_token, *out_row;
 };
+
+// e^t for t <= 0: 2^(t log2 e) with log2 e in two parts (one alone is 1e-8 short, for all values alike).
+__device__ __forceinline__ float exp_of(float t) {
+    float y = fmaf(t, 1.925963033e-8f, t * 1.442695022f);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+    return y;
+}
 
 template <typename T>
 __device__ __forceinline__ float logit(T x) {
@@ -110,7 +129,7 @@ struct SliceShared {
 // Every thread of the CTA calls it, after a barrier.
 __device__ __forceinline__ void rank_best(SliceShared& sh, int n, int k, uint64_t* __restrict__ out) {
     const int tid = threadIdx.x;
-    if (n > 2 * k && n > BS_THREADS) {  // a threshold again, of what has passed the first
+    if (n > 3 * k && n > 64) {  // a threshold again, of what has passed the first
         constexpr int N = BS_CAP / BS_THREADS;
         uint64_t key[N], best = 0;
 #pragma unroll
@@ -119,7 +138,8 @@ __device__ __forceinline__ void rank_best(SliceShared& sh, int n, int k, uint64_
             key[i] = at < n ? sh.buf[at] : 0;
             best = key[i] > best ? key[i] : best;
         }
-        const uint32_t least = reached((uint32_t)(best >> 32), k, sh.top[1]);
+        int reach;
+        const uint32_t least = reached((uint32_t)(best >> 32), k, sh.top, reach);
         if (tid == 0) sh.n = 0;
         __syncthreads();
 #pragma unroll
@@ -131,6 +151,7 @@ __device__ __forceinline__ void rank_best(SliceShared& sh, int n, int k, uint64_
     for (int i = tid; i < n; i += BS_THREADS) {
         const uint64_t mine = sh.buf[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j) rank += sh.buf[j] > mine;
         if (rank < k) out[rank] = mine;
     }
@@ -183,7 +204,8 @@ __device__ __noinline__ void slice_again(SliceShared& sh, const T* x, int64_t be
     rank_best(sh, sh.n, k, out);
 }
 
-template <typename T>
+// VEC: values of one load (16 bytes where the rows allow it, else one).
+template <typename T, int VEC>
 __global__ void __launch_bounds__(BS_THREADS) beam_slice_kernel(const __grid_constant__ SelectArgs A) {
     __shared__ SliceShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -194,42 +216,59 @@ __global__ void __launch_bounds__(BS_THREADS) beam_slice_kernel(const __grid_con
     const int begin = (int)(slice * A.per_slice), end = (int)min((int64_t)A.vocab, begin + A.per_slice);
     if (tid == 0) sh.n = 0;
     float m = -INFINITY, sum = 0.f, least = 0.f;
-    for (int at = begin; at < end; at += BS_TILE) {
-        float v[16];
-        const T* const p = x + at + tid;
-        if (at + BS_TILE <= end) {
+    // value i of the thread's is token at + place(i)
+    auto place = [&](int i) { return (i / VEC * BS_THREADS + tid) * VEC + i % VEC; };
+    struct alignas(16) Values {
+        T x[16];
+    };
+    auto load = [&](int at, Values& y) {
+        const T* const p = x + at;
+        if (VEC > 1 && at + BS_TILE <= end) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = logit(p[i * BS_THREADS]);
+            for (int i = 0; i < 16; i += VEC)
+                *reinterpret_cast<uint4*>(y.x + i) = __ldg(reinterpret_cast<const uint4*>(p + place(i)));
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                v[i] = at + i * BS_THREADS + tid < end ? logit(p[i * BS_THREADS]) : -INFINITY;
+            for (int i = 0; i < 16; ++i) y.x[i] = at + place(i) < end ? p[place(i)] : (T)-INFINITY;
         }
+    };
+    Values now;
+    load(begin, now);
+    for (int at = begin; at < end; at += BS_TILE) {
+        Values next;  // on its way while this one is looked at
+        if (at + BS_TILE < end) load(at + BS_TILE, next);
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = logit(now.x[i]);
         float top = v[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, v[i]);  // (a NaN only where there is nothing else)
         if (at == begin) {
-            const uint32_t o = reached(top > -INFINITY ? ordered(top) : 0, A.k, sh.top[0]);
+            int n;
+            const uint32_t o = reached(top > -INFINITY ? ordered(top) : 0, A.k, sh.top, n);
             // the value itself; where not enough threads have one, all that are no -inf pass
-            least = o ? __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o) : -FLT_MAX;
+            least = o > ordered(-FLT_MAX) ? __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o) : -FLT_MAX;
         }
         if (top > m) {
             sum *= expf(m - top);
             m = top;
         }
         const float base = m > -INFINITY ? m : 0.f;  // e^-inf is 0, and a NaN stays one
+        float more[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += expf(v[i] - base);
+        for (int i = 0; i < 16; ++i) more[i & 3] += exp_of(v[i] - base);
+        sum += (more[0] + more[1]) + (more[2] + more[3]);
         if (top >= least) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (v[i] >= least) {
                     const int to = atomicAdd(&sh.n, 1);
-                    if (to < BS_CAP) sh.buf[to] = beam_key(v[i], (uint32_t)(at + i * BS_THREADS + tid));
+                    if (to < BS_CAP) sh.buf[to] = beam_key(v[i], (uint32_t)(at + place(i)));
                 }
         }
+        now = next;
     }
-    const int64_t place = (int64_t)row * A.slices + slice;
+    const int64_t list = (int64_t)row * A.slices + slice;
     // the slice's maximum and sum
     float M = m;
 #pragma unroll
@@ -243,12 +282,12 @@ __global__ void __launch_bounds__(BS_THREADS) beam_slice_kernel(const __grid_con
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) sh.sum[warp] = d;
     const int n = sh.n;
-    if (n <= BS_CAP) rank_best(sh, n, A.k, A.list + place * A.k);
-    else slice_again(sh, x, (int64_t)begin, (int64_t)end, A.k, A.list + place * A.k);
+    if (n <= BS_CAP) rank_best(sh, n, A.k, A.list + list * A.k);
+    else slice_again(sh, x, (int64_t)begin, (int64_t)end, A.k, A.list + list * A.k);
     __syncthreads();
     if (tid == 0) {
         for (int i = 1; i < BS_WARPS; ++i) d += sh.sum[i];
-        A.meta[place] = SliceMeta{M, 0.f, d};
+        A.meta[list] = SliceMeta{M, 0.f, d};
     }
 }
 
@@ -270,15 +309,16 @@ __device__ __forceinline__ void put_choice(const SelectArgs& A, int g, int j, co
     A.out_row[at] = any ? g * A.beams + (int32_t)(y.place >> 32) : -1;
 }
 
-// Candidate c of group g: entry c % k of list c / k, a row's slice; v is -inf where there is none.  base:
-// score - log sum e^(x - M), and M.
-__device__ __forceinline__ Best candidate(const SelectArgs& A, int g, int c, const double2* base) {
-    const int l = c / A.k, b = l / A.slices;
+// Candidate c of group g, whose key is `key`: entry c % k of list c / k, a row's slice; v is -inf where
+// there is none.  base: score - log sum e^(x - M), and M; M is NaN for a row that has ended.
+__device__ __forceinline__ Best candidate(const SelectArgs& A, int c, uint64_t key, const double2* base) {
+    const int b = (int)A.of_slices.div(A.of_k.div((uint32_t)c));
+    const double2 y0 = base[b];
     Best y = {-INFINITY, ~0ull};
-    if (A.ended && A.ended[g * A.beams + b]) {
-        if (c == b * A.slices * A.k) y = Best{base[b].x, ((uint64_t)b << 32) | (uint32_t)A.end_token};
-    } else if (const uint64_t key = A.list[(int64_t)g * A.beams * A.slices * A.k + c]) {
-        y = Best{base[b].x + ((double)key_value(key) - base[b].y), ((uint64_t)b << 32) | key_place(key)};
+    if (y0.y != y0.y) {
+        if (c == b * A.slices * A.k) y = Best{y0.x, ((uint64_t)b << 32) | (uint32_t)A.end_token};
+    } else if (key) {
+        y = Best{y0.x + ((double)key_value(key) - y0.y), ((uint64_t)b << 32) | key_place(key)};
     }
     if (!(y.v > -INFINITY)) y.v = -INFINITY;  // NaN is no candidate
     return y;
@@ -286,7 +326,8 @@ __device__ __forceinline__ Best candidate(const SelectArgs& A, int g, int c, con
 
 // The group's choice where too many candidates reached the threshold: k rounds of a maximum over the CTA,
 // each behind the last one's.
-__device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, const double2* base) {
+__device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, const uint64_t* list,
+                                         const double2* base) {
     __shared__ Best sh_best[2][BS_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Best last = {INFINITY, 0};
@@ -294,7 +335,7 @@ __device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, cons
     for (int j = 0; j < A.k; ++j, first = false) {
         Best top = {-INFINITY, ~0ull};
         for (int c = tid; c < n; c += BS_THREADS) {
-            const Best y = candidate(A, g, c, base);
+            const Best y = candidate(A, c, list[c], base);
             if ((first || better(last, y)) && better(y, top)) top = y;
         }
 #pragma unroll
@@ -318,11 +359,17 @@ __device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, cons
 __global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_constant__ SelectArgs A) {
     extern __shared__ __align__(16) double2 base[];  // [beams]
     __shared__ Best buf[BS_GROUP_CAP];
-    __shared__ uint32_t sh_top[BS_WARPS];
+    __shared__ uint32_t sh_top[2][BS_WARPS];
     __shared__ int sh_n;
     const int tid = threadIdx.x, g = blockIdx.x, row0 = g * A.beams, k = A.k;
     if (tid == 0) sh_n = 0;
+    const int n = A.beams * A.slices * k;
+    const uint64_t* const list = A.list + (int64_t)g * n;
     pdl_wait();
+    constexpr int AHEAD = 4;  // a thread's first keys, on their way meanwhile
+    uint64_t key[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) key[i] = tid + i * BS_THREADS < n ? list[tid + i * BS_THREADS] : 0;
     // as many lanes to a row as it has slices
     int lanes = 1;
     while (lanes < 32 && lanes < A.slices) lanes *= 2;
@@ -331,45 +378,56 @@ __global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_con
         const int b = b0 + tid / lanes, row = row0 + b;
         const bool there = b < A.beams, end = there && A.ended && A.ended[row];
         const SliceMeta* const meta = A.meta + (int64_t)row * A.slices;
-        const int n = there && !end ? A.slices : 0;
+        const int slices = there && !end ? A.slices : 0;
         float M = -INFINITY;
         double s = 0;
-        for (int i = sub; i < n; i += lanes) M = fmaxf(M, meta[i].m);
+        for (int i = sub; i < slices; i += lanes) M = fmaxf(M, meta[i].m);
         for (int o = lanes / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        for (int i = sub; i < n; i += lanes) {
+        for (int i = sub; i < slices; i += lanes) {
             const SliceMeta y = meta[i];
             s += y.m > -INFINITY ? y.sum * exp((double)y.m - (double)M) : y.sum;
         }
         for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         // (a row of nothing but -inf has no candidates)
         if (there && sub == 0)
-            base[b] = make_double2((A.scores ? (double)A.scores[row] : 0.0) - (end ? 0.0 : log(s)), end ? 0.0 : (double)M);
+            base[b] = make_double2((A.scores ? (double)A.scores[row] : 0.0) - (end ? 0.0 : log(s)), end ? (double)NAN : (double)M);
     }
     __syncthreads();
-    const int n = A.beams * A.slices * k;
     // rounding down keeps the order, so that k values at or above it are above all below it
     auto low = [](double v) { return v > -INFINITY ? ordered(__double2float_rd(v)) : 0u; };
     uint32_t best = 0;
-    for (int c = tid; c < n; c += BS_THREADS) best = max(best, low(candidate(A, g, c, base).v));
-    const uint32_t least = max(reached(best, k, sh_top), 1u);
-    for (int c = tid; c < n; c += BS_THREADS) {
-        const Best y = candidate(A, g, c, base);
-        if (low(y.v) >= least) {
-            const int to = atomicAdd(&sh_n, 1);
-            if (to < BS_GROUP_CAP) buf[to] = y;
-        }
+    Best mine[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        const int c = tid + i * BS_THREADS;
+        mine[i] = Best{-INFINITY, ~0ull};
+        if (c < n) mine[i] = candidate(A, c, key[i], base);
+        best = max(best, low(mine[i].v));
     }
+    for (int c = tid + AHEAD * BS_THREADS; c < n; c += BS_THREADS)
+        best = max(best, low(candidate(A, c, list[c], base).v));
+    int reach;
+    const uint32_t least = max(reached(best, k, sh_top, reach), 1u);
+    auto take = [&](const Best& y) {
+        if (low(y.v) < least) return;
+        const int to = atomicAdd(&sh_n, 1);
+        if (to < BS_GROUP_CAP) buf[to] = y;
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) take(mine[i]);
+    for (int c = tid + AHEAD * BS_THREADS; c < n; c += BS_THREADS) take(candidate(A, c, list[c], base));
     __syncthreads();
     const int some = sh_n;
     if (some > BS_GROUP_CAP) {
-        group_again(A, g, n, base);
+        group_again(A, g, n, list, base);
         return;
     }
     for (int i = tid; i < some; i += BS_THREADS) {
-        const Best mine = buf[i];
+        const Best own = buf[i];
         int rank = 0;
-        for (int j = 0; j < some; ++j) rank += better(buf[j], mine);
-        if (rank < k) put_choice(A, g, rank, mine);
+#pragma unroll 4
+        for (int j = 0; j < some; ++j) rank += better(buf[j], own);
+        if (rank < k) put_choice(A, g, rank, own);
     }
     for (int j = some + tid; j < k; j += BS_THREADS) put_choice(A, g, j, Best{-INFINITY, ~0ull});
 }
@@ -445,6 +503,8 @@ extern "C" int ib_beam_select(int type, const void* logits, int64_t stride, cons
     a.slices = p.slices;
     a.end_token = end_token;
     a.per_slice = p.per_slice;
+    a.of_k = FastDiv::make((uint32_t)k);
+    a.of_slices = FastDiv::make((uint32_t)p.slices);
     a.list = reinterpret_cast<uint64_t*>((uint8_t*)workspace + p.list_off);
     a.meta = reinterpret_cast<SliceMeta*>((uint8_t*)workspace + p.meta_off);
     a.out_score = out_score;
@@ -452,8 +512,11 @@ extern "C" int ib_beam_select(int type, const void* logits, int64_t stride, cons
     a.out_row = out_row;
     cudaStream_t st = as_stream(stream);
     const dim3 grid((unsigned)(rows * p.slices));
-    IB_CUDA_CHECK(launch_pdl(type == IB_TYPE_F32 ? beam_slice_kernel<float> : beam_slice_kernel<__half>, grid,
-                             dim3(BS_THREADS), 0, st, false, a));
+    const int64_t size = type == IB_TYPE_F32 ? 4 : 2;
+    const bool wide = (((uintptr_t)logits | (uintptr_t)(rows > 1 ? stride * size : 0)) & 15) == 0;
+    auto* const slice = type == IB_TYPE_F32 ? (wide ? beam_slice_kernel<float, 4> : beam_slice_kernel<float, 1>)
+                                            : (wide ? beam_slice_kernel<__half, 8> : beam_slice_kernel<__half, 1>);
+    IB_CUDA_CHECK(launch_pdl(slice, grid, dim3(BS_THREADS), 0, st, false, a));
     const size_t smem = (size_t)beams * sizeof(double2);
     IB_CUDA_CHECK(launch_pdl(beam_group_kernel, dim3(n_groups), dim3(BS_THREADS), smem, st, true, a));
     return IB_OK;
