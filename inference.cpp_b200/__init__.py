@@ -663,6 +663,9 @@ def _seqs_of(pages, seqs):
 
 def _paged_list(pages, t, name, n):
     """Pointer of a contiguous int32 list of n entries on the pages' device."""
+    if t.dtype is _torch().int32 and t.shape == (n,) and t.device == pages.device \
+            and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype != _torch().int32:
         raise ValueError(f"{name}: dtype {t.dtype}, expected torch.int32")
     if t.dim() != 1 or t.shape[0] != n:
@@ -725,6 +728,8 @@ def kv_release(pages, seqs, slots, stream=None):
 
 def _workspace(pages, workspace):
     """(pointer, bytes) of a caller's workspace on the pages' device."""
+    if workspace.device == pages.device and workspace.is_contiguous():
+        return workspace.data_ptr(), workspace.nbytes
     if workspace.device != pages.device or not workspace.is_contiguous():
         raise ValueError(f"workspace: on {workspace.device}, contiguous "
                          f"{workspace.is_contiguous()}; expected contiguous on {pages.device}")
@@ -983,10 +988,10 @@ class BeamChoice(typing.NamedTuple):
 
 def _beam_shape(logits, beams, k):
     """(type, rows, vocab, groups, k) of a selection."""
-    torch = _torch()
-    type_ = {torch.float32: F32, torch.float16: F16}.get(logits.dtype)
+    torch, dtype = _torch(), logits.dtype
+    type_ = F32 if dtype is torch.float32 else F16 if dtype is torch.float16 else None
     if type_ is None or logits.dim() != 2 or not logits.is_cuda:
-        raise ValueError(f"logits: {logits.dtype} {tuple(logits.shape)} on {logits.device}, expected "
+        raise ValueError(f"logits: {dtype} {tuple(logits.shape)} on {logits.device}, expected "
                          f"float32 or float16 [rows, vocab] on a CUDA device")
     rows, vocab = logits.shape
     if beams < 1 or rows % beams:
@@ -1005,6 +1010,14 @@ def beam_select_workspace(logits, beams=1, k=None):
     return _torch().empty(n, dtype=_torch().uint8, device=logits.device)
 
 
+def _beam_ptr(t, name, dtype, shape, dev):
+    if t is None:
+        return None
+    if not (t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous()):
+        _paged_tensor(t, name, dtype, shape, dev)
+    return t.data_ptr()
+
+
 def beam_select(logits, scores=None, beams=1, k=None, ended=None, end_token=0, out=None,
                 workspace=None, stream=None):
     """The k (default: beams) best continuations of each group of `beams` rows of the logits [rows,
@@ -1015,26 +1028,22 @@ def beam_select(logits, scores=None, beams=1, k=None, ended=None, end_token=0, o
     workspace: beam_select_workspace(), allocated for the call when None."""
     torch = _torch()
     type_, rows, vocab, groups, k = _beam_shape(logits, beams, k)
-    dev = logits.device
+    dev, f32, i32 = logits.device, torch.float32, torch.int32
     st = _paged_stream(logits, stream)
     if out is None or workspace is None:
         with _allocating(logits, stream):
             if out is None:
                 out = BeamChoice(torch.empty(groups, k, device=dev),
-                                 *(torch.empty(groups, k, dtype=torch.int32, device=dev)
-                                   for _ in range(2)))
+                                 *(torch.empty(groups, k, dtype=i32, device=dev) for _ in range(2)))
             if workspace is None:
                 workspace = beam_select_workspace(logits, beams, k)
-    for t, name, dtype, shape in ((scores, "scores", torch.float32, (rows,)),
-                                  (ended, "ended", torch.int32, (rows,)),
-                                  (out.score, "out.score", torch.float32, (groups, k)),
-                                  (out.token, "out.token", torch.int32, (groups, k)),
-                                  (out.row, "out.row", torch.int32, (groups, k))):
-        if t is not None:
-            _paged_tensor(t, name, dtype, shape, dev)
+    score, token, row = out
+    per_row, per_group = (rows,), (groups, k)
     _call("ib_beam_select", type_, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
-          _ptr(scores), _ptr(ended), end_token, groups, beams, vocab, k, out.score.data_ptr(),
-          out.token.data_ptr(), out.row.data_ptr(), *_workspace(logits, workspace), st)
+          _beam_ptr(scores, "scores", f32, per_row, dev), _beam_ptr(ended, "ended", i32, per_row, dev),
+          end_token, groups, beams, vocab, k, _beam_ptr(score, "out.score", f32, per_group, dev),
+          _beam_ptr(token, "out.token", i32, per_group, dev),
+          _beam_ptr(row, "out.row", i32, per_group, dev), *_workspace(logits, workspace), st)
     return out
 
 
