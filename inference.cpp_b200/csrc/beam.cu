@@ -18,7 +18,7 @@
 #include <string>
 
 #include "common.cuh"
-#include "paged.cuh"
+#include "paged.cuh"  // FastDiv, checks
 #include "pdl.cuh"
 
 namespace ib {
@@ -491,6 +491,19 @@ extern "C" int ib_beam_select(int type, const void* logits, int64_t stride, cons
     const SelectPlan p = select_plan(rows, vocab, k);
     if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.bytes)
         return paged_refuse(who, "workspace missing, too small or not 256-byte aligned");
+    {
+        const int64_t size = type == IB_TYPE_F32 ? 4 : 2, out = (int64_t)n_groups * k * 4;
+        const void* const to[4] = {out_score, out_token, out_row, workspace};
+        const int64_t to_n[4] = {out, out, out, (int64_t)p.bytes};
+        bool bad = false;
+        for (int i = 0; i < 4; ++i) {
+            bad = bad || bytes_meet(to[i], to_n[i], logits, ((rows - 1) * stride + vocab) * size);
+            bad = bad || (scores && bytes_meet(to[i], to_n[i], scores, rows * 4));
+            bad = bad || (ended && bytes_meet(to[i], to_n[i], ended, rows * 4));
+            for (int j = 0; j < i; ++j) bad = bad || bytes_meet(to[i], to_n[i], to[j], to_n[j]);
+        }
+        if (bad) return paged_refuse(who, "results and workspace must not overlap the inputs or one another");
+    }
     SelectArgs a{};
     a.logits = logits;
     a.stride = stride;

@@ -948,6 +948,9 @@ extern "C" int ib_kv_reorder(const ib_kv_pages* pages, const ib_kv_seqs* seqs, i
     const size_t need = reorder_ws(seqs, n, workspace, &ws);
     if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < need)
         return paged_refuse(who, "workspace missing, too small or not 256-byte aligned");
+    for (const void* list : {(const void*)slots, (const void*)parents, (const void*)status})
+        if (bytes_meet(workspace, (int64_t)need, list, 4 * (int64_t)n))
+            return paged_refuse(who, "the workspace must not overlap the lists");
     const KvSeqsDev s = seqs_dev(pages, seqs);
     cudaStream_t st = as_stream(stream);
     kv_reorder_rows_kernel<<<n, KV_COPY_THREADS, 0, st>>>(s, n, slots, parents, ws);

@@ -163,6 +163,10 @@ int paged_refuse(const char* who, const char* what);  // sets the error, returns
 // (rows of different strides: whether their whole ranges meet).
 bool paged_rows_overlap(const float* a, int64_t sa, int64_t wa, const float* b, int64_t sb, int64_t wb,
                         int64_t n);
+// Whether [a, a + na) and [b, b + nb) share a byte.
+static inline bool bytes_meet(const void* a, int64_t na, const void* b, int64_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
 PagedView paged_view(const ib_kv_pages* p, const ib_kv_seqs* s, const ib_kv_batch* b, int n_heads,
                      const ib_kv_tree* t = nullptr);
 int paged_fault_take(int* code);            // paged.cu

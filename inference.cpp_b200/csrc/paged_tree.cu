@@ -202,7 +202,7 @@ static int tree_batch(const ib_kv_batch* b, const char* who) {
 
 // Whether [a, a + na) and [b, b + nb) of 32-bit values share any.
 static bool meet(const void* a, int64_t na, const void* b, int64_t nb) {
-    return (uintptr_t)a < (uintptr_t)b + 4 * nb && (uintptr_t)b < (uintptr_t)a + 4 * na;
+    return bytes_meet(a, 4 * na, b, 4 * nb);
 }
 
 }  // namespace ib
