@@ -1,7 +1,7 @@
 // Bookkeeping of the copies in paged_tensor.cu, without CUDA so that every order of events can be
 // gone through on the host (tests/cpp/copy_ring_test.cpp).
 //
-// Looks.  // K and V tiles go through a ring of slots in turn.  A V tile that has to be looked through
+// Looks.  K and V tiles go through a ring of slots in turn.  A V tile that has to be looked through
 // completes on a look barrier first: warp 9 arms it, all copying warps wait for it, look through
 // their share and only then arrive on the slot's "full" barrier.  Waits go by a phase's parity, so
 // a barrier may not be armed again before every warp has passed its last phase.  With one barrier
@@ -19,6 +19,21 @@
 #endif
 
 namespace ib {
+
+// K and V tiles of a segment of n key tiles in the order in which they are used: the e-th is K (even) or V
+// (odd) of key tile tile_order(e, n) / 2.  SPLIT (one query tile, two groups of softmax warps that take its
+// key tiles in turn): K0 K1 V0 K2 V1 K3 ..; otherwise K0 V0 K1 V1 ..
+template <bool SPLIT>
+IB_RING_FN int tile_order(int e, int n) {
+    if (!SPLIT) return e;
+    if (e < 2) return e == 0 ? 0 : n > 1 ? 2 : 1;
+    if (e >= 2 * n - 2) return 2 * (e - n) + 1;
+    return e & 1 ? e + 1 : e - 1;  // K of e / 2 + 1/2, V of e / 2 - 1
+}
+
+// Which of the three copying warps sees to a tile by itself (SPLIT with TMA): the ring's tiles in turn.  A
+// look is its warp's alone then, but the phases of all looks at a slot count: the others take them too.
+IB_RING_FN int tile_owner(int half) { return half % 3; }
 
 struct Looks {
     uint32_t parity = 0;  // of each barrier's next phase, a bit each

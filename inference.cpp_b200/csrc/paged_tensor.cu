@@ -293,16 +293,6 @@ struct TensorBars {
     uint64_t x_there, x_done;  // the second group's sums are in tensor memory; have been read
 };
 
-// K and V tiles of a segment of n key tiles in the order in which they are used: key tile 2 e or 2 e + 1
-// of tile number e.  SPLIT: K0 K1 V0 K2 V1 K3 ..
-template <bool SPLIT>
-__device__ __forceinline__ int tile_order(int e, int n) {
-    if constexpr (!SPLIT) return e;
-    if (e < 2) return e == 0 ? 0 : n > 1 ? 2 : 1;
-    if (e >= 2 * n - 2) return 2 * (e - n) + 1;
-    return e & 1 ? e + 1 : e - 1;  // K of e / 2 + 1/2, V of e / 2 - 1
-}
-
 template <typename KV, int HDP, bool TREE, bool SPLIT>
 __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
     attn_tensor_kernel(const __grid_constant__ TensorArgs TA) {
@@ -1036,7 +1026,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
                     const int pos = (it.kt0 + (tile_order<SPLIT>(e, n_kt) >> 1)) * KT + box_row;
                     return has_box && e < 2 * n_kt && pos <= last_lim ? it.s.row[w.ps.div((uint32_t)pos)] : -1;
                 };
-                int turn = half % 3 <= lw ? lw - half % 3 : 3 + lw - half % 3;  // this warp's next
+                int turn = (lw - tile_owner(half) + 3) % 3;  // this warp's next
                 [[maybe_unused]] int soon = SPLIT && box ? entry(turn) : -1;
 #pragma unroll 1
                 for (int e = 0; e < 2 * n_kt && ok; ++e, ++half) {

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from conftest import load_package
-from test_paged_cpu import BAD_BATCH, BAD_POOL, PTR, batch, pages, ref, seqs
+from test_paged_cpu import BAD_BATCH, BAD_POOL, PTR, _cpp, batch, pages, ref, seqs
 
 ib = load_package()
 FAR = PTR + (1 << 24)
@@ -219,3 +219,13 @@ def test_python_handles_refuse():
 def test_struct_layout():
     assert ctypes.sizeof(ib._CKVTree) == 24
     assert ib._CKVTree.depth.offset == 8 and ib._CKVTree.mask.offset == 16
+
+
+def test_roles_of_the_tree_kernel_come_to_their_ends(tmp_path):
+    """The programs of its warps in random orders: waits, slots, masks and looks as the kernel has them."""
+    assert "runs, 0 stuck, 0 faults" in _cpp(tmp_path, "split_ring_test")
+
+
+def test_the_search_finds_looks_that_are_not_counted(tmp_path):
+    """The same with warps that count only their own looks at a slot: some order never ends."""
+    assert "runs, 0 stuck, 0 faults" not in _cpp(tmp_path, "split_ring_test", "forget")
