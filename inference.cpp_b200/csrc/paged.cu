@@ -745,6 +745,7 @@ __global__ void __launch_bounds__(256)
                      const float* __restrict__ rope, int rope_len, const int32_t* __restrict__ depth,
                      KV* kpool, KV* vpool) {
     const int t = blockIdx.x;
+    if constexpr (TREE) pdl_wait();  // launched beside what comes before: the trees' plan, as a rule
     const int b = seq_of_token(w, t);
     if (b < 0) return;
     const SeqInfo s = seq_info(w, b);
@@ -1030,17 +1031,17 @@ static int kv_append(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_
     const int64_t layer_elems = pool_bytes(pages).layer_bytes / elem_bytes(pages);
     cudaStream_t st = as_stream(stream);
     auto launch = [&](auto* kern, auto* kpool, auto* vpool) {
-        kern<<<batch->n_tokens, 256, 0, st>>>(w, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride,
-                                              rope_table, rope_len, tree ? tree->depth : nullptr,
-                                              kpool + layer * layer_elems, vpool + layer * layer_elems);
+        return launch_pdl(kern, dim3(batch->n_tokens), dim3(256), 0, st, tree != nullptr, w, q, q_stride, k,
+                          k_stride, v, v_stride, q_out, q_out_stride, rope_table, rope_len,
+                          tree ? tree->depth : nullptr, kpool + layer * layer_elems,
+                          vpool + layer * layer_elems);
     };
     if (pages->type == IB_TYPE_F32)
-        launch(tree ? kv_append_kernel<float, true> : kv_append_kernel<float, false>, (float*)pages->k,
-               (float*)pages->v);
+        IB_CUDA_CHECK(launch(tree ? kv_append_kernel<float, true> : kv_append_kernel<float, false>,
+                             (float*)pages->k, (float*)pages->v));
     else
-        launch(tree ? kv_append_kernel<__half, true> : kv_append_kernel<__half, false>,
-               (__half*)pages->k, (__half*)pages->v);
-    IB_LAUNCH_CHECK("kv_append_kernel");
+        IB_CUDA_CHECK(launch(tree ? kv_append_kernel<__half, true> : kv_append_kernel<__half, false>,
+                             (__half*)pages->k, (__half*)pages->v));
     return IB_OK;
 }
 

@@ -28,6 +28,7 @@ __global__ void __launch_bounds__(TREE_THREADS)
                      const int32_t* __restrict__ parents, int max_nodes, int32_t* __restrict__ depth,
                      uint32_t* __restrict__ mask) {
     __shared__ int16_t up[IB_KV_MAX_NODES];
+    pdl_launch_dependents();
     int q0;
     const int n = tree_nodes(cu_q, slots, n_tokens, blockIdx.x, max_nodes, q0);
     for (int i = threadIdx.x; i < n; i += TREE_THREADS) {
