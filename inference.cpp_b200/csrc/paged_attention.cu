@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(WideCfg<KV, HDP>::NT)
     Piece piece = sh_piece;
     Segment it;
     const int G = w.H / w.Hkv, HD = w.HD;
-    while (next_segment(w, A.rule, piece, it)) {
+    while (next_segment<false>(w, A.rule, piece, it)) {
     const int row0 = it.row0, rows = it.rows, start = it.start;
     const int first_lim = all_see<TREE>(start, row0, G), last_lim = start + (row0 + rows - 1) / G;
     const int kt0 = it.kt0, kt1 = it.kt1;
@@ -941,85 +941,114 @@ __device__ __forceinline__ void join_parts(const JoinArgs& A, int item) {
 }
 
 // Tiles of many rows that find_piece cut, mostly in two: CTA (no, y) looks whether piece `no`
-// begins inside a tile, and is the first to do so there, and sees to its rows JOIN_ROWS y ...
+// begins inside a tile, and sees to its share of that tile's rows JOIN_ROWS y ..: as many CTAs as the
+// tile has cuts share it (one CTA took 44 us for trees of 230 rows over 12000 positions in eight parts).
 // All CTAs are on the SMs at once, since each has to plan first: with 32 rows to a CTA, four times
 // as many of them, the join of a mixed step took 36 us against 22 (cold caches).
 constexpr int JOIN_ROWS = 128, JOIN_THREADS = 512;
-static_assert(JOIN_THREADS == 4 * JOIN_ROWS, "");
-template <int HDP>
 __device__ __forceinline__ void join_pieces(const JoinArgs& A, int no, int y) {
     __shared__ Piece sh_piece;
     __shared__ int found;
     const PagedView& w = A.w;
+    const CutRule& rule = A.rule;
     const int tid = threadIdx.x;
-    const int G = w.H / w.Hkv, HD = w.HD, R = A.rule.R;
-    find_piece<JOIN_THREADS>(w, A.rule, no, &sh_piece, &found);
+    const int G = w.H / w.Hkv, HD = w.HD, R = rule.R;
+    find_piece<JOIN_THREADS>(w, rule, no, &sh_piece, &found);
     __syncthreads();
-    pdl_wait();
-    if (!found) return;
+    if (!found) return pdl_wait();
+    // the tile that the piece begins in
     Piece p = sh_piece;
-    Segment sg;
-    if (!next_segment(w, A.rule, p, sg)) return;
-    // the tile's work is [a, b), and pieces c0 .. c1 hold shares of it: the first one's is its last
+    const SeqInfo s = p.x.s;
+    const long long start_g = start_work(rule, s, G);
+    const TileAt t = tile_at<false>(w, rule, p, start_g);
+    // its work is [a, b), and pieces c0 .. c1 hold shares of it: the first one's is its last
     // segment (unless the tile begins with the piece), the others' is their first
-    const long long start_g = start_work(A.rule, sg.s, G);
-    const long long a = p.base + sg.hk * p.x.per_head + tiles_work(sg.tile, start_g, A.rule.slope());
-    const long long b = a + start_g + (long long)(sg.tile + 1) * A.rule.slope();
-    const int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
-    if (c0 != no - 1 || c1 >= A.rule.n_pieces) return;
-    const int n_parts = c1 - c0 + 1, first = 2 * c0 + (a == c0 * p.len ? 0 : 1);
-    // four lanes to a row: they read four times 16 bytes of eight rows, and write 64 of each
-    const int r = y * JOIN_ROWS + tid / 4, x = tid % 4, D4 = HD / 4;
-    if (r >= sg.rows) return;
-#pragma unroll 1
-    for (int d = x; d < HDP / 4; d += 16) {
-        float M = -INFINITY, l = 0.f;
-        float4 o[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-        for (int i = 0; i < n_parts; ++i) {
-            const int64_t part = i == 0 ? first : 2 * (c0 + i);
-            const float2 ml = A.part_ml[part * R + r];
-            float4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                v[k] = d + 4 * k < D4
-                           ? reinterpret_cast<const float4*>(A.part_acc)[(part * D4 + d + 4 * k) * R + r]
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float top = fmaxf(M, ml.x);
-            const float f = top == -INFINITY ? 1.f : ex2(M - top);
-            const float c = top == -INFINITY ? 1.f : ex2(ml.x - top);
-            M = top;
-            l = fmaf(l, f, c * ml.y);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                o[k].x = fmaf(o[k].x, f, c * v[k].x), o[k].y = fmaf(o[k].y, f, c * v[k].y);
-                o[k].z = fmaf(o[k].z, f, c * v[k].z), o[k].w = fmaf(o[k].w, f, c * v[k].w);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (d + 4 * k < D4) join_store(A, sg.s, sg.hk, sg.row0 + r, d + 4 * k, o[k], l);
+    const long long a = p.at - t.x0, b = a + t.all;
+    int c0 = (int)(a / p.len), c1 = (int)((b - 1) / p.len);
+    if (c0 == no || c1 >= rule.n_pieces) return pdl_wait();
+    const int share = no - c0 - 1, shares = c1 - c0;
+    const int first = 2 * c0 + (a == c0 * p.len ? 0 : 1), first_piece = c0;
+    const int row0 = t.tile * R, rows = min(R, s.n * G - row0);
+    if (rule.flat) {  // shares at its ends may be empty
+        const int nkt = seen_tiles(rule, s.L - s.n, row0, rows, G);
+        while (c0 < c1 && flat_cut(rule, (c0 + 1) * p.len - a, G, nkt) == 0) ++c0;
+        while (c0 < c1 && flat_cut(rule, c1 * p.len - a, G, nkt) == nkt) --c1;
+        if (c0 == c1) return pdl_wait();
     }
+    // A thread to 32 bytes of a row, four to 128, eight rows to a warp: the parts lie that way.
+    const int lg = R < JOIN_ROWS ? 6 : 7, y0 = y * JOIN_ROWS, D4 = HD / 4;
+    const int n = (HD + 31) / 32 * 4 << lg, begin = n * share / shares, end = n * (share + 1) / shares;
+    auto join = [&](auto units) {  // U of them at a time, so that enough is on its way
+        constexpr int U = decltype(units)::value;
+#pragma unroll 1
+        for (int e = begin + tid; e < end; e += U * JOIN_THREADS) {
+            int r[U], d[U];
+            bool ok[U];
+            float M[U], l[U];
+            float4 o[U][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int at = e + u * JOIN_THREADS;
+                r[u] = y0 + ((at >> 2) & ((1 << lg) - 1)), d[u] = ((at >> (lg + 2)) * 4 + (at & 3)) * 2;
+                ok[u] = at < end && r[u] < rows && d[u] < D4;
+                if (!ok[u]) r[u] = d[u] = 0;
+                M[u] = -INFINITY, l[u] = 0.f;
+                o[u][0] = o[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll(U == 1 ? 4 : 2)
+            for (int c = c0; c <= c1; ++c) {
+                const int64_t part = c == first_piece ? first : 2 * c;
+                float2 ml[U];
+                float4 v[U][2];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    ml[u] = A.part_ml[part * R + r[u]];
+                    const float4* const p =
+                        reinterpret_cast<const float4*>(A.part_acc) + (part * D4 + d[u]) * R + r[u];
+                    v[u][0] = p[0], v[u][1] = p[R];
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float top = fmaxf(M[u], ml[u].x);
+                    const float f = top == -INFINITY ? 1.f : ex2(M[u] - top);
+                    const float g = top == -INFINITY ? 1.f : ex2(ml[u].x - top);
+                    M[u] = top;
+                    l[u] = fmaf(l[u], f, g * ml[u].y);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float4& x = o[u][k];
+                        const float4& z = v[u][k];
+                        x.x = fmaf(x.x, f, g * z.x), x.y = fmaf(x.y, f, g * z.y);
+                        x.z = fmaf(x.z, f, g * z.z), x.w = fmaf(x.w, f, g * z.w);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (ok[u]) join_store(A, s, t.hk, row0 + r[u], d[u] + k, o[u][k], l[u]);
+        }
+    };
+    pdl_wait();
+    if (end - begin > JOIN_THREADS) join(std::integral_constant<int, 2>{});
+    else join(std::integral_constant<int, 1>{});
 }
 
 template <int WPR>
 __global__ void __launch_bounds__(8 * WPR * 32) join_parts_kernel(const __grid_constant__ JoinArgs A) {
     join_parts<WPR>(A, blockIdx.x);
 }
-template <int HDP>
 __global__ void __launch_bounds__(JOIN_THREADS, 2)
     join_pieces_kernel(const __grid_constant__ JoinArgs A) {
-    join_pieces<HDP>(A, blockIdx.x, blockIdx.y);
+    join_pieces(A, blockIdx.x, blockIdx.y);
 }
 // Both in one launch, the pieces first.
-template <int HDP>
 __global__ void __launch_bounds__(JOIN_THREADS, 2)
     join_both_kernel(const __grid_constant__ JoinArgs parts, const __grid_constant__ JoinArgs pieces) {
     constexpr int WPR = JOIN_THREADS / 256;
     const int n = pieces.rule.n_pieces, y = blockIdx.x / n;
-    if (y * JOIN_ROWS < pieces.rule.R) join_pieces<HDP>(pieces, blockIdx.x - y * n, y);
+    if (y * JOIN_ROWS < pieces.rule.R) join_pieces(pieces, blockIdx.x - y * n, y);
     else join_parts<WPR>(parts, blockIdx.x - (pieces.rule.R + JOIN_ROWS - 1) / JOIN_ROWS * n);
 }
 
@@ -1087,17 +1116,18 @@ constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 // The same for trees, whose wide kernel takes one query tile and its key tiles in turn (us, 16, 24, 32
 // and 48 rows, 32 heads):
 //   sequences over   FP16, 8 kv heads of 128                  FP16, 4 kv heads of 64
-//   2 x 30000        91:102  123:103  156:101  217:102        43:54   44:55   61:54   81:54
-//   8 x 2000         42:53   51:54    59:54    76:55          22:30   24:30   29:30   34:31
-//   32 x 2000        102:120 135:120  169:120  226:122        43:61   54:62   67:62   91:63
-//   64 x 400         67:119  89:119   113:120  161:121        34:53   46:52   45:53   63:54
+//   2 x 30000        91:88    123:88   156:86   217:87        43:50   44:50   61:49   81:50
+//   8 x 2000         42:50    50:50    58:49    76:50         22:30   24:30   29:30   34:30
+//   32 x 2000        101:116  135:117  169:116  226:117       43:55   53:55   67:55   90:56
+//   64 x 400         67:85    89:85    113:89   161:91        34:39   46:39   45:40   62:40
 //                    FP32, 8 kv heads of 128                  FP32, 4 kv heads of 64
-//   2 x 30000        219:319 318:320  410:321  571:324        67:95   73:96   103:94  141:95
-//   8 x 2000         78:114  90:115   115:114  160:116        30:43   34:44   43:44   54:44
-//   32 x 2000        212:346 296:347  389:347  581:349        65:103  86:104  109:102 147:103
-//   64 x 400         118:201 172:201  209:202  314:205        48:80   64:81   66:81   91:82
-template <int HDP>
-constexpr int narrow_tree_rows = HDP == 128 ? 24 : 32;
+//   2 x 30000        220:312  317:312  409:310  571:310       67:89   73:89   103:88  141:88
+//   8 x 2000         78:114   90:114   115:113  160:114       29:41   34:41   43:40   54:40
+//   32 x 2000        211:352  296:353  389:352  581:353       65:96   86:97   109:96  148:96
+//   64 x 400         118:192  172:193  209:193  313:195       48:59   64:59   66:59   90:60
+// (head_dim over 128, whose wide kernel is the causal one: as there)
+template <typename KV, int HDP>
+constexpr int narrow_tree_rows = HDP > 128 ? 32 : sizeof(KV) == 2 && HDP == 128 ? 16 : 24;
 
 // Wide tiles run on tcgen05 for head_dim up to 128.  Above, S and O of two query tiles do not fit
 // into tensor memory, nor FP32 sums of a row into a thread's registers; one query tile whose sums are
@@ -1128,7 +1158,7 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
         s.ml_off = take((size_t)2 * r.n_pieces * r.R * sizeof(float2));
     };
     const int64_t rows = b->n_tokens * G;
-    constexpr int NARROW = TREE ? narrow_tree_rows<HDP> : narrow_rows<KV, HDP>;
+    constexpr int NARROW = TREE ? narrow_tree_rows<KV, HDP> : narrow_rows<KV, HDP>;
     if (most_q * G <= NARROW) {
         add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
     } else {
@@ -1177,7 +1207,9 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
         const Share& s = plan.share[i];
         const JoinArgs j{a.w, s.rule, a.out, a.out_stride, reinterpret_cast<float*>(ws + s.acc_off),
                          reinterpret_cast<float2*>(ws + s.ml_off)};
-        if (s.rule.R > 8) {
+        if (s.rule.flat && max_pos <= s.rule.uncut - s.rule.KT) {
+            // (no tile is cut: flat_cut)
+        } else if (s.rule.R > 8) {
             pieces = j;
             n_pieces = (int64_t)s.rule.n_pieces * ((s.rule.R + JOIN_ROWS - 1) / JOIN_ROWS);
         } else if (max_pos > s.rule.least) {
@@ -1188,10 +1220,10 @@ static int run_plan(const ib_kv_pages* p, const ib_kv_batch* b, const Plan& plan
     }
     const unsigned rounds = n_pieces ? (unsigned)(n_pieces / pieces.rule.n_pieces) : 0;
     if (n_parts && n_pieces)
-        IB_CUDA_CHECK(launch_pdl(join_both_kernel<HDP>, dim3((unsigned)(n_pieces + n_parts)),
+        IB_CUDA_CHECK(launch_pdl(join_both_kernel, dim3((unsigned)(n_pieces + n_parts)),
                                  dim3(JOIN_THREADS), 0, st, true, parts, pieces));
     else if (n_pieces)
-        IB_CUDA_CHECK(launch_pdl(join_pieces_kernel<HDP>, dim3((unsigned)pieces.rule.n_pieces, rounds),
+        IB_CUDA_CHECK(launch_pdl(join_pieces_kernel, dim3((unsigned)pieces.rule.n_pieces, rounds),
                                  dim3(JOIN_THREADS), 0, st, true, pieces));
     else if (n_parts && n_parts <= kSMs)
         IB_CUDA_CHECK(launch_pdl(join_parts_kernel<4>, dim3((unsigned)n_parts), dim3(8 * 4 * 32), 0, st,

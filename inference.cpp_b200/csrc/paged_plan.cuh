@@ -17,8 +17,10 @@ constexpr int kSMs = 148;  // of a B200: the pieces aimed at, and so the workspa
 struct CutRule {
     int R, KT, min_rows, max_rows, n_pieces, least;
     int fixed = 0;  // positions that beginning a tile costs as much as (pieces)
-    // trees: every tile of a sequence costs the same, whole key tiles
+    // trees: every tile of a sequence costs the same, whole key tiles; none is cut so that a side has
+    // fewer than `least` positions, nor one of fewer than `uncut`
     bool flat = false;
+    int uncut = 0;
     bool split = false;  // tcgen05: one query tile, its key tiles shared out (paged_tensor.cu)
     __device__ __forceinline__ int slope() const { return flat ? 0 : R; }
 };
@@ -39,6 +41,22 @@ __device__ __forceinline__ long long add_work(long long a, long long b) {
 __device__ __forceinline__ long long start_work(const CutRule& rule, const SeqInfo& s, int G) {
     const int seen = rule.flat ? (max(s.L, 0) + rule.KT - 1) / rule.KT * rule.KT : max(s.L - s.n, 0);
     return (long long)G * (seen + rule.fixed);
+}
+
+// flat: the key tile of nkt at which a cut `x` into a tile's work falls.  What beginning a tile costs is
+// half on either side of it.  A cut close to an end falls on the end: the side that is left begins
+// no tile and has nothing to be joined.  Two kernels have to agree, so every step is rounded by itself.
+__device__ __forceinline__ int flat_cut(const CutRule& rule, long long x, int G, int nkt) {
+    const float per = __fdividef(1.f, (float)(G * rule.KT));
+    const int kt = __float2int_rn(__fsub_rn(__fmul_rn((float)x, per),
+                                            __fdividef((float)(rule.fixed / 2), (float)rule.KT)));
+    if (nkt * rule.KT < rule.uncut) return 2 * kt < nkt ? 0 : nkt;
+    const int few = (rule.least + rule.KT - 1) / rule.KT;
+    return kt < few ? 0 : nkt - kt < few ? nkt : kt;
+}
+// The key tiles that a tile's rows see.
+__device__ __forceinline__ int seen_tiles(const CutRule& rule, int start, int row0, int rows, int G) {
+    return (max(0, start + (row0 + rows - 1) / G + 1) + rule.KT - 1) / rule.KT;
 }
 
 __device__ __forceinline__ long long tiles_work(long long t, long long start_g, int R) {
@@ -142,10 +160,46 @@ __device__ __forceinline__ void find_piece(const PagedView& w, const CutRule& ru
     }
 }
 
+// The tile that work `p.at` of the piece's sequence is in.
+struct TileAt {
+    int hk, tile;
+    long long x0, all;  // how far into its work; all of it
+};
+template <bool FLAT>
+__device__ __forceinline__ TileAt tile_at(const PagedView& w, const CutRule& rule, const Piece& p,
+                                          long long start_g) {
+    TileAt t;
+    const int G = w.H / w.Hkv;
+    long long u = p.at - p.base;
+    t.hk = min((int)__fdividef((float)u, (float)p.x.per_head), w.Hkv - 1);  // to one
+    if (t.hk * p.x.per_head > u) --t.hk;
+    else if ((t.hk + 1) * p.x.per_head <= u) ++t.hk;
+    u -= t.hk * p.x.per_head;
+    const int tiles = (p.x.s.n * G + rule.R - 1) / rule.R;
+    int lo = 0;  // the last whose work begins at or before u
+    if constexpr (FLAT) {
+        while (lo + 1 < tiles && u >= start_g) ++lo, u -= start_g;
+        t.x0 = u;
+        t.all = start_g;
+    } else {
+        int hi = tiles;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (tiles_work(mid, start_g, rule.slope()) <= u) lo = mid;
+            else hi = mid;
+        }
+        t.x0 = u - tiles_work(lo, start_g, rule.slope());
+        t.all = start_g + (long long)(lo + 1) * rule.slope();
+    }
+    t.tile = lo;
+    return t;
+}
+
 // The next segment of a piece; false at its end.  Called by whole warps, each for itself.
+template <bool FLAT>
 __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& rule, Piece& p,
                                              Segment& g) {
-    if (p.at >= p.end) return false;
+    while (p.at < p.end) {
     if (p.at >= p.base + p.x.all) {  // on to the next sequence that takes part
         p.base += p.x.all;
         for (int b0 = p.b + 1;; b0 += 32) {
@@ -164,36 +218,35 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     const int G = w.H / w.Hkv;
     const SeqInfo& s = p.x.s;
     const long long start_g = start_work(rule, s, G);
-    long long u = p.at - p.base;
+    const TileAt t = tile_at<FLAT>(w, rule, p, start_g);
     g.s = s;
     g.start = s.L - s.n;
-    g.hk = min((int)__fdividef((float)u, (float)p.x.per_head), w.Hkv - 1);  // to one
-    if (g.hk * p.x.per_head > u) --g.hk;
-    else if ((g.hk + 1) * p.x.per_head <= u) ++g.hk;
-    u -= g.hk * p.x.per_head;
-    int lo = 0, hi = (s.n * G + rule.R - 1) / rule.R;  // the tile: the last whose work begins at or before u
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (tiles_work(mid, start_g, rule.slope()) <= u) lo = mid;
-        else hi = mid;
-    }
-    g.tile = lo;
-    g.row0 = lo * rule.R;
+    g.hk = t.hk;
+    g.tile = t.tile;
+    g.row0 = t.tile * rule.R;
     g.rows = min(rule.R, s.n * G - g.row0);
-    const long long all = start_g + (long long)(lo + 1) * rule.slope();
-    const long long x0 = u - tiles_work(lo, start_g, rule.slope());
+    const long long all = t.all, x0 = t.x0;
     const long long x1 = min(all, x0 + (p.end - p.at));
-    const int seen = max(0, g.start + (g.row0 + g.rows - 1) / G + 1);
-    const int nkt = (seen + rule.KT - 1) / rule.KT;
-    // the same value for a piece's end and the next one's beginning, and more for more work: that
-    // is all a cut needs (three integer divisions of 64 bits took a thousand cycles)
-    const float per = __fdividef((float)nkt, (float)all);
-    g.kt0 = x0 == 0 ? 0 : min(nkt, (int)((float)x0 * per));
-    g.kt1 = x1 == all ? nkt : min(nkt, (int)((float)x1 * per));
-    const bool whole = x0 == 0 && x1 == all;
+    const int nkt = seen_tiles(rule, g.start, g.row0, g.rows, G);
+    bool whole = x0 == 0 && x1 == all, none = false;
+    if constexpr (FLAT) {
+        g.kt0 = x0 == 0 ? 0 : flat_cut(rule, x0, G, nkt);
+        g.kt1 = x1 == all ? nkt : flat_cut(rule, x1, G, nkt);
+        // rows that see nothing are the first piece's
+        none = nkt == 0 ? x0 > 0 : g.kt0 == g.kt1;
+        whole = g.kt0 == 0 && g.kt1 == nkt;
+    } else {
+        // the same value for a piece's end and the next one's beginning, and more for more work: that
+        // is all a cut needs (three integer divisions of 64 bits took a thousand cycles)
+        const float per = __fdividef((float)nkt, (float)all);
+        g.kt0 = x0 == 0 ? 0 : min(nkt, (int)((float)x0 * per));
+        g.kt1 = x1 == all ? nkt : min(nkt, (int)((float)x1 * per));
+    }
     g.part = whole ? -1 : 2 * p.no + (p.at == p.no * p.len ? 0 : 1);
     p.at += x1 - x0;
-    return true;
+    if (!FLAT || !none) return true;
+    }
+    return false;
 }
 
 // ---- or into parts of tiles ----------------------------------------------------------------

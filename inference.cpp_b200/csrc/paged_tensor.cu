@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
     Segment it;
     auto next = [&]() -> bool {
         Piece p = sh_piece[warp];
-        const bool more = next_segment(w, A.rule, p, it);
+        const bool more = next_segment<TREE>(w, A.rule, p, it);
         __syncwarp();
         if (lane == 0) sh_piece[warp] = p;
         __syncwarp();
@@ -1430,11 +1430,18 @@ CutRule tensor_rule(int head_dim, int min_rows, int max_rows, bool split) {
     CutRule r = split ? rule_of<KV, true>(head_dim, min_rows, max_rows)
                       : rule_of<KV, false>(head_dim, min_rows, max_rows);
     if (TREE) {
-        // beginning a tile takes some 20k cycles, six key tiles' time: 32 trees of 12 to 24 nodes over
-        // 200 .. 4096 positions take 173 us with pieces of equal positions, 139 with 400 more to each
-        // tile, 132 with 700, 137 with 1500
+        // Beginning a tile takes some 20k cycles, as long as 800 positions on FP16 pages and 200 on FP32
+        // ones.  Eight batches of 32 trees of 12 to 24 nodes over 200 .. 4096 positions (FP16) take
+        // 160 us with 100, 151 with 200, 141 with 300, 132 with 500, 126 with 800; two documents of
+        // 20000 .. 32000 (FP32) 171.5, 171.5, 173, 174 and 176.
+        r.fixed = sizeof(KV) == 4 ? 200 : 800;
+        // Tiles of under 768 positions stay whole, and no side of a cut has less than two FP16 key tiles:
+        // a join takes as long as a few of them.  Four trees of 41 nodes over 104 .. 194 positions take
+        // 31 us so, 42 cut; 56 of 15 over 204 .. 472 (8 rows to a token) 78 and 88; 59 of 1 to 10 over
+        // 4 .. 1184 take 45 us, and 50 if tiles of under 1024 stay whole too.
         r.flat = true;
-        r.fixed = 800;
+        r.uncut = 768;
+        r.least = sizeof(KV) == 4 ? 128 : 256;
         r.split = split;
     }
     return r;
