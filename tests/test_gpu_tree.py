@@ -637,3 +637,29 @@ def test_a_step_captured_and_replayed(cuda, type_):
                 assert cuda.equal(getattr(a["seqs"], x), getattr(b["seqs"], x))
             assert cuda.equal(a["pages"].k, b["pages"].k) and cuda.equal(a["pages"].v, b["pages"].v)
     assert ib.check_fault() == 0
+
+
+@TYPES
+@pytest.mark.parametrize("H,Hkv,HD", [(8, 2, 128), (12, 1, 64), (24, 2, 96)])
+def test_attention_at_the_lengths_where_tiles_are_cut(cuda, type_, H, Hkv, HD):
+    """Few sequences, so that pieces are as short as they get, of contexts about the shortest one that
+    is cut; many short ones, so that pieces hold several tiles."""
+    for c in (1, 500, 639, 640, 641, 703, 704, 705, 767, 768, 769, 833, 896, 897, 1025, 1500):
+        run_tree(cuda, type_, H, Hkv, HD, 16, [40], [c], seed=c)
+    run_tree(cuda, type_, H, Hkv, HD, 16, [30, 41, 27], [700, 6000, 800], seed=4)
+    rng = random.Random(HD)
+    run_tree(cuda, type_, H, Hkv, HD, 16, [rng.randint(10, 40) for _ in range(150)],
+             [rng.choice([0, 3, 100, 300, 900]) for _ in range(150)], seed=5)
+
+
+@TYPES
+@pytest.mark.parametrize("n", [2, 40, 150])
+def test_attention_of_sequences_without_positions(cuda, type_, n):
+    """A length of zero: the tree's rows see nothing and are zeros, written once."""
+    pages, seqs, batch, tree, q, out, scale, _, _ = run_tree(cuda, type_, 8, 2, 64, 16, [n, 5, n], [900, 80, 10])
+    slot = batch.slots[2].item()
+    before = out.clone()
+    seqs.len[slot] = 0
+    ib.attention_paged(pages, seqs, batch, 1, q, scale, out=out, tree=tree)
+    assert cuda.equal(out[:n + 5], before[:n + 5]) and not bool(out[n + 5:2 * n + 5].any())
+    assert ib.check_fault() == 0
