@@ -407,7 +407,7 @@ int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parents, const in
  * path[j] move to position len - n + j (path in a sequence's rows, its nodes in order, as above or by
  * the caller's own verification), len becomes len - n + n_path and the pages behind it are given back.
  * n_path 0 drops all new tokens.  Recorded and passed over: n_path out of [0, n] (78: nothing is
- * changed); an entry that is no node behind the one before (78: the path ends there); a move into a
+ * changed); a length below the number of new tokens (73: likewise); an entry that is no node behind the one before (78: the path ends there); a move into a
  * page that others hold too (77).  Moves from or to a page that is not there are passed over. */
 int ib_kv_tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
                       const int32_t* path, const int32_t* n_path, void* stream);

@@ -227,6 +227,10 @@ __device__ __noinline__ void slice_again(SliceShared& sh, const T* x, int64_t be
     rank_best(sh, sh.n, k, out);
 }
 
+// Bound by the instructions of a value (17, and 10 cycles between two of a warp's): 16 groups of 8 beams over
+// 128256 FP32 logits, 62 MB, take 21 us with cold caches, 3.0 TB/s, issue slots 0.53; the call 22.9 us in a
+// graph, 74 before loads of 16 bytes a step ahead and a threshold of the first step's.  With four CTAs to the busiest SM, 3.5 to the
+// mean one; more and shorter slices cost what they gain (select_plan).
 // VEC: values of one load (16 bytes where the rows allow it, else one).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(BS_THREADS) beam_slice_kernel(const __grid_constant__ SelectArgs A) {
@@ -383,6 +387,9 @@ __device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, cons
     }
 }
 
+// A CTA per group, the slices' lists in its threads' registers where they fit.  A chain of reads, a
+// threshold's barriers and FP64 values: 8 us with cold caches for 16 groups of 8 rows of 4 slices; three to
+// four in a graph, where it is launched beside the slices.
 __global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_constant__ SelectArgs A) {
     extern __shared__ __align__(16) double2 base[];  // [beams]
     __shared__ Best buf[BS_GROUP_CAP];

@@ -423,7 +423,10 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
 // slots[i] becomes what slots[parents[i]] held, for all entries at once: a beam search's states follow
 // the selection.  Three kernels: what the slots give up and the new rows' whole pages, counted and the
 // rows put aside (a CTA per entry); who keeps a partial last page and which pages the others copy it
-// to (one CTA, as above); rows, lengths and copies (wide).
+// to (one CTA, as above); rows, lengths and copies (wide).  The first two are chains of dependent accesses,
+// 6 and 8 us with cold caches for 128 slots; the copy of 77 MB read and written (16 groups of 8 beams, 22
+// layers) takes 15 us cold, and all three 22.8 us in a graph, where each starts beside the one before; 9.6
+// us for four slots.
 struct ReorderWs {
     int32_t* row;   // [n][max_pages] the new rows
     int32_t* len;   // [n] the new lengths, -1: the entry is refused
@@ -736,7 +739,8 @@ __device__ __forceinline__ int seq_of_token(const PagedView& w, int t) {
 // count are looked up first: with a thread's first elements loaded before them 64 single tokens took
 // 4.33 us in a graph, 4.23 this way, a launch and its dependent loads; 6798 prompt tokens (32 heads
 // on 8, head_dim 128, FP32) 57.3 and 57.7 us, 5.8 TB/s, 0.89 of the measured rate.
-// TREE: token i of n is stored as position L - n + i all the same, but rotated by L - n + depth[t].
+// TREE: token i of n is stored as position L - n + i all the same, but rotated by L - n + depth[t] (64 trees
+// of 16 to 64 nodes, 32 heads on 8, FP16: 28.5 us with their plan, 4.0 TB/s).
 template <typename KV, bool TREE>
 __global__ void __launch_bounds__(256)
     kv_append_kernel(const PagedView w, const float* q, int64_t q_stride,

@@ -944,7 +944,9 @@ __device__ __forceinline__ void join_parts(const JoinArgs& A, int item) {
 // begins inside a tile, and sees to its share of that tile's rows JOIN_ROWS y ..: as many CTAs as the
 // tile has cuts share it (one CTA took 44 us for trees of 230 rows over 12000 positions in eight parts).
 // All CTAs are on the SMs at once, since each has to plan first: with 32 rows to a CTA, four times
-// as many of them, the join of a mixed step took 36 us against 22 (cold caches).
+// as many of them, the join of a mixed step took 36 us against 22 (cold caches).  The parts lie in L2; what bounds
+// it is the plan and a few dependent reads: 12.5 us with cold caches for 148 cut tiles of 32 trees, of which
+// some 6 are behind the attention kernel's end.
 constexpr int JOIN_ROWS = 128, JOIN_THREADS = 512;
 __device__ __forceinline__ void join_pieces(const JoinArgs& A, int no, int y) {
     __shared__ Piece sh_piece;
@@ -1170,7 +1172,7 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
         CutRule r;
         // trees: two query tiles that share their key tiles where the sequences fill them on average, one
         // elsewhere (two long documents of 33 to 63 nodes, FP32 pages: 181 us with two tiles, 203 with one; 32
-        // trees of 12 to 24 nodes, FP16: 213 and 133).  FP32 pages at head_dim above 64 have one anyway.
+        // trees of 12 to 24 nodes, FP16: 213 and 133, both before cuts were moved to where they gain).  FP32 pages at head_dim above 64 have one anyway.
         const bool split = TREE && ((sizeof(KV) == 4 && HDP == 128) || rows <= 128 * seqs);
         if constexpr (on_tcgen05<HDP>) r = tensor_rule<KV, TREE>(p->head_dim, narrow + 1, ALL, split);
         else r = wide_rule<KV, HDP>(narrow + 1, ALL);

@@ -32,7 +32,23 @@
 // Work per CTA is a piece of the batch (paged_plan.cuh); the copies run on into the next
 // segment.
 //
-// Measured: 2048 tokens behind 6144 (32 heads on 8, head_dim 128, FP16) 471 us, 1020 TFLOP/s of
+// Trees of drafted tokens mostly fill less than one query tile, so for them there is a second shape
+// (SPLIT): one query tile, whose key tiles the two softmax groups take in turn, each with a maximum, a
+// sum and an accumulator of its own.  A group's softmax has the other group's MMAs to hide behind, as
+// above.  At a segment's end the second group hands its maximum and sum over and the first one, which has
+// a thread for the same rows and so the same lanes of tensor memory, writes the results, while the second
+// one brings in the next segment's q.  The half of q that the other query tile would take goes to the
+// ring (five slots of FP16, four of FP32), and the copies bring K a tile ahead of V.  In tiles behind the
+// context a position counts where the node's bit is set.
+//
+// Measured, trees: 32 of 12 to 24 nodes over 200 .. 4096 positions (32 heads on 8, head_dim 128, FP16) 124
+// to 131 us and 127 with the join, 332 MB at 2.6 TB/s (232 with the kernel for chunks); tensor pipe 0.35,
+// issue 0.35.  A key tile takes 3.9k cycles to its 2.05k of MMAs: its scores, softmax (3.5k) and weighted
+// sum are a chain, and two groups hide half of it; a segment's beginning and end take 20k more, 1.7 of
+// them to a CTA.  Two documents of 33 to 63 nodes over 20001 .. 32000 (32 heads on 4, head_dim 64, FP32)
+// 182 us with two query tiles, 203 with one; tensor pipe 0.40.
+//
+// Measured, chunks: 2048 tokens behind 6144 (32 heads on 8, head_dim 128, FP16) 471 us, 1020 TFLOP/s of
 // MMAs, 0.63 of the measured rate of library FP16 products (421 to 427 us in runs of a few
 // milliseconds, before the power limit lowers the clock), and 299 us at head_dim 64; the tensor pipe
 // is busy 0.60 of the cycles.  A step of both query tiles takes 6.3k cycles to the MMAs' 4.1k: the bound is the softmax
