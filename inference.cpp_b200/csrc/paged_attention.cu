@@ -1131,6 +1131,18 @@ constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 template <typename KV, int HDP>
 constexpr int narrow_tree_rows = HDP > 128 ? 32 : sizeof(KV) == 2 && HDP == 128 ? 16 : 24;
 
+// Few trees over tables of short rows are the narrow kernel's whatever their rows: the wide one's start alone
+// takes 10 us and more, two tiles of eight rows to an SM less.  Narrow against wide (us, 32 heads; FP16 pages,
+// 8 kv heads of 128 and 4 of 64; FP32 pages likewise), by the positions of a sequence:
+//   trees x rows        tiles      100                            300                            700
+//   1 x 128, 1 x 256    128        16:21  14:20  19:29  16:25     18:23  16:22  27:45  18:35     26:26  20:25  44:79  26:28
+//   4 x 64, 4 x 128     256        14:16  12:14  19:24  14:16     24:20  19:17  39:40  24:23     35:26  26:20  56:76  35:25
+//   4 x 128, 4 x 256    512        32:21  25:21  46:29  30:26     40:23  30:23  64:45  39:36     52:29  37:29  97:80  54:35
+// so: two tiles to an SM, and 64000 positions in all of them.
+static bool few_short_trees(int64_t tiles, int64_t max_pos) {
+    return tiles <= 2 * kSMs && tiles * max_pos <= 64000;
+}
+
 // Wide tiles run on tcgen05 for head_dim up to 128.  Above, S and O of two query tiles do not fit
 // into tensor memory, nor FP32 sums of a row into a thread's registers; one query tile whose sums are
 // shared by both softmax groups would fit on FP16 pages and is not built, on FP32 pages the TF32 parts
@@ -1139,7 +1151,7 @@ template <int HDP>
 constexpr bool on_tcgen05 = HDP <= 128;
 
 template <typename KV, int HDP, bool TREE>
-static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
+static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads, int64_t max_pos) {
     constexpr int ALL = 0x7fffffff;
     const int64_t G = n_heads / p->n_kv_heads;
     const int64_t most_q = b->max_q > 0 ? std::min(b->max_q, b->n_tokens) : b->n_tokens;
@@ -1161,7 +1173,9 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads) {
     };
     const int64_t rows = b->n_tokens * G;
     constexpr int NARROW = TREE ? narrow_tree_rows<KV, HDP> : narrow_rows<KV, HDP>;
-    if (most_q * G <= NARROW) {
+    const bool short_ones =
+        TREE && on_tcgen05<HDP> && few_short_trees((rows / 8 + (seqs + 1) / 2) * p->n_kv_heads, max_pos);
+    if (most_q * G <= NARROW || short_ones) {
         add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
     } else {
         // trees: where a sequence has more rows on average, short ones are left to the wide kernel too (an
@@ -1241,7 +1255,8 @@ static int attention_paged(const ib_kv_pages* p, const ib_kv_batch* b, RowsArgs 
                            size_t* bytes, int64_t max_pos, cudaStream_t st) {
     auto go = [&](auto hdp) {
         constexpr int HDP = decltype(hdp)::value;
-        const Plan plan = a.mask ? make_plan<KV, HDP, true>(p, b, a.w.H) : make_plan<KV, HDP, false>(p, b, a.w.H);
+        const Plan plan = a.mask ? make_plan<KV, HDP, true>(p, b, a.w.H, max_pos)
+                                 : make_plan<KV, HDP, false>(p, b, a.w.H, max_pos);
         if (bytes) {
             *bytes = plan.bytes;
             return (int)IB_OK;
@@ -1271,7 +1286,7 @@ static size_t attention_workspace(const ib_kv_pages* pages, const ib_kv_seqs* se
     a.w = paged_view(pages, seqs, batch, n_heads, tree);
     if (tree) a.mask = tree->mask;
     size_t n = 0;
-    attention_paged_any(pages, batch, a, nullptr, &n, 0, nullptr);
+    attention_paged_any(pages, batch, a, nullptr, &n, (int64_t)seqs->max_pages * pages->page_size, nullptr);
     return n;
 }
 
@@ -1315,7 +1330,8 @@ static int attention_call(const ib_kv_pages* pages, const ib_kv_seqs* seqs, cons
         a.words = (tree->max_nodes + 31) / 32;
     }
     size_t need = 0;
-    attention_paged_any(pages, batch, a, nullptr, &need, 0, nullptr);
+    const int64_t max_pos = (int64_t)seqs->max_pages * pages->page_size;
+    attention_paged_any(pages, batch, a, nullptr, &need, max_pos, nullptr);
     if (!(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need))
         return paged_refuse(who, "workspace missing, too small or not 256-byte aligned");
     const int64_t layer_bytes = (int64_t)pages->n_pages * pages->n_kv_heads * pages->page_size *
@@ -1328,8 +1344,7 @@ static int attention_call(const ib_kv_pages* pages, const ib_kv_seqs* seqs, cons
     a.v = (const uint8_t*)pages->v + layer * layer_bytes;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.sectors = (((uintptr_t)out | (uintptr_t)(out_stride * 4)) & 31) == 0;
-    return attention_paged_any(pages, batch, a, workspace, nullptr,
-                               (int64_t)seqs->max_pages * pages->page_size, as_stream(stream));
+    return attention_paged_any(pages, batch, a, workspace, nullptr, max_pos, as_stream(stream));
 }
 
 extern "C" int ib_attention_paged(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
