@@ -1451,12 +1451,13 @@ CutRule tensor_rule(int head_dim, int min_rows, int max_rows, bool split) {
         // 160 us with 100, 151 with 200, 141 with 300, 132 with 500, 126 with 800; two documents of
         // 20000 .. 32000 (FP32) 171.5, 171.5, 173, 174 and 176.
         r.fixed = sizeof(KV) == 4 ? 200 : 800;
-        // Tiles of under 768 positions stay whole, and no side of a cut has less than two FP16 key tiles:
-        // a join takes as long as a few of them.  Four trees of 41 nodes over 104 .. 194 positions take
+        // Tiles of under 768 positions (FP32: 512) stay whole, and no side of a cut has less than two FP16 key
+        // tiles: a join takes as long as a few of them.  Four trees of 41 nodes over 104 .. 194 positions take
         // 31 us so, 42 cut; 56 of 15 over 204 .. 472 (8 rows to a token) 78 and 88; 59 of 1 to 10 over
-        // 4 .. 1184 take 45 us, and 50 if tiles of under 1024 stay whole too.
+        // 4 .. 1184 take 45 us, and 50 if tiles of under 1024 stay whole too.  FP32: four of 16 to 24 over
+        // 400 .. 750 (32 heads on 8 of 128) 43 us, 73 whole; 16 over 150 .. 350 46 us, 53 cut.
         r.flat = true;
-        r.uncut = 768;
+        r.uncut = sizeof(KV) == 4 ? 512 : 768;
         r.least = sizeof(KV) == 4 ? 128 : 256;
         r.split = split;
     }
