@@ -1175,12 +1175,15 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads, i
     constexpr int NARROW = TREE ? narrow_tree_rows<KV, HDP> : narrow_rows<KV, HDP>;
     const bool short_ones =
         TREE && on_tcgen05<HDP> && few_short_trees((rows / 8 + (seqs + 1) / 2) * p->n_kv_heads, max_pos);
-    if (most_q * G <= NARROW || short_ones) {
+    const bool few_rows = rows <= (int64_t)NARROW * b->n_seqs;  // to a sequence on average
+    if (most_q * G <= NARROW || short_ones || (TREE && few_rows && most_q * G <= 2 * NARROW)) {
         add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
     } else {
         // trees: where a sequence has more rows on average, short ones are left to the wide kernel too (an
-        // empty launch of the narrow one and its share of the join take 10 us)
-        const bool few = b->n_seqs == 1 || G > NARROW || (TREE && rows > (int64_t)NARROW * b->n_seqs);
+        // empty launch of the narrow one and its share of the join take 10 us), and where it has no more and
+        // none has twice as many, all are the narrow one's (59 trees of 4 to 40 rows over 4 .. 1184 positions,
+        // FP16, head_dim 48: 42 us on both kernels, 30 on the narrow one)
+        const bool few = b->n_seqs == 1 || G > NARROW || (TREE && !few_rows);
         const int narrow = few ? 0 : NARROW;
         if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
         CutRule r;
