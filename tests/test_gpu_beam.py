@@ -418,3 +418,91 @@ def test_reorder_follows_a_selection(cuda):
     assert out.row.tolist() == [[1, -1, -1], [4, 4, 4]] and out.token.tolist() == [[3, -1, -1], [7, 8, 9]]
     run_reorder(cuda, book, seqs, pages, list(range(6)), out.row.flatten().tolist())
     assert seqs.len.tolist() == [6, 0, 0, 6, 6, 6]
+
+
+def test_a_beam_step_captured_and_replayed(cuda):
+    """Extend, select and reorder in one graph, replayed with other logits, against the same calls made
+    one by one; two graphs with workspaces of their own on two streams."""
+    groups, beams, V, page = 2, 3, 5000, 4
+    n = groups * beams
+
+    def state(seed):
+        book = Book(n, 60, 300, page)
+        book.extend(list(range(n)), [5, 6, 7, 3, 4, 8])
+        s = dict(seqs=seqs_of(cuda, book), pages=pool(cuda, 2, 300, 1, page, 8, ib.F16, seed))
+        s["slots"], s["one"] = i32(cuda, range(n)), i32(cuda, [1] * n)
+        s["x"] = cuda.zeros(n, V, device="cuda")
+        s["scores"], s["ended"] = cuda.zeros(n, device="cuda"), i32(cuda, [0, 0, 0, 0, 1, 0])
+        s["out"] = ib.BeamChoice(*(cuda.zeros(groups, beams, dtype=t, device="cuda")
+                                   for t in (cuda.float32, cuda.int32, cuda.int32)))
+        s["ext"], s["status"] = i32(cuda, [0] * n), i32(cuda, [0] * n)
+        s["ws"] = ib.beam_select_workspace(s["x"], beams), ib.kv_reorder_workspace(s["seqs"], n)
+        return s
+
+    def step(s):
+        ib.kv_extend(s["pages"], s["seqs"], s["slots"], s["one"], status=s["ext"])
+        out = ib.beam_select(s["x"], s["scores"], beams=beams, ended=s["ended"], end_token=2, out=s["out"],
+                             workspace=s["ws"][0])
+        ib.kv_reorder(s["pages"], s["seqs"], s["slots"], out.row.view(-1), status=s["status"], workspace=s["ws"][1])
+        s["scores"].copy_(out.score.view(-1))
+
+    def held(s):
+        return [s["seqs"].table, s["seqs"].len, s["seqs"].refs, s["pages"].k, s["pages"].v, s["scores"]]
+
+    live, plain, graphs = [state(1), state(2)], [state(1), state(2)], []
+    for s in live:
+        before = [x.clone() for x in held(s)]
+        side = cuda.cuda.Stream()
+        side.wait_stream(cuda.cuda.current_stream())
+        with cuda.cuda.stream(side):
+            step(s)  # first use outside the capture
+        cuda.cuda.synchronize()
+        for x, y in zip(held(s), before):
+            x.copy_(y)
+        g = cuda.cuda.CUDAGraph()
+        with cuda.cuda.graph(g, stream=side):
+            step(s)
+        graphs.append((g, side))
+    for i in range(6):
+        for k, (a, b) in enumerate(zip(live, plain)):
+            x = 3 * cuda.randn(n, V, generator=cuda.Generator(device="cuda").manual_seed(10 * i + k), device="cuda")
+            a["x"].copy_(x), b["x"].copy_(x)
+        for g, side in graphs:
+            side.wait_stream(cuda.cuda.current_stream())
+            with cuda.cuda.stream(side):
+                g.replay()
+        cuda.cuda.synchronize()
+        for a, b in zip(live, plain):
+            step(b)
+            assert a["status"].tolist() == [1] * n
+            for x, y in zip(held(a) + list(a["out"]), held(b) + list(b["out"])):
+                assert cuda.equal(x, y)
+    assert ib.check_fault() == 0
+
+
+def test_select_and_reorder_on_a_given_stream(cuda):
+    """What a call makes itself is of the launch stream's memory pool; results are the same."""
+    book = Book(4, 5, 30, 4)
+    book.extend([0, 1, 2, 3], [6] * 4)
+    seqs, pages = seqs_of(cuda, book), pool(cuda, 2, 30, 1, 4, 8, ib.F32, 0)
+    x = cuda.randn(4, 3001, generator=cuda.Generator(device="cuda").manual_seed(3), device="cuda")
+    want = ib.beam_select(x, beams=2)
+    side = cuda.cuda.Stream()
+    side.wait_stream(cuda.cuda.current_stream())
+    got = ib.beam_select(x, beams=2, stream=side.cuda_stream)
+    status = ib.kv_reorder(pages, seqs, i32(cuda, [0, 1, 2, 3]), i32(cuda, want.row.flatten().tolist()),
+                           stream=side.cuda_stream)
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert cuda.equal(a, b)
+    reorder(book, [0, 1, 2, 3], want.row.flatten().tolist())
+    same(book, seqs)
+    assert status.tolist() == [1] * 4 and ib.check_fault() == 0
+
+
+@DT
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 4096), (1, 4097), (147, 4100), (149, 20000), (304, 15427), (360, 9000),
+                                        (700, 5000)])
+def test_select_however_the_rows_are_cut(cuda, dt, rows, vocab):
+    """Numbers of rows and values about those where the number of slices changes."""
+    check(cuda, random_logits(cuda, rows, vocab, getattr(cuda, dt), rows), k=min(7, vocab))

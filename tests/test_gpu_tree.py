@@ -663,3 +663,37 @@ def test_attention_of_sequences_without_positions(cuda, type_, n):
     ib.attention_paged(pages, seqs, batch, 1, q, scale, out=out, tree=tree)
     assert cuda.equal(out[:n + 5], before[:n + 5]) and not bool(out[n + 5:2 * n + 5].any())
     assert ib.check_fault() == 0
+
+
+@TYPES
+def test_a_step_on_a_given_stream(cuda, type_):
+    """Every call of a step with stream=, where what it makes itself is of that stream's memory pool."""
+    H, Hkv, HD, page, nodes, ctx = 8, 2, 64, 16, [40, 3, 60], [900, 33, 5]
+    cu, T = [0, 40, 43, 103], 103
+    rope = rope_table(cuda, 2000, HD)
+    results = []
+    for given in (False, True):
+        book = Book(3, 80, 300, page)
+        book.extend([0, 1, 2], ctx)
+        seqs, pages = seqs_of(cuda, book), pool(cuda, 2, 300, Hkv, page, HD, type_, 3)
+        qkv = cuda.randn(T, H + 2 * Hkv, HD, generator=cuda.Generator(device="cuda").manual_seed(1), device="cuda")
+        q, k, v = qkv.split([H, Hkv, Hkv], dim=1)
+        rng = random.Random(8)
+        parents = i32(cuda, flat([random_tree(rng, n) for n in nodes]))
+        tokens, best = (i32(cuda, [rng.randrange(2) for _ in range(T)]) for _ in range(2))
+        batch, slots = ib.KVBatch(i32(cuda, cu), T, max_q=60), i32(cuda, [0, 1, 2])
+        new = i32(cuda, nodes)
+        side = cuda.cuda.Stream()
+        side.wait_stream(cuda.cuda.current_stream())
+        kw = dict(stream=side.cuda_stream) if given else {}
+        ib.kv_extend(pages, seqs, slots, new, **kw)
+        tree = ib.kv_tree(batch, parents, **kw)
+        rot = ib.kv_append(pages, seqs, batch, 1, q, k, v, rope, tree=tree, **kw)
+        out = ib.attention_paged(pages, seqs, batch, 1, rot, 0.1, tree=tree, **kw)
+        path, n_path, nxt = ib.kv_tree_verify(batch, parents, tokens, best, **kw)
+        ib.kv_tree_accept(pages, seqs, batch, path, n_path, **kw)
+        cuda.cuda.synchronize()
+        results.append([out.clone(), path, n_path, nxt, seqs.table, seqs.len, seqs.refs, pages.k, pages.v])
+    for a, b in zip(*results):
+        assert cuda.equal(a, b)
+    assert ib.check_fault() == 0
