@@ -422,11 +422,11 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
 // ---- reorder ---------------------------------------------------------------------------
 // slots[i] becomes what slots[parents[i]] held, for all entries at once: a beam search's states follow
 // the selection.  Three kernels: what the slots give up and the new rows' whole pages, counted and the
-// rows put aside (a CTA per entry); who keeps a partial last page and which pages the others copy it
-// to (one CTA, as above); rows, lengths and copies (wide).  The first two are chains of dependent accesses,
-// 6 and 8 us with cold caches for 128 slots; the copy of 77 MB read and written (16 groups of 8 beams, 22
-// layers) takes 15 us cold, and all three 22.8 us in a graph, where each starts beside the one before; 9.6
-// us for four slots.
+// rows put aside (a CTA per entry, or a warp of the next kernel); who keeps a partial last page and which
+// pages the others copy it to (one CTA, as above); rows, lengths and copies (wide).  The first two are chains
+// of dependent accesses, 6 and 8 us with cold caches for 128 slots; the copy of 77 MB read and written (16
+// groups of 8 beams, 22 layers) takes 15 us cold, and all three 22.6 us in a graph, where each starts beside
+// the one before; 8.3 us for four slots.
 struct ReorderWs {
     int32_t* row;   // [n][max_pages] the new rows
     int32_t* len;   // [n] the new lengths, -1: the entry is refused
@@ -439,25 +439,17 @@ __device__ __forceinline__ int pages_of(const KvSeqsDev& s, int L) {
     return (L + s.page_size - 1) / s.page_size;
 }
 
-__global__ void __launch_bounds__(KV_COPY_THREADS)
-    kv_reorder_rows_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ slots,
-                           const int32_t* __restrict__ parents, const ReorderWs ws) {
-    __shared__ int named;
-    const int i = blockIdx.x, tid = threadIdx.x;
-    pdl_launch_dependents();
-    if (tid == 0) named = 0;
-    __syncthreads();
+// Entry i's, by NT threads; any(x): whether x holds for one of them.
+template <int NT, typename Any>
+__device__ __forceinline__ void reorder_row(const KvSeqsDev& s, int i, int n, const int32_t* slots,
+                                            const int32_t* parents, const ReorderWs& ws, int tid, Any any) {
     const int slot = slots[i], p = parents[i];
     bool ok = slot >= 0 && slot < s.n_slots && p >= -1 && p < n;
-    if (ok) {  // the first entry that names a slot has it
-        bool before = false;
-        for (int j = tid; j < i; j += KV_COPY_THREADS) before |= slots[j] == slot;
-        if (before) named = 1;
-    }
     const int from = ok && p >= 0 ? slots[p] : -1;
+    bool before = false;  // the first entry that names a slot has it
+    for (int j = tid; j < i; j += NT) before |= slots[j] == slot;
     if (p >= 0) ok = ok && from >= 0 && from < s.n_slots;
-    __syncthreads();
-    ok = ok && !named;
+    if (any(before)) ok = false;
     const int cap = s.max_pages * s.page_size;
     const int L0 = ok ? s.len[slot] : 0, L = ok && p >= 0 ? s.len[from] : 0;
     if (L0 < 0 || L0 > cap || L < 0 || L > cap) {
@@ -472,7 +464,7 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
     const int32_t* const old = s.table + (size_t)slot * s.max_pages;
     const int32_t* const row = s.table + (size_t)(p >= 0 ? from : slot) * s.max_pages;
     int32_t* const out = ws.row + (size_t)i * s.max_pages;
-    for (int j = tid; j < max(used, now); j += KV_COPY_THREADS) {
+    for (int j = tid; j < max(used, now); j += NT) {
         const int a = j < used ? old[j] : -1, z = j < now ? row[j] : -1;
         if (j < now) out[j] = z;
         if (j == full && j < now) ws.src[i] = z >= 0 && z < s.n_pages ? z : -1;
@@ -491,10 +483,19 @@ __global__ void __launch_bounds__(KV_COPY_THREADS)
         if (full == now) ws.src[i] = -1;
     }
 }
+__global__ void __launch_bounds__(KV_COPY_THREADS)
+    kv_reorder_rows_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ slots,
+                           const int32_t* __restrict__ parents, const ReorderWs ws) {
+    pdl_launch_dependents();
+    reorder_row<KV_COPY_THREADS>(s, blockIdx.x, n, slots, parents, ws, threadIdx.x,
+                                 [](bool x) { return __syncthreads_or(x); });
+}
 
 // One CTA.  A partial last page goes, as it is, to the entry whose slot has it already, else to the
 // first that takes it; one of a slot that keeps it (a refused entry's) to nobody.  The others get
 // pages, lowest first in list order; where there is none, status 0, and the slot is left empty.
+// ROWS: the rows too, a warp to an entry.
+template <bool ROWS>
 __global__ void __launch_bounds__(KV_PLAN_THREADS)
     kv_reorder_plan_kernel(const KvSeqsDev s, int n, const int32_t* __restrict__ slots,
                            const int32_t* __restrict__ parents, const ReorderWs ws,
@@ -506,7 +507,13 @@ __global__ void __launch_bounds__(KV_PLAN_THREADS)
     const int tid = threadIdx.x;
     pdl_launch_dependents();
     for (int i = tid; i < s.n_slots; i += KV_PLAN_THREADS) heir[i] = -2;  // nobody has given it up
-    pdl_wait();
+    if constexpr (ROWS) {
+        for (int i = tid >> 5; i < n; i += KV_PLAN_THREADS / 32)
+            reorder_row<32>(s, i, n, slots, parents, ws, tid & 31,
+                            [](bool x) { return __any_sync(0xffffffffu, x); });
+    } else {
+        pdl_wait();
+    }
     __syncthreads();
     for (int i = tid; i < n; i += KV_PLAN_THREADS)
         if (ws.len[i] >= 0) heir[slots[i]] = 0x7fffffff;
@@ -958,16 +965,28 @@ extern "C" int ib_kv_reorder(const ib_kv_pages* pages, const ib_kv_seqs* seqs, i
             return paged_refuse(who, "the workspace must not overlap the lists");
     const KvSeqsDev s = seqs_dev(pages, seqs);
     cudaStream_t st = as_stream(stream);
-    kv_reorder_rows_kernel<<<n, KV_COPY_THREADS, 0, st>>>(s, n, slots, parents, ws);
-    IB_LAUNCH_CHECK("kv_reorder_rows_kernel");
     constexpr size_t MOST = 2 * (size_t)IB_KV_MAX_SLOTS * 4;
     static DeviceOnce once;
     IB_CUDA_CHECK(once.run([] {
-        return cudaFuncSetAttribute(kv_reorder_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        const cudaError_t e = cudaFuncSetAttribute(kv_reorder_plan_kernel<true>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST);
+        if (e != cudaSuccess) return e;
+        return cudaFuncSetAttribute(kv_reorder_plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     (int)MOST);
     }));
-    IB_CUDA_CHECK(launch_pdl(kv_reorder_plan_kernel, dim3(1), dim3(KV_PLAN_THREADS),
-                             ((size_t)s.n_slots + n) * 4, st, true, s, n, slots, parents, ws, status));
+    const size_t sh = ((size_t)s.n_slots + n) * 4;
+    // few short rows: one launch less, of some 2.5 us of the host.  In a graph, on two launches and on three (us): 4
+    // slots of 22 pages 7.9 and 8.8, 16 of 65 9.3 and 9.5, 32 of 120 10.7 and 10.0, 32 of 240 11.9 and 10.0,
+    // 16 of 500 14.3 and 10.5.
+    if (n <= KV_PLAN_THREADS / 32 && s.max_pages <= 128) {
+        IB_CUDA_CHECK(launch_pdl(kv_reorder_plan_kernel<true>, dim3(1), dim3(KV_PLAN_THREADS), sh, st, false, s, n,
+                                 slots, parents, ws, status));
+    } else {
+        IB_CUDA_CHECK(launch_pdl(kv_reorder_rows_kernel, dim3(n), dim3(KV_COPY_THREADS), 0, st, false, s, n, slots,
+                                 parents, ws));
+        IB_CUDA_CHECK(launch_pdl(kv_reorder_plan_kernel<false>, dim3(1), dim3(KV_PLAN_THREADS), sh, st, true, s, n,
+                                 slots, parents, ws, status));
+    }
     int sms = 0;
     if ((r = sm_count(&sms)) != IB_OK) return r;
     const int64_t warps = (int64_t)n * pages->n_layers * 2 * pages->n_kv_heads;

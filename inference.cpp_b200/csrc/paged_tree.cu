@@ -225,9 +225,8 @@ extern "C" int ib_kv_tree_plan(const ib_kv_batch* batch, const int32_t* parents,
     if (!parents || !depth || !mask) return paged_refuse(who, "null pointer argument");
     if (meet(depth, n, parents, n) || meet(mask, nm, parents, n) || meet(depth, n, mask, nm))
         return paged_refuse(who, "parents, depth and mask must not overlap");
-    tree_plan_kernel<<<batch->n_seqs, TREE_THREADS, 0, as_stream(stream)>>>(
-        batch->cu_q, batch->slots, batch->n_tokens, parents, max_nodes, depth, mask);
-    IB_LAUNCH_CHECK("tree_plan_kernel");
+    IB_CUDA_CHECK(launch_pdl(tree_plan_kernel, dim3(batch->n_seqs), dim3(TREE_THREADS), 0, as_stream(stream),
+                             false, batch->cu_q, batch->slots, batch->n_tokens, parents, max_nodes, depth, mask));
     return IB_OK;
 }
 
@@ -249,9 +248,9 @@ extern "C" int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parent
         for (int k = 0; k < i; ++k) bad = bad || meet(out[i], out_n[i], out[k], out_n[k]);
         if (bad) return paged_refuse(who, "the results must not overlap the lists or one another");
     }
-    tree_verify_kernel<<<batch->n_seqs, 32, 0, as_stream(stream)>>>(
-        batch->cu_q, batch->slots, batch->n_tokens, parents, tokens, best, path, n_path, next);
-    IB_LAUNCH_CHECK("tree_verify_kernel");
+    IB_CUDA_CHECK(launch_pdl(tree_verify_kernel, dim3(batch->n_seqs), dim3(32), 0, as_stream(stream), false,
+                             batch->cu_q, batch->slots, batch->n_tokens, parents, tokens, best, path, n_path,
+                             next));
     return IB_OK;
 }
 

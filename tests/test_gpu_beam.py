@@ -506,3 +506,24 @@ def test_select_and_reorder_on_a_given_stream(cuda):
 def test_select_however_the_rows_are_cut(cuda, dt, rows, vocab):
     """Numbers of rows and values about those where the number of slices changes."""
     check(cuda, random_logits(cuda, rows, vocab, getattr(cuda, dt), rows), k=min(7, vocab))
+
+
+@pytest.mark.parametrize("n,max_pages", [(1, 3), (32, 128), (33, 128), (32, 129), (31, 40), (60, 300)])
+def test_reorder_of_few_and_many(cuda, n, max_pages):
+    """About the bounds where the rows go with the plan; slots named twice and entries refused among them."""
+    rng = random.Random(n + max_pages)
+    page = 4
+    book = Book(n + 3, max_pages, (n + 3) * max_pages // 2 + 40, page)
+    seqs, pages = seqs_of(cuda, book), pool(cuda, 2, len(book.refs), 2, page, 8, ib.F32, 0)
+    slots = rng.sample(range(n + 3), n)
+    new = [rng.randrange(0, max_pages * page // 3 + 1) for _ in slots]
+    assert ib.kv_extend(pages, seqs, i32(cuda, slots), i32(cuda, new)).tolist() == book.extend(slots, new)
+    for turn in range(6):
+        parents = [rng.randrange(-1, n) for _ in slots]
+        names = list(slots)
+        if turn > 2 and n > 2:
+            names[rng.randrange(n)] = names[rng.randrange(n)]
+            names[rng.randrange(n)] = rng.choice([-1, n + 3, names[0]])
+            parents[rng.randrange(n)] = n
+        run_reorder(cuda, book, seqs, pages, names, parents)
+    assert ib.check_fault() == 0
