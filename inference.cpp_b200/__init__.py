@@ -562,6 +562,15 @@ def _paged_tensor(t, name, dtype, shape, device):
     return t
 
 
+def _tensor_ptr(t, name, dtype, shape, dev):
+    """Pointer of such a tensor (None: none), without the messages' work where it is one."""
+    if t is None:
+        return None
+    if not (t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous()):
+        _paged_tensor(t, name, dtype, shape, dev)
+    return t.data_ptr()
+
+
 class KVPages:
     """A pool of KV pages: k and v each [n_layers, n_pages, n_kv_heads, page_size, head_dim],
     float32 or float16 CUDA tensors (kept here; the calls work on them in place)."""
@@ -921,9 +930,9 @@ def kv_append(pages, seqs, batch, layer, q, k, v, rope_table, q_out=None, stream
     vp, vs, _ = _paged_rows(v, "v", T, Hkv, HD, dev)
     op, os_, _ = _paged_rows(q_out, "q_out", T, H, HD, dev)
     n = rope_table.shape[0]
-    _paged_tensor(rope_table, "rope_table", torch.float32, (n, HD // 2, 2), dev)
+    rope = _tensor_ptr(rope_table, "rope_table", torch.float32, (n, HD // 2, 2), dev)
     st = _paged_stream(pages, stream, seqs, batch)
-    args = (layer, H, qp, qs, kp, ks, vp, vs, op, os_, rope_table.data_ptr(), n, st)
+    args = (layer, H, qp, qs, kp, ks, vp, vs, op, os_, rope, n, st)
     if tree is None:
         _call("ib_kv_append", pages._p, _seqs_of(pages, seqs), batch._p, *args)
     else:
@@ -1010,14 +1019,6 @@ def beam_select_workspace(logits, beams=1, k=None):
     return _torch().empty(n, dtype=_torch().uint8, device=logits.device)
 
 
-def _beam_ptr(t, name, dtype, shape, dev):
-    if t is None:
-        return None
-    if not (t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous()):
-        _paged_tensor(t, name, dtype, shape, dev)
-    return t.data_ptr()
-
-
 def beam_select(logits, scores=None, beams=1, k=None, ended=None, end_token=0, out=None,
                 workspace=None, stream=None):
     """The k (default: beams) best continuations of each group of `beams` rows of the logits [rows,
@@ -1040,10 +1041,10 @@ def beam_select(logits, scores=None, beams=1, k=None, ended=None, end_token=0, o
     score, token, row = out
     per_row, per_group = (rows,), (groups, k)
     _call("ib_beam_select", type_, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
-          _beam_ptr(scores, "scores", f32, per_row, dev), _beam_ptr(ended, "ended", i32, per_row, dev),
-          end_token, groups, beams, vocab, k, _beam_ptr(score, "out.score", f32, per_group, dev),
-          _beam_ptr(token, "out.token", i32, per_group, dev),
-          _beam_ptr(row, "out.row", i32, per_group, dev), *_workspace(logits, workspace), st)
+          _tensor_ptr(scores, "scores", f32, per_row, dev), _tensor_ptr(ended, "ended", i32, per_row, dev),
+          end_token, groups, beams, vocab, k, _tensor_ptr(score, "out.score", f32, per_group, dev),
+          _tensor_ptr(token, "out.token", i32, per_group, dev),
+          _tensor_ptr(row, "out.row", i32, per_group, dev), *_workspace(logits, workspace), st)
     return out
 
 
