@@ -92,6 +92,13 @@ struct Piece {
     SeqWork x;
 };
 
+// flat: a piece behind its first segment.
+struct Following {
+    long long left, start_g;  // work left to do; of a tile of the sequence
+    SeqInfo s;
+    int b, no, hk, tile, tiles;  // of the last segment; the sequence's tiles
+};
+
 // Piece `no` of the batch, into shared memory; found: whether there is one.  Every thread of the
 // CTA (NT of them) calls it; a barrier has to follow.
 template <int NT>
@@ -245,6 +252,54 @@ __device__ __forceinline__ bool next_segment(const PagedView& w, const CutRule& 
     g.part = whole ? -1 : 2 * p.no + (p.at == p.no * p.len ? 0 : 1);
     p.at += x1 - x0;
     if (!FLAT || !none) return true;
+    }
+    return false;
+}
+
+// flat: the segments behind a piece's first one, which begin with their tiles: little code, since each of a
+// CTA's roles has its own and misses the instruction cache there.
+__device__ __forceinline__ Following following(const PagedView& w, const CutRule& rule, const Piece& p,
+                                               const Segment& g) {
+    const int G = w.H / w.Hkv;
+    return Following{p.end - p.at, start_work(rule, p.x.s, G), p.x.s, p.b, p.no, g.hk, g.tile,
+                     (p.x.s.n * G + rule.R - 1) / rule.R};
+}
+__device__ __forceinline__ bool following_segment(const PagedView& w, const CutRule& rule, Following& p, Segment& g) {
+    const int G = w.H / w.Hkv;
+    while (p.left > 0) {
+        if (++p.tile == p.tiles) {
+            p.tile = 0;
+            if (++p.hk == w.Hkv) {
+                p.hk = 0;
+                for (int b0 = p.b + 1;; b0 += 32) {
+                    if (b0 >= w.n_seqs) return false;
+                    const int b = b0 + (int)(threadIdx.x & 31);
+                    const int rows = b < w.n_seqs ? seq_info(w, b).n * G : 0;
+                    const unsigned has = __ballot_sync(0xffffffffu, rows >= rule.min_rows && rows <= rule.max_rows);
+                    if (has) {
+                        p.b = b0 + __ffs(has) - 1;
+                        break;
+                    }
+                }
+                p.s = seq_info(w, p.b);
+                p.tiles = (p.s.n * G + rule.R - 1) / rule.R;
+                p.start_g = start_work(rule, p.s, G);
+            }
+        }
+        const SeqInfo& s = p.s;
+        g.s = s;
+        g.start = s.L - s.n;
+        g.hk = p.hk;
+        g.tile = p.tile;
+        g.row0 = p.tile * rule.R;
+        g.rows = min(rule.R, s.n * G - g.row0);
+        const long long x1 = min(p.start_g, p.left);
+        const int nkt = seen_tiles(rule, g.start, g.row0, g.rows, G);
+        g.kt0 = 0;
+        g.kt1 = x1 == p.start_g ? nkt : flat_cut(rule, x1, G, nkt);
+        g.part = g.kt1 == nkt ? -1 : 2 * p.no + 1;
+        p.left -= x1;
+        if (g.kt1 > 0 || nkt == 0) return true;
     }
     return false;
 }

@@ -62,6 +62,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "lookup.h"
@@ -319,7 +320,15 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) TensorBars<C::SLOTS> bar;
     __shared__ uint32_t tmem_base;
-    __shared__ Piece sh_piece[C::WARPS];  // the same one for each warp, out of its registers
+    // the same one for each warp, out of its registers
+    __shared__ std::conditional_t<TREE, Following, Piece> sh_piece[C::WARPS];
+    Piece* piece;
+    if constexpr (TREE) {
+        __shared__ Piece one;
+        piece = &one;
+    } else {
+        piece = sh_piece;
+    }
     __shared__ int found;
     // of the last key tiles: positions without a page; positions whose V is not finite
     constexpr int RECENT = C::RECENT;
@@ -333,13 +342,15 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (!A.beside) pdl_wait();
     pdl_launch_dependents();
-    find_piece<C::THREADS>(w, A.rule, blockIdx.x, sh_piece, &found);
+    find_piece<C::THREADS>(w, A.rule, blockIdx.x, piece, &found);
     __syncthreads();
     if (!found) {
         if (A.beside) pdl_wait();
         return;
     }
-    if (tid > 0 && tid < C::WARPS) sh_piece[tid] = sh_piece[0];
+    if constexpr (!TREE) {
+        if (tid > 0 && tid < C::WARPS) sh_piece[tid] = sh_piece[0];
+    }
     const uint32_t base = smem_u32(smem_raw);  // on a boundary of 1024 bytes, for the swizzle
     uint8_t* const base_ptr = smem_raw;
     if (tid == 0) {
@@ -384,8 +395,10 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
     const int G = w.H / w.Hkv, HD = w.HD;
     Segment it;
     auto next = [&]() -> bool {
-        Piece p = sh_piece[warp];
-        const bool more = next_segment<TREE>(w, A.rule, p, it);
+        auto p = sh_piece[warp];
+        bool more;
+        if constexpr (TREE) more = following_segment(w, A.rule, p, it);
+        else more = next_segment<false>(w, A.rule, p, it);
         __syncwarp();
         if (lane == 0) sh_piece[warp] = p;
         __syncwarp();
@@ -399,9 +412,14 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
 
     // The first segment here, for all roles: its code is brought in once.
     bool first = false;
-    if constexpr (SPLIT) first = next();
+    if constexpr (TREE) {
+        Piece p = *piece;
+        first = next_segment<true>(w, A.rule, p, it);
+        if (lane == 0 && first) sh_piece[warp] = following(w, A.rule, p, it);
+        __syncwarp();
+    }
     auto go_on = [&](bool& begun) -> bool {  // `begun`: false at a role's beginning
-        if (!SPLIT || begun) return next();
+        if (!TREE || begun) return next();
         begun = true;
         return first;
     };
@@ -420,7 +438,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
         const uint32_t o_at = tmem + ((uint32_t)wr << 16) + (uint32_t)(256 + 128 * t);
         [[maybe_unused]] const uint32_t ml_at = tmem + ((uint32_t)wr << 16) + (uint32_t)C::ML;
         int tiles = 0;      // key tiles so far, of all segments
-        if constexpr (!SPLIT) first = next();
+        if constexpr (!TREE) first = next();
         uint32_t seen = 0;  // and counted as the copies do (both groups')
         // SPLIT: the first group's key tiles so far, the one that used q last
         [[maybe_unused]] int firsts = 0, q_used = -1, exchanges = 0;
