@@ -1118,15 +1118,15 @@ constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 // The same for trees, whose wide kernel takes one query tile and its key tiles in turn (us, 16, 24, 32
 // and 48 rows, 32 heads):
 //   sequences over   FP16, 8 kv heads of 128                  FP16, 4 kv heads of 64
-//   2 x 30000        91:88    123:88   156:86   217:87        43:50   44:50   61:49   81:50
-//   8 x 2000         42:50    50:50    58:49    76:50         22:30   24:30   29:30   34:30
-//   32 x 2000        101:116  135:117  169:116  226:117       43:55   53:55   67:55   90:56
-//   64 x 400         67:85    89:85    113:89   161:91        34:39   46:39   45:40   62:40
+//   2 x 30000        91:88    123:88   156:86   217:87        43:50   44:50   61:49   81:49
+//   8 x 2000         42:49    50:50    58:50    76:50         22:30   24:30   29:29   34:29
+//   32 x 2000        101:114  135:115  169:114  226:115       43:53   53:53   67:53   90:53
+//   64 x 400         67:74    89:76    113:76   161:77        34:35   46:35   45:35   62:35
 //                    FP32, 8 kv heads of 128                  FP32, 4 kv heads of 64
-//   2 x 30000        220:312  317:312  409:310  571:310       67:89   73:89   103:88  141:88
-//   8 x 2000         78:114   90:114   115:113  160:114       29:41   34:41   43:40   54:40
-//   32 x 2000        211:352  296:353  389:352  581:353       65:96   86:97   109:96  148:96
-//   64 x 400         118:192  172:193  209:193  313:195       48:59   64:59   66:59   90:60
+//   2 x 30000        220:294  317:294  409:293  571:293       67:90   73:91   103:90  141:90
+//   8 x 2000         78:111   90:112   115:111  160:112       29:41   34:41   43:41   54:42
+//   32 x 2000        211:340  296:340  389:340  581:341       65:103  86:103  109:102 148:103
+//   64 x 400         118:172  172:173  209:174  313:176       48:56   64:56   66:56   90:56
 // (head_dim over 128, whose wide kernel is the causal one: as there)
 template <typename KV, int HDP>
 constexpr int narrow_tree_rows = HDP > 128 ? 32 : sizeof(KV) == 2 && HDP == 128 ? 16 : 24;

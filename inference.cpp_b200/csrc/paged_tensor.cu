@@ -41,9 +41,9 @@
 // ring (five slots of FP16, four of FP32), and the copies bring K a tile ahead of V.  In tiles behind the
 // context a position counts where the node's bit is set.
 //
-// Measured, trees: 32 of 12 to 24 nodes over 200 .. 4096 positions (32 heads on 8, head_dim 128, FP16) 124
-// to 131 us and 127 with the join, 332 MB at 2.6 TB/s (232 with the kernel for chunks); tensor pipe 0.35,
-// issue 0.35.  A key tile takes 3.9k cycles to its 2.05k of MMAs: its scores, softmax (3.5k) and weighted
+// Measured, trees: 32 of 12 to 24 nodes over 200 .. 4096 positions (32 heads on 8, head_dim 128, FP16) 127
+// to 132 us with the join, 332 MB at 2.6 TB/s (232 with the kernel for chunks); tensor pipe 0.35, issue
+// 0.35; 100 of 8 to 24 over 50 .. 900 163 us (180 while each role looked its segments up like the first).  A key tile takes 3.9k cycles to its 2.05k of MMAs: its scores, softmax (3.5k) and weighted
 // sum are a chain, and two groups hide half of it; a segment's beginning and end take 20k more, 1.7 of
 // them to a CTA.  Two documents of 33 to 63 nodes over 20001 .. 32000 (32 heads on 4, head_dim 64, FP32)
 // 182 us with two query tiles, 203 with one; tensor pipe 0.40.

@@ -697,3 +697,56 @@ def test_a_step_on_a_given_stream(cuda, type_):
     for a, b in zip(*results):
         assert cuda.equal(a, b)
     assert ib.check_fault() == 0
+
+
+def make_long(cuda, rng, page, *args, **kw):
+    """As make, with rows of the table for more than 64000 positions: what few trees over short rows
+    take another kernel for."""
+    seqs, batch, table, slots, n_pages, cu = make_short(cuda, rng, page, *args, **kw)
+    more = -(-64001 // page) - len(table[0])
+    table = [row + [-1] * more for row in table]
+    seqs = ib.KVSeqs(cuda.tensor(table, dtype=cuda.int32, device="cuda"), seqs.len, seqs.refs)
+    return seqs, batch, table, slots, n_pages, cu
+
+
+make_short = make
+BRANCHES = [(40, 8, 128), (140, 8, 128), (100, 2, 64), (20, 8, 48), (90, 4, 96)]
+
+
+@TYPES
+@pytest.mark.parametrize("case", ["nan", "inf", "bits", "shapes", "small", "holes", "pages", "values", "groups", "number", "lengths"])
+def test_attention_over_long_tables(cuda, type_, case, monkeypatch):
+    """The tests above on the kernels that few trees over short tables do not reach."""
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "make", make_long)
+    if case in ("nan", "inf"):
+        for n, H, HD in BRANCHES:
+            test_attention_rows_do_not_see_other_branches(cuda, type_, n, H, HD, float(case))
+    elif case == "bits":
+        test_attention_bits_of_later_nodes_do_not_count(cuda, type_)
+    elif case == "shapes":
+        test_attention_shapes_of_trees(cuda, type_)
+    elif case == "small":
+        for shape in SHAPES:
+            test_attention_small_trees(cuda, type_, *shape)
+            test_attention_large_trees(cuda, type_, *shape)
+    elif case == "holes":
+        for nodes in ([1, 2, 4, 0], [150, 1, 66, 9], [20, 12, 30, 9], [40, 50, 60, 70]):
+            test_attention_holes_and_empty_rows(cuda, type_, nodes)
+    elif case == "pages":
+        for page in (1, 2, 5, 7, 12, 100):
+            test_attention_odd_pages(cuda, type_, page, 96)
+    elif case == "values":
+        test_attention_wide_range_of_values(cuda, type_)
+    elif case == "groups":
+        for G in (1, 3, 16):
+            test_attention_groups(cuda, type_, G)
+    elif case == "number":
+        for n in (5, 9, 17, 31, 32, 33, 63, 64, 65, 96, 128, 129):
+            test_attention_every_number_of_nodes(cuda, type_, n)
+    else:
+        for H, Hkv, HD in ((8, 2, 128), (12, 1, 64)):
+            for c in (1, 127, 128, 129, 300, 511, 512, 513, 767, 768, 769, 1025):
+                run_tree(cuda, type_, H, Hkv, HD, 16, [40], [c], seed=c)
+        for n in (2, 40, 150):
+            test_attention_of_sequences_without_positions(cuda, type_, n)
