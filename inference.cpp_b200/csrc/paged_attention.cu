@@ -1181,8 +1181,10 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads, i
     } else {
         // trees: where a sequence has more rows on average, short ones are left to the wide kernel too (an
         // empty launch of the narrow one and its share of the join take 10 us), and where it has no more and
-        // none has twice as many, all are the narrow one's (59 trees of 4 to 40 rows over 4 .. 1184 positions,
-        // FP16, head_dim 48: 42 us on both kernels, 30 on the narrow one)
+        // none has twice as many, all are the narrow one's.  On both kernels and on the narrow one (us): 24 of 4
+        // to 28 rows over 500 .. 2000 positions (FP16, 8 kv heads of 128) 79 and 64, 60 of them over 100 .. 400
+        // 75 and 56; 60 of 4 to 44 (FP16, 8 of 64) 68 and 53; FP32 178 and 151, 92 and 69; at head_dim 256
+        // (24 of 4 to 56, 4 kv heads) 136 and 98, but 274 and 302 on FP32 pages.
         const bool few = b->n_seqs == 1 || G > NARROW || (TREE && !few_rows);
         const int narrow = few ? 0 : NARROW;
         if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
