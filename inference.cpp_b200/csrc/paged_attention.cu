@@ -1075,6 +1075,18 @@ static CutRule narrow_rule(int min_rows, int max_rows) {
     using C = NarrowCfg<KV, HDP>;
     return CutRule{C::R, C::KW, min_rows, max_rows, kSMs * C::CTAS * 2, 128};
 }
+// Trees, whose rows fill a tile: where every SM has a part, parts are 1024 positions (us, with 128 and with
+// 1024; two to four nodes, 32 heads on 8 of 128: 8 trees over 480, 900 and 200 .. 4096 positions, FP16, 21:17
+// 31:23 44:35; 48 over 240, 480, 100 .. 900 and 200 .. 4096 34:29 46:37 47:39 99:99; 24 on FP32 pages over 240,
+// 900 and 200 .. 4096 30:24 51:57 108:102; one over 60000 73:76).  Over tables of no more than 192 positions
+// nothing is cut, which takes a launch less: 10.2 and 9.0 us for 7 nodes over 130 (FP32, 6 heads of 48).
+template <typename KV, int HDP>
+static CutRule narrow_tree_rule(int min_rows, int max_rows, int64_t max_pos) {
+    CutRule r = narrow_rule<KV, HDP>(min_rows, max_rows);
+    r.filled = 1024;
+    if (max_pos <= 192) r.least = 192;
+    return r;
+}
 template <typename KV, int HDP>
 static CutRule wide_rule(int min_rows, int max_rows) {
     using C = WideCfg<KV, HDP>;
@@ -1177,7 +1189,7 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads, i
         TREE && on_tcgen05<HDP> && few_short_trees((rows / 8 + (seqs + 1) / 2) * p->n_kv_heads, max_pos);
     const bool few_rows = rows <= (int64_t)NARROW * b->n_seqs;  // to a sequence on average
     if (most_q * G <= NARROW || short_ones || (TREE && few_rows && most_q * G <= 2 * NARROW)) {
-        add(narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
+        add(TREE ? narrow_tree_rule<KV, HDP>(1, ALL, max_pos) : narrow_rule<KV, HDP>(1, ALL), seqs + rows / 8);
     } else {
         // trees: where a sequence has more rows on average, short ones are left to the wide kernel too (an
         // empty launch of the narrow one and its share of the join take 10 us), and where it has no more and
@@ -1187,7 +1199,8 @@ static Plan make_plan(const ib_kv_pages* p, const ib_kv_batch* b, int n_heads, i
         // (24 of 4 to 56, 4 kv heads) 136 and 98, but 274 and 302 on FP32 pages.
         const bool few = b->n_seqs == 1 || G > NARROW || (TREE && !few_rows);
         const int narrow = few ? 0 : NARROW;
-        if (narrow) add(narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
+        if (narrow)
+            add(TREE ? narrow_tree_rule<KV, HDP>(1, narrow, max_pos) : narrow_rule<KV, HDP>(1, narrow), std::min(seqs * (narrow / 8), seqs + rows / 8));
         CutRule r;
         // trees: two query tiles that share their key tiles where the sequences fill them on average, one
         // elsewhere (two long documents of 33 to 63 nodes, FP32 pages: 181 us with two tiles, 203 with one; 32

@@ -16,6 +16,7 @@ constexpr int kSMs = 148;  // of a B200: the pieces aimed at, and so the workspa
 // positions, in n_pieces pieces of at least `least` positions of one token.
 struct CutRule {
     int R, KT, min_rows, max_rows, n_pieces, least;
+    int filled = 0; // parts: at least so many positions where there is one for each SM (0: `least`)
     int fixed = 0;  // positions that beginning a tile costs as much as (pieces)
     // trees: every tile of a sequence costs the same, whole key tiles; none is cut so that a side has
     // fewer than `least` positions, nor one of fewer than `uncut`
@@ -353,8 +354,9 @@ __device__ __forceinline__ bool find_item(const PagedView& w, const CutRule& rul
 #pragma unroll
     for (int i = 0; i < NT / 32; ++i) units += sh_units[i];
     units = min(units, 1ll << 45) * w.Hkv;
-    const int len = (int)min(max((long long)(rule.least / rule.KT), (units + rule.n_pieces - 1) / rule.n_pieces),
-                             0x3fffffffll);
+    long long most = max((long long)(rule.least / rule.KT), (units + rule.n_pieces - 1) / rule.n_pieces);
+    if (rule.filled) most = max(most, min((long long)(rule.filled / rule.KT), (units + kSMs - 1) / kSMs));
+    const int len = (int)min(most, 0x3fffffffll);
     // cu_q can hold anything: counts are clamped to what cannot be, so that sums stay in range
     // (valid batches have at most 2^22 + n_seqs row tiles, see paged_check_batch)
     constexpr long long MOST = 1 << 23;
