@@ -1130,15 +1130,15 @@ constexpr int narrow_rows = sizeof(KV) == 4 && HDP == 128 ? 16 : 32;
 // The same for trees, whose wide kernel takes one query tile and its key tiles in turn (us, 16, 24, 32
 // and 48 rows, 32 heads):
 //   sequences over   FP16, 8 kv heads of 128                  FP16, 4 kv heads of 64
-//   2 x 30000        91:88    123:88   156:86   217:87        43:50   44:50   61:49   81:49
-//   8 x 2000         42:49    50:50    58:50    76:50         22:30   24:30   29:29   34:29
-//   32 x 2000        101:114  135:115  169:114  226:115       43:53   53:53   67:53   90:53
-//   64 x 400         67:74    89:76    113:76   161:77        34:35   46:35   45:35   62:35
+//   2 x 30000        92:87    123:87   155:85   217:86        42:50   46:50   62:49   82:49
+//   8 x 2000         36:49    37:50    62:49    70:50         20:30   24:30   23:29   26:29
+//   32 x 2000        102:112  137:113  170:112  228:112       44:53   50:53   69:53   92:53
+//   64 x 400         69:74    92:75    117:75   166:77        30:35   38:35   48:35   66:36
 //                    FP32, 8 kv heads of 128                  FP32, 4 kv heads of 64
-//   2 x 30000        220:294  317:294  409:293  571:293       67:90   73:91   103:90  141:90
-//   8 x 2000         78:111   90:112   115:111  160:112       29:41   34:41   43:41   54:42
-//   32 x 2000        211:340  296:340  389:340  581:341       65:103  86:103  109:102 148:103
-//   64 x 400         118:172  172:173  209:174  313:176       48:56   64:56   66:56   90:56
+//   2 x 30000        218:296  317:296  409:296  571:296       67:90   80:90   103:89  141:89
+//   8 x 2000         57:112   104:112  109:112  161:112       27:41   35:41   41:41   41:41
+//   32 x 2000        213:347  296:347  390:347  581:347       70:99   83:99   110:99  149:100
+//   64 x 400         120:174  174:175  214:176  319:178       43:55   51:55   68:55   93:55
 // (head_dim over 128, whose wide kernel is the causal one: as there)
 template <typename KV, int HDP>
 constexpr int narrow_tree_rows = HDP > 128 ? 32 : sizeof(KV) == 2 && HDP == 128 ? 16 : 24;
