@@ -750,3 +750,15 @@ def test_attention_over_long_tables(cuda, type_, case, monkeypatch):
                 run_tree(cuda, type_, H, Hkv, HD, 16, [40], [c], seed=c)
         for n in (2, 40, 150):
             test_attention_of_sequences_without_positions(cuda, type_, n)
+
+
+@TYPES
+@pytest.mark.parametrize("H,Hkv,HD", [(8, 2, 128), (6, 6, 48), (4, 1, 256)])
+def test_attention_of_few_rows_however_it_is_cut(cuda, type_, H, Hkv, HD):
+    """Few rows over tables of about 192 positions, below which nothing is cut, and about the lengths of one
+    and more parts, few trees and many."""
+    for page in (1, 16, 64):
+        for total in (127, 128, 129, 176, 191, 192, 193, 208, 256, 257):
+            run_tree(cuda, type_, H, Hkv, HD, page, [3], [total - 3], seed=total)
+    run_tree(cuda, type_, H, Hkv, HD, 16, [2, 4, 1], [1021, 1022, 2100], seed=2)
+    run_tree(cuda, type_, H, Hkv, HD, 16, [1 + i % 4 for i in range(90)], [(37 * i) % 1300 for i in range(90)], seed=3)
