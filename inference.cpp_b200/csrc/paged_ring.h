@@ -35,6 +35,15 @@ IB_RING_FN int tile_order(int e, int n) {
 // look is its warp's alone then, but the phases of all looks at a slot count: the others take them too.
 IB_RING_FN int tile_owner(int half) { return half % 3; }
 
+// The buffer of two in which the factors of a segment's rows lie (SPLIT, FP16 pages: the second group writes
+// them with q, the first one reads them up to the segment's end).  Segments without key tiles are not counted:
+// they stage no q and pass no barrier, so nothing would keep the second group from writing two ahead.
+struct ScaleTurn {
+    uint32_t n = 0;
+    IB_RING_FN int buffer() const { return (int)(n & 1); }
+    IB_RING_FN void next(int key_tiles) { n += key_tiles > 0; }
+};
+
 struct Looks {
     uint32_t parity = 0;  // of each barrier's next phase, a bit each
     static IB_RING_FN int bar(int slot) { return slot; }

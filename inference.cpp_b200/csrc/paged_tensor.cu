@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
     __shared__ __align__(16) uint16_t sh_gone[RECENT][8];
     __shared__ __align__(16) uint16_t sh_bad[F32 ? 1 : RECENT][8];
     __shared__ uint32_t sh_bad32[F32 ? RECENT : 1][C::SPLIT_WARPS][2];  // the same for FP32, of each splitting warp
-    __shared__ uint8_t sh_scale[2][SPLIT && !F32 ? 128 : 1];  // of the segment's rows (exponents), by its number
+    __shared__ uint8_t sh_scale[2][SPLIT && !F32 ? 128 : 1];  // of the segment's rows (exponents), see ScaleTurn
     // the second group's maximum and sum, where tensor memory has no columns left for them
     __shared__ float2 sh_ml[SPLIT && C::ML < 0 ? 128 : 1];
     const PagedView& w = A.w;
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
         uint32_t seen = 0;  // and counted as the copies do (both groups')
         // SPLIT: the first group's key tiles so far, the one that used q last
         [[maybe_unused]] int firsts = 0, q_used = -1, exchanges = 0;
-        [[maybe_unused]] uint32_t segs = 0;
+        [[maybe_unused]] ScaleTurn segs;
         bool ok = true;
         const float sign = A.scale_log2 < 0.f ? -1.f : 1.f;
         // The segment's q into this warp's 32 rows of the tile, HDP / 8 lanes to a row; returns the
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
         };
         // SPLIT: by the second group, whose registers are free then, the rows that there are spread over
         // its warps (the others' scores are not used).  The rows' factors, powers of two, go to sh_scale.
-        [[maybe_unused]] auto stage_split = [&](const Segment& sg, uint32_t seg) {
+        [[maybe_unused]] auto stage_split = [&](const Segment& sg, int buffer) {
             // (small loops: it is met once a segment, and its instructions come from far then)
             constexpr int LPR = HDP / 8, RPI = 32 / LPR, CPR = HDP / 4, RPC = 32 / CPR;
             if (sg.kt0 == sg.kt1) return;
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
                     split2(x0.x * up, x0.y * up, h.x, l.x), split2(x0.z * up, x0.w * up, h.y, l.y);
                     split2(x1.x * up, x1.y * up, h.z, l.z), split2(x1.z * up, x1.w * up, h.w, l.w);
                     *at0 = h, *at1 = l;
-                    if (d == 0) sh_scale[seg & 1][r] = (uint8_t)(__float_as_uint(down) >> 23);
+                    if (d == 0) sh_scale[buffer][r] = (uint8_t)(__float_as_uint(down) >> 23);
                 }
             }
             pt_fence_async();
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
                     // last: this group has waited for its own
                     if (q_used >= 0) ok = wait(&bar.s_full[0], q_used);
                     q_used = -1;
-                    if (ok) stage_split(cur, segs);
+                    if (ok) stage_split(cur, segs.buffer());
                 }
                 firsts += n_kt / 2;
                 if (n_kt > 0 && !(n_kt & 1)) q_used = firsts - 1;
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
             [[maybe_unused]] auto row_scale = [&]() -> float {
                 if constexpr (!SPLIT || F32) return sc;
                 else
-                    return fmaxf(fabsf(A.scale_log2) * __uint_as_float((uint32_t)sh_scale[segs & 1][r] << 23),
+                    return fmaxf(fabsf(A.scale_log2) * __uint_as_float((uint32_t)sh_scale[segs.buffer()][r] << 23),
                                  1e-37f);
             };
             // trees: the masks' bits of the key tile, read ahead of its scores; they serve until its O
@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
                         mbar_arrive(&bar.x_done);
                     }
                 }
-                ++segs;
+                segs.next(n_kt);
                 if (t == 1) continue;
             }
             if (r < rows && ok) {  // a row per thread

@@ -229,3 +229,13 @@ def test_roles_of_the_tree_kernel_come_to_their_ends(tmp_path):
 def test_the_search_finds_looks_that_are_not_counted(tmp_path):
     """The same with warps that count only their own looks at a slot: some order never ends."""
     assert "runs, 0 stuck, 0 faults" not in _cpp(tmp_path, "split_ring_test", "forget")
+
+
+def test_rows_factors_of_the_tree_kernel_are_their_segments_own(tmp_path):
+    """Every order of its softmax groups and MMAs over short batches, segments without key tiles among them."""
+    assert " 0 faults, 0 orders without an end" in _cpp(tmp_path, "split_scales_test")
+
+
+def test_the_search_finds_factors_of_another_segment(tmp_path):
+    """The same where segments without key tiles are counted as the others are."""
+    assert " 0 faults" not in _cpp(tmp_path, "split_scales_test", "all")

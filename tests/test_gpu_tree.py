@@ -762,3 +762,33 @@ def test_attention_of_few_rows_however_it_is_cut(cuda, type_, H, Hkv, HD):
             run_tree(cuda, type_, H, Hkv, HD, page, [3], [total - 3], seed=total)
     run_tree(cuda, type_, H, Hkv, HD, 16, [2, 4, 1], [1021, 1022, 2100], seed=2)
     run_tree(cuda, type_, H, Hkv, HD, 16, [1 + i % 4 for i in range(90)], [(37 * i) % 1300 for i in range(90)], seed=3)
+
+
+@TYPES
+@pytest.mark.parametrize("HD", [64, 128])
+def test_attention_with_empty_sequences_between_others(cuda, type_, HD):
+    """Trees whose rows see nothing between trees of queries of very different sizes: one and two in a row,
+    one kv head, so that a tile is a sequence, and contexts of two and four key tiles."""
+    H, page, n, B = 8, 16, 6, 600
+    rng = random.Random(HD)
+    empty = [b % 5 in (1, 3, 4) for b in range(B)]
+    nodes = [n] * B
+    ctx = [rng.choice([rng.randint(123, 250), rng.randint(379, 506)]) for _ in range(B)]
+    seqs, batch, table, slots, n_pages, cu = make(cuda, rng, page, nodes, [c + n for c in ctx], 0, True)
+    pages = pool(cuda, 2, n_pages, 1, page, HD, type_, 3)
+    for b in range(B):
+        if empty[b]:
+            seqs.len[slots[b]] = 0
+    parents = [random_tree(rng, n) for _ in nodes]
+    tree = plan_of(cuda, batch, parents, 0, n)
+    size = cuda.tensor([2.0 ** rng.randint(-5, 5) for _ in nodes], device="cuda").repeat_interleave(n)
+    q = cuda.randn(B * n, H, HD, generator=cuda.Generator(device="cuda").manual_seed(HD), device="cuda")
+    q = q * size[:, None, None]
+    scale = 1.0 / math.sqrt(HD)
+    ref, tol = tree_ref(cuda, pages, 1, table, slots, cu, [0 if e else n for e in empty], ctx, parents, q, scale)
+    there = ~ref.isnan()
+    for _ in range(20):
+        out = ib.attention_paged(pages, seqs, batch, 1, q, scale, out=cuda.full_like(q, 3.0), tree=tree)
+        assert bool(((out.double() - ref).abs() <= tol)[there].all())
+        assert not bool(out[~there].any())
+    assert ib.check_fault() == 0
