@@ -634,7 +634,7 @@ class KVBatch:
         self.cu_q = _paged_tensor(cu_q, "cu_q", torch.int32, (-1,), None)
         self.device = cu_q.device
         self.n_seqs, self.n_tokens = cu_q.numel() - 1, int(n_tokens)
-        self.slots, self.max_q = slots, int(max_q)
+        self.slots = slots
         if slots is not None:
             _paged_tensor(slots, "slots", torch.int32, (self.n_seqs,), self.device)
         self._c = _CKVBatch(self.n_seqs, self.n_tokens, int(max_q), cu_q.data_ptr(), _ptr(slots))
@@ -865,14 +865,15 @@ def _tree_of(pages, batch, tree):
 
 def kv_tree(batch, parents, max_nodes=0, out=None, stream=None):
     """The trees of a batch's new tokens from their parents: once a step, for every layer's
-    kv_append and attention_paged.  max_nodes: the most nodes of one sequence (0: the batch's
-    max_q, or its n_tokens); a sequence with more is left out of the step and recorded.  out: a
-    KVTree of such a batch, whose depth and mask are filled again.  Returns the KVTree."""
+    kv_append and attention_paged.  max_nodes: the most nodes of one sequence, which the masks have
+    room for (0: what the batch can have, its n_tokens up to KV_MAX_NODES; its max_q is a hint and
+    bounds nothing); a sequence with more is left out of the step and recorded.  out: a KVTree of
+    such a batch, whose depth and mask are filled again.  Returns the KVTree."""
     torch, T = _torch(), batch.n_tokens
     st = _paged_stream(batch, stream)
     p = _paged_list(batch, parents, "parents", T)
     if out is None:
-        max_nodes = int(max_nodes) or min(batch.max_q or T, T) or 1
+        max_nodes = int(max_nodes) or min(T, KV_MAX_NODES) or 1
         with _allocating(batch, stream):
             out = KVTree(parents, torch.zeros(T, dtype=torch.int32, device=batch.device),
                          torch.zeros(T, (max_nodes + 31) // 32, dtype=torch.int32,

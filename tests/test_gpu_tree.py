@@ -792,3 +792,18 @@ def test_attention_with_empty_sequences_between_others(cuda, type_, HD):
         assert bool(((out.double() - ref).abs() <= tol)[there].all())
         assert not bool(out[~there].any())
     assert ib.check_fault() == 0
+
+
+@TYPES
+@pytest.mark.parametrize("max_q", [0, 1, 7, 20])
+def test_a_hint_leaves_no_tree_out(cuda, type_, max_q):
+    """More nodes in all than one tree may have, with no hint, one that is too small and a right one."""
+    nodes, ctx = [20, 0] + [17] * 60, [100, 3] + [(29 * b) % 300 for b in range(60)]
+    pages, seqs, batch, tree, q, out, scale, _, _ = run_tree(cuda, type_, 8, 2, 64, 16, nodes, ctx, max_q=20, max_nodes=20)
+    batch = ib.KVBatch(batch.cu_q, batch.n_tokens, max_q=max_q, slots=batch.slots)
+    other = ib.kv_tree(batch, tree.parents)
+    assert cuda.equal(other.depth, tree.depth) and cuda.equal(other.mask[:, :1], tree.mask)
+    assert not bool(other.mask[:, 1:].any())
+    got = ib.attention_paged(pages, seqs, batch, 1, q, scale, tree=other)
+    assert bool(((got - out).abs() <= 2.0 ** -17 * pages.v.abs().max()).all())
+    assert ib.check_fault() == 0
