@@ -133,7 +133,9 @@ SIGNATURES = {
     "ib_attention_paged_tree": [_vp, _vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _f, _vp, _sz,
                                 _vp],
     "ib_kv_tree_verify": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ib_kv_tree_verify_max": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "ib_kv_tree_accept": [_vp, _vp, _vp, _vp, _vp, _vp],
+    "ib_kv_tree_accept_max": [_vp, _vp, _vp, _i, _vp, _vp, _vp],
     "ib_beam_select_workspace": [_i, _i, _i, _i],
     "ib_beam_select": [_i, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp],
     "ib_argmax": [_vp, _i, _vp, _vp],
@@ -863,6 +865,11 @@ def _tree_of(pages, batch, tree):
     return tree._p
 
 
+def _max_nodes_of(pages, batch, tree):
+    _tree_of(pages, batch, tree)
+    return tree.max_nodes
+
+
 def kv_tree(batch, parents, max_nodes=0, out=None, stream=None):
     """The trees of a batch's new tokens from their parents: once a step, for every layer's
     kv_append and attention_paged.  max_nodes: the most nodes of one sequence, which the masks have
@@ -886,12 +893,15 @@ def kv_tree(batch, parents, max_nodes=0, out=None, stream=None):
     return out
 
 
-def kv_tree_verify(batch, parents, tokens, best, path=None, n_path=None, next=None, stream=None):
+def kv_tree_verify(batch, parents, tokens, best, path=None, n_path=None, next=None, stream=None,
+                   tree=None):
     """Greedy verification of the batch's trees.  tokens: the nodes' tokens (node 0's is certain),
     best: what the model chose behind each node (beam_select with k = 1), int32 [n_tokens].
     Returns path [n_tokens] (the confirmed nodes of a sequence, in its rows, -1 behind them),
-    n_path and next [n_seqs] (the token behind the last confirmed node; -1: no nodes)."""
+    n_path and next [n_seqs] (the token behind the last confirmed node; -1: no nodes).  tree: the
+    step's; a sequence with more nodes than its max_nodes, which the step has left out, has none."""
     torch, T, n = _torch(), batch.n_tokens, batch.n_seqs
+    most = KV_MAX_NODES if tree is None else _max_nodes_of(batch, batch, tree)
     st = _paged_stream(batch, stream)
     if path is None or n_path is None or next is None:
         with _allocating(batch, stream):
@@ -899,19 +909,21 @@ def kv_tree_verify(batch, parents, tokens, best, path=None, n_path=None, next=No
             path = make(T) if path is None else path
             n_path = make(n) if n_path is None else n_path
             next = make(n) if next is None else next
-    _call("ib_kv_tree_verify", batch._p, _paged_list(batch, parents, "parents", T),
+    _call("ib_kv_tree_verify_max", batch._p, most, _paged_list(batch, parents, "parents", T),
           _paged_list(batch, tokens, "tokens", T), _paged_list(batch, best, "best", T),
           _paged_list(batch, path, "path", T), _paged_list(batch, n_path, "n_path", n),
           _paged_list(batch, next, "next", n), st)
     return path, n_path, next
 
 
-def kv_tree_accept(pages, seqs, batch, path, n_path, stream=None):
+def kv_tree_accept(pages, seqs, batch, path, n_path, stream=None, tree=None):
     """Of the batch's new tokens only the path stays in the cache: its K and V move together in
     every layer, the lengths follow, and the pages behind them are given back.  path, n_path: as
-    kv_tree_verify returns them, or the caller's own."""
+    kv_tree_verify returns them, or the caller's own.  tree: the step's; of a sequence with more
+    nodes than its max_nodes, which the step has left out, nothing stays."""
     st = _paged_stream(pages, stream, seqs, batch)
-    _call("ib_kv_tree_accept", pages._p, _seqs_of(pages, seqs), batch._p,
+    most = KV_MAX_NODES if tree is None else _max_nodes_of(pages, batch, tree)
+    _call("ib_kv_tree_accept_max", pages._p, _seqs_of(pages, seqs), batch._p, most,
           _paged_list(pages, path, "path", batch.n_tokens),
           _paged_list(pages, n_path, "n_path", batch.n_seqs), st)
 

@@ -62,12 +62,12 @@ __global__ void __launch_bounds__(TREE_THREADS)
 // of the path.  Bound by its launch and those reads, 5 us with cold caches for 32 trees of 16 to 64 nodes.
 __global__ void __launch_bounds__(32)
     tree_verify_kernel(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ slots, int n_tokens,
-                       const int32_t* __restrict__ parents, const int32_t* __restrict__ tokens,
-                       const int32_t* __restrict__ best, int32_t* __restrict__ path,
-                       int32_t* __restrict__ n_path, int32_t* __restrict__ next) {
+                       int max_nodes, const int32_t* __restrict__ parents,
+                       const int32_t* __restrict__ tokens, const int32_t* __restrict__ best,
+                       int32_t* __restrict__ path, int32_t* __restrict__ n_path, int32_t* __restrict__ next) {
     const int lane = threadIdx.x;
     int q0;
-    const int n = tree_nodes(cu_q, slots, n_tokens, blockIdx.x, IB_KV_MAX_NODES, q0);
+    const int n = tree_nodes(cu_q, slots, n_tokens, blockIdx.x, max_nodes, q0);
     int at = n > 0 ? 0 : -1, m = 0, want = 0;
     pdl_launch_dependents();
     if (at == 0) {
@@ -107,8 +107,9 @@ __global__ void __launch_bounds__(32)
 constexpr int ACCEPT_THREADS = 512, ACCEPT_CLUSTER = 8, ACCEPT_BATCH = 4;
 
 __global__ void __cluster_dims__(ACCEPT_CLUSTER) __launch_bounds__(ACCEPT_THREADS)
-    tree_accept_kernel(const PagedView w, int32_t* table, int32_t* len, int32_t* refs, const PoolBytes pool,
-                       const int32_t* __restrict__ path, const int32_t* __restrict__ n_path) {
+    tree_accept_kernel(const PagedView w, int max_nodes, int32_t* table, int32_t* len, int32_t* refs,
+                       const PoolBytes pool, const int32_t* __restrict__ path,
+                       const int32_t* __restrict__ n_path) {
     __shared__ int from[IB_KV_MAX_NODES], to[IB_KV_MAX_NODES];  // rows of head 0 in a layer, -1: no move
     __shared__ int bad, first;
     const int b = blockIdx.x / ACCEPT_CLUSTER, part = blockIdx.x % ACCEPT_CLUSTER;
@@ -121,9 +122,10 @@ __global__ void __cluster_dims__(ACCEPT_CLUSTER) __launch_bounds__(ACCEPT_THREAD
     int m = n_path[b];
     // nothing to do: left out of the step, no new tokens, or a slot that is none
     const bool idle = s.n == 0 || slot < 0 || slot >= w.n_slots;
-    if (idle || m < 0 || m > s.n || start < 0) {
+    const bool large = s.n > max_nodes;  // left out of the step: its K and V were never written
+    if (idle || start < 0 || large || m < 0 || m > s.n) {
         if (!idle && part == 0 && tid == 0) paged_fault(start < 0 ? PAGED_BAD_LEN : PAGED_BAD_TREE);
-        m = -1;
+        m = !idle && start >= 0 && large ? 0 : -1;
     }
     __syncthreads();
     for (int j = tid; j < m; j += ACCEPT_THREADS) {
@@ -230,12 +232,13 @@ extern "C" int ib_kv_tree_plan(const ib_kv_batch* batch, const int32_t* parents,
     return IB_OK;
 }
 
-extern "C" int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parents, const int32_t* tokens,
-                                 const int32_t* best, int32_t* path, int32_t* n_path, int32_t* next,
-                                 void* stream) {
-    const char* who = "ib_kv_tree_verify";
+static int tree_verify(const ib_kv_batch* batch, int max_nodes, const int32_t* parents,
+                       const int32_t* tokens, const int32_t* best, int32_t* path, int32_t* n_path,
+                       int32_t* next, void* stream, const char* who) {
     const int r = tree_batch(batch, who);
     if (r != IB_OK) return r;
+    if (max_nodes < 1 || max_nodes > IB_KV_MAX_NODES)
+        return paged_refuse(who, "max_nodes must be in [1, 1024]");
     if (batch->n_seqs == 0) return IB_OK;
     if (!parents || !tokens || !best || !path || !n_path || !next)
         return paged_refuse(who, "null pointer argument");
@@ -249,22 +252,49 @@ extern "C" int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parent
         if (bad) return paged_refuse(who, "the results must not overlap the lists or one another");
     }
     IB_CUDA_CHECK(launch_pdl(tree_verify_kernel, dim3(batch->n_seqs), dim3(32), 0, as_stream(stream), false,
-                             batch->cu_q, batch->slots, batch->n_tokens, parents, tokens, best, path, n_path,
-                             next));
+                             batch->cu_q, batch->slots, batch->n_tokens, max_nodes, parents, tokens, best,
+                             path, n_path, next));
+    return IB_OK;
+}
+
+extern "C" int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parents, const int32_t* tokens,
+                                 const int32_t* best, int32_t* path, int32_t* n_path, int32_t* next,
+                                 void* stream) {
+    return tree_verify(batch, IB_KV_MAX_NODES, parents, tokens, best, path, n_path, next, stream,
+                       "ib_kv_tree_verify");
+}
+
+extern "C" int ib_kv_tree_verify_max(const ib_kv_batch* batch, int max_nodes, const int32_t* parents,
+                                     const int32_t* tokens, const int32_t* best, int32_t* path,
+                                     int32_t* n_path, int32_t* next, void* stream) {
+    return tree_verify(batch, max_nodes, parents, tokens, best, path, n_path, next, stream,
+                       "ib_kv_tree_verify_max");
+}
+
+static int tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,
+                       int max_nodes, const int32_t* path, const int32_t* n_path, void* stream,
+                       const char* who) {
+    const int r = paged_check_batch(pages, seqs, batch, 0, pages ? pages->n_kv_heads : 0, who);
+    if (r != IB_OK) return r;
+    if (max_nodes < 1 || max_nodes > IB_KV_MAX_NODES)
+        return paged_refuse(who, "max_nodes must be in [1, 1024]");
+    if (batch->n_seqs == 0) return IB_OK;
+    if (!path || !n_path) return paged_refuse(who, "null pointer argument");
+    const PagedView w = paged_view(pages, seqs, batch, pages->n_kv_heads);
+    IB_CUDA_CHECK(launch_pdl(tree_accept_kernel, dim3(batch->n_seqs * ACCEPT_CLUSTER), dim3(ACCEPT_THREADS),
+                             0, as_stream(stream), true, w, max_nodes, seqs->table, seqs->len, seqs->refs,
+                             pool_bytes(pages), path, n_path));
     return IB_OK;
 }
 
 extern "C" int ib_kv_tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
                                  const ib_kv_batch* batch, const int32_t* path, const int32_t* n_path,
                                  void* stream) {
-    const char* who = "ib_kv_tree_accept";
-    const int r = paged_check_batch(pages, seqs, batch, 0, pages ? pages->n_kv_heads : 0, who);
-    if (r != IB_OK || batch->n_seqs == 0) return r;
-    if (!path || !n_path) return paged_refuse(who, "null pointer argument");
-    ib_kv_tree none{IB_KV_MAX_NODES, nullptr, nullptr};
-    const PagedView w = paged_view(pages, seqs, batch, pages->n_kv_heads, &none);
-    IB_CUDA_CHECK(launch_pdl(tree_accept_kernel, dim3(batch->n_seqs * ACCEPT_CLUSTER), dim3(ACCEPT_THREADS),
-                             0, as_stream(stream), true, w, seqs->table, seqs->len, seqs->refs,
-                             pool_bytes(pages), path, n_path));
-    return IB_OK;
+    return tree_accept(pages, seqs, batch, IB_KV_MAX_NODES, path, n_path, stream, "ib_kv_tree_accept");
+}
+
+extern "C" int ib_kv_tree_accept_max(const ib_kv_pages* pages, const ib_kv_seqs* seqs,
+                                     const ib_kv_batch* batch, int max_nodes, const int32_t* path,
+                                     const int32_t* n_path, void* stream) {
+    return tree_accept(pages, seqs, batch, max_nodes, path, n_path, stream, "ib_kv_tree_accept_max");
 }

@@ -239,3 +239,14 @@ def test_rows_factors_of_the_tree_kernel_are_their_segments_own(tmp_path):
 def test_the_search_finds_factors_of_another_segment(tmp_path):
     """The same where segments without key tiles are counted as the others are."""
     assert " 0 faults" not in _cpp(tmp_path, "split_scales_test", "all")
+
+
+def test_verify_and_accept_refuse_a_bad_limit():
+    L, b = ib.lib(), ref(batch(n_tokens=5, n_seqs=2))
+    for most in (0, -1, 1025):
+        assert L.ib_kv_tree_verify_max(b, most, PTR, PTR, PTR, FAR, FAR + 4096, FAR + 8192, None) == ib.IB_ERR_INVALID
+        assert "ib_kv_tree_verify_max: max_nodes" in ib.last_error()
+        assert L.ib_kv_tree_accept_max(ref(pages()), ref(seqs()), b, most, PTR, PTR, None) == ib.IB_ERR_INVALID
+        assert "ib_kv_tree_accept_max: max_nodes" in ib.last_error()
+    assert L.ib_kv_tree_verify_max(b, 8, PTR, PTR, PTR, PTR, FAR, FAR + 4096, None) == ib.IB_ERR_INVALID
+    assert L.ib_kv_tree_accept_max(ref(pages()), ref(seqs()), None, 8, PTR, PTR, None) == ib.IB_ERR_INVALID

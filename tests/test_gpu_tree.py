@@ -807,3 +807,55 @@ def test_a_hint_leaves_no_tree_out(cuda, type_, max_q):
     got = ib.attention_paged(pages, seqs, batch, 1, q, scale, tree=other)
     assert bool(((got - out).abs() <= 2.0 ** -17 * pages.v.abs().max()).all())
     assert ib.check_fault() == 0
+
+
+@TYPES
+@pytest.mark.parametrize("n,most", [(9, 8), (40, 32), (1030, 1024), (1025, 1000)])
+def test_a_step_with_a_tree_that_is_too_large(cuda, type_, n, most):
+    """Left out of plan, append and attention, it has no path, and nothing of it stays in the cache."""
+    H, Hkv, HD, page = 4, 2, 64, 16
+    nodes, ctx = [5, n, 7], [30, 50, 11]
+    cu, T = [0, 5, 5 + n, 12 + n], 12 + n
+    book = Book(3, 90, 200, page)
+    book.extend([0, 1, 2], ctx)
+    seqs, pages = seqs_of(cuda, book), pool(cuda, 2, 200, Hkv, page, HD, type_, 3)
+    k, v = pages.k.clone(), pages.v.clone()
+    batch, new = ib.KVBatch(i32(cuda, cu), T), i32(cuda, nodes)
+    assert ib.kv_extend(pages, seqs, i32(cuda, [0, 1, 2]), new).tolist() == [1, 1, 1]
+    table = seqs.table.clone()
+    parents = i32(cuda, [-1, 0, 0, 1, 2] + [i - 1 for i in range(n)] + [-1, 0, 1, 2, 3, 4, 5])
+    tokens = i32(cuda, [4] * T)
+    tree = ib.kv_tree(batch, parents, most)
+    qkv = cuda.randn(T, H + 2 * Hkv, HD, generator=cuda.Generator(device="cuda").manual_seed(1), device="cuda")
+    q, kn, vn = qkv.split([H, Hkv, Hkv], dim=1)
+    rope = rope_table(cuda, 2000, HD)
+    for layer in range(2):
+        rot = ib.kv_append(pages, seqs, batch, layer, q, kn, vn, rope, tree=tree)
+        out = ib.attention_paged(pages, seqs, batch, layer, rot, 0.1, tree=tree, out=cuda.full((T, H, HD), 3.0, device="cuda"))
+        assert bool((out[5:5 + n] == 3.0).all()) and not bool((out[:5] == 3.0).any())
+    path, n_path, nxt = ib.kv_tree_verify(batch, parents, tokens, tokens, tree=tree)
+    assert n_path.tolist() == [3, 0, 7] and nxt.tolist() == [4, -1, 4]
+    assert path.tolist() == [0, 1, 3, -1, -1] + [-1] * n + list(range(7))
+    with pytest.raises(RuntimeError, match="78"):
+        ib.check_fault()
+    mine = n_path.clone()
+    mine[1] = 3  # and a path of the caller's own
+    path[5:8] = i32(cuda, [0, 1, 2])
+    refs = seqs.refs.clone()
+    for paths in (n_path, mine):
+        seqs.table.copy_(table)
+        seqs.refs.copy_(refs)
+        seqs.len.copy_(i32(cuda, [c + m for c, m in zip(ctx, nodes)]))
+        ib.kv_tree_accept(pages, seqs, batch, path, paths, tree=tree)
+        assert seqs.len.tolist() == [33, 50, 18]
+        with pytest.raises(RuntimeError, match="78"):
+            ib.check_fault()
+        kept = [[x if j < -(-L // page) else -1 for j, x in enumerate(row)] for row, L in zip(table.tolist(), (33, 50, 18))]
+        assert seqs.table.tolist() == kept
+        held = [x for row in kept for x in row if x >= 0]
+        assert seqs.refs.tolist() == [int(p in held) for p in range(200)]
+    for b in range(3):  # what was there before the step is as it was
+        for p in range(ctx[b]):
+            at = table[b, p // page].item()
+            assert cuda.equal(pages.k[:, at, :, p % page], k[:, at, :, p % page])
+            assert cuda.equal(pages.v[:, at, :, p % page], v[:, at, :, p % page])
