@@ -5,8 +5,6 @@
 //
 // A sequence's n new tokens are nodes 0 .. n - 1; node i is stored at position L - n + i and stands
 // at L - n + depth(i) of the text, behind its ancestors: depth(i) = number of ancestors in the tree.
-#include <cooperative_groups.h>
-
 #include <string>
 
 #include "common.cuh"
@@ -97,56 +95,77 @@ __global__ void __launch_bounds__(32)
 }
 
 // ---- accept ------------------------------------------------------------------------------
-// A cluster of CTAs per sequence.  A path's nodes are in order, so entry j of it comes from a row at
-// or behind its own place and rows can be moved in that order; a thread has 16 bytes of a row of one
-// (layer, K or V, head) and takes them through all moves, a few loads in flight at a time, without
-// waiting for others.  Once every CTA of the cluster is through, the first one gives back the pages
-// behind the new end.  Bound by latency (length, path, table, reference count, row, one after the other):
-// with the verification before it 11.5 us in a graph for 32 trees of 16 to 64 nodes through 32 layers
-// (7.9 MB), 6.4 for one of 7 nodes.
-constexpr int ACCEPT_THREADS = 512, ACCEPT_CLUSTER = 8, ACCEPT_BATCH = 4;
+// Two kernels: the moves, and what the sequences give back.  Whether others hold a page too is decided by
+// the counts before the call, so no count changes before every sequence has its moves behind it (in
+// one kernel a sequence that gave up a page could let another's move into it through for some layers
+// and not for others).
+//
+// A path's nodes are in order, so entry j of it comes from a row at or behind its own place and rows can
+// be moved in that order; a thread has 16 bytes of a row of one (layer, K or V, head) and takes them
+// through all moves, a few loads in flight at a time, without waiting for others.  Bound by latency
+// (length, path, table, reference count, row, one after the other): with the verification before it
+// 11.2 us in a graph for 32 trees of 16 to 64 nodes through 32 layers (7.9 MB), 6.4 for one of 7 nodes, as
+// in one kernel with a cluster's barrier (11.3, 6.5); the second launch is 2 us of the host.
+constexpr int ACCEPT_THREADS = 512, ACCEPT_CTAS = 8, ACCEPT_BATCH = 4;
 
-__global__ void __cluster_dims__(ACCEPT_CLUSTER) __launch_bounds__(ACCEPT_THREADS)
-    tree_accept_kernel(const PagedView w, int max_nodes, int32_t* table, int32_t* len, int32_t* refs,
-                       const PoolBytes pool, const int32_t* __restrict__ path,
-                       const int32_t* __restrict__ n_path) {
+// What stays of sequence b: its first m new tokens' places; -1: it is left as it is.
+struct Accepted {
+    SeqInfo s;
+    int slot, start, m;
+};
+__device__ __forceinline__ Accepted accepted(const PagedView& w, int max_nodes, const int32_t* n_path, int b,
+                                             bool record) {
+    Accepted a;
+    a.s = seq_info(w, b);
+    a.slot = w.slots ? w.slots[b] : b;
+    a.start = a.s.L - a.s.n;
+    a.m = n_path[b];
+    // nothing to do: left out of the step, no new tokens, or a slot that is none
+    const bool idle = a.s.n == 0 || a.slot < 0 || a.slot >= w.n_slots;
+    const bool large = a.s.n > max_nodes;  // left out of the step: its K and V were never written
+    if (idle || a.start < 0 || large || a.m < 0 || a.m > a.s.n) {
+        if (!idle && record) paged_fault(a.start < 0 ? PAGED_BAD_LEN : PAGED_BAD_TREE);
+        a.m = !idle && a.start >= 0 && large ? 0 : -1;
+    }
+    return a;
+}
+// Whether entry j of a path of n nodes is one behind the entry before.
+__device__ __forceinline__ bool path_goes_on(const int32_t* path, int j, int n) {
+    return path[j] > (j ? path[j - 1] : -1) && path[j] < n;
+}
+
+__global__ void __launch_bounds__(ACCEPT_THREADS)
+    tree_move_kernel(const PagedView w, int max_nodes, const PoolBytes pool, const int32_t* __restrict__ path,
+                     const int32_t* __restrict__ n_path) {
     __shared__ int from[IB_KV_MAX_NODES], to[IB_KV_MAX_NODES];  // rows of head 0 in a layer, -1: no move
     __shared__ int bad, first;
-    const int b = blockIdx.x / ACCEPT_CLUSTER, part = blockIdx.x % ACCEPT_CLUSTER;
+    const int b = blockIdx.x / ACCEPT_CTAS, part = blockIdx.x % ACCEPT_CTAS;
     const int tid = threadIdx.x;
     if (tid == 0) bad = first = IB_KV_MAX_NODES;
     pdl_wait();
-    const SeqInfo s = seq_info(w, b);
-    const int slot = w.slots ? w.slots[b] : b;
-    const int start = s.L - s.n;
-    int m = n_path[b];
-    // nothing to do: left out of the step, no new tokens, or a slot that is none
-    const bool idle = s.n == 0 || slot < 0 || slot >= w.n_slots;
-    const bool large = s.n > max_nodes;  // left out of the step: its K and V were never written
-    if (idle || start < 0 || large || m < 0 || m > s.n) {
-        if (!idle && part == 0 && tid == 0) paged_fault(start < 0 ? PAGED_BAD_LEN : PAGED_BAD_TREE);
-        m = !idle && start >= 0 && large ? 0 : -1;
-    }
+    pdl_launch_dependents();
+    const Accepted a = accepted(w, max_nodes, n_path, b, part == 0 && tid == 0);
+    int m = a.m;
     __syncthreads();
     for (int j = tid; j < m; j += ACCEPT_THREADS) {
-        const int c = path[s.q0 + j], before = j ? path[s.q0 + j - 1] : -1;
-        if (c <= before || c >= s.n) {
+        if (!path_goes_on(path + a.s.q0, j, a.s.n)) {
             atomicMin(&bad, j);
             continue;
         }
+        const int c = path[a.s.q0 + j];
         if (c != j) atomicMin(&first, j);
         auto row = [&](int pos, bool written) -> int {
             const int col = (int)w.ps.div((uint32_t)pos);
-            const int page = page_at(w, s.row[col]);
+            const int page = page_at(w, a.s.row[col]);
             if (page >= 0 && written && w.refs[page] > 1) {
                 paged_fault(PAGED_SHARED);  // others hold it too: not written
                 return -1;
             }
             return page < 0 ? -1 : page * w.Hkv * w.page_size + (pos - col * w.page_size);
         };
-        const int a = c == j ? -1 : row(start + c, false);
-        const int z = c == j ? -1 : row(start + j, true);
-        from[j] = z < 0 ? -1 : a;
+        const int x = c == j ? -1 : row(a.start + c, false);
+        const int z = c == j ? -1 : row(a.start + j, true);
+        from[j] = z < 0 ? -1 : x;
         to[j] = z;
     }
     __syncthreads();
@@ -157,7 +176,7 @@ __global__ void __cluster_dims__(ACCEPT_CLUSTER) __launch_bounds__(ACCEPT_THREAD
     const int per_row = pool.row_bytes / 16;
     const int per_layer = 2 * w.Hkv * per_row;
     const int64_t items = first < m ? (int64_t)pool.n_layers * per_layer : 0;
-    for (int64_t i = (int64_t)part * ACCEPT_THREADS + tid; i < items; i += ACCEPT_CLUSTER * ACCEPT_THREADS) {
+    for (int64_t i = (int64_t)part * ACCEPT_THREADS + tid; i < items; i += ACCEPT_CTAS * ACCEPT_THREADS) {
         const int layer = (int)(i / per_layer);
         int r = (int)(i - (int64_t)layer * per_layer);
         const int x = r % per_row;
@@ -177,13 +196,28 @@ __global__ void __cluster_dims__(ACCEPT_CLUSTER) __launch_bounds__(ACCEPT_THREAD
                     *reinterpret_cast<uint4*>(base + (int64_t)to[j0 + k] * pool.row_bytes) = y[k];
         }
     }
-    // every CTA has read the length and the table
-    cooperative_groups::this_cluster().sync();
-    if (part || m < 0) return;
-    const int now = start + m;
-    const int keep = (now + w.page_size - 1) / w.page_size, used = (s.L + w.page_size - 1) / w.page_size;
-    int32_t* const row = table + (size_t)slot * w.max_pages;
-    for (int j = keep + tid; j < used; j += ACCEPT_THREADS) {
+}
+
+// Lengths, and the pages behind them given back: a CTA to a sequence.  It starts beside the moves, which
+// change nothing that it reads, and waits for them before it changes what they read.
+constexpr int GIVE_THREADS = 128;
+__global__ void __launch_bounds__(GIVE_THREADS)
+    tree_give_back_kernel(const PagedView w, int max_nodes, int32_t* table, int32_t* len, int32_t* refs,
+                          const int32_t* __restrict__ path, const int32_t* __restrict__ n_path) {
+    __shared__ int bad;
+    const int b = blockIdx.x, tid = threadIdx.x;
+    if (tid == 0) bad = IB_KV_MAX_NODES;
+    const Accepted a = accepted(w, max_nodes, n_path, b, false);
+    __syncthreads();
+    for (int j = tid; j < a.m; j += GIVE_THREADS)
+        if (!path_goes_on(path + a.s.q0, j, a.s.n)) atomicMin(&bad, j);
+    __syncthreads();
+    const int now = a.start + min(a.m, bad);
+    const int keep = (now + w.page_size - 1) / w.page_size, used = (a.s.L + w.page_size - 1) / w.page_size;
+    pdl_wait();
+    if (a.m < 0) return;
+    int32_t* const row = table + (size_t)a.slot * w.max_pages;
+    for (int j = keep + tid; j < used; j += GIVE_THREADS) {
         const int t = row[j];
         row[j] = -1;
         if (t >= 0 && t < w.n_pages) {
@@ -195,7 +229,7 @@ __global__ void __cluster_dims__(ACCEPT_CLUSTER) __launch_bounds__(ACCEPT_THREAD
             paged_fault(PAGED_BAD_PAGE);
         }
     }
-    if (tid == 0) len[slot] = now;
+    if (tid == 0) len[a.slot] = now;
 }
 
 static int tree_batch(const ib_kv_batch* b, const char* who) {
@@ -281,9 +315,11 @@ static int tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const i
     if (batch->n_seqs == 0) return IB_OK;
     if (!path || !n_path) return paged_refuse(who, "null pointer argument");
     const PagedView w = paged_view(pages, seqs, batch, pages->n_kv_heads);
-    IB_CUDA_CHECK(launch_pdl(tree_accept_kernel, dim3(batch->n_seqs * ACCEPT_CLUSTER), dim3(ACCEPT_THREADS),
-                             0, as_stream(stream), true, w, max_nodes, seqs->table, seqs->len, seqs->refs,
-                             pool_bytes(pages), path, n_path));
+    cudaStream_t st = as_stream(stream);
+    IB_CUDA_CHECK(launch_pdl(tree_move_kernel, dim3(batch->n_seqs * ACCEPT_CTAS), dim3(ACCEPT_THREADS), 0, st,
+                             true, w, max_nodes, pool_bytes(pages), path, n_path));
+    IB_CUDA_CHECK(launch_pdl(tree_give_back_kernel, dim3(batch->n_seqs), dim3(GIVE_THREADS), 0, st, true, w,
+                             max_nodes, seqs->table, seqs->len, seqs->refs, path, n_path));
     return IB_OK;
 }
 

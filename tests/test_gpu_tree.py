@@ -859,3 +859,35 @@ def test_a_step_with_a_tree_that_is_too_large(cuda, type_, n, most):
             at = table[b, p // page].item()
             assert cuda.equal(pages.k[:, at, :, p % page], k[:, at, :, p % page])
             assert cuda.equal(pages.v[:, at, :, p % page], v[:, at, :, p % page])
+
+
+@TYPES
+def test_accept_by_the_counts_before_the_call(cuda, type_):
+    """Sequences forked with their nodes: a page that one of the two gives back in the call is not written
+    by the other, in any layer."""
+    page, ctx, n, pairs = 4, 5, 11, 64
+    book = Book(2 * pairs, 4, 4 * pairs + 8, page)
+    assert book.extend(range(pairs), [ctx + n] * pairs) == [1] * pairs
+    status, copies = book.fork(range(pairs), range(pairs, 2 * pairs))
+    assert status == [1] * pairs and not copies
+    pages = pool(cuda, 24, 4 * pairs + 8, 2, page, 64, type_, 1)
+    k, v = pages.k.clone(), pages.v.clone()
+    cu = i32(cuda, range(0, 2 * pairs * n + 1, n))
+    long, short = [1, 3, 4, 7, 8, 10], [0]  # entries for pages 1 and 2; 2 and 3 are given back by the others
+    path = i32(cuda, [x for p in (long, short) for _ in range(pairs) for x in p + [-1] * (n - len(p))])
+    n_path = i32(cuda, [len(long)] * pairs + [len(short)] * pairs)
+    for order in (range(2 * pairs), [b // 2 + pairs * (b % 2) for b in range(2 * pairs)]):
+        slots = i32(cuda, order)
+        seqs = seqs_of(cuda, book)
+        batch = ib.KVBatch(cu, 2 * pairs * n, slots=slots)
+        rows = slots.long()  # of the lists, which go by slots
+        ib.kv_tree_accept(pages, seqs, batch, path.view(-1, n)[rows].flatten().contiguous(), n_path[rows].contiguous())
+        assert cuda.equal(pages.k, k) and cuda.equal(pages.v, v)
+        with pytest.raises(RuntimeError, match="77"):
+            ib.check_fault()
+        assert seqs.len.tolist() == [ctx + len(long)] * pairs + [ctx + len(short)] * pairs
+        for b in range(2 * pairs):
+            keep = 3 if b < pairs else 2
+            assert seqs.table[b].tolist() == book.table[b][:keep] + [-1] * (4 - keep)
+            held = book.table[b % pairs]
+            assert [seqs.refs[p].item() for p in held] == [2, 2, 1, 0]
