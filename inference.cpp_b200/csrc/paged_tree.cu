@@ -274,7 +274,8 @@ static int tree_verify(const ib_kv_batch* batch, int max_nodes, const int32_t* p
     if (max_nodes < 1 || max_nodes > IB_KV_MAX_NODES)
         return paged_refuse(who, "max_nodes must be in [1, 1024]");
     if (batch->n_seqs == 0) return IB_OK;
-    if (!parents || !tokens || !best || !path || !n_path || !next)
+    // (lists of no nodes may be null)
+    if ((batch->n_tokens && (!parents || !tokens || !best || !path)) || !n_path || !next)
         return paged_refuse(who, "null pointer argument");
     const int64_t T = batch->n_tokens, B = batch->n_seqs;
     const void* const out[3] = {path, n_path, next};
@@ -313,7 +314,7 @@ static int tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const i
     if (max_nodes < 1 || max_nodes > IB_KV_MAX_NODES)
         return paged_refuse(who, "max_nodes must be in [1, 1024]");
     if (batch->n_seqs == 0) return IB_OK;
-    if (!path || !n_path) return paged_refuse(who, "null pointer argument");
+    if ((batch->n_tokens && !path) || !n_path) return paged_refuse(who, "null pointer argument");
     const PagedView w = paged_view(pages, seqs, batch, pages->n_kv_heads);
     cudaStream_t st = as_stream(stream);
     IB_CUDA_CHECK(launch_pdl(tree_move_kernel, dim3(batch->n_seqs * ACCEPT_CTAS), dim3(ACCEPT_THREADS), 0, st,

@@ -891,3 +891,28 @@ def test_accept_by_the_counts_before_the_call(cuda, type_):
             assert seqs.table[b].tolist() == book.table[b][:keep] + [-1] * (4 - keep)
             held = book.table[b % pairs]
             assert [seqs.refs[p].item() for p in held] == [2, 2, 1, 0]
+
+
+@TYPES
+def test_a_step_without_tokens(cuda, type_):
+    """Every sequence left out, or none with a new token: each call of the step is allowed and changes nothing."""
+    H, Hkv, HD, page = 4, 2, 64, 16
+    book = Book(3, 9, 30, page)
+    book.extend([0, 1, 2], [30, 50, 11])
+    seqs, pages = seqs_of(cuda, book), pool(cuda, 2, 30, Hkv, page, HD, type_, 3)
+    k, v = pages.k.clone(), pages.v.clone()
+    none = i32(cuda, [])
+    for slots in (None, i32(cuda, [-1, -1, -1])):
+        batch = ib.KVBatch(i32(cuda, [0, 0, 0, 0]), 0, slots=slots)
+        tree = ib.kv_tree(batch, none)
+        q = cuda.zeros(0, H, HD, device="cuda")
+        kn = cuda.zeros(0, Hkv, HD, device="cuda")
+        ib.kv_append(pages, seqs, batch, 1, q, kn, kn, rope_table(cuda, 100, HD), tree=tree)
+        assert ib.attention_paged(pages, seqs, batch, 1, q, 0.1, tree=tree).shape == q.shape
+        for kw in ({}, dict(tree=tree)):
+            path, n_path, nxt = ib.kv_tree_verify(batch, none, none, none, **kw)
+            assert path.numel() == 0 and n_path.tolist() == [0] * 3 and nxt.tolist() == [-1] * 3
+            ib.kv_tree_accept(pages, seqs, batch, path, n_path, **kw)
+        assert seqs.len.tolist() == book.len and seqs.refs.tolist() == book.refs and seqs.table.tolist() == book.table
+    assert cuda.equal(pages.k, k) and cuda.equal(pages.v, v)
+    assert ib.check_fault() == 0
