@@ -427,8 +427,8 @@ int ib_kv_tree_accept_max(const ib_kv_pages* pages, const ib_kv_seqs* seqs, cons
  *     scores[r] + logits[r][t] - log sum_t' e^logits[r][t'];
  * a row with ended[r] != 0 offers end_token alone, with the value scores[r], and its logits are not
  * read.  A group's k largest go to out_score, out_token and out_row [n_groups][k] (out_row: the row),
- * largest first, equal values in the order of row and token.  Values are compared in more than FP32
- * and rounded once.  Those that are -inf or NaN are no candidates: a banned token's -inf, a row whose
+ * largest first, equal values in the order of row and token; inside a row the order is that of its
+ * logits.  Values are compared in more than FP32 and rounded once.  Those that are -inf or NaN are no candidates: a banned token's -inf, a row whose
  * score is -inf, all of a row with a NaN or +inf logit.  Places without a candidate: -inf, -1, -1.
  * scores and ended may be NULL (zeros).  With beams = 1 it is the rows' top k; with k = 1 their first
  * maximum, as ib_argmax.  beams in [1, IB_BEAM_MAX_BEAMS], n_groups x beams <= 2^20, vocab <= 2^28,

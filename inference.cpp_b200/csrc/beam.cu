@@ -322,12 +322,15 @@ __global__ void __launch_bounds__(BS_THREADS) beam_slice_kernel(const __grid_con
     }
 }
 
+// Of two candidates of a row the one with the larger key is better, whatever their values round to in 64 bits.
 struct Best {
     double v;
-    uint64_t place;  // row in the group, token
+    uint64_t key;  // of the logit and its token
+    int row;       // in the group
 };
+constexpr int BS_NO_ROW = 0x7fffffff;
 __device__ __forceinline__ bool better(const Best& a, const Best& b) {
-    return a.v > b.v || (a.v == b.v && a.place < b.place);
+    return a.v > b.v || (a.v == b.v && (a.row < b.row || (a.row == b.row && a.key > b.key)));
 }
 
 constexpr int BS_GROUP_CAP = 1024;
@@ -336,8 +339,8 @@ __device__ __forceinline__ void put_choice(const SelectArgs& A, int g, int j, co
     const bool any = y.v > -INFINITY;
     const int64_t at = (int64_t)g * A.k + j;
     A.out_score[at] = any ? (float)y.v : -INFINITY;
-    A.out_token[at] = any ? (int32_t)(uint32_t)y.place : -1;
-    A.out_row[at] = any ? g * A.beams + (int32_t)(y.place >> 32) : -1;
+    A.out_token[at] = any ? (int32_t)key_place(y.key) : -1;
+    A.out_row[at] = any ? g * A.beams + y.row : -1;
 }
 
 // Candidate c of group g, whose key is `key`: entry c % k of list c / k, a row's slice; v is -inf where
@@ -345,13 +348,14 @@ __device__ __forceinline__ void put_choice(const SelectArgs& A, int g, int j, co
 __device__ __forceinline__ Best candidate(const SelectArgs& A, int c, uint64_t key, const double2* base) {
     const int b = (int)A.of_slices.div(A.of_k.div((uint32_t)c));
     const double2 y0 = base[b];
-    Best y = {-INFINITY, ~0ull};
+    Best y = {-INFINITY, 0, BS_NO_ROW};
     if (y0.y != y0.y) {
-        if (c == b * A.slices * A.k) y = Best{y0.x, ((uint64_t)b << 32) | (uint32_t)A.end_token};
+        if (c == b * A.slices * A.k) y = Best{y0.x, beam_key(0.f, (uint32_t)A.end_token), b};
     } else if (key) {
-        y = Best{y0.x + ((double)key_value(key) - y0.y), ((uint64_t)b << 32) | key_place(key)};
+        y = Best{y0.x + ((double)key_value(key) - y0.y), key, b};
     }
     if (!(y.v > -INFINITY)) y.v = -INFINITY;  // NaN is no candidate
+    y.v += 0.0;                               // -0 and 0 are equal
     return y;
 }
 
@@ -361,10 +365,10 @@ __device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, cons
                                          const double2* base) {
     __shared__ Best sh_best[2][BS_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    Best last = {INFINITY, 0};
+    Best last = {INFINITY, 0, 0};
     bool first = true;
     for (int j = 0; j < A.k; ++j, first = false) {
-        Best top = {-INFINITY, ~0ull};
+        Best top = {-INFINITY, 0, BS_NO_ROW};
         for (int c = tid; c < n; c += BS_THREADS) {
             const Best y = candidate(A, c, list[c], base);
             if ((first || better(last, y)) && better(y, top)) top = y;
@@ -373,7 +377,8 @@ __device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, cons
         for (int o = 16; o > 0; o >>= 1) {
             Best y;
             y.v = __shfl_xor_sync(0xffffffffu, top.v, o);
-            y.place = __shfl_xor_sync(0xffffffffu, top.place, o);
+            y.key = __shfl_xor_sync(0xffffffffu, top.key, o);
+            y.row = __shfl_xor_sync(0xffffffffu, top.row, o);
             if (better(y, top)) top = y;
         }
         if (lane == 0) sh_best[j & 1][warp] = top;
@@ -392,7 +397,9 @@ __device__ __noinline__ void group_again(const SelectArgs& A, int g, int n, cons
 // four in a graph, where it is launched beside the slices.
 __global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_constant__ SelectArgs A) {
     extern __shared__ __align__(16) double2 base[];  // [beams]
-    __shared__ Best buf[BS_GROUP_CAP];
+    __shared__ double buf_v[BS_GROUP_CAP];  // of those that are ranked; the rest is read where values are equal
+    __shared__ uint64_t buf_key[BS_GROUP_CAP];
+    __shared__ int buf_row[BS_GROUP_CAP];
     __shared__ uint32_t sh_top[2][BS_WARPS];
     __shared__ int sh_n;
     const int tid = threadIdx.x, g = blockIdx.x, row0 = g * A.beams, k = A.k;
@@ -430,26 +437,28 @@ __global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_con
     // rounding down keeps the order, so that k values at or above it are above all below it
     auto low = [](double v) { return v > -INFINITY ? ordered(__double2float_rd(v)) : 0u; };
     uint32_t best = 0;
-    Best mine[AHEAD];
+    double mine[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
         const int c = tid + i * BS_THREADS;
-        mine[i] = Best{-INFINITY, ~0ull};
-        if (c < n) mine[i] = candidate(A, c, key[i], base);
-        best = max(best, low(mine[i].v));
+        mine[i] = c < n ? candidate(A, c, key[i], base).v : -INFINITY;
+        best = max(best, low(mine[i]));
     }
     for (int c = tid + AHEAD * BS_THREADS; c < n; c += BS_THREADS)
         best = max(best, low(candidate(A, c, list[c], base).v));
     int reach;
     const uint32_t least = max(reached(best, k, sh_top, reach), 1u);
     auto take = [&](const Best& y) {
-        if (low(y.v) < least) return;
         const int to = atomicAdd(&sh_n, 1);
-        if (to < BS_GROUP_CAP) buf[to] = y;
+        if (to < BS_GROUP_CAP) buf_v[to] = y.v, buf_key[to] = y.key, buf_row[to] = y.row;
     };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) take(mine[i]);
-    for (int c = tid + AHEAD * BS_THREADS; c < n; c += BS_THREADS) take(candidate(A, c, list[c], base));
+    for (int i = 0; i < AHEAD; ++i)
+        if (low(mine[i]) >= least) take(candidate(A, tid + i * BS_THREADS, key[i], base));
+    for (int c = tid + AHEAD * BS_THREADS; c < n; c += BS_THREADS) {
+        const Best y = candidate(A, c, list[c], base);
+        if (low(y.v) >= least) take(y);
+    }
     __syncthreads();
     const int some = sh_n;
     if (some > BS_GROUP_CAP) {
@@ -457,13 +466,16 @@ __global__ void __launch_bounds__(BS_THREADS) beam_group_kernel(const __grid_con
         return;
     }
     for (int i = tid; i < some; i += BS_THREADS) {
-        const Best own = buf[i];
+        const Best own = {buf_v[i], buf_key[i], buf_row[i]};
         int rank = 0;
 #pragma unroll 4
-        for (int j = 0; j < some; ++j) rank += better(buf[j], own);
+        for (int j = 0; j < some; ++j) {
+            rank += buf_v[j] > own.v;
+            if (buf_v[j] == own.v && j != i) rank += better(Best{own.v, buf_key[j], buf_row[j]}, own);
+        }
         if (rank < k) put_choice(A, g, rank, own);
     }
-    for (int j = some + tid; j < k; j += BS_THREADS) put_choice(A, g, j, Best{-INFINITY, ~0ull});
+    for (int j = some + tid; j < k; j += BS_THREADS) put_choice(A, g, j, Best{-INFINITY, 0, BS_NO_ROW});
 }
 
 // How a call is cut.

@@ -527,3 +527,47 @@ def test_reorder_of_few_and_many(cuda, n, max_pages):
             parents[rng.randrange(n)] = n
         run_reorder(cuda, book, seqs, pages, names, parents)
     assert ib.check_fault() == 0
+
+
+@pytest.mark.parametrize("vocab", [300, 5000, 40000])
+def test_select_orders_a_row_by_its_logits(cuda, vocab):
+    """Values that 64 bits do not tell apart once the log sum is taken off (logits next to zero, large scores):
+    a row's order is that of its logits, and with k = 1 the choice is the first maximum."""
+    x = cuda.full((2, vocab), -3.0, device="cuda")
+    at = [2, 7, vocab // 2, vocab - 300 + 50, vocab - 1]
+    x[:, at] = cuda.tensor([1e-30, 3e-30, 2e-30, -1e-30, 3e-30], device="cuda")
+    order = [at[1], at[4], at[2], at[0], at[3]]
+    one = cuda.zeros(1, dtype=cuda.int32, device="cuda")
+    ib.argmax(x[0].contiguous(), vocab, one)
+    assert one.item() == at[1]
+    for scores in (None, cuda.tensor([-1.5, -4.0], device="cuda"), cuda.tensor([1e25, 1e24], device="cuda")):
+        for k in (1, 2, 5):
+            out = ib.beam_select(x, scores, k=k)
+            assert out.token.tolist() == [order[:k]] * 2 and out.row.tolist() == [[0] * k, [1] * k]
+        out = ib.beam_select(x, scores, beams=2, k=10)
+        if scores is not None and scores[0] > 1e24:  # all of the first row's values are above the second's
+            assert out.token.tolist() == [order + [0, 1, 3, 4, 5]] and out.row.tolist() == [[0] * 10]
+        else:
+            assert out.token.tolist() == [order * 2] and out.row.tolist() == [[0] * 5 + [1] * 5]
+    # many rows of them: the kernel's slow path
+    out = ib.beam_select(x.repeat(400, 1), beams=800, k=128)
+    assert out.row.tolist() == [[i // 5 for i in range(128)]] and out.token.tolist() == [(order * 26)[:128]]
+    assert ib.check_fault() == 0
+
+
+@DT
+def test_select_signed_zeros_are_equal(cuda, dt):
+    """Ended rows that offer 0 and -0, and logits of both: the lowest row and token win."""
+    ones = cuda.ones(64, dtype=cuda.int32, device="cuda")
+    x = cuda.zeros(64, 100, dtype=getattr(cuda, dt), device="cuda")
+    for at in (0, 3, 63):
+        scores = cuda.zeros(64, device="cuda")
+        scores[at] = -0.0
+        for k in (1, 8, 9):
+            out = ib.beam_select(x, scores, beams=64, k=k, ended=ones, end_token=5)
+            assert out.row.tolist() == [list(range(k))] and out.token.tolist() == [[5] * k]
+            assert not bool(out.score.any())
+    x[:, ::2] = -0.0
+    out = ib.beam_select(x, beams=64, k=8)
+    assert out.row.tolist() == [[0] * 8] and out.token.tolist() == [list(range(8))]
+    assert ib.check_fault() == 0
