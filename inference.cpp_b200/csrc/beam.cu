@@ -11,6 +11,12 @@
 // memory and are ranked at the end.  A second kernel, a CTA per group, makes the rows' log sums of the
 // slices' and picks the group's k best in 64 bits, through a threshold again: candidates of different
 // beams may be closer than FP32 tells apart.
+//
+// What that holds.  Inside a row the choice and its order are exact.  A row's log sum has the error of its FP32
+// parts: a thread adds 16 weights e^(x - m) in a step of 4096 values, the threads' and slices' sums are joined
+// in 64 bits, so with S steps to a slice it is off by at most (S + 1) (A + 24) 2^-24, A = sum p (max x - x).
+// Candidates of different rows that are closer than their rows' errors come in either order, and the
+// errors, not the candidates, depend on how the rows are cut.
 #include <cuda_fp16.h>
 #include <float.h>
 
@@ -121,9 +127,12 @@ __device__ __forceinline__ Two add(Two a, Two b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t.x) : "l"(a.x), "l"(b.x));
     return t;
 }
-// e^t for t <= 0: 2^(t log2 e) with log2 e in two parts (one alone is 1e-8 short, for all values alike).
+// e^t for t <= 0: 2^(t log2 e) with log2 e in two parts (one alone is 1e-8 short, for all values alike).  Off by
+// at most (4 + 2 |t|) 2^-24 of itself: 2^-22 of ex2.approx, and two roundings of its argument.
 __device__ __forceinline__ Two exp_of(Two t) {
-    const Two hi = Two::of(1.442695022f, 1.442695022f), lo = Two::of(1.925963033e-8f, 1.925963033e-8f);
+    constexpr double LOG2E = 1.4426950408889634;
+    constexpr float HI = (float)LOG2E, LO = (float)(LOG2E - (double)HI);
+    const Two hi = Two::of(HI, HI), lo = Two::of(LO, LO);
     Two y;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y.x) : "l"(t.x), "l"(hi.x));
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(y.x) : "l"(t.x), "l"(lo.x));

@@ -571,3 +571,21 @@ def test_select_signed_zeros_are_equal(cuda, dt):
     out = ib.beam_select(x, beams=64, k=8)
     assert out.row.tolist() == [[0] * 8] and out.token.tolist() == [list(range(8))]
     assert ib.check_fault() == 0
+
+
+def test_select_weights_of_a_log_sum(cuda):
+    """The weights e^t of a row's log sum, t from 0 down: rows of 256 zeros, one among each 16 values, and t.
+    With w the weights' share of the sum, |error| <= |v| 2^-24 (the result's rounding) + w (4 + 2 |t|) 2^-24 (a
+    weight: 2^-22 of the instruction, two roundings of its argument) + 8 2^-24 (a thread's sum)."""
+    t = -np.concatenate([np.geomspace(1e-7, 100, 1500), np.linspace(0, 20, 500), [87.0, 88.0, 103.0, 104.0, 1e4, 3e38]])
+    t = t.astype(np.float32)
+    x = cuda.tensor(t, device="cuda")[:, None].repeat(1, 4096)
+    x[:, 0:1024:4] = 0.0
+    out = ib.beam_select(x, k=1)
+    t = t.astype(np.float64)
+    weight = 15 * np.exp(t)
+    want = -(math.log(256) + np.log1p(weight))
+    got = out.score.flatten().cpu().numpy().astype(np.float64)
+    tol = (np.abs(want) + weight / (1 + weight) * (4 + 2 * np.abs(t)) + 8) * 2.0 ** -24
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+    assert not bool(out.token.any()) and ib.check_fault() == 0
