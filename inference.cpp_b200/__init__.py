@@ -739,8 +739,6 @@ def kv_release(pages, seqs, slots, stream=None):
 
 def _workspace(pages, workspace):
     """(pointer, bytes) of a caller's workspace on the pages' device."""
-    if workspace.device == pages.device and workspace.is_contiguous():
-        return workspace.data_ptr(), workspace.nbytes
     if workspace.device != pages.device or not workspace.is_contiguous():
         raise ValueError(f"workspace: on {workspace.device}, contiguous "
                          f"{workspace.is_contiguous()}; expected contiguous on {pages.device}")

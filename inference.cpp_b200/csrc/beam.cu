@@ -24,7 +24,7 @@
 #include <string>
 
 #include "common.cuh"
-#include "paged.cuh"  // FastDiv, checks
+#include "paged.cuh"  // FastDiv, kSMs, checks
 #include "pdl.cuh"
 
 namespace ib {
@@ -47,15 +47,6 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 __device__ __forceinline__ uint32_t key_place(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
 
-__device__ __forceinline__ uint64_t shfl_max(uint64_t x) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t y = __shfl_xor_sync(0xffffffffu, x, o);
-        x = y > x ? y : x;
-    }
-    return x;
-}
-
 // Numbers that sort as the values do (no NaN).
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -64,8 +55,8 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 
 // A number that at least k of the CTA's threads' `best` reach, where that many are above 0 (else 0).  First
 // the least of the warps' n-th largest, n = k / BS_WARPS rounded up; then, where many more reach it,
-// halving between it and the largest of all, a barrier a step, until a quarter more than k do or a few
-// steps are over.  n: how many reach it.
+// halving between it and the largest of all, a barrier a step, until no more than a quarter above k do or the
+// interval is used up (at most 32 steps: it is one of 32-bit numbers).  n: how many reach it.
 __device__ __forceinline__ uint32_t reached(uint32_t best, int k, uint32_t (&sh)[2][BS_WARPS], int& n) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t top = 0, most = 0, x = best;
@@ -101,7 +92,7 @@ struct SelectArgs {
     int64_t stride;
     const float* scores;     // null: zeros
     const int32_t* ended;    // null: none
-    int rows, beams, vocab, k, slices, end_token;
+    int beams, vocab, k, slices, end_token;
     int64_t per_slice;       // values
     FastDiv of_k, of_slices;
     uint64_t* list;          // [row][slice][k] keys, largest first, zeros behind
@@ -494,7 +485,6 @@ struct SelectPlan {
     size_t list_off, meta_off, bytes;
 };
 
-constexpr int kSMs = 148;  // of a B200
 static SelectPlan select_plan(int64_t rows, int64_t vocab, int k) {
     SelectPlan p;
     const int64_t tiles = (vocab + BS_TILE - 1) / BS_TILE;
@@ -572,7 +562,6 @@ extern "C" int ib_beam_select(int type, const void* logits, int64_t stride, cons
     a.stride = stride;
     a.scores = scores;
     a.ended = ended;
-    a.rows = (int)rows;
     a.beams = beams;
     a.vocab = vocab;
     a.k = k;

@@ -13,6 +13,8 @@
 
 namespace ib {
 
+constexpr int kSMs = 148;  // of a B200: how a call's work is cut, and so its workspace, follow it
+
 // Codes of the paged kernels' fault word.
 enum {
     PAGED_BAD_SLOT = 71,   // a slot outside [0, n_slots)

@@ -9,8 +9,6 @@
 
 namespace ib {
 
-constexpr int kSMs = 148;  // of a B200: the pieces aimed at, and so the workspace, follow it
-
 // ---- cutting a batch into pieces ---------------------------------------------------------
 // Sequences with rows in [min_rows, max_rows] take part, in tiles of R rows and key tiles of KT
 // positions, in n_pieces pieces of at least `least` positions of one token.

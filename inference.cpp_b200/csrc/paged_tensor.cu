@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
                     ok = ok && wait(&bar.kv_full[h % C::SLOTS], h / C::SLOTS);
                     // written by cp.async, read by the tensor core (stores are followed by a fence of their
                     // own, TMA needs none)
-                    if (!SPLIT || (!F32 && !TA.box)) pt_fence_async();
+                    pt_fence_async();
                 };
                 if constexpr (SPLIT) {
                     // Every K and V tile once, in the ring's order: O of key tile j, then the scores of key tile
@@ -929,7 +929,7 @@ __global__ void __launch_bounds__(TensorCfg<KV, HDP, SPLIT>::THREADS, 1)
                             advance();
                         }
                         if (s) ok = ok && wait(&bar.kv_full[slot], uses);
-                        if (!SPLIT || (!F32 && !TA.box)) pt_fence_async();  // written by cp.async
+                        if (!F32 && !TA.box) pt_fence_async();  // written by cp.async
                         if (j >= 0) {
                             if (j == 0) {  // the last segment's masks and its second group's sums have been read
 #pragma unroll 1
