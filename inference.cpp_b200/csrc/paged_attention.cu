@@ -1079,7 +1079,10 @@ static CutRule narrow_rule(int min_rows, int max_rows) {
 // 1024; two to four nodes, 32 heads on 8 of 128: 8 trees over 480, 900 and 200 .. 4096 positions, FP16, 21:17
 // 31:23 44:35; 48 over 240, 480, 100 .. 900 and 200 .. 4096 34:29 46:37 47:39 99:99; 24 on FP32 pages over 240,
 // 900 and 200 .. 4096 30:24 51:57 108:102; one over 60000 73:76).  Over tables of no more than 192 positions
-// nothing is cut, which takes a launch less: 10.2 and 9.0 us for 7 nodes over 130 (FP32, 6 heads of 48).
+// nothing is cut, which takes a launch less (us over tables of 144 to 192 positions, cut at 128 and whole; one and
+// four nodes): FP32, 6 heads of 48, 1 tree 9.8:9.1 10.1:9.0, 64 trees 21:15 22:16; 32 heads on 8 of 128, FP16, 1 tree
+// 10.5:9.3 11.1:9.9, 4 trees 10.8:10.7 14.6:10.6, 64 trees 30:22 53:36; FP32, 1 tree 12.5:12.4 13.2:13.0, 64 trees
+// 42:33 77:60; 4 of 64, FP16, 64 trees 17.5:11.3 25.2:25.1.
 template <typename KV, int HDP>
 static CutRule narrow_tree_rule(int min_rows, int max_rows, int64_t max_pos) {
     CutRule r = narrow_rule<KV, HDP>(min_rows, max_rows);
@@ -1144,15 +1147,20 @@ template <typename KV, int HDP>
 constexpr int narrow_tree_rows = HDP > 128 ? 32 : sizeof(KV) == 2 && HDP == 128 ? 16 : 24;
 
 // Few trees over tables of short rows are the narrow kernel's whatever their rows: the wide one's start alone
-// takes 10 us and more, two tiles of eight rows to an SM less.  Narrow against wide (us, 32 heads; FP16 pages,
-// 8 kv heads of 128 and 4 of 64; FP32 pages likewise), by the positions of a sequence:
-//   trees x rows        tiles      100                            300                            700
-//   1 x 128, 1 x 256    128        16:21  14:20  19:29  16:25     18:23  16:22  27:45  18:35     26:26  20:25  44:79  26:28
-//   4 x 64, 4 x 128     256        14:16  12:14  19:24  14:16     24:20  19:17  39:40  24:23     35:26  26:20  56:76  35:25
-//   4 x 128, 4 x 256    512        32:21  25:21  46:29  30:26     40:23  30:23  64:45  39:36     52:29  37:29  97:80  54:35
-// so: two tiles to an SM, and 64000 positions in all of them.
+// takes 10 us and more, two tiles of eight rows to an SM less.  Narrow against wide (us in a graph, 32 heads; FP16
+// pages, 8 kv heads of 128 and 4 of 64; FP32 pages likewise), by the tables' positions:
+//   trees x rows  tiles        224                           480                           720
+//   1 x 256       264, 132     16:28  16:20  22:34  17:29    21:36  17:25  32:54  20:28    27:35  18:25  41:38  22:28
+//   4 x 64        272, 136     16:17  16:14  23:32  17:20    21:22  17:17  33:52  20:22    27:26  18:20  43:42  23:23
+//   8 x 64        544, 272     29:17  15:14  40:32  17:20    40:22  16:18  62:54  23:28    50:33  19:22  83:67  30:30
+//   4 x 256       1040, 520    49:28  22:20  72:34  28:29    65:36  28:25  117:55 41:32    80:48  34:29  158:66 52:32
+// and fewer tiles, by tiles x positions:
+//                 tiles        64000                         100000                        140000
+//   1 x 64        72, 36       18:23  16:20  24:36  20:24    21:23  18:21  33:37  23:26    23:24  21:22  39:38  28:34
+//   2 x 128       264, 132     17:21  17:18  24:33  20:22    19:23  18:20  29:43  23:23    22:25  20:20  34:38  27:23
+// so: two tiles to an SM, and 128000 positions in all of them.
 static bool few_short_trees(int64_t tiles, int64_t max_pos) {
-    return tiles <= 2 * kSMs && tiles * max_pos <= 64000;
+    return tiles <= 2 * kSMs && tiles * max_pos <= 128000;
 }
 
 // Wide tiles run on tcgen05 for head_dim up to 128.  Above, S and O of two query tiles do not fit
