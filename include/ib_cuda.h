@@ -400,7 +400,8 @@ int ib_attention_paged_tree(const ib_kv_pages* pages, const ib_kv_seqs* seqs, co
  * tokens, best [n_tokens], ib_beam_select with k = 1 for the last).  Sequence b's path, n_path[b]
  * nodes, is written to its rows of path [n_tokens] (-1 behind it), and next[b] = best of its last node,
  * the token to go on with.  A sequence without nodes (left out, or more than IB_KV_MAX_NODES):
- * n_path 0, next -1.  Results must not overlap the lists.
+ * n_path 0, next -1.  Results must not overlap the lists.  (Here and below a list [n_tokens] of a
+ * batch without tokens may be NULL.)
  * ib_kv_tree_verify_max: the same for a step whose trees have a max_nodes of their own: a sequence
  * with more has no nodes, as in its append and attention. */
 int ib_kv_tree_verify(const ib_kv_batch* batch, const int32_t* parents, const int32_t* tokens,
@@ -413,8 +414,8 @@ int ib_kv_tree_verify_max(const ib_kv_batch* batch, int max_nodes, const int32_t
  * the caller's own verification), len becomes len - n + n_path and the pages behind it are given back.
  * n_path 0 drops all new tokens.  Recorded and passed over: n_path out of [0, n] (78: nothing is
  * changed); a length below the number of new tokens (73: likewise); an entry that is no node behind
- * the one before (78: the path ends there); a move into a page that others hold too (77).  Moves from
- * or to a page that is not there are passed over.  A sequence with more new tokens than
+ * the one before (78: the path ends there); a move into a page that others hold too, by the counts before
+ * the call (77).  Moves from or to a page that is not there are passed over.  A sequence with more new tokens than
  * IB_KV_MAX_NODES was left out of the step, so nothing has been written for them: all are dropped (78).
  * ib_kv_tree_accept_max: the same with the max_nodes of the step's trees. */
 int ib_kv_tree_accept(const ib_kv_pages* pages, const ib_kv_seqs* seqs, const ib_kv_batch* batch,

@@ -227,10 +227,11 @@ __device__ __noinline__ void slice_again(SliceShared& sh, const T* x, int64_t be
     rank_best(sh, sh.n, k, out);
 }
 
-// Bound by the instructions of a value (17, and 10 cycles between two of a warp's): 16 groups of 8 beams over
-// 128256 FP32 logits, 62 MB, take 21 us with cold caches, 3.0 TB/s, issue slots 0.53; the call 22.9 us in a
-// graph, 74 before loads of 16 bytes a step ahead and a threshold of the first step's.  With four CTAs to the busiest SM, 3.5 to the
-// mean one; more and shorter slices cost what they gain (select_plan).
+// 16 groups of 8 beams over 128256 FP32 logits, 62 MB, take 21 us with cold caches, 3.0 TB/s; the call 23 us in
+// a graph, 74 before loads of 16 bytes a step ahead and a threshold of the first step's.  Neither HBM (0.36) nor
+// issue slots (0.53) are used up: a step's instructions, 17 to a value, wait for one another (10 cycles
+// between two of a warp's), and four CTAs are on the busiest SM, 3.5 on the mean one; more and shorter
+// slices cost what they gain (select_plan).
 // VEC: values of one load (16 bytes where the rows allow it, else one).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(BS_THREADS) beam_slice_kernel(const __grid_constant__ SelectArgs A) {
