@@ -12,7 +12,8 @@
 // Products of FP32 operands keep 2^-20 or better on the tensor cores:
 //   FP16 pages  q = hi + lo and p = hi + lo in FP16, K and V as they are: two products.  q rows
 //               are scaled to a largest element in [256, 512) and p by 2^10, powers of two that
-//               keep the lo parts out of FP16's subnormals.
+//               keep the lo parts out of FP16's subnormals (a p below 2^-13 of the row's largest,
+//               whose lo part gets there, is off by at most 2^-35 of that largest).
 //   FP32 pages  both operands as TF32 hi + lo, hi hi + hi lo + lo hi: three products, with the
 //               range of FP32.
 // The MMA adds to its FP32 accumulator by cutting, half a unit of the accumulator per step on

@@ -2,7 +2,8 @@
 // with head_dim over 64) -- the chunks of prompts.
 //
 // Two query tiles of 128 rows share each key tile.  As on mma.sync, FP32 operands are pairs hi + lo
-// and 2^-21 of every product is kept:
+// and 2^-21 of every product is kept (of a weight on FP16 pages 2^-35 of the row's largest, where that is
+// more: it is where FP16 ends):
 //   FP16 pages  q and p as FP16 pairs (q scaled to a largest element in [256, 512), p by 2^10),
 //               K and V as they are: two MMAs; key tiles of 128 positions
 //     S = q_lo K' + q_hi K'      A: q in shared memory, B: K            M 128, N 128
